@@ -305,6 +305,87 @@ int smx_energy_virial_noalloc(const double* node_energies, int num_nodes, const 
                               const double* node_forces, long num_edges, double* out7, void* stream,
                               char* errbuf, int errbuf_len);
 
+/* Rows routed to groups and back, for callers that treat the atoms of a batch differently by group: per-atom arrays (rows of `width`
+ * values) are copied into the order of the groups, and results in that order are summed back with weights. No counterpart in the
+ * reference. Every row n names `slots` groups, ids[n * slots + s]; an id outside [0, num_groups) is an empty slot. The pairs (n, s) are
+ * sorted by group, equal ones in the order of the list:
+ *   order[p]      n * slots + s of the p-th pair; empty slots follow behind the last group, in the order of the list (num_rows * slots entries)
+ *   position[n * slots + s]   p, or -1 for an empty slot
+ *   offsets[g]    first p of group g; offsets[num_groups] = number of pairs in groups (num_groups + 1 entries)
+ * smx_route_dispatch copies rows[position[n, s], :] = x[n, :]; smx_route_combine makes y[n, :] = base[n, :] + sum_s weights[n, s] *
+ * rows[position[n, s], :], slots in order (`weights` NULL: ones, `base` NULL: zero; `base` may be `y`). It is also the gradient of
+ * dispatch (rows = gradient of the sorted rows, weights and base NULL). smx_route_combine_backward makes grad_rows[position[n, s], :] =
+ * weights[n, s] * grad_y[n, :] and, unless NULL, grad_weights[n, s] = <grad_y[n, :], rows[position[n, s], :]> (zero in empty slots).
+ * Values of empty slots (their weights, rows behind the last group) are never read. Rows behind the last group of `rows` / `grad_rows`
+ * are left as they were, or zeroed with `zero_tail` != 0. Sorted rows are contiguous, the others have a row stride in elements.
+ * `precision` (SMX_FP32 or SMX_FP64) is the type of all values, and of the sums.
+ * These calls need no evaluator: all pointers are device pointers on the current GPU, work is issued on `stream` (a cudaStream_t, may be
+ * NULL), nothing is allocated and nothing waits, so they can be captured into a graph. The plan of more than 8,192 pairs needs a
+ * workspace of smx_route_plan_bytes bytes; calls that may overlap on the device need one each. The same call gives the same bits.
+ * Limits: num_groups and slots as below, num_rows * slots below 2^31 - 2^11. Messages go to `errbuf` (capacity `errbuf_len`, may be
+ * NULL); smx_route_plan_bytes returns -1 for sizes that smx_route_plan refuses. */
+enum { SMX_ROUTE_MAX_GROUPS = 1024, SMX_ROUTE_MAX_SLOTS = 64 };
+long smx_route_plan_bytes(long num_rows, int slots, int num_groups);
+int smx_route_plan(const int* ids, long num_rows, int slots, int num_groups, int* order, int* position, int* offsets, void* workspace,
+                   long workspace_bytes, void* stream, char* errbuf, int errbuf_len);
+int smx_route_dispatch(int precision, const void* x, long x_stride, long num_rows, int slots, long width, const int* position,
+                       const int* offsets, int num_groups, void* rows, int zero_tail, void* stream, char* errbuf, int errbuf_len);
+int smx_route_combine(int precision, const void* rows, const int* position, long num_rows, int slots, long width, const void* weights,
+                      const void* base, long base_stride, void* y, long y_stride, void* stream, char* errbuf, int errbuf_len);
+int smx_route_combine_backward(int precision, const void* grad_y, long grad_y_stride, const void* rows, const int* position,
+                               const int* offsets, int num_groups, long num_rows, int slots, long width, const void* weights,
+                               void* grad_rows, void* grad_weights, int zero_tail, void* stream, char* errbuf, int errbuf_len);
+
+/* Channel-mixing linears with low-rank adapters beside the shared weights: fine-tuned variants of one model, each a few matrices, used side by
+ * side on the atoms of a batch (a second whole model costs its spline tables again: 59 GB in float64 for 89 elements at 128 channels and L_max = 1).
+ * An atom's row of `x` holds, degree after degree, `components` rows of in_channels values; its row of `y` the same with out_channels (the
+ * layout of M0 / H1, of Phi1 and of A1). With a plan of smx_route_plan over adapters as groups, each component m of degree l of atom n becomes
+ *   y = x shared_l + sum_s w[n, s] (x down_l[g]) up_l[g],   g = ids[n, s],
+ * `shared` [in][out] (NULL: none), `down` [groups][in][rank], `up` [groups][rank][out], `weights` [num_rows][slots] (NULL: ones). Atoms
+ * without a group get the shared product.
+ * The matrices are laid out for the products by smx_adapter_prepare into `tiles` (smx_adapter_tiles_bytes bytes): the shared weights with
+ * SMX_ADAPTER_SHARED in `parts`, the adapters with SMX_ADAPTER_MATRICES. Every later call reads the matrices there: after changing values,
+ * prepare again. `shared`, `down` and `up` themselves are read by smx_adapter_prepare only (`shared` being NULL or not counts in every call).
+ * smx_adapter_forward writes y and, unless `hidden` is NULL, the products x down of every pair (smx_adapter_hidden_elements values, a layout
+ * of the library's own), which smx_adapter_backward then need not compute again.
+ * smx_adapter_backward reads grad_y, x (and hidden) and writes, each unless NULL, grad_x, the degrees' grad_down / grad_up (both, for all
+ * degrees or none; groups without atoms get zeros) and grad_weights [num_rows][slots] (zero in empty slots). The shared weights are
+ * frozen: they have no gradient here.
+ * float32: products on the tensor cores from operands split in two (3xTF32), sums in float32; float64 throughout otherwise. Sums over
+ * atoms are split into chunks of a fixed number of rows and added in order: the same call gives the same bits.
+ * The rules of the smx_route_* calls hold: device pointers on the current GPU, `stream`, no allocation, no wait, a workspace of
+ * smx_adapter_workspace_bytes bytes for each call that may overlap with another one, errors through `errbuf`. The size functions
+ * return -1 for calls that are refused. Limits: rank, degrees as below, those of the routing. */
+enum { SMX_ADAPTER_MAX_RANK = 64, SMX_ADAPTER_MAX_DEGREES = 8 };
+enum { SMX_ADAPTER_SHARED = 1, SMX_ADAPTER_MATRICES = 2 };
+typedef struct smx_adapter_degree {
+    int components, in_channels, out_channels;
+    const void *shared, *down, *up;
+    void *grad_down, *grad_up;
+} smx_adapter_degree;
+typedef struct smx_adapter_linear {
+    int precision, num_degrees, num_groups, rank, slots;
+    long num_rows;
+    smx_adapter_degree degrees[8];
+    void* tiles;                             /* of smx_adapter_prepare */
+    const int *order, *position, *offsets;   /* of smx_route_plan */
+    const void* weights;
+    const void* x;      long x_stride;       /* strides: elements from atom to atom */
+    void* y;            long y_stride;
+    const void* grad_y; long grad_y_stride;
+    void* grad_x;       long grad_x_stride;
+    void* grad_weights;
+    void* hidden;
+    void* workspace;    long workspace_bytes;
+    void* stream;
+} smx_adapter_linear;
+long smx_adapter_tiles_bytes(const smx_adapter_linear* call);
+int smx_adapter_prepare(const smx_adapter_linear* call, int parts, char* errbuf, int errbuf_len);
+long smx_adapter_hidden_elements(const smx_adapter_linear* call);
+long smx_adapter_workspace_bytes(const smx_adapter_linear* call, int backward);
+int smx_adapter_forward(const smx_adapter_linear* call, char* errbuf, int errbuf_len);
+int smx_adapter_backward(const smx_adapter_linear* call, char* errbuf, int errbuf_len);
+
 #ifdef __cplusplus
 }
 #endif

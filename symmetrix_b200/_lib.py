@@ -24,7 +24,12 @@ EXPORTED_SYMBOLS = [
     "smx_energy_virial_noalloc", "smx_sync", "smx_set_stream", "smx_restrict_nodes", "smx_set_active_nodes", "smx_resize_rows", "smx_device_ptr",
     "smx_halo_pack", "smx_halo_unpack", "smx_halo_unpack_add", "smx_halo_cache_lists", "smx_atom_forces", "smx_active_counts", "smx_debug_expire_waits",
     "smx_comm_unique_id", "smx_comm_init", "smx_comm_destroy", "smx_halo_exchange", "smx_allreduce_sum", "smx_model_digest",
+    "smx_route_plan_bytes", "smx_route_plan", "smx_route_dispatch", "smx_route_combine", "smx_route_combine_backward",
+    "smx_adapter_tiles_bytes", "smx_adapter_prepare", "smx_adapter_hidden_elements", "smx_adapter_workspace_bytes", "smx_adapter_forward", "smx_adapter_backward",
 ]
+ROUTE_MAX_GROUPS, ROUTE_MAX_SLOTS = 1024, 64
+ADAPTER_MAX_RANK, ADAPTER_MAX_DEGREES = 64, 8
+ADAPTER_SHARED, ADAPTER_MATRICES = 1, 2
 
 
 class ModelInfo(ctypes.Structure):
@@ -35,6 +40,22 @@ class ModelInfo(ctypes.Structure):
         ("has_zbl", ctypes.c_int), ("precision", ctypes.c_int), ("device", ctypes.c_int),
         ("num_interactions", ctypes.c_int),
     ]
+
+
+class AdapterDegree(ctypes.Structure):
+    _fields_ = [("components", ctypes.c_int), ("in_channels", ctypes.c_int), ("out_channels", ctypes.c_int),
+                ("shared", ctypes.c_void_p), ("down", ctypes.c_void_p), ("up", ctypes.c_void_p),
+                ("grad_down", ctypes.c_void_p), ("grad_up", ctypes.c_void_p)]
+
+
+class AdapterCall(ctypes.Structure):
+    _fields_ = [("precision", ctypes.c_int), ("num_degrees", ctypes.c_int), ("num_groups", ctypes.c_int), ("rank", ctypes.c_int),
+                ("slots", ctypes.c_int), ("num_rows", ctypes.c_long), ("degrees", AdapterDegree * ADAPTER_MAX_DEGREES), ("tiles", ctypes.c_void_p),
+                ("order", ctypes.c_void_p), ("position", ctypes.c_void_p), ("offsets", ctypes.c_void_p), ("weights", ctypes.c_void_p),
+                ("x", ctypes.c_void_p), ("x_stride", ctypes.c_long), ("y", ctypes.c_void_p), ("y_stride", ctypes.c_long),
+                ("grad_y", ctypes.c_void_p), ("grad_y_stride", ctypes.c_long), ("grad_x", ctypes.c_void_p), ("grad_x_stride", ctypes.c_long),
+                ("grad_weights", ctypes.c_void_p), ("hidden", ctypes.c_void_p), ("workspace", ctypes.c_void_p),
+                ("workspace_bytes", ctypes.c_long), ("stream", ctypes.c_void_p)]
 
 
 _lib = None
@@ -99,5 +120,22 @@ def load():
     lib.smx_allreduce_sum.argtypes = [vp, dp, ctypes.c_int]
     lib.smx_model_digest.argtypes = [ctypes.c_char_p, ctypes.c_int, ctypes.POINTER(ctypes.c_ulonglong), ctypes.POINTER(ctypes.c_int)]
     lib.smx_energy_virial_noalloc.argtypes = [dp, ctypes.c_int, dp, dp, ctypes.c_long, dp, vp, ctypes.c_char_p, ctypes.c_int]
+    cl, ci, err = ctypes.c_long, ctypes.c_int, [ctypes.c_char_p, ctypes.c_int]
+    lib.smx_route_plan_bytes.argtypes = [cl, ci, ci]
+    lib.smx_route_plan_bytes.restype = cl
+    lib.smx_route_plan.argtypes = [ip, cl, ci, ci, ip, ip, ip, vp, cl, vp, *err]
+    lib.smx_route_dispatch.argtypes = [ci, vp, cl, cl, ci, cl, ip, ip, ci, vp, ci, vp, *err]
+    lib.smx_route_combine.argtypes = [ci, vp, ip, cl, ci, cl, vp, vp, cl, vp, cl, vp, *err]
+    lib.smx_route_combine_backward.argtypes = [ci, vp, cl, vp, ip, ip, ci, cl, ci, cl, vp, vp, vp, ci, vp, *err]
+    call = ctypes.POINTER(AdapterCall)
+    lib.smx_adapter_tiles_bytes.argtypes = [call]
+    lib.smx_adapter_tiles_bytes.restype = cl
+    lib.smx_adapter_prepare.argtypes = [call, ci, *err]
+    lib.smx_adapter_hidden_elements.argtypes = [call]
+    lib.smx_adapter_hidden_elements.restype = cl
+    lib.smx_adapter_workspace_bytes.argtypes = [call, ci]
+    lib.smx_adapter_workspace_bytes.restype = cl
+    lib.smx_adapter_forward.argtypes = [call, *err]
+    lib.smx_adapter_backward.argtypes = [call, *err]
     _lib = lib
     return lib

@@ -1,0 +1,671 @@
+// Linears of all degrees with low-rank adapters of many requests beside the shared weights (smx_adapter_*).
+//
+// A row is (atom n, component m of degree l). With slots s, group g = g(n, s), mixing weight w = w[n, s]:
+//   forward   t = x A_g,  y = x W + sum_s w t B_g
+//   backward  h = gy B_g^T,  gx = gy W^T + sum_s w h A_g^T,  gA_g = sum w x^T h,  gB_g = sum w t^T gy,  gw = sum_(l, m) <t, h>
+// The backward pass to x is the forward pass with the transposed matrices, so one kernel does both.
+//
+// Rows are taken in the order of the routing (csrc/routing.cu), in tiles that never mix groups. With one slot a row belongs to one tile: the
+// tile's kernel makes the shared product, its own adapter's and their sum, so x is read and y is written once. With more slots the shared product
+// runs over all rows, the adapters' products go to a workspace in sorted order, and the routing's combine adds them to the output in slot
+// order. Sums over rows (gA, gB) are split into chunks of a fixed number of rows, whose partial sums are added in order: no atomics.
+#include "adapters.hpp"
+
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <climits>
+#include <cstdint>
+
+#include "common.cuh"
+#include "routing.hpp"
+
+namespace smx {
+namespace {
+
+constexpr int kMaxDegrees = SMX_ADAPTER_MAX_DEGREES, kMaxRank = SMX_ADAPTER_MAX_RANK;
+
+// One degree of a pass: out rows = in rows . W + weight (in rows . first_g) . second_g. Matrices are addressed by strides, so that a
+// transposed one is the same memory.
+template <typename T>
+struct PassDegree {
+    int comps, Kd, Nc;
+    long long in_off, out_off;
+    const T* W; long long w_k, w_n;
+    const T* first; long long f_group, f_k, f_r;
+    const T* second; long long s_group, s_r, s_n;
+    T* hidden;                                  // [pairs * comps][rank] in sorted order, or null
+};
+template <typename T>
+struct Pass {
+    PassDegree<T> degree[kMaxDegrees];
+    int rank, groups, slots;
+    long long num_rows, pairs;
+    const int* order; const int* offsets;
+    const T* weights;
+    const T* in; long long in_stride;
+    T* out; long long out_stride;               // null: only the hidden rows
+    int sorted;        // tiles by group, atoms through `order`; else all rows in their own order and no adapters
+    int out_sorted;    // out rows by sorted position (workspace), else by atom
+    int tail;          // the rows without a group are a last group of their own
+};
+
+// Rows of a tile: pairs [pair0, pair0 + ...) of one group, rows counted in components from row0 of the group.
+struct TileRows { int group; long long first_pair, row0, rows; };
+
+// The tile-th tile of `size` rows, groups one after the other (group `groups`: the pairs behind the last group, if `tail`). Called by one warp.
+__device__ __forceinline__ bool find_tile(const int* __restrict__ offsets, int groups, bool tail, long long pairs, int comps, int size, long long tile,
+                                          TileRows& out) {
+    const int lane = threadIdx.x & 31;
+    long long run = 0;
+    for (int g0 = 0; g0 <= groups; g0 += 32) {
+        const int g = g0 + lane;
+        long long first = 0, rows = 0;
+        if (g < groups || (g == groups && tail)) {
+            first = offsets[g];
+            rows = ((g < groups ? offsets[g + 1] : pairs) - first) * comps;
+        }
+        const long long tiles = (rows + size - 1) / size;
+        long long incl = tiles;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const long long up = __shfl_up_sync(0xffffffffu, incl, d);
+            if (lane >= d) incl += up;
+        }
+        const long long begin = run + incl - tiles;
+        const unsigned hit = __ballot_sync(0xffffffffu, tile >= begin && tile < begin + tiles);
+        if (hit) {
+            const int src = __ffs(hit) - 1;
+            out.group = __shfl_sync(0xffffffffu, g, src);
+            out.first_pair = __shfl_sync(0xffffffffu, first, src);
+            const long long b = __shfl_sync(0xffffffffu, begin, src), r = __shfl_sync(0xffffffffu, rows, src);
+            out.row0 = (tile - b) * size;
+            out.rows = min(static_cast<long long>(size), r - out.row0);
+            return true;
+        }
+        run += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    return false;
+}
+
+// ------------------------------------------------------------------------------------------- pass, plain tiles
+constexpr int kPlainBM = 32, kPlainBN = 64, kPlainBK = 32, kPlainThreads = 128;
+
+template <typename T>
+__global__ void __launch_bounds__(kPlainThreads) adapter_pass_plain_kernel(const __grid_constant__ Pass<T> pass) {
+    const PassDegree<T>& d = pass.degree[blockIdx.z];
+    const int col0 = blockIdx.y * kPlainBN;
+    if (col0 >= d.Nc) return;
+    __shared__ TileRows tile;
+    __shared__ int found;
+    __shared__ long long in_base[kPlainBM], out_base[kPlainBM], hid_row[kPlainBM];
+    __shared__ T weight[kPlainBM];
+    __shared__ T As[kPlainBM][kPlainBK + 1];
+    __shared__ T Bs[kPlainBK][kPlainBN + 1];
+    __shared__ T Hs[kPlainBM][kMaxRank + 1];
+    const int tid = threadIdx.x;
+    if (tid < 32) {
+        TileRows t{};
+        bool ok;
+        if (pass.sorted) {
+            ok = find_tile(pass.offsets, pass.groups, pass.tail != 0, pass.pairs, d.comps, kPlainBM, blockIdx.x, t);
+        } else {
+            const long long all = pass.num_rows * d.comps;
+            t.group = pass.groups; t.first_pair = 0; t.row0 = static_cast<long long>(blockIdx.x) * kPlainBM;
+            t.rows = min(static_cast<long long>(kPlainBM), all - t.row0);
+            ok = t.rows > 0;
+        }
+        if (tid == 0) { tile = t; found = ok ? 1 : 0; }
+    }
+    __syncthreads();
+    if (!found) return;
+    const int rows = static_cast<int>(tile.rows), g = tile.group, R = pass.rank;
+    const bool adapter = g < pass.groups;
+    if (tid < rows) {
+        const long long r = tile.row0 + tid, p = tile.first_pair + r / d.comps;
+        const int m = static_cast<int>(r % d.comps);
+        const long long pair = pass.sorted ? pass.order[p] : p, n = pass.sorted ? pair / pass.slots : p;
+        in_base[tid] = n * pass.in_stride + d.in_off + static_cast<long long>(m) * d.Kd;
+        out_base[tid] = (pass.out_sorted ? p : n) * pass.out_stride + d.out_off + static_cast<long long>(m) * d.Nc;
+        hid_row[tid] = p * d.comps + m;
+        weight[tid] = adapter && pass.weights ? pass.weights[pair] : T(1);
+    }
+    const int tr = (tid >> 4) * 4, tc = (tid & 15) * 4;       // four rows, four columns a thread
+    T acc[4][4] = {};
+    T hid[kMaxRank / 4];
+#pragma unroll
+    for (int q = 0; q < kMaxRank / 4; ++q) hid[q] = T(0);
+    const int hr = tid >> 2, hc = tid & 3;                      // hidden value hc + 4 q of row hr
+    __syncthreads();
+    const T* first = adapter ? d.first + g * d.f_group : nullptr;
+    for (int k0 = 0; k0 < d.Kd; k0 += kPlainBK) {
+        for (int i = tid; i < kPlainBM * kPlainBK; i += kPlainThreads) {
+            const int r = i / kPlainBK, k = i % kPlainBK;
+            As[r][k] = r < rows && k0 + k < d.Kd ? pass.in[in_base[r] + k0 + k] : T(0);
+        }
+        if (d.W)
+            for (int i = tid; i < kPlainBK * kPlainBN; i += kPlainThreads) {
+                const int k = i / kPlainBN, c = i % kPlainBN;
+                Bs[k][c] = k0 + k < d.Kd && col0 + c < d.Nc ? d.W[(k0 + k) * d.w_k + (col0 + c) * d.w_n] : T(0);
+            }
+        __syncthreads();
+        if (d.W)
+            for (int k = 0; k < kPlainBK; ++k) {
+                T a[4], b[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) { a[q] = As[tr + q][k]; b[q] = Bs[k][tc + q]; }
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[i][j] += a[i] * b[j];
+            }
+        if (adapter)
+            for (int k = 0; k < kPlainBK && k0 + k < d.Kd; ++k) {
+                const T a = As[hr][k];
+                const T* f = first + (k0 + k) * d.f_k;
+#pragma unroll
+                for (int q = 0; q < kMaxRank / 4; ++q)
+                    if (hc + 4 * q < R) hid[q] += a * f[(hc + 4 * q) * d.f_r];
+            }
+        __syncthreads();
+    }
+    if (adapter) {
+#pragma unroll
+        for (int q = 0; q < kMaxRank / 4; ++q) {
+            const int r = hc + 4 * q;
+            if (r < R && hr < rows) {
+                if (d.hidden && blockIdx.y == 0) d.hidden[hid_row[hr] * R + r] = hid[q];
+                Hs[hr][r] = weight[hr] * hid[q];
+            }
+        }
+        __syncthreads();
+        if (!pass.out) return;
+        const T* second = d.second + g * d.s_group;
+        for (int r = 0; r < R; ++r) {
+            T b[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) b[j] = col0 + tc + j < d.Nc ? second[r * d.s_r + (col0 + tc + j) * d.s_n] : T(0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const T h = tr + i < rows ? Hs[tr + i][r] : T(0);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[i][j] += h * b[j];
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (tr + i < rows && col0 + tc + j < d.Nc) pass.out[out_base[tr + i] + col0 + tc + j] = acc[i][j];
+}
+
+// ------------------------------------------------------------------------------------------- gradients of the adapters
+// part[chunk][k][r] = sum over the chunk's rows of a[row][k] weight[row] h[row][r]; a is x with h = gy B^T, or gy with h = x A.
+constexpr int kGradChunk = 512, kGradCols = 32, kGradRows = 32, kGradThreads = 128;
+template <typename T>
+struct GradProblem {
+    int comps, Kd;
+    const T* a; long long a_stride, a_off;
+    const T* hidden;                             // [pairs * comps][rank], not weighted
+    T* part;                                     // [chunks][Kd][rank]
+    T* grad; long long g_group, g_k, g_r;        // gA: [group][k][r], gB: [group][r][k]
+};
+template <typename T>
+struct GradPass {
+    GradProblem<T> problem[2 * kMaxDegrees];
+    int rank, groups, slots;
+    long long pairs;
+    const int* order; const int* offsets;
+    const T* weights;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kGradThreads) adapter_grad_kernel(const __grid_constant__ GradPass<T> pass) {
+    const GradProblem<T>& d = pass.problem[blockIdx.z];
+    const int k0 = blockIdx.y * kGradCols;
+    if (k0 >= d.Kd) return;
+    __shared__ TileRows tile;
+    __shared__ int found;
+    __shared__ T As[kGradRows][kGradCols + 1];
+    __shared__ T Hs[kGradRows][kMaxRank + 1];
+    const int tid = threadIdx.x, R = pass.rank;
+    if (tid < 32) {
+        TileRows t{};
+        const bool ok = find_tile(pass.offsets, pass.groups, false, pass.pairs, d.comps, kGradChunk, blockIdx.x, t);
+        if (tid == 0) { tile = t; found = ok ? 1 : 0; }
+    }
+    __syncthreads();
+    if (!found) return;
+    T acc[kMaxRank / 4];
+#pragma unroll
+    for (int q = 0; q < kMaxRank / 4; ++q) acc[q] = T(0);
+    const int kc = tid >> 2, rc = tid & 3;
+    for (int r0 = 0; r0 < tile.rows; r0 += kGradRows) {
+        for (int i = tid; i < kGradRows * kGradCols; i += kGradThreads) {
+            const int rr = i / kGradCols, k = i % kGradCols;
+            T v = T(0);
+            if (r0 + rr < tile.rows && k0 + k < d.Kd) {
+                const long long r = tile.row0 + r0 + rr, p = tile.first_pair + r / d.comps;
+                const int m = static_cast<int>(r % d.comps);
+                v = d.a[static_cast<long long>(pass.order[p] / pass.slots) * d.a_stride + d.a_off + static_cast<long long>(m) * d.Kd + k0 + k];
+            }
+            As[rr][k] = v;
+        }
+        for (int i = tid; i < kGradRows * R; i += kGradThreads) {
+            const int rr = i / R, q = i % R;
+            T v = T(0);
+            if (r0 + rr < tile.rows) {
+                const long long r = tile.row0 + r0 + rr, p = tile.first_pair + r / d.comps;
+                v = d.hidden[(tile.first_pair * d.comps + r) * R + q];
+                if (pass.weights) v *= pass.weights[pass.order[p]];
+            }
+            Hs[rr][q] = v;
+        }
+        __syncthreads();
+        for (int rr = 0; rr < kGradRows; ++rr) {
+            const T a = As[rr][kc];
+#pragma unroll
+            for (int q = 0; q < kMaxRank / 4; ++q)
+                if (rc + 4 * q < R) acc[q] += a * Hs[rr][rc + 4 * q];
+        }
+        __syncthreads();
+    }
+    if (k0 + kc < d.Kd)
+#pragma unroll
+        for (int q = 0; q < kMaxRank / 4; ++q)
+            if (rc + 4 * q < R) d.part[(static_cast<long long>(blockIdx.x) * d.Kd + k0 + kc) * R + rc + 4 * q] = acc[q];
+}
+
+// grad of group blockIdx.x: its chunks added in order (none: zero).
+template <typename T>
+__global__ void __launch_bounds__(256) adapter_grad_sum_kernel(const __grid_constant__ GradPass<T> pass) {
+    const GradProblem<T>& d = pass.problem[blockIdx.z];
+    const int g = blockIdx.x, R = pass.rank;
+    __shared__ long long sh[2];
+    if (threadIdx.x < 32) {
+        long long before = 0;
+        for (int q = threadIdx.x; q < g; q += 32)
+            before += (static_cast<long long>(pass.offsets[q + 1] - pass.offsets[q]) * d.comps + kGradChunk - 1) / kGradChunk;
+#pragma unroll
+        for (int s = 16; s > 0; s >>= 1) before += __shfl_xor_sync(0xffffffffu, before, s);
+        if (threadIdx.x == 0) {
+            sh[0] = before;
+            sh[1] = (static_cast<long long>(pass.offsets[g + 1] - pass.offsets[g]) * d.comps + kGradChunk - 1) / kGradChunk;
+        }
+    }
+    __syncthreads();
+    const long long c0 = sh[0], chunks = sh[1];
+    const long long size = static_cast<long long>(d.Kd) * R;
+    for (long long i = static_cast<long long>(blockIdx.y) * 256 + threadIdx.x; i < size; i += 256LL * gridDim.y) {
+        T s = T(0);
+        for (long long c = 0; c < chunks; ++c) s += d.part[(c0 + c) * size + i];
+        d.grad[g * d.g_group + (i / R) * d.g_k + (i % R) * d.g_r] = s;
+    }
+}
+
+// gw of every pair: a warp adds the products of both hidden rows over components, degree after degree. Empty slots get zero.
+template <typename T>
+struct WeightGrad {
+    const T* t[kMaxDegrees]; const T* h[kMaxDegrees];
+    int comps[kMaxDegrees];
+    int degrees, rank;
+    long long pairs;
+    const int* position;
+    T* grad;
+};
+template <typename T>
+__global__ void __launch_bounds__(256) adapter_weight_grad_kernel(const __grid_constant__ WeightGrad<T> a) {
+    const int lane = threadIdx.x & 31;
+    for (long long i = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) >> 5; i < a.pairs; i += (static_cast<long long>(gridDim.x) * 256) >> 5) {
+        const int p = a.position[i];
+        T s = T(0);
+        if (p >= 0)
+            for (int d = 0; d < a.degrees; ++d) {
+                const int n = a.comps[d] * a.rank;
+                const T* t = a.t[d] + static_cast<long long>(p) * n;
+                const T* h = a.h[d] + static_cast<long long>(p) * n;
+                for (int q = lane; q < n; q += 32) s += t[q] * h[q];
+            }
+#pragma unroll
+        for (int w = 16; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
+        if (lane == 0) a.grad[i] = s;
+    }
+}
+
+// ------------------------------------------------------------------------------------------- layout of the matrices
+struct CopyList {
+    static constexpr int kMost = 3 * kMaxDegrees;
+    const void* src[kMost]; void* dst[kMost];
+    long long count[kMost];
+};
+template <typename T>
+__global__ void __launch_bounds__(256) adapter_copy_kernel(const __grid_constant__ CopyList list) {
+    const T* src = static_cast<const T*>(list.src[blockIdx.y]);
+    T* dst = static_cast<T*>(list.dst[blockIdx.y]);
+    for (long long i = blockIdx.x * 256LL + threadIdx.x; i < list.count[blockIdx.y]; i += 256LL * gridDim.x) dst[i] = src[i];
+}
+
+// ------------------------------------------------------------------------------------------- host side
+void launched(const char* what) {
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) throw CudaError(std::string(what) + ": " + cudaGetErrorString(e));
+}
+
+struct Widths { long in = 0, out = 0; long long comps = 0; };
+Widths widths(const smx_adapter_linear& c) {
+    Widths w;
+    for (int d = 0; d < c.num_degrees; ++d) {
+        w.in += static_cast<long>(c.degrees[d].components) * c.degrees[d].in_channels;
+        w.out += static_cast<long>(c.degrees[d].components) * c.degrees[d].out_channels;
+        w.comps += c.degrees[d].components;
+    }
+    return w;
+}
+
+void check_call(const smx_adapter_linear& c) {
+    if (c.precision != SMX_FP32 && c.precision != SMX_FP64) throw ArgError("smx_adapter: precision must be 32 or 64");
+    if (c.num_degrees < 1 || c.num_degrees > kMaxDegrees) throw ArgError("smx_adapter: the number of degrees must lie in 1 .. " + std::to_string(kMaxDegrees));
+    if (c.rank < 1 || c.rank > kMaxRank) throw ArgError("smx_adapter: the rank must lie in 1 .. " + std::to_string(kMaxRank));
+    route_plan_bytes(c.num_rows, c.slots, c.num_groups);       // sizes shared with the routing
+    for (int d = 0; d < c.num_degrees; ++d) {
+        const smx_adapter_degree& g = c.degrees[d];
+        if (g.components < 1 || g.components > 1024 || g.in_channels < 1 || g.out_channels < 1 || g.in_channels > (1 << 20) || g.out_channels > (1 << 20))
+            throw ArgError("smx_adapter: a degree needs 1 .. 1024 components and 1 .. 1048576 channels");
+        // grid.x counts row tiles
+        if (static_cast<long long>(c.num_rows) * c.slots * g.components / kPlainBM + c.num_groups + 1 > INT_MAX) throw ArgError("smx_adapter: too many rows");
+    }
+}
+void check_plan(const smx_adapter_linear& c) {
+    check_call(c);
+    if (!c.tiles) throw ArgError("smx_adapter: null tiles");
+    if (!c.offsets || (c.num_rows > 0 && (!c.order || !c.position))) throw ArgError("smx_adapter: null plan");
+}
+
+void check_rows(const char* what, const void* p, long stride, long width, long rows, bool written) {
+    if (rows > 0 && !p) throw ArgError(std::string("smx_adapter: null ") + what);
+    if (stride < 0 || (written && rows > 1 && stride < width)) throw ArgError(std::string("smx_adapter: bad row stride of ") + what);
+}
+
+// Workspace: hidden rows of both directions (backward), sorted products (several slots), partial sums (backward); parts start on 256 bytes.
+struct Workspace {
+    char* base;
+    size_t used = 0;
+    template <typename T>
+    T* take(size_t n) {
+        T* p = base ? reinterpret_cast<T*>(base + used) : nullptr;
+        used += (n * sizeof(T) + 255) / 256 * 256;
+        return p;
+    }
+};
+
+long long grad_chunks(const smx_adapter_linear& c, int comps) {
+    return static_cast<long long>(c.num_rows) * c.slots * comps / kGradChunk + c.num_groups;
+}
+
+template <typename T>
+struct Buffers {
+    T* back_hidden = nullptr; T* hidden = nullptr; T* products = nullptr; T* parts[2 * kMaxDegrees] = {};
+    size_t bytes = 0;
+};
+template <typename T>
+Buffers<T> lay_out(const smx_adapter_linear& c, bool backward) {
+    Buffers<T> b;
+    Workspace ws{static_cast<char*>(c.workspace)};
+    const Widths w = widths(c);
+    const size_t pairs = static_cast<size_t>(c.num_rows) * c.slots;
+    if (c.slots > 1) b.products = ws.take<T>(pairs * (backward ? std::max(w.in, w.out) : w.out));
+    if (backward) {
+        b.back_hidden = ws.take<T>(pairs * w.comps * c.rank);
+        if (!c.hidden) b.hidden = ws.take<T>(pairs * w.comps * c.rank);
+        for (int d = 0; d < c.num_degrees; ++d) {
+            b.parts[2 * d] = ws.take<T>(static_cast<size_t>(grad_chunks(c, c.degrees[d].components)) * c.degrees[d].in_channels * c.rank);
+            b.parts[2 * d + 1] = ws.take<T>(static_cast<size_t>(grad_chunks(c, c.degrees[d].components)) * c.degrees[d].out_channels * c.rank);
+        }
+    }
+    b.bytes = ws.used;
+    return b;
+}
+
+// The matrices of a degree inside `tiles`.
+template <typename T>
+struct Matrices { T *shared, *down, *up; };
+template <typename T>
+size_t tile_layout(const smx_adapter_linear& c, Matrices<T> (&m)[kMaxDegrees]) {
+    Workspace ws{static_cast<char*>(c.tiles)};
+    for (int d = 0; d < c.num_degrees; ++d) {
+        const smx_adapter_degree& g = c.degrees[d];
+        const size_t I = g.in_channels, O = g.out_channels;
+        m[d].shared = g.shared ? ws.take<T>(I * O) : nullptr;
+        m[d].down = ws.take<T>(I * c.rank * c.num_groups);
+        m[d].up = ws.take<T>(O * c.rank * c.num_groups);
+    }
+    return ws.used;
+}
+template <typename T>
+void prepare(const smx_adapter_linear& c, int parts) {
+    Matrices<T> m[kMaxDegrees];
+    tile_layout<T>(c, m);
+    CopyList list{};
+    int n = 0;
+    long long most = 0;
+    auto add = [&](const void* src, T* dst, long long count) {
+        if (!src) throw ArgError("smx_adapter_prepare: null matrix");
+        list.src[n] = src; list.dst[n] = dst; list.count[n++] = count;
+        most = std::max(most, count);
+    };
+    for (int d = 0; d < c.num_degrees; ++d) {
+        const smx_adapter_degree& g = c.degrees[d];
+        const long long I = g.in_channels, O = g.out_channels;
+        if ((parts & SMX_ADAPTER_SHARED) && g.shared) add(g.shared, m[d].shared, I * O);
+        if (parts & SMX_ADAPTER_MATRICES) {
+            add(g.down, m[d].down, I * c.rank * c.num_groups);
+            add(g.up, m[d].up, O * c.rank * c.num_groups);
+        }
+    }
+    if (!n) return;
+    adapter_copy_kernel<T><<<dim3(static_cast<unsigned>(std::min<long long>(256, (most + 255) / 256)), n), 256, 0, static_cast<cudaStream_t>(c.stream)>>>(list);
+    launched("adapter_copy_kernel");
+}
+
+template <typename T>
+Pass<T> make_pass(const smx_adapter_linear& c, bool transposed, T* hidden) {
+    Pass<T> p{};
+    Matrices<T> m[kMaxDegrees];
+    tile_layout<T>(c, m);
+    long long in_off = 0, out_off = 0;
+    const size_t pairs = static_cast<size_t>(c.num_rows) * c.slots;
+    for (int q = 0; q < c.num_degrees; ++q) {
+        const smx_adapter_degree& g = c.degrees[q];
+        PassDegree<T>& d = p.degree[q];
+        const long long I = g.in_channels, O = g.out_channels, R = c.rank;
+        const T *shared = m[q].shared, *down = m[q].down, *up = m[q].up;
+        d.comps = g.components;
+        d.in_off = in_off; d.out_off = out_off;
+        d.W = shared;
+        if (!transposed) {
+            d.Kd = g.in_channels; d.Nc = g.out_channels;
+            d.w_k = O; d.w_n = 1;
+            d.first = down; d.f_group = I * R; d.f_k = R; d.f_r = 1;
+            d.second = up; d.s_group = R * O; d.s_r = O; d.s_n = 1;
+        } else {
+            d.Kd = g.out_channels; d.Nc = g.in_channels;
+            d.w_k = 1; d.w_n = O;
+            d.first = up; d.f_group = R * O; d.f_k = 1; d.f_r = O;
+            d.second = down; d.s_group = I * R; d.s_r = 1; d.s_n = R;
+        }
+        d.hidden = hidden;
+        if (hidden) hidden += pairs * g.components * R;
+        in_off += static_cast<long long>(g.components) * d.Kd;
+        out_off += static_cast<long long>(g.components) * d.Nc;
+    }
+    p.rank = c.rank; p.groups = c.num_groups; p.slots = c.slots;
+    p.num_rows = c.num_rows; p.pairs = static_cast<long long>(pairs);
+    p.order = c.order; p.offsets = c.offsets;
+    p.weights = static_cast<const T*>(c.weights);
+    return p;
+}
+
+template <typename T>
+void launch_pass(const Pass<T>& p, int degrees, cudaStream_t stream) {
+    long long rows = 0;
+    int cols = 0;
+    for (int d = 0; d < degrees; ++d) {
+        rows = std::max(rows, (p.sorted ? p.pairs : p.num_rows) * p.degree[d].comps);
+        cols = std::max(cols, p.degree[d].Nc);
+    }
+    const long long tiles = p.sorted ? rows / kPlainBM + p.groups + 1 : (rows + kPlainBM - 1) / kPlainBM;
+    const dim3 grid(static_cast<unsigned>(tiles), (cols + kPlainBN - 1) / kPlainBN, degrees);
+    adapter_pass_plain_kernel<T><<<grid, kPlainThreads, 0, stream>>>(p);
+    launched("adapter_pass_plain_kernel");
+}
+
+// out = in W + adapters, in either direction; `hidden` (may be null) receives in . first of every pair. Without `out` that is all.
+template <typename T>
+void run_pass(const smx_adapter_linear& c, bool transposed, const T* in, long in_stride, T* out, long out_stride, T* hidden, T* products) {
+    if (c.num_rows == 0) return;
+    const cudaStream_t stream = static_cast<cudaStream_t>(c.stream);
+    const Widths w = widths(c);
+    const long out_width = transposed ? w.in : w.out;
+    Pass<T> p = make_pass<T>(c, transposed, hidden);
+    p.in = in; p.in_stride = in_stride;
+    p.sorted = 1;
+    if (!out) {
+        for (int d = 0; d < c.num_degrees; ++d) { p.degree[d].W = nullptr; p.degree[d].Nc = 1; }      // one (unused) block of columns
+        launch_pass(p, c.num_degrees, stream);
+        return;
+    }
+    if (c.slots == 1) {
+        p.out = out; p.out_stride = out_stride; p.tail = 1;
+        launch_pass(p, c.num_degrees, stream);
+        return;
+    }
+    // several slots: the shared product of all rows, every pair's own product, and their weighted sum in slot order
+    Pass<T> shared = make_pass<T>(c, transposed, nullptr);
+    shared.in = in; shared.in_stride = in_stride; shared.out = out; shared.out_stride = out_stride;
+    launch_pass(shared, c.num_degrees, stream);
+    for (int d = 0; d < c.num_degrees; ++d) p.degree[d].W = nullptr;
+    p.weights = nullptr;
+    p.out = products; p.out_stride = out_width; p.out_sorted = 1;
+    launch_pass(p, c.num_degrees, stream);
+    route_combine<T>(products, c.position, c.num_rows, c.slots, out_width, static_cast<const T*>(c.weights), out, out_stride, out, out_stride, stream);
+}
+
+template <typename T>
+void forward(const smx_adapter_linear& c) {
+    const Buffers<T> b = lay_out<T>(c, false);
+    if (c.workspace_bytes < 0 || static_cast<size_t>(c.workspace_bytes) < b.bytes || (b.bytes && !c.workspace))
+        throw ArgError("smx_adapter_forward: the workspace is smaller than smx_adapter_workspace_bytes says");
+    const Widths w = widths(c);
+    check_rows("x", c.x, c.x_stride, w.in, c.num_rows, false);
+    check_rows("y", c.y, c.y_stride, w.out, c.num_rows, true);
+    run_pass<T>(c, false, static_cast<const T*>(c.x), c.x_stride, static_cast<T*>(c.y), c.y_stride, static_cast<T*>(c.hidden), b.products);
+}
+
+template <typename T>
+void backward(const smx_adapter_linear& c) {
+    const Buffers<T> b = lay_out<T>(c, true);
+    if (c.workspace_bytes < 0 || static_cast<size_t>(c.workspace_bytes) < b.bytes || (b.bytes && !c.workspace))
+        throw ArgError("smx_adapter_backward: the workspace is smaller than smx_adapter_workspace_bytes says");
+    const Widths w = widths(c);
+    check_rows("grad_y", c.grad_y, c.grad_y_stride, w.out, c.num_rows, false);
+    if (c.grad_x) check_rows("grad_x", c.grad_x, c.grad_x_stride, w.in, c.num_rows, true);
+    bool adapters = false;
+    for (int d = 0; d < c.num_degrees; ++d) {
+        const bool any = c.degrees[d].grad_down || c.degrees[d].grad_up;
+        if (any && !(c.degrees[d].grad_down && c.degrees[d].grad_up)) throw ArgError("smx_adapter_backward: grad_down and grad_up come together");
+        if (d > 0 && any != adapters) throw ArgError("smx_adapter_backward: the adapters' gradients are wanted for all degrees or none");
+        adapters = any;
+    }
+    const bool hidden_needed = adapters || c.grad_weights;
+    if (!hidden_needed && !c.grad_x) return;
+    if (adapters || (c.grad_weights && !c.hidden)) check_rows("x", c.x, c.x_stride, w.in, c.num_rows, false);
+    const cudaStream_t stream = static_cast<cudaStream_t>(c.stream);
+    const size_t pairs = static_cast<size_t>(c.num_rows) * c.slots;
+    const T* x = static_cast<const T*>(c.x);
+    const T* gy = static_cast<const T*>(c.grad_y);
+    run_pass<T>(c, true, gy, c.grad_y_stride, static_cast<T*>(c.grad_x), c.grad_x_stride, b.back_hidden, b.products);
+    if (!hidden_needed) return;
+    const T* hidden = static_cast<const T*>(c.hidden);
+    if (!hidden) {
+        run_pass<T>(c, false, x, c.x_stride, nullptr, 0, b.hidden, nullptr);
+        hidden = b.hidden;
+    }
+    GradPass<T> gp{};
+    gp.rank = c.rank; gp.groups = c.num_groups; gp.slots = c.slots; gp.pairs = static_cast<long long>(pairs);
+    gp.order = c.order; gp.offsets = c.offsets; gp.weights = static_cast<const T*>(c.weights);
+    WeightGrad<T> wg{};
+    long long in_off = 0, out_off = 0, hid_off = 0, chunks = 0;
+    int cols = 0;
+    for (int q = 0; q < c.num_degrees; ++q) {
+        const smx_adapter_degree& g = c.degrees[q];
+        GradProblem<T>&a = gp.problem[2 * q], &u = gp.problem[2 * q + 1];
+        const long long I = g.in_channels, O = g.out_channels, R = c.rank;
+        a.comps = u.comps = g.components;
+        a.Kd = g.in_channels; u.Kd = g.out_channels;
+        a.a = x; a.a_stride = c.x_stride; a.a_off = in_off; a.hidden = b.back_hidden + hid_off;
+        u.a = gy; u.a_stride = c.grad_y_stride; u.a_off = out_off; u.hidden = hidden + hid_off;
+        a.part = b.parts[2 * q]; u.part = b.parts[2 * q + 1];
+        a.grad = static_cast<T*>(g.grad_down); a.g_group = I * R; a.g_k = R; a.g_r = 1;
+        u.grad = static_cast<T*>(g.grad_up); u.g_group = R * O; u.g_k = 1; u.g_r = O;
+        wg.t[q] = hidden + hid_off; wg.h[q] = b.back_hidden + hid_off; wg.comps[q] = g.components;
+        in_off += g.components * I; out_off += g.components * O; hid_off += static_cast<long long>(pairs) * g.components * R;
+        chunks = std::max(chunks, grad_chunks(c, g.components));
+        cols = std::max(cols, std::max(g.in_channels, g.out_channels));
+    }
+    if (adapters) {
+        if (pairs > 0) {
+            adapter_grad_kernel<T><<<dim3(static_cast<unsigned>(chunks), (cols + kGradCols - 1) / kGradCols, 2 * c.num_degrees), kGradThreads, 0, stream>>>(gp);
+            launched("adapter_grad_kernel");
+        }
+        const int slabs = static_cast<int>(std::min<long long>(64, (static_cast<long long>(cols) * c.rank + 255) / 256));
+        adapter_grad_sum_kernel<T><<<dim3(c.num_groups, slabs, 2 * c.num_degrees), 256, 0, stream>>>(gp);
+        launched("adapter_grad_sum_kernel");
+    }
+    if (c.grad_weights && pairs > 0) {
+        wg.degrees = c.num_degrees; wg.rank = c.rank; wg.pairs = static_cast<long long>(pairs); wg.position = c.position;
+        wg.grad = static_cast<T*>(c.grad_weights);
+        adapter_weight_grad_kernel<T><<<static_cast<unsigned>(std::min<long long>((wg.pairs + 7) / 8, 148 * 32)), 256, 0, stream>>>(wg);
+        launched("adapter_weight_grad_kernel");
+    }
+}
+
+}  // namespace
+
+size_t adapter_hidden_elements(const smx_adapter_linear& c) {
+    check_call(c);
+    return static_cast<size_t>(c.num_rows) * c.slots * widths(c).comps * c.rank;
+}
+size_t adapter_workspace_bytes(const smx_adapter_linear& c, bool backward) {
+    check_call(c);
+    smx_adapter_linear empty = c;
+    empty.workspace = nullptr;
+    return c.precision == SMX_FP32 ? lay_out<float>(empty, backward).bytes : lay_out<double>(empty, backward).bytes;
+}
+size_t adapter_tiles_bytes(const smx_adapter_linear& c) {
+    check_call(c);
+    smx_adapter_linear empty = c;
+    empty.tiles = nullptr;
+    Matrices<float> f[kMaxDegrees];
+    Matrices<double> d[kMaxDegrees];
+    return c.precision == SMX_FP32 ? tile_layout<float>(empty, f) : tile_layout<double>(empty, d);
+}
+void adapter_prepare(const smx_adapter_linear& c, int parts) {
+    check_call(c);
+    if (!c.tiles) throw ArgError("smx_adapter_prepare: null tiles");
+    if (parts & ~(SMX_ADAPTER_SHARED | SMX_ADAPTER_MATRICES)) throw ArgError("smx_adapter_prepare: unknown part");
+    if (c.precision == SMX_FP32) prepare<float>(c, parts);
+    else prepare<double>(c, parts);
+}
+void adapter_forward(const smx_adapter_linear& c) {
+    check_plan(c);
+    if (c.precision == SMX_FP32) forward<float>(c);
+    else forward<double>(c);
+}
+void adapter_backward(const smx_adapter_linear& c) {
+    check_plan(c);
+    if (c.precision == SMX_FP32) backward<float>(c);
+    else backward<double>(c);
+}
+
+}  // namespace smx

@@ -2,16 +2,20 @@
 // and dispatch to the evaluator of the handle's precision.
 #include <cuda_runtime.h>
 
+#include <cstdio>
 #include <cstring>
 #include <memory>
 #include <stdexcept>
 #include <string>
+#include <type_traits>
 
 #include "../../include/symmetrix_b200.h"
+#include "adapters.hpp"
 #include "common.cuh"
 #include "evaluator_base.hpp"
 #include "model_cache.hpp"
 #include "nccl_transport.hpp"
+#include "routing.hpp"
 
 // =================================================================================================
 // extern "C" entry points
@@ -42,6 +46,34 @@ int guarded(smx_handle h, Fn&& fn) {
         h->impl->last_error = e.what();
         return SMX_ERR_INVALID_ARGUMENT;
     }
+}
+
+// Calls without an evaluator: the message goes to the caller's buffer.
+template <typename Fn>
+int guarded_free(char* errbuf, int errbuf_len, Fn&& fn) {
+    auto fail = [&](int status, const char* what) {
+        if (errbuf && errbuf_len > 0) std::snprintf(errbuf, static_cast<size_t>(errbuf_len), "%s", what);
+        return status;
+    };
+    try {
+        fn();
+        return SMX_OK;
+    } catch (const smx::ArgError& e) { return fail(SMX_ERR_INVALID_ARGUMENT, e.what());
+    } catch (const smx::CudaError& e) { return fail(SMX_ERR_CUDA, e.what());
+    } catch (const std::exception& e) { return fail(SMX_ERR_INVALID_ARGUMENT, e.what()); }
+}
+template <typename Fn>
+long size_or_refusal(Fn&& fn) {
+    try {
+        return static_cast<long>(fn());
+    } catch (const std::exception&) { return -1; }
+}
+// Calls fn with a null pointer of the precision's type.
+template <typename Fn>
+void with_precision(int precision, const char* what, Fn&& fn) {
+    if (precision == SMX_FP32) fn(static_cast<float*>(nullptr));
+    else if (precision == SMX_FP64) fn(static_cast<double*>(nullptr));
+    else throw smx::ArgError(std::string(what) + ": precision must be 32 or 64");
 }
 }  // namespace
 
@@ -315,6 +347,77 @@ int smx_evaluate(smx_handle h, int num_atoms, const double* positions, const int
 int smx_get_edges(smx_handle h, int* num_neigh, int* neigh_indices, int* neigh_types, int* shifts, double* xyz, double* r,
                   int mem_space) {
     return guarded(h, [&](smx::EvaluatorBase& e) { e.get_edges(num_neigh, neigh_indices, neigh_types, shifts, xyz, r, mem_space); });
+}
+
+long smx_route_plan_bytes(long num_rows, int slots, int num_groups) {
+    return size_or_refusal([&] { return smx::route_plan_bytes(num_rows, slots, num_groups); });
+}
+int smx_route_plan(const int* ids, long num_rows, int slots, int num_groups, int* order, int* position, int* offsets, void* workspace,
+                   long workspace_bytes, void* stream, char* errbuf, int errbuf_len) {
+    return guarded_free(errbuf, errbuf_len, [&] {
+        if (workspace_bytes < 0) throw smx::ArgError("smx_route_plan: negative workspace size");
+        smx::route_plan(ids, num_rows, slots, num_groups, order, position, offsets, workspace, static_cast<size_t>(workspace_bytes),
+                        static_cast<cudaStream_t>(stream));
+    });
+}
+int smx_route_dispatch(int precision, const void* x, long x_stride, long num_rows, int slots, long width, const int* position,
+                       const int* offsets, int num_groups, void* rows, int zero_tail, void* stream, char* errbuf, int errbuf_len) {
+    return guarded_free(errbuf, errbuf_len, [&] {
+        with_precision(precision, "smx_route_dispatch", [&](auto* t) {
+            using T = std::remove_pointer_t<decltype(t)>;
+            smx::route_dispatch<T>(static_cast<const T*>(x), x_stride, num_rows, slots, width, position, offsets, num_groups, static_cast<T*>(rows),
+                                   zero_tail != 0, static_cast<cudaStream_t>(stream));
+        });
+    });
+}
+int smx_route_combine(int precision, const void* rows, const int* position, long num_rows, int slots, long width, const void* weights,
+                      const void* base, long base_stride, void* y, long y_stride, void* stream, char* errbuf, int errbuf_len) {
+    return guarded_free(errbuf, errbuf_len, [&] {
+        with_precision(precision, "smx_route_combine", [&](auto* t) {
+            using T = std::remove_pointer_t<decltype(t)>;
+            smx::route_combine<T>(static_cast<const T*>(rows), position, num_rows, slots, width, static_cast<const T*>(weights),
+                                  static_cast<const T*>(base), base_stride, static_cast<T*>(y), y_stride, static_cast<cudaStream_t>(stream));
+        });
+    });
+}
+int smx_route_combine_backward(int precision, const void* grad_y, long grad_y_stride, const void* rows, const int* position,
+                               const int* offsets, int num_groups, long num_rows, int slots, long width, const void* weights,
+                               void* grad_rows, void* grad_weights, int zero_tail, void* stream, char* errbuf, int errbuf_len) {
+    return guarded_free(errbuf, errbuf_len, [&] {
+        with_precision(precision, "smx_route_combine_backward", [&](auto* t) {
+            using T = std::remove_pointer_t<decltype(t)>;
+            smx::route_combine_backward<T>(static_cast<const T*>(grad_y), grad_y_stride, static_cast<const T*>(rows), position, offsets, num_groups,
+                                           num_rows, slots, width, static_cast<const T*>(weights), static_cast<T*>(grad_rows),
+                                           static_cast<T*>(grad_weights), zero_tail != 0, static_cast<cudaStream_t>(stream));
+        });
+    });
+}
+long smx_adapter_tiles_bytes(const smx_adapter_linear* call) {
+    return call ? size_or_refusal([&] { return smx::adapter_tiles_bytes(*call); }) : -1;
+}
+int smx_adapter_prepare(const smx_adapter_linear* call, int parts, char* errbuf, int errbuf_len) {
+    return guarded_free(errbuf, errbuf_len, [&] {
+        if (!call) throw smx::ArgError("smx_adapter_prepare: null call");
+        smx::adapter_prepare(*call, parts);
+    });
+}
+long smx_adapter_hidden_elements(const smx_adapter_linear* call) {
+    return call ? size_or_refusal([&] { return smx::adapter_hidden_elements(*call); }) : -1;
+}
+long smx_adapter_workspace_bytes(const smx_adapter_linear* call, int backward) {
+    return call ? size_or_refusal([&] { return smx::adapter_workspace_bytes(*call, backward != 0); }) : -1;
+}
+int smx_adapter_forward(const smx_adapter_linear* call, char* errbuf, int errbuf_len) {
+    return guarded_free(errbuf, errbuf_len, [&] {
+        if (!call) throw smx::ArgError("smx_adapter_forward: null call");
+        smx::adapter_forward(*call);
+    });
+}
+int smx_adapter_backward(const smx_adapter_linear* call, char* errbuf, int errbuf_len) {
+    return guarded_free(errbuf, errbuf_len, [&] {
+        if (!call) throw smx::ArgError("smx_adapter_backward: null call");
+        smx::adapter_backward(*call);
+    });
 }
 
 }  // extern "C"

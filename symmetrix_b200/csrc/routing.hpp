@@ -1,0 +1,26 @@
+// Host-side entry points of the row routing and of the linears with low-rank adapters, shared by the extern "C" layer and the
+// evaluator. All work is issued on the given stream of the current device; nothing allocates, nothing waits. Argument errors and launch
+// failures throw (common.cuh).
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include "../../include/symmetrix_b200.h"
+
+namespace smx {
+
+size_t route_plan_bytes(long num_rows, int slots, int num_groups);
+void route_plan(const int* ids, long num_rows, int slots, int num_groups, int* order, int* position, int* offsets, void* workspace,
+                size_t workspace_bytes, cudaStream_t stream);
+template <typename T>
+void route_dispatch(const T* x, long x_stride, long num_rows, int slots, long width, const int* position, const int* offsets, int num_groups,
+                    T* rows, bool zero_tail, cudaStream_t stream);
+template <typename T>
+void route_combine(const T* rows, const int* position, long num_rows, int slots, long width, const T* weights, const T* base, long base_stride,
+                   T* y, long y_stride, cudaStream_t stream);
+template <typename T>
+void route_combine_backward(const T* grad_y, long grad_y_stride, const T* rows, const int* position, const int* offsets, int num_groups,
+                            long num_rows, int slots, long width, const T* weights, T* grad_rows, T* grad_weights, bool zero_tail,
+                            cudaStream_t stream);
+
+}  // namespace smx
