@@ -355,7 +355,7 @@ int smx_route_combine_backward(int precision, const void* grad_y, long grad_y_st
  * atoms are split into chunks of a fixed number of rows and added in order: the same call gives the same bits.
  * The rules of the smx_route_* calls hold: device pointers on the current GPU, `stream`, no allocation, no wait, a workspace of
  * smx_adapter_workspace_bytes bytes for each call that may overlap with another one, errors through `errbuf`. The size functions
- * return -1 for calls that are refused. Limits: rank, degrees as below, those of the routing. */
+ * return -1 for calls that are refused. `tiles`, `hidden` and `workspace` start on 16-byte boundaries. Limits: rank, degrees as below, those of the routing. */
 enum { SMX_ADAPTER_MAX_RANK = 64, SMX_ADAPTER_MAX_DEGREES = 8 };
 enum { SMX_ADAPTER_SHARED = 1, SMX_ADAPTER_MATRICES = 2 };
 typedef struct smx_adapter_degree {

@@ -344,6 +344,8 @@ class AdapterLinear:
         call.x, call.grad_y = _ptr(x), _ptr(grad_y)
         if hidden is not None:
             hidden = _values(hidden, "hidden", (self._library.smx_adapter_hidden_elements(ctypes.byref(call)),), dt, dev).contiguous()
+            if hidden.data_ptr() % 16:
+                hidden = hidden.clone()
             call.hidden = _ptr(hidden) if hidden.numel() else None
         grad_x = grad_down = grad_up = grad_weights = None
         if want_x:

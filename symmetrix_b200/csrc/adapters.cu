@@ -53,9 +53,10 @@ struct Pass {
 // Rows of a tile: pairs [pair0, pair0 + ...) of one group, rows counted in components from row0 of the group.
 struct TileRows { int group; long long first_pair, row0, rows; };
 
-// The tile-th tile of `size` rows, groups one after the other (group `groups`: the pairs behind the last group, if `tail`). Called by one warp.
+// The tile-th tile of `size` rows, groups one after the other (group `groups`: the pairs behind the last group, if `tail`); false, and the number
+// of tiles, if there is none. Called by one warp.
 __device__ __forceinline__ bool find_tile(const int* __restrict__ offsets, int groups, bool tail, long long pairs, int comps, int size, long long tile,
-                                          TileRows& out) {
+                                          TileRows& out, long long& tiles_in_all) {
     const int lane = threadIdx.x & 31;
     long long run = 0;
     for (int g0 = 0; g0 <= groups; g0 += 32) {
@@ -85,6 +86,7 @@ __device__ __forceinline__ bool find_tile(const int* __restrict__ offsets, int g
         }
         run += __shfl_sync(0xffffffffu, incl, 31);
     }
+    tiles_in_all = run;
     return false;
 }
 
@@ -106,9 +108,10 @@ __global__ void __launch_bounds__(kPlainThreads) adapter_pass_plain_kernel(const
     const int tid = threadIdx.x;
     if (tid < 32) {
         TileRows t{};
+        long long all_tiles;
         bool ok;
         if (pass.sorted) {
-            ok = find_tile(pass.offsets, pass.groups, pass.tail != 0, pass.pairs, d.comps, kPlainBM, blockIdx.x, t);
+            ok = find_tile(pass.offsets, pass.groups, pass.tail != 0, pass.pairs, d.comps, kPlainBM, blockIdx.x, t, all_tiles);
         } else {
             const long long all = pass.num_rows * d.comps;
             t.group = pass.groups; t.first_pair = 0; t.row0 = static_cast<long long>(blockIdx.x) * kPlainBM;
@@ -232,7 +235,8 @@ __global__ void __launch_bounds__(kGradThreads) adapter_grad_kernel(const __grid
     const int tid = threadIdx.x, R = pass.rank;
     if (tid < 32) {
         TileRows t{};
-        const bool ok = find_tile(pass.offsets, pass.groups, false, pass.pairs, d.comps, kGradChunk, blockIdx.x, t);
+        long long all_tiles;
+        const bool ok = find_tile(pass.offsets, pass.groups, false, pass.pairs, d.comps, kGradChunk, blockIdx.x, t, all_tiles);
         if (tid == 0) { tile = t; found = ok ? 1 : 0; }
     }
     __syncthreads();
@@ -333,6 +337,14 @@ __global__ void __launch_bounds__(256) adapter_weight_grad_kernel(const __grid_c
     }
 }
 
+}  // namespace
+}  // namespace smx
+
+#include "adapters_f32.cuh"
+
+namespace smx {
+namespace {
+
 // ------------------------------------------------------------------------------------------- layout of the matrices
 struct CopyList {
     static constexpr int kMost = 3 * kMaxDegrees;
@@ -376,9 +388,15 @@ void check_call(const smx_adapter_linear& c) {
         if (static_cast<long long>(c.num_rows) * c.slots * g.components / kPlainBM + c.num_groups + 1 > INT_MAX) throw ArgError("smx_adapter: too many rows");
     }
 }
+// buffers whose layout is the library's own are read and written in 16-byte pieces
+void check_aligned(const smx_adapter_linear& c) {
+    for (const void* p : {static_cast<const void*>(c.tiles), static_cast<const void*>(c.hidden), static_cast<const void*>(c.workspace)})
+        if (reinterpret_cast<uintptr_t>(p) & 15) throw ArgError("smx_adapter: tiles, hidden and workspace must start on 16-byte boundaries");
+}
 void check_plan(const smx_adapter_linear& c) {
     check_call(c);
     if (!c.tiles) throw ArgError("smx_adapter: null tiles");
+    check_aligned(c);
     if (!c.offsets || (c.num_rows > 0 && (!c.order || !c.position))) throw ArgError("smx_adapter: null plan");
 }
 
@@ -427,51 +445,102 @@ Buffers<T> lay_out(const smx_adapter_linear& c, bool backward) {
     return b;
 }
 
-// The matrices of a degree inside `tiles`.
+// The matrices of a degree inside `tiles`: float64 as they are, float32 as operand images of both directions (index 1: transposed).
+struct Matrices {
+    const void *shared[2], *down[2], *up[2];
+    size_t down_group[2], up_group[2];           // values from adapter to adapter
+};
 template <typename T>
-struct Matrices { T *shared, *down, *up; };
-template <typename T>
-size_t tile_layout(const smx_adapter_linear& c, Matrices<T> (&m)[kMaxDegrees]) {
+size_t tile_layout(const smx_adapter_linear& c, Matrices (&m)[kMaxDegrees]) {
     Workspace ws{static_cast<char*>(c.tiles)};
+    const int Rp = padded_rank(c.rank);
     for (int d = 0; d < c.num_degrees; ++d) {
         const smx_adapter_degree& g = c.degrees[d];
         const size_t I = g.in_channels, O = g.out_channels;
-        m[d].shared = g.shared ? ws.take<T>(I * O) : nullptr;
-        m[d].down = ws.take<T>(I * c.rank * c.num_groups);
-        m[d].up = ws.take<T>(O * c.rank * c.num_groups);
+        for (int back = 0; back < 2; ++back) {
+            if (sizeof(T) == 8) {
+                if (back) continue;
+                m[d].shared[0] = g.shared ? ws.take<T>(I * O) : nullptr;
+                m[d].down[0] = ws.take<T>(I * c.rank * c.num_groups);
+                m[d].up[0] = ws.take<T>(O * c.rank * c.num_groups);
+                continue;
+            }
+            // `down` is the first factor forward and the second one backward, `up` the other way round
+            const int K = back ? g.out_channels : g.in_channels, N = back ? g.in_channels : g.out_channels;
+            const size_t tile = 2 * kTsTileBytes / sizeof(float);
+            const size_t first = static_cast<size_t>(ts_chunks(K)) * 2 * Rp * kTsChunk, second = static_cast<size_t>(ts_blocks(N)) * ts_chunks(Rp) * tile;
+            m[d].shared[back] = g.shared ? ws.take<T>(static_cast<size_t>(ts_blocks(N)) * ts_chunks(K) * tile) : nullptr;
+            m[d].down_group[back] = back ? second : first;
+            m[d].up_group[back] = back ? first : second;
+            m[d].down[back] = ws.take<T>(m[d].down_group[back] * c.num_groups);
+            m[d].up[back] = ws.take<T>(m[d].up_group[back] * c.num_groups);
+        }
     }
     return ws.used;
 }
-template <typename T>
+
 void prepare(const smx_adapter_linear& c, int parts) {
-    Matrices<T> m[kMaxDegrees];
-    tile_layout<T>(c, m);
-    CopyList list{};
+    Matrices m[kMaxDegrees];
+    const cudaStream_t stream = static_cast<cudaStream_t>(c.stream);
+    for (int d = 0; d < c.num_degrees; ++d)
+        if ((parts & SMX_ADAPTER_MATRICES) && (!c.degrees[d].down || !c.degrees[d].up)) throw ArgError("smx_adapter_prepare: null matrix");
     int n = 0;
     long long most = 0;
-    auto add = [&](const void* src, T* dst, long long count) {
-        if (!src) throw ArgError("smx_adapter_prepare: null matrix");
-        list.src[n] = src; list.dst[n] = dst; list.count[n++] = count;
-        most = std::max(most, count);
+    if (c.precision == SMX_FP64) {
+        tile_layout<double>(c, m);
+        CopyList list{};
+        auto add = [&](const void* src, const void* dst, long long count) {
+            list.src[n] = src; list.dst[n] = const_cast<void*>(dst); list.count[n++] = count;
+            most = std::max(most, count);
+        };
+        for (int d = 0; d < c.num_degrees; ++d) {
+            const smx_adapter_degree& g = c.degrees[d];
+            const long long I = g.in_channels, O = g.out_channels;
+            if ((parts & SMX_ADAPTER_SHARED) && g.shared) add(g.shared, m[d].shared[0], I * O);
+            if (parts & SMX_ADAPTER_MATRICES) {
+                add(g.down, m[d].down[0], I * c.rank * c.num_groups);
+                add(g.up, m[d].up[0], O * c.rank * c.num_groups);
+            }
+        }
+        if (!n) return;
+        adapter_copy_kernel<double><<<dim3(static_cast<unsigned>(std::min<long long>(256, (most + 255) / 256)), n), 256, 0, stream>>>(list);
+        launched("adapter_copy_kernel");
+        return;
+    }
+    tile_layout<float>(c, m);
+    ImageList list{};
+    auto add = [&](const void* src, const void* dst, int groups, long long group_stride, int K, long long k_stride, int N, long long n_stride, int rows) {
+        ImageSegment& s = list.segment[n++];
+        s.src = static_cast<const float*>(src); s.dst = static_cast<float*>(const_cast<void*>(dst));
+        s.groups = groups; s.group_stride = group_stride; s.K = K; s.k_stride = k_stride; s.N = N; s.n_stride = n_stride;
+        s.rows = rows; s.blocks = (N + rows - 1) / rows; s.chunks = ts_chunks(K);
+        most = std::max(most, static_cast<long long>(groups) * s.blocks * s.chunks * rows * 8);
     };
+    const int R = c.rank, Rp = padded_rank(R);
     for (int d = 0; d < c.num_degrees; ++d) {
         const smx_adapter_degree& g = c.degrees[d];
-        const long long I = g.in_channels, O = g.out_channels;
-        if ((parts & SMX_ADAPTER_SHARED) && g.shared) add(g.shared, m[d].shared, I * O);
+        const int I = g.in_channels, O = g.out_channels;
+        if ((parts & SMX_ADAPTER_SHARED) && g.shared) {
+            add(g.shared, m[d].shared[0], 1, 0, I, O, O, 1, 128);
+            add(g.shared, m[d].shared[1], 1, 0, O, 1, I, O, 128);
+        }
         if (parts & SMX_ADAPTER_MATRICES) {
-            add(g.down, m[d].down, I * c.rank * c.num_groups);
-            add(g.up, m[d].up, O * c.rank * c.num_groups);
+            const long long down = static_cast<long long>(I) * R, up = static_cast<long long>(R) * O;
+            add(g.down, m[d].down[0], c.num_groups, down, I, R, R, 1, Rp);
+            add(g.up, m[d].up[0], c.num_groups, up, R, O, O, 1, 128);
+            add(g.up, m[d].up[1], c.num_groups, up, O, 1, R, O, Rp);
+            add(g.down, m[d].down[1], c.num_groups, down, R, 1, I, R, 128);
         }
     }
     if (!n) return;
-    adapter_copy_kernel<T><<<dim3(static_cast<unsigned>(std::min<long long>(256, (most + 255) / 256)), n), 256, 0, static_cast<cudaStream_t>(c.stream)>>>(list);
-    launched("adapter_copy_kernel");
+    adapter_image_kernel<<<dim3(static_cast<unsigned>(std::min<long long>(1024, (most + 255) / 256)), n), 256, 0, stream>>>(list);
+    launched("adapter_image_kernel");
 }
 
 template <typename T>
 Pass<T> make_pass(const smx_adapter_linear& c, bool transposed, T* hidden) {
     Pass<T> p{};
-    Matrices<T> m[kMaxDegrees];
+    Matrices m[kMaxDegrees];
     tile_layout<T>(c, m);
     long long in_off = 0, out_off = 0;
     const size_t pairs = static_cast<size_t>(c.num_rows) * c.slots;
@@ -479,7 +548,7 @@ Pass<T> make_pass(const smx_adapter_linear& c, bool transposed, T* hidden) {
         const smx_adapter_degree& g = c.degrees[q];
         PassDegree<T>& d = p.degree[q];
         const long long I = g.in_channels, O = g.out_channels, R = c.rank;
-        const T *shared = m[q].shared, *down = m[q].down, *up = m[q].up;
+        const T *shared = static_cast<const T*>(m[q].shared[0]), *down = static_cast<const T*>(m[q].down[0]), *up = static_cast<const T*>(m[q].up[0]);
         d.comps = g.components;
         d.in_off = in_off; d.out_off = out_off;
         d.W = shared;
@@ -506,8 +575,7 @@ Pass<T> make_pass(const smx_adapter_linear& c, bool transposed, T* hidden) {
     return p;
 }
 
-template <typename T>
-void launch_pass(const Pass<T>& p, int degrees, cudaStream_t stream) {
+void launch_pass(const smx_adapter_linear&, bool, const Pass<double>& p, int degrees, cudaStream_t stream) {
     long long rows = 0;
     int cols = 0;
     for (int d = 0; d < degrees; ++d) {
@@ -516,8 +584,53 @@ void launch_pass(const Pass<T>& p, int degrees, cudaStream_t stream) {
     }
     const long long tiles = p.sorted ? rows / kPlainBM + p.groups + 1 : (rows + kPlainBM - 1) / kPlainBM;
     const dim3 grid(static_cast<unsigned>(tiles), (cols + kPlainBN - 1) / kPlainBN, degrees);
-    adapter_pass_plain_kernel<T><<<grid, kPlainThreads, 0, stream>>>(p);
+    adapter_pass_plain_kernel<double><<<grid, kPlainThreads, 0, stream>>>(p);
     launched("adapter_pass_plain_kernel");
+}
+
+void launch_pass(const smx_adapter_linear& c, bool transposed, const Pass<float>& p, int degrees, cudaStream_t stream) {
+    Matrices m[kMaxDegrees];
+    tile_layout<float>(c, m);
+    TsPass t{};
+    long long tiles = 0;
+    for (int q = 0; q < degrees; ++q) {
+        const PassDegree<float>& d = p.degree[q];
+        TsDegree& e = t.degree[q];
+        e.comps = d.comps; e.Kd = d.Kd; e.Nc = d.Nc; e.in_off = d.in_off; e.out_off = d.out_off; e.hidden = d.hidden;
+        e.W = d.W ? static_cast<const float*>(m[q].shared[transposed]) : nullptr;
+        e.first = static_cast<const float*>(transposed ? m[q].up[1] : m[q].down[0]);
+        e.first_group = static_cast<long long>(transposed ? m[q].up_group[1] : m[q].down_group[0]);
+        e.second = static_cast<const float*>(transposed ? m[q].down[1] : m[q].up[0]);
+        e.second_group = static_cast<long long>(transposed ? m[q].down_group[1] : m[q].up_group[0]);
+        const long long rows = (p.sorted ? p.pairs : p.num_rows) * d.comps;
+        tiles += (p.sorted ? rows / kTsRows + p.groups + 1 : (rows + kTsRows - 1) / kTsRows) * (p.out ? ts_blocks(d.Nc) : 1);
+    }
+    t.degrees = degrees; t.rank = p.rank; t.groups = p.groups; t.slots = p.slots; t.num_rows = p.num_rows; t.pairs = p.pairs;
+    t.order = p.order; t.offsets = p.offsets; t.weights = p.weights; t.in = p.in; t.in_stride = p.in_stride; t.out = p.out; t.out_stride = p.out_stride;
+    t.sorted = p.sorted; t.out_sorted = p.out_sorted; t.tail = p.tail;
+    if (tiles > INT_MAX) throw ArgError("smx_adapter: too many rows");
+    const int smem = 2 * (128 + padded_rank(p.rank)) * 256 + 1024;
+    SMX_CUDA(cudaFuncSetAttribute(adapter_pass_f32_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * (128 + 64) * 256 + 1024));
+    adapter_pass_f32_kernel<<<static_cast<unsigned>(tiles), kTsThreads, smem, stream>>>(t);
+    launched("adapter_pass_f32_kernel");
+}
+
+void launch_grads(const GradPass<double>& gp, int problems, long long chunks, int cols, cudaStream_t stream) {
+    adapter_grad_kernel<double><<<dim3(static_cast<unsigned>(chunks), (cols + kGradCols - 1) / kGradCols, problems), kGradThreads, 0, stream>>>(gp);
+    launched("adapter_grad_kernel");
+}
+void launch_grads(const GradPass<float>& gp, int problems, long long, int, cudaStream_t stream) {
+    TsGrad t{};
+    long long ctas = 0;
+    for (int q = 0; q < problems; ++q) {
+        t.problem[q] = gp.problem[q];
+        ctas += (gp.pairs * gp.problem[q].comps / kGradChunk + gp.groups) * ts_blocks(gp.problem[q].Kd);
+    }
+    t.problems = problems; t.rank = gp.rank; t.groups = gp.groups; t.slots = gp.slots; t.pairs = gp.pairs;
+    t.order = gp.order; t.offsets = gp.offsets; t.weights = gp.weights;
+    if (ctas > INT_MAX) throw ArgError("smx_adapter: too many rows");
+    adapter_grad_f32_kernel<<<static_cast<unsigned>(ctas), kTsThreads, padded_rank(gp.rank) * 256 + 1024, stream>>>(t);
+    launched("adapter_grad_f32_kernel");
 }
 
 // out = in W + adapters, in either direction; `hidden` (may be null) receives in . first of every pair. Without `out` that is all.
@@ -532,22 +645,22 @@ void run_pass(const smx_adapter_linear& c, bool transposed, const T* in, long in
     p.sorted = 1;
     if (!out) {
         for (int d = 0; d < c.num_degrees; ++d) { p.degree[d].W = nullptr; p.degree[d].Nc = 1; }      // one (unused) block of columns
-        launch_pass(p, c.num_degrees, stream);
+        launch_pass(c, transposed, p, c.num_degrees, stream);
         return;
     }
     if (c.slots == 1) {
         p.out = out; p.out_stride = out_stride; p.tail = 1;
-        launch_pass(p, c.num_degrees, stream);
+        launch_pass(c, transposed, p, c.num_degrees, stream);
         return;
     }
     // several slots: the shared product of all rows, every pair's own product, and their weighted sum in slot order
     Pass<T> shared = make_pass<T>(c, transposed, nullptr);
     shared.in = in; shared.in_stride = in_stride; shared.out = out; shared.out_stride = out_stride;
-    launch_pass(shared, c.num_degrees, stream);
+    launch_pass(c, transposed, shared, c.num_degrees, stream);
     for (int d = 0; d < c.num_degrees; ++d) p.degree[d].W = nullptr;
     p.weights = nullptr;
     p.out = products; p.out_stride = out_width; p.out_sorted = 1;
-    launch_pass(p, c.num_degrees, stream);
+    launch_pass(c, transposed, p, c.num_degrees, stream);
     route_combine<T>(products, c.position, c.num_rows, c.slots, out_width, static_cast<const T*>(c.weights), out, out_stride, out, out_stride, stream);
 }
 
@@ -615,8 +728,7 @@ void backward(const smx_adapter_linear& c) {
     }
     if (adapters) {
         if (pairs > 0) {
-            adapter_grad_kernel<T><<<dim3(static_cast<unsigned>(chunks), (cols + kGradCols - 1) / kGradCols, 2 * c.num_degrees), kGradThreads, 0, stream>>>(gp);
-            launched("adapter_grad_kernel");
+            launch_grads(gp, 2 * c.num_degrees, chunks, cols, stream);
         }
         const int slabs = static_cast<int>(std::min<long long>(64, (static_cast<long long>(cols) * c.rank + 255) / 256));
         adapter_grad_sum_kernel<T><<<dim3(c.num_groups, slabs, 2 * c.num_degrees), 256, 0, stream>>>(gp);
@@ -646,16 +758,15 @@ size_t adapter_tiles_bytes(const smx_adapter_linear& c) {
     check_call(c);
     smx_adapter_linear empty = c;
     empty.tiles = nullptr;
-    Matrices<float> f[kMaxDegrees];
-    Matrices<double> d[kMaxDegrees];
-    return c.precision == SMX_FP32 ? tile_layout<float>(empty, f) : tile_layout<double>(empty, d);
+    Matrices m[kMaxDegrees];
+    return c.precision == SMX_FP32 ? tile_layout<float>(empty, m) : tile_layout<double>(empty, m);
 }
 void adapter_prepare(const smx_adapter_linear& c, int parts) {
     check_call(c);
     if (!c.tiles) throw ArgError("smx_adapter_prepare: null tiles");
+    check_aligned(c);
     if (parts & ~(SMX_ADAPTER_SHARED | SMX_ADAPTER_MATRICES)) throw ArgError("smx_adapter_prepare: unknown part");
-    if (c.precision == SMX_FP32) prepare<float>(c, parts);
-    else prepare<double>(c, parts);
+    prepare(c, parts);
 }
 void adapter_forward(const smx_adapter_linear& c) {
     check_plan(c);

@@ -83,7 +83,7 @@ def _adapter_call(**over):
     ({"num_groups": 0}, "groups"), ({"num_groups": 1025}, "groups"), ({"slots": 0}, "slots"), ({"num_rows": -1}, "negative"),
     ({"num_rows": 1 << 31}, "32-bit"), ({"degree_components": 0}, "components"), ({"degree_in_channels": 0}, "channels"),
     ({"degree_out_channels": (1 << 20) + 1}, "channels"), ({"tiles": None}, "tiles"), ({"order": None}, "plan"), ({"offsets": None}, "plan"),
-    ({"x": None}, "null x"), ({"y": None}, "null y"), ({"y_stride": 31}, "stride of y"), ({"x_stride": -1}, "stride of x"),
+    ({"tiles": P + 8}, "16-byte"), ({"hidden": P + 4}, "16-byte"), ({"workspace": P + 8}, "16-byte"), ({"x": None}, "null x"), ({"y": None}, "null y"), ({"y_stride": 31}, "stride of y"), ({"x_stride": -1}, "stride of x"),
 ])
 def test_forward_refusals(over, message):
     c = _adapter_call(**over)
