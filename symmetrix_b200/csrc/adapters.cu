@@ -588,6 +588,23 @@ void launch_pass(const smx_adapter_linear&, bool, const Pass<double>& p, int deg
     launched("adapter_pass_plain_kernel");
 }
 
+int sm_count() {
+    int dev = 0, n = 0;
+    SMX_CUDA(cudaGetDevice(&dev));
+    SMX_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
+    return n;
+}
+template <int HP>
+void launch_ts(const TsPass& t, long long tiles, cudaStream_t stream) {
+    using L = TsPassLayout<HP>;
+    // the warps' shares of registers are drawn from what the launch gives: fewer than planned and they would wait for ever
+    cudaFuncAttributes a{};
+    SMX_CUDA(cudaFuncGetAttributes(&a, adapter_pass_f32_kernel<HP>));
+    if (a.numRegs < kTsRegsLaunch) throw CudaError("adapter_pass_f32_kernel was built with too few registers");
+    SMX_CUDA(cudaFuncSetAttribute(adapter_pass_f32_kernel<HP>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::smem));
+    adapter_pass_f32_kernel<HP><<<static_cast<unsigned>(std::min<long long>(tiles, sm_count())), kTsPassThreads, L::smem, stream>>>(t);
+    launched("adapter_pass_f32_kernel");
+}
 void launch_pass(const smx_adapter_linear& c, bool transposed, const Pass<float>& p, int degrees, cudaStream_t stream) {
     Matrices m[kMaxDegrees];
     tile_layout<float>(c, m);
@@ -609,10 +626,18 @@ void launch_pass(const smx_adapter_linear& c, bool transposed, const Pass<float>
     t.order = p.order; t.offsets = p.offsets; t.weights = p.weights; t.in = p.in; t.in_stride = p.in_stride; t.out = p.out; t.out_stride = p.out_stride;
     t.sorted = p.sorted; t.out_sorted = p.out_sorted; t.tail = p.tail;
     if (tiles > INT_MAX) throw ArgError("smx_adapter: too many rows");
-    const int smem = 2 * (128 + padded_rank(p.rank)) * 256 + 1024;
-    SMX_CUDA(cudaFuncSetAttribute(adapter_pass_f32_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * (128 + 64) * 256 + 1024));
-    adapter_pass_f32_kernel<<<static_cast<unsigned>(tiles), kTsThreads, smem, stream>>>(t);
-    launched("adapter_pass_f32_kernel");
+    bool bare = false;
+    for (int q = 0; q < degrees; ++q) bare = bare || !p.degree[q].W;
+    if (bare && p.out && (p.tail || !p.sorted)) {        // with one slot a pair is an atom
+        const Widths w = widths(c);
+        adapter_zero_rows_kernel<<<static_cast<unsigned>(std::min<long long>(p.num_rows, 8LL * sm_count())), 256, 0, stream>>>(
+            p.offsets, p.groups, p.num_rows, p.sorted ? p.order : nullptr, p.out, p.out_stride, static_cast<int>(transposed ? w.in : w.out));
+        launched("adapter_zero_rows_kernel");
+    }
+    if (padded_rank(p.rank) == 16) launch_ts<1>(t, tiles, stream);
+    else if (padded_rank(p.rank) == 32) launch_ts<2>(t, tiles, stream);
+    else if (padded_rank(p.rank) == 48) launch_ts<3>(t, tiles, stream);
+    else launch_ts<4>(t, tiles, stream);
 }
 
 void launch_grads(const GradPass<double>& gp, int problems, long long chunks, int cols, cudaStream_t stream) {
@@ -629,7 +654,9 @@ void launch_grads(const GradPass<float>& gp, int problems, long long, int, cudaS
     t.problems = problems; t.rank = gp.rank; t.groups = gp.groups; t.slots = gp.slots; t.pairs = gp.pairs;
     t.order = gp.order; t.offsets = gp.offsets; t.weights = gp.weights;
     if (ctas > INT_MAX) throw ArgError("smx_adapter: too many rows");
-    adapter_grad_f32_kernel<<<static_cast<unsigned>(ctas), kTsThreads, padded_rank(gp.rank) * 256 + 1024, stream>>>(t);
+    const int HP = padded_rank(gp.rank) / 16;
+    const auto kernel = HP == 1 ? adapter_grad_f32_kernel<1> : HP == 2 ? adapter_grad_f32_kernel<2> : HP == 3 ? adapter_grad_f32_kernel<3> : adapter_grad_f32_kernel<4>;
+    kernel<<<static_cast<unsigned>(ctas), kTsThreads, 16 * HP * 256 + 1024, stream>>>(t);
     launched("adapter_grad_f32_kernel");
 }
 

@@ -12,8 +12,6 @@ namespace {
 
 constexpr int kTsRows = 128, kTsThreads = 128, kTsChunk = 32;              // rows and inner values of a step
 constexpr int kTsTileBytes = 128 * kTsChunk * 4;                           // 128 columns x 32 inner values
-constexpr int kTsSlot = 192;                                               // TMEM: D and hidden columns 0 .. 191, row operand 192 .. 255
-constexpr int kTsColumns = 256;
 
 inline int padded_rank(int rank) { return (rank + 15) & ~15; }
 inline int ts_chunks(int k) { return (k + kTsChunk - 1) / kTsChunk; }
@@ -70,13 +68,14 @@ __device__ __forceinline__ void ts_mma(uint32_t d, uint32_t a, uint64_t b_desc, 
 __device__ __forceinline__ uint32_t ts_idesc(int n) {
     return (1u << 4) | (2u << 7) | (2u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | ((128u >> 4) << 24);
 }
-// The products of one chunk of `steps` x 8 inner values: row operand hi at column a_hi, lo at a_lo; weights hi at b, lo at b + b_lo bytes.
+// The products of one chunk of `steps` x 8 inner values: row operand hi at column a_hi, lo at a_lo; weights hi at b_hi, lo at b_lo. The
+// remainders' products come first, while the sum is small: the tensor core cuts its sums, so an addition costs up to 2^-23 of the sum.
 __device__ __forceinline__ void ts_chunk(uint32_t d, uint32_t a_hi, uint32_t a_lo, uint32_t b_hi, uint32_t b_lo, uint32_t idesc, int steps, bool accumulate) {
     for (int ks = 0; ks < steps; ++ks) {
         ts_mma(d, a_lo + 8 * ks, tc5_smem_desc(b_hi + 32 * ks), idesc, accumulate || ks > 0);
         ts_mma(d, a_hi + 8 * ks, tc5_smem_desc(b_lo + 32 * ks), idesc, true);
-        ts_mma(d, a_hi + 8 * ks, tc5_smem_desc(b_hi + 32 * ks), idesc, true);
     }
+    for (int ks = 0; ks < steps; ++ks) ts_mma(d, a_hi + 8 * ks, tc5_smem_desc(b_hi + 32 * ks), idesc, true);
 }
 __device__ __forceinline__ void ts_commit(unsigned long long* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -141,33 +140,76 @@ struct TsPass {
     float* out; long long out_stride;
     int sorted, out_sorted, tail;                // as in Pass
 };
-struct TsWork { int degree, block; TileRows rows; };
+struct TsWork { long long index; int degree, block, found; TileRows rows; };
 
-// The t-th tile of the pass: degrees, then groups, then row tiles, then column blocks (so that a row tile's blocks run side by side and
-// its rows come from L2 after the first). Called by one warp.
-__device__ __forceinline__ bool ts_find(const TsPass& p, long long t, TsWork& w) {
-    for (int q = 0; q < p.degrees; ++q) {
-        const TsDegree& d = p.degree[q];
-        const int blocks = p.out ? (d.Nc + 127) / 128 : 1;
-        long long tiles;
-        if (p.sorted) {
-            if (find_tile(p.offsets, p.groups, p.tail != 0, p.pairs, d.comps, kTsRows, t / blocks, w.rows, tiles)) {
-                w.degree = q; w.block = static_cast<int>(t % blocks);
+// The tiles of a pass one after the other: degrees, then groups, then row tiles, then column blocks (so that a row tile's blocks run side by
+// side and its rows come from L2 after the first). A cursor remembers the 32 groups it stands at; `t` may only grow. Called by one warp.
+struct TsCursor {
+    int q = 0, g0 = 0;
+    long long before = 0, run = 0;               // work items before degree q, row tiles of degree q before group g0
+    __device__ __forceinline__ bool find(const TsPass& p, long long t, TsWork& w) {
+        const int lane = threadIdx.x & 31;
+        w.found = 0;
+        w.index = t;
+        while (q < p.degrees) {
+            const TsDegree& d = p.degree[q];
+            const int blocks = p.out ? (d.Nc + 127) / 128 : 1;
+            const long long tile = (t - before) / blocks;
+            const int g = g0 + lane;
+            long long first = 0, rows = 0;
+            if (p.sorted) {
+                if (g < p.groups || (g == p.groups && p.tail)) {
+                    first = p.offsets[g];
+                    rows = ((g < p.groups ? p.offsets[g + 1] : p.pairs) - first) * d.comps;
+                }
+            } else if (g == 0) {
+                rows = p.num_rows * d.comps;
+            }
+            const long long tiles = (rows + kTsRows - 1) / kTsRows;
+            long long incl = tiles;
+#pragma unroll
+            for (int s = 1; s < 32; s <<= 1) {
+                const long long up = __shfl_up_sync(0xffffffffu, incl, s);
+                if (lane >= s) incl += up;
+            }
+            const long long begin = run + incl - tiles;
+            const unsigned hit = __ballot_sync(0xffffffffu, tile >= begin && tile < begin + tiles);
+            if (hit) {
+                const int src = __ffs(hit) - 1;
+                w.found = 1; w.degree = q; w.block = static_cast<int>((t - before) % blocks);
+                w.rows.group = p.sorted ? __shfl_sync(0xffffffffu, g, src) : p.groups;
+                w.rows.first_pair = __shfl_sync(0xffffffffu, first, src);
+                const long long b = __shfl_sync(0xffffffffu, begin, src), r = __shfl_sync(0xffffffffu, rows, src);
+                w.rows.row0 = (tile - b) * kTsRows;
+                w.rows.rows = min(static_cast<long long>(kTsRows), r - w.rows.row0);
                 return true;
             }
-        } else {
-            const long long all = p.num_rows * d.comps;
-            tiles = (all + kTsRows - 1) / kTsRows;
-            if (t / blocks < tiles) {
-                w.degree = q; w.block = static_cast<int>(t % blocks);
-                w.rows.group = p.groups; w.rows.first_pair = 0; w.rows.row0 = t / blocks * kTsRows;
-                w.rows.rows = min(static_cast<long long>(kTsRows), all - w.rows.row0);
-                return true;
-            }
+            run += __shfl_sync(0xffffffffu, incl, 31);
+            g0 += 32;
+            if (g0 > p.groups || !p.sorted) { before += run * blocks; ++q; g0 = 0; run = 0; }
         }
-        t -= tiles * blocks;
+        return false;
     }
-    return false;
+};
+
+// What a tile consists of: `nx` chunks of inner values into [shared | hidden] columns, then `rounds` of 32 hidden values into the tile.
+struct TsShape {
+    int group, rows, col0, cols, main_cols, hid_col, nx, rounds;
+    bool adapter;
+};
+__device__ __forceinline__ TsShape ts_shape(const TsPass& p, const TsWork& w) {
+    const TsDegree& d = p.degree[w.degree];
+    TsShape s;
+    s.group = w.rows.group;
+    s.rows = static_cast<int>(w.rows.rows);
+    s.col0 = w.block * 128;
+    s.adapter = s.group < p.groups;
+    s.cols = p.out ? min(128, (d.Nc - s.col0 + 15) & ~15) : 0;
+    s.main_cols = d.W ? s.cols : 0;
+    s.hid_col = s.main_cols ? s.main_cols : 128;
+    s.nx = s.adapter || s.main_cols ? (d.Kd + kTsChunk - 1) / kTsChunk : 0;      // neither: nothing but zeros
+    s.rounds = s.adapter && p.out ? (p.rank + 31) / 32 : 0;
+    return s;
 }
 
 // 32 inner values of a row from k0 on, zero beyond the row's end.
@@ -193,234 +235,429 @@ __device__ __forceinline__ void ts_load_chunk(const float* row, int k0, int Kd, 
     }
 }
 
-// A CTA of 128 threads makes a tile of 128 rows x 128 columns, two CTAs to an SM (256 TMEM columns each). A thread owns a row: it loads 32
-// of its values ahead, splits the previous 32 and stores them to tensor memory; thread 0 issues the products with [W | first_g] (one
-// instruction for the shared and the hidden columns), whose images arrive by bulk copies two chunks ahead. Then every thread takes its hidden
-// row out of tensor memory, keeps it if wanted, weights and splits it in place, and the products with second_g are added to the tile.
-// Waits are bounded; a tile whose wait runs out is filled with NaN.
-__global__ void __launch_bounds__(kTsThreads, 2) adapter_pass_f32_kernel(const __grid_constant__ TsPass pass) {
-    extern __shared__ unsigned char ts_smem_raw[];
-    __shared__ __align__(8) unsigned long long mma_bar, b_bar[2];
-    __shared__ uint32_t tmem_slot;
-    __shared__ long long out_base[kTsRows];
-    __shared__ TsWork shared_work;
-    __shared__ int found, failed;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    if (warp == 0) {
-        TsWork w{};
-        const bool ok = ts_find(pass, blockIdx.x, w);
-        if (lane == 0) { shared_work = w; found = ok ? 1 : 0; failed = 0; }
+// One value into the tile (and its hidden rows, where it writes them), by `count` threads.
+__device__ __forceinline__ void ts_fill(const TsPass& p, const TsWork& w, int thread, int count, float value) {
+    const TsDegree& d = p.degree[w.degree];
+    const TsShape s = ts_shape(p, w);
+    for (int i = thread; i < s.rows; i += count) {
+        const long long r = w.rows.row0 + i, pair = w.rows.first_pair + r / d.comps, m = r % d.comps;
+        const long long n = p.sorted ? p.order[pair] / p.slots : pair;
+        if (p.out)
+            for (int c = s.col0; c < min(d.Nc, s.col0 + 128); ++c) p.out[(p.out_sorted ? pair : n) * p.out_stride + d.out_off + m * d.Nc + c] = value;
+        if (s.adapter && d.hidden && w.block == 0)
+            for (int q = 0; q < p.rank; ++q) d.hidden[(pair * d.comps + m) * p.rank + q] = value;
     }
-    __syncthreads();
-    if (!found) return;
-    const TsDegree& d = pass.degree[shared_work.degree];
-    const int g = shared_work.rows.group, rows = static_cast<int>(shared_work.rows.rows), block = shared_work.block;
-    const bool adapter = g < pass.groups, outputs = pass.out != nullptr;
-    const int R = pass.rank, Rp = (R + 15) & ~15, col0 = block * 128;
-    const int NB = outputs ? min(128, (d.Nc - col0 + 15) & ~15) : 0;        // columns of the tile
-    const int main_cols = d.W && outputs ? NB : 0;
-    const int first_rows = adapter ? Rp : 0;
-    const int hid_col = main_cols ? main_cols : 128;                        // TMEM column of the hidden values
-    const int nx = (d.Kd + kTsChunk - 1) / kTsChunk, ne = adapter && outputs ? (Rp + 31) / 32 : 0;
+}
 
-    if (!adapter && !main_cols) {                    // no product at all: zeros
-        if (tid < rows) {
-            const long long r = shared_work.rows.row0 + tid, p = shared_work.rows.first_pair + r / d.comps;
-            const long long n = pass.sorted ? pass.order[p] / pass.slots : p;
-            float* to = pass.out + (pass.out_sorted ? p : n) * pass.out_stride + d.out_off + (r % d.comps) * d.Nc;
-            for (int c = col0; c < min(d.Nc, col0 + 128); ++c) to[c] = 0.f;
-        }
-        return;
+// Waits of the pass kernel: bounded, and given up at once when another one ran out.
+__device__ __forceinline__ bool ts_wait(unsigned long long* bar, unsigned parity, int* failed) {
+    const uint32_t addr = smem_u32(bar);
+    for (unsigned spin = 0; spin < kMbarSpinLimit; ++spin) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done) : "r"(addr), "r"(parity) : "memory");
+        if (done) return true;
+        if ((spin & 63u) == 63u && *reinterpret_cast<volatile int*>(failed)) return false;
+    }
+    atomicExch(failed, 1);
+    return false;
+}
+__device__ __forceinline__ bool ts_wait_warp(unsigned long long* bar, unsigned parity, int* failed) {
+    return __all_sync(0xffffffffu, ts_wait(bar, parity, failed));
+}
+template <int N> __device__ __forceinline__ void ts_registers_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void ts_registers_less() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// Rows without a group where a linear has no shared weights for them; all `rows` rows without a plan.
+__global__ void __launch_bounds__(256) adapter_zero_rows_kernel(const int* __restrict__ offsets, int groups, long long rows, const int* __restrict__ order,
+                                                                float* __restrict__ out, long long stride, int width) {
+    for (long long p = (order ? offsets[groups] : 0) + blockIdx.x; p < rows; p += gridDim.x)
+        for (int c = threadIdx.x; c < width; c += 256) out[(order ? order[p] : p) * stride + c] = 0.f;
+}
+
+// One persistent CTA per SM walks tiles of 128 rows x 128 columns; its warps are specialised, so that the parts of neighbouring tiles overlap:
+//   warp 0      weight images: bulk copies of a chunk's [W | first_g] tiles, or of a round's second_g tiles, into a ring of stages
+//   warp 1      the products (one thread)
+//   warp 2      finds the tiles (a ring of four, ahead of all others)
+//   warps 4-7   rows: a thread loads its row 96 values ahead, splits 32 at a time and stores them to the tensor memory's row operand
+//   warps 8-11  sums: a thread adds its row's partial sums of every chunk in registers (the tensor core cuts its sums instead of
+//               rounding them: sums of 32 inner values, remainder products first, keep that at float32's level; one sum over 128 inner values was off five
+//               times as far), weights and splits the hidden row into the operand of the second product, adds that, and writes the row
+// Products run in the order chunk 0 of tile i + 1, rounds of tile i, chunks 1 .. of tile i + 1: the hidden rows are on their way through the
+// registers meanwhile. TMEM: two partial sums of 128 + Rp columns, one (Rp > 32) or two row operands and one hidden operand of 64 each.
+// Every wait is bounded; if one runs out, the CTA gives up and fills its remaining tiles with NaN.
+constexpr int kTsPassThreads = 384, kTsStages = 4, kTsWorkRing = 4;
+constexpr int kTsRegsControl = 80, kTsRegsRows = 184, kTsRegsSums = 240, kTsRegsLaunch = 168;
+static_assert(kTsRegsControl + kTsRegsRows + kTsRegsSums <= 3 * kTsRegsLaunch, "the registers of the launch are shared out");
+template <int HP>                                    // hidden columns / 16
+struct TsPassLayout {
+    static constexpr int Rp = 16 * HP, sum_cols = 128 + Rp, slots = HP > 2 ? 1 : 2;
+    static constexpr int slot0 = 2 * sum_cols, hidden0 = slot0 + 64 * slots;
+    static constexpr uint32_t stage_bytes = sum_cols * 256u;
+    static constexpr int smem = kTsStages * static_cast<int>(stage_bytes) + 1024;
+    static_assert(hidden0 + 64 <= 512, "tensor memory has 512 columns");
+};
+
+template <int HP>
+__global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(const __grid_constant__ TsPass pass) {
+    using L = TsPassLayout<HP>;
+    extern __shared__ unsigned char ts_smem_raw[];
+    __shared__ __align__(8) unsigned long long work_full[kTsWorkRing], work_free[kTsWorkRing], b_full[kTsStages], b_free[kTsStages], a_full[2], a_free[2],
+        d_full[2], d_free[2], t_full, t_free;
+    __shared__ TsWork work[kTsWorkRing];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int failed;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    unsigned char* stages = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(ts_smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    if (threadIdx.x == 0) {
+        failed = 0;
+        for (int q = 0; q < kTsWorkRing; ++q) { mbar_init(&work_full[q], 1); mbar_init(&work_free[q], 10); }
+        for (int q = 0; q < kTsStages; ++q) { mbar_init(&b_full[q], 1); mbar_init(&b_free[q], 1); }
+        for (int q = 0; q < 2; ++q) { mbar_init(&a_full[q], 4); mbar_init(&a_free[q], 1); mbar_init(&d_full[q], 1); mbar_init(&d_free[q], 4); }
+        mbar_init(&t_full, 4);
+        mbar_init(&t_free, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(kTsColumns) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    const float* in_row = nullptr;
-    float weight = 1.f;
-    long long hid_row = 0;
-    {
-        long long ob = -1;
-        if (tid < rows) {
-            const long long r = shared_work.rows.row0 + tid, p = shared_work.rows.first_pair + r / d.comps;
-            const int m = static_cast<int>(r % d.comps);
-            const long long pair = pass.sorted ? pass.order[p] : p, n = pass.sorted ? pair / pass.slots : p;
-            in_row = pass.in + n * pass.in_stride + d.in_off + static_cast<long long>(m) * d.Kd;
-            ob = (pass.out_sorted ? p : n) * pass.out_stride + d.out_off + static_cast<long long>(m) * d.Nc;
-            hid_row = p * d.comps + m;
-            if (adapter && pass.weights) weight = pass.weights[pair];
-        }
-        out_base[tid] = ob;
-    }
-    // values every row of the pass is aligned to: 8 (32-byte loads), 4 or fewer
-    const unsigned long long bits = static_cast<unsigned long long>(pass.in_stride | d.in_off | d.Kd) * 4u | reinterpret_cast<uintptr_t>(pass.in);
-    const int align = (bits & 31) == 0 ? 8 : (bits & 15) == 0 ? 4 : 1;
-
-    unsigned char* stages = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(ts_smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    const uint32_t stage_bytes = (128u + Rp) * 256u;
-    auto copy_chunk = [&](int j) {        // thread 0
-        unsigned char* s = stages + (j & 1) * stage_bytes;
-        unsigned long long* bar = &b_bar[j & 1];
-        if (j < nx) {
-            const uint32_t half = (main_cols + first_rows) * 128u;
-            mbar_expect_tx(bar, 2 * half);
-            if (main_cols) {
-                const float* w = d.W + (static_cast<long long>(block) * nx + j) * (2 * kTsTileBytes / 4);
-                bulk_copy_g2s(s, w, main_cols * 128u, bar);
-                bulk_copy_g2s(s + half, w + kTsTileBytes / 4, main_cols * 128u, bar);
-            }
-            if (first_rows) {
-                const float* f = d.first + g * d.first_group + static_cast<long long>(j) * 2 * Rp * kTsChunk;
-                bulk_copy_g2s(s + main_cols * 128u, f, Rp * 128u, bar);
-                bulk_copy_g2s(s + half + main_cols * 128u, f + Rp * kTsChunk, Rp * 128u, bar);
-            }
-        } else {
-            const uint32_t half = NB * 128u;
-            mbar_expect_tx(bar, 2 * half);
-            const float* f = d.second + g * d.second_group + (static_cast<long long>(block) * ((Rp + 31) / 32) + (j - nx)) * (2 * kTsTileBytes / 4);
-            bulk_copy_g2s(s, f, half, bar);
-            bulk_copy_g2s(s + half, f + kTsTileBytes / 4, half, bar);
-        }
-    };
-    if (tid == 0) {
-        mbar_init(&mma_bar, 1);
-        mbar_init(&b_bar[0], 1);
-        mbar_init(&b_bar[1], 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        copy_chunk(0);
-        if (nx + ne > 1) copy_chunk(1);
-    }
     ts_fence_before();
     __syncthreads();
     ts_fence_after();
-    const uint32_t tmem = tmem_slot, lanes = tmem + (static_cast<uint32_t>(warp * 32) << 16);
-    int copied = nx + ne > 1 ? 2 : 1, seen = 0;      // thread 0: chunks whose copies were issued, and waited for
-    auto waited = [&](bool ok) { if (!ok) atomicMax(&failed, 1); };
-    auto issue = [&](int j, bool accumulate) {       // thread 0: the products of chunk j
-        waited(mbar_wait(&b_bar[j & 1], (j >> 1) & 1));
-        seen = j + 1;
-        if (*reinterpret_cast<volatile int*>(&failed)) return;
-        ts_fence_after();
-        const uint32_t b = smem_u32(stages + (j & 1) * stage_bytes);
-        if (j < nx) {
-            const int n = main_cols + first_rows;
-            ts_chunk(tmem + (main_cols ? 0 : 128), tmem + kTsSlot, tmem + kTsSlot + 32, b, b + n * 128u, ts_idesc(n), 4, accumulate);
-        } else {
-            const int e = j - nx;
-            ts_chunk(tmem, tmem + hid_col + 32 * e, tmem + kTsSlot + 32 * e, b, b + NB * 128u, ts_idesc(NB), min(4, Rp / 8 - 4 * e), accumulate);
-        }
-    };
+    const uint32_t tmem = tmem_slot;
 
-    float cur[32], next[32];
-    ts_load_chunk(in_row, 0, d.Kd, align, cur);
-    auto step = [&](int j, float (&v)[32]) {
-        if (j > 0) {
-            if (!*reinterpret_cast<volatile int*>(&failed)) waited(mbar_wait(&mma_bar, (j - 1) & 1));
-            ts_fence_after();
-            if (tid == 0 && j + 1 < nx + ne && !*reinterpret_cast<volatile int*>(&failed)) { copy_chunk(j + 1); copied = j + 2; }
+    if (warp < 4) {
+        ts_registers_less<kTsRegsControl>();
+        if (warp == 2) {
+            TsCursor cursor;
+            long long t = blockIdx.x;
+            for (int i = 0;; ++i) {
+                const int slot = i % kTsWorkRing;
+                if (i >= kTsWorkRing && !ts_wait_warp(&work_free[slot], (i / kTsWorkRing - 1) & 1, &failed)) break;
+                TsWork w{};
+                while (cursor.find(pass, t, w)) {
+                    t += gridDim.x;
+                    if (ts_shape(pass, w).nx > 0) break;                 // no shared weights and no adapter: adapter_zero_rows_kernel's
+                }
+                if (lane == 0) { work[slot] = w; mbar_arrive(&work_full[slot]); }
+                __syncwarp();
+                if (!w.found) break;
+            }
+        } else if (warp == 0 && lane == 0) {
+            int n = 0;                                                   // chunks copied so far
+            bool ok = true;
+            auto stage_free = [&]() { return ok = ok && (n < kTsStages || ts_wait(&b_free[n % kTsStages], (n / kTsStages - 1) & 1, &failed)); };
+            auto chunk = [&](const TsWork& w, const TsShape& s, int j) {
+                if (!stage_free()) return;
+                const TsDegree& d = pass.degree[w.degree];
+                unsigned char* to = stages + (n % kTsStages) * L::stage_bytes;
+                unsigned long long* bar = &b_full[n % kTsStages];
+                const uint32_t half = (s.main_cols + (s.adapter ? L::Rp : 0)) * 128u;
+                mbar_expect_tx(bar, 2 * half);
+                if (s.main_cols) {
+                    const float* m = d.W + (static_cast<long long>(w.block) * s.nx + j) * (2 * kTsTileBytes / 4);
+                    bulk_copy_g2s(to, m, s.main_cols * 128u, bar);
+                    bulk_copy_g2s(to + half, m + kTsTileBytes / 4, s.main_cols * 128u, bar);
+                }
+                if (s.adapter) {
+                    const float* m = d.first + s.group * d.first_group + static_cast<long long>(j) * 2 * L::Rp * kTsChunk;
+                    bulk_copy_g2s(to + s.main_cols * 128u, m, L::Rp * 128u, bar);
+                    bulk_copy_g2s(to + half + s.main_cols * 128u, m + L::Rp * kTsChunk, L::Rp * 128u, bar);
+                }
+                ++n;
+            };
+            auto rounds = [&](const TsWork& w, const TsShape& s) {
+                const TsDegree& d = pass.degree[w.degree];
+                for (int e = 0; e < s.rounds; ++e) {
+                    if (!stage_free()) return;
+                    unsigned char* to = stages + (n % kTsStages) * L::stage_bytes;
+                    unsigned long long* bar = &b_full[n % kTsStages];
+                    const uint32_t half = s.cols * 128u;
+                    mbar_expect_tx(bar, 2 * half);
+                    const float* m = d.second + s.group * d.second_group + (static_cast<long long>(w.block) * s.rounds + e) * (2 * kTsTileBytes / 4);
+                    bulk_copy_g2s(to, m, half, bar);
+                    bulk_copy_g2s(to + half, m + kTsTileBytes / 4, half, bar);
+                    ++n;
+                }
+            };
+            TsWork last{};
+            TsShape last_shape{};
+            for (int i = 0; ok; ++i) {
+                const int slot = i % kTsWorkRing;
+                ok = ts_wait(&work_full[slot], (i / kTsWorkRing) & 1, &failed);
+                if (!ok) break;
+                const TsWork w = work[slot];
+                mbar_arrive(&work_free[slot]);
+                TsShape s{};
+                if (w.found) s = ts_shape(pass, w);
+                if (w.found) chunk(w, s, 0);
+                rounds(last, last_shape);
+                for (int j = 1; j < s.nx; ++j) chunk(w, s, j);
+                if (!w.found) break;
+                last = w;
+                last_shape = s;
+            }
+            if (!ok)                                                     // copies in flight write into this CTA's memory: wait for them (bounded)
+                for (int q = max(0, n - kTsStages); q < n; ++q) mbar_wait(&b_full[q % kTsStages], (q / kTsStages) & 1);
+        } else if (warp == 1 && lane == 0) {
+            int nb = 0, na = 0, nt = 0, nd = 0;                          // stages, row operands, hidden operands and partial sums used so far
+            bool ok = true;
+            auto sums_free = [&]() { return ok = ok && (nd < 2 || ts_wait(&d_free[nd & 1], ((nd >> 1) - 1) & 1, &failed)); };
+            auto chunk = [&](const TsShape& s) {
+                const int slot = L::slots == 2 ? na & 1 : 0, use = L::slots == 2 ? na >> 1 : na;
+                if (!sums_free()) return;
+                ok = ts_wait(&a_full[slot], use & 1, &failed) && ts_wait(&b_full[nb % kTsStages], (nb / kTsStages) & 1, &failed);
+                if (!ok) return;
+                ts_fence_after();
+                const int cols = s.main_cols + (s.adapter ? L::Rp : 0);
+                const uint32_t d = tmem + (nd & 1) * L::sum_cols + (s.main_cols ? 0 : 128), a = tmem + L::slot0 + 64 * slot;
+                const uint32_t b = smem_u32(stages + (nb % kTsStages) * L::stage_bytes);
+                ts_chunk(d, a, a + 32, b, b + cols * 128u, ts_idesc(cols), 4, false);
+                ts_commit(&d_full[nd & 1]);
+                ts_commit(&a_free[slot]);
+                ts_commit(&b_free[nb % kTsStages]);
+                ++nb; ++na; ++nd;
+            };
+            auto rounds = [&](const TsShape& s) {
+                if (s.rounds == 0 || !sums_free()) return;
+                for (int e = 0; e < s.rounds; ++e) {
+                    ok = ts_wait(&t_full, nt & 1, &failed) && ts_wait(&b_full[nb % kTsStages], (nb / kTsStages) & 1, &failed);
+                    if (!ok) return;
+                    ts_fence_after();
+                    const uint32_t a = tmem + L::hidden0, b = smem_u32(stages + (nb % kTsStages) * L::stage_bytes);
+                    ts_chunk(tmem + (nd & 1) * L::sum_cols, a, a + 32, b, b + s.cols * 128u, ts_idesc(s.cols), min(4, L::Rp / 8 - 4 * e), e > 0);
+                    ts_commit(&t_free);
+                    ts_commit(&b_free[nb % kTsStages]);
+                    ++nb; ++nt;
+                }
+                ts_commit(&d_full[nd & 1]);
+                ++nd;
+            };
+            TsShape last{};
+            for (int i = 0; ok; ++i) {
+                const int slot = i % kTsWorkRing;
+                ok = ts_wait(&work_full[slot], (i / kTsWorkRing) & 1, &failed);
+                if (!ok) break;
+                const TsWork w = work[slot];
+                mbar_arrive(&work_free[slot]);
+                TsShape s{};
+                if (w.found) s = ts_shape(pass, w);
+                if (w.found) chunk(s);
+                if (ok) rounds(last);
+                for (int j = 1; j < s.nx && ok; ++j) chunk(s);
+                if (!w.found) break;
+                last = s;
+            }
         }
-        float lo[32];
-#pragma unroll
-        for (int q = 0; q < 32; ++q) ts_split(v[q], v[q], lo[q]);
-        ts_store32(lanes + kTsSlot, v);
-        ts_store32(lanes + kTsSlot + 32, lo);
-        if (j + 2 < nx) ts_load_chunk(in_row, (j + 2) * kTsChunk, d.Kd, align, v);
-        ts_wait_store();
-        ts_fence_before();
-        __syncthreads();
-        if (tid == 0 && !*reinterpret_cast<volatile int*>(&failed)) {
-            issue(j, j > 0);
-            ts_commit(&mma_bar);
-        }
-    };
-    if (nx > 1) ts_load_chunk(in_row, kTsChunk, d.Kd, align, next);
-    for (int j = 0; j < nx; j += 2) {
-        step(j, cur);
-        if (j + 1 < nx) step(j + 1, next);
-    }
-    __syncthreads();                                 // `failed` as thread 0 left it
-    if (!*reinterpret_cast<volatile int*>(&failed)) waited(mbar_wait(&mma_bar, (nx - 1) & 1));
-    ts_fence_after();
-    if (adapter) {
-        if (tid == 0 && nx + 1 < nx + ne && !*reinterpret_cast<volatile int*>(&failed)) { copy_chunk(nx + 1); copied = nx + 2; }
-        for (int r0 = 0; r0 < Rp; r0 += 16) {
-            float h[16], lo[16];
-            ts_load16(lanes + hid_col + r0, h);
-            if (d.hidden && block == 0 && tid < rows) {
-                float* to = d.hidden + hid_row * R + r0;
-                if ((R & 3) == 0) {
-#pragma unroll
-                    for (int q = 0; q < 16; q += 4)
-                        if (r0 + q < R) *reinterpret_cast<float4*>(to + q) = make_float4(h[q], h[q + 1], h[q + 2], h[q + 3]);
-                } else {
-#pragma unroll
-                    for (int q = 0; q < 16; ++q)
-                        if (r0 + q < R) to[q] = h[q];
+    } else if (warp < 8) {
+        ts_registers_more<kTsRegsRows>();
+        const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+        const int tid = threadIdx.x & 127;
+        // values every row of a degree is aligned to: 8 (32-byte loads), 4 or fewer
+        auto alignment = [&](const TsDegree& d) {
+            const unsigned long long bits = static_cast<unsigned long long>(pass.in_stride | d.in_off | d.Kd) * 4u | reinterpret_cast<uintptr_t>(pass.in);
+            return (bits & 31) == 0 ? 8 : (bits & 15) == 0 ? 4 : 1;
+        };
+        const float* row = nullptr;                  // of the tile that is being loaded
+        int tiles = 0, at = 0, chunks = 0, Kd = 0, align = 1;
+        bool more = true, ok = true;
+        // loads the next chunk of the sequence of tiles; false when there is none
+        auto load = [&](float (&v)[32]) -> bool {
+            while (at >= chunks && more) {
+                const int slot = tiles % kTsWorkRing;
+                if (!ts_wait_warp(&work_full[slot], (tiles / kTsWorkRing) & 1, &failed)) { ok = more = false; break; }
+                const TsWork w = work[slot];
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&work_free[slot]);
+                ++tiles;
+                if (!w.found) { more = false; break; }
+                const TsShape s = ts_shape(pass, w);
+                const TsDegree& d = pass.degree[w.degree];
+                at = 0; chunks = s.nx; Kd = d.Kd; align = alignment(d);
+                row = nullptr;
+                if (tid < s.rows) {
+                    const long long r = w.rows.row0 + tid, p = w.rows.first_pair + r / d.comps;
+                    const long long n = pass.sorted ? pass.order[p] / pass.slots : p;
+                    row = pass.in + n * pass.in_stride + d.in_off + (r % d.comps) * d.Kd;
                 }
             }
-            if (!ne) continue;
+            if (at >= chunks) return false;
+            ts_load_chunk(row, at * kTsChunk, Kd, align, v);
+            ++at;
+            return true;
+        };
+        int na = 0;
+        auto store = [&](float (&v)[32]) {
+            const int slot = L::slots == 2 ? na & 1 : 0, use = L::slots == 2 ? na >> 1 : na;
+            if (use > 0 && !ts_wait_warp(&a_free[slot], (use - 1) & 1, &failed)) { ok = false; return; }
+            ts_fence_after();
+            float lo[32];
 #pragma unroll
-            for (int q = 0; q < 16; ++q) ts_split(weight * h[q], h[q], lo[q]);
-            ts_store16(lanes + hid_col + r0, h);
-            ts_store16(lanes + kTsSlot + r0, lo);
-        }
-        if (ne) {
+            for (int q = 0; q < 32; ++q) ts_split(v[q], v[q], lo[q]);
+            ts_store32(lanes + L::slot0 + 64 * slot, v);
+            ts_store32(lanes + L::slot0 + 64 * slot + 32, lo);
             ts_wait_store();
             ts_fence_before();
-            __syncthreads();
-            if (tid == 0 && !*reinterpret_cast<volatile int*>(&failed)) {
-                for (int e = 0; e < ne; ++e) issue(nx + e, main_cols > 0 || e > 0);
-                ts_commit(&mma_bar);
-            }
-            __syncthreads();
-            if (!*reinterpret_cast<volatile int*>(&failed)) waited(mbar_wait(&mma_bar, nx & 1));
-            ts_fence_after();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&a_full[slot]);
+            ++na;
+        };
+        float v0[32], v1[32], v2[32];
+        bool h0 = load(v0), h1 = load(v1), h2 = load(v2);
+        while (ok) {
+            if (!h0) break;
+            store(v0); if (!ok) break; h0 = load(v0);
+            if (!h1) break;
+            store(v1); if (!ok) break; h1 = load(v1);
+            if (!h2) break;
+            store(v2); if (!ok) break; h2 = load(v2);
         }
-    }
-    __syncthreads();
-    const bool bad = *reinterpret_cast<volatile int*>(&failed) != 0;
-    if (bad && tid == 0)                             // copies that may be in flight get one more bounded wait before their memory is given back
-        for (int j = seen; j < copied; ++j) mbar_wait(&b_bar[j & 1], (j >> 1) & 1);
-    if (outputs) {
-        // a thread's row leaves through the idle stages so that a store instruction writes whole rows (16-byte groups XOR-ed with the row)
-        float* stage = reinterpret_cast<float*>(stages) + warp * (32 * 128);
-        if (bad) __syncthreads();
-        for (int cc = 0; cc < NB; cc += 16) {
-            float v[16];
-            ts_load16(lanes + cc, v);
+    } else {
+        ts_registers_more<kTsRegsSums>();
+        const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+        const int tid = threadIdx.x & 127, R = pass.rank;
+        int sum_at = 0, nt = 0, i = 0;               // uses of the partial sums before the tile, hidden operands, tiles
+        bool ok = true, last_rounds = false;
+        TsWork w{};
+        auto next_work = [&](TsWork& to) {
+            const int slot = i % kTsWorkRing;
+            if (!ts_wait_warp(&work_full[slot], (i / kTsWorkRing) & 1, &failed)) { ok = false; return; }
+            to = work[slot];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&work_free[slot]);
+            ++i;
+        };
+        next_work(w);
+        while (ok && w.found) {
+            const TsShape s = ts_shape(pass, w);
+            const TsDegree& d = pass.degree[w.degree];
+            float* out_row = nullptr;
+            float* hid_row = nullptr;
+            float weight = 1.f;
+            if (tid < s.rows) {
+                const long long r = w.rows.row0 + tid, p = w.rows.first_pair + r / d.comps;
+                const int m = static_cast<int>(r % d.comps);
+                const long long pair = pass.sorted ? pass.order[p] : p, n = pass.sorted ? pair / pass.slots : p;
+                if (pass.out) out_row = pass.out + (pass.out_sorted ? p : n) * pass.out_stride + d.out_off + static_cast<long long>(m) * d.Nc + s.col0;
+                if (s.adapter && d.hidden && w.block == 0) hid_row = d.hidden + (p * d.comps + m) * R;
+                if (s.adapter && pass.weights) weight = pass.weights[pair];
+            }
+            float sum[128], hid[16 * HP];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int grp = cc / 4 + j;
-                const float4 f = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-                *reinterpret_cast<float4*>(stage + lane * 128 + ((grp ^ lane) << 2)) = bad ? make_float4(NAN, NAN, NAN, NAN) : f;
+            for (int q = 0; q < 128; ++q) sum[q] = 0.f;
+#pragma unroll
+            for (int q = 0; q < 16 * HP; ++q) hid[q] = 0.f;
+            auto add_columns = [&](uint32_t from, int cols) {
+#pragma unroll
+                for (int cc = 0; cc < 8; ++cc)
+                    if (16 * cc < cols) {
+                        float v[16];
+                        ts_load16(from + 16 * cc, v);
+#pragma unroll
+                        for (int q = 0; q < 16; ++q) sum[16 * cc + q] += v[q];
+                    }
+            };
+            for (int j = 0; j < s.nx; ++j) {
+                const int use = sum_at + j + (j > 0 && last_rounds ? 1 : 0);
+                if (!ts_wait_warp(&d_full[use & 1], (use >> 1) & 1, &failed)) { ok = false; break; }
+                ts_fence_after();
+                const uint32_t from = lanes + (use & 1) * L::sum_cols;
+                add_columns(from, s.main_cols);
+                if (s.adapter)
+#pragma unroll
+                    for (int cc = 0; cc < HP; ++cc) {
+                        float v[16];
+                        ts_load16(from + s.hid_col + 16 * cc, v);
+#pragma unroll
+                        for (int q = 0; q < 16; ++q) hid[16 * cc + q] += v[q];
+                    }
+                ts_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&d_free[use & 1]);
             }
-        }
-        __syncwarp();
-        const unsigned long long obits = static_cast<unsigned long long>(pass.out_stride | d.out_off | d.Nc) * 4u | reinterpret_cast<uintptr_t>(pass.out);
-        const bool wide = (obits & 15) == 0;
-        const int col = col0 + lane * 4;
-        if (lane * 4 < NB)
-#pragma unroll 4
-            for (int r = 0; r < 32; ++r) {
-                const long long ob = out_base[warp * 32 + r];
-                if (ob < 0) continue;
-                const float4 o = *reinterpret_cast<const float4*>(stage + r * 128 + ((lane ^ r) << 2));
-                float* dst = pass.out + ob + col;
-                if (wide && col + 3 < d.Nc) {
-                    *reinterpret_cast<float4*>(dst) = o;
+            if (!ok) break;
+            sum_at += s.nx + (last_rounds ? 1 : 0);
+            if (hid_row) {
+                if ((R & 3) == 0) {
+#pragma unroll
+                    for (int q = 0; q < 16 * HP; q += 4)
+                        if (q < R) *reinterpret_cast<float4*>(hid_row + q) = make_float4(hid[q], hid[q + 1], hid[q + 2], hid[q + 3]);
                 } else {
-                    const float ov[4] = {o.x, o.y, o.z, o.w};
 #pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        if (col + q < d.Nc) dst[q] = ov[q];
+                    for (int q = 0; q < 16 * HP; ++q)
+                        if (q < R) hid_row[q] = hid[q];
                 }
             }
-    } else if (bad && adapter && d.hidden && tid < rows) {
-        for (int q = 0; q < R; ++q) d.hidden[hid_row * R + q] = NAN;
+            TsWork next{};
+            if (s.rounds == 0) {
+                next_work(next);
+            } else {
+#pragma unroll
+                for (int e = 0; e < (HP + 1) / 2; ++e) {
+                    if (nt > 0 && !ts_wait_warp(&t_free, (nt - 1) & 1, &failed)) { ok = false; break; }
+                    ts_fence_after();
+#pragma unroll
+                    for (int cc = 2 * e; cc < 2 * e + 2 && cc < HP; ++cc) {
+                        float hi[16], lo[16];
+#pragma unroll
+                        for (int q = 0; q < 16; ++q) ts_split(weight * hid[16 * cc + q], hi[q], lo[q]);
+                        ts_store16(lanes + L::hidden0 + 16 * (cc - 2 * e), hi);
+                        ts_store16(lanes + L::hidden0 + 32 + 16 * (cc - 2 * e), lo);
+                    }
+                    ts_wait_store();
+                    ts_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&t_full);
+                    ++nt;
+                }
+                if (!ok) break;
+                next_work(next);                     // whether its first chunk comes before the rounds
+                if (!ok) break;
+                const int use = sum_at + (next.found ? 1 : 0);
+                if (!ts_wait_warp(&d_full[use & 1], (use >> 1) & 1, &failed)) { ok = false; break; }
+                ts_fence_after();
+                add_columns(lanes + (use & 1) * L::sum_cols, s.cols);
+                ts_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&d_free[use & 1]);
+            }
+            if (!ok) break;
+            last_rounds = s.rounds > 0;
+            if (out_row) {
+                const int left = d.Nc - s.col0;
+                const uintptr_t bits = reinterpret_cast<uintptr_t>(out_row);
+#pragma unroll
+                for (int q = 0; q < 128; q += 8) {
+                    if (q + 8 <= left && (bits & 31) == 0) {
+                        asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out_row + q), "f"(sum[q]), "f"(sum[q + 1]), "f"(sum[q + 2]),
+                                     "f"(sum[q + 3]), "f"(sum[q + 4]), "f"(sum[q + 5]), "f"(sum[q + 6]), "f"(sum[q + 7]) : "memory");
+                    } else if (q + 8 <= left && (bits & 15) == 0) {
+                        *reinterpret_cast<float4*>(out_row + q) = make_float4(sum[q], sum[q + 1], sum[q + 2], sum[q + 3]);
+                        *reinterpret_cast<float4*>(out_row + q + 4) = make_float4(sum[q + 4], sum[q + 5], sum[q + 6], sum[q + 7]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (q + e < left) out_row[q + e] = sum[q + e];
+                    }
+                }
+            }
+            w = next;
+        }
+        if (!ok) {
+            // NaN into the tile at hand and all that would have followed
+            TsCursor cursor;
+            TsWork lost{};
+            for (long long t = w.found ? w.index : blockIdx.x; cursor.find(pass, t, lost); t += gridDim.x) ts_fill(pass, lost, tid, 128, NAN);
+        }
     }
+    __syncwarp();
     ts_fence_before();
     __syncthreads();
-    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTsColumns) : "memory");
+    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
 // ------------------------------------------------------------------------------------------- gradients of the adapters
@@ -434,9 +671,10 @@ struct TsGrad {
 
 // part[chunk][k][r] as in adapter_grad_kernel: D[k, r] = sum over rows a[row][k] (w h)[row][r]. A thread owns an inner index k of 128 and
 // loads a[row][k] of 32 rows (a warp reads 128 consecutive bytes of each), which is the row operand's transpose for nothing; the hidden values
-// are split into shared memory. One accumulator of at most 64 columns: four CTAs to an SM.
+// are split into shared memory. The sums of every 32 rows are added in registers, as in the pass kernel.
 constexpr int kTsGradColumns = 128, kTsGradSlot = 64;
-__global__ void __launch_bounds__(kTsThreads, 4) adapter_grad_f32_kernel(const __grid_constant__ TsGrad pass) {
+template <int HP>
+__global__ void __launch_bounds__(kTsThreads, HP > 2 ? 2 : HP == 2 ? 3 : 4) adapter_grad_f32_kernel(const __grid_constant__ TsGrad pass) {
     extern __shared__ unsigned char ts_smem_raw[];
     __shared__ __align__(8) unsigned long long mma_bar;
     __shared__ uint32_t tmem_slot;
@@ -463,7 +701,8 @@ __global__ void __launch_bounds__(kTsThreads, 4) adapter_grad_f32_kernel(const _
     __syncthreads();
     if (!found) return;
     const GradProblem<float>& d = pass.problem[which];
-    const int R = pass.rank, Rp = (R + 15) & ~15, rows = static_cast<int>(tile.rows), k = k_block * 128 + tid;
+    constexpr int Rp = 16 * HP;
+    const int R = pass.rank, rows = static_cast<int>(tile.rows), k = k_block * 128 + tid;
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(kTsGradColumns) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -492,7 +731,7 @@ __global__ void __launch_bounds__(kTsThreads, 4) adapter_grad_f32_kernel(const _
     const uint32_t tmem = tmem_slot, lanes = tmem + (static_cast<uint32_t>(warp * 32) << 16);
     const float* hidden = d.hidden + (tile.first_pair * d.comps + tile.row0) * R;
     const int hid_values = 32 * R;
-    float a[32], h[16];
+    float a[32], h[4 * HP];
     auto load = [&](int s) {
 #pragma unroll
         for (int q = 0; q < 32; ++q) {
@@ -500,25 +739,37 @@ __global__ void __launch_bounds__(kTsThreads, 4) adapter_grad_f32_kernel(const _
             a[q] = i < rows && k < d.Kd ? __ldg(d.a + a_base[i] + k) : 0.f;
         }
 #pragma unroll
-        for (int q = 0; q < 16; ++q) {
+        for (int q = 0; q < 4 * HP; ++q) {
             const int e = tid + q * kTsThreads;
             h[q] = e < hid_values && s * 32 + e / R < rows ? __ldg(hidden + static_cast<long long>(s) * hid_values + e) * row_weight[s * 32 + e / R] : 0.f;
         }
     };
     const int steps = (rows + 31) / 32;
+    float sum[Rp];
+#pragma unroll
+    for (int q = 0; q < Rp; ++q) sum[q] = 0.f;
+    auto add_step = [&](int s) {                     // the sums of step s into registers
+        if (!*reinterpret_cast<volatile int*>(&failed) && !mbar_wait(&mma_bar, s & 1)) atomicMax(&failed, 1);
+        __syncwarp();
+        ts_fence_after();
+#pragma unroll
+        for (int r0 = 0; r0 < Rp; r0 += 16) {
+            float v[16];
+            ts_load16(lanes + r0, v);
+#pragma unroll
+            for (int q = 0; q < 16; ++q) sum[r0 + q] += v[q];
+        }
+    };
     load(0);
     for (int s = 0; s < steps; ++s) {
-        if (s > 0) {
-            if (!*reinterpret_cast<volatile int*>(&failed) && !mbar_wait(&mma_bar, (s - 1) & 1)) atomicMax(&failed, 1);
-            ts_fence_after();
-        }
+        if (s > 0) add_step(s - 1);
         float lo[32];
 #pragma unroll
         for (int q = 0; q < 32; ++q) ts_split(a[q], a[q], lo[q]);
         ts_store32(lanes + kTsGradSlot, a);
         ts_store32(lanes + kTsGradSlot + 32, lo);
 #pragma unroll
-        for (int q = 0; q < 16; ++q) {
+        for (int q = 0; q < 4 * HP; ++q) {
             const int e = tid + q * kTsThreads;
             if (e < hid_values) {
                 const int i = e / R, r = e % R;
@@ -537,24 +788,19 @@ __global__ void __launch_bounds__(kTsThreads, 4) adapter_grad_f32_kernel(const _
         if (tid == 0 && !*reinterpret_cast<volatile int*>(&failed)) {
             ts_fence_after();
             const uint32_t b = smem_u32(B);
-            ts_chunk(tmem, tmem + kTsGradSlot, tmem + kTsGradSlot + 32, b, b + Rp * 128, ts_idesc(Rp), 4, s > 0);
+            ts_chunk(tmem, tmem + kTsGradSlot, tmem + kTsGradSlot + 32, b, b + Rp * 128, ts_idesc(Rp), 4, false);
             ts_commit(&mma_bar);
         }
     }
     __syncthreads();
-    if (!*reinterpret_cast<volatile int*>(&failed) && !mbar_wait(&mma_bar, (steps - 1) & 1)) atomicMax(&failed, 1);
+    add_step(steps - 1);
     __syncthreads();
-    ts_fence_after();
     const bool bad = *reinterpret_cast<volatile int*>(&failed) != 0;
-    for (int r0 = 0; r0 < Rp; r0 += 16) {
-        float v[16];
-        ts_load16(lanes + r0, v);
-        if (k < d.Kd) {
-            float* to = d.part + (chunk_index * d.Kd + k) * R + r0;
+    if (k < d.Kd) {
+        float* to = d.part + (chunk_index * d.Kd + k) * R;
 #pragma unroll
-            for (int q = 0; q < 16; ++q)
-                if (r0 + q < R) to[q] = bad ? NAN : v[q];
-        }
+        for (int q = 0; q < Rp; ++q)
+            if (q < R) to[q] = bad ? NAN : sum[q];
     }
     ts_fence_before();
     __syncthreads();
