@@ -17,9 +17,11 @@ inline int padded_rank(int rank) { return (rank + 15) & ~15; }
 inline int ts_chunks(int k) { return (k + kTsChunk - 1) / kTsChunk; }
 inline int ts_blocks(int n) { return (n + 127) / 128; }
 
+// x = hi + lo, both rounded to TF32 (half away from zero; as integers, since conversions run at a quarter of the rate). The tensor core
+// cuts its operands to their 11 leading bits, so lo need not be: half a step is added to it.
 __device__ __forceinline__ void ts_split(float x, float& hi, float& lo) {
-    hi = __uint_as_float(to_tf32(x));
-    lo = __uint_as_float(to_tf32(x - hi));
+    hi = __uint_as_float((__float_as_uint(x) + 0x1000u) & kTc5HiMask);
+    lo = __uint_as_float(__float_as_uint(x - hi) + 0x1000u);
 }
 
 __device__ __forceinline__ void ts_store32(uint32_t taddr, const float (&v)[32]) {
@@ -40,6 +42,12 @@ __device__ __forceinline__ void ts_store16(uint32_t taddr, const float (&v)[16])
         ::"r"(taddr), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]),
         "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15])
         : "memory");
+}
+__device__ __forceinline__ void ts_load32(uint32_t taddr, float (&v)[32]) {
+    uint32_t u[32];
+    tc5_ld32(taddr, u);
+#pragma unroll
+    for (int q = 0; q < 32; ++q) v[q] = __uint_as_float(u[q]);
 }
 __device__ __forceinline__ void ts_load16(uint32_t taddr, float (&v)[16]) {
     uint32_t u[16];
@@ -192,9 +200,10 @@ struct TsCursor {
     }
 };
 
-// What a tile consists of: `nx` chunks of inner values into [shared | hidden] columns, then `rounds` of 32 hidden values into the tile.
+// What a tile consists of: `nx` chunks of 32 inner values into [shared | hidden] columns, two of them to a partial sum (`sums`), then `rounds` of
+// 32 hidden values into the tile.
 struct TsShape {
-    int group, rows, col0, cols, main_cols, hid_col, nx, rounds;
+    int group, rows, col0, cols, main_cols, hid_col, nx, sums, rounds;
     bool adapter;
 };
 __device__ __forceinline__ TsShape ts_shape(const TsPass& p, const TsWork& w) {
@@ -208,31 +217,9 @@ __device__ __forceinline__ TsShape ts_shape(const TsPass& p, const TsWork& w) {
     s.main_cols = d.W ? s.cols : 0;
     s.hid_col = s.main_cols ? s.main_cols : 128;
     s.nx = s.adapter || s.main_cols ? (d.Kd + kTsChunk - 1) / kTsChunk : 0;      // neither: nothing but zeros
+    s.sums = (s.nx + 1) / 2;
     s.rounds = s.adapter && p.out ? (p.rank + 31) / 32 : 0;
     return s;
-}
-
-// 32 inner values of a row from k0 on, zero beyond the row's end.
-__device__ __forceinline__ void ts_load_chunk(const float* row, int k0, int Kd, int align, float (&v)[32]) {
-    if (row && k0 + 32 <= Kd && align >= 4) {
-        if (align >= 8) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-                asm volatile("ld.global.nc.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                             : "=f"(v[8 * q]), "=f"(v[8 * q + 1]), "=f"(v[8 * q + 2]), "=f"(v[8 * q + 3]), "=f"(v[8 * q + 4]), "=f"(v[8 * q + 5]),
-                               "=f"(v[8 * q + 6]), "=f"(v[8 * q + 7])
-                             : "l"(row + k0 + 8 * q));
-        } else {
-#pragma unroll
-            for (int q = 0; q < 8; ++q) {
-                const float4 f = __ldg(reinterpret_cast<const float4*>(row + k0) + q);
-                v[4 * q] = f.x; v[4 * q + 1] = f.y; v[4 * q + 2] = f.z; v[4 * q + 3] = f.w;
-            }
-        }
-    } else {
-#pragma unroll
-        for (int q = 0; q < 32; ++q) v[q] = row && k0 + q < Kd ? __ldg(row + k0 + q) : 0.f;
-    }
 }
 
 // One value into the tile (and its hidden rows, where it writes them), by `count` threads.
@@ -278,47 +265,66 @@ __global__ void __launch_bounds__(256) adapter_zero_rows_kernel(const int* __res
         for (int c = threadIdx.x; c < width; c += 256) out[(order ? order[p] : p) * stride + c] = 0.f;
 }
 
+__device__ __forceinline__ void cp_async4(void* smem, const void* gmem) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(smem)), "l"(gmem) : "memory");
+}
+
 // One persistent CTA per SM walks tiles of 128 rows x 128 columns; its warps are specialised, so that the parts of neighbouring tiles overlap:
 //   warp 0      weight images: bulk copies of a chunk's [W | first_g] tiles, or of a round's second_g tiles, into a ring of stages
 //   warp 1      the products (one thread)
-//   warp 2      finds the tiles (a ring of four, ahead of all others)
-//   warps 4-7   rows: a thread loads its row 96 values ahead, splits 32 at a time and stores them to the tensor memory's row operand
-//   warps 8-11  sums: a thread adds its row's partial sums of every chunk in registers (the tensor core cuts its sums instead of
-//               rounding them: sums of 32 inner values, remainder products first, keep that at float32's level; one sum over 128 inner values was off five
-//               times as far), weights and splits the hidden row into the operand of the second product, adds that, and writes the row
-// Products run in the order chunk 0 of tile i + 1, rounds of tile i, chunks 1 .. of tile i + 1: the hidden rows are on their way through the
-// registers meanwhile. TMEM: two partial sums of 128 + Rp columns, one (Rp > 32) or two row operands and one hidden operand of 64 each.
+//   warp 2      finds the tiles and looks up their atoms and weights (a ring of four, ahead of all others)
+//   warp 3      rows: 64 values of each by asynchronous copies of 16 bytes (4 where rows start on no 16-byte boundary) into a ring of two stages
+//               (loads and stores by the thread that owns a row touch 32 rows an instruction; a bulk copy of 256 bytes took 70 cycles to issue)
+//   warps 4-7   a thread splits 32 values of its row at a time and stores them to the tensor memory's row operand
+//   warps 8-15  a thread adds half of its row's partial sums of every 64 inner values in registers (the tensor core cuts its sums instead of
+//               rounding them: a single sum over 128 inner values was off five times as far as float32) and writes its half of the row, 16
+//               columns at a time through shared memory, while the products of the next tile run
+// TMEM: two partial sums of 128 + Rp columns, taken in turn, and two or three row operands of 64. The shared columns of a tile's last two
+// sums stay where they are while its hidden row is weighted, split and stored into their hidden columns (head in the last one's, remainder in
+// the other's); the products with second_g go on top of the last sum, and both are read then.
 // Every wait is bounded; if one runs out, the CTA gives up and fills its remaining tiles with NaN.
-constexpr int kTsPassThreads = 384, kTsStages = 4, kTsWorkRing = 4;
-constexpr int kTsRegsControl = 80, kTsRegsRows = 184, kTsRegsSums = 240, kTsRegsLaunch = 168;
-static_assert(kTsRegsControl + kTsRegsRows + kTsRegsSums <= 3 * kTsRegsLaunch, "the registers of the launch are shared out");
+constexpr int kTsPassThreads = 512, kTsWorkRing = 4, kTsRowStages = 2;
+constexpr int kTsRowValues = 64, kTsRowPitch = kTsRowValues + 4;              // floats: threads that read their rows 16 bytes at a time hit all banks
+constexpr int kTsOutPitch = 20;
+constexpr int kTsRegsControl = 72, kTsRegsRows = 120, kTsRegsSums = 160, kTsRegsLaunch = 128;
+static_assert(kTsRegsControl + kTsRegsRows + 2 * kTsRegsSums <= 4 * kTsRegsLaunch, "the registers of the launch are shared out");
 template <int HP>                                    // hidden columns / 16
 struct TsPassLayout {
-    static constexpr int Rp = 16 * HP, sum_cols = 128 + Rp, slots = HP > 2 ? 1 : 2;
-    static constexpr int slot0 = 2 * sum_cols, hidden0 = slot0 + 64 * slots;
+    static constexpr int Rp = 16 * HP, sum_cols = 128 + Rp, slots = HP > 2 ? 2 : 3, stages = HP > 2 ? 2 : 3;
+    static constexpr int slot0 = 2 * sum_cols;
     static constexpr uint32_t stage_bytes = sum_cols * 256u;
-    static constexpr int smem = kTsStages * static_cast<int>(stage_bytes) + 1024;
-    static_assert(hidden0 + 64 <= 512, "tensor memory has 512 columns");
+    static constexpr int row_floats = kTsRows * kTsRowPitch, out_floats = 32 * kTsOutPitch;
+    static constexpr int smem = stages * static_cast<int>(stage_bytes) + (kTsRowStages * row_floats + 8 * out_floats) * 4 + 1024;
+    static_assert(slot0 + 64 * slots <= 512, "tensor memory has 512 columns");
+    static_assert(smem + 9 * 1024 <= 227 * 1024, "shared memory of one CTA per SM");
 };
 
 template <int HP>
 __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(const __grid_constant__ TsPass pass) {
     using L = TsPassLayout<HP>;
+    constexpr int NS = L::stages;
     extern __shared__ unsigned char ts_smem_raw[];
-    __shared__ __align__(8) unsigned long long work_full[kTsWorkRing], work_free[kTsWorkRing], b_full[kTsStages], b_free[kTsStages], a_full[2], a_free[2],
-        d_full[2], d_free[2], t_full, t_free;
+    __shared__ __align__(8) unsigned long long work_full[kTsWorkRing], work_free[kTsWorkRing], b_full[NS], b_free[NS], x_full[kTsRowStages],
+        x_free[kTsRowStages], a_full[3], a_free[3], d_full[2], d_free[2], t_full, t_done;
     __shared__ TsWork work[kTsWorkRing];
+    __shared__ int work_atom[kTsWorkRing][kTsRows], work_place[kTsWorkRing][kTsRows];      // row of `in`, sorted position
+    __shared__ short work_comp[kTsWorkRing][kTsRows];
+    __shared__ float work_weight[kTsWorkRing][kTsRows];
     __shared__ uint32_t tmem_slot;
     __shared__ int failed;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     unsigned char* stages = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(ts_smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    float* row_stages = reinterpret_cast<float*>(stages + NS * L::stage_bytes);
+    float* out_stages = row_stages + kTsRowStages * L::row_floats;
     if (threadIdx.x == 0) {
         failed = 0;
-        for (int q = 0; q < kTsWorkRing; ++q) { mbar_init(&work_full[q], 1); mbar_init(&work_free[q], 10); }
-        for (int q = 0; q < kTsStages; ++q) { mbar_init(&b_full[q], 1); mbar_init(&b_free[q], 1); }
-        for (int q = 0; q < 2; ++q) { mbar_init(&a_full[q], 4); mbar_init(&a_free[q], 1); mbar_init(&d_full[q], 1); mbar_init(&d_free[q], 4); }
-        mbar_init(&t_full, 4);
-        mbar_init(&t_free, 1);
+        for (int q = 0; q < kTsWorkRing; ++q) { mbar_init(&work_full[q], 1); mbar_init(&work_free[q], 15); }
+        for (int q = 0; q < NS; ++q) { mbar_init(&b_full[q], 1); mbar_init(&b_free[q], 1); }
+        for (int q = 0; q < kTsRowStages; ++q) { mbar_init(&x_full[q], 32); mbar_init(&x_free[q], 4); }
+        for (int q = 0; q < 3; ++q) { mbar_init(&a_full[q], 4); mbar_init(&a_free[q], 1); }
+        for (int q = 0; q < 2; ++q) { mbar_init(&d_full[q], 1); mbar_init(&d_free[q], 8); }
+        mbar_init(&t_full, 8);
+        mbar_init(&t_done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) {
@@ -343,19 +349,97 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
                     t += gridDim.x;
                     if (ts_shape(pass, w).nx > 0) break;                 // no shared weights and no adapter: adapter_zero_rows_kernel's
                 }
-                if (lane == 0) { work[slot] = w; mbar_arrive(&work_full[slot]); }
+                if (w.found) {
+                    const int comps = pass.degree[w.degree].comps;
+                    const long long p0 = w.rows.first_pair + w.rows.row0 / comps;
+                    const int m0 = static_cast<int>(w.rows.row0 % comps);
+                    const bool weighted = w.rows.group < pass.groups && pass.weights;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int at = lane + 32 * q;
+                        int atom = 0, place = 0, comp = 0;
+                        float weight = 1.f;
+                        if (at < w.rows.rows) {
+                            const int ahead = (m0 + at) / comps;
+                            place = static_cast<int>(p0) + ahead;
+                            comp = m0 + at - ahead * comps;
+                            const int pair = pass.sorted ? pass.order[place] : place;
+                            atom = pass.sorted ? pair / pass.slots : pair;
+                            if (weighted) weight = pass.weights[pair];
+                        }
+                        work_atom[slot][at] = atom;
+                        work_place[slot][at] = place;
+                        work_comp[slot][at] = static_cast<short>(comp);
+                        work_weight[slot][at] = weight;
+                    }
+                }
+                if (lane == 0) work[slot] = w;
                 __syncwarp();
+                if (lane == 0) mbar_arrive(&work_full[slot]);
                 if (!w.found) break;
             }
+        } else if (warp == 3) {
+            int n = 0;                                                   // stages filled so far
+            bool ok = true;
+            for (int i = 0; ok; ++i) {
+                const int slot = i % kTsWorkRing;
+                if (!ts_wait_warp(&work_full[slot], (i / kTsWorkRing) & 1, &failed)) { ok = false; break; }
+                const TsWork w = work[slot];
+                if (!w.found) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&work_free[slot]);
+                    break;
+                }
+                const TsDegree& d = pass.degree[w.degree];
+                const int rows = static_cast<int>(w.rows.rows);
+                const unsigned long long bits = static_cast<unsigned long long>(pass.in_stride | d.in_off | d.Kd) * 4u | reinterpret_cast<uintptr_t>(pass.in);
+                const bool wide = (bits & 15) == 0;
+                const float* from[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int at = lane + 32 * q;
+                    from[q] = pass.in + work_atom[slot][at] * pass.in_stride + d.in_off + work_comp[slot][at] * d.Kd;
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&work_free[slot]);
+                for (int k0 = 0; k0 < d.Kd && ok; k0 += kTsRowValues) {
+                    const int st = n % kTsRowStages, left = min(kTsRowValues, d.Kd - k0);
+                    if (n >= kTsRowStages && !ts_wait_warp(&x_free[st], (n / kTsRowStages - 1) & 1, &failed)) { ok = false; break; }
+                    float* to = row_stages + st * L::row_floats;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const unsigned long long mine = reinterpret_cast<unsigned long long>(from[q] + k0);
+                        if (wide) {                  // two rows an instruction, 16 bytes a lane
+                            const int c = (lane & 15) * 4;
+#pragma unroll 4
+                            for (int r = 0; r < 32; r += 2) {
+                                const int row = r + (lane >> 4);
+                                const float* src = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, mine, row)) + c;
+                                if (32 * q + row < rows && c < left) cp_async16(to + (32 * q + row) * kTsRowPitch + c, src, 16);
+                            }
+                        } else {
+#pragma unroll 4
+                            for (int row = 0; row < 32; ++row) {
+                                const float* src = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, mine, row));
+                                if (32 * q + row < rows)
+                                    for (int c = lane; c < left; c += 32) cp_async4(to + (32 * q + row) * kTsRowPitch + c, src + c);
+                            }
+                        }
+                    }
+                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&x_full[st])) : "memory");
+                    ++n;
+                }
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");             // none may be in flight when the CTA ends
         } else if (warp == 0 && lane == 0) {
             int n = 0;                                                   // chunks copied so far
             bool ok = true;
-            auto stage_free = [&]() { return ok = ok && (n < kTsStages || ts_wait(&b_free[n % kTsStages], (n / kTsStages - 1) & 1, &failed)); };
+            auto stage_free = [&]() { return ok = ok && (n < NS || ts_wait(&b_free[n % NS], (n / NS - 1) & 1, &failed)); };
             auto chunk = [&](const TsWork& w, const TsShape& s, int j) {
                 if (!stage_free()) return;
                 const TsDegree& d = pass.degree[w.degree];
-                unsigned char* to = stages + (n % kTsStages) * L::stage_bytes;
-                unsigned long long* bar = &b_full[n % kTsStages];
+                unsigned char* to = stages + (n % NS) * L::stage_bytes;
+                unsigned long long* bar = &b_full[n % NS];
                 const uint32_t half = (s.main_cols + (s.adapter ? L::Rp : 0)) * 128u;
                 mbar_expect_tx(bar, 2 * half);
                 if (s.main_cols) {
@@ -374,8 +458,8 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
                 const TsDegree& d = pass.degree[w.degree];
                 for (int e = 0; e < s.rounds; ++e) {
                     if (!stage_free()) return;
-                    unsigned char* to = stages + (n % kTsStages) * L::stage_bytes;
-                    unsigned long long* bar = &b_full[n % kTsStages];
+                    unsigned char* to = stages + (n % NS) * L::stage_bytes;
+                    unsigned long long* bar = &b_full[n % NS];
                     const uint32_t half = s.cols * 128u;
                     mbar_expect_tx(bar, 2 * half);
                     const float* m = d.second + s.group * d.second_group + (static_cast<long long>(w.block) * s.rounds + e) * (2 * kTsTileBytes / 4);
@@ -384,274 +468,271 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
                     ++n;
                 }
             };
-            TsWork last{};
-            TsShape last_shape{};
             for (int i = 0; ok; ++i) {
                 const int slot = i % kTsWorkRing;
                 ok = ts_wait(&work_full[slot], (i / kTsWorkRing) & 1, &failed);
                 if (!ok) break;
                 const TsWork w = work[slot];
                 mbar_arrive(&work_free[slot]);
-                TsShape s{};
-                if (w.found) s = ts_shape(pass, w);
-                if (w.found) chunk(w, s, 0);
-                rounds(last, last_shape);
-                for (int j = 1; j < s.nx; ++j) chunk(w, s, j);
                 if (!w.found) break;
-                last = w;
-                last_shape = s;
+                const TsShape s = ts_shape(pass, w);
+                for (int j = 0; j < s.nx; ++j) chunk(w, s, j);
+                rounds(w, s);
             }
-            if (!ok)                                                     // copies in flight write into this CTA's memory: wait for them (bounded)
-                for (int q = max(0, n - kTsStages); q < n; ++q) mbar_wait(&b_full[q % kTsStages], (q / kTsStages) & 1);
+            if (!ok)
+                for (int q = max(0, n - NS); q < n; ++q) mbar_wait(&b_full[q % NS], (q / NS) & 1);
         } else if (warp == 1 && lane == 0) {
-            int nb = 0, na = 0, nt = 0, nd = 0;                          // stages, row operands, hidden operands and partial sums used so far
+            int nb = 0, na = 0, nt = 0, nd = 0;                          // stages, row operands, hidden rows and partial sums used so far
             bool ok = true;
-            auto sums_free = [&]() { return ok = ok && (nd < 2 || ts_wait(&d_free[nd & 1], ((nd >> 1) - 1) & 1, &failed)); };
-            auto chunk = [&](const TsShape& s) {
-                const int slot = L::slots == 2 ? na & 1 : 0, use = L::slots == 2 ? na >> 1 : na;
-                if (!sums_free()) return;
-                ok = ts_wait(&a_full[slot], use & 1, &failed) && ts_wait(&b_full[nb % kTsStages], (nb / kTsStages) & 1, &failed);
+            auto chunk = [&](const TsShape& s, int j) {
+                const int slot = na % L::slots;
+                if ((j & 1) == 0 && nd >= 2) ok = ts_wait(&d_free[nd & 1], ((nd >> 1) - 1) & 1, &failed);
+                ok = ok && ts_wait(&a_full[slot], (na / L::slots) & 1, &failed) && ts_wait(&b_full[nb % NS], (nb / NS) & 1, &failed);
                 if (!ok) return;
                 ts_fence_after();
                 const int cols = s.main_cols + (s.adapter ? L::Rp : 0);
                 const uint32_t d = tmem + (nd & 1) * L::sum_cols + (s.main_cols ? 0 : 128), a = tmem + L::slot0 + 64 * slot;
-                const uint32_t b = smem_u32(stages + (nb % kTsStages) * L::stage_bytes);
-                ts_chunk(d, a, a + 32, b, b + cols * 128u, ts_idesc(cols), 4, false);
-                ts_commit(&d_full[nd & 1]);
+                const uint32_t b = smem_u32(stages + (nb % NS) * L::stage_bytes);
+                ts_chunk(d, a, a + 32, b, b + cols * 128u, ts_idesc(cols), 4, (j & 1) != 0);
                 ts_commit(&a_free[slot]);
-                ts_commit(&b_free[nb % kTsStages]);
-                ++nb; ++na; ++nd;
+                ts_commit(&b_free[nb % NS]);
+                ++nb; ++na;
+                if ((j & 1) != 0 || j + 1 == s.nx) { ts_commit(&d_full[nd & 1]); ++nd; }
             };
             auto rounds = [&](const TsShape& s) {
-                if (s.rounds == 0 || !sums_free()) return;
-                for (int e = 0; e < s.rounds; ++e) {
-                    ok = ts_wait(&t_full, nt & 1, &failed) && ts_wait(&b_full[nb % kTsStages], (nb / kTsStages) & 1, &failed);
+                if (s.rounds == 0) return;
+                const int sum = (nd - 1) & 1;        // the last one's
+                ok = ts_wait(&t_full, nt & 1, &failed);
+                for (int e = 0; e < s.rounds && ok; ++e) {
+                    ok = ts_wait(&b_full[nb % NS], (nb / NS) & 1, &failed);
                     if (!ok) return;
                     ts_fence_after();
-                    const uint32_t a = tmem + L::hidden0, b = smem_u32(stages + (nb % kTsStages) * L::stage_bytes);
-                    ts_chunk(tmem + (nd & 1) * L::sum_cols, a, a + 32, b, b + s.cols * 128u, ts_idesc(s.cols), min(4, L::Rp / 8 - 4 * e), e > 0);
-                    ts_commit(&t_free);
-                    ts_commit(&b_free[nb % kTsStages]);
-                    ++nb; ++nt;
+                    const uint32_t hi = tmem + sum * L::sum_cols + s.hid_col + 32 * e, lo = tmem + (sum ^ 1) * L::sum_cols + s.hid_col + 32 * e;
+                    const uint32_t b = smem_u32(stages + (nb % NS) * L::stage_bytes);
+                    ts_chunk(tmem + sum * L::sum_cols, hi, lo, b, b + s.cols * 128u, ts_idesc(s.cols), min(4, L::Rp / 8 - 4 * e), s.main_cols > 0 || e > 0);
+                    ts_commit(&b_free[nb % NS]);
+                    ++nb;
                 }
-                ts_commit(&d_full[nd & 1]);
-                ++nd;
+                ts_commit(&t_done);
+                ++nt;
             };
-            TsShape last{};
             for (int i = 0; ok; ++i) {
                 const int slot = i % kTsWorkRing;
                 ok = ts_wait(&work_full[slot], (i / kTsWorkRing) & 1, &failed);
                 if (!ok) break;
                 const TsWork w = work[slot];
                 mbar_arrive(&work_free[slot]);
-                TsShape s{};
-                if (w.found) s = ts_shape(pass, w);
-                if (w.found) chunk(s);
-                if (ok) rounds(last);
-                for (int j = 1; j < s.nx && ok; ++j) chunk(s);
                 if (!w.found) break;
-                last = s;
+                const TsShape s = ts_shape(pass, w);
+                for (int j = 0; j < s.nx && ok; ++j) chunk(s, j);
+                if (ok) rounds(s);
             }
         }
     } else if (warp < 8) {
-        ts_registers_more<kTsRegsRows>();
+        ts_registers_less<kTsRegsRows>();
         const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
         const int tid = threadIdx.x & 127;
-        // values every row of a degree is aligned to: 8 (32-byte loads), 4 or fewer
-        auto alignment = [&](const TsDegree& d) {
-            const unsigned long long bits = static_cast<unsigned long long>(pass.in_stride | d.in_off | d.Kd) * 4u | reinterpret_cast<uintptr_t>(pass.in);
-            return (bits & 31) == 0 ? 8 : (bits & 15) == 0 ? 4 : 1;
-        };
-        const float* row = nullptr;                  // of the tile that is being loaded
-        int tiles = 0, at = 0, chunks = 0, Kd = 0, align = 1;
-        bool more = true, ok = true;
-        // loads the next chunk of the sequence of tiles; false when there is none
-        auto load = [&](float (&v)[32]) -> bool {
-            while (at >= chunks && more) {
-                const int slot = tiles % kTsWorkRing;
-                if (!ts_wait_warp(&work_full[slot], (tiles / kTsWorkRing) & 1, &failed)) { ok = more = false; break; }
-                const TsWork w = work[slot];
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&work_free[slot]);
-                ++tiles;
-                if (!w.found) { more = false; break; }
-                const TsShape s = ts_shape(pass, w);
-                const TsDegree& d = pass.degree[w.degree];
-                at = 0; chunks = s.nx; Kd = d.Kd; align = alignment(d);
-                row = nullptr;
-                if (tid < s.rows) {
-                    const long long r = w.rows.row0 + tid, p = w.rows.first_pair + r / d.comps;
-                    const long long n = pass.sorted ? pass.order[p] / pass.slots : p;
-                    row = pass.in + n * pass.in_stride + d.in_off + (r % d.comps) * d.Kd;
-                }
-            }
-            if (at >= chunks) return false;
-            ts_load_chunk(row, at * kTsChunk, Kd, align, v);
-            ++at;
-            return true;
-        };
-        int na = 0;
-        auto store = [&](float (&v)[32]) {
-            const int slot = L::slots == 2 ? na & 1 : 0, use = L::slots == 2 ? na >> 1 : na;
-            if (use > 0 && !ts_wait_warp(&a_free[slot], (use - 1) & 1, &failed)) { ok = false; return; }
-            ts_fence_after();
-            float lo[32];
-#pragma unroll
-            for (int q = 0; q < 32; ++q) ts_split(v[q], v[q], lo[q]);
-            ts_store32(lanes + L::slot0 + 64 * slot, v);
-            ts_store32(lanes + L::slot0 + 64 * slot + 32, lo);
-            ts_wait_store();
-            ts_fence_before();
+        int nx = 0, na = 0;                          // row stages and row operands used so far
+        bool ok = true;
+        for (int i = 0; ok; ++i) {
+            const int slot = i % kTsWorkRing;
+            if (!ts_wait_warp(&work_full[slot], (i / kTsWorkRing) & 1, &failed)) break;
+            const TsWork w = work[slot];
             __syncwarp();
-            if (lane == 0) mbar_arrive(&a_full[slot]);
-            ++na;
-        };
-        float v0[32], v1[32], v2[32];
-        bool h0 = load(v0), h1 = load(v1), h2 = load(v2);
-        while (ok) {
-            if (!h0) break;
-            store(v0); if (!ok) break; h0 = load(v0);
-            if (!h1) break;
-            store(v1); if (!ok) break; h1 = load(v1);
-            if (!h2) break;
-            store(v2); if (!ok) break; h2 = load(v2);
+            if (lane == 0) mbar_arrive(&work_free[slot]);
+            if (!w.found) break;
+            const int Kd = pass.degree[w.degree].Kd;
+            const bool live = tid < w.rows.rows;
+            for (int k0 = 0; k0 < Kd && ok; k0 += kTsChunk) {
+                const int st = nx % kTsRowStages;
+                if (k0 % kTsRowValues == 0 && !ts_wait_warp(&x_full[st], (nx / kTsRowStages) & 1, &failed)) { ok = false; break; }
+                const float* from = row_stages + st * L::row_floats + tid * kTsRowPitch + k0 % kTsRowValues;
+                float v[32], lo[32];
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    const float4 f = live ? *reinterpret_cast<const float4*>(from + 4 * q) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    v[4 * q] = f.x; v[4 * q + 1] = f.y; v[4 * q + 2] = f.z; v[4 * q + 3] = f.w;
+                }
+                if (k0 + kTsChunk > Kd)              // what the stage holds behind the row's end is no value
+#pragma unroll
+                    for (int q = 0; q < 32; ++q) v[q] = k0 + q < Kd ? v[q] : 0.f;
+                if (k0 % kTsRowValues != 0 || k0 + kTsChunk >= Kd) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&x_free[st]);
+                    ++nx;
+                }
+#pragma unroll
+                for (int q = 0; q < 32; ++q) ts_split(v[q], v[q], lo[q]);
+                const int op = na % L::slots;
+                if (na >= L::slots && !ts_wait_warp(&a_free[op], (na / L::slots - 1) & 1, &failed)) { ok = false; break; }
+                ts_fence_after();
+                ts_store32(lanes + L::slot0 + 64 * op, v);
+                ts_store32(lanes + L::slot0 + 64 * op + 32, lo);
+                ts_wait_store();
+                ts_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&a_full[op]);
+                ++na;
+            }
         }
     } else {
         ts_registers_more<kTsRegsSums>();
         const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-        const int tid = threadIdx.x & 127, R = pass.rank;
-        int sum_at = 0, nt = 0, i = 0;               // uses of the partial sums before the tile, hidden operands, tiles
-        bool ok = true, last_rounds = false;
+        const int tid = threadIdx.x & 127, half = (warp - 8) >> 2, R = pass.rank;
+        constexpr int kLower = (HP + 1) / 2;         // blocks of 16 hidden columns of the lower half; the upper half has the others
+        const int hid0 = half ? kLower : 0, hid_blocks = half ? HP - kLower : kLower;
+        float* out_stage = out_stages + (warp - 8) * L::out_floats;
+        int nd = 0, nt = 0, i = 0;                   // partial sums and hidden rows used so far, tiles
+        bool ok = true;
         TsWork w{};
-        auto next_work = [&](TsWork& to) {
+        int atom = 0, place = 0, comp = 0;
+        float weight = 1.f;
+        auto next_work = [&]() {
             const int slot = i % kTsWorkRing;
             if (!ts_wait_warp(&work_full[slot], (i / kTsWorkRing) & 1, &failed)) { ok = false; return; }
-            to = work[slot];
+            w = work[slot];
+            atom = work_atom[slot][tid];
+            place = work_place[slot][tid];
+            comp = work_comp[slot][tid];
+            weight = work_weight[slot][tid];
             __syncwarp();
             if (lane == 0) mbar_arrive(&work_free[slot]);
             ++i;
         };
-        next_work(w);
+        next_work();
+        long long at_hand = blockIdx.x;              // for the tiles to give up
         while (ok && w.found) {
+            at_hand = w.index;
             const TsShape s = ts_shape(pass, w);
             const TsDegree& d = pass.degree[w.degree];
-            float* out_row = nullptr;
+            const float mix = weight;
+            const bool live = tid < s.rows;
+            long long out_at = -1;
             float* hid_row = nullptr;
-            float weight = 1.f;
-            if (tid < s.rows) {
-                const long long r = w.rows.row0 + tid, p = w.rows.first_pair + r / d.comps;
-                const int m = static_cast<int>(r % d.comps);
-                const long long pair = pass.sorted ? pass.order[p] : p, n = pass.sorted ? pair / pass.slots : p;
-                if (pass.out) out_row = pass.out + (pass.out_sorted ? p : n) * pass.out_stride + d.out_off + static_cast<long long>(m) * d.Nc + s.col0;
-                if (s.adapter && d.hidden && w.block == 0) hid_row = d.hidden + (p * d.comps + m) * R;
-                if (s.adapter && pass.weights) weight = pass.weights[pair];
-            }
-            float sum[128], hid[16 * HP];
+            if (live && pass.out) out_at = (pass.out_sorted ? place : atom) * pass.out_stride + d.out_off + static_cast<long long>(comp) * d.Nc + s.col0 + 64 * half;
+            if (live && s.adapter && d.hidden && w.block == 0) hid_row = d.hidden + (static_cast<long long>(place) * d.comps + comp) * R + 16 * hid0;
+            const int left = d.Nc - s.col0 - 64 * half;                  // columns of this half that exist
+            float sum[64], hid[16 * kLower];
 #pragma unroll
-            for (int q = 0; q < 128; ++q) sum[q] = 0.f;
+            for (int q = 0; q < 64; ++q) sum[q] = 0.f;
 #pragma unroll
-            for (int q = 0; q < 16 * HP; ++q) hid[q] = 0.f;
-            auto add_columns = [&](uint32_t from, int cols) {
+            for (int q = 0; q < 16 * kLower; ++q) hid[q] = 0.f;
+            auto add_columns = [&](uint32_t from, int cols) {            // of [0, cols) those of this half
 #pragma unroll
-                for (int cc = 0; cc < 8; ++cc)
-                    if (16 * cc < cols) {
-                        float v[16];
-                        ts_load16(from + 16 * cc, v);
+                for (int cc = 0; cc < 2; ++cc)
+                    if (64 * half + 32 * cc < cols) {                    // 16 columns of a last, odd block may be another's: never used
+                        float v[32];
+                        ts_load32(from + 64 * half + 32 * cc, v);
 #pragma unroll
-                        for (int q = 0; q < 16; ++q) sum[16 * cc + q] += v[q];
+                        for (int q = 0; q < 32; ++q) sum[32 * cc + q] += v[q];
                     }
             };
-            for (int j = 0; j < s.nx; ++j) {
-                const int use = sum_at + j + (j > 0 && last_rounds ? 1 : 0);
-                if (!ts_wait_warp(&d_full[use & 1], (use >> 1) & 1, &failed)) { ok = false; break; }
+            auto release = [&](int use) {
+                ts_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&d_free[use & 1]);
+            };
+            const int stay = s.rounds > 0 ? max(0, s.sums - 2) : s.sums;     // from this sum on the shared columns stay until the end
+            for (int j = 0; j < s.sums; ++j, ++nd) {
+                if (!ts_wait_warp(&d_full[nd & 1], (nd >> 1) & 1, &failed)) { ok = false; break; }
                 ts_fence_after();
-                const uint32_t from = lanes + (use & 1) * L::sum_cols;
-                add_columns(from, s.main_cols);
+                const uint32_t from = lanes + (nd & 1) * L::sum_cols;
                 if (s.adapter)
 #pragma unroll
-                    for (int cc = 0; cc < HP; ++cc) {
-                        float v[16];
-                        ts_load16(from + s.hid_col + 16 * cc, v);
+                    for (int cc = 0; cc < kLower; ++cc)
+                        if (cc < hid_blocks) {
+                            float v[16];
+                            ts_load16(from + s.hid_col + 16 * (hid0 + cc), v);
 #pragma unroll
-                        for (int q = 0; q < 16; ++q) hid[16 * cc + q] += v[q];
-                    }
-                ts_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&d_free[use & 1]);
-            }
-            if (!ok) break;
-            sum_at += s.nx + (last_rounds ? 1 : 0);
-            if (hid_row) {
-                if ((R & 3) == 0) {
-#pragma unroll
-                    for (int q = 0; q < 16 * HP; q += 4)
-                        if (q < R) *reinterpret_cast<float4*>(hid_row + q) = make_float4(hid[q], hid[q + 1], hid[q + 2], hid[q + 3]);
-                } else {
-#pragma unroll
-                    for (int q = 0; q < 16 * HP; ++q)
-                        if (q < R) hid_row[q] = hid[q];
+                            for (int q = 0; q < 16; ++q) hid[16 * cc + q] += v[q];
+                        }
+                if (j < stay) {
+                    add_columns(from, s.main_cols);
+                    release(nd);
                 }
             }
-            TsWork next{};
-            if (s.rounds == 0) {
-                next_work(next);
-            } else {
+            if (!ok) break;
+            if (s.rounds > 0) {
+                // the halves read and store hidden blocks of their own; where the tile has one sum, the other partial sum is the previous tile's, which
+                // the other half's warp may still be reading
+                if (s.sums == 1 && nd > 1 && !ts_wait_warp(&d_free[nd & 1], ((nd - 2) >> 1) & 1, &failed)) { ok = false; break; }
+                const uint32_t hi_at = lanes + ((nd - 1) & 1) * L::sum_cols + s.hid_col, lo_at = lanes + (nd & 1) * L::sum_cols + s.hid_col;
 #pragma unroll
-                for (int e = 0; e < (HP + 1) / 2; ++e) {
-                    if (nt > 0 && !ts_wait_warp(&t_free, (nt - 1) & 1, &failed)) { ok = false; break; }
-                    ts_fence_after();
-#pragma unroll
-                    for (int cc = 2 * e; cc < 2 * e + 2 && cc < HP; ++cc) {
+                for (int cc = 0; cc < kLower; ++cc)
+                    if (cc < hid_blocks) {
                         float hi[16], lo[16];
 #pragma unroll
-                        for (int q = 0; q < 16; ++q) ts_split(weight * hid[16 * cc + q], hi[q], lo[q]);
-                        ts_store16(lanes + L::hidden0 + 16 * (cc - 2 * e), hi);
-                        ts_store16(lanes + L::hidden0 + 32 + 16 * (cc - 2 * e), lo);
+                        for (int q = 0; q < 16; ++q) ts_split(mix * hid[16 * cc + q], hi[q], lo[q]);
+                        ts_store16(hi_at + 16 * (hid0 + cc), hi);
+                        ts_store16(lo_at + 16 * (hid0 + cc), lo);
                     }
-                    ts_wait_store();
-                    ts_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&t_full);
-                    ++nt;
-                }
-                if (!ok) break;
-                next_work(next);                     // whether its first chunk comes before the rounds
-                if (!ok) break;
-                const int use = sum_at + (next.found ? 1 : 0);
-                if (!ts_wait_warp(&d_full[use & 1], (use >> 1) & 1, &failed)) { ok = false; break; }
-                ts_fence_after();
-                add_columns(lanes + (use & 1) * L::sum_cols, s.cols);
+                ts_wait_store();
                 ts_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&d_free[use & 1]);
+                if (lane == 0) mbar_arrive(&t_full);
             }
-            if (!ok) break;
-            last_rounds = s.rounds > 0;
-            if (out_row) {
-                const int left = d.Nc - s.col0;
-                const uintptr_t bits = reinterpret_cast<uintptr_t>(out_row);
+            if (hid_row) {
+                const int n = min(16 * hid_blocks, R - 16 * hid0);
 #pragma unroll
-                for (int q = 0; q < 128; q += 8) {
-                    if (q + 8 <= left && (bits & 31) == 0) {
-                        asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out_row + q), "f"(sum[q]), "f"(sum[q + 1]), "f"(sum[q + 2]),
-                                     "f"(sum[q + 3]), "f"(sum[q + 4]), "f"(sum[q + 5]), "f"(sum[q + 6]), "f"(sum[q + 7]) : "memory");
-                    } else if (q + 8 <= left && (bits & 15) == 0) {
-                        *reinterpret_cast<float4*>(out_row + q) = make_float4(sum[q], sum[q + 1], sum[q + 2], sum[q + 3]);
-                        *reinterpret_cast<float4*>(out_row + q + 4) = make_float4(sum[q + 4], sum[q + 5], sum[q + 6], sum[q + 7]);
+                for (int q = 0; q < 16 * kLower; q += 4) {
+                    if ((R & 3) == 0) {
+                        if (q < n) *reinterpret_cast<float4*>(hid_row + q) = make_float4(hid[q], hid[q + 1], hid[q + 2], hid[q + 3]);
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            if (q + e < left) out_row[q + e] = sum[q + e];
+                        for (int e = 0; e < 4; ++e)
+                            if (q + e < n) hid_row[q + e] = hid[q + e];
                     }
                 }
             }
-            w = next;
+            if (s.rounds > 0) {
+                if (!ts_wait_warp(&t_done, nt & 1, &failed)) { ok = false; break; }
+                ++nt;
+                ts_fence_after();
+                for (int use = nd - (s.sums - stay); use < nd; ++use) {
+                    // without shared weights only the last one has such columns
+                    if (s.main_cols || use == nd - 1) add_columns(lanes + (use & 1) * L::sum_cols, s.cols);
+                    release(use);
+                }
+            }
+            next_work();
+            if (!ok) break;
+            if (pass.out) {
+                const unsigned long long bits = static_cast<unsigned long long>(pass.out_stride | d.out_off | d.Nc) * 4u | reinterpret_cast<uintptr_t>(pass.out);
+                const bool wide = (bits & 15) == 0;
+                const int c = (lane & 3) * 4;
+                long long at[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) at[r] = __shfl_sync(0xffffffffu, out_at, 8 * r + (lane >> 2));
+#pragma unroll
+                for (int c0 = 0; c0 < 64; c0 += 16) {
+                    if (c0 >= left) continue;
+                    __syncwarp();
+#pragma unroll
+                    for (int q = 0; q < 16; q += 4)
+                        *reinterpret_cast<float4*>(out_stage + lane * kTsOutPitch + q) = make_float4(sum[c0 + q], sum[c0 + q + 1], sum[c0 + q + 2], sum[c0 + q + 3]);
+                    __syncwarp();
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        if (at[r] < 0) continue;
+                        const float4 f = *reinterpret_cast<const float4*>(out_stage + (8 * r + (lane >> 2)) * kTsOutPitch + c);
+                        float* dst = pass.out + at[r] + c0 + c;
+                        if (wide && c0 + c + 4 <= left) {
+                            *reinterpret_cast<float4*>(dst) = f;
+                        } else {
+                            const float v[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (c0 + c + e < left) dst[e] = v[e];
+                        }
+                    }
+                }
+            }
         }
         if (!ok) {
             // NaN into the tile at hand and all that would have followed
             TsCursor cursor;
             TsWork lost{};
-            for (long long t = w.found ? w.index : blockIdx.x; cursor.find(pass, t, lost); t += gridDim.x) ts_fill(pass, lost, tid, 128, NAN);
+            for (long long t = at_hand; cursor.find(pass, t, lost); t += gridDim.x) ts_fill(pass, lost, tid, 128, NAN);
         }
     }
     __syncwarp();
