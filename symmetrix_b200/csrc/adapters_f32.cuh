@@ -17,11 +17,12 @@ inline int padded_rank(int rank) { return (rank + 15) & ~15; }
 inline int ts_chunks(int k) { return (k + kTsChunk - 1) / kTsChunk; }
 inline int ts_blocks(int n) { return (n + 127) / 128; }
 
-// x = hi + lo, both rounded to TF32 (half away from zero; as integers, since conversions run at a quarter of the rate). The tensor core
-// cuts its operands to their 11 leading bits, so lo need not be: half a step is added to it.
+// x = hi + lo, both rounded to TF32's 11 bits (half away from zero; as integers, since conversions run at a quarter of the rate). Bits below
+// those must be zero: left in, they cost more than the tensor core's cut of its operands explains (6.6e-7 instead of 2.5e-7 in the sums over rows).
+__device__ __forceinline__ float ts_round(float x) { return __uint_as_float((__float_as_uint(x) + 0x1000u) & kTc5HiMask); }
 __device__ __forceinline__ void ts_split(float x, float& hi, float& lo) {
-    hi = __uint_as_float((__float_as_uint(x) + 0x1000u) & kTc5HiMask);
-    lo = __uint_as_float(__float_as_uint(x - hi) + 0x1000u);
+    hi = ts_round(x);
+    lo = ts_round(x - hi);
 }
 
 __device__ __forceinline__ void ts_store32(uint32_t taddr, const float (&v)[32]) {
@@ -78,12 +79,20 @@ __device__ __forceinline__ uint32_t ts_idesc(int n) {
 }
 // The products of one chunk of `steps` x 8 inner values: row operand hi at column a_hi, lo at a_lo; weights hi at b_hi, lo at b_lo. The
 // remainders' products come first, while the sum is small: the tensor core cuts its sums, so an addition costs up to 2^-23 of the sum.
+// Descriptors of one step ahead are 32 bytes on, two units of their address field.
 __device__ __forceinline__ void ts_chunk(uint32_t d, uint32_t a_hi, uint32_t a_lo, uint32_t b_hi, uint32_t b_lo, uint32_t idesc, int steps, bool accumulate) {
-    for (int ks = 0; ks < steps; ++ks) {
-        ts_mma(d, a_lo + 8 * ks, tc5_smem_desc(b_hi + 32 * ks), idesc, accumulate || ks > 0);
-        ts_mma(d, a_hi + 8 * ks, tc5_smem_desc(b_lo + 32 * ks), idesc, true);
+    const uint64_t hi = tc5_smem_desc(b_hi), lo = tc5_smem_desc(b_lo);
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+        if (ks >= steps) break;
+        ts_mma(d, a_lo + 8 * ks, hi + 2 * ks, idesc, accumulate || ks > 0);
+        ts_mma(d, a_hi + 8 * ks, lo + 2 * ks, idesc, true);
     }
-    for (int ks = 0; ks < steps; ++ks) ts_mma(d, a_hi + 8 * ks, tc5_smem_desc(b_hi + 32 * ks), idesc, true);
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+        if (ks >= steps) break;
+        ts_mma(d, a_hi + 8 * ks, hi + 2 * ks, idesc, true);
+    }
 }
 __device__ __forceinline__ void ts_commit(unsigned long long* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -152,6 +161,9 @@ struct TsWork { long long index; int degree, block, found; TileRows rows; };
 
 // The tiles of a pass one after the other: degrees, then groups, then row tiles, then column blocks (so that a row tile's blocks run side by
 // side and its rows come from L2 after the first). A cursor remembers the 32 groups it stands at; `t` may only grow. Called by one warp.
+__device__ __forceinline__ long long ts_divide(long long a, int b) {      // mostly 32 bits, for which there is a short way
+    return (a >> 31) == 0 ? static_cast<int>(a) / b : a / b;
+}
 struct TsCursor {
     int q = 0, g0 = 0;
     long long before = 0, run = 0;               // work items before degree q, row tiles of degree q before group g0
@@ -162,7 +174,7 @@ struct TsCursor {
         while (q < p.degrees) {
             const TsDegree& d = p.degree[q];
             const int blocks = p.out ? (d.Nc + 127) / 128 : 1;
-            const long long tile = (t - before) / blocks;
+            const long long tile = ts_divide(t - before, blocks);
             const int g = g0 + lane;
             long long first = 0, rows = 0;
             if (p.sorted) {
@@ -184,7 +196,7 @@ struct TsCursor {
             const unsigned hit = __ballot_sync(0xffffffffu, tile >= begin && tile < begin + tiles);
             if (hit) {
                 const int src = __ffs(hit) - 1;
-                w.found = 1; w.degree = q; w.block = static_cast<int>((t - before) % blocks);
+                w.found = 1; w.degree = q; w.block = static_cast<int>(t - before - tile * blocks);
                 w.rows.group = p.sorted ? __shfl_sync(0xffffffffu, g, src) : p.groups;
                 w.rows.first_pair = __shfl_sync(0xffffffffu, first, src);
                 const long long b = __shfl_sync(0xffffffffu, begin, src), r = __shfl_sync(0xffffffffu, rows, src);
@@ -269,6 +281,10 @@ __device__ __forceinline__ void cp_async4(void* smem, const void* gmem) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(smem)), "l"(gmem) : "memory");
 }
 
+__device__ __forceinline__ void ts_bulk(uint32_t to, const float* from, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to), "l"(from), "r"(bytes), "r"(bar) : "memory");
+}
+
 // One persistent CTA per SM walks tiles of 128 rows x 128 columns; its warps are specialised, so that the parts of neighbouring tiles overlap:
 //   warp 0      weight images: bulk copies of a chunk's [W | first_g] tiles, or of a round's second_g tiles, into a ring of stages
 //   warp 1      the products (one thread)
@@ -277,15 +293,14 @@ __device__ __forceinline__ void cp_async4(void* smem, const void* gmem) {
 //               (loads and stores by the thread that owns a row touch 32 rows an instruction; a bulk copy of 256 bytes took 70 cycles to issue)
 //   warps 4-7   a thread splits 32 values of its row at a time and stores them to the tensor memory's row operand
 //   warps 8-15  a thread adds half of its row's partial sums of every 64 inner values in registers (the tensor core cuts its sums instead of
-//               rounding them: a single sum over 128 inner values was off five times as far as float32) and writes its half of the row, 16
-//               columns at a time through shared memory, while the products of the next tile run
+//               rounding them: a single sum over 128 inner values was off five times as far as float32) and writes its half of the row
+//               while the products of the next tile run
 // TMEM: two partial sums of 128 + Rp columns, taken in turn, and two or three row operands of 64. The shared columns of a tile's last two
 // sums stay where they are while its hidden row is weighted, split and stored into their hidden columns (head in the last one's, remainder in
 // the other's); the products with second_g go on top of the last sum, and both are read then.
 // Every wait is bounded; if one runs out, the CTA gives up and fills its remaining tiles with NaN.
 constexpr int kTsPassThreads = 512, kTsWorkRing = 4, kTsRowStages = 2;
 constexpr int kTsRowValues = 64, kTsRowPitch = kTsRowValues + 4;              // floats: threads that read their rows 16 bytes at a time hit all banks
-constexpr int kTsOutPitch = 20;
 constexpr int kTsRegsControl = 72, kTsRegsRows = 120, kTsRegsSums = 160, kTsRegsLaunch = 128;
 static_assert(kTsRegsControl + kTsRegsRows + 2 * kTsRegsSums <= 4 * kTsRegsLaunch, "the registers of the launch are shared out");
 template <int HP>                                    // hidden columns / 16
@@ -293,8 +308,8 @@ struct TsPassLayout {
     static constexpr int Rp = 16 * HP, sum_cols = 128 + Rp, slots = HP > 2 ? 2 : 3, stages = HP > 2 ? 2 : 3;
     static constexpr int slot0 = 2 * sum_cols;
     static constexpr uint32_t stage_bytes = sum_cols * 256u;
-    static constexpr int row_floats = kTsRows * kTsRowPitch, out_floats = 32 * kTsOutPitch;
-    static constexpr int smem = stages * static_cast<int>(stage_bytes) + (kTsRowStages * row_floats + 8 * out_floats) * 4 + 1024;
+    static constexpr int row_floats = kTsRows * kTsRowPitch;
+    static constexpr int smem = stages * static_cast<int>(stage_bytes) + kTsRowStages * row_floats * 4 + 1024;
     static_assert(slot0 + 64 * slots <= 512, "tensor memory has 512 columns");
     static_assert(smem + 9 * 1024 <= 227 * 1024, "shared memory of one CTA per SM");
 };
@@ -315,7 +330,6 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     unsigned char* stages = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(ts_smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     float* row_stages = reinterpret_cast<float*>(stages + NS * L::stage_bytes);
-    float* out_stages = row_stages + kTsRowStages * L::row_floats;
     if (threadIdx.x == 0) {
         failed = 0;
         for (int q = 0; q < kTsWorkRing; ++q) { mbar_init(&work_full[q], 1); mbar_init(&work_free[q], 15); }
@@ -351,8 +365,8 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
                 }
                 if (w.found) {
                     const int comps = pass.degree[w.degree].comps;
-                    const long long p0 = w.rows.first_pair + w.rows.row0 / comps;
-                    const int m0 = static_cast<int>(w.rows.row0 % comps);
+                    const long long q0 = ts_divide(w.rows.row0, comps), p0 = w.rows.first_pair + q0;
+                    const int m0 = static_cast<int>(w.rows.row0 - q0 * comps);
                     const bool weighted = w.rows.group < pass.groups && pass.weights;
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
@@ -432,41 +446,25 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
             }
             asm volatile("cp.async.wait_all;" ::: "memory");             // none may be in flight when the CTA ends
         } else if (warp == 0 && lane == 0) {
-            int n = 0;                                                   // chunks copied so far
+            int n = 0, st = 0;                                           // chunks copied so far, stage of the next one
+            unsigned round = 1;                                          // parity of the stage's last use but one
             bool ok = true;
-            auto stage_free = [&]() { return ok = ok && (n < NS || ts_wait(&b_free[n % NS], (n / NS - 1) & 1, &failed)); };
-            auto chunk = [&](const TsWork& w, const TsShape& s, int j) {
-                if (!stage_free()) return;
-                const TsDegree& d = pass.degree[w.degree];
-                unsigned char* to = stages + (n % NS) * L::stage_bytes;
-                unsigned long long* bar = &b_full[n % NS];
-                const uint32_t half = (s.main_cols + (s.adapter ? L::Rp : 0)) * 128u;
-                mbar_expect_tx(bar, 2 * half);
-                if (s.main_cols) {
-                    const float* m = d.W + (static_cast<long long>(w.block) * s.nx + j) * (2 * kTsTileBytes / 4);
-                    bulk_copy_g2s(to, m, s.main_cols * 128u, bar);
-                    bulk_copy_g2s(to + half, m + kTsTileBytes / 4, s.main_cols * 128u, bar);
+            const uint32_t base = smem_u32(stages);
+            // one chunk: `rows_a` rows of tile a and then `rows_b` of tile b, heads and remainders; tiles hold `half_a` / `half_b` floats of each
+            auto copy = [&](const float* a, int half_a, uint32_t rows_a, const float* b, int half_b, uint32_t rows_b) {
+                if (n >= NS && !ts_wait(&b_free[st], round, &failed)) { ok = false; return; }
+                const uint32_t bar = smem_u32(&b_full[st]), to = base + st * L::stage_bytes, half = (rows_a + rows_b) * 128u;
+                asm volatile("{\n\t.reg .b64 t;\n\tmbarrier.arrive.expect_tx.shared::cta.b64 t, [%0], %1;\n\t}" ::"r"(bar), "r"(2 * half) : "memory");
+                if (rows_a) {
+                    ts_bulk(to, a, rows_a * 128u, bar);
+                    ts_bulk(to + half, a + half_a, rows_a * 128u, bar);
                 }
-                if (s.adapter) {
-                    const float* m = d.first + s.group * d.first_group + static_cast<long long>(j) * 2 * L::Rp * kTsChunk;
-                    bulk_copy_g2s(to + s.main_cols * 128u, m, L::Rp * 128u, bar);
-                    bulk_copy_g2s(to + half + s.main_cols * 128u, m + L::Rp * kTsChunk, L::Rp * 128u, bar);
+                if (rows_b) {
+                    ts_bulk(to + rows_a * 128u, b, rows_b * 128u, bar);
+                    ts_bulk(to + half + rows_a * 128u, b + half_b, rows_b * 128u, bar);
                 }
                 ++n;
-            };
-            auto rounds = [&](const TsWork& w, const TsShape& s) {
-                const TsDegree& d = pass.degree[w.degree];
-                for (int e = 0; e < s.rounds; ++e) {
-                    if (!stage_free()) return;
-                    unsigned char* to = stages + (n % NS) * L::stage_bytes;
-                    unsigned long long* bar = &b_full[n % NS];
-                    const uint32_t half = s.cols * 128u;
-                    mbar_expect_tx(bar, 2 * half);
-                    const float* m = d.second + s.group * d.second_group + (static_cast<long long>(w.block) * s.rounds + e) * (2 * kTsTileBytes / 4);
-                    bulk_copy_g2s(to, m, half, bar);
-                    bulk_copy_g2s(to + half, m + kTsTileBytes / 4, half, bar);
-                    ++n;
-                }
+                if (++st == NS) { st = 0; round ^= 1u; }
             };
             for (int i = 0; ok; ++i) {
                 const int slot = i % kTsWorkRing;
@@ -476,46 +474,28 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
                 mbar_arrive(&work_free[slot]);
                 if (!w.found) break;
                 const TsShape s = ts_shape(pass, w);
-                for (int j = 0; j < s.nx; ++j) chunk(w, s, j);
-                rounds(w, s);
+                const TsDegree& d = pass.degree[w.degree];
+                const float* shared = d.W + static_cast<long long>(w.block) * s.nx * (2 * kTsTileBytes / 4);
+                const float* first = d.first + s.group * d.first_group;
+                const float* second = d.second + s.group * d.second_group + static_cast<long long>(w.block) * s.rounds * (2 * kTsTileBytes / 4);
+                for (int j = 0; j < s.nx && ok; ++j) {
+                    copy(shared, kTsTileBytes / 4, s.main_cols, first, L::Rp * kTsChunk, s.adapter ? L::Rp : 0);
+                    shared += 2 * kTsTileBytes / 4;
+                    first += 2 * L::Rp * kTsChunk;
+                }
+                for (int e = 0; e < s.rounds && ok; ++e) {
+                    copy(second, kTsTileBytes / 4, s.cols, nullptr, 0, 0);
+                    second += 2 * kTsTileBytes / 4;
+                }
             }
-            if (!ok)
+            if (!ok)                                                     // copies in flight write into this CTA's memory: wait for them (bounded)
                 for (int q = max(0, n - NS); q < n; ++q) mbar_wait(&b_full[q % NS], (q / NS) & 1);
         } else if (warp == 1 && lane == 0) {
-            int nb = 0, na = 0, nt = 0, nd = 0;                          // stages, row operands, hidden rows and partial sums used so far
+            // stages, row operands and partial sums in turn, each with the parity of its next use; hidden rows
+            int st = 0, op = 0, sum = 0, nd = 0;
+            unsigned st_par = 0, op_par = 0, sum_par = 1, hid_par = 0;
             bool ok = true;
-            auto chunk = [&](const TsShape& s, int j) {
-                const int slot = na % L::slots;
-                if ((j & 1) == 0 && nd >= 2) ok = ts_wait(&d_free[nd & 1], ((nd >> 1) - 1) & 1, &failed);
-                ok = ok && ts_wait(&a_full[slot], (na / L::slots) & 1, &failed) && ts_wait(&b_full[nb % NS], (nb / NS) & 1, &failed);
-                if (!ok) return;
-                ts_fence_after();
-                const int cols = s.main_cols + (s.adapter ? L::Rp : 0);
-                const uint32_t d = tmem + (nd & 1) * L::sum_cols + (s.main_cols ? 0 : 128), a = tmem + L::slot0 + 64 * slot;
-                const uint32_t b = smem_u32(stages + (nb % NS) * L::stage_bytes);
-                ts_chunk(d, a, a + 32, b, b + cols * 128u, ts_idesc(cols), 4, (j & 1) != 0);
-                ts_commit(&a_free[slot]);
-                ts_commit(&b_free[nb % NS]);
-                ++nb; ++na;
-                if ((j & 1) != 0 || j + 1 == s.nx) { ts_commit(&d_full[nd & 1]); ++nd; }
-            };
-            auto rounds = [&](const TsShape& s) {
-                if (s.rounds == 0) return;
-                const int sum = (nd - 1) & 1;        // the last one's
-                ok = ts_wait(&t_full, nt & 1, &failed);
-                for (int e = 0; e < s.rounds && ok; ++e) {
-                    ok = ts_wait(&b_full[nb % NS], (nb / NS) & 1, &failed);
-                    if (!ok) return;
-                    ts_fence_after();
-                    const uint32_t hi = tmem + sum * L::sum_cols + s.hid_col + 32 * e, lo = tmem + (sum ^ 1) * L::sum_cols + s.hid_col + 32 * e;
-                    const uint32_t b = smem_u32(stages + (nb % NS) * L::stage_bytes);
-                    ts_chunk(tmem + sum * L::sum_cols, hi, lo, b, b + s.cols * 128u, ts_idesc(s.cols), min(4, L::Rp / 8 - 4 * e), s.main_cols > 0 || e > 0);
-                    ts_commit(&b_free[nb % NS]);
-                    ++nb;
-                }
-                ts_commit(&t_done);
-                ++nt;
-            };
+            const uint32_t base = smem_u32(stages);
             for (int i = 0; ok; ++i) {
                 const int slot = i % kTsWorkRing;
                 ok = ts_wait(&work_full[slot], (i / kTsWorkRing) & 1, &failed);
@@ -524,8 +504,41 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
                 mbar_arrive(&work_free[slot]);
                 if (!w.found) break;
                 const TsShape s = ts_shape(pass, w);
-                for (int j = 0; j < s.nx && ok; ++j) chunk(s, j);
-                if (ok) rounds(s);
+                const int cols = s.main_cols + (s.adapter ? L::Rp : 0);
+                const uint32_t idesc = ts_idesc(cols), d0 = tmem + (s.main_cols ? 0 : 128);
+                for (int j = 0; j < s.nx; ++j) {
+                    if ((j & 1) == 0 && nd >= 2) ok = ts_wait(&d_free[sum], sum_par, &failed);
+                    ok = ok && ts_wait(&a_full[op], op_par, &failed) && ts_wait(&b_full[st], st_par, &failed);
+                    if (!ok) break;
+                    ts_fence_after();
+                    const uint32_t a = tmem + L::slot0 + 64 * op, b = base + st * L::stage_bytes;
+                    ts_chunk(d0 + sum * L::sum_cols, a, a + 32, b, b + cols * 128u, idesc, 4, (j & 1) != 0);
+                    ts_commit(&a_free[op]);
+                    ts_commit(&b_free[st]);
+                    if (++op == L::slots) { op = 0; op_par ^= 1u; }
+                    if (++st == NS) { st = 0; st_par ^= 1u; }
+                    if ((j & 1) != 0 || j + 1 == s.nx) {
+                        ts_commit(&d_full[sum]);
+                        ++nd;
+                        sum ^= 1;
+                        if (sum == 0) sum_par ^= 1u;
+                    }
+                }
+                if (!ok || s.rounds == 0) continue;
+                const uint32_t last = tmem + (sum ^ 1) * L::sum_cols, other = tmem + sum * L::sum_cols;
+                ok = ts_wait(&t_full, hid_par, &failed);
+                for (int e = 0; e < s.rounds && ok; ++e) {
+                    ok = ts_wait(&b_full[st], st_par, &failed);
+                    if (!ok) break;
+                    ts_fence_after();
+                    const uint32_t b = base + st * L::stage_bytes;
+                    ts_chunk(last, last + s.hid_col + 32 * e, other + s.hid_col + 32 * e, b, b + s.cols * 128u, ts_idesc(s.cols), min(4, L::Rp / 8 - 4 * e),
+                             s.main_cols > 0 || e > 0);
+                    ts_commit(&b_free[st]);
+                    if (++st == NS) { st = 0; st_par ^= 1u; }
+                }
+                ts_commit(&t_done);
+                hid_par ^= 1u;
             }
         }
     } else if (warp < 8) {
@@ -543,31 +556,37 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
             if (!w.found) break;
             const int Kd = pass.degree[w.degree].Kd;
             const bool live = tid < w.rows.rows;
-            for (int k0 = 0; k0 < Kd && ok; k0 += kTsChunk) {
+            // the next 32 values are read while the current ones are split and stored
+            float next[32];
+            auto read = [&](int k0) {
                 const int st = nx % kTsRowStages;
-                if (k0 % kTsRowValues == 0 && !ts_wait_warp(&x_full[st], (nx / kTsRowStages) & 1, &failed)) { ok = false; break; }
+                if (k0 % kTsRowValues == 0 && !ts_wait_warp(&x_full[st], (nx / kTsRowStages) & 1, &failed)) { ok = false; return; }
                 const float* from = row_stages + st * L::row_floats + tid * kTsRowPitch + k0 % kTsRowValues;
-                float v[32], lo[32];
 #pragma unroll
                 for (int q = 0; q < 8; ++q) {
-                    const float4 f = live ? *reinterpret_cast<const float4*>(from + 4 * q) : make_float4(0.f, 0.f, 0.f, 0.f);
-                    v[4 * q] = f.x; v[4 * q + 1] = f.y; v[4 * q + 2] = f.z; v[4 * q + 3] = f.w;
+                    const float4 f = *reinterpret_cast<const float4*>(from + 4 * q);
+                    next[4 * q] = f.x; next[4 * q + 1] = f.y; next[4 * q + 2] = f.z; next[4 * q + 3] = f.w;
                 }
-                if (k0 + kTsChunk > Kd)              // what the stage holds behind the row's end is no value
+                if (k0 % kTsRowValues != 0 || k0 + kTsChunk >= Kd) ++nx;
+            };
+            read(0);
+            for (int k0 = 0; k0 < Kd && ok; k0 += kTsChunk) {
+                float v[32], lo[32];
+                if (!live || k0 + kTsChunk > Kd)     // what the stage holds behind the tile's or the row's end is no value
 #pragma unroll
-                    for (int q = 0; q < 32; ++q) v[q] = k0 + q < Kd ? v[q] : 0.f;
-                if (k0 % kTsRowValues != 0 || k0 + kTsChunk >= Kd) {
+                    for (int q = 0; q < 32; ++q) next[q] = live && k0 + q < Kd ? next[q] : 0.f;
+#pragma unroll
+                for (int q = 0; q < 32; ++q) ts_split(next[q], v[q], lo[q]);
+                if (k0 % kTsRowValues != 0 || k0 + kTsChunk >= Kd) {     // the stage has been read (its values are in registers)
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&x_free[st]);
-                    ++nx;
+                    if (lane == 0) mbar_arrive(&x_free[(nx - 1) % kTsRowStages]);
                 }
-#pragma unroll
-                for (int q = 0; q < 32; ++q) ts_split(v[q], v[q], lo[q]);
                 const int op = na % L::slots;
                 if (na >= L::slots && !ts_wait_warp(&a_free[op], (na / L::slots - 1) & 1, &failed)) { ok = false; break; }
                 ts_fence_after();
                 ts_store32(lanes + L::slot0 + 64 * op, v);
                 ts_store32(lanes + L::slot0 + 64 * op + 32, lo);
+                if (k0 + kTsChunk < Kd) read(k0 + kTsChunk);
                 ts_wait_store();
                 ts_fence_before();
                 __syncwarp();
@@ -581,7 +600,6 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
         const int tid = threadIdx.x & 127, half = (warp - 8) >> 2, R = pass.rank;
         constexpr int kLower = (HP + 1) / 2;         // blocks of 16 hidden columns of the lower half; the upper half has the others
         const int hid0 = half ? kLower : 0, hid_blocks = half ? HP - kLower : kLower;
-        float* out_stage = out_stages + (warp - 8) * L::out_floats;
         int nd = 0, nt = 0, i = 0;                   // partial sums and hidden rows used so far, tiles
         bool ok = true;
         TsWork w{};
@@ -607,9 +625,9 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
             const TsDegree& d = pass.degree[w.degree];
             const float mix = weight;
             const bool live = tid < s.rows;
-            long long out_at = -1;
+            float* out_row = nullptr;
             float* hid_row = nullptr;
-            if (live && pass.out) out_at = (pass.out_sorted ? place : atom) * pass.out_stride + d.out_off + static_cast<long long>(comp) * d.Nc + s.col0 + 64 * half;
+            if (live && pass.out) out_row = pass.out + (pass.out_sorted ? place : atom) * pass.out_stride + d.out_off + static_cast<long long>(comp) * d.Nc + s.col0 + 64 * half;
             if (live && s.adapter && d.hidden && w.block == 0) hid_row = d.hidden + (static_cast<long long>(place) * d.comps + comp) * R + 16 * hid0;
             const int left = d.Nc - s.col0 - 64 * half;                  // columns of this half that exist
             float sum[64], hid[16 * kLower];
@@ -696,35 +714,21 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
             }
             next_work();
             if (!ok) break;
-            if (pass.out) {
-                const unsigned long long bits = static_cast<unsigned long long>(pass.out_stride | d.out_off | d.Nc) * 4u | reinterpret_cast<uintptr_t>(pass.out);
-                const bool wide = (bits & 15) == 0;
-                const int c = (lane & 3) * 4;
-                long long at[4];
+            if (out_row) {
+                const uintptr_t bits = reinterpret_cast<uintptr_t>(out_row);
+                if (left >= 64 && (bits & 31) == 0) {
 #pragma unroll
-                for (int r = 0; r < 4; ++r) at[r] = __shfl_sync(0xffffffffu, out_at, 8 * r + (lane >> 2));
+                    for (int q = 0; q < 64; q += 8)
+                        asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out_row + q), "f"(sum[q]), "f"(sum[q + 1]), "f"(sum[q + 2]),
+                                     "f"(sum[q + 3]), "f"(sum[q + 4]), "f"(sum[q + 5]), "f"(sum[q + 6]), "f"(sum[q + 7]) : "memory");
+                } else if ((left & 3) == 0 && (bits & 15) == 0) {
 #pragma unroll
-                for (int c0 = 0; c0 < 64; c0 += 16) {
-                    if (c0 >= left) continue;
-                    __syncwarp();
+                    for (int q = 0; q < 64; q += 4)
+                        if (q < left) *reinterpret_cast<float4*>(out_row + q) = make_float4(sum[q], sum[q + 1], sum[q + 2], sum[q + 3]);
+                } else {
 #pragma unroll
-                    for (int q = 0; q < 16; q += 4)
-                        *reinterpret_cast<float4*>(out_stage + lane * kTsOutPitch + q) = make_float4(sum[c0 + q], sum[c0 + q + 1], sum[c0 + q + 2], sum[c0 + q + 3]);
-                    __syncwarp();
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        if (at[r] < 0) continue;
-                        const float4 f = *reinterpret_cast<const float4*>(out_stage + (8 * r + (lane >> 2)) * kTsOutPitch + c);
-                        float* dst = pass.out + at[r] + c0 + c;
-                        if (wide && c0 + c + 4 <= left) {
-                            *reinterpret_cast<float4*>(dst) = f;
-                        } else {
-                            const float v[4] = {f.x, f.y, f.z, f.w};
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                if (c0 + c + e < left) dst[e] = v[e];
-                        }
-                    }
+                    for (int q = 0; q < 64; ++q)
+                        if (q < left) out_row[q] = sum[q];
                 }
             }
         }
