@@ -625,7 +625,7 @@ void launch_pass(const smx_adapter_linear& c, bool transposed, const Pass<float>
     t.degrees = degrees; t.rank = p.rank; t.groups = p.groups; t.slots = p.slots; t.num_rows = p.num_rows; t.pairs = p.pairs;
     t.order = p.order; t.offsets = p.offsets; t.weights = p.weights; t.in = p.in; t.in_stride = p.in_stride; t.out = p.out; t.out_stride = p.out_stride;
     t.sorted = p.sorted; t.out_sorted = p.out_sorted; t.tail = p.tail;
-    if (tiles > INT_MAX) throw ArgError("smx_adapter: too many rows");
+    if (tiles > INT_MAX - 4096) throw ArgError("smx_adapter: too many rows");
     bool bare = false;
     for (int q = 0; q < degrees; ++q) bare = bare || !p.degree[q].W;
     if (bare && p.out && (p.tail || !p.sorted)) {        // with one slot a pair is an atom

@@ -82,17 +82,13 @@ __device__ __forceinline__ uint32_t ts_idesc(int n) {
 // Descriptors of one step ahead are 32 bytes on, two units of their address field.
 __device__ __forceinline__ void ts_chunk(uint32_t d, uint32_t a_hi, uint32_t a_lo, uint32_t b_hi, uint32_t b_lo, uint32_t idesc, int steps, bool accumulate) {
     const uint64_t hi = tc5_smem_desc(b_hi), lo = tc5_smem_desc(b_lo);
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-        if (ks >= steps) break;
+#pragma unroll 1
+    for (int ks = 0; ks < steps; ++ks) {
         ts_mma(d, a_lo + 8 * ks, hi + 2 * ks, idesc, accumulate || ks > 0);
         ts_mma(d, a_hi + 8 * ks, lo + 2 * ks, idesc, true);
     }
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-        if (ks >= steps) break;
-        ts_mma(d, a_hi + 8 * ks, hi + 2 * ks, idesc, true);
-    }
+#pragma unroll 1
+    for (int ks = 0; ks < steps; ++ks) ts_mma(d, a_hi + 8 * ks, hi + 2 * ks, idesc, true);
 }
 __device__ __forceinline__ void ts_commit(unsigned long long* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -157,51 +153,44 @@ struct TsPass {
     float* out; long long out_stride;
     int sorted, out_sorted, tail;                // as in Pass
 };
-struct TsWork { long long index; int degree, block, found; TileRows rows; };
+struct TsWork { int index, degree, block, found; TileRows rows; };
 
 // The tiles of a pass one after the other: degrees, then groups, then row tiles, then column blocks (so that a row tile's blocks run side by
 // side and its rows come from L2 after the first). A cursor remembers the 32 groups it stands at; `t` may only grow. Called by one warp.
-__device__ __forceinline__ long long ts_divide(long long a, int b) {      // mostly 32 bits, for which there is a short way
-    return (a >> 31) == 0 ? static_cast<int>(a) / b : a / b;
-}
 struct TsCursor {
     int q = 0, g0 = 0;
-    long long before = 0, run = 0;               // work items before degree q, row tiles of degree q before group g0
-    __device__ __forceinline__ bool find(const TsPass& p, long long t, TsWork& w) {
+    int before = 0, run = 0;                     // work items before degree q, row tiles of degree q before group g0 (the host keeps them below 2^31)
+    __device__ __forceinline__ bool find(const TsPass& p, int t, TsWork& w) {
         const int lane = threadIdx.x & 31;
         w.found = 0;
         w.index = t;
         while (q < p.degrees) {
             const TsDegree& d = p.degree[q];
             const int blocks = p.out ? (d.Nc + 127) / 128 : 1;
-            const long long tile = ts_divide(t - before, blocks);
-            const int g = g0 + lane;
-            long long first = 0, rows = 0;
-            if (p.sorted) {
-                if (g < p.groups || (g == p.groups && p.tail)) {
-                    first = p.offsets[g];
-                    rows = ((g < p.groups ? p.offsets[g + 1] : p.pairs) - first) * d.comps;
-                }
-            } else if (g == 0) {
-                rows = p.num_rows * d.comps;
+            const int tile = (t - before) / blocks, g = g0 + lane;
+            int first = 0, count = 0;            // pairs of the group (rows of the array where there is no plan)
+            if (!p.sorted) {
+                if (g == 0) count = static_cast<int>(p.num_rows);
+            } else if (g < p.groups || (g == p.groups && p.tail)) {
+                first = p.offsets[g];
+                count = (g < p.groups ? p.offsets[g + 1] : static_cast<int>(p.pairs)) - first;
             }
-            const long long tiles = (rows + kTsRows - 1) / kTsRows;
-            long long incl = tiles;
+            const int tiles = static_cast<int>((static_cast<long long>(count) * d.comps + kTsRows - 1) / kTsRows);
+            int incl = tiles;
 #pragma unroll
             for (int s = 1; s < 32; s <<= 1) {
-                const long long up = __shfl_up_sync(0xffffffffu, incl, s);
+                const int up = __shfl_up_sync(0xffffffffu, incl, s);
                 if (lane >= s) incl += up;
             }
-            const long long begin = run + incl - tiles;
+            const int begin = run + incl - tiles;
             const unsigned hit = __ballot_sync(0xffffffffu, tile >= begin && tile < begin + tiles);
             if (hit) {
                 const int src = __ffs(hit) - 1;
-                w.found = 1; w.degree = q; w.block = static_cast<int>(t - before - tile * blocks);
-                w.rows.group = p.sorted ? __shfl_sync(0xffffffffu, g, src) : p.groups;
+                w.found = 1; w.degree = q; w.block = t - before - tile * blocks;
+                w.rows.group = p.sorted ? g0 + src : p.groups;
                 w.rows.first_pair = __shfl_sync(0xffffffffu, first, src);
-                const long long b = __shfl_sync(0xffffffffu, begin, src), r = __shfl_sync(0xffffffffu, rows, src);
-                w.rows.row0 = (tile - b) * kTsRows;
-                w.rows.rows = min(static_cast<long long>(kTsRows), r - w.rows.row0);
+                w.rows.row0 = static_cast<long long>(tile - __shfl_sync(0xffffffffu, begin, src)) * kTsRows;
+                w.rows.rows = min(static_cast<long long>(kTsRows), static_cast<long long>(__shfl_sync(0xffffffffu, count, src)) * d.comps - w.rows.row0);
                 return true;
             }
             run += __shfl_sync(0xffffffffu, incl, 31);
@@ -249,20 +238,24 @@ __device__ __forceinline__ void ts_fill(const TsPass& p, const TsWork& w, int th
 }
 
 // Waits of the pass kernel: bounded, and given up at once when another one ran out.
+__device__ __forceinline__ bool ts_try(uint32_t addr, unsigned parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done) : "r"(addr), "r"(parity) : "memory");
+    return done != 0;
+}
 __device__ __forceinline__ bool ts_wait(unsigned long long* bar, unsigned parity, int* failed) {
     const uint32_t addr = smem_u32(bar);
-    for (unsigned spin = 0; spin < kMbarSpinLimit; ++spin) {
-        uint32_t done;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(done) : "r"(addr), "r"(parity) : "memory");
-        if (done) return true;
-        if ((spin & 63u) == 63u && *reinterpret_cast<volatile int*>(failed)) return false;
+#pragma unroll 1
+    for (unsigned spin = 0; !ts_try(addr, parity); ++spin) {
+        if ((spin & 63u) != 63u) continue;
+        if (*reinterpret_cast<volatile int*>(failed)) return false;
+        if (spin >= kMbarSpinLimit) { atomicExch(failed, 1); return false; }
     }
-    atomicExch(failed, 1);
-    return false;
+    return true;
 }
 __device__ __forceinline__ bool ts_wait_warp(unsigned long long* bar, unsigned parity, int* failed) {
     return __all_sync(0xffffffffu, ts_wait(bar, parity, failed));
@@ -311,7 +304,7 @@ struct TsPassLayout {
     static constexpr int row_floats = kTsRows * kTsRowPitch;
     static constexpr int smem = stages * static_cast<int>(stage_bytes) + kTsRowStages * row_floats * 4 + 1024;
     static_assert(slot0 + 64 * slots <= 512, "tensor memory has 512 columns");
-    static_assert(smem + 9 * 1024 <= 227 * 1024, "shared memory of one CTA per SM");
+    static_assert(smem + 15 * 1024 <= 227 * 1024, "shared memory of one CTA per SM");
 };
 
 template <int HP>
@@ -322,7 +315,8 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
     __shared__ __align__(8) unsigned long long work_full[kTsWorkRing], work_free[kTsWorkRing], b_full[NS], b_free[NS], x_full[kTsRowStages],
         x_free[kTsRowStages], a_full[3], a_free[3], d_full[2], d_free[2], t_full, t_done;
     __shared__ TsWork work[kTsWorkRing];
-    __shared__ int work_atom[kTsWorkRing][kTsRows], work_place[kTsWorkRing][kTsRows];      // row of `in`, sorted position
+    __shared__ long long work_in[kTsWorkRing][kTsRows], work_out[kTsWorkRing][kTsRows];    // where its rows start, in `in`, in `out` without the tile's
+    __shared__ int work_place[kTsWorkRing][kTsRows];                                       // first column; sorted position and component
     __shared__ short work_comp[kTsWorkRing][kTsRows];
     __shared__ float work_weight[kTsWorkRing][kTsRows];
     __shared__ uint32_t tmem_slot;
@@ -354,7 +348,7 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
         ts_registers_less<kTsRegsControl>();
         if (warp == 2) {
             TsCursor cursor;
-            long long t = blockIdx.x;
+            int t = blockIdx.x;
             for (int i = 0;; ++i) {
                 const int slot = i % kTsWorkRing;
                 if (i >= kTsWorkRing && !ts_wait_warp(&work_free[slot], (i / kTsWorkRing - 1) & 1, &failed)) break;
@@ -364,27 +358,21 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
                     if (ts_shape(pass, w).nx > 0) break;                 // no shared weights and no adapter: adapter_zero_rows_kernel's
                 }
                 if (w.found) {
-                    const int comps = pass.degree[w.degree].comps;
-                    const long long q0 = ts_divide(w.rows.row0, comps), p0 = w.rows.first_pair + q0;
-                    const int m0 = static_cast<int>(w.rows.row0 - q0 * comps);
+                    const TsDegree& d = pass.degree[w.degree];
+                    const int comps = d.comps;
+                    const long long q0 = w.rows.row0 < (1LL << 31) ? static_cast<int>(w.rows.row0) / comps : w.rows.row0 / comps;
+                    const int p0 = static_cast<int>(w.rows.first_pair + q0), m0 = static_cast<int>(w.rows.row0 - q0 * comps);
                     const bool weighted = w.rows.group < pass.groups && pass.weights;
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const int at = lane + 32 * q;
-                        int atom = 0, place = 0, comp = 0;
-                        float weight = 1.f;
-                        if (at < w.rows.rows) {
-                            const int ahead = (m0 + at) / comps;
-                            place = static_cast<int>(p0) + ahead;
-                            comp = m0 + at - ahead * comps;
-                            const int pair = pass.sorted ? pass.order[place] : place;
-                            atom = pass.sorted ? pair / pass.slots : pair;
-                            if (weighted) weight = pass.weights[pair];
-                        }
-                        work_atom[slot][at] = atom;
+#pragma unroll 2
+                    for (int at = lane; at < kTsRows; at += 32) {
+                        const bool live = at < w.rows.rows;
+                        const int ahead = (m0 + at) / comps, place = live ? p0 + ahead : p0, comp = live ? m0 + at - ahead * comps : 0;
+                        const int pair = pass.sorted ? pass.order[place] : place, atom = pass.sorted && pass.slots > 1 ? pair / pass.slots : pair;
+                        work_in[slot][at] = atom * pass.in_stride + d.in_off + comp * d.Kd;
+                        work_out[slot][at] = (pass.out_sorted ? place : atom) * pass.out_stride + d.out_off + static_cast<long long>(comp) * d.Nc;
                         work_place[slot][at] = place;
                         work_comp[slot][at] = static_cast<short>(comp);
-                        work_weight[slot][at] = weight;
+                        work_weight[slot][at] = weighted ? pass.weights[pair] : 1.f;
                     }
                 }
                 if (lane == 0) work[slot] = w;
@@ -393,7 +381,8 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
                 if (!w.found) break;
             }
         } else if (warp == 3) {
-            int n = 0;                                                   // stages filled so far
+            int n = 0, st = 0;                                           // stages filled so far, the next one
+            unsigned round = 1;                                          // parity of its last use but one
             bool ok = true;
             for (int i = 0; ok; ++i) {
                 const int slot = i % kTsWorkRing;
@@ -408,41 +397,28 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
                 const int rows = static_cast<int>(w.rows.rows);
                 const unsigned long long bits = static_cast<unsigned long long>(pass.in_stride | d.in_off | d.Kd) * 4u | reinterpret_cast<uintptr_t>(pass.in);
                 const bool wide = (bits & 15) == 0;
-                const float* from[4];
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int at = lane + 32 * q;
-                    from[q] = pass.in + work_atom[slot][at] * pass.in_stride + d.in_off + work_comp[slot][at] * d.Kd;
+                for (int k0 = 0; k0 < d.Kd; k0 += kTsRowValues) {
+                    const int left = min(kTsRowValues, d.Kd - k0);
+                    if (n >= kTsRowStages && !ts_wait_warp(&x_free[st], round, &failed)) { ok = false; break; }
+                    float* to = row_stages + st * L::row_floats;
+                    const float* from = pass.in + k0;
+                    if (wide) {                      // two rows an instruction, 16 bytes a lane
+                        const int c = (lane & 15) * 4;
+                        if (c < left)
+#pragma unroll 4
+                            for (int r = lane >> 4; r < rows; r += 2) cp_async16(to + r * kTsRowPitch + c, from + work_in[slot][r] + c, 16);
+                    } else {
+#pragma unroll 1
+                        for (int r = 0; r < rows; ++r)
+                            for (int c = lane; c < left; c += 32) cp_async4(to + r * kTsRowPitch + c, from + work_in[slot][r] + c);
+                    }
+                    __syncwarp();
+                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&x_full[st])) : "memory");
+                    ++n;
+                    if (++st == kTsRowStages) { st = 0; round ^= 1u; }
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&work_free[slot]);
-                for (int k0 = 0; k0 < d.Kd && ok; k0 += kTsRowValues) {
-                    const int st = n % kTsRowStages, left = min(kTsRowValues, d.Kd - k0);
-                    if (n >= kTsRowStages && !ts_wait_warp(&x_free[st], (n / kTsRowStages - 1) & 1, &failed)) { ok = false; break; }
-                    float* to = row_stages + st * L::row_floats;
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const unsigned long long mine = reinterpret_cast<unsigned long long>(from[q] + k0);
-                        if (wide) {                  // two rows an instruction, 16 bytes a lane
-                            const int c = (lane & 15) * 4;
-#pragma unroll 4
-                            for (int r = 0; r < 32; r += 2) {
-                                const int row = r + (lane >> 4);
-                                const float* src = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, mine, row)) + c;
-                                if (32 * q + row < rows && c < left) cp_async16(to + (32 * q + row) * kTsRowPitch + c, src, 16);
-                            }
-                        } else {
-#pragma unroll 4
-                            for (int row = 0; row < 32; ++row) {
-                                const float* src = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, mine, row));
-                                if (32 * q + row < rows)
-                                    for (int c = lane; c < left; c += 32) cp_async4(to + (32 * q + row) * kTsRowPitch + c, src + c);
-                            }
-                        }
-                    }
-                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&x_full[st])) : "memory");
-                    ++n;
-                }
             }
             asm volatile("cp.async.wait_all;" ::: "memory");             // none may be in flight when the CTA ends
         } else if (warp == 0 && lane == 0) {
@@ -450,18 +426,18 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
             unsigned round = 1;                                          // parity of the stage's last use but one
             bool ok = true;
             const uint32_t base = smem_u32(stages);
-            // one chunk: `rows_a` rows of tile a and then `rows_b` of tile b, heads and remainders; tiles hold `half_a` / `half_b` floats of each
-            auto copy = [&](const float* a, int half_a, uint32_t rows_a, const float* b, int half_b, uint32_t rows_b) {
+            // one chunk: `rows_a` rows of a 128-column tile and then `rows_b` of a hidden tile, heads and remainders
+            auto copy = [&](const float* a, uint32_t rows_a, const float* b, uint32_t rows_b) {
                 if (n >= NS && !ts_wait(&b_free[st], round, &failed)) { ok = false; return; }
                 const uint32_t bar = smem_u32(&b_full[st]), to = base + st * L::stage_bytes, half = (rows_a + rows_b) * 128u;
                 asm volatile("{\n\t.reg .b64 t;\n\tmbarrier.arrive.expect_tx.shared::cta.b64 t, [%0], %1;\n\t}" ::"r"(bar), "r"(2 * half) : "memory");
                 if (rows_a) {
                     ts_bulk(to, a, rows_a * 128u, bar);
-                    ts_bulk(to + half, a + half_a, rows_a * 128u, bar);
+                    ts_bulk(to + half, a + kTsTileBytes / 4, rows_a * 128u, bar);
                 }
                 if (rows_b) {
                     ts_bulk(to + rows_a * 128u, b, rows_b * 128u, bar);
-                    ts_bulk(to + half + rows_a * 128u, b + half_b, rows_b * 128u, bar);
+                    ts_bulk(to + half + rows_a * 128u, b + L::Rp * kTsChunk, rows_b * 128u, bar);
                 }
                 ++n;
                 if (++st == NS) { st = 0; round ^= 1u; }
@@ -478,14 +454,16 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
                 const float* shared = d.W + static_cast<long long>(w.block) * s.nx * (2 * kTsTileBytes / 4);
                 const float* first = d.first + s.group * d.first_group;
                 const float* second = d.second + s.group * d.second_group + static_cast<long long>(w.block) * s.rounds * (2 * kTsTileBytes / 4);
-                for (int j = 0; j < s.nx && ok; ++j) {
-                    copy(shared, kTsTileBytes / 4, s.main_cols, first, L::Rp * kTsChunk, s.adapter ? L::Rp : 0);
-                    shared += 2 * kTsTileBytes / 4;
-                    first += 2 * L::Rp * kTsChunk;
-                }
-                for (int e = 0; e < s.rounds && ok; ++e) {
-                    copy(second, kTsTileBytes / 4, s.cols, nullptr, 0, 0);
-                    second += 2 * kTsTileBytes / 4;
+#pragma unroll 1
+                for (int j = 0; j < s.nx + s.rounds && ok; ++j) {
+                    if (j < s.nx) {
+                        copy(shared, s.main_cols, first, s.adapter ? L::Rp : 0);
+                        shared += 2 * kTsTileBytes / 4;
+                        first += 2 * L::Rp * kTsChunk;
+                    } else {
+                        copy(second, s.cols, nullptr, 0);
+                        second += 2 * kTsTileBytes / 4;
+                    }
                 }
             }
             if (!ok)                                                     // copies in flight write into this CTA's memory: wait for them (bounded)
@@ -504,48 +482,60 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
                 mbar_arrive(&work_free[slot]);
                 if (!w.found) break;
                 const TsShape s = ts_shape(pass, w);
-                const int cols = s.main_cols + (s.adapter ? L::Rp : 0);
-                const uint32_t idesc = ts_idesc(cols), d0 = tmem + (s.main_cols ? 0 : 128);
-                for (int j = 0; j < s.nx; ++j) {
-                    if ((j & 1) == 0 && nd >= 2) ok = ts_wait(&d_free[sum], sum_par, &failed);
-                    ok = ok && ts_wait(&a_full[op], op_par, &failed) && ts_wait(&b_full[st], st_par, &failed);
-                    if (!ok) break;
-                    ts_fence_after();
-                    const uint32_t a = tmem + L::slot0 + 64 * op, b = base + st * L::stage_bytes;
-                    ts_chunk(d0 + sum * L::sum_cols, a, a + 32, b, b + cols * 128u, idesc, 4, (j & 1) != 0);
-                    ts_commit(&a_free[op]);
-                    ts_commit(&b_free[st]);
-                    if (++op == L::slots) { op = 0; op_par ^= 1u; }
-                    if (++st == NS) { st = 0; st_par ^= 1u; }
-                    if ((j & 1) != 0 || j + 1 == s.nx) {
-                        ts_commit(&d_full[sum]);
-                        ++nd;
-                        sum ^= 1;
-                        if (sum == 0) sum_par ^= 1u;
+                // chunks of inner values, then rounds of hidden values on top of the last sum: one piece of code, which stays in the instruction cache
+#pragma unroll 1
+                for (int j = 0; j < s.nx + s.rounds; ++j) {
+                    const bool inner = j < s.nx;
+                    const int e = j - s.nx;
+                    int cols, steps = 4;
+                    uint32_t d, hi, lo;
+                    bool add;
+                    if (inner) {
+                        if ((j & 1) == 0 && nd >= 2) ok = ts_wait(&d_free[sum], sum_par, &failed);
+                        ok = ok && ts_wait(&a_full[op], op_par, &failed);
+                        cols = s.main_cols + (s.adapter ? L::Rp : 0);
+                        d = tmem + sum * L::sum_cols + (s.main_cols ? 0 : 128);
+                        hi = tmem + L::slot0 + 64 * op;
+                        lo = hi + 32;
+                        add = (j & 1) != 0;
+                    } else {
+                        if (e == 0) ok = ts_wait(&t_full, hid_par, &failed);
+                        cols = s.cols;
+                        steps = min(4, L::Rp / 8 - 4 * e);
+                        d = tmem + (sum ^ 1) * L::sum_cols;
+                        hi = d + s.hid_col + 32 * e;
+                        lo = tmem + sum * L::sum_cols + s.hid_col + 32 * e;
+                        add = s.main_cols > 0 || e > 0;
                     }
-                }
-                if (!ok || s.rounds == 0) continue;
-                const uint32_t last = tmem + (sum ^ 1) * L::sum_cols, other = tmem + sum * L::sum_cols;
-                ok = ts_wait(&t_full, hid_par, &failed);
-                for (int e = 0; e < s.rounds && ok; ++e) {
-                    ok = ts_wait(&b_full[st], st_par, &failed);
+                    ok = ok && ts_wait(&b_full[st], st_par, &failed);
                     if (!ok) break;
                     ts_fence_after();
                     const uint32_t b = base + st * L::stage_bytes;
-                    ts_chunk(last, last + s.hid_col + 32 * e, other + s.hid_col + 32 * e, b, b + s.cols * 128u, ts_idesc(s.cols), min(4, L::Rp / 8 - 4 * e),
-                             s.main_cols > 0 || e > 0);
+                    ts_chunk(d, hi, lo, b, b + cols * 128u, ts_idesc(cols), steps, add);
                     ts_commit(&b_free[st]);
                     if (++st == NS) { st = 0; st_par ^= 1u; }
+                    if (inner) {
+                        ts_commit(&a_free[op]);
+                        if (++op == L::slots) { op = 0; op_par ^= 1u; }
+                        if ((j & 1) != 0 || j + 1 == s.nx) {
+                            ts_commit(&d_full[sum]);
+                            ++nd;
+                            sum ^= 1;
+                            if (sum == 0) sum_par ^= 1u;
+                        }
+                    } else if (e + 1 == s.rounds) {
+                        ts_commit(&t_done);
+                        hid_par ^= 1u;
+                    }
                 }
-                ts_commit(&t_done);
-                hid_par ^= 1u;
             }
         }
     } else if (warp < 8) {
         ts_registers_less<kTsRegsRows>();
         const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
         const int tid = threadIdx.x & 127;
-        int nx = 0, na = 0;                          // row stages and row operands used so far
+        int st = 0, op = 0, na = 0;                  // row stage and row operand in turn, operands so far
+        unsigned st_par = 0, op_par = 1;             // parity of the stage's next use, of the operand's last one
         bool ok = true;
         for (int i = 0; ok; ++i) {
             const int slot = i % kTsWorkRing;
@@ -556,42 +546,40 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
             if (!w.found) break;
             const int Kd = pass.degree[w.degree].Kd;
             const bool live = tid < w.rows.rows;
-            // the next 32 values are read while the current ones are split and stored
-            float next[32];
-            auto read = [&](int k0) {
-                const int st = nx % kTsRowStages;
-                if (k0 % kTsRowValues == 0 && !ts_wait_warp(&x_full[st], (nx / kTsRowStages) & 1, &failed)) { ok = false; return; }
-                const float* from = row_stages + st * L::row_floats + tid * kTsRowPitch + k0 % kTsRowValues;
-#pragma unroll
-                for (int q = 0; q < 8; ++q) {
-                    const float4 f = *reinterpret_cast<const float4*>(from + 4 * q);
-                    next[4 * q] = f.x; next[4 * q + 1] = f.y; next[4 * q + 2] = f.z; next[4 * q + 3] = f.w;
-                }
-                if (k0 % kTsRowValues != 0 || k0 + kTsChunk >= Kd) ++nx;
-            };
-            read(0);
-            for (int k0 = 0; k0 < Kd && ok; k0 += kTsChunk) {
-                float v[32], lo[32];
-                if (!live || k0 + kTsChunk > Kd)     // what the stage holds behind the tile's or the row's end is no value
-#pragma unroll
-                    for (int q = 0; q < 32; ++q) next[q] = live && k0 + q < Kd ? next[q] : 0.f;
-#pragma unroll
-                for (int q = 0; q < 32; ++q) ts_split(next[q], v[q], lo[q]);
-                if (k0 % kTsRowValues != 0 || k0 + kTsChunk >= Kd) {     // the stage has been read (its values are in registers)
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&x_free[(nx - 1) % kTsRowStages]);
-                }
-                const int op = na % L::slots;
-                if (na >= L::slots && !ts_wait_warp(&a_free[op], (na / L::slots - 1) & 1, &failed)) { ok = false; break; }
+            for (int k0 = 0; k0 < Kd; k0 += kTsChunk) {
+                if (k0 % kTsRowValues == 0 && !ts_wait_warp(&x_full[st], st_par, &failed)) { ok = false; break; }
+                if (na >= L::slots && !ts_wait_warp(&a_free[op], op_par, &failed)) { ok = false; break; }
                 ts_fence_after();
-                ts_store32(lanes + L::slot0 + 64 * op, v);
-                ts_store32(lanes + L::slot0 + 64 * op + 32, lo);
-                if (k0 + kTsChunk < Kd) read(k0 + kTsChunk);
+                const float* from = row_stages + st * L::row_floats + tid * kTsRowPitch + k0 % kTsRowValues;
+                const uint32_t to = lanes + L::slot0 + 64 * op;
+                const int good = live ? Kd - k0 : 0;                     // what the stage holds behind the tile's or the row's end is no value
+#pragma unroll 1
+                for (int q = 0; q < kTsChunk; q += 16) {
+                    float v[16], lo[16];
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4) {
+                        const float4 f = *reinterpret_cast<const float4*>(from + q + e);
+                        v[e] = f.x; v[e + 1] = f.y; v[e + 2] = f.z; v[e + 3] = f.w;
+                    }
+                    if (good < q + 16)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) v[e] = q + e < good ? v[e] : 0.f;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) ts_split(v[e], v[e], lo[e]);
+                    ts_store16(to + q, v);
+                    ts_store16(to + 32 + q, lo);
+                }
+                if (k0 % kTsRowValues != 0 || k0 + kTsChunk >= Kd) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&x_free[st]);
+                    if (++st == kTsRowStages) { st = 0; st_par ^= 1u; }
+                }
                 ts_wait_store();
                 ts_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&a_full[op]);
                 ++na;
+                if (++op == L::slots) { op = 0; op_par ^= 1u; }
             }
         }
     } else {
@@ -603,13 +591,14 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
         int nd = 0, nt = 0, i = 0;                   // partial sums and hidden rows used so far, tiles
         bool ok = true;
         TsWork w{};
-        int atom = 0, place = 0, comp = 0;
+        long long out_at = 0;
+        int place = 0, comp = 0;
         float weight = 1.f;
         auto next_work = [&]() {
             const int slot = i % kTsWorkRing;
             if (!ts_wait_warp(&work_full[slot], (i / kTsWorkRing) & 1, &failed)) { ok = false; return; }
             w = work[slot];
-            atom = work_atom[slot][tid];
+            out_at = work_out[slot][tid];
             place = work_place[slot][tid];
             comp = work_comp[slot][tid];
             weight = work_weight[slot][tid];
@@ -618,7 +607,7 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
             ++i;
         };
         next_work();
-        long long at_hand = blockIdx.x;              // for the tiles to give up
+        int at_hand = blockIdx.x;              // for the tiles to give up
         while (ok && w.found) {
             at_hand = w.index;
             const TsShape s = ts_shape(pass, w);
@@ -627,7 +616,7 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
             const bool live = tid < s.rows;
             float* out_row = nullptr;
             float* hid_row = nullptr;
-            if (live && pass.out) out_row = pass.out + (pass.out_sorted ? place : atom) * pass.out_stride + d.out_off + static_cast<long long>(comp) * d.Nc + s.col0 + 64 * half;
+            if (live && pass.out) out_row = pass.out + out_at + s.col0 + 64 * half;
             if (live && s.adapter && d.hidden && w.block == 0) hid_row = d.hidden + (static_cast<long long>(place) * d.comps + comp) * R + 16 * hid0;
             const int left = d.Nc - s.col0 - 64 * half;                  // columns of this half that exist
             float sum[64], hid[16 * kLower];
@@ -736,7 +725,7 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
             // NaN into the tile at hand and all that would have followed
             TsCursor cursor;
             TsWork lost{};
-            for (long long t = at_hand; cursor.find(pass, t, lost); t += gridDim.x) ts_fill(pass, lost, tid, 128, NAN);
+            for (int t = at_hand; cursor.find(pass, t, lost); t += gridDim.x) ts_fill(pass, lost, tid, 128, NAN);
         }
     }
     __syncwarp();
