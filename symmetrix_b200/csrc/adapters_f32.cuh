@@ -279,7 +279,8 @@ __device__ __forceinline__ void ts_bulk(uint32_t to, const float* from, uint32_t
 }
 
 // One persistent CTA per SM walks tiles of 128 rows x 128 columns; its warps are specialised, so that the parts of neighbouring tiles overlap:
-//   warp 0      weight images: bulk copies of a chunk's [W | first_g] tiles, or of a round's second_g tiles, into a ring of stages
+//   warp 0      weight images: bulk copies of a chunk's [W | first_g] tiles, or of a round's second_g tiles, into a ring of stages; a stage
+//               is these tiles in shared memory and 32 values of the rows in tensor memory, with one barrier for both
 //   warp 1      the products (one thread)
 //   warp 2      finds the tiles and looks up their atoms and weights (a ring of four, ahead of all others)
 //   warp 3      rows: 64 values of each by asynchronous copies of 16 bytes (4 where rows start on no 16-byte boundary) into a ring of two stages
@@ -288,7 +289,7 @@ __device__ __forceinline__ void ts_bulk(uint32_t to, const float* from, uint32_t
 //   warps 8-15  a thread adds half of its row's partial sums of every 64 inner values in registers (the tensor core cuts its sums instead of
 //               rounding them: a single sum over 128 inner values was off five times as far as float32) and writes its half of the row
 //               while the products of the next tile run
-// TMEM: two partial sums of 128 + Rp columns, taken in turn, and two or three row operands of 64. The shared columns of a tile's last two
+// TMEM: two partial sums of 128 + Rp columns, taken in turn, and the stages' row operands of 64. The shared columns of a tile's last two
 // sums stay where they are while its hidden row is weighted, split and stored into their hidden columns (head in the last one's, remainder in
 // the other's); the products with second_g go on top of the last sum, and both are read then.
 // Every wait is bounded; if one runs out, the CTA gives up and fills its remaining tiles with NaN.
@@ -298,12 +299,12 @@ constexpr int kTsRegsControl = 72, kTsRegsRows = 120, kTsRegsSums = 160, kTsRegs
 static_assert(kTsRegsControl + kTsRegsRows + 2 * kTsRegsSums <= 4 * kTsRegsLaunch, "the registers of the launch are shared out");
 template <int HP>                                    // hidden columns / 16
 struct TsPassLayout {
-    static constexpr int Rp = 16 * HP, sum_cols = 128 + Rp, slots = HP > 2 ? 2 : 3, stages = HP > 2 ? 2 : 3;
+    static constexpr int Rp = 16 * HP, sum_cols = 128 + Rp, stages = HP > 2 ? 2 : 3;
     static constexpr int slot0 = 2 * sum_cols;
     static constexpr uint32_t stage_bytes = sum_cols * 256u;
     static constexpr int row_floats = kTsRows * kTsRowPitch;
     static constexpr int smem = stages * static_cast<int>(stage_bytes) + kTsRowStages * row_floats * 4 + 1024;
-    static_assert(slot0 + 64 * slots <= 512, "tensor memory has 512 columns");
+    static_assert(slot0 + 64 * stages <= 512, "tensor memory has 512 columns");
     static_assert(smem + 15 * 1024 <= 227 * 1024, "shared memory of one CTA per SM");
 };
 
@@ -312,8 +313,8 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
     using L = TsPassLayout<HP>;
     constexpr int NS = L::stages;
     extern __shared__ unsigned char ts_smem_raw[];
-    __shared__ __align__(8) unsigned long long work_full[kTsWorkRing], work_free[kTsWorkRing], b_full[NS], b_free[NS], x_full[kTsRowStages],
-        x_free[kTsRowStages], a_full[3], a_free[3], d_full[2], d_free[2], t_full, t_done;
+    __shared__ __align__(8) unsigned long long work_full[kTsWorkRing], work_free[kTsWorkRing], full[NS], free[NS], x_full[kTsRowStages],
+        x_free[kTsRowStages], d_full[2], d_free[2], t_full, t_done;
     __shared__ TsWork work[kTsWorkRing];
     __shared__ long long work_in[kTsWorkRing][kTsRows], work_out[kTsWorkRing][kTsRows];    // where its rows start, in `in`, in `out` without the tile's
     __shared__ int work_place[kTsWorkRing][kTsRows];                                       // first column; sorted position and component
@@ -327,9 +328,8 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
     if (threadIdx.x == 0) {
         failed = 0;
         for (int q = 0; q < kTsWorkRing; ++q) { mbar_init(&work_full[q], 1); mbar_init(&work_free[q], 15); }
-        for (int q = 0; q < NS; ++q) { mbar_init(&b_full[q], 1); mbar_init(&b_free[q], 1); }
+        for (int q = 0; q < NS; ++q) { mbar_init(&full[q], 5); mbar_init(&free[q], 1); }
         for (int q = 0; q < kTsRowStages; ++q) { mbar_init(&x_full[q], 32); mbar_init(&x_free[q], 4); }
-        for (int q = 0; q < 3; ++q) { mbar_init(&a_full[q], 4); mbar_init(&a_free[q], 1); }
         for (int q = 0; q < 2; ++q) { mbar_init(&d_full[q], 1); mbar_init(&d_free[q], 8); }
         mbar_init(&t_full, 8);
         mbar_init(&t_done, 1);
@@ -428,8 +428,8 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
             const uint32_t base = smem_u32(stages);
             // one chunk: `rows_a` rows of a 128-column tile and then `rows_b` of a hidden tile, heads and remainders
             auto copy = [&](const float* a, uint32_t rows_a, const float* b, uint32_t rows_b) {
-                if (n >= NS && !ts_wait(&b_free[st], round, &failed)) { ok = false; return; }
-                const uint32_t bar = smem_u32(&b_full[st]), to = base + st * L::stage_bytes, half = (rows_a + rows_b) * 128u;
+                if (n >= NS && !ts_wait(&free[st], round, &failed)) { ok = false; return; }
+                const uint32_t bar = smem_u32(&full[st]), to = base + st * L::stage_bytes, half = (rows_a + rows_b) * 128u;
                 asm volatile("{\n\t.reg .b64 t;\n\tmbarrier.arrive.expect_tx.shared::cta.b64 t, [%0], %1;\n\t}" ::"r"(bar), "r"(2 * half) : "memory");
                 if (rows_a) {
                     ts_bulk(to, a, rows_a * 128u, bar);
@@ -467,11 +467,10 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
                 }
             }
             if (!ok)                                                     // copies in flight write into this CTA's memory: wait for them (bounded)
-                for (int q = max(0, n - NS); q < n; ++q) mbar_wait(&b_full[q % NS], (q / NS) & 1);
+                for (int q = max(0, n - NS); q < n; ++q) mbar_wait(&full[q % NS], (q / NS) & 1);
         } else if (warp == 1 && lane == 0) {
-            // stages, row operands and partial sums in turn, each with the parity of its next use; hidden rows
-            int st = 0, op = 0, sum = 0, nd = 0;
-            unsigned st_par = 0, op_par = 0, sum_par = 1, hid_par = 0;
+            int st = 0, sum = 0, nd = 0;                                 // stage and partial sum in turn, with the parity of their next and last use
+            unsigned st_par = 0, sum_par = 1, hid_par = 0;
             bool ok = true;
             const uint32_t base = smem_u32(stages);
             for (int i = 0; ok; ++i) {
@@ -492,10 +491,9 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
                     bool add;
                     if (inner) {
                         if ((j & 1) == 0 && nd >= 2) ok = ts_wait(&d_free[sum], sum_par, &failed);
-                        ok = ok && ts_wait(&a_full[op], op_par, &failed);
                         cols = s.main_cols + (s.adapter ? L::Rp : 0);
                         d = tmem + sum * L::sum_cols + (s.main_cols ? 0 : 128);
-                        hi = tmem + L::slot0 + 64 * op;
+                        hi = tmem + L::slot0 + 64 * st;
                         lo = hi + 32;
                         add = (j & 1) != 0;
                     } else {
@@ -507,16 +505,14 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
                         lo = tmem + sum * L::sum_cols + s.hid_col + 32 * e;
                         add = s.main_cols > 0 || e > 0;
                     }
-                    ok = ok && ts_wait(&b_full[st], st_par, &failed);
+                    ok = ok && ts_wait(&full[st], st_par, &failed);
                     if (!ok) break;
                     ts_fence_after();
                     const uint32_t b = base + st * L::stage_bytes;
                     ts_chunk(d, hi, lo, b, b + cols * 128u, ts_idesc(cols), steps, add);
-                    ts_commit(&b_free[st]);
+                    ts_commit(&free[st]);
                     if (++st == NS) { st = 0; st_par ^= 1u; }
                     if (inner) {
-                        ts_commit(&a_free[op]);
-                        if (++op == L::slots) { op = 0; op_par ^= 1u; }
                         if ((j & 1) != 0 || j + 1 == s.nx) {
                             ts_commit(&d_full[sum]);
                             ++nd;
@@ -534,7 +530,7 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
         ts_registers_less<kTsRegsRows>();
         const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
         const int tid = threadIdx.x & 127;
-        int st = 0, op = 0, na = 0;                  // row stage and row operand in turn, operands so far
+        int st = 0, op = 0, na = 0;                  // row stage and operand stage in turn, operands so far
         unsigned st_par = 0, op_par = 1;             // parity of the stage's next use, of the operand's last one
         bool ok = true;
         for (int i = 0; ok; ++i) {
@@ -544,14 +540,24 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
             __syncwarp();
             if (lane == 0) mbar_arrive(&work_free[slot]);
             if (!w.found) break;
+            const TsShape s = ts_shape(pass, w);
             const int Kd = pass.degree[w.degree].Kd;
-            const bool live = tid < w.rows.rows;
-            for (int k0 = 0; k0 < Kd; k0 += kTsChunk) {
-                if (k0 % kTsRowValues == 0 && !ts_wait_warp(&x_full[st], st_par, &failed)) { ok = false; break; }
-                if (na >= L::slots && !ts_wait_warp(&a_free[op], op_par, &failed)) { ok = false; break; }
+            const bool live = tid < s.rows;
+            for (int j = 0; j < s.nx + s.rounds; ++j) {
+                const int k0 = j * kTsChunk;
+                const bool inner = j < s.nx;
+                if (inner && k0 % kTsRowValues == 0 && !ts_wait_warp(&x_full[st], st_par, &failed)) { ok = false; break; }
+                if (na >= NS && !ts_wait_warp(&free[op], op_par, &failed)) { ok = false; break; }
+                ++na;
+                unsigned long long* const bar = &full[op];
+                const uint32_t to = lanes + L::slot0 + 64 * op;
+                if (++op == NS) { op = 0; op_par ^= 1u; }
+                if (!inner) {                        // a round of hidden values has the stage's weights, not its row operand
+                    if (lane == 0) mbar_arrive(bar);
+                    continue;
+                }
                 ts_fence_after();
                 const float* from = row_stages + st * L::row_floats + tid * kTsRowPitch + k0 % kTsRowValues;
-                const uint32_t to = lanes + L::slot0 + 64 * op;
                 const int good = live ? Kd - k0 : 0;                     // what the stage holds behind the tile's or the row's end is no value
 #pragma unroll 1
                 for (int q = 0; q < kTsChunk; q += 16) {
@@ -577,9 +583,7 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
                 ts_wait_store();
                 ts_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&a_full[op]);
-                ++na;
-                if (++op == L::slots) { op = 0; op_par ^= 1u; }
+                if (lane == 0) mbar_arrive(bar);
             }
         }
     } else {
