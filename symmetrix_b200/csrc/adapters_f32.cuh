@@ -289,9 +289,9 @@ __device__ __forceinline__ void ts_bulk(uint32_t to, const float* from, uint32_t
 //   warps 8-15  a thread adds half of its row's partial sums of every 64 inner values in registers (the tensor core cuts its sums instead of
 //               rounding them: a single sum over 128 inner values was off five times as far as float32) and writes its half of the row
 //               while the products of the next tile run
-// TMEM: two partial sums of 128 + Rp columns, taken in turn, and the stages' row operands of 64. The shared columns of a tile's last two
-// sums stay where they are while its hidden row is weighted, split and stored into their hidden columns (head in the last one's, remainder in
-// the other's); the products with second_g go on top of the last sum, and both are read then.
+// TMEM: two partial sums of 128 + Rp columns, taken in turn, and the stages' row operands of 64. The hidden row of a tile is weighted, split and
+// stored into the hidden columns of its last two sums (head in the last one's, remainder in the other's); the products with second_g go on
+// top of the last sum, which is read after them.
 // Every wait is bounded; if one runs out, the CTA gives up and fills its remaining tiles with NaN.
 constexpr int kTsPassThreads = 512, kTsWorkRing = 4, kTsRowStages = 2;
 constexpr int kTsRowValues = 64, kTsRowPitch = kTsRowValues + 4;              // floats: threads that read their rows 16 bytes at a time hit all banks
@@ -643,7 +643,8 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&d_free[use & 1]);
             };
-            const int stay = s.rounds > 0 ? max(0, s.sums - 2) : s.sums;     // from this sum on the shared columns stay until the end
+            // with rounds, the last sum's shared columns are read at the end, and the last two are given back there
+            const int stay = s.rounds > 0 ? s.sums - 1 : s.sums, kept = s.rounds > 0 ? min(2, s.sums) : 0;
             for (int j = 0; j < s.sums; ++j, ++nd) {
                 if (!ts_wait_warp(&d_full[nd & 1], (nd >> 1) & 1, &failed)) { ok = false; break; }
                 ts_fence_after();
@@ -657,10 +658,8 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
 #pragma unroll
                             for (int q = 0; q < 16; ++q) hid[16 * cc + q] += v[q];
                         }
-                if (j < stay) {
-                    add_columns(from, s.main_cols);
-                    release(nd);
-                }
+                if (j < stay) add_columns(from, s.main_cols);
+                if (j < s.sums - kept) release(nd);
             }
             if (!ok) break;
             if (s.rounds > 0) {
@@ -699,11 +698,9 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
                 if (!ts_wait_warp(&t_done, nt & 1, &failed)) { ok = false; break; }
                 ++nt;
                 ts_fence_after();
-                for (int use = nd - (s.sums - stay); use < nd; ++use) {
-                    // without shared weights only the last one has such columns
-                    if (s.main_cols || use == nd - 1) add_columns(lanes + (use & 1) * L::sum_cols, s.cols);
-                    release(use);
-                }
+                if (kept == 2) release(nd - 2);
+                add_columns(lanes + ((nd - 1) & 1) * L::sum_cols, s.cols);
+                release(nd - 1);
             }
             next_work();
             if (!ok) break;
