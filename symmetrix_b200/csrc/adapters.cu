@@ -16,6 +16,7 @@
 #include <algorithm>
 #include <climits>
 #include <cstdint>
+#include <type_traits>
 
 #include "common.cuh"
 #include "routing.hpp"
@@ -25,16 +26,14 @@ namespace {
 
 constexpr int kMaxDegrees = SMX_ADAPTER_MAX_DEGREES, kMaxRank = SMX_ADAPTER_MAX_RANK;
 
-// One degree of a pass: out rows = in rows . W + weight (in rows . first_g) . second_g. Matrices are addressed by strides, so that a
-// transposed one is the same memory.
+// One pass over the rows, in either direction: out rows = in rows . W + weight (in rows . first_g) . second_g, degree by degree.
 template <typename T>
 struct PassDegree {
     int comps, Kd, Nc;
     long long in_off, out_off;
-    const T* W; long long w_k, w_n;
-    const T* first; long long f_group, f_k, f_r;
-    const T* second; long long s_group, s_r, s_n;
-    T* hidden;                                  // [pairs * comps][rank] in sorted order, or null
+    const T* W; const T* first; const T* second;     // in the kernels' layouts; W null: no shared weights
+    long long first_group, second_group;             // values from adapter to adapter
+    T* hidden;                                       // [pairs * comps][rank] in sorted order, or null
 };
 template <typename T>
 struct Pass {
@@ -44,7 +43,7 @@ struct Pass {
     const int* order; const int* offsets;
     const T* weights;
     const T* in; long long in_stride;
-    T* out; long long out_stride;               // null: only the hidden rows
+    T* out; long long out_stride;                    // null: only the hidden rows
     int sorted;        // tiles by group, atoms through `order`; else all rows in their own order and no adapters
     int out_sorted;    // out rows by sorted position (workspace), else by atom
     int tail;          // the rows without a group are a last group of their own
@@ -90,122 +89,9 @@ __device__ __forceinline__ bool find_tile(const int* __restrict__ offsets, int g
     return false;
 }
 
-// ------------------------------------------------------------------------------------------- pass, plain tiles
-constexpr int kPlainBM = 32, kPlainBN = 64, kPlainBK = 32, kPlainThreads = 128;
-
-template <typename T>
-__global__ void __launch_bounds__(kPlainThreads) adapter_pass_plain_kernel(const __grid_constant__ Pass<T> pass) {
-    const PassDegree<T>& d = pass.degree[blockIdx.z];
-    const int col0 = blockIdx.y * kPlainBN;
-    if (col0 >= d.Nc) return;
-    __shared__ TileRows tile;
-    __shared__ int found;
-    __shared__ long long in_base[kPlainBM], out_base[kPlainBM], hid_row[kPlainBM];
-    __shared__ T weight[kPlainBM];
-    __shared__ T As[kPlainBM][kPlainBK + 1];
-    __shared__ T Bs[kPlainBK][kPlainBN + 1];
-    __shared__ T Hs[kPlainBM][kMaxRank + 1];
-    const int tid = threadIdx.x;
-    if (tid < 32) {
-        TileRows t{};
-        long long all_tiles;
-        bool ok;
-        if (pass.sorted) {
-            ok = find_tile(pass.offsets, pass.groups, pass.tail != 0, pass.pairs, d.comps, kPlainBM, blockIdx.x, t, all_tiles);
-        } else {
-            const long long all = pass.num_rows * d.comps;
-            t.group = pass.groups; t.first_pair = 0; t.row0 = static_cast<long long>(blockIdx.x) * kPlainBM;
-            t.rows = min(static_cast<long long>(kPlainBM), all - t.row0);
-            ok = t.rows > 0;
-        }
-        if (tid == 0) { tile = t; found = ok ? 1 : 0; }
-    }
-    __syncthreads();
-    if (!found) return;
-    const int rows = static_cast<int>(tile.rows), g = tile.group, R = pass.rank;
-    const bool adapter = g < pass.groups;
-    if (tid < rows) {
-        const long long r = tile.row0 + tid, p = tile.first_pair + r / d.comps;
-        const int m = static_cast<int>(r % d.comps);
-        const long long pair = pass.sorted ? pass.order[p] : p, n = pass.sorted ? pair / pass.slots : p;
-        in_base[tid] = n * pass.in_stride + d.in_off + static_cast<long long>(m) * d.Kd;
-        out_base[tid] = (pass.out_sorted ? p : n) * pass.out_stride + d.out_off + static_cast<long long>(m) * d.Nc;
-        hid_row[tid] = p * d.comps + m;
-        weight[tid] = adapter && pass.weights ? pass.weights[pair] : T(1);
-    }
-    const int tr = (tid >> 4) * 4, tc = (tid & 15) * 4;       // four rows, four columns a thread
-    T acc[4][4] = {};
-    T hid[kMaxRank / 4];
-#pragma unroll
-    for (int q = 0; q < kMaxRank / 4; ++q) hid[q] = T(0);
-    const int hr = tid >> 2, hc = tid & 3;                      // hidden value hc + 4 q of row hr
-    __syncthreads();
-    const T* first = adapter ? d.first + g * d.f_group : nullptr;
-    for (int k0 = 0; k0 < d.Kd; k0 += kPlainBK) {
-        for (int i = tid; i < kPlainBM * kPlainBK; i += kPlainThreads) {
-            const int r = i / kPlainBK, k = i % kPlainBK;
-            As[r][k] = r < rows && k0 + k < d.Kd ? pass.in[in_base[r] + k0 + k] : T(0);
-        }
-        if (d.W)
-            for (int i = tid; i < kPlainBK * kPlainBN; i += kPlainThreads) {
-                const int k = i / kPlainBN, c = i % kPlainBN;
-                Bs[k][c] = k0 + k < d.Kd && col0 + c < d.Nc ? d.W[(k0 + k) * d.w_k + (col0 + c) * d.w_n] : T(0);
-            }
-        __syncthreads();
-        if (d.W)
-            for (int k = 0; k < kPlainBK; ++k) {
-                T a[4], b[4];
-#pragma unroll
-                for (int q = 0; q < 4; ++q) { a[q] = As[tr + q][k]; b[q] = Bs[k][tc + q]; }
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[i][j] += a[i] * b[j];
-            }
-        if (adapter)
-            for (int k = 0; k < kPlainBK && k0 + k < d.Kd; ++k) {
-                const T a = As[hr][k];
-                const T* f = first + (k0 + k) * d.f_k;
-#pragma unroll
-                for (int q = 0; q < kMaxRank / 4; ++q)
-                    if (hc + 4 * q < R) hid[q] += a * f[(hc + 4 * q) * d.f_r];
-            }
-        __syncthreads();
-    }
-    if (adapter) {
-#pragma unroll
-        for (int q = 0; q < kMaxRank / 4; ++q) {
-            const int r = hc + 4 * q;
-            if (r < R && hr < rows) {
-                if (d.hidden && blockIdx.y == 0) d.hidden[hid_row[hr] * R + r] = hid[q];
-                Hs[hr][r] = weight[hr] * hid[q];
-            }
-        }
-        __syncthreads();
-        if (!pass.out) return;
-        const T* second = d.second + g * d.s_group;
-        for (int r = 0; r < R; ++r) {
-            T b[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) b[j] = col0 + tc + j < d.Nc ? second[r * d.s_r + (col0 + tc + j) * d.s_n] : T(0);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const T h = tr + i < rows ? Hs[tr + i][r] : T(0);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] += h * b[j];
-            }
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (tr + i < rows && col0 + tc + j < d.Nc) pass.out[out_base[tr + i] + col0 + tc + j] = acc[i][j];
-}
-
 // ------------------------------------------------------------------------------------------- gradients of the adapters
 // part[chunk][k][r] = sum over the chunk's rows of a[row][k] weight[row] h[row][r]; a is x with h = gy B^T, or gy with h = x A.
-constexpr int kGradChunk = 512, kGradCols = 32, kGradRows = 32, kGradThreads = 128;
+constexpr int kGradChunk = 512;
 template <typename T>
 struct GradProblem {
     int comps, Kd;
@@ -222,64 +108,6 @@ struct GradPass {
     const int* order; const int* offsets;
     const T* weights;
 };
-
-template <typename T>
-__global__ void __launch_bounds__(kGradThreads) adapter_grad_kernel(const __grid_constant__ GradPass<T> pass) {
-    const GradProblem<T>& d = pass.problem[blockIdx.z];
-    const int k0 = blockIdx.y * kGradCols;
-    if (k0 >= d.Kd) return;
-    __shared__ TileRows tile;
-    __shared__ int found;
-    __shared__ T As[kGradRows][kGradCols + 1];
-    __shared__ T Hs[kGradRows][kMaxRank + 1];
-    const int tid = threadIdx.x, R = pass.rank;
-    if (tid < 32) {
-        TileRows t{};
-        long long all_tiles;
-        const bool ok = find_tile(pass.offsets, pass.groups, false, pass.pairs, d.comps, kGradChunk, blockIdx.x, t, all_tiles);
-        if (tid == 0) { tile = t; found = ok ? 1 : 0; }
-    }
-    __syncthreads();
-    if (!found) return;
-    T acc[kMaxRank / 4];
-#pragma unroll
-    for (int q = 0; q < kMaxRank / 4; ++q) acc[q] = T(0);
-    const int kc = tid >> 2, rc = tid & 3;
-    for (int r0 = 0; r0 < tile.rows; r0 += kGradRows) {
-        for (int i = tid; i < kGradRows * kGradCols; i += kGradThreads) {
-            const int rr = i / kGradCols, k = i % kGradCols;
-            T v = T(0);
-            if (r0 + rr < tile.rows && k0 + k < d.Kd) {
-                const long long r = tile.row0 + r0 + rr, p = tile.first_pair + r / d.comps;
-                const int m = static_cast<int>(r % d.comps);
-                v = d.a[static_cast<long long>(pass.order[p] / pass.slots) * d.a_stride + d.a_off + static_cast<long long>(m) * d.Kd + k0 + k];
-            }
-            As[rr][k] = v;
-        }
-        for (int i = tid; i < kGradRows * R; i += kGradThreads) {
-            const int rr = i / R, q = i % R;
-            T v = T(0);
-            if (r0 + rr < tile.rows) {
-                const long long r = tile.row0 + r0 + rr, p = tile.first_pair + r / d.comps;
-                v = d.hidden[(tile.first_pair * d.comps + r) * R + q];
-                if (pass.weights) v *= pass.weights[pass.order[p]];
-            }
-            Hs[rr][q] = v;
-        }
-        __syncthreads();
-        for (int rr = 0; rr < kGradRows; ++rr) {
-            const T a = As[rr][kc];
-#pragma unroll
-            for (int q = 0; q < kMaxRank / 4; ++q)
-                if (rc + 4 * q < R) acc[q] += a * Hs[rr][rc + 4 * q];
-        }
-        __syncthreads();
-    }
-    if (k0 + kc < d.Kd)
-#pragma unroll
-        for (int q = 0; q < kMaxRank / 4; ++q)
-            if (rc + 4 * q < R) d.part[(static_cast<long long>(blockIdx.x) * d.Kd + k0 + kc) * R + rc + 4 * q] = acc[q];
-}
 
 // grad of group blockIdx.x: its chunks added in order (none: zero).
 template <typename T>
@@ -341,22 +169,10 @@ __global__ void __launch_bounds__(256) adapter_weight_grad_kernel(const __grid_c
 }  // namespace smx
 
 #include "adapters_f32.cuh"
+#include "adapters_f64.cuh"
 
 namespace smx {
 namespace {
-
-// ------------------------------------------------------------------------------------------- layout of the matrices
-struct CopyList {
-    static constexpr int kMost = 3 * kMaxDegrees;
-    const void* src[kMost]; void* dst[kMost];
-    long long count[kMost];
-};
-template <typename T>
-__global__ void __launch_bounds__(256) adapter_copy_kernel(const __grid_constant__ CopyList list) {
-    const T* src = static_cast<const T*>(list.src[blockIdx.y]);
-    T* dst = static_cast<T*>(list.dst[blockIdx.y]);
-    for (long long i = blockIdx.x * 256LL + threadIdx.x; i < list.count[blockIdx.y]; i += 256LL * gridDim.x) dst[i] = src[i];
-}
 
 // ------------------------------------------------------------------------------------------- host side
 void launched(const char* what) {
@@ -384,8 +200,6 @@ void check_call(const smx_adapter_linear& c) {
         const smx_adapter_degree& g = c.degrees[d];
         if (g.components < 1 || g.components > 1024 || g.in_channels < 1 || g.out_channels < 1 || g.in_channels > (1 << 20) || g.out_channels > (1 << 20))
             throw ArgError("smx_adapter: a degree needs 1 .. 1024 components and 1 .. 1048576 channels");
-        // grid.x counts row tiles
-        if (static_cast<long long>(c.num_rows) * c.slots * g.components / kPlainBM + c.num_groups + 1 > INT_MAX) throw ArgError("smx_adapter: too many rows");
     }
 }
 // buffers whose layout is the library's own are read and written in 16-byte pieces
@@ -445,7 +259,7 @@ Buffers<T> lay_out(const smx_adapter_linear& c, bool backward) {
     return b;
 }
 
-// The matrices of a degree inside `tiles`: float64 as they are, float32 as operand images of both directions (index 1: transposed).
+// The matrices of a degree inside `tiles`, for both directions (index 1: transposed): float32 as operand images, float64 with aligned rows.
 struct Matrices {
     const void *shared[2], *down[2], *up[2];
     size_t down_group[2], up_group[2];           // values from adapter to adapter
@@ -456,17 +270,18 @@ size_t tile_layout(const smx_adapter_linear& c, Matrices (&m)[kMaxDegrees]) {
     const int Rp = padded_rank(c.rank);
     for (int d = 0; d < c.num_degrees; ++d) {
         const smx_adapter_degree& g = c.degrees[d];
-        const size_t I = g.in_channels, O = g.out_channels;
         for (int back = 0; back < 2; ++back) {
-            if (sizeof(T) == 8) {
-                if (back) continue;
-                m[d].shared[0] = g.shared ? ws.take<T>(I * O) : nullptr;
-                m[d].down[0] = ws.take<T>(I * c.rank * c.num_groups);
-                m[d].up[0] = ws.take<T>(O * c.rank * c.num_groups);
-                continue;
-            }
             // `down` is the first factor forward and the second one backward, `up` the other way round
             const int K = back ? g.out_channels : g.in_channels, N = back ? g.in_channels : g.out_channels;
+            if (sizeof(T) == 8) {
+                const size_t first = static_cast<size_t>(K) * even(c.rank), second = static_cast<size_t>(c.rank) * even(N);
+                m[d].shared[back] = g.shared ? ws.take<T>(static_cast<size_t>(K) * even(N)) : nullptr;
+                m[d].down_group[back] = back ? second : first;
+                m[d].up_group[back] = back ? first : second;
+                m[d].down[back] = ws.take<T>(m[d].down_group[back] * c.num_groups);
+                m[d].up[back] = ws.take<T>(m[d].up_group[back] * c.num_groups);
+                continue;
+            }
             const size_t tile = 2 * kTsTileBytes / sizeof(float);
             const size_t first = static_cast<size_t>(ts_chunks(K)) * 2 * Rp * kTsChunk, second = static_cast<size_t>(ts_blocks(N)) * ts_chunks(Rp) * tile;
             m[d].shared[back] = g.shared ? ws.take<T>(static_cast<size_t>(ts_blocks(N)) * ts_chunks(K) * tile) : nullptr;
@@ -488,23 +303,32 @@ void prepare(const smx_adapter_linear& c, int parts) {
     long long most = 0;
     if (c.precision == SMX_FP64) {
         tile_layout<double>(c, m);
-        CopyList list{};
-        auto add = [&](const void* src, const void* dst, long long count) {
-            list.src[n] = src; list.dst[n] = const_cast<void*>(dst); list.count[n++] = count;
-            most = std::max(most, count);
+        DoubleList list{};
+        auto add = [&](const void* src, const void* dst, int groups, long long group_stride, int K, long long k_stride, int N, long long n_stride) {
+            DoubleSegment& s = list.segment[n++];
+            s.src = static_cast<const double*>(src); s.dst = static_cast<double*>(const_cast<void*>(dst));
+            s.groups = groups; s.group_stride = group_stride; s.K = K; s.k_stride = k_stride; s.N = N; s.n_stride = n_stride; s.ld = even(N);
+            most = std::max(most, static_cast<long long>(groups) * K * s.ld);
         };
+        const int R = c.rank;
         for (int d = 0; d < c.num_degrees; ++d) {
             const smx_adapter_degree& g = c.degrees[d];
-            const long long I = g.in_channels, O = g.out_channels;
-            if ((parts & SMX_ADAPTER_SHARED) && g.shared) add(g.shared, m[d].shared[0], I * O);
+            const int I = g.in_channels, O = g.out_channels;
+            if ((parts & SMX_ADAPTER_SHARED) && g.shared) {
+                add(g.shared, m[d].shared[0], 1, 0, I, O, O, 1);
+                add(g.shared, m[d].shared[1], 1, 0, O, 1, I, O);
+            }
             if (parts & SMX_ADAPTER_MATRICES) {
-                add(g.down, m[d].down[0], I * c.rank * c.num_groups);
-                add(g.up, m[d].up[0], O * c.rank * c.num_groups);
+                const long long down = static_cast<long long>(I) * R, up = static_cast<long long>(R) * O;
+                add(g.down, m[d].down[0], c.num_groups, down, I, R, R, 1);
+                add(g.up, m[d].up[0], c.num_groups, up, R, O, O, 1);
+                add(g.up, m[d].up[1], c.num_groups, up, O, 1, R, O);
+                add(g.down, m[d].down[1], c.num_groups, down, R, 1, I, R);
             }
         }
         if (!n) return;
-        adapter_copy_kernel<double><<<dim3(static_cast<unsigned>(std::min<long long>(256, (most + 255) / 256)), n), 256, 0, stream>>>(list);
-        launched("adapter_copy_kernel");
+        adapter_layout_kernel<<<dim3(static_cast<unsigned>(std::min<long long>(1024, (most + 255) / 256)), n), 256, 0, stream>>>(list);
+        launched("adapter_layout_kernel");
         return;
     }
     tile_layout<float>(c, m);
@@ -547,24 +371,18 @@ Pass<T> make_pass(const smx_adapter_linear& c, bool transposed, T* hidden) {
     for (int q = 0; q < c.num_degrees; ++q) {
         const smx_adapter_degree& g = c.degrees[q];
         PassDegree<T>& d = p.degree[q];
-        const long long I = g.in_channels, O = g.out_channels, R = c.rank;
-        const T *shared = static_cast<const T*>(m[q].shared[0]), *down = static_cast<const T*>(m[q].down[0]), *up = static_cast<const T*>(m[q].up[0]);
         d.comps = g.components;
         d.in_off = in_off; d.out_off = out_off;
-        d.W = shared;
-        if (!transposed) {
-            d.Kd = g.in_channels; d.Nc = g.out_channels;
-            d.w_k = O; d.w_n = 1;
-            d.first = down; d.f_group = I * R; d.f_k = R; d.f_r = 1;
-            d.second = up; d.s_group = R * O; d.s_r = O; d.s_n = 1;
-        } else {
-            d.Kd = g.out_channels; d.Nc = g.in_channels;
-            d.w_k = 1; d.w_n = O;
-            d.first = up; d.f_group = R * O; d.f_k = 1; d.f_r = O;
-            d.second = down; d.s_group = I * R; d.s_r = 1; d.s_n = R;
-        }
+        d.Kd = transposed ? g.out_channels : g.in_channels;
+        d.Nc = transposed ? g.in_channels : g.out_channels;
+        const int back = transposed ? 1 : 0;
+        d.W = static_cast<const T*>(m[q].shared[back]);
+        d.first = static_cast<const T*>(transposed ? m[q].up[1] : m[q].down[0]);
+        d.second = static_cast<const T*>(transposed ? m[q].down[1] : m[q].up[0]);
+        d.first_group = static_cast<long long>(transposed ? m[q].up_group[1] : m[q].down_group[0]);
+        d.second_group = static_cast<long long>(transposed ? m[q].down_group[1] : m[q].up_group[0]);
         d.hidden = hidden;
-        if (hidden) hidden += pairs * g.components * R;
+        if (hidden) hidden += pairs * g.components * c.rank;
         in_off += static_cast<long long>(g.components) * d.Kd;
         out_off += static_cast<long long>(g.components) * d.Nc;
     }
@@ -573,19 +391,6 @@ Pass<T> make_pass(const smx_adapter_linear& c, bool transposed, T* hidden) {
     p.order = c.order; p.offsets = c.offsets;
     p.weights = static_cast<const T*>(c.weights);
     return p;
-}
-
-void launch_pass(const smx_adapter_linear&, bool, const Pass<double>& p, int degrees, cudaStream_t stream) {
-    long long rows = 0;
-    int cols = 0;
-    for (int d = 0; d < degrees; ++d) {
-        rows = std::max(rows, (p.sorted ? p.pairs : p.num_rows) * p.degree[d].comps);
-        cols = std::max(cols, p.degree[d].Nc);
-    }
-    const long long tiles = p.sorted ? rows / kPlainBM + p.groups + 1 : (rows + kPlainBM - 1) / kPlainBM;
-    const dim3 grid(static_cast<unsigned>(tiles), (cols + kPlainBN - 1) / kPlainBN, degrees);
-    adapter_pass_plain_kernel<double><<<grid, kPlainThreads, 0, stream>>>(p);
-    launched("adapter_pass_plain_kernel");
 }
 
 int sm_count() {
@@ -606,19 +411,13 @@ void launch_ts(const TsPass& t, long long tiles, cudaStream_t stream) {
     launched("adapter_pass_f32_kernel");
 }
 void launch_pass(const smx_adapter_linear& c, bool transposed, const Pass<float>& p, int degrees, cudaStream_t stream) {
-    Matrices m[kMaxDegrees];
-    tile_layout<float>(c, m);
     TsPass t{};
     long long tiles = 0;
     for (int q = 0; q < degrees; ++q) {
         const PassDegree<float>& d = p.degree[q];
         TsDegree& e = t.degree[q];
         e.comps = d.comps; e.Kd = d.Kd; e.Nc = d.Nc; e.in_off = d.in_off; e.out_off = d.out_off; e.hidden = d.hidden;
-        e.W = d.W ? static_cast<const float*>(m[q].shared[transposed]) : nullptr;
-        e.first = static_cast<const float*>(transposed ? m[q].up[1] : m[q].down[0]);
-        e.first_group = static_cast<long long>(transposed ? m[q].up_group[1] : m[q].down_group[0]);
-        e.second = static_cast<const float*>(transposed ? m[q].down[1] : m[q].up[0]);
-        e.second_group = static_cast<long long>(transposed ? m[q].down_group[1] : m[q].up_group[0]);
+        e.W = d.W; e.first = d.first; e.first_group = d.first_group; e.second = d.second; e.second_group = d.second_group;
         const long long rows = (p.sorted ? p.pairs : p.num_rows) * d.comps;
         tiles += (p.sorted ? rows / kTsRows + p.groups + 1 : (rows + kTsRows - 1) / kTsRows) * (p.out ? ts_blocks(d.Nc) : 1);
     }
@@ -640,11 +439,62 @@ void launch_pass(const smx_adapter_linear& c, bool transposed, const Pass<float>
     else launch_ts<4>(t, tiles, stream);
 }
 
-void launch_grads(const GradPass<double>& gp, int problems, long long chunks, int cols, cudaStream_t stream) {
-    adapter_grad_kernel<double><<<dim3(static_cast<unsigned>(chunks), (cols + kGradCols - 1) / kGradCols, problems), kGradThreads, 0, stream>>>(gp);
-    launched("adapter_grad_kernel");
+// float64: tiles of 64 x 64, or of 16 x 32 while those leave SMs idle.
+template <int BM, int BN, int WM, int WN, int NR, int ST>
+void launch_dp(const DpPass& t, long long tiles, cudaStream_t stream) {
+    using L = DpLayout<BM, BN, NR, ST>;
+    if (tiles > INT_MAX) throw ArgError("smx_adapter: too many rows");
+    const auto kernel = adapter_pass_f64_kernel<BM, BN, WM, WN, NR, ST>;
+    if (L::smem > 40 * 1024) SMX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::smem));
+    kernel<<<static_cast<unsigned>(tiles), kDpThreads, L::smem, stream>>>(t);
+    launched("adapter_pass_f64_kernel");
 }
-void launch_grads(const GradPass<float>& gp, int problems, long long, int, cudaStream_t stream) {
+void launch_pass(const smx_adapter_linear&, bool, const Pass<double>& p, int degrees, cudaStream_t stream) {
+    DpPass t{};
+    for (int q = 0; q < degrees; ++q) {
+        const PassDegree<double>& d = p.degree[q];
+        DpDegree& e = t.degree[q];
+        e.comps = d.comps; e.Kd = d.Kd; e.Nc = d.Nc; e.ldw = even(d.Nc); e.in_off = d.in_off; e.out_off = d.out_off; e.hidden = d.hidden;
+        if (!p.out) e.ldw = 0;
+        e.W = d.W; e.first = d.first; e.first_group = d.first_group; e.second = d.second; e.second_group = d.second_group;
+    }
+    t.degrees = degrees; t.rank = p.rank; t.groups = p.groups; t.slots = p.slots; t.num_rows = p.num_rows; t.pairs = p.pairs;
+    t.order = p.order; t.offsets = p.offsets; t.weights = p.weights; t.in = p.in; t.in_stride = p.in_stride; t.out = p.out; t.out_stride = p.out_stride;
+    t.sorted = p.sorted; t.out_sorted = p.out_sorted; t.tail = p.tail;
+    auto tiles = [&](int BM, int BN) {
+        long long n = 0;
+        for (int q = 0; q < degrees; ++q) {
+            const long long rows = (p.sorted ? p.pairs : p.num_rows) * p.degree[q].comps;
+            n += (p.sorted ? rows / BM + p.groups + 1 : (rows + BM - 1) / BM) * (p.out ? (p.degree[q].Nc + BN - 1) / BN : 1);
+        }
+        return n;
+    };
+    auto by_rank = [&](auto nr) {
+        constexpr int NR = decltype(nr)::value;
+        if (tiles(64, 64) <= 2LL * sm_count()) launch_dp<16, 32, 1, 4, NR, 4>(t, tiles(16, 32), stream);
+        else launch_dp<64, 64, 2, 2, NR, 3>(t, tiles(64, 64), stream);
+    };
+    if (p.rank <= 8) by_rank(std::integral_constant<int, 1>{});
+    else if (p.rank <= 16) by_rank(std::integral_constant<int, 2>{});
+    else if (p.rank <= 32) by_rank(std::integral_constant<int, 4>{});
+    else by_rank(std::integral_constant<int, 8>{});
+}
+
+void launch_grads(const GradPass<double>& gp, int problems, cudaStream_t stream) {
+    DpGrad t{};
+    long long ctas = 0;
+    for (int q = 0; q < problems; ++q) {
+        t.problem[q] = gp.problem[q];
+        ctas += (gp.pairs * gp.problem[q].comps / kGradChunk + gp.groups) * ((gp.problem[q].Kd + kDpGradK - 1) / kDpGradK);
+    }
+    t.problems = problems; t.rank = gp.rank; t.groups = gp.groups; t.slots = gp.slots; t.pairs = gp.pairs;
+    t.order = gp.order; t.offsets = gp.offsets; t.weights = gp.weights;
+    if (ctas > INT_MAX) throw ArgError("smx_adapter: too many rows");
+    const auto kernel = gp.rank <= 8 ? adapter_grad_f64_kernel<1> : gp.rank <= 16 ? adapter_grad_f64_kernel<2> : gp.rank <= 32 ? adapter_grad_f64_kernel<4> : adapter_grad_f64_kernel<8>;
+    kernel<<<static_cast<unsigned>(ctas), kDpThreads, 0, stream>>>(t);
+    launched("adapter_grad_f64_kernel");
+}
+void launch_grads(const GradPass<float>& gp, int problems, cudaStream_t stream) {
     TsGrad t{};
     long long ctas = 0;
     for (int q = 0; q < problems; ++q) {
@@ -735,7 +585,7 @@ void backward(const smx_adapter_linear& c) {
     gp.rank = c.rank; gp.groups = c.num_groups; gp.slots = c.slots; gp.pairs = static_cast<long long>(pairs);
     gp.order = c.order; gp.offsets = c.offsets; gp.weights = static_cast<const T*>(c.weights);
     WeightGrad<T> wg{};
-    long long in_off = 0, out_off = 0, hid_off = 0, chunks = 0;
+    long long in_off = 0, out_off = 0, hid_off = 0;
     int cols = 0;
     for (int q = 0; q < c.num_degrees; ++q) {
         const smx_adapter_degree& g = c.degrees[q];
@@ -750,12 +600,11 @@ void backward(const smx_adapter_linear& c) {
         u.grad = static_cast<T*>(g.grad_up); u.g_group = R * O; u.g_k = 1; u.g_r = O;
         wg.t[q] = hidden + hid_off; wg.h[q] = b.back_hidden + hid_off; wg.comps[q] = g.components;
         in_off += g.components * I; out_off += g.components * O; hid_off += static_cast<long long>(pairs) * g.components * R;
-        chunks = std::max(chunks, grad_chunks(c, g.components));
         cols = std::max(cols, std::max(g.in_channels, g.out_channels));
     }
     if (adapters) {
         if (pairs > 0) {
-            launch_grads(gp, 2 * c.num_degrees, chunks, cols, stream);
+            launch_grads(gp, 2 * c.num_degrees, stream);
         }
         const int slabs = static_cast<int>(std::min<long long>(64, (static_cast<long long>(cols) * c.rank + 255) / 256));
         adapter_grad_sum_kernel<T><<<dim3(c.num_groups, slabs, 2 * c.num_degrees), 256, 0, stream>>>(gp);
