@@ -386,6 +386,21 @@ long smx_adapter_workspace_bytes(const smx_adapter_linear* call, int backward);
 int smx_adapter_forward(const smx_adapter_linear* call, char* errbuf, int errbuf_len);
 int smx_adapter_backward(const smx_adapter_linear* call, char* errbuf, int errbuf_len);
 
+/* Adapters of an evaluator's own linears: smx_compute, smx_evaluate and the stages then evaluate every node with the variant of the model that
+ * it is assigned, in one call for all variants. `linear` is "H1" (compute_H1: M0 to H1), "A1" (compute_A1: Phi1 to A1) or, in three-block
+ * models, "Am" or "Hm" (there beside the weights of Mm). smx_set_adapters gives a linear `num_adapters` adapters of rank `rank`, host arrays of
+ * doubles, degree after degree: down [num_adapters][in][rank], up [num_adapters][rank][K], with in = K for "H1" / "Hm" and K times the
+ * number of paths of the degree for "A1" / "Am", in the file's order of paths; the counts are checked. All linears that have adapters have the same number of them; 0
+ * takes a linear's away. smx_assign_adapters names the adapters of nodes 0 .. num_nodes - 1 (host arrays ids[num_nodes * slots], weights of the
+ * same size or NULL for ones), as smx_route_plan reads them: an id outside the adapters is an empty slot, a node without any runs the model as it is. The
+ * assignment stays until the next one (0 nodes: none, the model for all) or until the number of adapters changes; an evaluation with more nodes
+ * than assigned is refused, one with fewer uses the first. smx_adapter_gradients returns, after a whole evaluation, the gradients of the
+ * total energy by a linear's adapters (in the layout of smx_set_adapters) and by the weights [active nodes * slots]; any may be NULL. */
+int smx_set_adapters(smx_handle h, const char* linear, int num_adapters, int rank, const double* down, long down_count,
+                     const double* up, long up_count);
+int smx_assign_adapters(smx_handle h, int num_nodes, int slots, const int* ids, const double* weights);
+int smx_adapter_gradients(smx_handle h, const char* linear, double* grad_down, double* grad_up, double* grad_weights);
+
 #ifdef __cplusplus
 }
 #endif

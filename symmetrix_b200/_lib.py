@@ -24,7 +24,7 @@ EXPORTED_SYMBOLS = [
     "smx_energy_virial_noalloc", "smx_sync", "smx_set_stream", "smx_restrict_nodes", "smx_set_active_nodes", "smx_resize_rows", "smx_device_ptr",
     "smx_halo_pack", "smx_halo_unpack", "smx_halo_unpack_add", "smx_halo_cache_lists", "smx_atom_forces", "smx_active_counts", "smx_debug_expire_waits",
     "smx_comm_unique_id", "smx_comm_init", "smx_comm_destroy", "smx_halo_exchange", "smx_allreduce_sum", "smx_model_digest",
-    "smx_route_plan_bytes", "smx_route_plan", "smx_route_dispatch", "smx_route_combine", "smx_route_combine_backward",
+    "smx_set_adapters", "smx_assign_adapters", "smx_adapter_gradients", "smx_route_plan_bytes", "smx_route_plan", "smx_route_dispatch", "smx_route_combine", "smx_route_combine_backward",
     "smx_adapter_tiles_bytes", "smx_adapter_prepare", "smx_adapter_hidden_elements", "smx_adapter_workspace_bytes", "smx_adapter_forward", "smx_adapter_backward",
 ]
 ROUTE_MAX_GROUPS, ROUTE_MAX_SLOTS = 1024, 64
@@ -120,6 +120,9 @@ def load():
     lib.smx_allreduce_sum.argtypes = [vp, dp, ctypes.c_int]
     lib.smx_model_digest.argtypes = [ctypes.c_char_p, ctypes.c_int, ctypes.POINTER(ctypes.c_ulonglong), ctypes.POINTER(ctypes.c_int)]
     lib.smx_energy_virial_noalloc.argtypes = [dp, ctypes.c_int, dp, dp, ctypes.c_long, dp, vp, ctypes.c_char_p, ctypes.c_int]
+    lib.smx_set_adapters.argtypes = [vp, ctypes.c_char_p, ctypes.c_int, ctypes.c_int, dp, ctypes.c_long, dp, ctypes.c_long]
+    lib.smx_assign_adapters.argtypes = [vp, ctypes.c_int, ctypes.c_int, ip, dp]
+    lib.smx_adapter_gradients.argtypes = [vp, ctypes.c_char_p, dp, dp, dp]
     cl, ci, err = ctypes.c_long, ctypes.c_int, [ctypes.c_char_p, ctypes.c_int]
     lib.smx_route_plan_bytes.argtypes = [cl, ci, ci]
     lib.smx_route_plan_bytes.restype = cl

@@ -178,6 +178,7 @@ namespace {
 void launched(const char* what) {
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) throw CudaError(std::string(what) + ": " + cudaGetErrorString(e));
+    ++operator_launches;
 }
 
 struct Widths { long in = 0, out = 0; long long comps = 0; };

@@ -349,6 +349,21 @@ int smx_get_edges(smx_handle h, int* num_neigh, int* neigh_indices, int* neigh_t
     return guarded(h, [&](smx::EvaluatorBase& e) { e.get_edges(num_neigh, neigh_indices, neigh_types, shifts, xyz, r, mem_space); });
 }
 
+int smx_set_adapters(smx_handle h, const char* linear, int num_adapters, int rank, const double* down, long down_count, const double* up, long up_count) {
+    return guarded(h, [&](smx::EvaluatorBase& e) {
+        if (!linear) throw smx::ArgError("smx_set_adapters: null name");
+        e.set_adapters(linear, num_adapters, rank, down, down_count, up, up_count);
+    });
+}
+int smx_assign_adapters(smx_handle h, int num_nodes, int slots, const int* ids, const double* weights) {
+    return guarded(h, [&](smx::EvaluatorBase& e) { e.assign_adapters(num_nodes, slots, ids, weights); });
+}
+int smx_adapter_gradients(smx_handle h, const char* linear, double* grad_down, double* grad_up, double* grad_weights) {
+    return guarded(h, [&](smx::EvaluatorBase& e) {
+        if (!linear) throw smx::ArgError("smx_adapter_gradients: null name");
+        e.adapter_gradients(linear, grad_down, grad_up, grad_weights);
+    });
+}
 long smx_route_plan_bytes(long num_rows, int slots, int num_groups) {
     return size_or_refusal([&] { return smx::route_plan_bytes(num_rows, slots, num_groups); });
 }

@@ -20,6 +20,7 @@
 #include <nvtx3/nvToolsExt.h>
 
 #include "../../include/symmetrix_b200.h"
+#include "adapters.hpp"
 #include "common.cuh"
 #include "kernels.cuh"
 #include "gemm_tcgen05.cuh"
@@ -30,6 +31,7 @@
 #include "edge_plan.hpp"
 #include "neighbors.cuh"
 #include "nccl_transport.hpp"
+#include "routing.hpp"
 
 namespace smx {
 
@@ -969,11 +971,240 @@ public:
         run_poly(1, true);
     }
 
+    // ---- low-rank adapters beside the channel-mixing linears (no counterpart in the reference): every node's own, or a weighted mixture of
+    // several, added to the linear's weights (csrc/adapters.cu). A linear without them, or an evaluator without an assignment, runs the model.
+    struct AdapterSet {
+        int rank = 0;
+        std::vector<std::unique_ptr<DevBuf<T>>> down, up;         // per degree, only until they are laid out
+        DevBuf<unsigned char> tiles;
+        DevBuf<T> hidden;                                         // in . down of the last forward pass, for the gradients
+        int hidden_nodes = -1;
+    };
+    std::map<std::string, AdapterSet> adapters;
+    int num_adapters = 0;                                         // of every linear that has some
+    DevBuf<int> adapter_ids, adapter_plan;                        // as assigned; order, position and offsets of the first `adapter_planned` nodes
+    DevBuf<T> adapter_weights;
+    DevBuf<unsigned char> adapter_workspace;
+    int adapter_nodes = 0, adapter_slots = 0, adapter_planned = -1;
+    bool adapter_weighted = false;
+
+    // The linear `name` as a call: shapes and arrays. `rows` of x and y are the nodes'.
+    smx_adapter_linear adapter_linear(const std::string& name) {
+        smx_adapter_linear c{};
+        const int K = model.K;
+        const bool tensor = name == "A1" || name == "Am", deep_name = name == "Am" || name == "Hm";
+        if (!tensor && name != "H1" && name != "Hm") throw ArgError("adapters: the linears are \"H1\", \"A1\" and, in three-block models, \"Am\", \"Hm\"");
+        if (deep_name) require_deep("adapters of the middle block");
+        c.precision = sizeof(T) == 4 ? SMX_FP32 : SMX_FP64;
+        c.num_degrees = tensor ? kLmaxSH + 1 : model.L_max + 1;
+        const T* w = name == "H1" ? H1_w.p : name == "Hm" ? Hm_w.p : name == "Am" ? Am_w.p : A1_w.p;
+        const auto& off = name == "Am" ? model.Am_w_off : model.A1_w_off;
+        for (int l = 0; l < c.num_degrees; ++l) {
+            smx_adapter_degree& d = c.degrees[l];
+            d.components = 2 * l + 1;
+            d.in_channels = tensor ? model.tp.n_e[l] * K : K;
+            d.out_channels = K;
+            d.shared = tensor ? w + off[l] : w + static_cast<size_t>(l) * K * K;
+        }
+        c.num_groups = std::max(1, num_adapters);
+        c.slots = std::max(1, adapter_slots);
+        c.x_stride = c.grad_x_stride = static_cast<long>(tensor ? model.tp.Q : model.num_LM) * K;
+        c.y_stride = c.grad_y_stride = static_cast<long>(tensor ? kNumLm : model.num_LM) * K;
+        c.stream = stream;
+        auto it = adapters.find(name);
+        if (it != adapters.end()) { c.rank = it->second.rank; c.tiles = it->second.tiles.p; }
+        return c;
+    }
+    // Down matrices of "A1" / "Am" have a block of K rows for each path of a degree: from the file's order of paths to the kernels', or back.
+    std::vector<double> adapter_paths(const std::string& name, const double* down, int count, int rank, bool to_kernels) const {
+        std::vector<double> out;
+        const int K = model.K;
+        const TPTable& tp = model.tp;
+        if (name == "H1" || name == "Hm") {
+            out.assign(down, down + static_cast<size_t>(model.L_max + 1) * count * K * rank);
+            return out;
+        }
+        std::vector<int> kernel_block[kLmaxSH + 1];
+        for (int pf = 0; pf < tp.P; ++pf) {
+            const int c = model.path_file_to_canon[pf];
+            kernel_block[tp.l[c]].push_back(tp.e[c]);
+        }
+        const size_t block = static_cast<size_t>(K) * rank;
+        size_t at = 0;
+        for (int l = 0; l <= kLmaxSH; ++l) {
+            out.resize(at + static_cast<size_t>(count) * tp.n_e[l] * block);
+            for (int g = 0; g < count; ++g, at += tp.n_e[l] * block)
+                for (int e = 0; e < tp.n_e[l]; ++e) {
+                    const size_t file = at + e * block, kern = at + kernel_block[l][e] * block;
+                    std::copy(down + (to_kernels ? file : kern), down + (to_kernels ? file : kern) + block, out.begin() + (to_kernels ? kern : file));
+                }
+        }
+        return out;
+    }
+    // Whether the linear has adapters and nodes that use them; then the plan of the active nodes is up to date.
+    bool adapters_on(const char* name) {
+        if (adapter_nodes == 0 || N == 0 || adapters.find(name) == adapters.end()) return false;
+        if (adapter_nodes < N) throw ArgError("adapters are assigned to " + std::to_string(adapter_nodes) + " nodes, the evaluation has " + std::to_string(N));
+        if (adapter_planned != N) {
+            const size_t pairs = static_cast<size_t>(N) * adapter_slots;
+            adapter_plan.resize(2 * pairs + num_adapters + 1, stream);
+            adapter_workspace.resize(route_plan_bytes(N, adapter_slots, num_adapters), stream);
+            const long before = operator_launches;
+            route_plan(adapter_ids.p, N, adapter_slots, num_adapters, adapter_plan.p, adapter_plan.p + pairs, adapter_plan.p + 2 * pairs,
+                       adapter_workspace.p, adapter_workspace.n, stream);
+            launches += operator_launches - before;
+            adapter_planned = N;
+        }
+        return true;
+    }
+    smx_adapter_linear adapter_call(const char* name) {
+        smx_adapter_linear c = adapter_linear(name);
+        const size_t pairs = static_cast<size_t>(N) * adapter_slots;
+        c.num_rows = N;
+        c.order = adapter_plan.p; c.position = adapter_plan.p + pairs; c.offsets = adapter_plan.p + 2 * pairs;
+        c.weights = adapter_weighted ? adapter_weights.p : nullptr;
+        return c;
+    }
+    void adapter_run(smx_adapter_linear& c, bool back) {
+        adapter_workspace.resize(adapter_workspace_bytes(c, back), stream);
+        c.workspace = adapter_workspace.p;
+        c.workspace_bytes = static_cast<long>(adapter_workspace.n);
+        const long before = operator_launches;
+        if (back) adapter_backward(c);
+        else adapter_forward(c);
+        launches += operator_launches - before;
+    }
+    void adapter_compute(const char* name, const T* x, T* y) {
+        AdapterSet& a = adapters.at(name);
+        smx_adapter_linear c = adapter_call(name);
+        a.hidden.resize(adapter_hidden_elements(c), stream);
+        a.hidden_nodes = N;
+        c.x = x; c.y = y; c.hidden = a.hidden.p;
+        adapter_run(c, false);
+    }
+    void adapter_reverse(const char* name, const T* grad_y, T* grad_x) {
+        smx_adapter_linear c = adapter_call(name);
+        c.grad_y = grad_y; c.grad_x = grad_x;
+        adapter_run(c, true);
+    }
+
+    void set_adapters(const std::string& name, int count, int rank, const double* down, long down_count, const double* up, long up_count) override {
+        SMX_CUDA(cudaSetDevice(device));
+        smx_adapter_linear c = adapter_linear(name);
+        if (count < 0) throw ArgError("smx_set_adapters: negative number of adapters");
+        bool others = false;
+        for (const auto& a : adapters) others = others || a.first != name;
+        if (count == 0) {
+            adapters.erase(name);
+            if (!others) drop_assignment(0);
+            return;
+        }
+        if (others && count != num_adapters) throw ArgError("smx_set_adapters: the linears of an evaluator have the same number of adapters, here " + std::to_string(num_adapters));
+        if (!down || !up) throw ArgError("smx_set_adapters: null pointer");
+        c.num_groups = count;
+        c.rank = rank;
+        const size_t bytes = adapter_tiles_bytes(c);              // refuses bad ranks and counts
+        size_t want_down = 0, want_up = 0;
+        for (int l = 0; l < c.num_degrees; ++l) {
+            want_down += static_cast<size_t>(count) * c.degrees[l].in_channels * rank;
+            want_up += static_cast<size_t>(count) * c.degrees[l].out_channels * rank;
+        }
+        if (down_count != static_cast<long>(want_down) || up_count != static_cast<long>(want_up))
+            throw ArgError("smx_set_adapters: " + name + " takes " + std::to_string(want_down) + " and " + std::to_string(want_up) + " values");
+        if (count != num_adapters) drop_assignment(count);
+        AdapterSet& a = adapters[name];
+        a.rank = rank;
+        a.hidden_nodes = -1;
+        a.tiles.resize(bytes, stream);
+        c.tiles = a.tiles.p;
+        DevBuf<T> d_down, d_up;
+        d_down.upload(cast_vec<T>(adapter_paths(name, down, count, rank, true)), stream);
+        d_up.upload(cast_vec<T>(std::vector<double>(up, up + want_up)), stream);
+        const T *at_down = d_down.p, *at_up = d_up.p;
+        for (int l = 0; l < c.num_degrees; ++l) {
+            c.degrees[l].down = at_down; c.degrees[l].up = at_up;
+            at_down += static_cast<size_t>(count) * c.degrees[l].in_channels * rank;
+            at_up += static_cast<size_t>(count) * c.degrees[l].out_channels * rank;
+        }
+        const long before = operator_launches;
+        adapter_prepare(c, SMX_ADAPTER_SHARED | SMX_ADAPTER_MATRICES);
+        launches += operator_launches - before;
+        SMX_CUDA(cudaStreamSynchronize(stream));                  // the uploads are temporary
+    }
+    void drop_assignment(int count) {
+        num_adapters = count;
+        adapter_nodes = 0; adapter_slots = 0; adapter_planned = -1;
+    }
+    void assign_adapters(int num_nodes, int slots, const int* ids, const double* weights) override {
+        SMX_CUDA(cudaSetDevice(device));
+        if (num_nodes < 0) throw ArgError("smx_assign_adapters: negative number of nodes");
+        if (num_nodes == 0) { adapter_nodes = 0; adapter_planned = -1; return; }
+        if (num_adapters == 0) throw ArgError("smx_assign_adapters: no adapters have been set");
+        if (!ids) throw ArgError("smx_assign_adapters: null pointer");
+        route_plan_bytes(num_nodes, slots, num_adapters);         // refuses bad sizes
+        const size_t pairs = static_cast<size_t>(num_nodes) * slots;
+        adapter_ids.upload(std::vector<int>(ids, ids + pairs), stream);
+        if (weights) adapter_weights.upload(cast_vec<T>(std::vector<double>(weights, weights + pairs)), stream);
+        SMX_CUDA(cudaStreamSynchronize(stream));
+        adapter_weighted = weights != nullptr;
+        adapter_nodes = num_nodes; adapter_slots = slots; adapter_planned = -1;
+        for (auto& a : adapters) a.second.hidden_nodes = -1;
+    }
+    void adapter_gradients(const std::string& name, double* down, double* up, double* weights) override {
+        require_edges();
+        SMX_CUDA(cudaSetDevice(device));
+        if (!adapters_on(name.c_str())) throw ArgError("smx_adapter_gradients: " + name + " has no adapters, or no node uses any");
+        AdapterSet& a = adapters.at(name);
+        smx_adapter_linear c = adapter_call(name.c_str());
+        const DevBuf<T>& x = name == "H1" ? M0 : name == "Hm" ? Mm : name == "Am" ? Phim : Phi1;
+        const DevBuf<T>& gy = name == "H1" ? H1_adj : name == "Hm" ? Hm_adj : name == "Am" ? Am_adj : A1_adj;
+        if (a.hidden_nodes != N || x.n != static_cast<size_t>(N) * c.x_stride || gy.n < static_cast<size_t>(N) * c.grad_y_stride)
+            throw ArgError("smx_adapter_gradients: no evaluation of the current nodes with these adapters has been made");
+        c.x = x.p; c.grad_y = gy.p; c.hidden = a.hidden.p;
+        size_t downs = 0, ups = 0;
+        for (int l = 0; l < c.num_degrees; ++l) {
+            downs += static_cast<size_t>(num_adapters) * c.degrees[l].in_channels * a.rank;
+            ups += static_cast<size_t>(num_adapters) * c.degrees[l].out_channels * a.rank;
+        }
+        DevBuf<T> d_down, d_up, d_w;
+        if (down || up) {
+            d_down.resize(downs, stream);
+            d_up.resize(ups, stream);
+            T *at_down = d_down.p, *at_up = d_up.p;
+            for (int l = 0; l < c.num_degrees; ++l) {
+                c.degrees[l].grad_down = at_down; c.degrees[l].grad_up = at_up;
+                at_down += static_cast<size_t>(num_adapters) * c.degrees[l].in_channels * a.rank;
+                at_up += static_cast<size_t>(num_adapters) * c.degrees[l].out_channels * a.rank;
+            }
+        }
+        if (weights) {
+            d_w.resize(static_cast<size_t>(N) * adapter_slots, stream);
+            c.grad_weights = d_w.p;
+        }
+        adapter_run(c, true);
+        auto bring = [&](const DevBuf<T>& b, double* to) {
+            if (!to) return;
+            std::vector<T> h(b.n);
+            SMX_CUDA(cudaMemcpyAsync(h.data(), b.p, b.n * sizeof(T), cudaMemcpyDeviceToHost, stream));
+            SMX_CUDA(cudaStreamSynchronize(stream));
+            for (size_t i = 0; i < h.size(); ++i) to[i] = static_cast<double>(h[i]);
+        };
+        bring(d_down, down);
+        if (down) {
+            const std::vector<double> ordered = adapter_paths(name, down, num_adapters, a.rank, false);
+            std::copy(ordered.begin(), ordered.end(), down);
+        }
+        bring(d_up, up);
+        bring(d_w, weights);
+        check_kernel_status();
+    }
+
     void compute_H1() {   // MACE::compute_H1, mace.cpp:397-423
         const int K = model.K, nLM = model.num_LM;
         if (M0.n != static_cast<size_t>(N) * nLM * K) throw ArgError("compute_H1: M0 has not been computed");
         H1.resize(static_cast<size_t>(N) * nLM * K, stream);
         h1_rows = N;
+        if (adapters_on("H1")) { adapter_compute("H1", M0.p, H1.p); return; }
         std::vector<GemmProblem<T>> list;
         for (int l = 0; l <= model.L_max; ++l)
             list.push_back(problem(M0.p, H1.p, H1_w.p + static_cast<size_t>(l) * K * K, false, 0, 2 * l + 1, 1LL * nLM * K,
@@ -984,6 +1215,7 @@ public:
         const int K = model.K, nLM = model.num_LM;
         if (H1_adj.n < static_cast<size_t>(N) * nLM * K) throw ArgError("reverse_H1: H1_adj has not been computed");
         M0_adj.resize(static_cast<size_t>(N) * nLM * K, stream);
+        if (adapters_on("H1")) { adapter_reverse("H1", H1_adj.p, M0_adj.p); return; }
         std::vector<GemmProblem<T>> list;
         for (int l = 0; l <= model.L_max; ++l)
             list.push_back(problem(H1_adj.p, M0_adj.p, H1_w.p + static_cast<size_t>(l) * K * K, false, 0, 2 * l + 1, 1LL * nLM * K,
@@ -1295,6 +1527,8 @@ public:
         const auto& off = which == 2 ? model.Am_w_off : model.A1_w_off;
         if (phi.n != static_cast<size_t>(N) * tp.Q * K) throw ArgError(std::string(what) + ": the tensor product has not been computed");
         out.resize(static_cast<size_t>(N) * kNumLm * K, stream);
+        const char* name = which == 2 ? "Am" : "A1";
+        if (adapters_on(name)) { adapter_compute(name, phi.p, out.p); return; }
         std::vector<GemmProblem<T>> list;
         for (int l = 0; l <= kLmaxSH; ++l)
             list.push_back(problem(phi.p, out.p, w + off[l], false, 0, 2 * l + 1, 1LL * tp.Q * K, 1LL * tp.lme_off[l] * K,
@@ -1310,6 +1544,8 @@ public:
         const auto& off = which == 2 ? model.Am_w_off : model.A1_w_off;
         if (adj.n != static_cast<size_t>(N) * kNumLm * K) throw ArgError(std::string(what) + ": the adjoint of A has not been computed");
         dphi.resize(static_cast<size_t>(N) * tp.Q * K, stream);
+        const char* name = which == 2 ? "Am" : "A1";
+        if (adapters_on(name)) { adapter_reverse(name, adj.p, dphi.p); return; }
         std::vector<GemmProblem<T>> list;
         int max_cols = K;
         for (int l = 0; l <= kLmaxSH; ++l) {
@@ -1353,6 +1589,11 @@ public:
                 merged.back().accumulate = 0;
                 add_product(merged.back(), mix[l]);
             }
+        if (adapters_on("Hm")) {
+            adapter_compute("Hm", Mm.p, Hm.p);
+            run_gemms(residual, static_cast<long long>(2 * model.L_max + 1) * N, K, static_cast<long long>(model.num_LM) * N);
+            return;
+        }
         run_gemms_pair(mix, residual, merged, static_cast<long long>(2 * model.L_max + 1) * N, K, static_cast<long long>(model.num_LM) * N);
     }
     void reverse_Hm() {
@@ -1362,7 +1603,9 @@ public:
         if (H1_adj.n < static_cast<size_t>(N) * nLM * K) throw ArgError("reverse_Hm: H1_adj has not been computed");
         Mm_adj.resize(static_cast<size_t>(N) * nLM * K, stream);
         std::vector<GemmProblem<T>> list;
-        for (int l = 0; l <= model.L_max; ++l)
+        const bool adapted = adapters_on("Hm");
+        if (adapted) adapter_reverse("Hm", Hm_adj.p, Mm_adj.p);
+        for (int l = 0; l <= model.L_max && !adapted; ++l)
             list.push_back(problem(Hm_adj.p, Mm_adj.p, Hm_w.p + static_cast<size_t>(l) * K * K, false, 0, 2 * l + 1, 1LL * nLM * K,
                                    1LL * l * l * K, K, 1LL * nLM * K, 1LL * l * l * K, K, K, K, K, true, false));
         for (int a = 0; a < model.num_elements; ++a)

@@ -53,6 +53,9 @@ public:
                                  double r_cut, int mem_space) = 0;
     virtual long evaluate(int natoms, const double* pos, const int* types, const double* cell, const int* pbc, double r_cut, double* forces,
                           double* energies, double* virial, double* energy) = 0;
+    virtual void set_adapters(const std::string& name, int count, int rank, const double* down, long down_count, const double* up, long up_count) = 0;
+    virtual void assign_adapters(int num_nodes, int slots, const int* ids, const double* weights) = 0;
+    virtual void adapter_gradients(const std::string& name, double* down, double* up, double* weights) = 0;
     virtual void get_edges(int* num_neigh, int* neigh_indices, int* neigh_types, int* shifts, double* xyz, double* r, int mem_space) = 0;
 };
 

@@ -337,9 +337,12 @@ RowGrid row_grid(long num_rows, long units) {
 void launched(const char* what) {
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) throw CudaError(std::string(what) + ": " + cudaGetErrorString(e));
+    ++operator_launches;
 }
 
 }  // namespace
+
+thread_local long operator_launches = 0;
 
 size_t route_plan_bytes(long num_rows, int slots, int num_groups) {
     check_sizes("smx_route_plan", num_rows, slots, num_groups);

@@ -9,6 +9,9 @@
 
 namespace smx {
 
+// Kernels that this thread launched here and in csrc/adapters.cu.
+extern thread_local long operator_launches;
+
 size_t route_plan_bytes(long num_rows, int slots, int num_groups);
 void route_plan(const int* ids, long num_rows, int slots, int num_groups, int* order, int* position, int* offsets, void* workspace,
                 size_t workspace_bytes, cudaStream_t stream);

@@ -303,6 +303,68 @@ class MACE:
     def compute_current(self) -> None:
         self._check(self._lib.smx_compute_current(self._h))
 
+    # ------------------------------------------------------------------ adapters (fine-tuned variants side by side)
+    def _adapter_shapes(self, linear: str):
+        """(input channels, output channels) of every degree of a linear that can have adapters."""
+        if linear in ("H1", "Hm"):
+            return [(self.num_channels, self.num_channels)] * (self.L_max + 1)
+        if linear in ("A1", "Am"):
+            from .modelgen.generate import tp_paths
+            l_out = [p[0] for p in tp_paths(self.l_max, self.L_max)]
+            return [(l_out.count(l) * self.num_channels, self.num_channels) for l in range(self.l_max + 1)]
+        raise ValueError("the linears with adapters are 'H1', 'A1' and, in three-block models, 'Am' and 'Hm'")
+
+    def set_adapters(self, linear: str, down, up) -> None:
+        """Low-rank adapters of a linear (``smx_set_adapters``): per degree ``down[l]`` of shape ``[adapters, in_l, rank]`` and ``up[l]`` of shape
+        ``[adapters, rank, K]``; ``in_l`` is K for "H1" and "Hm", K times the degree's number of paths for "A1" and "Am". Empty lists take
+        them away."""
+        if len(down) == 0 and len(up) == 0:
+            self._check(self._lib.smx_set_adapters(self._h, linear.encode(), 0, 0, None, 0, None, 0))
+            return
+        shapes = self._adapter_shapes(linear)
+        down, up = [np.ascontiguousarray(a, dtype=np.float64) for a in down], [np.ascontiguousarray(b, dtype=np.float64) for b in up]
+        if len(down) != len(shapes) or len(up) != len(shapes) or any(a.ndim != 3 for a in (*down, *up)):
+            raise ValueError(f"{linear} needs a three-dimensional array for each of its {len(shapes)} degrees")
+        count, rank = down[0].shape[0], down[0].shape[2]
+        for (i, o), a, b in zip(shapes, down, up):
+            if a.shape != (count, i, rank) or b.shape != (count, rank, o):
+                raise ValueError(f"{linear}: expected shapes {(count, i, rank)} and {(count, rank, o)}, got {a.shape} and {b.shape}")
+        d, u = np.concatenate([a.ravel() for a in down]), np.concatenate([b.ravel() for b in up])
+        self._check(self._lib.smx_set_adapters(self._h, linear.encode(), count, rank, ctypes.c_void_p(d.ctypes.data), d.size,
+                                               ctypes.c_void_p(u.ctypes.data), u.size))
+        self._adapters = dict(getattr(self, "_adapters", {}), **{linear: (count, rank)})
+
+    def assign_adapters(self, ids, weights=None) -> None:
+        """Names every node's adapters (``smx_assign_adapters``): ``ids`` of shape ``[nodes]`` or ``[nodes, slots]`` (other values than
+        ``0 .. adapters - 1``: none), ``weights`` of the same shape. ``None`` assigns none: the model for all nodes."""
+        if ids is None:
+            self._check(self._lib.smx_assign_adapters(self._h, 0, 1, None, None))
+            return
+        i = np.ascontiguousarray(ids, dtype=np.int32)
+        if i.ndim not in (1, 2):
+            raise ValueError("ids must have shape [nodes] or [nodes, slots]")
+        w = None if weights is None else np.ascontiguousarray(weights, dtype=np.float64)
+        if w is not None and w.shape != i.shape:
+            raise ValueError("weights must have the shape of ids")
+        slots = 1 if i.ndim == 1 else i.shape[1]
+        self._check(self._lib.smx_assign_adapters(self._h, i.shape[0], slots, ctypes.c_void_p(i.ctypes.data), None if w is None else ctypes.c_void_p(w.ctypes.data)))
+        self._adapter_slots = slots
+
+    def adapter_gradients(self, linear: str):
+        """(gradients by ``down``, by ``up``, by the weights) of the total energy of the last whole evaluation (``smx_adapter_gradients``),
+        shaped like the arguments of :meth:`set_adapters` and ``[nodes, slots]``."""
+        shapes = self._adapter_shapes(linear)
+        count, rank = getattr(self, "_adapters", {}).get(linear, (0, 0))
+        d = [np.empty(count * i * rank) for i, _ in shapes]
+        u = [np.empty(count * o * rank) for _, o in shapes]
+        flat_d, flat_u = np.empty(sum(a.size for a in d)), np.empty(sum(b.size for b in u))
+        w = np.empty((self.active_counts()[0], getattr(self, "_adapter_slots", 1)))
+        self._check(self._lib.smx_adapter_gradients(self._h, linear.encode(), ctypes.c_void_p(flat_d.ctypes.data), ctypes.c_void_p(flat_u.ctypes.data),
+                                                    ctypes.c_void_p(w.ctypes.data)))
+        split = lambda flat, sizes: np.split(flat, np.cumsum(sizes)[:-1])  # noqa: E731
+        return ([a.reshape(count, i, rank) for a, (i, _) in zip(split(flat_d, [a.size for a in d]), shapes)],
+                [b.reshape(count, rank, o) for b, (_, o) in zip(split(flat_u, [b.size for b in u]), shapes)], w)
+
     # ------------------------------------------------------------------ helpers for decomposed drivers
     def sync(self) -> None:
         self._check(self._lib.smx_sync(self._h))
