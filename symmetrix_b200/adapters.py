@@ -11,6 +11,7 @@ Rows may have any stride between atoms; other strides than one inside a row are 
 from __future__ import annotations
 
 import ctypes
+import threading
 from collections import namedtuple
 
 from . import _lib
@@ -19,19 +20,29 @@ from .mace import SymmetrixError
 AdapterGradients = namedtuple("AdapterGradients", ["x", "down", "up", "weights"])
 
 
-def _call(status: int, err) -> None:
+class _Errors(threading.local):
+    def __init__(self):
+        self.buffer = ctypes.create_string_buffer(256)
+
+
+_errors = _Errors()
+
+
+def _call(fn, index: int, *args) -> None:
+    """A call of the library on device `index` (the message of a failure goes to a buffer of the thread)."""
+    import torch
+    if torch.cuda.current_device() == index:
+        status = fn(*args, _errors.buffer, 256)
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, _errors.buffer, 256)
     if status != _lib.SMX_OK:
-        raise SymmetrixError(status, err.value.decode())
+        raise SymmetrixError(status, _errors.buffer.value.decode())
 
 
 def _precision(dtype) -> int:
     import torch
-    return _lib.SMX_FP32 if dtype == torch.float32 else _lib.SMX_FP64
-
-
-def _stream(device) -> int:
-    import torch
-    return torch.cuda.current_stream(device).cuda_stream
+    return _lib.SMX_FP32 if dtype is torch.float32 else _lib.SMX_FP64
 
 
 def _ptr(t):
@@ -39,15 +50,15 @@ def _ptr(t):
 
 
 def _values(t, what: str, shape, dtype=None, device=None):
-    """`t` checked: a float32 / float64 CUDA tensor of the given shape (None: any extent), of unit stride inside the last dimension."""
+    """`t` checked: a float32 / float64 CUDA tensor of the given shape (None: any extent)."""
     import torch
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{what} must be a CUDA tensor")
-    if t.dtype not in (torch.float32, torch.float64) if dtype is None else t.dtype != dtype:
+    if t.dtype is not dtype if dtype is not None else t.dtype not in (torch.float32, torch.float64):
         raise ValueError(f"{what} has dtype {t.dtype}, expected {'float32 or float64' if dtype is None else dtype}")
     if device is not None and t.device != device:
         raise ValueError(f"{what} is on {t.device}, expected {device}")
-    if t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape)):
+    if t.shape != shape and (t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape))):
         raise ValueError(f"{what} has shape {tuple(t.shape)}, expected {tuple('any' if n is None else n for n in shape)}")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{what} requires gradients, but this operator is not recorded by autograd: use torch.no_grad() and its backward method")
@@ -57,9 +68,11 @@ def _values(t, what: str, shape, dtype=None, device=None):
 def _rows(t, what: str, shape, dtype=None, device=None):
     """(tensor, row stride) of a two-dimensional array of rows."""
     t = _values(t, what, shape, dtype, device)
-    if t.shape[1] > 1 and t.stride(1) != 1:
+    rows, step = t.stride()
+    if step != 1 and t.shape[1] > 1:
         t = t.contiguous()
-    return t, (t.stride(0) if t.shape[0] > 1 else t.shape[1])
+        rows = t.stride(0)
+    return t, (rows if t.shape[0] > 1 else t.shape[1])
 
 
 def _out(t, what: str, shape, dtype, device):
@@ -105,74 +118,85 @@ class RowRouting:
         if need < 0:
             raise ValueError(f"{self.num_rows} rows with {self.slots} slots and {self.num_groups} groups: the limits are {_lib.ROUTE_MAX_SLOTS} slots, "
                              f"{_lib.ROUTE_MAX_GROUPS} groups and 2^31 - 2^11 pairs, and one slot and group at least")
-        pairs = self.num_rows * self.slots
-        plan = torch.empty(2 * pairs + self.num_groups + 1, dtype=torch.int32, device=self.device)
-        self.order, self.position, self.offsets = plan[:pairs], plan[pairs:2 * pairs].view(self.num_rows, self.slots), plan[2 * pairs:]
-        self._plan = plan
-        self.update(ids)
+        self._need, self._index = need, self.device.index
+        self._pairs = self.num_rows * self.slots
+        self._plan = ids.new_empty(2 * self._pairs + self.num_groups + 1)
+        base = self._plan.data_ptr()
+        self._order, self._position, self._offsets = base, base + 4 * self._pairs, base + 8 * self._pairs
+        self._home = torch.cuda.current_stream(self._index).cuda_stream
+        self._make(ids)
+
+    @property
+    def order(self):
+        return self._plan[:self._pairs]
+
+    @property
+    def position(self):
+        return self._plan[self._pairs:2 * self._pairs].view(self.num_rows, self.slots)
+
+    @property
+    def offsets(self):
+        return self._plan[2 * self._pairs:]
 
     def update(self, ids) -> None:
         """The plan of other ids of the same shape, in the same tensors."""
         import torch
-        if not isinstance(ids, torch.Tensor) or ids.dtype != torch.int32 or ids.device != self.device or ids.numel() != self.num_rows * self.slots \
+        if not isinstance(ids, torch.Tensor) or ids.dtype != torch.int32 or ids.device != self.device or ids.numel() != self._pairs \
                 or ids.dim() not in (1, 2) or ids.shape[0] != self.num_rows:
             raise ValueError(f"ids must be an int32 tensor of {self.num_rows} rows with {self.slots} slots on {self.device}")
+        self._make(ids)
+
+    def _make(self, ids):
+        import torch
         ids = ids.contiguous()
-        need = self._library.smx_route_plan_bytes(self.num_rows, self.slots, self.num_groups)
-        with torch.cuda.device(self.device):
-            ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-            err = ctypes.create_string_buffer(256)
-            _call(self._library.smx_route_plan(_ptr(ids), self.num_rows, self.slots, self.num_groups, _ptr(self.order), _ptr(self.position),
-                                               _ptr(self.offsets), _ptr(ws), need, self._use(), err, 256), err)
+        ws = torch.empty(self._need, dtype=torch.uint8, device=self.device) if self._need else None
+        _call(self._library.smx_route_plan, self._index, ids.data_ptr(), self.num_rows, self.slots, self.num_groups, self._order, self._position,
+              self._offsets, _ptr(ws), self._need, self._use())
 
     def _use(self) -> int:
         """The current stream; the plan's memory stays until its work is done there, wherever the plan was made."""
         import torch
-        stream = torch.cuda.current_stream(self.device)
-        if not hasattr(self, "_home"):
-            self._home = stream.cuda_stream
-        elif stream.cuda_stream != self._home:
+        stream = torch.cuda.current_stream(self._index)
+        handle = stream.cuda_stream
+        if handle != self._home:
             self._plan.record_stream(stream)
-        return stream.cuda_stream
+        return handle
 
     def _weights(self, weights, dtype):
         if weights is None:
             return None
-        shape = (self.num_rows,) if weights.dim() == 1 and self.slots == 1 else (self.num_rows, self.slots)
+        shape = (self.num_rows,) if self.slots == 1 and weights.dim() == 1 else (self.num_rows, self.slots)
         return _values(weights, "weights", shape, dtype, self.device).contiguous()
 
     def dispatch(self, x, out=None):
         """``[rows * slots, width]``: every row of ``x`` once per group it goes to, in sorted order. Rows behind the last group are zero, or
         left as they were in ``out``."""
-        import torch
         x, stride = _rows(x, "x", (self.num_rows, None), None, self.device)
-        shape = (self.num_rows * self.slots, x.shape[1])
-        rows = torch.empty(shape, dtype=x.dtype, device=self.device) if out is None else _out(out, "out", shape, x.dtype, self.device)[0]
-        if not rows.is_contiguous():
-            raise ValueError("out must be contiguous")
-        if out is not None:
+        shape = (self._pairs, x.shape[1])
+        if out is None:
+            rows = x.new_empty(shape)
+        else:
+            rows = _out(out, "out", shape, x.dtype, self.device)[0]
+            if not rows.is_contiguous():
+                raise ValueError("out must be contiguous")
             _apart(rows, x)
-        with torch.cuda.device(self.device):
-            err = ctypes.create_string_buffer(256)
-            _call(self._library.smx_route_dispatch(_precision(x.dtype), _ptr(x), stride, self.num_rows, self.slots, x.shape[1], _ptr(self.position),
-                                                   _ptr(self.offsets), self.num_groups, _ptr(rows), int(out is None), self._use(), err, 256), err)
+        _call(self._library.smx_route_dispatch, self._index, _precision(x.dtype), x.data_ptr(), stride, self.num_rows, self.slots, shape[1],
+              self._position, self._offsets, self.num_groups, rows.data_ptr(), int(out is None), self._use())
         return rows
 
     def combine(self, rows, weights=None, base=None, out=None):
         """``base + sum_s weights[:, s] * rows[position[:, s]]`` (weights None: ones; base None: zero; ``out`` may be ``base``)."""
-        import torch
-        rows = _values(rows, "rows", (self.num_rows * self.slots, None), None, self.device).contiguous()
+        rows = _values(rows, "rows", (self._pairs, None), None, self.device).contiguous()
         width, dtype = rows.shape[1], rows.dtype
         weights = self._weights(weights, dtype)
         base, base_stride = (None, 0) if base is None else _rows(base, "base", (self.num_rows, width), dtype, self.device)
-        y = torch.empty((self.num_rows, width), dtype=dtype, device=self.device) if out is None else out
-        y, y_stride = _out(y, "out", (self.num_rows, width), dtype, self.device)
-        if out is not None:
+        if out is None:
+            y, y_stride = rows.new_empty((self.num_rows, width)), width
+        else:
+            y, y_stride = _out(out, "out", (self.num_rows, width), dtype, self.device)
             _apart(y, rows, weights, None if base is not None and base.data_ptr() == y.data_ptr() and base_stride == y_stride else base)
-        with torch.cuda.device(self.device):
-            err = ctypes.create_string_buffer(256)
-            _call(self._library.smx_route_combine(_precision(dtype), _ptr(rows), _ptr(self.position), self.num_rows, self.slots, width, _ptr(weights),
-                                                  _ptr(base), base_stride, _ptr(y), y_stride, self._use(), err, 256), err)
+        _call(self._library.smx_route_combine, self._index, _precision(dtype), rows.data_ptr(), self._position, self.num_rows, self.slots, width,
+              _ptr(weights), _ptr(base), base_stride, y.data_ptr(), y_stride, self._use())
         return y
 
     def dispatch_backward(self, grad_rows):
@@ -182,19 +206,15 @@ class RowRouting:
     def combine_backward(self, grad_y, rows=None, weights=None):
         """(gradient of ``rows``, gradient of ``weights``) of ``combine``; the latter is None without ``rows``. The gradient of ``base`` is
         ``grad_y``."""
-        import torch
         grad_y, stride = _rows(grad_y, "grad_y", (self.num_rows, None), None, self.device)
         width, dtype = grad_y.shape[1], grad_y.dtype
         weights = self._weights(weights, dtype)
         if rows is not None:
-            rows = _values(rows, "rows", (self.num_rows * self.slots, width), dtype, self.device).contiguous()
-        grad_rows = torch.empty((self.num_rows * self.slots, width), dtype=dtype, device=self.device)
-        grad_weights = None if rows is None else torch.empty((self.num_rows, self.slots), dtype=dtype, device=self.device)
-        with torch.cuda.device(self.device):
-            err = ctypes.create_string_buffer(256)
-            _call(self._library.smx_route_combine_backward(_precision(dtype), _ptr(grad_y), stride, _ptr(rows), _ptr(self.position), _ptr(self.offsets),
-                                                           self.num_groups, self.num_rows, self.slots, width, _ptr(weights), _ptr(grad_rows),
-                                                           _ptr(grad_weights), 1, self._use(), err, 256), err)
+            rows = _values(rows, "rows", (self._pairs, width), dtype, self.device).contiguous()
+        grad_rows = grad_y.new_empty((self._pairs, width))
+        grad_weights = None if rows is None else grad_y.new_empty((self.num_rows, self.slots))
+        _call(self._library.smx_route_combine_backward, self._index, _precision(dtype), grad_y.data_ptr(), stride, _ptr(rows), self._position,
+              self._offsets, self.num_groups, self.num_rows, self.slots, width, _ptr(weights), grad_rows.data_ptr(), _ptr(grad_weights), 1, self._use())
         return grad_rows, grad_weights
 
 
@@ -238,6 +258,8 @@ class AdapterLinear:
         need = self._library.smx_adapter_tiles_bytes(ctypes.byref(f))
         if need < 0:
             raise ValueError("the sizes exceed what smx_adapter_forward supports")
+        self._index = self.device.index
+        self._home = torch.cuda.current_stream(self._index).cuda_stream
         self._tiles = torch.empty(need, dtype=torch.uint8, device=self.device)
         f.tiles = self._tiles.data_ptr()
         self.set_adapters(down, up)
@@ -246,15 +268,12 @@ class AdapterLinear:
 
     # ------------------------------------------------------------------ matrices
     def _prepare(self, parts, shared, down, up):
-        import torch
         call = self._copy()
         for q in range(call.num_degrees):
             d = call.degrees[q]
             d.shared, d.down, d.up = _ptr(shared[q]) if shared else d.shared, _ptr(down[q]) if down else None, _ptr(up[q]) if up else None
-        with torch.cuda.device(self.device):
-            call.stream = self._use()
-            err = ctypes.create_string_buffer(256)
-            _call(self._library.smx_adapter_prepare(ctypes.byref(call), parts, err, 256), err)
+        call.stream = self._use()
+        _call(self._library.smx_adapter_prepare, self._index, ctypes.byref(call), parts)
 
     def set_adapters(self, down, up) -> None:
         """Other values of the adapters, of the same shapes."""
@@ -282,12 +301,11 @@ class AdapterLinear:
 
     def _use(self) -> int:
         import torch
-        stream = torch.cuda.current_stream(self.device)
-        if not hasattr(self, "_home"):
-            self._home = stream.cuda_stream
-        elif stream.cuda_stream != self._home:
+        stream = torch.cuda.current_stream(self._index)
+        handle = stream.cuda_stream
+        if handle != self._home:
             self._tiles.record_stream(stream)
-        return stream.cuda_stream
+        return handle
 
     def _begin(self, routing, weights):
         if not isinstance(routing, RowRouting):
@@ -299,7 +317,7 @@ class AdapterLinear:
         weights = routing._weights(weights, self.dtype)
         call = self._copy()
         call.num_rows, call.slots = routing.num_rows, routing.slots
-        call.order, call.position, call.offsets = _ptr(routing.order), _ptr(routing.position), _ptr(routing.offsets)
+        call.order, call.position, call.offsets = routing._order, routing._position, routing._offsets
         call.weights = _ptr(weights)
         return call, weights
 
@@ -308,27 +326,26 @@ class AdapterLinear:
         need = self._library.smx_adapter_workspace_bytes(ctypes.byref(call), backward)
         if need < 0:
             raise ValueError("the sizes exceed what smx_adapter_forward supports")
-        with torch.cuda.device(self.device):
-            ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-            call.workspace, call.workspace_bytes = _ptr(ws), need
-            call.stream = self._use()
+        ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+        call.workspace, call.workspace_bytes = _ptr(ws), need
+        call.stream = self._use()
+        if call.stream != routing._home:
             routing._use()
-            err = ctypes.create_string_buffer(256)
-            _call(fn(ctypes.byref(call), err, 256), err)
+        _call(fn, self._index, ctypes.byref(call))
 
     def forward(self, x, routing: RowRouting, weights=None, out=None, keep_hidden: bool = False):
         """``y``, or ``(y, hidden)`` with ``keep_hidden``: the products ``x down`` of every pair, for ``backward``."""
-        import torch
         call, weights = self._begin(routing, weights)
         x, call.x_stride = _rows(x, "x", (routing.num_rows, self.in_width), self.dtype, self.device)
-        y = torch.empty((routing.num_rows, self.out_width), dtype=self.dtype, device=self.device) if out is None else out
-        y, call.y_stride = _out(y, "out", (routing.num_rows, self.out_width), self.dtype, self.device)
-        if out is not None:
+        if out is None:
+            y, call.y_stride = x.new_empty((routing.num_rows, self.out_width)), self.out_width
+        else:
+            y, call.y_stride = _out(out, "out", (routing.num_rows, self.out_width), self.dtype, self.device)
             _apart(y, x, weights)
         call.x, call.y = _ptr(x), _ptr(y)
         hidden = None
         if keep_hidden:
-            hidden = torch.empty(self._library.smx_adapter_hidden_elements(ctypes.byref(call)), dtype=self.dtype, device=self.device)
+            hidden = x.new_empty(self._library.smx_adapter_hidden_elements(ctypes.byref(call)))
             call.hidden = _ptr(hidden) if hidden.numel() else None
         self._run(self._library.smx_adapter_forward, call, 0, routing)
         return (y, hidden) if keep_hidden else y

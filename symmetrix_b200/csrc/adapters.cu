@@ -394,20 +394,18 @@ Pass<T> make_pass(const smx_adapter_linear& c, bool transposed, T* hidden) {
     return p;
 }
 
-int sm_count() {
-    int dev = 0, n = 0;
-    SMX_CUDA(cudaGetDevice(&dev));
-    SMX_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
-    return n;
-}
 template <int HP>
 void launch_ts(const TsPass& t, long long tiles, cudaStream_t stream) {
     using L = TsPassLayout<HP>;
     // the warps' shares of registers are drawn from what the launch gives: fewer than planned and they would wait for ever
-    cudaFuncAttributes a{};
-    SMX_CUDA(cudaFuncGetAttributes(&a, adapter_pass_f32_kernel<HP>));
-    if (a.numRegs < kTsRegsLaunch) throw CudaError("adapter_pass_f32_kernel was built with too few registers");
-    SMX_CUDA(cudaFuncSetAttribute(adapter_pass_f32_kernel<HP>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::smem));
+    static std::atomic<bool> done[64];
+    if (first_on_device(done)) {
+        cudaFuncAttributes a{};
+        SMX_CUDA(cudaFuncGetAttributes(&a, adapter_pass_f32_kernel<HP>));
+        if (a.numRegs < kTsRegsLaunch) throw CudaError("adapter_pass_f32_kernel was built with too few registers");
+        SMX_CUDA(cudaFuncSetAttribute(adapter_pass_f32_kernel<HP>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::smem));
+        mark_on_device(done);
+    }
     adapter_pass_f32_kernel<HP><<<static_cast<unsigned>(std::min<long long>(tiles, sm_count())), kTsPassThreads, L::smem, stream>>>(t);
     launched("adapter_pass_f32_kernel");
 }
@@ -446,7 +444,11 @@ void launch_dp(const DpPass& t, long long tiles, cudaStream_t stream) {
     using L = DpLayout<BM, BN, NR, ST>;
     if (tiles > INT_MAX) throw ArgError("smx_adapter: too many rows");
     const auto kernel = adapter_pass_f64_kernel<BM, BN, WM, WN, NR, ST>;
-    if (L::smem > 40 * 1024) SMX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::smem));
+    static std::atomic<bool> done[64];
+    if (first_on_device(done)) {
+        SMX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::smem));
+        mark_on_device(done);
+    }
     kernel<<<static_cast<unsigned>(tiles), kDpThreads, L::smem, stream>>>(t);
     launched("adapter_pass_f64_kernel");
 }
@@ -506,7 +508,13 @@ void launch_grads(const GradPass<float>& gp, int problems, cudaStream_t stream) 
     t.order = gp.order; t.offsets = gp.offsets; t.weights = gp.weights;
     if (ctas > INT_MAX) throw ArgError("smx_adapter: too many rows");
     const int HP = padded_rank(gp.rank) / 16;
-    const auto kernel = HP == 1 ? adapter_grad_f32_kernel<1> : HP == 2 ? adapter_grad_f32_kernel<2> : HP == 3 ? adapter_grad_f32_kernel<3> : adapter_grad_f32_kernel<4>;
+    if (HP <= 2) {
+        const auto kernel = HP == 1 ? adapter_grad_rows_f32_kernel<1> : adapter_grad_rows_f32_kernel<2>;
+        kernel<<<static_cast<unsigned>(ctas), kTsThreads, 0, stream>>>(t);
+        launched("adapter_grad_rows_f32_kernel");
+        return;
+    }
+    const auto kernel = HP == 3 ? adapter_grad_f32_kernel<3> : adapter_grad_f32_kernel<4>;
     kernel<<<static_cast<unsigned>(ctas), kTsThreads, 16 * HP * 256 + 1024, stream>>>(t);
     launched("adapter_grad_f32_kernel");
 }

@@ -744,7 +744,121 @@ struct TsGrad {
     const float* weights;
 };
 
-// part[chunk][k][r] as in adapter_grad_kernel: D[k, r] = sum over rows a[row][k] (w h)[row][r]. A thread owns an inner index k of 128 and
+// Rank up to 32: part[chunk][k][r] = sum over the chunk's rows of a[row][k] (weight h)[row][r] on the FMA pipes, two hidden columns an instruction. A warp
+// takes a quarter of the rows, a lane four inner indices (512 consecutive bytes of a row a load); the weighted hidden rows come from
+// shared memory. No tile is turned or split, so the rows stream through; on the tensor cores a product with 16 columns takes as long as one with 96.
+template <int NH>                                    // hidden columns / 16
+__global__ void __launch_bounds__(kTsThreads, NH == 1 ? 4 : 2) adapter_grad_rows_f32_kernel(const __grid_constant__ TsGrad pass) {
+    constexpr int Rp = 16 * NH, kStep = 64;
+    __shared__ __align__(16) float hs[kStep * Rp];
+    __shared__ __align__(16) float joined[128 * Rp];
+    __shared__ long long a_base[kGradChunk];
+    __shared__ float row_weight[kGradChunk];
+    __shared__ TileRows tile;
+    __shared__ int which, k_block;
+    __shared__ long long chunk_index;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (warp == 0) {
+        long long t = blockIdx.x, tiles = 0;
+        TileRows rows{};
+        int hit = -1, kb = 0;
+        for (int q = 0; q < pass.problems; ++q) {
+            const int blocks = (pass.problem[q].Kd + 127) / 128;
+            if (find_tile(pass.offsets, pass.groups, false, pass.pairs, pass.problem[q].comps, kGradChunk, t / blocks, rows, tiles)) {
+                hit = q; kb = static_cast<int>(t % blocks); t /= blocks;
+                break;
+            }
+            t -= tiles * blocks;
+        }
+        if (lane == 0) { which = hit; k_block = kb; chunk_index = t; tile = rows; }
+    }
+    __syncthreads();
+    if (which < 0) return;
+    const GradProblem<float>& d = pass.problem[which];
+    const int R = pass.rank, rows = static_cast<int>(tile.rows), k = k_block * 128 + 4 * lane, left = d.Kd - k;
+    const long long q0 = tile.row0 / d.comps;
+    const int m0 = static_cast<int>(tile.row0 - q0 * d.comps);
+    for (int i = tid; i < rows; i += kTsThreads) {
+        const int ahead = (m0 + i) / d.comps, pair = pass.order[tile.first_pair + q0 + ahead];
+        a_base[i] = static_cast<long long>(pair / pass.slots) * d.a_stride + d.a_off + static_cast<long long>(m0 + i - ahead * d.comps) * d.Kd;
+        row_weight[i] = pass.weights ? pass.weights[pair] : 1.f;
+    }
+    const bool wide = ((d.a_stride | d.a_off | d.Kd) & 3) == 0 && (reinterpret_cast<uintptr_t>(d.a) & 15) == 0;
+    const float* hidden = d.hidden + (tile.first_pair * d.comps + tile.row0) * R;
+    unsigned long long acc[4][Rp / 2];               // pairs of hidden columns
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int j = 0; j < Rp / 2; ++j) acc[q][j] = 0ull;
+    constexpr int kAhead = 8;
+    for (int r0 = 0; r0 < rows; r0 += kStep) {
+        const int n = min(kStep, rows - r0);
+        __syncthreads();
+        for (int i = tid; i < kStep * Rp; i += kTsThreads) {
+            const int r = i / Rp, c = i % Rp;
+            hs[i] = r < n && c < R ? __ldg(hidden + static_cast<long long>(r0 + r) * R + c) * row_weight[r0 + r] : 0.f;
+        }
+        __syncthreads();
+#pragma unroll 1
+        for (int g = 0; g < kStep / 4; g += kAhead) {            // rows warp + 4 g .. of the step
+            float4 a[kAhead];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const int r = warp + 4 * (g + u);
+                a[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (r >= n) continue;
+                const float* from = d.a + a_base[r0 + r] + k;
+                if (wide) {
+                    if (left > 0) a[u] = __ldg(reinterpret_cast<const float4*>(from));
+                } else {
+                    if (left > 0) a[u].x = __ldg(from);
+                    if (left > 1) a[u].y = __ldg(from + 1);
+                    if (left > 2) a[u].z = __ldg(from + 2);
+                    if (left > 3) a[u].w = __ldg(from + 3);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const ulonglong2* h = reinterpret_cast<const ulonglong2*>(hs + (warp + 4 * (g + u)) * Rp);
+                const float v[4] = {a[u].x, a[u].y, a[u].z, a[u].w};
+                unsigned long long twice[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) asm("mov.b64 %0, {%1, %1};" : "=l"(twice[q]) : "f"(v[q]));
+#pragma unroll
+                for (int j = 0; j < Rp / 4; ++j) {
+                    const ulonglong2 two = h[j];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc[q][2 * j]) : "l"(twice[q]), "l"(two.x));
+                        asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc[q][2 * j + 1]) : "l"(twice[q]), "l"(two.y));
+                    }
+                }
+            }
+        }
+    }
+    // the warps' sums in turn
+    for (int turn = 0; turn < 4; ++turn) {
+        __syncthreads();
+        if (warp != turn) continue;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int j = 0; j < Rp / 2; ++j) {
+                float x, y;
+                asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(acc[q][j]));
+                float* to = joined + (2 * j) * 128 + 4 * lane + q;
+                to[0] = turn ? to[0] + x : x;
+                to[128] = turn ? to[128] + y : y;
+            }
+    }
+    __syncthreads();
+    for (int i = tid; i < 128 * R; i += kTsThreads) {
+        const int kk = i / R, r = i - kk * R;
+        if (k_block * 128 + kk < d.Kd) d.part[(chunk_index * d.Kd + k_block * 128) * R + i] = joined[r * 128 + kk];
+    }
+}
+
+// Higher ranks, on the tensor cores: D[k, r] = sum over rows a[row][k] (w h)[row][r]. A thread owns an inner index k of 128 and
 // loads a[row][k] of 32 rows (a warp reads 128 consecutive bytes of each), which is the row operand's transpose for nothing; the hidden values
 // are split into shared memory. The sums of every 32 rows are added in registers, as in the pass kernel.
 constexpr int kTsGradColumns = 128, kTsGradSlot = 64;

@@ -299,13 +299,6 @@ __global__ void __launch_bounds__(256) route_combine_backward_kernel(const V* __
 }
 
 // ------------------------------------------------------------------------------------------- host side
-int sm_count() {
-    int dev = 0, n = 0;
-    SMX_CUDA(cudaGetDevice(&dev));
-    SMX_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
-    return n;
-}
-
 void check_sizes(const char* what, long num_rows, int slots, int num_groups) {
     if (num_rows < 0) throw ArgError(std::string(what) + ": negative number of rows");
     if (slots < 1 || slots > SMX_ROUTE_MAX_SLOTS) throw ArgError(std::string(what) + ": slots must lie in 1 .. " + std::to_string(SMX_ROUTE_MAX_SLOTS));
@@ -344,6 +337,28 @@ void launched(const char* what) {
 
 thread_local long operator_launches = 0;
 
+int sm_count() {
+    static std::atomic<int> count[64];
+    int dev = 0;
+    SMX_CUDA(cudaGetDevice(&dev));
+    const int known = dev < 64 ? count[dev].load(std::memory_order_relaxed) : 0;
+    if (known) return known;
+    int n = 0;
+    SMX_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
+    if (dev < 64) count[dev].store(n, std::memory_order_relaxed);
+    return n;
+}
+bool first_on_device(std::atomic<bool> (&done)[64]) {
+    int dev = 0;
+    SMX_CUDA(cudaGetDevice(&dev));
+    return dev >= 64 || !done[dev].load(std::memory_order_acquire);
+}
+void mark_on_device(std::atomic<bool> (&done)[64]) {
+    int dev = 0;
+    SMX_CUDA(cudaGetDevice(&dev));
+    if (dev < 64) done[dev].store(true, std::memory_order_release);
+}
+
 size_t route_plan_bytes(long num_rows, int slots, int num_groups) {
     check_sizes("smx_route_plan", num_rows, slots, num_groups);
     const long long pairs = static_cast<long long>(num_rows) * slots;
@@ -364,7 +379,11 @@ void route_plan(const int* ids, long num_rows, int slots, int num_groups, int* o
         int warps = static_cast<int>(std::min<long long>(32, std::max<long long>(1, (pairs + 31) / 32)));
         while (warps > 1 && (warps + 1) * bins > 32768) warps /= 2;
         const int smem = ((warps + 1) * bins + 1) * static_cast<int>(sizeof(int));
-        if (smem > 48 * 1024) SMX_CUDA(cudaFuncSetAttribute(route_plan_small_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+        static std::atomic<bool> done[64];
+        if (smem > 48 * 1024 && first_on_device(done)) {
+            SMX_CUDA(cudaFuncSetAttribute(route_plan_small_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+            mark_on_device(done);
+        }
         const int threads = std::max(128, 32 * warps);
         route_plan_small_kernel<<<1, threads, smem, stream>>>(ids, static_cast<int>(pairs), num_groups, warps, order, position, offsets);
         launched("route_plan_small_kernel");

@@ -5,12 +5,19 @@
 
 #include <cuda_runtime.h>
 
+#include <atomic>
+
 #include "../../include/symmetrix_b200.h"
 
 namespace smx {
 
 // Kernels that this thread launched here and in csrc/adapters.cu.
 extern thread_local long operator_launches;
+
+// SMs of the current device; and tables of devices on which a kernel's attributes have been set, which is done once on each.
+int sm_count();
+bool first_on_device(std::atomic<bool> (&done)[64]);
+void mark_on_device(std::atomic<bool> (&done)[64]);
 
 size_t route_plan_bytes(long num_rows, int slots, int num_groups);
 void route_plan(const int* ids, long num_rows, int slots, int num_groups, int* order, int* position, int* offsets, void* workspace,
