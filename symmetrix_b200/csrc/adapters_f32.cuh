@@ -93,6 +93,14 @@ __device__ __forceinline__ void ts_chunk(uint32_t d, uint32_t a_hi, uint32_t a_l
 __device__ __forceinline__ void ts_commit(unsigned long long* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+// A value that is the same in all lanes, known to be so by the compiler: it can live in the uniform registers that the instructions issued by one lane
+// take their operands from.
+__device__ __forceinline__ int ts_uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+__device__ __forceinline__ bool ts_elect() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
 __device__ __forceinline__ void ts_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void ts_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void ts_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -283,9 +291,10 @@ __device__ __forceinline__ void ts_bulk(uint32_t to, const float* from, uint32_t
 //               is these tiles in shared memory and 32 values of the rows in tensor memory, with one barrier for both
 //   warp 1      the products (one thread)
 //   warp 2      finds the tiles and looks up their atoms and weights (a ring of four, ahead of all others)
-//   warp 3      rows: 64 values of each by asynchronous copies of 16 bytes (4 where rows start on no 16-byte boundary) into a ring of two stages
-//               (loads and stores by the thread that owns a row touch 32 rows an instruction; a bulk copy of 256 bytes took 70 cycles to issue)
-//   warps 4-7   a thread splits 32 values of its row at a time and stores them to the tensor memory's row operand
+//   warps 4-7   rows: a warp copies 32 values of each of its 32 rows asynchronously, 16 bytes a lane (4 where rows start on no 16-byte boundary), three
+//               chunks ahead; a thread splits those of its row and stores them to the tensor memory's row operand. (Loads and stores by
+//               the thread that owns a row touch 32 rows an instruction; a bulk copy takes 70 cycles to issue; one warp that copied for all
+//               four took longer than the products: 184 us instead of 160 at 98,304 atoms.)
 //   warps 8-15  a thread adds half of its row's partial sums of every 64 inner values in registers (the tensor core cuts its sums instead of
 //               rounding them: a single sum over 128 inner values was off five times as far as float32) and writes its half of the row
 //               while the products of the next tile run
@@ -293,8 +302,8 @@ __device__ __forceinline__ void ts_bulk(uint32_t to, const float* from, uint32_t
 // stored into the hidden columns of its last two sums (head in the last one's, remainder in the other's); the products with second_g go on
 // top of the last sum, which is read after them.
 // Every wait is bounded; if one runs out, the CTA gives up and fills its remaining tiles with NaN.
-constexpr int kTsPassThreads = 512, kTsWorkRing = 4, kTsRowStages = 2;
-constexpr int kTsRowValues = 64, kTsRowPitch = kTsRowValues + 4;              // floats: threads that read their rows 16 bytes at a time hit all banks
+constexpr int kTsPassThreads = 512, kTsWorkRing = 4, kTsRowStages = 4;
+constexpr int kTsRowPitch = kTsChunk + 4;                                     // floats: threads that read their rows 16 bytes at a time hit all banks
 constexpr int kTsRegsControl = 72, kTsRegsRows = 120, kTsRegsSums = 160, kTsRegsLaunch = 128;
 static_assert(kTsRegsControl + kTsRegsRows + 2 * kTsRegsSums <= 4 * kTsRegsLaunch, "the registers of the launch are shared out");
 template <int HP>                                    // hidden columns / 16
@@ -313,8 +322,7 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
     using L = TsPassLayout<HP>;
     constexpr int NS = L::stages;
     extern __shared__ unsigned char ts_smem_raw[];
-    __shared__ __align__(8) unsigned long long work_full[kTsWorkRing], work_free[kTsWorkRing], full[NS], free[NS], x_full[kTsRowStages],
-        x_free[kTsRowStages], d_full[2], d_free[2], t_full, t_done;
+    __shared__ __align__(8) unsigned long long work_full[kTsWorkRing], work_free[kTsWorkRing], full[NS], free[NS], d_full[2], d_free[2], t_full, t_done;
     __shared__ TsWork work[kTsWorkRing];
     __shared__ long long work_in[kTsWorkRing][kTsRows], work_out[kTsWorkRing][kTsRows];    // where its rows start, in `in`, in `out` without the tile's
     __shared__ int work_place[kTsWorkRing][kTsRows];                                       // first column; sorted position and component
@@ -322,14 +330,13 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
     __shared__ float work_weight[kTsWorkRing][kTsRows];
     __shared__ uint32_t tmem_slot;
     __shared__ int failed;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = ts_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     unsigned char* stages = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(ts_smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     float* row_stages = reinterpret_cast<float*>(stages + NS * L::stage_bytes);
     if (threadIdx.x == 0) {
         failed = 0;
-        for (int q = 0; q < kTsWorkRing; ++q) { mbar_init(&work_full[q], 1); mbar_init(&work_free[q], 15); }
+        for (int q = 0; q < kTsWorkRing; ++q) { mbar_init(&work_full[q], 1); mbar_init(&work_free[q], 14); }
         for (int q = 0; q < NS; ++q) { mbar_init(&full[q], 5); mbar_init(&free[q], 1); }
-        for (int q = 0; q < kTsRowStages; ++q) { mbar_init(&x_full[q], 32); mbar_init(&x_free[q], 4); }
         for (int q = 0; q < 2; ++q) { mbar_init(&d_full[q], 1); mbar_init(&d_free[q], 8); }
         mbar_init(&t_full, 8);
         mbar_init(&t_done, 1);
@@ -380,47 +387,6 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
                 if (lane == 0) mbar_arrive(&work_full[slot]);
                 if (!w.found) break;
             }
-        } else if (warp == 3) {
-            int n = 0, st = 0;                                           // stages filled so far, the next one
-            unsigned round = 1;                                          // parity of its last use but one
-            bool ok = true;
-            for (int i = 0; ok; ++i) {
-                const int slot = i % kTsWorkRing;
-                if (!ts_wait_warp(&work_full[slot], (i / kTsWorkRing) & 1, &failed)) { ok = false; break; }
-                const TsWork w = work[slot];
-                if (!w.found) {
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&work_free[slot]);
-                    break;
-                }
-                const TsDegree& d = pass.degree[w.degree];
-                const int rows = static_cast<int>(w.rows.rows);
-                const unsigned long long bits = static_cast<unsigned long long>(pass.in_stride | d.in_off | d.Kd) * 4u | reinterpret_cast<uintptr_t>(pass.in);
-                const bool wide = (bits & 15) == 0;
-                for (int k0 = 0; k0 < d.Kd; k0 += kTsRowValues) {
-                    const int left = min(kTsRowValues, d.Kd - k0);
-                    if (n >= kTsRowStages && !ts_wait_warp(&x_free[st], round, &failed)) { ok = false; break; }
-                    float* to = row_stages + st * L::row_floats;
-                    const float* from = pass.in + k0;
-                    if (wide) {                      // two rows an instruction, 16 bytes a lane
-                        const int c = (lane & 15) * 4;
-                        if (c < left)
-#pragma unroll 4
-                            for (int r = lane >> 4; r < rows; r += 2) cp_async16(to + r * kTsRowPitch + c, from + work_in[slot][r] + c, 16);
-                    } else {
-#pragma unroll 1
-                        for (int r = 0; r < rows; ++r)
-                            for (int c = lane; c < left; c += 32) cp_async4(to + r * kTsRowPitch + c, from + work_in[slot][r] + c);
-                    }
-                    __syncwarp();
-                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&x_full[st])) : "memory");
-                    ++n;
-                    if (++st == kTsRowStages) { st = 0; round ^= 1u; }
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&work_free[slot]);
-            }
-            asm volatile("cp.async.wait_all;" ::: "memory");             // none may be in flight when the CTA ends
         } else if (warp == 0 && lane == 0) {
             int n = 0, st = 0;                                           // chunks copied so far, stage of the next one
             unsigned round = 1;                                          // parity of the stage's last use but one
@@ -468,85 +434,139 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
             }
             if (!ok)                                                     // copies in flight write into this CTA's memory: wait for them (bounded)
                 for (int q = max(0, n - NS); q < n; ++q) mbar_wait(&full[q % NS], (q / NS) & 1);
-        } else if (warp == 1 && lane == 0) {
+        } else if (warp == 1) {
             int st = 0, sum = 0, nd = 0;                                 // stage and partial sum in turn, with the parity of their next and last use
             unsigned st_par = 0, sum_par = 1, hid_par = 0;
             bool ok = true;
-            const uint32_t base = smem_u32(stages);
+            const bool leader = ts_elect();
+            const uint32_t base = smem_u32(stages), t0 = ts_uniform(tmem);
             for (int i = 0; ok; ++i) {
                 const int slot = i % kTsWorkRing;
-                ok = ts_wait(&work_full[slot], (i / kTsWorkRing) & 1, &failed);
+                ok = ts_wait_warp(&work_full[slot], (i / kTsWorkRing) & 1, &failed);
                 if (!ok) break;
                 const TsWork w = work[slot];
-                mbar_arrive(&work_free[slot]);
-                if (!w.found) break;
+                __syncwarp();
+                if (leader) mbar_arrive(&work_free[slot]);
+                if (!ts_uniform(w.found)) break;
                 const TsShape s = ts_shape(pass, w);
+                const int nx = ts_uniform(s.nx), items = nx + ts_uniform(s.rounds), main_cols = ts_uniform(s.main_cols), out_cols = ts_uniform(s.cols),
+                          in_cols = main_cols + ts_uniform(s.adapter ? L::Rp : 0), hid_col = ts_uniform(s.hid_col);
                 // chunks of inner values, then rounds of hidden values on top of the last sum: one piece of code, which stays in the instruction cache
 #pragma unroll 1
-                for (int j = 0; j < s.nx + s.rounds; ++j) {
-                    const bool inner = j < s.nx;
-                    const int e = j - s.nx;
+                for (int j = 0; j < items; ++j) {
+                    const bool inner = j < nx;
+                    const int e = j - nx;
                     int cols, steps = 4;
                     uint32_t d, hi, lo;
                     bool add;
                     if (inner) {
-                        if ((j & 1) == 0 && nd >= 2) ok = ts_wait(&d_free[sum], sum_par, &failed);
-                        cols = s.main_cols + (s.adapter ? L::Rp : 0);
-                        d = tmem + sum * L::sum_cols + (s.main_cols ? 0 : 128);
-                        hi = tmem + L::slot0 + 64 * st;
+                        if ((j & 1) == 0 && nd >= 2) ok = ts_wait_warp(&d_free[sum], sum_par, &failed);
+                        cols = in_cols;
+                        d = t0 + sum * L::sum_cols + (main_cols ? 0 : 128);
+                        hi = t0 + L::slot0 + 64 * st;
                         lo = hi + 32;
                         add = (j & 1) != 0;
                     } else {
-                        if (e == 0) ok = ts_wait(&t_full, hid_par, &failed);
-                        cols = s.cols;
+                        if (e == 0) ok = ts_wait_warp(&t_full, hid_par, &failed);
+                        cols = out_cols;
                         steps = min(4, L::Rp / 8 - 4 * e);
-                        d = tmem + (sum ^ 1) * L::sum_cols;
-                        hi = d + s.hid_col + 32 * e;
-                        lo = tmem + sum * L::sum_cols + s.hid_col + 32 * e;
-                        add = s.main_cols > 0 || e > 0;
+                        d = t0 + (sum ^ 1) * L::sum_cols;
+                        hi = d + hid_col + 32 * e;
+                        lo = t0 + sum * L::sum_cols + hid_col + 32 * e;
+                        add = main_cols > 0 || e > 0;
                     }
-                    ok = ok && ts_wait(&full[st], st_par, &failed);
+                    ok = ok && ts_wait_warp(&full[st], st_par, &failed);
                     if (!ok) break;
                     ts_fence_after();
                     const uint32_t b = base + st * L::stage_bytes;
-                    ts_chunk(d, hi, lo, b, b + cols * 128u, ts_idesc(cols), steps, add);
-                    ts_commit(&free[st]);
-                    if (++st == NS) { st = 0; st_par ^= 1u; }
-                    if (inner) {
-                        if ((j & 1) != 0 || j + 1 == s.nx) {
-                            ts_commit(&d_full[sum]);
-                            ++nd;
-                            sum ^= 1;
-                            if (sum == 0) sum_par ^= 1u;
-                        }
-                    } else if (e + 1 == s.rounds) {
-                        ts_commit(&t_done);
-                        hid_par ^= 1u;
+                    const bool last_sum = inner && ((j & 1) != 0 || j + 1 == nx), last_round = !inner && j + 1 == items;
+                    if (leader) {
+                        ts_chunk(d, hi, lo, b, b + cols * 128u, ts_idesc(cols), steps, add);
+                        ts_commit(&free[st]);
+                        if (last_sum) ts_commit(&d_full[sum]);
+                        if (last_round) ts_commit(&t_done);
                     }
+                    __syncwarp();
+                    if (++st == NS) { st = 0; st_par ^= 1u; }
+                    if (last_sum) {
+                        ++nd;
+                        sum ^= 1;
+                        if (sum == 0) sum_par ^= 1u;
+                    }
+                    if (last_round) hid_par ^= 1u;
                 }
             }
         }
     } else if (warp < 8) {
         ts_registers_less<kTsRegsRows>();
         const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-        const int tid = threadIdx.x & 127;
-        int st = 0, op = 0, na = 0;                  // row stage and operand stage in turn, operands so far
-        unsigned st_par = 0, op_par = 1;             // parity of the stage's next use, of the operand's last one
+        const int tid = threadIdx.x & 127, first = tid & ~31;            // the warp's rows are its own: no barrier but the work's
+        float* const rows_at = row_stages + first * kTsRowPitch;
+        int op = 0, na = 0, xs = 0;                  // operand stage and row stage in turn, operands so far
+        unsigned op_par = 1;                         // parity of the operand stage's last use
         bool ok = true;
+        // copies run kTsRowStages - 1 chunks ahead of what is split, across tiles
+        int ahead_tile = 0, ahead = 0, ahead_nx = 0, ahead_slot = 0, ahead_Kd = 0, ahead_rows = 0;
+        bool more = true, wide = false;
+        const float* from = nullptr;
+        auto copy_next = [&](int stage) {
+            if (more && ahead == ahead_nx) {
+                ahead_slot = ahead_tile % kTsWorkRing;
+                if (!ts_wait_warp(&work_full[ahead_slot], (ahead_tile / kTsWorkRing) & 1, &failed)) {
+                    ok = more = false;
+                } else {
+                    const TsWork& w = work[ahead_slot];
+                    more = w.found != 0;
+                    if (more) {
+                        const TsDegree& d = pass.degree[w.degree];
+                        const unsigned long long bits = static_cast<unsigned long long>(pass.in_stride | d.in_off | d.Kd) * 4u | reinterpret_cast<uintptr_t>(pass.in);
+                        wide = (bits & 15) == 0;
+                        ahead = 0; ahead_Kd = d.Kd; ahead_nx = (d.Kd + kTsChunk - 1) / kTsChunk;
+                        ahead_rows = min(32, static_cast<int>(w.rows.rows) - first);
+                        from = pass.in;
+                        ++ahead_tile;
+                    }
+                }
+            }
+            if (more) {
+                float* to = rows_at + stage * L::row_floats;
+                const long long* where = work_in[ahead_slot] + first;
+                const int left = min(kTsChunk, ahead_Kd - ahead * kTsChunk);
+                if (wide) {                          // four rows an instruction, 16 bytes a lane
+                    const int c = (lane & 7) * 4;
+                    if (c < left)
+#pragma unroll 4
+                        for (int r = lane >> 3; r < ahead_rows; r += 4) cp_async16(to + r * kTsRowPitch + c, from + where[r] + c, 16);
+                } else if (lane < left) {
+#pragma unroll 1
+                    for (int r = 0; r < ahead_rows; ++r) cp_async4(to + r * kTsRowPitch + lane, from + where[r] + lane);
+                }
+                from += kTsChunk;
+                ++ahead;
+            }
+            cp_async_commit();
+        };
+        for (int q = 0; q < kTsRowStages - 1; ++q) copy_next(q);
         for (int i = 0; ok; ++i) {
             const int slot = i % kTsWorkRing;
             if (!ts_wait_warp(&work_full[slot], (i / kTsWorkRing) & 1, &failed)) break;
             const TsWork w = work[slot];
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&work_free[slot]);
-            if (!w.found) break;
+            if (!w.found) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&work_free[slot]);
+                break;
+            }
             const TsShape s = ts_shape(pass, w);
             const int Kd = pass.degree[w.degree].Kd;
             const bool live = tid < s.rows;
             for (int j = 0; j < s.nx + s.rounds; ++j) {
-                const int k0 = j * kTsChunk;
                 const bool inner = j < s.nx;
-                if (inner && k0 % kTsRowValues == 0 && !ts_wait_warp(&x_full[st], st_par, &failed)) { ok = false; break; }
+                if (inner) {
+                    cp_async_wait<kTsRowStages - 2>();
+                    __syncwarp();                    // the chunk is there for all lanes, and all have read the one before
+                    copy_next(xs == 0 ? kTsRowStages - 1 : xs - 1);
+                    if (!ok) break;
+                }
                 if (na >= NS && !ts_wait_warp(&free[op], op_par, &failed)) { ok = false; break; }
                 ++na;
                 unsigned long long* const bar = &full[op];
@@ -557,14 +577,15 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
                     continue;
                 }
                 ts_fence_after();
-                const float* from = row_stages + st * L::row_floats + tid * kTsRowPitch + k0 % kTsRowValues;
-                const int good = live ? Kd - k0 : 0;                     // what the stage holds behind the tile's or the row's end is no value
+                const float* row = row_stages + xs * L::row_floats + tid * kTsRowPitch;
+                if (++xs == kTsRowStages) xs = 0;
+                const int good = live ? Kd - j * kTsChunk : 0;           // what the stage holds behind the tile's or the row's end is no value
 #pragma unroll 1
                 for (int q = 0; q < kTsChunk; q += 16) {
                     float v[16], lo[16];
 #pragma unroll
                     for (int e = 0; e < 16; e += 4) {
-                        const float4 f = *reinterpret_cast<const float4*>(from + q + e);
+                        const float4 f = *reinterpret_cast<const float4*>(row + q + e);
                         v[e] = f.x; v[e + 1] = f.y; v[e + 2] = f.z; v[e + 3] = f.w;
                     }
                     if (good < q + 16)
@@ -575,17 +596,15 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
                     ts_store16(to + q, v);
                     ts_store16(to + 32 + q, lo);
                 }
-                if (k0 % kTsRowValues != 0 || k0 + kTsChunk >= Kd) {
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&x_free[st]);
-                    if (++st == kTsRowStages) { st = 0; st_par ^= 1u; }
-                }
                 ts_wait_store();
                 ts_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar);
             }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&work_free[slot]);
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");                 // none may be in flight when the CTA ends
     } else {
         ts_registers_more<kTsRegsSums>();
         const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
