@@ -468,15 +468,17 @@ void launch_pass(const smx_adapter_linear&, bool, const Pass<double>& p, int deg
         long long n = 0;
         for (int q = 0; q < degrees; ++q) {
             const long long rows = (p.sorted ? p.pairs : p.num_rows) * p.degree[q].comps;
-            n += (p.sorted ? rows / BM + p.groups + 1 : (rows + BM - 1) / BM) * (p.out ? (p.degree[q].Nc + BN - 1) / BN : 1);
+            const bool all = !p.out || (BM == 64 && !p.degree[q].W);         // one CTA makes all blocks of columns
+            n += (p.sorted ? rows / BM + p.groups + 1 : (rows + BM - 1) / BM) * (all ? 1 : (p.degree[q].Nc + BN - 1) / BN);
         }
         return n;
     };
     auto by_rank = [&](auto nr) {
         constexpr int NR = decltype(nr)::value;
         if (tiles(64, 64) <= 2LL * sm_count()) launch_dp<16, 32, 1, 4, NR, 4>(t, tiles(16, 32), stream);
-        else launch_dp<64, 64, 2, 2, NR, 3>(t, tiles(64, 64), stream);
+        else launch_dp<64, 64, 2, 2, NR, 2>(t, tiles(64, 64), stream);
     };
+    if (!p.sorted && tiles(64, 64) > 2LL * sm_count()) { launch_dp<64, 64, 2, 2, 0, 2>(t, tiles(64, 64), stream); return; }
     if (p.rank <= 8) by_rank(std::integral_constant<int, 1>{});
     else if (p.rank <= 16) by_rank(std::integral_constant<int, 2>{});
     else if (p.rank <= 32) by_rank(std::integral_constant<int, 4>{});
@@ -502,7 +504,8 @@ void launch_grads(const GradPass<float>& gp, int problems, cudaStream_t stream) 
     long long ctas = 0;
     for (int q = 0; q < problems; ++q) {
         t.problem[q] = gp.problem[q];
-        ctas += (gp.pairs * gp.problem[q].comps / kGradChunk + gp.groups) * ts_blocks(gp.problem[q].Kd);
+        const int cols = padded_rank(gp.rank) == 32 ? 64 : 128;
+        ctas += (gp.pairs * gp.problem[q].comps / kGradChunk + gp.groups) * ((gp.problem[q].Kd + cols - 1) / cols);
     }
     t.problems = problems; t.rank = gp.rank; t.groups = gp.groups; t.slots = gp.slots; t.pairs = gp.pairs;
     t.order = gp.order; t.offsets = gp.offsets; t.weights = gp.weights;

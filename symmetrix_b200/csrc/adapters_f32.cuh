@@ -291,7 +291,7 @@ __device__ __forceinline__ void ts_bulk(uint32_t to, const float* from, uint32_t
 //               is these tiles in shared memory and 32 values of the rows in tensor memory, with one barrier for both
 //   warp 1      the products (one thread)
 //   warp 2      finds the tiles and looks up their atoms and weights (a ring of four, ahead of all others)
-//   warps 4-7   rows: a warp copies 32 values of each of its 32 rows asynchronously, 16 bytes a lane (4 where rows start on no 16-byte boundary), three
+//   warps 4-7   rows: a warp copies 32 values of each of its 32 rows asynchronously, 16 bytes a lane (4 where rows start on no 16-byte boundary), four
 //               chunks ahead; a thread splits those of its row and stores them to the tensor memory's row operand. (Loads and stores by
 //               the thread that owns a row touch 32 rows an instruction; a bulk copy takes 70 cycles to issue; one warp that copied for all
 //               four took longer than the products: 184 us instead of 160 at 98,304 atoms.)
@@ -302,7 +302,7 @@ __device__ __forceinline__ void ts_bulk(uint32_t to, const float* from, uint32_t
 // stored into the hidden columns of its last two sums (head in the last one's, remainder in the other's); the products with second_g go on
 // top of the last sum, which is read after them.
 // Every wait is bounded; if one runs out, the CTA gives up and fills its remaining tiles with NaN.
-constexpr int kTsPassThreads = 512, kTsWorkRing = 4, kTsRowStages = 4;
+constexpr int kTsPassThreads = 512, kTsWorkRing = 4, kTsRowStages = 5;
 constexpr int kTsRowPitch = kTsChunk + 4;                                     // floats: threads that read their rows 16 bytes at a time hit all banks
 constexpr int kTsRegsControl = 72, kTsRegsRows = 120, kTsRegsSums = 160, kTsRegsLaunch = 128;
 static_assert(kTsRegsControl + kTsRegsRows + 2 * kTsRegsSums <= 4 * kTsRegsLaunch, "the registers of the launch are shared out");
@@ -764,13 +764,13 @@ struct TsGrad {
 };
 
 // Rank up to 32: part[chunk][k][r] = sum over the chunk's rows of a[row][k] (weight h)[row][r] on the FMA pipes, two hidden columns an instruction. A warp
-// takes a quarter of the rows, a lane four inner indices (512 consecutive bytes of a row a load); the weighted hidden rows come from
+// takes a quarter of the rows, a lane four inner indices (two from rank 17 on: the sums of four would leave two CTAs an SM); the weighted hidden rows come from
 // shared memory. No tile is turned or split, so the rows stream through; on the tensor cores a product with 16 columns takes as long as one with 96.
 template <int NH>                                    // hidden columns / 16
-__global__ void __launch_bounds__(kTsThreads, NH == 1 ? 4 : 2) adapter_grad_rows_f32_kernel(const __grid_constant__ TsGrad pass) {
-    constexpr int Rp = 16 * NH, kStep = 64;
+__global__ void __launch_bounds__(kTsThreads, 4) adapter_grad_rows_f32_kernel(const __grid_constant__ TsGrad pass) {
+    constexpr int Rp = 16 * NH, kStep = 64, kPer = 4 / NH, kCols = 32 * kPer;         // inner indices of a lane, of the CTA
     __shared__ __align__(16) float hs[kStep * Rp];
-    __shared__ __align__(16) float joined[128 * Rp];
+    __shared__ __align__(16) float joined[kCols * Rp];
     __shared__ long long a_base[kGradChunk];
     __shared__ float row_weight[kGradChunk];
     __shared__ TileRows tile;
@@ -782,7 +782,7 @@ __global__ void __launch_bounds__(kTsThreads, NH == 1 ? 4 : 2) adapter_grad_rows
         TileRows rows{};
         int hit = -1, kb = 0;
         for (int q = 0; q < pass.problems; ++q) {
-            const int blocks = (pass.problem[q].Kd + 127) / 128;
+            const int blocks = (pass.problem[q].Kd + kCols - 1) / kCols;
             if (find_tile(pass.offsets, pass.groups, false, pass.pairs, pass.problem[q].comps, kGradChunk, t / blocks, rows, tiles)) {
                 hit = q; kb = static_cast<int>(t % blocks); t /= blocks;
                 break;
@@ -794,7 +794,7 @@ __global__ void __launch_bounds__(kTsThreads, NH == 1 ? 4 : 2) adapter_grad_rows
     __syncthreads();
     if (which < 0) return;
     const GradProblem<float>& d = pass.problem[which];
-    const int R = pass.rank, rows = static_cast<int>(tile.rows), k = k_block * 128 + 4 * lane, left = d.Kd - k;
+    const int R = pass.rank, rows = static_cast<int>(tile.rows), k = k_block * kCols + kPer * lane, left = d.Kd - k;
     const long long q0 = tile.row0 / d.comps;
     const int m0 = static_cast<int>(tile.row0 - q0 * d.comps);
     for (int i = tid; i < rows; i += kTsThreads) {
@@ -802,11 +802,11 @@ __global__ void __launch_bounds__(kTsThreads, NH == 1 ? 4 : 2) adapter_grad_rows
         a_base[i] = static_cast<long long>(pair / pass.slots) * d.a_stride + d.a_off + static_cast<long long>(m0 + i - ahead * d.comps) * d.Kd;
         row_weight[i] = pass.weights ? pass.weights[pair] : 1.f;
     }
-    const bool wide = ((d.a_stride | d.a_off | d.Kd) & 3) == 0 && (reinterpret_cast<uintptr_t>(d.a) & 15) == 0;
+    const bool wide = ((d.a_stride | d.a_off | d.Kd) & (kPer - 1)) == 0 && (reinterpret_cast<uintptr_t>(d.a) & (4 * kPer - 1)) == 0;
     const float* hidden = d.hidden + (tile.first_pair * d.comps + tile.row0) * R;
-    unsigned long long acc[4][Rp / 2];               // pairs of hidden columns
+    unsigned long long acc[kPer][Rp / 2];            // pairs of hidden columns
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
+    for (int q = 0; q < kPer; ++q)
 #pragma unroll
         for (int j = 0; j < Rp / 2; ++j) acc[q][j] = 0ull;
     constexpr int kAhead = 8;
@@ -820,34 +820,35 @@ __global__ void __launch_bounds__(kTsThreads, NH == 1 ? 4 : 2) adapter_grad_rows
         __syncthreads();
 #pragma unroll 1
         for (int g = 0; g < kStep / 4; g += kAhead) {            // rows warp + 4 g .. of the step
-            float4 a[kAhead];
+            float a[kAhead][kPer];
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
                 const int r = warp + 4 * (g + u);
-                a[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (r >= n) continue;
-                const float* from = d.a + a_base[r0 + r] + k;
+                const float* src = r < n ? d.a + a_base[r0 + r] + k : nullptr;
                 if (wide) {
-                    if (left > 0) a[u] = __ldg(reinterpret_cast<const float4*>(from));
+                    if constexpr (kPer == 4) {
+                        const float4 f = src && left > 0 ? __ldg(reinterpret_cast<const float4*>(src)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        a[u][0] = f.x; a[u][1] = f.y; a[u][2] = f.z; a[u][3] = f.w;
+                    } else {
+                        const float2 f = src && left > 0 ? __ldg(reinterpret_cast<const float2*>(src)) : make_float2(0.f, 0.f);
+                        a[u][0] = f.x; a[u][1] = f.y;
+                    }
                 } else {
-                    if (left > 0) a[u].x = __ldg(from);
-                    if (left > 1) a[u].y = __ldg(from + 1);
-                    if (left > 2) a[u].z = __ldg(from + 2);
-                    if (left > 3) a[u].w = __ldg(from + 3);
+#pragma unroll
+                    for (int q = 0; q < kPer; ++q) a[u][q] = src && q < left ? __ldg(src + q) : 0.f;
                 }
             }
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
                 const ulonglong2* h = reinterpret_cast<const ulonglong2*>(hs + (warp + 4 * (g + u)) * Rp);
-                const float v[4] = {a[u].x, a[u].y, a[u].z, a[u].w};
-                unsigned long long twice[4];
+                unsigned long long twice[kPer];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) asm("mov.b64 %0, {%1, %1};" : "=l"(twice[q]) : "f"(v[q]));
+                for (int q = 0; q < kPer; ++q) asm("mov.b64 %0, {%1, %1};" : "=l"(twice[q]) : "f"(a[u][q]));
 #pragma unroll
                 for (int j = 0; j < Rp / 4; ++j) {
                     const ulonglong2 two = h[j];
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
+                    for (int q = 0; q < kPer; ++q) {
                         asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc[q][2 * j]) : "l"(twice[q]), "l"(two.x));
                         asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc[q][2 * j + 1]) : "l"(twice[q]), "l"(two.y));
                     }
@@ -860,20 +861,20 @@ __global__ void __launch_bounds__(kTsThreads, NH == 1 ? 4 : 2) adapter_grad_rows
         __syncthreads();
         if (warp != turn) continue;
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
+        for (int q = 0; q < kPer; ++q)
 #pragma unroll
             for (int j = 0; j < Rp / 2; ++j) {
                 float x, y;
                 asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(acc[q][j]));
-                float* to = joined + (2 * j) * 128 + 4 * lane + q;
+                float* to = joined + (2 * j) * kCols + kPer * lane + q;
                 to[0] = turn ? to[0] + x : x;
-                to[128] = turn ? to[128] + y : y;
+                to[kCols] = turn ? to[kCols] + y : y;
             }
     }
     __syncthreads();
-    for (int i = tid; i < 128 * R; i += kTsThreads) {
+    for (int i = tid; i < kCols * R; i += kTsThreads) {
         const int kk = i / R, r = i - kk * R;
-        if (k_block * 128 + kk < d.Kd) d.part[(chunk_index * d.Kd + k_block * 128) * R + i] = joined[r * 128 + kk];
+        if (k_block * kCols + kk < d.Kd) d.part[(chunk_index * d.Kd + k_block * kCols) * R + i] = joined[r * kCols + kk];
     }
 }
 

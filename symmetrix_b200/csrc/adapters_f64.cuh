@@ -59,7 +59,8 @@ struct DpLayout {
 
 // A CTA of four warps (WM x WN) makes BM rows x BN columns of one degree and adapter: in . W and in . first_g from the same row fragments (the warps of
 // a row of warps share the inner values of the latter among them and add up through shared memory), then the weighted hidden rows times
-// second_g on top. ST stages of 16 inner values are in flight.
+// second_g on top. ST stages of 16 inner values are in flight. NR: hidden columns / 8; 0: shared weights alone, fewer registers and stages' bytes.
+// Without shared weights a CTA of big tiles makes all blocks of columns from one hidden tile.
 template <int BM, int BN, int WM, int WN, int NR, int ST>
 __global__ void __launch_bounds__(kDpThreads) adapter_pass_f64_kernel(const __grid_constant__ DpPass pass) {
     using L = DpLayout<BM, BN, NR, ST>;
@@ -77,7 +78,7 @@ __global__ void __launch_bounds__(kDpThreads) adapter_pass_f64_kernel(const __gr
         long long at = blockIdx.x;
         for (int q = 0; q < pass.degrees && hit < 0; ++q) {
             const DpDegree& d = pass.degree[q];
-            const int blocks = pass.out ? (d.Nc + BN - 1) / BN : 1;
+            const int blocks = pass.out && !(BM == 64 && !d.W) ? (d.Nc + BN - 1) / BN : 1;
             const long long row_tile = at / blocks;
             long long tiles;
             bool ok;
@@ -98,8 +99,9 @@ __global__ void __launch_bounds__(kDpThreads) adapter_pass_f64_kernel(const __gr
     __syncthreads();
     if (which < 0) return;
     const DpDegree& d = pass.degree[which];
-    const int rows = static_cast<int>(tile.rows), g = tile.group, R = pass.rank, col0 = col_block * BN, ldf = (R + 1) & ~1;
-    const bool adapter = g < pass.groups, shared = d.W && pass.out;
+    const int rows = static_cast<int>(tile.rows), g = tile.group, R = pass.rank, ldf = (R + 1) & ~1;
+    int col0 = col_block * BN;
+    const bool adapter = NR > 0 && g < pass.groups, shared = d.W && pass.out;
     for (int i = tid; i < BM; i += kDpThreads) {
         long long ib = -1, ob = -1, hr = 0;
         double w = 1.0;
@@ -146,26 +148,28 @@ __global__ void __launch_bounds__(kDpThreads) adapter_pass_f64_kernel(const __gr
             }
         if (adapter)
             for (int i = tid; i < kDpBK * 4 * NR; i += kDpThreads) {
-                const int k = i / (4 * NR), c = (i % (4 * NR)) * 2;
+                constexpr int per = NR > 0 ? 4 * NR : 1;
+                const int k = i / per, c = (i % per) * 2;
                 const int bytes = k0 + k < d.Kd && c < ldf ? 16 : 0;
                 dp_copy16(Fs + k * SF + c, first + (bytes ? static_cast<long long>(k0 + k) * ldf + c : 0), bytes);
             }
     };
     const int chunks = adapter || shared ? (d.Kd + kDpBK - 1) / kDpBK : 0;
-    if (adapter && pass.out) {
+    auto copy_second = [&]() {
         const double* second = d.second + g * d.second_group;
         for (int i = tid; i < 8 * NR * (BN / 2); i += kDpThreads) {
             const int r = i / (BN / 2), c = (i % (BN / 2)) * 2;
             const int bytes = r < R && col0 + c < d.ldw ? 16 : 0;
             dp_copy16(S2 + r * SB + c, second + (bytes ? static_cast<long long>(r) * d.ldw + col0 + c : 0), bytes);
         }
-    }
+    };
+    if (adapter && pass.out) copy_second();
 #pragma unroll
     for (int s = 0; s < ST - 1; ++s) {
         if (s < chunks) issue(s);
         cp_async_commit();
     }
-    double acc[MB][NB][2], hid[MB][NR][2];
+    double acc[MB][NB][2], hid[MB][NR > 0 ? NR : 1][2];
 #pragma unroll
     for (int i = 0; i < MB; ++i) {
 #pragma unroll
@@ -231,6 +235,11 @@ __global__ void __launch_bounds__(kDpThreads) adapter_pass_f64_kernel(const __gr
         }
         if (!pass.out) return;
         __syncthreads();
+    }
+    const bool out_wide = ((pass.out_stride | d.out_off | d.Nc) & 1) == 0 && (reinterpret_cast<uintptr_t>(pass.out) & 15) == 0;
+    const int end = BM == 64 && !d.W ? d.Nc : min(d.Nc, col0 + BN);
+    for (;;) {
+        if (adapter)
 #pragma unroll 2
         for (int r0 = 0; r0 < R; r0 += 4) {              // hidden columns beyond the rank are sums over zeros
             double a[MB];
@@ -243,23 +252,34 @@ __global__ void __launch_bounds__(kDpThreads) adapter_pass_f64_kernel(const __gr
                 for (int i = 0; i < MB; ++i) dmma_m8n8k4(acc[i][j][0], acc[i][j][1], a[i], b);
             }
         }
-    }
-    const bool out_wide = ((pass.out_stride | d.out_off | d.Nc) & 1) == 0 && (reinterpret_cast<uintptr_t>(pass.out) & 15) == 0;
 #pragma unroll
-    for (int i = 0; i < MB; ++i) {
-        const long long ob = out_base[wm * MB * 8 + i * 8 + fr];
-        if (ob < 0) continue;
+        for (int i = 0; i < MB; ++i) {
+            const long long ob = out_base[wm * MB * 8 + i * 8 + fr];
+            if (ob < 0) continue;
 #pragma unroll
-        for (int j = 0; j < NB; ++j) {
-            const int c = col0 + wn * NB * 8 + 8 * j + 2 * fk;
-            double* to = pass.out + ob + c;
-            if (out_wide && c < d.Nc) {
-                *reinterpret_cast<double2*>(to) = make_double2(acc[i][j][0], acc[i][j][1]);
-            } else {
-                if (c < d.Nc) to[0] = acc[i][j][0];
-                if (c + 1 < d.Nc) to[1] = acc[i][j][1];
+            for (int j = 0; j < NB; ++j) {
+                const int c = col0 + wn * NB * 8 + 8 * j + 2 * fk;
+                double* to = pass.out + ob + c;
+                if (out_wide && c < d.Nc) {
+                    *reinterpret_cast<double2*>(to) = make_double2(acc[i][j][0], acc[i][j][1]);
+                } else {
+                    if (c < d.Nc) to[0] = acc[i][j][0];
+                    if (c + 1 < d.Nc) to[1] = acc[i][j][1];
+                }
             }
         }
+        col0 += BN;
+        if (col0 >= end) break;
+        // the next block of columns of a tile without shared weights
+        __syncthreads();
+        if (adapter) copy_second();
+        cp_async_commit();
+        cp_async_wait<0>();
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+            for (int j = 0; j < NB; ++j) acc[i][j][0] = acc[i][j][1] = 0.0;
+        __syncthreads();
     }
 }
 

@@ -244,16 +244,19 @@ __global__ void __launch_bounds__(256) route_combine_kernel(const V* __restrict_
     }
 }
 
-// A warp per row; the row's gradient is read once for up to kSlotBlock slots.
+// A warp per row, or a CTA (kWarps = 8) where there are too few rows to fill the GPU with warps; the row's gradient is read once for up to
+// kSlotBlock slots.
 constexpr int kSlotBlock = 4;
-template <typename T, typename V>
+template <typename T, typename V, int kWarps>
 __global__ void __launch_bounds__(256) route_combine_backward_kernel(const V* __restrict__ grad_y, long long grad_y_stride, const V* __restrict__ rows,
                                                                      const int* __restrict__ position, const int* __restrict__ offsets, int groups,
                                                                      long long num_rows, int slots, int units, const T* __restrict__ weights,
                                                                      V* __restrict__ grad_rows, T* __restrict__ grad_weights, int zero_tail) {
     using L = Lanes<T, V>;
-    const int lane = threadIdx.x & 31;
-    const long long warp = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5, warps = (static_cast<long long>(gridDim.x) * blockDim.x) >> 5;
+    constexpr int kLanes = 32 * kWarps;
+    __shared__ T parts[kWarps][kSlotBlock];
+    const int lane = threadIdx.x % kLanes;
+    const long long warp = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) / kLanes, warps = static_cast<long long>(gridDim.x) * blockDim.x / kLanes;
     for (long long n = warp; n < num_rows; n += warps) {
         for (int s0 = 0; s0 < slots; s0 += kSlotBlock) {
             int p[kSlotBlock];
@@ -264,7 +267,7 @@ __global__ void __launch_bounds__(256) route_combine_backward_kernel(const V* __
                 w[q] = p[q] >= 0 ? (weights ? weights[n * slots + s0 + q] : T(1)) : T(0);
                 dot[q] = T(0);
             }
-            for (int u = lane; u < units; u += 32) {
+            for (int u = lane; u < units; u += kLanes) {
                 L g;
                 g.v = grad_y[n * grad_y_stride + u];
 #pragma unroll
@@ -287,7 +290,17 @@ __global__ void __launch_bounds__(256) route_combine_backward_kernel(const V* __
                 for (int q = 0; q < kSlotBlock; ++q) {
 #pragma unroll
                     for (int d = 16; d > 0; d >>= 1) dot[q] += __shfl_xor_sync(0xffffffffu, dot[q], d);
-                    if (lane == 0 && s0 + q < slots) grad_weights[n * slots + s0 + q] = dot[q];
+                    if (kWarps == 1 && lane == 0 && s0 + q < slots) grad_weights[n * slots + s0 + q] = dot[q];
+                    if (kWarps > 1 && (lane & 31) == 0) parts[lane >> 5][q] = dot[q];
+                }
+                if constexpr (kWarps > 1) {
+                    __syncthreads();
+                    if (lane < kSlotBlock && s0 + lane < slots) {
+                        T sum = T(0);
+                        for (int w = 0; w < kWarps; ++w) sum += parts[w][lane];
+                        grad_weights[n * slots + s0 + lane] = sum;
+                    }
+                    __syncthreads();
                 }
             }
         }
@@ -295,7 +308,7 @@ __global__ void __launch_bounds__(256) route_combine_backward_kernel(const V* __
     if (!zero_tail) return;
     const V zero{};
     for (long long p = offsets[groups] + warp; p < num_rows * slots; p += warps)
-        for (int u = lane; u < units; u += 32) grad_rows[p * units + u] = zero;
+        for (int u = lane; u < units; u += kLanes) grad_rows[p * units + u] = zero;
 }
 
 // ------------------------------------------------------------------------------------------- host side
@@ -455,10 +468,13 @@ void route_combine_backward(const T* grad_y, long grad_y_stride, const T* rows, 
     auto go = [&](auto unit) {
         using V = decltype(unit);
         constexpr long per = sizeof(V) / sizeof(T);
-        const unsigned grid = static_cast<unsigned>(std::max<long long>(1, std::min<long long>((num_rows + 7) / 8, 64LL * sm_count())));
-        route_combine_backward_kernel<T, V><<<grid, 256, 0, stream>>>(reinterpret_cast<const V*>(grad_y), grad_y_stride / per, reinterpret_cast<const V*>(rows),
-                                                                      position, offsets, num_groups, num_rows, slots, static_cast<int>(width / per), weights,
-                                                                      reinterpret_cast<V*>(grad_rows), grad_weights, zero_tail ? 1 : 0);
+        // CTAs of eight rows leave SMs without one below 8 x 4 x SMs rows
+        const bool few = num_rows < 32LL * sm_count() && width / per > 64;
+        const auto kernel = few ? route_combine_backward_kernel<T, V, 8> : route_combine_backward_kernel<T, V, 1>;
+        const unsigned grid = static_cast<unsigned>(std::max<long long>(1, std::min<long long>(few ? num_rows : (num_rows + 7) / 8, 64LL * sm_count())));
+        kernel<<<grid, 256, 0, stream>>>(reinterpret_cast<const V*>(grad_y), grad_y_stride / per, reinterpret_cast<const V*>(rows), position, offsets,
+                                         num_groups, num_rows, slots, static_cast<int>(width / per), weights, reinterpret_cast<V*>(grad_rows),
+                                         grad_weights, zero_tail ? 1 : 0);
     };
     if (wide_rows<T>({grad_y, rows, grad_rows}, {grad_y_stride, width})) go(typename Wide<T>::type{});
     else go(T{});
