@@ -131,7 +131,14 @@ __global__ void __launch_bounds__(256) adapter_grad_sum_kernel(const __grid_cons
     const long long size = static_cast<long long>(d.Kd) * R;
     for (long long i = static_cast<long long>(blockIdx.y) * 256 + threadIdx.x; i < size; i += 256LL * gridDim.y) {
         T s = T(0);
-        for (long long c = 0; c < chunks; ++c) s += d.part[(c0 + c) * size + i];
+        const T* part = d.part + c0 * size + i;
+        for (long long c = 0; c < chunks; c += 8) {                // eight loads in flight, added in order
+            T v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v[u] = c + u < chunks ? part[(c + u) * size] : T(0);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) s += v[u];
+        }
         d.grad[g * d.g_group + (i / R) * d.g_k + (i % R) * d.g_r] = s;
     }
 }
@@ -513,7 +520,14 @@ void launch_grads(const GradPass<float>& gp, int problems, cudaStream_t stream) 
     const int HP = padded_rank(gp.rank) / 16;
     if (HP <= 2) {
         const auto kernel = HP == 1 ? adapter_grad_rows_f32_kernel<1> : adapter_grad_rows_f32_kernel<2>;
-        kernel<<<static_cast<unsigned>(ctas), kTsThreads, 0, stream>>>(t);
+        const int smem = kGradChunk * 16 * HP * static_cast<int>(sizeof(float));          // at most 64 KB
+        static std::atomic<bool> done[64];
+        if (first_on_device(done)) {
+            for (const auto kern : {adapter_grad_rows_f32_kernel<1>, adapter_grad_rows_f32_kernel<2>})
+                SMX_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kGradChunk * 32 * static_cast<int>(sizeof(float))));
+            mark_on_device(done);
+        }
+        kernel<<<static_cast<unsigned>(ctas), kTsThreads, smem, stream>>>(t);
         launched("adapter_grad_rows_f32_kernel");
         return;
     }

@@ -763,14 +763,15 @@ struct TsGrad {
     const float* weights;
 };
 
-// Rank up to 32: part[chunk][k][r] = sum over the chunk's rows of a[row][k] (weight h)[row][r] on the FMA pipes, two hidden columns an instruction. A warp
-// takes a quarter of the rows, a lane four inner indices (two from rank 17 on: the sums of four would leave two CTAs an SM); the weighted hidden rows come from
-// shared memory. No tile is turned or split, so the rows stream through; on the tensor cores a product with 16 columns takes as long as one with 96.
+// Rank up to 32: part[chunk][k][r] = sum over the chunk's rows of (weight a)[row][k] h[row][r] on the FMA pipes, two hidden columns an instruction. The
+// chunk's hidden rows are copied to shared memory once; then every warp walks a quarter of the rows by itself, a lane with four inner indices
+// (two from rank 17 on: the sums of four would leave two CTAs an SM), four rows ahead. No tile is turned or split; on the tensor cores
+// a product with 16 columns takes as long as one with 96.
 template <int NH>                                    // hidden columns / 16
-__global__ void __launch_bounds__(kTsThreads, 4) adapter_grad_rows_f32_kernel(const __grid_constant__ TsGrad pass) {
-    constexpr int Rp = 16 * NH, kStep = 64, kPer = 4 / NH, kCols = 32 * kPer;         // inner indices of a lane, of the CTA
-    __shared__ __align__(16) float hs[kStep * Rp];
-    __shared__ __align__(16) float joined[kCols * Rp];
+__global__ void __launch_bounds__(kTsThreads, NH == 1 ? 4 : 3) adapter_grad_rows_f32_kernel(const __grid_constant__ TsGrad pass) {
+    constexpr int Rp = 16 * NH, kPer = 4 / NH, kCols = 32 * kPer, kAhead = 4;          // inner indices of a lane, of the CTA
+    extern __shared__ __align__(16) unsigned char ts_smem_raw[];
+    float* const hs = reinterpret_cast<float*>(ts_smem_raw);                             // [kGradChunk][Rp], afterwards the warps' sums [Rp][kCols]
     __shared__ long long a_base[kGradChunk];
     __shared__ float row_weight[kGradChunk];
     __shared__ TileRows tile;
@@ -795,6 +796,20 @@ __global__ void __launch_bounds__(kTsThreads, 4) adapter_grad_rows_f32_kernel(co
     if (which < 0) return;
     const GradProblem<float>& d = pass.problem[which];
     const int R = pass.rank, rows = static_cast<int>(tile.rows), k = k_block * kCols + kPer * lane, left = d.Kd - k;
+    const float* hidden = d.hidden + (tile.first_pair * d.comps + tile.row0) * R;
+    if ((R & 3) == 0) {                              // rows of hidden values follow one another: 16 bytes at a time
+        for (int i = tid; i < rows * (Rp / 4); i += kTsThreads) {
+            const int r = i / (Rp / 4), c = (i % (Rp / 4)) * 4;
+            cp_async16(hs + r * Rp + c, hidden + (c < R ? r * R + c : 0), c < R ? 16 : 0);
+        }
+    } else {
+        for (int i = tid; i < rows * Rp; i += kTsThreads) {
+            const int r = i / Rp, c = i % Rp;
+            if (c < R) cp_async4(hs + i, hidden + r * R + c);
+            else hs[i] = 0.f;
+        }
+    }
+    cp_async_commit();
     const long long q0 = tile.row0 / d.comps;
     const int m0 = static_cast<int>(tile.row0 - q0 * d.comps);
     for (int i = tid; i < rows; i += kTsThreads) {
@@ -803,60 +818,64 @@ __global__ void __launch_bounds__(kTsThreads, 4) adapter_grad_rows_f32_kernel(co
         row_weight[i] = pass.weights ? pass.weights[pair] : 1.f;
     }
     const bool wide = ((d.a_stride | d.a_off | d.Kd) & (kPer - 1)) == 0 && (reinterpret_cast<uintptr_t>(d.a) & (4 * kPer - 1)) == 0;
-    const float* hidden = d.hidden + (tile.first_pair * d.comps + tile.row0) * R;
     unsigned long long acc[kPer][Rp / 2];            // pairs of hidden columns
 #pragma unroll
     for (int q = 0; q < kPer; ++q)
 #pragma unroll
         for (int j = 0; j < Rp / 2; ++j) acc[q][j] = 0ull;
-    constexpr int kAhead = 8;
-    for (int r0 = 0; r0 < rows; r0 += kStep) {
-        const int n = min(kStep, rows - r0);
-        __syncthreads();
-        for (int i = tid; i < kStep * Rp; i += kTsThreads) {
-            const int r = i / Rp, c = i % Rp;
-            hs[i] = r < n && c < R ? __ldg(hidden + static_cast<long long>(r0 + r) * R + c) * row_weight[r0 + r] : 0.f;
-        }
-        __syncthreads();
-#pragma unroll 1
-        for (int g = 0; g < kStep / 4; g += kAhead) {            // rows warp + 4 g .. of the step
-            float a[kAhead][kPer];
+    cp_async_wait<0>();
+    __syncthreads();
+    auto load = [&](int r0, float (&a)[kAhead][kPer]) {          // rows r0, r0 + 4, ..
 #pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                const int r = warp + 4 * (g + u);
-                const float* src = r < n ? d.a + a_base[r0 + r] + k : nullptr;
-                if (wide) {
-                    if constexpr (kPer == 4) {
-                        const float4 f = src && left > 0 ? __ldg(reinterpret_cast<const float4*>(src)) : make_float4(0.f, 0.f, 0.f, 0.f);
-                        a[u][0] = f.x; a[u][1] = f.y; a[u][2] = f.z; a[u][3] = f.w;
-                    } else {
-                        const float2 f = src && left > 0 ? __ldg(reinterpret_cast<const float2*>(src)) : make_float2(0.f, 0.f);
-                        a[u][0] = f.x; a[u][1] = f.y;
-                    }
+        for (int u = 0; u < kAhead; ++u) {
+            const int r = r0 + 4 * u;
+            const float* src = r < rows ? d.a + a_base[r] + k : nullptr;
+            if (wide) {
+                if constexpr (kPer == 4) {
+                    const float4 f = src && left > 0 ? __ldg(reinterpret_cast<const float4*>(src)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    a[u][0] = f.x; a[u][1] = f.y; a[u][2] = f.z; a[u][3] = f.w;
                 } else {
-#pragma unroll
-                    for (int q = 0; q < kPer; ++q) a[u][q] = src && q < left ? __ldg(src + q) : 0.f;
+                    const float2 f = src && left > 0 ? __ldg(reinterpret_cast<const float2*>(src)) : make_float2(0.f, 0.f);
+                    a[u][0] = f.x; a[u][1] = f.y;
                 }
+            } else {
+#pragma unroll
+                for (int q = 0; q < kPer; ++q) a[u][q] = src && q < left ? __ldg(src + q) : 0.f;
             }
+        }
+    };
+    auto add = [&](int r0, const float (&a)[kAhead][kPer]) {
 #pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                const ulonglong2* h = reinterpret_cast<const ulonglong2*>(hs + (warp + 4 * (g + u)) * Rp);
-                unsigned long long twice[kPer];
+        for (int u = 0; u < kAhead; ++u) {
+            const int r = r0 + 4 * u;
+            if (r >= rows) break;
+            const ulonglong2* h = reinterpret_cast<const ulonglong2*>(hs + r * Rp);
+            const float w = row_weight[r];
+            unsigned long long twice[kPer];
 #pragma unroll
-                for (int q = 0; q < kPer; ++q) asm("mov.b64 %0, {%1, %1};" : "=l"(twice[q]) : "f"(a[u][q]));
+            for (int q = 0; q < kPer; ++q) asm("mov.b64 %0, {%1, %1};" : "=l"(twice[q]) : "f"(w * a[u][q]));
 #pragma unroll
-                for (int j = 0; j < Rp / 4; ++j) {
-                    const ulonglong2 two = h[j];
+            for (int j = 0; j < Rp / 4; ++j) {
+                const ulonglong2 two = h[j];
 #pragma unroll
-                    for (int q = 0; q < kPer; ++q) {
-                        asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc[q][2 * j]) : "l"(twice[q]), "l"(two.x));
-                        asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc[q][2 * j + 1]) : "l"(twice[q]), "l"(two.y));
-                    }
+                for (int q = 0; q < kPer; ++q) {
+                    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc[q][2 * j]) : "l"(twice[q]), "l"(two.x));
+                    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc[q][2 * j + 1]) : "l"(twice[q]), "l"(two.y));
                 }
             }
         }
+    };
+    float a0[kAhead][kPer], a1[kAhead][kPer];
+    load(warp, a0);
+#pragma unroll 1
+    for (int r0 = warp; r0 < rows; r0 += 8 * kAhead) {
+        load(r0 + 4 * kAhead, a1);
+        add(r0, a0);
+        load(r0 + 8 * kAhead, a0);
+        add(r0 + 4 * kAhead, a1);
     }
     // the warps' sums in turn
+    float* const joined = hs;
     for (int turn = 0; turn < 4; ++turn) {
         __syncthreads();
         if (warp != turn) continue;
