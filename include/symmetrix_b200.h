@@ -320,7 +320,8 @@ int smx_energy_virial_noalloc(const double* node_energies, int num_nodes, const 
  * are left as they were, or zeroed with `zero_tail` != 0. Sorted rows are contiguous, the others have a row stride in elements.
  * `precision` (SMX_FP32 or SMX_FP64) is the type of all values, and of the sums.
  * These calls need no evaluator: all pointers are device pointers on the current GPU, work is issued on `stream` (a cudaStream_t, may be
- * NULL), nothing is allocated and nothing waits, so they can be captured into a graph. The plan of more than 8,192 pairs needs a
+ * NULL), nothing is allocated and nothing waits, so they can be captured into a graph (the first call of a kind on a GPU, which sets the
+ * attributes of its kernels, comes before). The plan of more than 8,192 pairs needs a
  * workspace of smx_route_plan_bytes bytes; calls that may overlap on the device need one each. The same call gives the same bits.
  * Limits: num_groups and slots as below, num_rows * slots below 2^31 - 2^11. Messages go to `errbuf` (capacity `errbuf_len`, may be
  * NULL); smx_route_plan_bytes returns -1 for sizes that smx_route_plan refuses. */
@@ -351,7 +352,8 @@ int smx_route_combine_backward(int precision, const void* grad_y, long grad_y_st
  * smx_adapter_backward reads grad_y, x (and hidden) and writes, each unless NULL, grad_x, the degrees' grad_down / grad_up (both, for all
  * degrees or none; groups without atoms get zeros) and grad_weights [num_rows][slots] (zero in empty slots). The shared weights are
  * frozen: they have no gradient here.
- * float32: products on the tensor cores from operands split in two (3xTF32), sums in float32; float64 throughout otherwise. Sums over
+ * float32: products on the tensor cores from operands split in two (3xTF32), sums in float32, for magnitudes up to 2^127 (infinities in x or
+ * the matrices give NaN); float64 throughout otherwise. Sums over
  * atoms are split into chunks of a fixed number of rows and added in order: the same call gives the same bits.
  * The rules of the smx_route_* calls hold: device pointers on the current GPU, `stream`, no allocation, no wait, a workspace of
  * smx_adapter_workspace_bytes bytes for each call that may overlap with another one, errors through `errbuf`. The size functions

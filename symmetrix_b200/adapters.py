@@ -3,8 +3,8 @@
 ``RowRouting`` sorts the rows of per-atom arrays by group (``smx_route_*``), ``AdapterLinear`` is a channel-mixing linear of all degrees with
 every atom's own low-rank adapter, or weighted mixture of adapters, beside the shared weights (``smx_adapter_*``). Both work on CUDA tensors
 (float32 or float64) and issue their work on torch's current stream of the tensors' device. Nothing waits for the GPU, so both can be captured
-into CUDA graphs. They are not recorded by autograd: the backward passes are methods, and inputs that require gradients are refused while
-torch records.
+into CUDA graphs (the first call of a kind on a GPU comes before a capture). They are not recorded by autograd: the backward passes are
+methods, and inputs that require gradients are refused while torch records.
 
 Rows may have any stride between atoms; other strides than one inside a row are copied first.
 """
@@ -38,6 +38,13 @@ def _call(fn, index: int, *args) -> None:
             status = fn(*args, _errors.buffer, 256)
     if status != _lib.SMX_OK:
         raise SymmetrixError(status, _errors.buffer.value.decode())
+
+
+def _stream(index: int) -> int:
+    """The handle of torch's current stream on device `index`."""
+    import torch
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)       # without making a Stream object, a tenth of the time
+    return raw(index) if raw is not None else torch.cuda.current_stream(index).cuda_stream
 
 
 def _precision(dtype) -> int:
@@ -123,7 +130,7 @@ class RowRouting:
         self._plan = ids.new_empty(2 * self._pairs + self.num_groups + 1)
         base = self._plan.data_ptr()
         self._order, self._position, self._offsets = base, base + 4 * self._pairs, base + 8 * self._pairs
-        self._home = torch.cuda.current_stream(self._index).cuda_stream
+        self._home = _stream(self._index)
         self._make(ids)
 
     @property
@@ -155,17 +162,16 @@ class RowRouting:
 
     def _use(self) -> int:
         """The current stream; the plan's memory stays until its work is done there, wherever the plan was made."""
-        import torch
-        stream = torch.cuda.current_stream(self._index)
-        handle = stream.cuda_stream
+        handle = _stream(self._index)
         if handle != self._home:
-            self._plan.record_stream(stream)
+            import torch
+            self._plan.record_stream(torch.cuda.current_stream(self._index))
         return handle
 
     def _weights(self, weights, dtype):
         if weights is None:
             return None
-        shape = (self.num_rows,) if self.slots == 1 and weights.dim() == 1 else (self.num_rows, self.slots)
+        shape = (self.num_rows,) if self.slots == 1 and getattr(weights, "ndim", 2) == 1 else (self.num_rows, self.slots)
         return _values(weights, "weights", shape, dtype, self.device).contiguous()
 
     def dispatch(self, x, out=None):
@@ -259,7 +265,7 @@ class AdapterLinear:
         if need < 0:
             raise ValueError("the sizes exceed what smx_adapter_forward supports")
         self._index = self.device.index
-        self._home = torch.cuda.current_stream(self._index).cuda_stream
+        self._home = _stream(self._index)
         self._tiles = torch.empty(need, dtype=torch.uint8, device=self.device)
         f.tiles = self._tiles.data_ptr()
         self.set_adapters(down, up)
@@ -300,11 +306,10 @@ class AdapterLinear:
         return call
 
     def _use(self) -> int:
-        import torch
-        stream = torch.cuda.current_stream(self._index)
-        handle = stream.cuda_stream
+        handle = _stream(self._index)
         if handle != self._home:
-            self._tiles.record_stream(stream)
+            import torch
+            self._tiles.record_stream(torch.cuda.current_stream(self._index))
         return handle
 
     def _begin(self, routing, weights):

@@ -511,28 +511,20 @@ void launch_grads(const GradPass<float>& gp, int problems, cudaStream_t stream) 
     long long ctas = 0;
     for (int q = 0; q < problems; ++q) {
         t.problem[q] = gp.problem[q];
-        const int cols = padded_rank(gp.rank) == 32 ? 64 : 128;
-        ctas += (gp.pairs * gp.problem[q].comps / kGradChunk + gp.groups) * ((gp.problem[q].Kd + cols - 1) / cols);
+        ctas += (gp.pairs * gp.problem[q].comps / kGradChunk + gp.groups) * ts_blocks(gp.problem[q].Kd);
     }
     t.problems = problems; t.rank = gp.rank; t.groups = gp.groups; t.slots = gp.slots; t.pairs = gp.pairs;
     t.order = gp.order; t.offsets = gp.offsets; t.weights = gp.weights;
     if (ctas > INT_MAX) throw ArgError("smx_adapter: too many rows");
-    const int HP = padded_rank(gp.rank) / 16;
-    if (HP <= 2) {
-        const auto kernel = HP == 1 ? adapter_grad_rows_f32_kernel<1> : adapter_grad_rows_f32_kernel<2>;
-        const int smem = kGradChunk * 16 * HP * static_cast<int>(sizeof(float));          // at most 64 KB
-        static std::atomic<bool> done[64];
-        if (first_on_device(done)) {
-            for (const auto kern : {adapter_grad_rows_f32_kernel<1>, adapter_grad_rows_f32_kernel<2>})
-                SMX_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kGradChunk * 32 * static_cast<int>(sizeof(float))));
-            mark_on_device(done);
-        }
-        kernel<<<static_cast<unsigned>(ctas), kTsThreads, smem, stream>>>(t);
-        launched("adapter_grad_rows_f32_kernel");
-        return;
+    const int NH = padded_rank(gp.rank) / 16;
+    static std::atomic<bool> done[64];
+    if (first_on_device(done)) {
+        for (const auto kern : {adapter_grad_f32_kernel<1>, adapter_grad_f32_kernel<2>, adapter_grad_f32_kernel<3>, adapter_grad_f32_kernel<4>})
+            SMX_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kGradChunk * 64 * static_cast<int>(sizeof(float))));
+        mark_on_device(done);
     }
-    const auto kernel = HP == 3 ? adapter_grad_f32_kernel<3> : adapter_grad_f32_kernel<4>;
-    kernel<<<static_cast<unsigned>(ctas), kTsThreads, 16 * HP * 256 + 1024, stream>>>(t);
+    const auto kernel = NH == 1 ? adapter_grad_f32_kernel<1> : NH == 2 ? adapter_grad_f32_kernel<2> : NH == 3 ? adapter_grad_f32_kernel<3> : adapter_grad_f32_kernel<4>;
+    kernel<<<static_cast<unsigned>(ctas), kTsThreads, kGradChunk * 16 * NH * static_cast<int>(sizeof(float)), stream>>>(t);
     launched("adapter_grad_f32_kernel");
 }
 

@@ -763,13 +763,15 @@ struct TsGrad {
     const float* weights;
 };
 
-// Rank up to 32: part[chunk][k][r] = sum over the chunk's rows of (weight a)[row][k] h[row][r] on the FMA pipes, two hidden columns an instruction. The
-// chunk's hidden rows are copied to shared memory once; then every warp walks a quarter of the rows by itself, a lane with four inner indices
-// (two from rank 17 on: the sums of four would leave two CTAs an SM), four rows ahead. No tile is turned or split; on the tensor cores
-// a product with 16 columns takes as long as one with 96.
+// part[chunk][k][r] = sum over the chunk's rows of (weight a)[row][k] h[row][r] on the FMA pipes, two hidden columns an instruction. The chunk's
+// hidden rows are copied to shared memory once; then every warp walks its rows by itself, a lane with four inner indices and 16 hidden columns
+// (the warps of a CTA share out first the hidden columns, then the rows), four rows ahead. On the tensor cores a product with 16 columns
+// takes as long as one with 96, and the rows would have to be turned and split: 177 us where this takes 92 (8,001 atoms behind the tensor
+// product, rank 16; FMA pipes 40 % busy, issue slots 44 %).
 template <int NH>                                    // hidden columns / 16
-__global__ void __launch_bounds__(kTsThreads, NH == 1 ? 4 : 3) adapter_grad_rows_f32_kernel(const __grid_constant__ TsGrad pass) {
-    constexpr int Rp = 16 * NH, kPer = 4 / NH, kCols = 32 * kPer, kAhead = 4;          // inner indices of a lane, of the CTA
+__global__ void __launch_bounds__(kTsThreads, NH == 4 ? 3 : 4) adapter_grad_f32_kernel(const __grid_constant__ TsGrad pass) {
+    constexpr int Rp = 16 * NH, kPer = 4, kCols = 32 * kPer, kAhead = 4;               // inner indices of a lane, of the CTA
+    constexpr int kRowWarps = NH == 1 ? 4 : NH == 2 ? 2 : 1;                             // warps that share the rows of 16 hidden columns
     extern __shared__ __align__(16) unsigned char ts_smem_raw[];
     float* const hs = reinterpret_cast<float*>(ts_smem_raw);                             // [kGradChunk][Rp], afterwards the warps' sums [Rp][kCols]
     __shared__ long long a_base[kGradChunk];
@@ -777,7 +779,7 @@ __global__ void __launch_bounds__(kTsThreads, NH == 1 ? 4 : 3) adapter_grad_rows
     __shared__ TileRows tile;
     __shared__ int which, k_block;
     __shared__ long long chunk_index;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, col16 = 16 * (warp / kRowWarps);
     if (warp == 0) {
         long long t = blockIdx.x, tiles = 0;
         TileRows rows{};
@@ -818,26 +820,21 @@ __global__ void __launch_bounds__(kTsThreads, NH == 1 ? 4 : 3) adapter_grad_rows
         row_weight[i] = pass.weights ? pass.weights[pair] : 1.f;
     }
     const bool wide = ((d.a_stride | d.a_off | d.Kd) & (kPer - 1)) == 0 && (reinterpret_cast<uintptr_t>(d.a) & (4 * kPer - 1)) == 0;
-    unsigned long long acc[kPer][Rp / 2];            // pairs of hidden columns
+    unsigned long long acc[kPer][8];                 // pairs of hidden columns
 #pragma unroll
     for (int q = 0; q < kPer; ++q)
 #pragma unroll
-        for (int j = 0; j < Rp / 2; ++j) acc[q][j] = 0ull;
+        for (int j = 0; j < 8; ++j) acc[q][j] = 0ull;
     cp_async_wait<0>();
     __syncthreads();
-    auto load = [&](int r0, float (&a)[kAhead][kPer]) {          // rows r0, r0 + 4, ..
+    auto load = [&](int r0, float (&a)[kAhead][kPer]) {          // rows r0, r0 + kRowWarps, ..
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-            const int r = r0 + 4 * u;
+            const int r = r0 + kRowWarps * u;
             const float* src = r < rows ? d.a + a_base[r] + k : nullptr;
             if (wide) {
-                if constexpr (kPer == 4) {
-                    const float4 f = src && left > 0 ? __ldg(reinterpret_cast<const float4*>(src)) : make_float4(0.f, 0.f, 0.f, 0.f);
-                    a[u][0] = f.x; a[u][1] = f.y; a[u][2] = f.z; a[u][3] = f.w;
-                } else {
-                    const float2 f = src && left > 0 ? __ldg(reinterpret_cast<const float2*>(src)) : make_float2(0.f, 0.f);
-                    a[u][0] = f.x; a[u][1] = f.y;
-                }
+                const float4 f = src && left > 0 ? __ldg(reinterpret_cast<const float4*>(src)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                a[u][0] = f.x; a[u][1] = f.y; a[u][2] = f.z; a[u][3] = f.w;
             } else {
 #pragma unroll
                 for (int q = 0; q < kPer; ++q) a[u][q] = src && q < left ? __ldg(src + q) : 0.f;
@@ -847,15 +844,15 @@ __global__ void __launch_bounds__(kTsThreads, NH == 1 ? 4 : 3) adapter_grad_rows
     auto add = [&](int r0, const float (&a)[kAhead][kPer]) {
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-            const int r = r0 + 4 * u;
+            const int r = r0 + kRowWarps * u;
             if (r >= rows) break;
-            const ulonglong2* h = reinterpret_cast<const ulonglong2*>(hs + r * Rp);
+            const ulonglong2* h = reinterpret_cast<const ulonglong2*>(hs + r * Rp + col16);
             const float w = row_weight[r];
             unsigned long long twice[kPer];
 #pragma unroll
             for (int q = 0; q < kPer; ++q) asm("mov.b64 %0, {%1, %1};" : "=l"(twice[q]) : "f"(w * a[u][q]));
 #pragma unroll
-            for (int j = 0; j < Rp / 4; ++j) {
+            for (int j = 0; j < 4; ++j) {
                 const ulonglong2 two = h[j];
 #pragma unroll
                 for (int q = 0; q < kPer; ++q) {
@@ -866,26 +863,28 @@ __global__ void __launch_bounds__(kTsThreads, NH == 1 ? 4 : 3) adapter_grad_rows
         }
     };
     float a0[kAhead][kPer], a1[kAhead][kPer];
-    load(warp, a0);
+    const bool idle = col16 >= Rp;                   // three blocks of hidden columns leave a warp without one
+    const int first_row = idle ? rows : warp % kRowWarps;
+    load(first_row, a0);
 #pragma unroll 1
-    for (int r0 = warp; r0 < rows; r0 += 8 * kAhead) {
-        load(r0 + 4 * kAhead, a1);
+    for (int r0 = first_row; r0 < rows; r0 += 2 * kRowWarps * kAhead) {
+        load(r0 + kRowWarps * kAhead, a1);
         add(r0, a0);
-        load(r0 + 8 * kAhead, a0);
-        add(r0 + 4 * kAhead, a1);
+        load(r0 + 2 * kRowWarps * kAhead, a0);
+        add(r0 + kRowWarps * kAhead, a1);
     }
     // the warps' sums in turn
     float* const joined = hs;
-    for (int turn = 0; turn < 4; ++turn) {
+    for (int turn = 0; turn < kRowWarps; ++turn) {
         __syncthreads();
-        if (warp != turn) continue;
+        if (idle || warp % kRowWarps != turn) continue;
 #pragma unroll
         for (int q = 0; q < kPer; ++q)
 #pragma unroll
-            for (int j = 0; j < Rp / 2; ++j) {
+            for (int j = 0; j < 8; ++j) {
                 float x, y;
                 asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(acc[q][j]));
-                float* to = joined + (2 * j) * kCols + kPer * lane + q;
+                float* to = joined + (col16 + 2 * j) * kCols + kPer * lane + q;
                 to[0] = turn ? to[0] + x : x;
                 to[kCols] = turn ? to[kCols] + y : y;
             }
@@ -895,144 +894,6 @@ __global__ void __launch_bounds__(kTsThreads, NH == 1 ? 4 : 3) adapter_grad_rows
         const int kk = i / R, r = i - kk * R;
         if (k_block * kCols + kk < d.Kd) d.part[(chunk_index * d.Kd + k_block * kCols) * R + i] = joined[r * kCols + kk];
     }
-}
-
-// Higher ranks, on the tensor cores: D[k, r] = sum over rows a[row][k] (w h)[row][r]. A thread owns an inner index k of 128 and
-// loads a[row][k] of 32 rows (a warp reads 128 consecutive bytes of each), which is the row operand's transpose for nothing; the hidden values
-// are split into shared memory. The sums of every 32 rows are added in registers, as in the pass kernel.
-constexpr int kTsGradColumns = 128, kTsGradSlot = 64;
-template <int HP>
-__global__ void __launch_bounds__(kTsThreads, HP > 2 ? 2 : HP == 2 ? 3 : 4) adapter_grad_f32_kernel(const __grid_constant__ TsGrad pass) {
-    extern __shared__ unsigned char ts_smem_raw[];
-    __shared__ __align__(8) unsigned long long mma_bar;
-    __shared__ uint32_t tmem_slot;
-    __shared__ long long a_base[kGradChunk];
-    __shared__ float row_weight[kGradChunk];
-    __shared__ TileRows tile;
-    __shared__ int which, found, failed, k_block;
-    __shared__ long long chunk_index;
-    const int tid = threadIdx.x, warp = tid >> 5;
-    if (warp == 0) {
-        long long t = blockIdx.x, tiles = 0;
-        TileRows rows{};
-        int hit = -1, kb = 0;
-        for (int q = 0; q < pass.problems; ++q) {
-            const int blocks = (pass.problem[q].Kd + 127) / 128;
-            if (find_tile(pass.offsets, pass.groups, false, pass.pairs, pass.problem[q].comps, kGradChunk, t / blocks, rows, tiles)) {
-                hit = q; kb = static_cast<int>(t % blocks); t /= blocks;
-                break;
-            }
-            t -= tiles * blocks;
-        }
-        if (tid == 0) { which = hit; found = hit >= 0; k_block = kb; chunk_index = t; tile = rows; failed = 0; }
-    }
-    __syncthreads();
-    if (!found) return;
-    const GradProblem<float>& d = pass.problem[which];
-    constexpr int Rp = 16 * HP;
-    const int R = pass.rank, rows = static_cast<int>(tile.rows), k = k_block * 128 + tid;
-    if (warp == 0) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(kTsGradColumns) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    for (int i = tid; i < kGradChunk; i += kTsThreads) {
-        long long base = -1;
-        float w = 0.f;
-        if (i < rows) {
-            const long long r = tile.row0 + i;
-            const int pair = pass.order[tile.first_pair + r / d.comps];
-            base = static_cast<long long>(pair / pass.slots) * d.a_stride + d.a_off + (r % d.comps) * d.Kd;
-            w = pass.weights ? pass.weights[pair] : 1.f;
-        }
-        a_base[i] = base;
-        row_weight[i] = w;
-    }
-    unsigned char* B = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(ts_smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    for (int i = tid; i < Rp * 16; i += kTsThreads) reinterpret_cast<float4*>(B)[i] = make_float4(0.f, 0.f, 0.f, 0.f);      // padding rows stay zero
-    if (tid == 0) {
-        mbar_init(&mma_bar, 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    ts_fence_before();
-    __syncthreads();
-    ts_fence_after();
-    const uint32_t tmem = tmem_slot, lanes = tmem + (static_cast<uint32_t>(warp * 32) << 16);
-    const float* hidden = d.hidden + (tile.first_pair * d.comps + tile.row0) * R;
-    const int hid_values = 32 * R;
-    float a[32], h[4 * HP];
-    auto load = [&](int s) {
-#pragma unroll
-        for (int q = 0; q < 32; ++q) {
-            const int i = s * 32 + q;
-            a[q] = i < rows && k < d.Kd ? __ldg(d.a + a_base[i] + k) : 0.f;
-        }
-#pragma unroll
-        for (int q = 0; q < 4 * HP; ++q) {
-            const int e = tid + q * kTsThreads;
-            h[q] = e < hid_values && s * 32 + e / R < rows ? __ldg(hidden + static_cast<long long>(s) * hid_values + e) * row_weight[s * 32 + e / R] : 0.f;
-        }
-    };
-    const int steps = (rows + 31) / 32;
-    float sum[Rp];
-#pragma unroll
-    for (int q = 0; q < Rp; ++q) sum[q] = 0.f;
-    auto add_step = [&](int s) {                     // the sums of step s into registers
-        if (!*reinterpret_cast<volatile int*>(&failed) && !mbar_wait(&mma_bar, s & 1)) atomicMax(&failed, 1);
-        __syncwarp();
-        ts_fence_after();
-#pragma unroll
-        for (int r0 = 0; r0 < Rp; r0 += 16) {
-            float v[16];
-            ts_load16(lanes + r0, v);
-#pragma unroll
-            for (int q = 0; q < 16; ++q) sum[r0 + q] += v[q];
-        }
-    };
-    load(0);
-    for (int s = 0; s < steps; ++s) {
-        if (s > 0) add_step(s - 1);
-        float lo[32];
-#pragma unroll
-        for (int q = 0; q < 32; ++q) ts_split(a[q], a[q], lo[q]);
-        ts_store32(lanes + kTsGradSlot, a);
-        ts_store32(lanes + kTsGradSlot + 32, lo);
-#pragma unroll
-        for (int q = 0; q < 4 * HP; ++q) {
-            const int e = tid + q * kTsThreads;
-            if (e < hid_values) {
-                const int i = e / R, r = e % R;
-                float hi, l;
-                ts_split(h[q], hi, l);
-                const int off = tc5_swizzled_group(r, i >> 2) + (i & 3) * 4;
-                *reinterpret_cast<float*>(B + off) = hi;
-                *reinterpret_cast<float*>(B + Rp * 128 + off) = l;
-            }
-        }
-        if (s + 1 < steps) load(s + 1);
-        ts_wait_store();
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        ts_fence_before();
-        __syncthreads();
-        if (tid == 0 && !*reinterpret_cast<volatile int*>(&failed)) {
-            ts_fence_after();
-            const uint32_t b = smem_u32(B);
-            ts_chunk(tmem, tmem + kTsGradSlot, tmem + kTsGradSlot + 32, b, b + Rp * 128, ts_idesc(Rp), 4, false);
-            ts_commit(&mma_bar);
-        }
-    }
-    __syncthreads();
-    add_step(steps - 1);
-    __syncthreads();
-    const bool bad = *reinterpret_cast<volatile int*>(&failed) != 0;
-    if (k < d.Kd) {
-        float* to = d.part + (chunk_index * d.Kd + k) * R;
-#pragma unroll
-        for (int q = 0; q < Rp; ++q)
-            if (q < R) to[q] = bad ? NAN : sum[q];
-    }
-    ts_fence_before();
-    __syncthreads();
-    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTsGradColumns) : "memory");
 }
 
 }  // namespace

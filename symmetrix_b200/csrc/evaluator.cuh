@@ -975,7 +975,6 @@ public:
     // several, added to the linear's weights (csrc/adapters.cu). A linear without them, or an evaluator without an assignment, runs the model.
     struct AdapterSet {
         int rank = 0;
-        std::vector<std::unique_ptr<DevBuf<T>>> down, up;         // per degree, only until they are laid out
         DevBuf<unsigned char> tiles;
         DevBuf<T> hidden;                                         // in . down of the last forward pass, for the gradients
         int hidden_nodes = -1;

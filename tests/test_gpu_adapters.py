@@ -443,6 +443,46 @@ def test_linear_refusals():
             bad()
 
 
+def test_offsets_beyond_32_bits():
+    """Arrays of more than 2^32 bytes and 2^31 values: rows at both ends against their definition."""
+    n, width = 270_001, 8192
+    ids = (torch.arange(n, device="cuda", dtype=torch.int32) * 7) % 5
+    ids[::11] = -1
+    routing = RowRouting(ids, 5)
+    order, position, offsets = plan_of(ids[:, None], 5)
+    x = torch.randn(n, width, device="cuda")
+    rows = routing.dispatch(x)
+    probe = [0, 1, n // 2, n - 2, n - 1]
+    for r in probe:
+        p = int(position[r, 0])
+        if p >= 0:
+            assert torch.equal(rows[p], x[r])
+    assert (rows[int(offsets[-1]):] == 0).all()
+    y = routing.combine(rows, base=x)
+    grad_rows, grad_weights = routing.combine_backward(x, rows)
+    for r in probe:
+        assert torch.equal(y[r], 2 * x[r] if position[r, 0] >= 0 else x[r])
+        if position[r, 0] >= 0:
+            assert torch.equal(grad_rows[int(position[r, 0])], x[r])
+            exact = (x[r].double() ** 2).sum().item()
+            assert abs(grad_weights[r, 0].item() - exact) <= width * 2.0 ** -23 * exact
+    del x, rows, y, grad_rows
+    n = 2 ** 31 // 128 + 5
+    for dtype in (torch.float32, torch.float64):
+        gen = torch.Generator("cuda").manual_seed(1)
+        rand = lambda *s: torch.randn(*s, generator=gen, device="cuda", dtype=dtype)  # noqa: E731
+        ids = torch.arange(n, device="cuda", dtype=torch.int32) % 3
+        shared, down, up = rand(128, 32), rand(3, 128, 4) / 11, rand(3, 4, 32)
+        x = rand(n, 128)
+        y = AdapterLinear([shared], [down], [up]).forward(x, RowRouting(ids, 3))
+        for r in (0, n // 2, n - 1):
+            g = int(ids[r])
+            v, w, a, b = host(x[r]), host(shared), host(down[g]), host(up[g])
+            size = np.abs(v) @ np.abs(w) + np.abs(v) @ np.abs(a) @ np.abs(b)
+            assert (np.abs(host(y[r]) - v @ w - v @ a @ b) <= (128 + 4 + 24) * EPS[dtype] * size).all()
+        del x, y
+
+
 # ------------------------------------------------------------------------------------------- used together
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
