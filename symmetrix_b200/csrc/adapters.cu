@@ -6,9 +6,9 @@
 // The backward pass to x is the forward pass with the transposed matrices, so one kernel does both.
 //
 // Rows are taken in the order of the routing (csrc/routing.cu), in tiles that never mix groups. With one slot a row belongs to one tile: the
-// tile's kernel makes the shared product, its own adapter's and their sum, so x is read and y is written once. With more slots the shared product
-// runs over all rows, the adapters' products go to a workspace in sorted order, and the routing's combine adds them to the output in slot
-// order. Sums over rows (gA, gB) are split into chunks of a fixed number of rows, whose partial sums are added in order: no atomics.
+// tile's kernel makes the shared product, its own adapter's and their sum, so x is read and y is written once. With more slots the plan is split
+// by slot: the first slot's pass is that of one slot, the others' add their products to the rows it wrote, in slot order (a row is in one
+// tile of a slot's pass, so nothing races). Sums over rows (gA, gB) are split into chunks of a fixed number of rows, whose partial sums are added in order: no atomics.
 #include "adapters.hpp"
 
 #include <cuda_runtime.h>
@@ -39,13 +39,13 @@ template <typename T>
 struct Pass {
     PassDegree<T> degree[kMaxDegrees];
     int rank, groups, slots;
-    long long num_rows, pairs;
+    long long pairs;                                 // places in all
     const int* order; const int* offsets;
+    const int* places;                               // of a slot (csrc/routing.hpp), with its offsets; null: the plan itself
     const T* weights;
     const T* in; long long in_stride;
     T* out; long long out_stride;                    // null: only the hidden rows
-    int sorted;        // tiles by group, atoms through `order`; else all rows in their own order and no adapters
-    int out_sorted;    // out rows by sorted position (workspace), else by atom
+    int add;           // to `out`, instead of writing it
     int tail;          // the rows without a group are a last group of their own
 };
 
@@ -227,7 +227,7 @@ void check_rows(const char* what, const void* p, long stride, long width, long r
     if (stride < 0 || (written && rows > 1 && stride < width)) throw ArgError(std::string("smx_adapter: bad row stride of ") + what);
 }
 
-// Workspace: hidden rows of both directions (backward), sorted products (several slots), partial sums (backward); parts start on 256 bytes.
+// Workspace: the plan by slots (several slots), hidden rows of both directions and partial sums (backward); parts start on 256 bytes.
 struct Workspace {
     char* base;
     size_t used = 0;
@@ -245,7 +245,8 @@ long long grad_chunks(const smx_adapter_linear& c, int comps) {
 
 template <typename T>
 struct Buffers {
-    T* back_hidden = nullptr; T* hidden = nullptr; T* products = nullptr; T* parts[2 * kMaxDegrees] = {};
+    T* back_hidden = nullptr; T* hidden = nullptr; T* parts[2 * kMaxDegrees] = {};
+    int* places = nullptr; int* slot_offsets = nullptr; void* scratch = nullptr;
     size_t bytes = 0;
 };
 template <typename T>
@@ -254,7 +255,11 @@ Buffers<T> lay_out(const smx_adapter_linear& c, bool backward) {
     Workspace ws{static_cast<char*>(c.workspace)};
     const Widths w = widths(c);
     const size_t pairs = static_cast<size_t>(c.num_rows) * c.slots;
-    if (c.slots > 1) b.products = ws.take<T>(pairs * (backward ? std::max(w.in, w.out) : w.out));
+    if (c.slots > 1) {
+        b.places = ws.take<int>(pairs);
+        b.slot_offsets = ws.take<int>(static_cast<size_t>(c.slots) * (c.num_groups + 1));
+        b.scratch = ws.take<char>(route_slots_bytes(c.num_rows, c.slots));
+    }
     if (backward) {
         b.back_hidden = ws.take<T>(pairs * w.comps * c.rank);
         if (!c.hidden) b.hidden = ws.take<T>(pairs * w.comps * c.rank);
@@ -395,7 +400,7 @@ Pass<T> make_pass(const smx_adapter_linear& c, bool transposed, T* hidden) {
         out_off += static_cast<long long>(g.components) * d.Nc;
     }
     p.rank = c.rank; p.groups = c.num_groups; p.slots = c.slots;
-    p.num_rows = c.num_rows; p.pairs = static_cast<long long>(pairs);
+    p.pairs = static_cast<long long>(pairs);
     p.order = c.order; p.offsets = c.offsets;
     p.weights = static_cast<const T*>(c.weights);
     return p;
@@ -424,19 +429,18 @@ void launch_pass(const smx_adapter_linear& c, bool transposed, const Pass<float>
         TsDegree& e = t.degree[q];
         e.comps = d.comps; e.Kd = d.Kd; e.Nc = d.Nc; e.in_off = d.in_off; e.out_off = d.out_off; e.hidden = d.hidden;
         e.W = d.W; e.first = d.first; e.first_group = d.first_group; e.second = d.second; e.second_group = d.second_group;
-        const long long rows = (p.sorted ? p.pairs : p.num_rows) * d.comps;
-        tiles += (p.sorted ? rows / kTsRows + p.groups + 1 : (rows + kTsRows - 1) / kTsRows) * (p.out ? ts_blocks(d.Nc) : 1);
+        tiles += (p.pairs * d.comps / kTsRows + p.groups + 1) * (p.out ? ts_blocks(d.Nc) : 1);
     }
-    t.degrees = degrees; t.rank = p.rank; t.groups = p.groups; t.slots = p.slots; t.num_rows = p.num_rows; t.pairs = p.pairs;
-    t.order = p.order; t.offsets = p.offsets; t.weights = p.weights; t.in = p.in; t.in_stride = p.in_stride; t.out = p.out; t.out_stride = p.out_stride;
-    t.sorted = p.sorted; t.out_sorted = p.out_sorted; t.tail = p.tail;
+    t.degrees = degrees; t.rank = p.rank; t.groups = p.groups; t.slots = p.slots; t.pairs = p.pairs;
+    t.order = p.order; t.offsets = p.offsets; t.places = p.places; t.weights = p.weights; t.in = p.in; t.in_stride = p.in_stride; t.out = p.out; t.out_stride = p.out_stride;
+    t.add = p.add; t.tail = p.tail;
     if (tiles > INT_MAX - 4096) throw ArgError("smx_adapter: too many rows");
     bool bare = false;
     for (int q = 0; q < degrees; ++q) bare = bare || !p.degree[q].W;
-    if (bare && p.out && (p.tail || !p.sorted)) {        // with one slot a pair is an atom
+    if (bare && p.out && p.tail) {
         const Widths w = widths(c);
-        adapter_zero_rows_kernel<<<static_cast<unsigned>(std::min<long long>(p.num_rows, 8LL * sm_count())), 256, 0, stream>>>(
-            p.offsets, p.groups, p.num_rows, p.sorted ? p.order : nullptr, p.out, p.out_stride, static_cast<int>(transposed ? w.in : w.out));
+        adapter_zero_rows_kernel<<<static_cast<unsigned>(std::min<long long>(p.pairs, 8LL * sm_count())), 256, 0, stream>>>(
+            p.offsets, p.groups, p.pairs, p.order, p.places, p.slots, p.out, p.out_stride, static_cast<int>(transposed ? w.in : w.out));
         launched("adapter_zero_rows_kernel");
     }
     if (padded_rank(p.rank) == 16) launch_ts<1>(t, tiles, stream);
@@ -468,15 +472,15 @@ void launch_pass(const smx_adapter_linear&, bool, const Pass<double>& p, int deg
         if (!p.out) e.ldw = 0;
         e.W = d.W; e.first = d.first; e.first_group = d.first_group; e.second = d.second; e.second_group = d.second_group;
     }
-    t.degrees = degrees; t.rank = p.rank; t.groups = p.groups; t.slots = p.slots; t.num_rows = p.num_rows; t.pairs = p.pairs;
-    t.order = p.order; t.offsets = p.offsets; t.weights = p.weights; t.in = p.in; t.in_stride = p.in_stride; t.out = p.out; t.out_stride = p.out_stride;
-    t.sorted = p.sorted; t.out_sorted = p.out_sorted; t.tail = p.tail;
+    t.degrees = degrees; t.rank = p.rank; t.groups = p.groups; t.slots = p.slots; t.pairs = p.pairs;
+    t.order = p.order; t.offsets = p.offsets; t.places = p.places; t.weights = p.weights; t.in = p.in; t.in_stride = p.in_stride; t.out = p.out; t.out_stride = p.out_stride;
+    t.add = p.add; t.tail = p.tail;
     auto tiles = [&](int BM, int BN) {
         long long n = 0;
         for (int q = 0; q < degrees; ++q) {
-            const long long rows = (p.sorted ? p.pairs : p.num_rows) * p.degree[q].comps;
+            const long long rows = p.pairs * p.degree[q].comps;
             const bool all = !p.out || (BM == 64 && !p.degree[q].W);         // one CTA makes all blocks of columns
-            n += (p.sorted ? rows / BM + p.groups + 1 : (rows + BM - 1) / BM) * (all ? 1 : (p.degree[q].Nc + BN - 1) / BN);
+            n += (rows / BM + p.groups + 1) * (all ? 1 : (p.degree[q].Nc + BN - 1) / BN);
         }
         return n;
     };
@@ -485,7 +489,6 @@ void launch_pass(const smx_adapter_linear&, bool, const Pass<double>& p, int deg
         if (tiles(64, 64) <= 2LL * sm_count()) launch_dp<16, 32, 1, 4, NR, 4>(t, tiles(16, 32), stream);
         else launch_dp<64, 64, 2, 2, NR, 2>(t, tiles(64, 64), stream);
     };
-    if (!p.sorted && tiles(64, 64) > 2LL * sm_count()) { launch_dp<64, 64, 2, 2, 0, 2>(t, tiles(64, 64), stream); return; }
     if (p.rank <= 8) by_rank(std::integral_constant<int, 1>{});
     else if (p.rank <= 16) by_rank(std::integral_constant<int, 2>{});
     else if (p.rank <= 32) by_rank(std::integral_constant<int, 4>{});
@@ -530,33 +533,28 @@ void launch_grads(const GradPass<float>& gp, int problems, cudaStream_t stream) 
 
 // out = in W + adapters, in either direction; `hidden` (may be null) receives in . first of every pair. Without `out` that is all.
 template <typename T>
-void run_pass(const smx_adapter_linear& c, bool transposed, const T* in, long in_stride, T* out, long out_stride, T* hidden, T* products) {
+void run_pass(const smx_adapter_linear& c, bool transposed, const T* in, long in_stride, T* out, long out_stride, T* hidden, const Buffers<T>& b) {
     if (c.num_rows == 0) return;
     const cudaStream_t stream = static_cast<cudaStream_t>(c.stream);
-    const Widths w = widths(c);
-    const long out_width = transposed ? w.in : w.out;
     Pass<T> p = make_pass<T>(c, transposed, hidden);
     p.in = in; p.in_stride = in_stride;
-    p.sorted = 1;
     if (!out) {
         for (int d = 0; d < c.num_degrees; ++d) { p.degree[d].W = nullptr; p.degree[d].Nc = 1; }      // one (unused) block of columns
         launch_pass(c, transposed, p, c.num_degrees, stream);
         return;
     }
-    if (c.slots == 1) {
-        p.out = out; p.out_stride = out_stride; p.tail = 1;
+    p.out = out; p.out_stride = out_stride; p.tail = 1;
+    if (c.slots > 1) route_slots(c.order, c.num_rows, c.slots, c.offsets, c.num_groups, b.places, b.slot_offsets, b.scratch, stream);
+    for (int s = 0; s < c.slots; ++s) {
+        if (c.slots > 1) {
+            p.places = b.places + static_cast<size_t>(s) * c.num_rows;
+            p.offsets = b.slot_offsets + static_cast<size_t>(s) * (c.num_groups + 1);
+            p.pairs = c.num_rows;
+        }
         launch_pass(c, transposed, p, c.num_degrees, stream);
-        return;
+        p.add = 1; p.tail = 0;
+        for (int d = 0; d < c.num_degrees; ++d) p.degree[d].W = nullptr;
     }
-    // several slots: the shared product of all rows, every pair's own product, and their weighted sum in slot order
-    Pass<T> shared = make_pass<T>(c, transposed, nullptr);
-    shared.in = in; shared.in_stride = in_stride; shared.out = out; shared.out_stride = out_stride;
-    launch_pass(c, transposed, shared, c.num_degrees, stream);
-    for (int d = 0; d < c.num_degrees; ++d) p.degree[d].W = nullptr;
-    p.weights = nullptr;
-    p.out = products; p.out_stride = out_width; p.out_sorted = 1;
-    launch_pass(c, transposed, p, c.num_degrees, stream);
-    route_combine<T>(products, c.position, c.num_rows, c.slots, out_width, static_cast<const T*>(c.weights), out, out_stride, out, out_stride, stream);
 }
 
 template <typename T>
@@ -567,7 +565,7 @@ void forward(const smx_adapter_linear& c) {
     const Widths w = widths(c);
     check_rows("x", c.x, c.x_stride, w.in, c.num_rows, false);
     check_rows("y", c.y, c.y_stride, w.out, c.num_rows, true);
-    run_pass<T>(c, false, static_cast<const T*>(c.x), c.x_stride, static_cast<T*>(c.y), c.y_stride, static_cast<T*>(c.hidden), b.products);
+    run_pass<T>(c, false, static_cast<const T*>(c.x), c.x_stride, static_cast<T*>(c.y), c.y_stride, static_cast<T*>(c.hidden), b);
 }
 
 template <typename T>
@@ -592,11 +590,11 @@ void backward(const smx_adapter_linear& c) {
     const size_t pairs = static_cast<size_t>(c.num_rows) * c.slots;
     const T* x = static_cast<const T*>(c.x);
     const T* gy = static_cast<const T*>(c.grad_y);
-    run_pass<T>(c, true, gy, c.grad_y_stride, static_cast<T*>(c.grad_x), c.grad_x_stride, b.back_hidden, b.products);
+    run_pass<T>(c, true, gy, c.grad_y_stride, static_cast<T*>(c.grad_x), c.grad_x_stride, b.back_hidden, b);
     if (!hidden_needed) return;
     const T* hidden = static_cast<const T*>(c.hidden);
     if (!hidden) {
-        run_pass<T>(c, false, x, c.x_stride, nullptr, 0, b.hidden, nullptr);
+        run_pass<T>(c, false, x, c.x_stride, nullptr, 0, b.hidden, b);
         hidden = b.hidden;
     }
     GradPass<T> gp{};

@@ -154,12 +154,12 @@ struct TsDegree {
 struct TsPass {
     TsDegree degree[SMX_ADAPTER_MAX_DEGREES];
     int degrees, rank, groups, slots;
-    long long num_rows, pairs;
-    const int* order; const int* offsets;
+    long long pairs;
+    const int* order; const int* offsets; const int* places;
     const float* weights;
     const float* in; long long in_stride;
     float* out; long long out_stride;
-    int sorted, out_sorted, tail;                // as in Pass
+    int add, tail;                               // as in Pass
 };
 struct TsWork { int index, degree, block, found; TileRows rows; };
 
@@ -176,10 +176,8 @@ struct TsCursor {
             const TsDegree& d = p.degree[q];
             const int blocks = p.out ? (d.Nc + 127) / 128 : 1;
             const int tile = (t - before) / blocks, g = g0 + lane;
-            int first = 0, count = 0;            // pairs of the group (rows of the array where there is no plan)
-            if (!p.sorted) {
-                if (g == 0) count = static_cast<int>(p.num_rows);
-            } else if (g < p.groups || (g == p.groups && p.tail)) {
+            int first = 0, count = 0;            // places of the group
+            if (g < p.groups || (g == p.groups && p.tail)) {
                 first = p.offsets[g];
                 count = (g < p.groups ? p.offsets[g + 1] : static_cast<int>(p.pairs)) - first;
             }
@@ -195,7 +193,7 @@ struct TsCursor {
             if (hit) {
                 const int src = __ffs(hit) - 1;
                 w.found = 1; w.degree = q; w.block = t - before - tile * blocks;
-                w.rows.group = p.sorted ? g0 + src : p.groups;
+                w.rows.group = g0 + src;
                 w.rows.first_pair = __shfl_sync(0xffffffffu, first, src);
                 w.rows.row0 = static_cast<long long>(tile - __shfl_sync(0xffffffffu, begin, src)) * kTsRows;
                 w.rows.rows = min(static_cast<long long>(kTsRows), static_cast<long long>(__shfl_sync(0xffffffffu, count, src)) * d.comps - w.rows.row0);
@@ -203,7 +201,7 @@ struct TsCursor {
             }
             run += __shfl_sync(0xffffffffu, incl, 31);
             g0 += 32;
-            if (g0 > p.groups || !p.sorted) { before += run * blocks; ++q; g0 = 0; run = 0; }
+            if (g0 > p.groups) { before += run * blocks; ++q; g0 = 0; run = 0; }
         }
         return false;
     }
@@ -236,12 +234,12 @@ __device__ __forceinline__ void ts_fill(const TsPass& p, const TsWork& w, int th
     const TsDegree& d = p.degree[w.degree];
     const TsShape s = ts_shape(p, w);
     for (int i = thread; i < s.rows; i += count) {
-        const long long r = w.rows.row0 + i, pair = w.rows.first_pair + r / d.comps, m = r % d.comps;
-        const long long n = p.sorted ? p.order[pair] / p.slots : pair;
+        const long long r = w.rows.row0 + i, at = w.rows.first_pair + r / d.comps, m = r % d.comps;
+        const long long place = p.places ? p.places[at] : at, n = p.order[place] / p.slots;
         if (p.out)
-            for (int c = s.col0; c < min(d.Nc, s.col0 + 128); ++c) p.out[(p.out_sorted ? pair : n) * p.out_stride + d.out_off + m * d.Nc + c] = value;
+            for (int c = s.col0; c < min(d.Nc, s.col0 + 128); ++c) p.out[n * p.out_stride + d.out_off + m * d.Nc + c] = value;
         if (s.adapter && d.hidden && w.block == 0)
-            for (int q = 0; q < p.rank; ++q) d.hidden[(pair * d.comps + m) * p.rank + q] = value;
+            for (int q = 0; q < p.rank; ++q) d.hidden[(place * d.comps + m) * p.rank + q] = value;
     }
 }
 
@@ -271,11 +269,13 @@ __device__ __forceinline__ bool ts_wait_warp(unsigned long long* bar, unsigned p
 template <int N> __device__ __forceinline__ void ts_registers_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void ts_registers_less() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
-// Rows without a group where a linear has no shared weights for them; all `rows` rows without a plan.
+// Rows without a group where a linear has no shared weights for them.
 __global__ void __launch_bounds__(256) adapter_zero_rows_kernel(const int* __restrict__ offsets, int groups, long long rows, const int* __restrict__ order,
-                                                                float* __restrict__ out, long long stride, int width) {
-    for (long long p = (order ? offsets[groups] : 0) + blockIdx.x; p < rows; p += gridDim.x)
-        for (int c = threadIdx.x; c < width; c += 256) out[(order ? order[p] : p) * stride + c] = 0.f;
+                                                                const int* __restrict__ places, int slots, float* __restrict__ out, long long stride, int width) {
+    for (long long p = offsets[groups] + blockIdx.x; p < rows; p += gridDim.x) {
+        const long long n = order[places ? places[p] : p] / slots;
+        for (int c = threadIdx.x; c < width; c += 256) out[n * stride + c] = 0.f;
+    }
 }
 
 __device__ __forceinline__ void cp_async4(void* smem, const void* gmem) {
@@ -291,7 +291,7 @@ __device__ __forceinline__ void ts_bulk(uint32_t to, const float* from, uint32_t
 //               is these tiles in shared memory and 32 values of the rows in tensor memory, with one barrier for both
 //   warp 1      the products (one thread)
 //   warp 2      finds the tiles and looks up their atoms and weights (a ring of four, ahead of all others)
-//   warps 4-7   rows: a warp copies 32 values of each of its 32 rows asynchronously, 16 bytes a lane (4 where rows start on no 16-byte boundary), four
+//   warps 4-7   rows: a warp copies 32 values of each of its 32 rows asynchronously, 16 bytes a lane (4 where rows start on no 16-byte boundary), three
 //               chunks ahead; a thread splits those of its row and stores them to the tensor memory's row operand. (Loads and stores by
 //               the thread that owns a row touch 32 rows an instruction; a bulk copy takes 70 cycles to issue; one warp that copied for all
 //               four took longer than the products: 184 us instead of 160 at 98,304 atoms.)
@@ -302,8 +302,9 @@ __device__ __forceinline__ void ts_bulk(uint32_t to, const float* from, uint32_t
 // stored into the hidden columns of its last two sums (head in the last one's, remainder in the other's); the products with second_g go on
 // top of the last sum, which is read after them.
 // Every wait is bounded; if one runs out, the CTA gives up and fills its remaining tiles with NaN.
-constexpr int kTsPassThreads = 512, kTsWorkRing = 4, kTsRowStages = 5;
+constexpr int kTsPassThreads = 512, kTsWorkRing = 4, kTsRowStages = 4;
 constexpr int kTsRowPitch = kTsChunk + 4;                                     // floats: threads that read their rows 16 bytes at a time hit all banks
+constexpr int kTsOutPitch = 17;                                               // floats of a row in the way out of rows that are not aligned
 constexpr int kTsRegsControl = 72, kTsRegsRows = 120, kTsRegsSums = 160, kTsRegsLaunch = 128;
 static_assert(kTsRegsControl + kTsRegsRows + 2 * kTsRegsSums <= 4 * kTsRegsLaunch, "the registers of the launch are shared out");
 template <int HP>                                    // hidden columns / 16
@@ -312,9 +313,9 @@ struct TsPassLayout {
     static constexpr int slot0 = 2 * sum_cols;
     static constexpr uint32_t stage_bytes = sum_cols * 256u;
     static constexpr int row_floats = kTsRows * kTsRowPitch;
-    static constexpr int smem = stages * static_cast<int>(stage_bytes) + kTsRowStages * row_floats * 4 + 1024;
+    static constexpr int smem = stages * static_cast<int>(stage_bytes) + (kTsRowStages * row_floats + 8 * 32 * kTsOutPitch) * 4 + 1024;
     static_assert(slot0 + 64 * stages <= 512, "tensor memory has 512 columns");
-    static_assert(smem + 15 * 1024 <= 227 * 1024, "shared memory of one CTA per SM");
+    static_assert(smem + 14 * 1024 <= 227 * 1024, "shared memory of one CTA per SM");
 };
 
 template <int HP>
@@ -373,10 +374,10 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
 #pragma unroll 2
                     for (int at = lane; at < kTsRows; at += 32) {
                         const bool live = at < w.rows.rows;
-                        const int ahead = (m0 + at) / comps, place = live ? p0 + ahead : p0, comp = live ? m0 + at - ahead * comps : 0;
-                        const int pair = pass.sorted ? pass.order[place] : place, atom = pass.sorted && pass.slots > 1 ? pair / pass.slots : pair;
+                        const int ahead = (m0 + at) / comps, comp = live ? m0 + at - ahead * comps : 0, listed = live ? p0 + ahead : p0;
+                        const int place = pass.places ? pass.places[listed] : listed, pair = pass.order[place], atom = pass.slots > 1 ? pair / pass.slots : pair;
                         work_in[slot][at] = atom * pass.in_stride + d.in_off + comp * d.Kd;
-                        work_out[slot][at] = (pass.out_sorted ? place : atom) * pass.out_stride + d.out_off + static_cast<long long>(comp) * d.Nc;
+                        work_out[slot][at] = atom * pass.out_stride + d.out_off + static_cast<long long>(comp) * d.Nc;
                         work_place[slot][at] = place;
                         work_comp[slot][at] = static_cast<short>(comp);
                         work_weight[slot][at] = weighted ? pass.weights[pair] : 1.f;
@@ -723,21 +724,43 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
             }
             next_work();
             if (!ok) break;
-            if (out_row) {
-                const uintptr_t bits = reinterpret_cast<uintptr_t>(out_row);
+            if (pass.out) {
+                const unsigned long long bits = static_cast<unsigned long long>(pass.out_stride | d.out_off | d.Nc) * 4u | reinterpret_cast<uintptr_t>(pass.out);
                 if (left >= 64 && (bits & 31) == 0) {
+                    if (out_row) {
 #pragma unroll
-                    for (int q = 0; q < 64; q += 8)
-                        asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out_row + q), "f"(sum[q]), "f"(sum[q + 1]), "f"(sum[q + 2]),
-                                     "f"(sum[q + 3]), "f"(sum[q + 4]), "f"(sum[q + 5]), "f"(sum[q + 6]), "f"(sum[q + 7]) : "memory");
-                } else if ((left & 3) == 0 && (bits & 15) == 0) {
+                        for (int q = 0; q < 64; q += 8) {
+                            if (pass.add) {
+                                float v[8];
+                                asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]),
+                                             "=f"(v[5]), "=f"(v[6]), "=f"(v[7]) : "l"(out_row + q) : "memory");
 #pragma unroll
-                    for (int q = 0; q < 64; q += 4)
-                        if (q < left) *reinterpret_cast<float4*>(out_row + q) = make_float4(sum[q], sum[q + 1], sum[q + 2], sum[q + 3]);
+                                for (int e = 0; e < 8; ++e) sum[q + e] += v[e];
+                            }
+                            asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out_row + q), "f"(sum[q]), "f"(sum[q + 1]), "f"(sum[q + 2]),
+                                         "f"(sum[q + 3]), "f"(sum[q + 4]), "f"(sum[q + 5]), "f"(sum[q + 6]), "f"(sum[q + 7]) : "memory");
+                        }
+                    }
                 } else {
+                    // 16 columns of the warp's rows at a time through shared memory, so that a store touches two rows instead of 32
+                    float* const stage = row_stages + kTsRowStages * L::row_floats + (warp - 8) * 32 * kTsOutPitch;
+                    const unsigned long long mine = reinterpret_cast<unsigned long long>(out_row);
 #pragma unroll
-                    for (int q = 0; q < 64; ++q)
-                        if (q < left) out_row[q] = sum[q];
+                    for (int c0 = 0; c0 < 64; c0 += 16) {
+                        if (c0 >= left) continue;
+                        __syncwarp();
+#pragma unroll
+                        for (int q = 0; q < 16; ++q) stage[lane * kTsOutPitch + q] = sum[c0 + q];
+                        __syncwarp();
+                        const int c = lane & 15;
+#pragma unroll 4
+                        for (int r = lane >> 4; r < 32; r += 2) {
+                            float* to = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, mine, r));
+                            if (!to || c0 + c >= left) continue;
+                            const float v = stage[r * kTsOutPitch + c];
+                            to[c0 + c] = pass.add ? to[c0 + c] + v : v;
+                        }
+                    }
                 }
             }
         }

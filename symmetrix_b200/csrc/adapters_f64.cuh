@@ -36,12 +36,12 @@ struct DpDegree {
 struct DpPass {
     DpDegree degree[SMX_ADAPTER_MAX_DEGREES];
     int degrees, rank, groups, slots;
-    long long num_rows, pairs;
-    const int* order; const int* offsets;
+    long long pairs;
+    const int* order; const int* offsets; const int* places;
     const double* weights;
     const double* in; long long in_stride;
     double* out; long long out_stride;
-    int sorted, out_sorted, tail;                // as in Pass
+    int add, tail;                               // as in Pass
 };
 
 __device__ __forceinline__ void dp_copy16(double* smem, const double* gmem, int bytes) { cp_async16(smem, gmem, bytes); }
@@ -59,8 +59,8 @@ struct DpLayout {
 
 // A CTA of four warps (WM x WN) makes BM rows x BN columns of one degree and adapter: in . W and in . first_g from the same row fragments (the warps of
 // a row of warps share the inner values of the latter among them and add up through shared memory), then the weighted hidden rows times
-// second_g on top. ST stages of 16 inner values are in flight. NR: hidden columns / 8; 0: shared weights alone, fewer registers and stages' bytes.
-// Without shared weights a CTA of big tiles makes all blocks of columns from one hidden tile.
+// second_g on top. ST stages of 16 inner values are in flight. NR: hidden columns / 8. Without shared weights
+// a CTA of big tiles makes all blocks of columns from one hidden tile.
 template <int BM, int BN, int WM, int WN, int NR, int ST>
 __global__ void __launch_bounds__(kDpThreads) adapter_pass_f64_kernel(const __grid_constant__ DpPass pass) {
     using L = DpLayout<BM, BN, NR, ST>;
@@ -81,17 +81,7 @@ __global__ void __launch_bounds__(kDpThreads) adapter_pass_f64_kernel(const __gr
             const int blocks = pass.out && !(BM == 64 && !d.W) ? (d.Nc + BN - 1) / BN : 1;
             const long long row_tile = at / blocks;
             long long tiles;
-            bool ok;
-            if (pass.sorted) {
-                ok = find_tile(pass.offsets, pass.groups, pass.tail != 0, pass.pairs, d.comps, BM, row_tile, t, tiles);
-            } else {
-                const long long all = pass.num_rows * d.comps;
-                tiles = (all + BM - 1) / BM;
-                ok = row_tile < tiles;
-                t.group = pass.groups; t.first_pair = 0; t.row0 = row_tile * BM;
-                t.rows = min(static_cast<long long>(BM), all - t.row0);
-            }
-            if (ok) { hit = q; cb = static_cast<int>(at % blocks); }
+            if (find_tile(pass.offsets, pass.groups, pass.tail != 0, pass.pairs, d.comps, BM, row_tile, t, tiles)) { hit = q; cb = static_cast<int>(at % blocks); }
             else at -= tiles * blocks;
         }
         if (lane == 0) { which = hit; col_block = cb; tile = t; }
@@ -101,16 +91,17 @@ __global__ void __launch_bounds__(kDpThreads) adapter_pass_f64_kernel(const __gr
     const DpDegree& d = pass.degree[which];
     const int rows = static_cast<int>(tile.rows), g = tile.group, R = pass.rank, ldf = (R + 1) & ~1;
     int col0 = col_block * BN;
-    const bool adapter = NR > 0 && g < pass.groups, shared = d.W && pass.out;
+    const bool adapter = g < pass.groups, shared = d.W && pass.out;
     for (int i = tid; i < BM; i += kDpThreads) {
         long long ib = -1, ob = -1, hr = 0;
         double w = 1.0;
         if (i < rows) {
-            const long long r = tile.row0 + i, p = tile.first_pair + r / d.comps;
+            const long long r = tile.row0 + i, listed = tile.first_pair + r / d.comps, p = pass.places ? pass.places[listed] : listed;
             const int m = static_cast<int>(r % d.comps);
-            const long long pair = pass.sorted ? pass.order[p] : p, n = pass.sorted ? pair / pass.slots : p;
+            const int pair = pass.order[p];
+            const long long n = pair / pass.slots;
             ib = n * pass.in_stride + d.in_off + static_cast<long long>(m) * d.Kd;
-            ob = (pass.out_sorted ? p : n) * pass.out_stride + d.out_off + static_cast<long long>(m) * d.Nc;
+            ob = n * pass.out_stride + d.out_off + static_cast<long long>(m) * d.Nc;
             hr = p * d.comps + m;
             if (adapter && pass.weights) w = pass.weights[pair];
         }
@@ -148,8 +139,7 @@ __global__ void __launch_bounds__(kDpThreads) adapter_pass_f64_kernel(const __gr
             }
         if (adapter)
             for (int i = tid; i < kDpBK * 4 * NR; i += kDpThreads) {
-                constexpr int per = NR > 0 ? 4 * NR : 1;
-                const int k = i / per, c = (i % per) * 2;
+                const int k = i / (4 * NR), c = (i % (4 * NR)) * 2;
                 const int bytes = k0 + k < d.Kd && c < ldf ? 16 : 0;
                 dp_copy16(Fs + k * SF + c, first + (bytes ? static_cast<long long>(k0 + k) * ldf + c : 0), bytes);
             }
@@ -169,7 +159,7 @@ __global__ void __launch_bounds__(kDpThreads) adapter_pass_f64_kernel(const __gr
         if (s < chunks) issue(s);
         cp_async_commit();
     }
-    double acc[MB][NB][2], hid[MB][NR > 0 ? NR : 1][2];
+    double acc[MB][NB][2], hid[MB][NR][2];
 #pragma unroll
     for (int i = 0; i < MB; ++i) {
 #pragma unroll
@@ -261,10 +251,15 @@ __global__ void __launch_bounds__(kDpThreads) adapter_pass_f64_kernel(const __gr
                 const int c = col0 + wn * NB * 8 + 8 * j + 2 * fk;
                 double* to = pass.out + ob + c;
                 if (out_wide && c < d.Nc) {
-                    *reinterpret_cast<double2*>(to) = make_double2(acc[i][j][0], acc[i][j][1]);
+                    double2 v = make_double2(acc[i][j][0], acc[i][j][1]);
+                    if (pass.add) {
+                        const double2 old = *reinterpret_cast<const double2*>(to);
+                        v.x += old.x; v.y += old.y;
+                    }
+                    *reinterpret_cast<double2*>(to) = v;
                 } else {
-                    if (c < d.Nc) to[0] = acc[i][j][0];
-                    if (c + 1 < d.Nc) to[1] = acc[i][j][1];
+                    if (c < d.Nc) to[0] = pass.add ? to[0] + acc[i][j][0] : acc[i][j][0];
+                    if (c + 1 < d.Nc) to[1] = pass.add ? to[1] + acc[i][j][1] : acc[i][j][1];
                 }
             }
         }

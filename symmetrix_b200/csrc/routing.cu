@@ -25,16 +25,20 @@ constexpr int kMaxGroups = SMX_ROUTE_MAX_GROUPS;
 // ------------------------------------------------------------------------------------------- plan
 // Pairs are counted and ranked by warps that own consecutive pairs: 32 at a time, lanes of equal group found with match_any, one counter
 // per (warp, group) in shared memory that only that warp touches. Equal keys therefore keep their order.
+// kSlots: the keys are the slots of pairs, ids[i] = n * groups + slot (see route_slots).
+template <bool kSlots>
 __device__ __forceinline__ int route_key(const int* ids, long long i, int groups) {
     const int g = ids[i];
+    if (kSlots) return g % groups;
     return (g < 0 || g >= groups) ? groups : g;
 }
 
+template <bool kSlots>
 __device__ __forceinline__ void route_count(const int* __restrict__ ids, long long begin, long long end, int groups, int* __restrict__ hist) {
     const int lane = threadIdx.x & 31;
     for (long long i0 = begin; i0 < end; i0 += 32) {
         const bool in = i0 + lane < end;
-        const int g = in ? route_key(ids, i0 + lane, groups) : groups + 1;
+        const int g = in ? route_key<kSlots>(ids, i0 + lane, groups) : groups + 1;
         const unsigned same = __match_any_sync(0xffffffffu, g);
         if (in && lane == __ffs(same) - 1) hist[g] += __popc(same);
         __syncwarp();
@@ -42,12 +46,13 @@ __device__ __forceinline__ void route_count(const int* __restrict__ ids, long lo
 }
 
 // `next[g]`: where this warp's next pair of group g goes.
+template <bool kSlots>
 __device__ __forceinline__ void route_place(const int* __restrict__ ids, long long begin, long long end, int groups, int* __restrict__ next,
                                             int* __restrict__ order, int* __restrict__ position) {
     const int lane = threadIdx.x & 31;
     for (long long i0 = begin; i0 < end; i0 += 32) {
         const bool in = i0 + lane < end;
-        const int g = in ? route_key(ids, i0 + lane, groups) : groups + 1;
+        const int g = in ? route_key<kSlots>(ids, i0 + lane, groups) : groups + 1;
         const unsigned same = __match_any_sync(0xffffffffu, g);
         int first = 0;
         if (in) first = next[g];
@@ -55,7 +60,7 @@ __device__ __forceinline__ void route_place(const int* __restrict__ ids, long lo
         if (in) {
             const int p = first + __popc(same & ((1u << lane) - 1u));
             order[p] = static_cast<int>(i0 + lane);
-            position[i0 + lane] = g < groups ? p : -1;
+            if (!kSlots) position[i0 + lane] = g < groups ? p : -1;
             if (lane == __ffs(same) - 1) next[g] = first + __popc(same);
         }
         __syncwarp();
@@ -97,6 +102,7 @@ __device__ __forceinline__ void cta_scan(int* v, int n, int* sums) {
 
 // Few pairs: one CTA does all three steps.
 constexpr int kSmallPlanThreads = 1024, kSmallPlanPairs = 8192;
+template <bool kSlots>
 __global__ void __launch_bounds__(kSmallPlanThreads) route_plan_small_kernel(const int* __restrict__ ids, int pairs, int groups, int warps_used,
                                                                              int* __restrict__ order, int* __restrict__ position,
                                                                              int* __restrict__ offsets) {
@@ -109,7 +115,7 @@ __global__ void __launch_bounds__(kSmallPlanThreads) route_plan_small_kernel(con
     __syncthreads();
     const int per = ((pairs + warps_used - 1) / warps_used + 31) & ~31;
     const int begin = min(pairs, warp * per), end = min(pairs, begin + per);
-    if (warp < warps_used) route_count(ids, begin, end, groups, hist + warp * bins);
+    if (warp < warps_used) route_count<kSlots>(ids, begin, end, groups, hist + warp * bins);
     __syncthreads();
     for (int g = threadIdx.x; g < bins; g += blockDim.x) {
         int run = 0;
@@ -119,15 +125,16 @@ __global__ void __launch_bounds__(kSmallPlanThreads) route_plan_small_kernel(con
     __syncthreads();
     cta_scan(total, bins, sums);
     for (int g = threadIdx.x; g < bins; g += blockDim.x) {
-        offsets[g] = total[g];                  // bins = groups + 1 entries: the start of the empty slots is the end of the groups
+        if (!kSlots) offsets[g] = total[g];     // bins = groups + 1 entries: the start of the empty slots is the end of the groups
         for (int w = 0; w < warps_used; ++w) hist[w * bins + g] += total[g];
     }
     __syncthreads();
-    if (warp < warps_used) route_place(ids, begin, end, groups, hist + warp * bins, order, position);
+    if (warp < warps_used) route_place<kSlots>(ids, begin, end, groups, hist + warp * bins, order, position);
 }
 
 // Many pairs: counts per chunk, a scan over the chunks of every group, then the ranks. chunk_hist is [bins][chunks].
 constexpr int kPlanWarps = 8, kPlanThreads = 32 * kPlanWarps, kPlanChunk = 2048;
+template <bool kSlots>
 __global__ void __launch_bounds__(kPlanThreads) route_count_kernel(const int* __restrict__ ids, long long pairs, int groups, int chunks,
                                                                    int* __restrict__ chunk_hist) {
     extern __shared__ int route_smem[];
@@ -136,7 +143,7 @@ __global__ void __launch_bounds__(kPlanThreads) route_count_kernel(const int* __
     __syncthreads();
     constexpr int per = kPlanChunk / kPlanWarps;
     const long long begin = min(pairs, static_cast<long long>(blockIdx.x) * kPlanChunk + warp * per), end = min(pairs, begin + per);
-    route_count(ids, begin, end, groups, route_smem + warp * bins);
+    route_count<kSlots>(ids, begin, end, groups, route_smem + warp * bins);
     __syncthreads();
     for (int g = threadIdx.x; g < bins; g += kPlanThreads) {
         int sum = 0;
@@ -163,6 +170,7 @@ __global__ void __launch_bounds__(256) route_scan_kernel(int bins, int chunks, i
     }
     if (lane == 0) total[g] = run;
 }
+template <bool kSlots>
 __global__ void __launch_bounds__(kPlanThreads) route_place_kernel(const int* __restrict__ ids, long long pairs, int groups, int chunks,
                                                                    const int* __restrict__ chunk_prefix, const int* __restrict__ total,
                                                                    int* __restrict__ order, int* __restrict__ position, int* __restrict__ offsets) {
@@ -177,15 +185,31 @@ __global__ void __launch_bounds__(kPlanThreads) route_place_kernel(const int* __
     cta_scan(start, bins, sums);
     constexpr int per = kPlanChunk / kPlanWarps;
     const long long begin = min(pairs, static_cast<long long>(blockIdx.x) * kPlanChunk + warp * per), end = min(pairs, begin + per);
-    route_count(ids, begin, end, groups, hist + warp * bins);
+    route_count<kSlots>(ids, begin, end, groups, hist + warp * bins);
     __syncthreads();
     for (int g = threadIdx.x; g < bins; g += kPlanThreads) {
-        if (blockIdx.x == 0) offsets[g] = start[g];
+        if (!kSlots && blockIdx.x == 0) offsets[g] = start[g];
         int run = start[g] + chunk_prefix[static_cast<long long>(g) * chunks + blockIdx.x];
         for (int w = 0; w < kPlanWarps; ++w) { const int c = hist[w * bins + g]; hist[w * bins + g] = run; run += c; }
     }
     __syncthreads();
-    route_place(ids, begin, end, groups, hist + warp * bins, order, position);
+    route_place<kSlots>(ids, begin, end, groups, hist + warp * bins, order, position);
+}
+
+// The first of slot s's places (sorted positions, ascending) in or behind group g, for all g and s: they are runs of num_rows places.
+__global__ void __launch_bounds__(256) route_slot_offsets_kernel(const int* __restrict__ places, int num_rows, int slots, const int* __restrict__ offsets,
+                                                                 int groups, int* __restrict__ slot_offsets) {
+    const int t = blockIdx.x * 256 + threadIdx.x;
+    if (t >= slots * (groups + 1)) return;
+    const int* run = places + static_cast<long long>(t / (groups + 1)) * num_rows;
+    const int bound = offsets[t % (groups + 1)];
+    int lo = 0, hi = num_rows;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (run[mid] < bound) lo = mid + 1;
+        else hi = mid;
+    }
+    slot_offsets[t] = lo;
 }
 
 // ------------------------------------------------------------------------------------------- rows
@@ -380,12 +404,9 @@ size_t route_plan_bytes(long num_rows, int slots, int num_groups) {
     return static_cast<size_t>((num_groups + 1) * (chunks + 1) * sizeof(int));
 }
 
-void route_plan(const int* ids, long num_rows, int slots, int num_groups, int* order, int* position, int* offsets, void* workspace,
-                size_t workspace_bytes, cudaStream_t stream) {
-    const size_t need = route_plan_bytes(num_rows, slots, num_groups);
-    const long long pairs = static_cast<long long>(num_rows) * slots;
-    if (!offsets || (pairs > 0 && (!ids || !order || !position))) throw ArgError("smx_route_plan: null pointer");
-    if (workspace_bytes < need || (need && !workspace)) throw ArgError("smx_route_plan: the workspace is smaller than smx_route_plan_bytes says");
+namespace {
+template <bool kSlots>
+void counting_sort(const int* ids, long long pairs, int num_groups, int* order, int* position, int* offsets, void* workspace, cudaStream_t stream) {
     const int bins = num_groups + 1;
     if (pairs <= kSmallPlanPairs) {
         // a warp for every 32 pairs, as far as their counters fit into 128 KB
@@ -394,11 +415,11 @@ void route_plan(const int* ids, long num_rows, int slots, int num_groups, int* o
         const int smem = ((warps + 1) * bins + 1) * static_cast<int>(sizeof(int));
         static std::atomic<bool> done[64];
         if (smem > 48 * 1024 && first_on_device(done)) {
-            SMX_CUDA(cudaFuncSetAttribute(route_plan_small_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+            SMX_CUDA(cudaFuncSetAttribute(route_plan_small_kernel<kSlots>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
             mark_on_device(done);
         }
         const int threads = std::max(128, 32 * warps);
-        route_plan_small_kernel<<<1, threads, smem, stream>>>(ids, static_cast<int>(pairs), num_groups, warps, order, position, offsets);
+        route_plan_small_kernel<kSlots><<<1, threads, smem, stream>>>(ids, static_cast<int>(pairs), num_groups, warps, order, position, offsets);
         launched("route_plan_small_kernel");
         return;
     }
@@ -406,13 +427,32 @@ void route_plan(const int* ids, long num_rows, int slots, int num_groups, int* o
     int* hist = static_cast<int*>(workspace);
     int* total = hist + static_cast<size_t>(bins) * chunks;
     const int smem = kPlanWarps * bins * static_cast<int>(sizeof(int));
-    route_count_kernel<<<chunks, kPlanThreads, smem, stream>>>(ids, pairs, num_groups, chunks, hist);
+    route_count_kernel<kSlots><<<chunks, kPlanThreads, smem, stream>>>(ids, pairs, num_groups, chunks, hist);
     launched("route_count_kernel");
     route_scan_kernel<<<(bins * 32 + 255) / 256, 256, 0, stream>>>(bins, chunks, hist, total);
     launched("route_scan_kernel");
-    route_place_kernel<<<chunks, kPlanThreads, smem + (bins + 1) * static_cast<int>(sizeof(int)), stream>>>(ids, pairs, num_groups, chunks, hist, total,
-                                                                                                           order, position, offsets);
+    route_place_kernel<kSlots><<<chunks, kPlanThreads, smem + (bins + 1) * static_cast<int>(sizeof(int)), stream>>>(ids, pairs, num_groups, chunks, hist, total,
+                                                                                                                   order, position, offsets);
     launched("route_place_kernel");
+}
+}  // namespace
+
+void route_plan(const int* ids, long num_rows, int slots, int num_groups, int* order, int* position, int* offsets, void* workspace,
+                size_t workspace_bytes, cudaStream_t stream) {
+    const size_t need = route_plan_bytes(num_rows, slots, num_groups);
+    const long long pairs = static_cast<long long>(num_rows) * slots;
+    if (!offsets || (pairs > 0 && (!ids || !order || !position))) throw ArgError("smx_route_plan: null pointer");
+    if (workspace_bytes < need || (need && !workspace)) throw ArgError("smx_route_plan: the workspace is smaller than smx_route_plan_bytes says");
+    counting_sort<false>(ids, pairs, num_groups, order, position, offsets, workspace, stream);
+}
+
+size_t route_slots_bytes(long num_rows, int slots) { return route_plan_bytes(num_rows * slots, 1, slots); }
+void route_slots(const int* order, long num_rows, int slots, const int* offsets, int num_groups, int* places, int* slot_offsets, void* workspace,
+                 cudaStream_t stream) {
+    counting_sort<true>(order, static_cast<long long>(num_rows) * slots, slots, places, nullptr, nullptr, workspace, stream);
+    const int n = slots * (num_groups + 1);
+    route_slot_offsets_kernel<<<(n + 255) / 256, 256, 0, stream>>>(places, static_cast<int>(num_rows), slots, offsets, num_groups, slot_offsets);
+    launched("route_slot_offsets_kernel");
 }
 
 template <typename T>

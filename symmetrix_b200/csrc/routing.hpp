@@ -22,6 +22,11 @@ void mark_on_device(std::atomic<bool> (&done)[64]);
 size_t route_plan_bytes(long num_rows, int slots, int num_groups);
 void route_plan(const int* ids, long num_rows, int slots, int num_groups, int* order, int* position, int* offsets, void* workspace,
                 size_t workspace_bytes, cudaStream_t stream);
+// The plan slot by slot: places[s * num_rows ..] are the sorted positions of slot s's pairs, ascending, so grouped, empty ones last;
+// slot_offsets[s * (num_groups + 1) + g] is where group g begins among them. A row is in every slot's list once.
+size_t route_slots_bytes(long num_rows, int slots);
+void route_slots(const int* order, long num_rows, int slots, const int* offsets, int num_groups, int* places, int* slot_offsets, void* workspace,
+                 cudaStream_t stream);
 template <typename T>
 void route_dispatch(const T* x, long x_stride, long num_rows, int slots, long width, const int* position, const int* offsets, int num_groups,
                     T* rows, bool zero_tail, cudaStream_t stream);
