@@ -612,6 +612,8 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
         const int tid = threadIdx.x & 127, half = (warp - 8) >> 2, R = pass.rank;
         constexpr int kLower = (HP + 1) / 2;         // blocks of 16 hidden columns of the lower half; the upper half has the others
         const int hid0 = half ? kLower : 0, hid_blocks = half ? HP - kLower : kLower;
+        float* const out_stage = row_stages + kTsRowStages * L::row_floats + (warp - 8) * 32 * kTsOutPitch;
+        const unsigned long long out_bits = static_cast<unsigned long long>(pass.out_stride) * 4u | reinterpret_cast<uintptr_t>(pass.out);
         int nd = 0, nt = 0, i = 0;                   // partial sums and hidden rows used so far, tiles
         bool ok = true;
         TsWork w{};
@@ -643,9 +645,39 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
             if (live && pass.out) out_row = pass.out + out_at + s.col0 + 64 * half;
             if (live && s.adapter && d.hidden && w.block == 0) hid_row = d.hidden + (static_cast<long long>(place) * d.comps + comp) * R + 16 * hid0;
             const int left = d.Nc - s.col0 - 64 * half;                  // columns of this half that exist
+            const bool out_wide = left >= 64 && ((out_bits | 4u * static_cast<unsigned>(d.out_off | d.Nc)) & 31) == 0;
             float sum[64], hid[16 * kLower];
 #pragma unroll
             for (int q = 0; q < 64; ++q) sum[q] = 0.f;
+            if (pass.add) {
+                // what the earlier slots left comes in while the products run
+                if (out_wide) {
+                    if (out_row)
+#pragma unroll
+                        for (int q = 0; q < 64; q += 8)
+                            asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];" : "=f"(sum[q]), "=f"(sum[q + 1]), "=f"(sum[q + 2]), "=f"(sum[q + 3]),
+                                         "=f"(sum[q + 4]), "=f"(sum[q + 5]), "=f"(sum[q + 6]), "=f"(sum[q + 7]) : "l"(out_row + q) : "memory");
+                } else {
+                    const unsigned long long mine = reinterpret_cast<unsigned long long>(out_row);
+#pragma unroll
+                    for (int c0 = 0; c0 < 64; c0 += 16) {
+                        if (c0 >= left) continue;
+                        const int c = c0 + (lane & 15);
+                        float v[16];
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            const float* from = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, mine, 2 * r + (lane >> 4)));
+                            v[r] = from && c < left ? from[c] : 0.f;
+                        }
+                        __syncwarp();
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) out_stage[(2 * r + (lane >> 4)) * kTsOutPitch + (lane & 15)] = v[r];
+                        __syncwarp();
+#pragma unroll
+                        for (int q = 0; q < 16; ++q) sum[c0 + q] = out_stage[lane * kTsOutPitch + q];
+                    }
+                }
+            }
 #pragma unroll
             for (int q = 0; q < 16 * kLower; ++q) hid[q] = 0.f;
             auto add_columns = [&](uint32_t from, int cols) {            // of [0, cols) those of this half
@@ -724,44 +756,30 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
             }
             next_work();
             if (!ok) break;
-            if (pass.out) {
-                const unsigned long long bits = static_cast<unsigned long long>(pass.out_stride | d.out_off | d.Nc) * 4u | reinterpret_cast<uintptr_t>(pass.out);
-                if (left >= 64 && (bits & 31) == 0) {
-                    if (out_row) {
+            if (out_wide) {
+                if (out_row)
 #pragma unroll
-                        for (int q = 0; q < 64; q += 8) {
-                            if (pass.add) {
-                                float v[8];
-                                asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]),
-                                             "=f"(v[5]), "=f"(v[6]), "=f"(v[7]) : "l"(out_row + q) : "memory");
+                    for (int q = 0; q < 64; q += 8)
+                        asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out_row + q), "f"(sum[q]), "f"(sum[q + 1]), "f"(sum[q + 2]),
+                                     "f"(sum[q + 3]), "f"(sum[q + 4]), "f"(sum[q + 5]), "f"(sum[q + 6]), "f"(sum[q + 7]) : "memory");
+            } else if (pass.out) {
+                // 16 columns of the warp's rows at a time through shared memory, so that a store touches two rows instead of 32
+                const unsigned long long mine = reinterpret_cast<unsigned long long>(out_row);
 #pragma unroll
-                                for (int e = 0; e < 8; ++e) sum[q + e] += v[e];
-                            }
-                            asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out_row + q), "f"(sum[q]), "f"(sum[q + 1]), "f"(sum[q + 2]),
-                                         "f"(sum[q + 3]), "f"(sum[q + 4]), "f"(sum[q + 5]), "f"(sum[q + 6]), "f"(sum[q + 7]) : "memory");
-                        }
-                    }
-                } else {
-                    // 16 columns of the warp's rows at a time through shared memory, so that a store touches two rows instead of 32
-                    float* const stage = row_stages + kTsRowStages * L::row_floats + (warp - 8) * 32 * kTsOutPitch;
-                    const unsigned long long mine = reinterpret_cast<unsigned long long>(out_row);
+                for (int c0 = 0; c0 < 64; c0 += 16) {
+                    if (c0 >= left) continue;
+                    __syncwarp();
 #pragma unroll
-                    for (int c0 = 0; c0 < 64; c0 += 16) {
-                        if (c0 >= left) continue;
-                        __syncwarp();
-#pragma unroll
-                        for (int q = 0; q < 16; ++q) stage[lane * kTsOutPitch + q] = sum[c0 + q];
-                        __syncwarp();
-                        const int c = lane & 15;
+                    for (int q = 0; q < 16; ++q) out_stage[lane * kTsOutPitch + q] = sum[c0 + q];
+                    __syncwarp();
+                    const int c = c0 + (lane & 15);
 #pragma unroll 4
-                        for (int r = lane >> 4; r < 32; r += 2) {
-                            float* to = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, mine, r));
-                            if (!to || c0 + c >= left) continue;
-                            const float v = stage[r * kTsOutPitch + c];
-                            to[c0 + c] = pass.add ? to[c0 + c] + v : v;
-                        }
+                    for (int r = lane >> 4; r < 32; r += 2) {
+                        float* to = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, mine, r));
+                        if (to && c < left) to[c] = out_stage[r * kTsOutPitch + (c - c0)];
                     }
                 }
+                __syncwarp();
             }
         }
         if (!ok) {

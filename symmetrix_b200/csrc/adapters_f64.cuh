@@ -160,14 +160,32 @@ __global__ void __launch_bounds__(kDpThreads) adapter_pass_f64_kernel(const __gr
         cp_async_commit();
     }
     double acc[MB][NB][2], hid[MB][NR][2];
+    const int fr = lane >> 2, fk = lane & 3;
+    const bool out_wide = ((pass.out_stride | d.out_off | d.Nc) & 1) == 0 && (reinterpret_cast<uintptr_t>(pass.out) & 15) == 0;
+    auto begin_sums = [&]() {                            // from zero, or from what the earlier slots left
 #pragma unroll
-    for (int i = 0; i < MB; ++i) {
+        for (int i = 0; i < MB; ++i) {
+            const long long ob = pass.add ? out_base[wm * MB * 8 + i * 8 + fr] : -1;
 #pragma unroll
-        for (int j = 0; j < NB; ++j) acc[i][j][0] = acc[i][j][1] = 0.0;
+            for (int j = 0; j < NB; ++j) {
+                const int c = col0 + wn * NB * 8 + 8 * j + 2 * fk;
+                const double* from = pass.out + ob + c;
+                double2 v = make_double2(0.0, 0.0);
+                if (ob >= 0 && out_wide && c < d.Nc) {
+                    v = *reinterpret_cast<const double2*>(from);
+                } else if (ob >= 0) {
+                    if (c < d.Nc) v.x = from[0];
+                    if (c + 1 < d.Nc) v.y = from[1];
+                }
+                acc[i][j][0] = v.x; acc[i][j][1] = v.y;
+            }
+        }
+    };
+    begin_sums();
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
 #pragma unroll
         for (int j = 0; j < NR; ++j) hid[i][j][0] = hid[i][j][1] = 0.0;
-    }
-    const int fr = lane >> 2, fk = lane & 3;
     for (int t = 0; t < chunks; ++t) {
         cp_async_wait<ST - 2>();
         __syncthreads();                                 // chunk t is there, and the stage of chunk t - 1 has been read
@@ -226,7 +244,6 @@ __global__ void __launch_bounds__(kDpThreads) adapter_pass_f64_kernel(const __gr
         if (!pass.out) return;
         __syncthreads();
     }
-    const bool out_wide = ((pass.out_stride | d.out_off | d.Nc) & 1) == 0 && (reinterpret_cast<uintptr_t>(pass.out) & 15) == 0;
     const int end = BM == 64 && !d.W ? d.Nc : min(d.Nc, col0 + BN);
     for (;;) {
         if (adapter)
@@ -251,15 +268,10 @@ __global__ void __launch_bounds__(kDpThreads) adapter_pass_f64_kernel(const __gr
                 const int c = col0 + wn * NB * 8 + 8 * j + 2 * fk;
                 double* to = pass.out + ob + c;
                 if (out_wide && c < d.Nc) {
-                    double2 v = make_double2(acc[i][j][0], acc[i][j][1]);
-                    if (pass.add) {
-                        const double2 old = *reinterpret_cast<const double2*>(to);
-                        v.x += old.x; v.y += old.y;
-                    }
-                    *reinterpret_cast<double2*>(to) = v;
+                    *reinterpret_cast<double2*>(to) = make_double2(acc[i][j][0], acc[i][j][1]);
                 } else {
-                    if (c < d.Nc) to[0] = pass.add ? to[0] + acc[i][j][0] : acc[i][j][0];
-                    if (c + 1 < d.Nc) to[1] = pass.add ? to[1] + acc[i][j][1] : acc[i][j][1];
+                    if (c < d.Nc) to[0] = acc[i][j][0];
+                    if (c + 1 < d.Nc) to[1] = acc[i][j][1];
                 }
             }
         }
@@ -269,11 +281,8 @@ __global__ void __launch_bounds__(kDpThreads) adapter_pass_f64_kernel(const __gr
         __syncthreads();
         if (adapter) copy_second();
         cp_async_commit();
+        begin_sums();
         cp_async_wait<0>();
-#pragma unroll
-        for (int i = 0; i < MB; ++i)
-#pragma unroll
-            for (int j = 0; j < NB; ++j) acc[i][j][0] = acc[i][j][1] = 0.0;
         __syncthreads();
     }
 }

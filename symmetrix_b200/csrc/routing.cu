@@ -196,20 +196,22 @@ __global__ void __launch_bounds__(kPlanThreads) route_place_kernel(const int* __
     route_place<kSlots>(ids, begin, end, groups, hist + warp * bins, order, position);
 }
 
-// The first of slot s's places (sorted positions, ascending) in or behind group g, for all g and s: they are runs of num_rows places.
+// Where group g begins among slot s's places (sorted positions, ascending; runs of num_rows): a warp each, cutting the run into 33 pieces per step.
 __global__ void __launch_bounds__(256) route_slot_offsets_kernel(const int* __restrict__ places, int num_rows, int slots, const int* __restrict__ offsets,
                                                                  int groups, int* __restrict__ slot_offsets) {
-    const int t = blockIdx.x * 256 + threadIdx.x;
+    const int t = (blockIdx.x * 256 + threadIdx.x) >> 5, lane = threadIdx.x & 31;
     if (t >= slots * (groups + 1)) return;
     const int* run = places + static_cast<long long>(t / (groups + 1)) * num_rows;
     const int bound = offsets[t % (groups + 1)];
-    int lo = 0, hi = num_rows;
+    long long lo = 0, hi = num_rows;                 // the answer lies in lo .. hi
     while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (run[mid] < bound) lo = mid + 1;
-        else hi = mid;
+        const long long at = lo + (hi - lo) * (lane + 1) / 33;                  // ascending, below hi
+        const int below = __popc(__ballot_sync(0xffffffffu, run[at] < bound));  // a prefix of the lanes
+        const long long next = __shfl_sync(0xffffffffu, at, below & 31), last = __shfl_sync(0xffffffffu, at, below ? below - 1 : 0);
+        if (below < 32) hi = next;
+        if (below) lo = last + 1;
     }
-    slot_offsets[t] = lo;
+    if (lane == 0) slot_offsets[t] = static_cast<int>(lo);
 }
 
 // ------------------------------------------------------------------------------------------- rows
@@ -451,7 +453,7 @@ void route_slots(const int* order, long num_rows, int slots, const int* offsets,
                  cudaStream_t stream) {
     counting_sort<true>(order, static_cast<long long>(num_rows) * slots, slots, places, nullptr, nullptr, workspace, stream);
     const int n = slots * (num_groups + 1);
-    route_slot_offsets_kernel<<<(n + 255) / 256, 256, 0, stream>>>(places, static_cast<int>(num_rows), slots, offsets, num_groups, slot_offsets);
+    route_slot_offsets_kernel<<<(n + 7) / 8, 256, 0, stream>>>(places, static_cast<int>(num_rows), slots, offsets, num_groups, slot_offsets);
     launched("route_slot_offsets_kernel");
 }
 
