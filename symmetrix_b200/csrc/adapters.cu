@@ -406,19 +406,20 @@ Pass<T> make_pass(const smx_adapter_linear& c, bool transposed, T* hidden) {
     return p;
 }
 
-template <int HP>
+template <int HP, bool kWide>
 void launch_ts(const TsPass& t, long long tiles, cudaStream_t stream) {
-    using L = TsPassLayout<HP>;
+    using L = TsPassLayout<HP, kWide>;
+    const auto kernel = adapter_pass_f32_kernel<HP, kWide>;
     // the warps' shares of registers are drawn from what the launch gives: fewer than planned and they would wait for ever
     static std::atomic<bool> done[64];
     if (first_on_device(done)) {
         cudaFuncAttributes a{};
-        SMX_CUDA(cudaFuncGetAttributes(&a, adapter_pass_f32_kernel<HP>));
+        SMX_CUDA(cudaFuncGetAttributes(&a, kernel));
         if (a.numRegs < kTsRegsLaunch) throw CudaError("adapter_pass_f32_kernel was built with too few registers");
-        SMX_CUDA(cudaFuncSetAttribute(adapter_pass_f32_kernel<HP>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::smem));
+        SMX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::smem));
         mark_on_device(done);
     }
-    adapter_pass_f32_kernel<HP><<<static_cast<unsigned>(std::min<long long>(tiles, sm_count())), kTsPassThreads, L::smem, stream>>>(t);
+    kernel<<<static_cast<unsigned>(std::min<long long>(tiles, sm_count())), kTsPassThreads, L::smem, stream>>>(t);
     launched("adapter_pass_f32_kernel");
 }
 void launch_pass(const smx_adapter_linear& c, bool transposed, const Pass<float>& p, int degrees, cudaStream_t stream) {
@@ -443,10 +444,17 @@ void launch_pass(const smx_adapter_linear& c, bool transposed, const Pass<float>
             p.offsets, p.groups, p.pairs, p.order, p.places, p.slots, p.out, p.out_stride, static_cast<int>(transposed ? w.in : w.out));
         launched("adapter_zero_rows_kernel");
     }
-    if (padded_rank(p.rank) == 16) launch_ts<1>(t, tiles, stream);
-    else if (padded_rank(p.rank) == 32) launch_ts<2>(t, tiles, stream);
-    else if (padded_rank(p.rank) == 48) launch_ts<3>(t, tiles, stream);
-    else launch_ts<4>(t, tiles, stream);
+    bool wide = ((static_cast<unsigned long long>(p.out_stride) * 4u | reinterpret_cast<uintptr_t>(p.out)) & 31) == 0;
+    for (int q = 0; q < degrees; ++q) wide = wide && p.degree[q].out_off % 8 == 0 && p.degree[q].Nc % 64 == 0;
+    auto by_rank = [&](auto w) {
+        constexpr bool kWide = decltype(w)::value;
+        if (padded_rank(p.rank) == 16) launch_ts<1, kWide>(t, tiles, stream);
+        else if (padded_rank(p.rank) == 32) launch_ts<2, kWide>(t, tiles, stream);
+        else if (padded_rank(p.rank) == 48) launch_ts<3, kWide>(t, tiles, stream);
+        else launch_ts<4, kWide>(t, tiles, stream);
+    };
+    if (wide || !p.out) by_rank(std::true_type{});
+    else by_rank(std::false_type{});
 }
 
 // float64: tiles of 64 x 64, or of 16 x 32 while those leave SMs idle.

@@ -291,7 +291,7 @@ __device__ __forceinline__ void ts_bulk(uint32_t to, const float* from, uint32_t
 //               is these tiles in shared memory and 32 values of the rows in tensor memory, with one barrier for both
 //   warp 1      the products (one thread)
 //   warp 2      finds the tiles and looks up their atoms and weights (a ring of four, ahead of all others)
-//   warps 4-7   rows: a warp copies 32 values of each of its 32 rows asynchronously, 16 bytes a lane (4 where rows start on no 16-byte boundary), three
+//   warps 4-7   rows: a warp copies 32 values of each of its 32 rows asynchronously, 16 bytes a lane (4 where rows start on no 16-byte boundary), three or four
 //               chunks ahead; a thread splits those of its row and stores them to the tensor memory's row operand. (Loads and stores by
 //               the thread that owns a row touch 32 rows an instruction; a bulk copy takes 70 cycles to issue; one warp that copied for all
 //               four took longer than the products: 184 us instead of 160 at 98,304 atoms.)
@@ -302,26 +302,29 @@ __device__ __forceinline__ void ts_bulk(uint32_t to, const float* from, uint32_t
 // stored into the hidden columns of its last two sums (head in the last one's, remainder in the other's); the products with second_g go on
 // top of the last sum, which is read after them.
 // Every wait is bounded; if one runs out, the CTA gives up and fills its remaining tiles with NaN.
-constexpr int kTsPassThreads = 512, kTsWorkRing = 4, kTsRowStages = 4;
+constexpr int kTsPassThreads = 512, kTsWorkRing = 4;
 constexpr int kTsRowPitch = kTsChunk + 4;                                     // floats: threads that read their rows 16 bytes at a time hit all banks
 constexpr int kTsOutPitch = 17;                                               // floats of a row in the way out of rows that are not aligned
 constexpr int kTsRegsControl = 72, kTsRegsRows = 120, kTsRegsSums = 160, kTsRegsLaunch = 128;
 static_assert(kTsRegsControl + kTsRegsRows + 2 * kTsRegsSums <= 4 * kTsRegsLaunch, "the registers of the launch are shared out");
-template <int HP>                                    // hidden columns / 16
+// HP: hidden columns / 16. kWide: every row's half of a tile starts on 32 bytes and is 64 columns long, so nothing is staged on its way out and the
+// rows have five stages instead of four (160 us instead of 165 at 98,304 atoms, 128 channels, rank 32).
+template <int HP, bool kWide>
 struct TsPassLayout {
+    static constexpr int row_stages = kWide ? 5 : 4;
     static constexpr int Rp = 16 * HP, sum_cols = 128 + Rp, stages = HP > 2 ? 2 : 3;
     static constexpr int slot0 = 2 * sum_cols;
     static constexpr uint32_t stage_bytes = sum_cols * 256u;
     static constexpr int row_floats = kTsRows * kTsRowPitch;
-    static constexpr int smem = stages * static_cast<int>(stage_bytes) + (kTsRowStages * row_floats + 8 * 32 * kTsOutPitch) * 4 + 1024;
+    static constexpr int smem = stages * static_cast<int>(stage_bytes) + (row_stages * row_floats + (kWide ? 0 : 8 * 32 * kTsOutPitch)) * 4 + 1024;
     static_assert(slot0 + 64 * stages <= 512, "tensor memory has 512 columns");
     static_assert(smem + 14 * 1024 <= 227 * 1024, "shared memory of one CTA per SM");
 };
 
-template <int HP>
+template <int HP, bool kWide>
 __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(const __grid_constant__ TsPass pass) {
-    using L = TsPassLayout<HP>;
-    constexpr int NS = L::stages;
+    using L = TsPassLayout<HP, kWide>;
+    constexpr int NS = L::stages, RS = L::row_stages;
     extern __shared__ unsigned char ts_smem_raw[];
     __shared__ __align__(8) unsigned long long work_full[kTsWorkRing], work_free[kTsWorkRing], full[NS], free[NS], d_full[2], d_free[2], t_full, t_done;
     __shared__ TsWork work[kTsWorkRing];
@@ -506,7 +509,7 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
         int op = 0, na = 0, xs = 0;                  // operand stage and row stage in turn, operands so far
         unsigned op_par = 1;                         // parity of the operand stage's last use
         bool ok = true;
-        // copies run kTsRowStages - 1 chunks ahead of what is split, across tiles
+        // copies run row_stages - 1 chunks ahead of what is split, across tiles
         int ahead_tile = 0, ahead = 0, ahead_nx = 0, ahead_slot = 0, ahead_Kd = 0, ahead_rows = 0;
         bool more = true, wide = false;
         const float* from = nullptr;
@@ -539,7 +542,7 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
 #pragma unroll 4
                         for (int r = lane >> 3; r < ahead_rows; r += 4) cp_async16(to + r * kTsRowPitch + c, from + where[r] + c, 16);
                 } else if (lane < left) {
-#pragma unroll 1
+#pragma unroll 4
                     for (int r = 0; r < ahead_rows; ++r) cp_async4(to + r * kTsRowPitch + lane, from + where[r] + lane);
                 }
                 from += kTsChunk;
@@ -547,7 +550,7 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
             }
             cp_async_commit();
         };
-        for (int q = 0; q < kTsRowStages - 1; ++q) copy_next(q);
+        for (int q = 0; q < RS - 1; ++q) copy_next(q);
         for (int i = 0; ok; ++i) {
             const int slot = i % kTsWorkRing;
             if (!ts_wait_warp(&work_full[slot], (i / kTsWorkRing) & 1, &failed)) break;
@@ -563,9 +566,9 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
             for (int j = 0; j < s.nx + s.rounds; ++j) {
                 const bool inner = j < s.nx;
                 if (inner) {
-                    cp_async_wait<kTsRowStages - 2>();
+                    cp_async_wait<RS - 2>();
                     __syncwarp();                    // the chunk is there for all lanes, and all have read the one before
-                    copy_next(xs == 0 ? kTsRowStages - 1 : xs - 1);
+                    copy_next(xs == 0 ? RS - 1 : xs - 1);
                     if (!ok) break;
                 }
                 if (na >= NS && !ts_wait_warp(&free[op], op_par, &failed)) { ok = false; break; }
@@ -579,7 +582,7 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
                 }
                 ts_fence_after();
                 const float* row = row_stages + xs * L::row_floats + tid * kTsRowPitch;
-                if (++xs == kTsRowStages) xs = 0;
+                if (++xs == RS) xs = 0;
                 const int good = live ? Kd - j * kTsChunk : 0;           // what the stage holds behind the tile's or the row's end is no value
 #pragma unroll 1
                 for (int q = 0; q < kTsChunk; q += 16) {
@@ -612,7 +615,7 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
         const int tid = threadIdx.x & 127, half = (warp - 8) >> 2, R = pass.rank;
         constexpr int kLower = (HP + 1) / 2;         // blocks of 16 hidden columns of the lower half; the upper half has the others
         const int hid0 = half ? kLower : 0, hid_blocks = half ? HP - kLower : kLower;
-        float* const out_stage = row_stages + kTsRowStages * L::row_floats + (warp - 8) * 32 * kTsOutPitch;
+        float* const out_stage = row_stages + RS * L::row_floats + (warp - 8) * 32 * kTsOutPitch;
         const unsigned long long out_bits = static_cast<unsigned long long>(pass.out_stride) * 4u | reinterpret_cast<uintptr_t>(pass.out);
         int nd = 0, nt = 0, i = 0;                   // partial sums and hidden rows used so far, tiles
         bool ok = true;
@@ -645,7 +648,7 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
             if (live && pass.out) out_row = pass.out + out_at + s.col0 + 64 * half;
             if (live && s.adapter && d.hidden && w.block == 0) hid_row = d.hidden + (static_cast<long long>(place) * d.comps + comp) * R + 16 * hid0;
             const int left = d.Nc - s.col0 - 64 * half;                  // columns of this half that exist
-            const bool out_wide = left >= 64 && ((out_bits | 4u * static_cast<unsigned>(d.out_off | d.Nc)) & 31) == 0;
+            const bool out_wide = kWide ? left >= 64 : left >= 64 && ((out_bits | 4u * static_cast<unsigned>(d.out_off | d.Nc)) & 31) == 0;
             float sum[64], hid[16 * kLower];
 #pragma unroll
             for (int q = 0; q < 64; ++q) sum[q] = 0.f;
@@ -657,7 +660,7 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
                         for (int q = 0; q < 64; q += 8)
                             asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];" : "=f"(sum[q]), "=f"(sum[q + 1]), "=f"(sum[q + 2]), "=f"(sum[q + 3]),
                                          "=f"(sum[q + 4]), "=f"(sum[q + 5]), "=f"(sum[q + 6]), "=f"(sum[q + 7]) : "l"(out_row + q) : "memory");
-                } else {
+                } else if constexpr (!kWide) {
                     const unsigned long long mine = reinterpret_cast<unsigned long long>(out_row);
 #pragma unroll
                     for (int c0 = 0; c0 < 64; c0 += 16) {
@@ -762,7 +765,7 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
                     for (int q = 0; q < 64; q += 8)
                         asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out_row + q), "f"(sum[q]), "f"(sum[q + 1]), "f"(sum[q + 2]),
                                      "f"(sum[q + 3]), "f"(sum[q + 4]), "f"(sum[q + 5]), "f"(sum[q + 6]), "f"(sum[q + 7]) : "memory");
-            } else if (pass.out) {
+            } else if (!kWide && pass.out) {
                 // 16 columns of the warp's rows at a time through shared memory, so that a store touches two rows instead of 32
                 const unsigned long long mine = reinterpret_cast<unsigned long long>(out_row);
 #pragma unroll
