@@ -323,6 +323,32 @@ def test_linear_without_rows(dtype, slots):
     assert all((g == 0).all() for g in (*grads.down, *grads.up))
 
 
+MANY_SLOTS = [
+    # plans of one CTA and of several, rows that are aligned and not, more than one block of columns, the most slots
+    ([1], [221], [221], 6000, 2, 1, 38),
+    ([1, 3], [44, 44], [44, 44], 3100, 3, 40, 14),
+    ([1, 3], [128, 128], [192, 192], 4500, 2, 5, 24),
+    ([1], [72], [264], 70, 64, 9, 4),
+    ([2], [64], [64], 200, 64, 3, 64),
+    ([1], [19], [3], 1, 64, 2, 1),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+@pytest.mark.parametrize("shape", MANY_SLOTS, ids=lambda s: "x".join(str(v).replace(" ", "") for v in s))
+@pytest.mark.parametrize("kind", ["random", "same", "outside"])
+def test_linear_with_many_slots(dtype, shape, kind):
+    """Every slot adds to what the slots before it left; "same" gives a row's slots one adapter, which counts as often as it is listed."""
+    for shared in (True, False):
+        case = Case(dtype, *shape, kind="random" if kind == "same" else kind, shared=shared)
+        if kind == "same":
+            case.ids = case.ids[:, :1].expand(-1, case.slots).contiguous()
+        _, _, y, grads = everything(case)
+        case.check(y, grads)
+        _, _, again, other = everything(case)
+        assert torch.equal(y, again) and torch.equal(grads.x, other.x) and torch.equal(grads.weights, other.weights)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
 def test_unused_adapters_and_other_requests_do_not_matter(dtype):
     """Adapters that nobody names may hold anything; an atom's result does not depend on the batch it is in beyond its roundings."""
