@@ -90,7 +90,8 @@ __device__ __forceinline__ bool find_tile(const int* __restrict__ offsets, int g
 }
 
 // ------------------------------------------------------------------------------------------- gradients of the adapters
-// part[chunk][k][r] = sum over the chunk's rows of a[row][k] weight[row] h[row][r]; a is x with h = gy B^T, or gy with h = x A.
+// part[chunk][k][r] = sum over the chunk's rows of a[row][k] weight[row] h[row][r]; a is x with h = gy B^T, or gy with h = x A. A chunk has 512 rows,
+// fewer where those would leave SMs idle (818 atoms of 2 slots and 26 channels, rank 55: 23 us with 64 rows, 118 with 512).
 constexpr int kGradChunk = 512;
 template <typename T>
 struct GradProblem {
@@ -103,7 +104,7 @@ struct GradProblem {
 template <typename T>
 struct GradPass {
     GradProblem<T> problem[2 * kMaxDegrees];
-    int rank, groups, slots;
+    int rank, groups, slots, chunk;
     long long pairs;
     const int* order; const int* offsets;
     const T* weights;
@@ -118,12 +119,12 @@ __global__ void __launch_bounds__(256) adapter_grad_sum_kernel(const __grid_cons
     if (threadIdx.x < 32) {
         long long before = 0;
         for (int q = threadIdx.x; q < g; q += 32)
-            before += (static_cast<long long>(pass.offsets[q + 1] - pass.offsets[q]) * d.comps + kGradChunk - 1) / kGradChunk;
+            before += (static_cast<long long>(pass.offsets[q + 1] - pass.offsets[q]) * d.comps + pass.chunk - 1) / pass.chunk;
 #pragma unroll
         for (int s = 16; s > 0; s >>= 1) before += __shfl_xor_sync(0xffffffffu, before, s);
         if (threadIdx.x == 0) {
             sh[0] = before;
-            sh[1] = (static_cast<long long>(pass.offsets[g + 1] - pass.offsets[g]) * d.comps + kGradChunk - 1) / kGradChunk;
+            sh[1] = (static_cast<long long>(pass.offsets[g + 1] - pass.offsets[g]) * d.comps + pass.chunk - 1) / pass.chunk;
         }
     }
     __syncthreads();
@@ -239,8 +240,21 @@ struct Workspace {
     }
 };
 
+int grad_chunk(const smx_adapter_linear& c) {
+    const int cols = c.precision == SMX_FP64 ? kDpGradK : 128;           // inner indices of a CTA
+    int chunk = kGradChunk;
+    for (; chunk > 64; chunk /= 2) {
+        long long ctas = 0;
+        for (int d = 0; d < c.num_degrees; ++d) {
+            const smx_adapter_degree& g = c.degrees[d];
+            ctas += (static_cast<long long>(c.num_rows) * c.slots * g.components / chunk) * ((g.in_channels + cols - 1) / cols + (g.out_channels + cols - 1) / cols);
+        }
+        if (ctas >= 296) break;                                          // two per SM; a constant, so that sizes do not depend on the device
+    }
+    return chunk;
+}
 long long grad_chunks(const smx_adapter_linear& c, int comps) {
-    return static_cast<long long>(c.num_rows) * c.slots * comps / kGradChunk + c.num_groups;
+    return static_cast<long long>(c.num_rows) * c.slots * comps / grad_chunk(c) + c.num_groups;
 }
 
 template <typename T>
@@ -486,16 +500,17 @@ void launch_pass(const smx_adapter_linear&, bool, const Pass<double>& p, int deg
     auto tiles = [&](int BM, int BN) {
         long long n = 0;
         for (int q = 0; q < degrees; ++q) {
-            const long long rows = p.pairs * p.degree[q].comps;
-            const bool all = !p.out || (BM == 64 && !p.degree[q].W);         // one CTA makes all blocks of columns
-            n += (rows / BM + p.groups + 1) * (all ? 1 : (p.degree[q].Nc + BN - 1) / BN);
+            const bool all = !p.out || (t.whole && !p.degree[q].W);          // one CTA makes all blocks of columns
+            n += (p.pairs * p.degree[q].comps / BM + p.groups + 1) * (all ? 1 : (p.degree[q].Nc + BN - 1) / BN);
         }
         return n;
     };
     auto by_rank = [&](auto nr) {
         constexpr int NR = decltype(nr)::value;
-        if (tiles(64, 64) <= 2LL * sm_count()) launch_dp<16, 32, 1, 4, NR, 4>(t, tiles(16, 32), stream);
-        else launch_dp<64, 64, 2, 2, NR, 2>(t, tiles(64, 64), stream);
+        t.whole = 1;
+        if (tiles(64, 64) > 2LL * sm_count()) { launch_dp<64, 64, 2, 2, NR, 2>(t, tiles(64, 64), stream); return; }
+        t.whole = tiles(16, 32) > 2LL * sm_count();
+        launch_dp<16, 32, 1, 4, NR, 4>(t, tiles(16, 32), stream);
     };
     if (p.rank <= 8) by_rank(std::integral_constant<int, 1>{});
     else if (p.rank <= 16) by_rank(std::integral_constant<int, 2>{});
@@ -508,9 +523,9 @@ void launch_grads(const GradPass<double>& gp, int problems, cudaStream_t stream)
     long long ctas = 0;
     for (int q = 0; q < problems; ++q) {
         t.problem[q] = gp.problem[q];
-        ctas += (gp.pairs * gp.problem[q].comps / kGradChunk + gp.groups) * ((gp.problem[q].Kd + kDpGradK - 1) / kDpGradK);
+        ctas += (gp.pairs * gp.problem[q].comps / gp.chunk + gp.groups) * ((gp.problem[q].Kd + kDpGradK - 1) / kDpGradK);
     }
-    t.problems = problems; t.rank = gp.rank; t.groups = gp.groups; t.slots = gp.slots; t.pairs = gp.pairs;
+    t.problems = problems; t.rank = gp.rank; t.groups = gp.groups; t.slots = gp.slots; t.chunk = gp.chunk; t.pairs = gp.pairs;
     t.order = gp.order; t.offsets = gp.offsets; t.weights = gp.weights;
     if (ctas > INT_MAX) throw ArgError("smx_adapter: too many rows");
     const auto kernel = gp.rank <= 8 ? adapter_grad_f64_kernel<1> : gp.rank <= 16 ? adapter_grad_f64_kernel<2> : gp.rank <= 32 ? adapter_grad_f64_kernel<4> : adapter_grad_f64_kernel<8>;
@@ -522,9 +537,9 @@ void launch_grads(const GradPass<float>& gp, int problems, cudaStream_t stream) 
     long long ctas = 0;
     for (int q = 0; q < problems; ++q) {
         t.problem[q] = gp.problem[q];
-        ctas += (gp.pairs * gp.problem[q].comps / kGradChunk + gp.groups) * ts_blocks(gp.problem[q].Kd);
+        ctas += (gp.pairs * gp.problem[q].comps / gp.chunk + gp.groups) * ts_blocks(gp.problem[q].Kd);
     }
-    t.problems = problems; t.rank = gp.rank; t.groups = gp.groups; t.slots = gp.slots; t.pairs = gp.pairs;
+    t.problems = problems; t.rank = gp.rank; t.groups = gp.groups; t.slots = gp.slots; t.chunk = gp.chunk; t.pairs = gp.pairs;
     t.order = gp.order; t.offsets = gp.offsets; t.weights = gp.weights;
     if (ctas > INT_MAX) throw ArgError("smx_adapter: too many rows");
     const int NH = padded_rank(gp.rank) / 16;
@@ -535,7 +550,7 @@ void launch_grads(const GradPass<float>& gp, int problems, cudaStream_t stream) 
         mark_on_device(done);
     }
     const auto kernel = NH == 1 ? adapter_grad_f32_kernel<1> : NH == 2 ? adapter_grad_f32_kernel<2> : NH == 3 ? adapter_grad_f32_kernel<3> : adapter_grad_f32_kernel<4>;
-    kernel<<<static_cast<unsigned>(ctas), kTsThreads, kGradChunk * 16 * NH * static_cast<int>(sizeof(float)), stream>>>(t);
+    kernel<<<static_cast<unsigned>(ctas), kTsThreads, std::max(gp.chunk, 128) * 16 * NH * static_cast<int>(sizeof(float)), stream>>>(t);
     launched("adapter_grad_f32_kernel");
 }
 
@@ -606,7 +621,7 @@ void backward(const smx_adapter_linear& c) {
         hidden = b.hidden;
     }
     GradPass<T> gp{};
-    gp.rank = c.rank; gp.groups = c.num_groups; gp.slots = c.slots; gp.pairs = static_cast<long long>(pairs);
+    gp.rank = c.rank; gp.groups = c.num_groups; gp.slots = c.slots; gp.chunk = grad_chunk(c); gp.pairs = static_cast<long long>(pairs);
     gp.order = c.order; gp.offsets = c.offsets; gp.weights = static_cast<const T*>(c.weights);
     WeightGrad<T> wg{};
     long long in_off = 0, out_off = 0, hid_off = 0;

@@ -801,7 +801,7 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
 // ------------------------------------------------------------------------------------------- gradients of the adapters
 struct TsGrad {
     GradProblem<float> problem[2 * SMX_ADAPTER_MAX_DEGREES];
-    int problems, rank, groups, slots;
+    int problems, rank, groups, slots, chunk;
     long long pairs;
     const int* order; const int* offsets;
     const float* weights;
@@ -817,7 +817,7 @@ __global__ void __launch_bounds__(kTsThreads, NH == 4 ? 3 : 4) adapter_grad_f32_
     constexpr int Rp = 16 * NH, kPer = 4, kCols = 32 * kPer, kAhead = 4;               // inner indices of a lane, of the CTA
     constexpr int kRowWarps = NH == 1 ? 4 : NH == 2 ? 2 : 1;                             // warps that share the rows of 16 hidden columns
     extern __shared__ __align__(16) unsigned char ts_smem_raw[];
-    float* const hs = reinterpret_cast<float*>(ts_smem_raw);                             // [kGradChunk][Rp], afterwards the warps' sums [Rp][kCols]
+    float* const hs = reinterpret_cast<float*>(ts_smem_raw);                             // [chunk][Rp], afterwards the warps' sums [Rp][kCols]
     __shared__ long long a_base[kGradChunk];
     __shared__ float row_weight[kGradChunk];
     __shared__ TileRows tile;
@@ -830,7 +830,7 @@ __global__ void __launch_bounds__(kTsThreads, NH == 4 ? 3 : 4) adapter_grad_f32_
         int hit = -1, kb = 0;
         for (int q = 0; q < pass.problems; ++q) {
             const int blocks = (pass.problem[q].Kd + kCols - 1) / kCols;
-            if (find_tile(pass.offsets, pass.groups, false, pass.pairs, pass.problem[q].comps, kGradChunk, t / blocks, rows, tiles)) {
+            if (find_tile(pass.offsets, pass.groups, false, pass.pairs, pass.problem[q].comps, pass.chunk, t / blocks, rows, tiles)) {
                 hit = q; kb = static_cast<int>(t % blocks); t /= blocks;
                 break;
             }

@@ -42,6 +42,7 @@ struct DpPass {
     const double* in; long long in_stride;
     double* out; long long out_stride;
     int add, tail;                               // as in Pass
+    int whole;                                   // a CTA makes all blocks of columns of a tile without shared weights
 };
 
 __device__ __forceinline__ void dp_copy16(double* smem, const double* gmem, int bytes) { cp_async16(smem, gmem, bytes); }
@@ -59,8 +60,10 @@ struct DpLayout {
 
 // A CTA of four warps (WM x WN) makes BM rows x BN columns of one degree and adapter: in . W and in . first_g from the same row fragments (the warps of
 // a row of warps share the inner values of the latter among them and add up through shared memory), then the weighted hidden rows times
-// second_g on top. ST stages of 16 inner values are in flight. NR: hidden columns / 8. Without shared weights
-// a CTA of big tiles makes all blocks of columns from one hidden tile.
+// second_g on top. ST stages of 16 inner values are in flight. NR: hidden columns / 8.
+// A tile without shared weights makes its blocks of columns one after another from one hidden tile, unless its CTAs are few (11,772 rows of 256
+// channels, rank 4: 31 us, and 116 with a CTA for every block). Measured with shared weights: 80,120 rows of 128 channels, rank 8: 140 us, 19 TFLOP/s;
+// 28,260 of rank 32: 137 us. The double-precision pipes bound it, with the waits of tiles that run in less than two full rounds of the SMs.
 template <int BM, int BN, int WM, int WN, int NR, int ST>
 __global__ void __launch_bounds__(kDpThreads) adapter_pass_f64_kernel(const __grid_constant__ DpPass pass) {
     using L = DpLayout<BM, BN, NR, ST>;
@@ -78,7 +81,7 @@ __global__ void __launch_bounds__(kDpThreads) adapter_pass_f64_kernel(const __gr
         long long at = blockIdx.x;
         for (int q = 0; q < pass.degrees && hit < 0; ++q) {
             const DpDegree& d = pass.degree[q];
-            const int blocks = pass.out && !(BM == 64 && !d.W) ? (d.Nc + BN - 1) / BN : 1;
+            const int blocks = pass.out && (!pass.whole || d.W) ? (d.Nc + BN - 1) / BN : 1;
             const long long row_tile = at / blocks;
             long long tiles;
             if (find_tile(pass.offsets, pass.groups, pass.tail != 0, pass.pairs, d.comps, BM, row_tile, t, tiles)) { hit = q; cb = static_cast<int>(at % blocks); }
@@ -244,7 +247,7 @@ __global__ void __launch_bounds__(kDpThreads) adapter_pass_f64_kernel(const __gr
         if (!pass.out) return;
         __syncthreads();
     }
-    const int end = BM == 64 && !d.W ? d.Nc : min(d.Nc, col0 + BN);
+    const int end = pass.whole && !d.W ? d.Nc : min(d.Nc, col0 + BN);
     for (;;) {
         if (adapter)
 #pragma unroll 2
@@ -291,7 +294,7 @@ __global__ void __launch_bounds__(kDpThreads) adapter_pass_f64_kernel(const __gr
 // of them and all hidden columns; 16 rows a step, double-buffered.
 struct DpGrad {
     GradProblem<double> problem[2 * SMX_ADAPTER_MAX_DEGREES];
-    int problems, rank, groups, slots;
+    int problems, rank, groups, slots, chunk;
     long long pairs;
     const int* order; const int* offsets;
     const double* weights;
@@ -314,7 +317,7 @@ __global__ void __launch_bounds__(kDpThreads) adapter_grad_f64_kernel(const __gr
         int hit = -1, kb = 0;
         for (int q = 0; q < pass.problems; ++q) {
             const int blocks = (pass.problem[q].Kd + kDpGradK - 1) / kDpGradK;
-            if (find_tile(pass.offsets, pass.groups, false, pass.pairs, pass.problem[q].comps, kGradChunk, t / blocks, rows, tiles)) {
+            if (find_tile(pass.offsets, pass.groups, false, pass.pairs, pass.problem[q].comps, pass.chunk, t / blocks, rows, tiles)) {
                 hit = q; kb = static_cast<int>(t % blocks); t /= blocks;
                 break;
             }
@@ -326,7 +329,7 @@ __global__ void __launch_bounds__(kDpThreads) adapter_grad_f64_kernel(const __gr
     if (which < 0) return;
     const GradProblem<double>& d = pass.problem[which];
     const int R = pass.rank, rows = static_cast<int>(tile.rows), k0 = k_block * kDpGradK;
-    for (int i = tid; i < kGradChunk; i += kDpThreads) {
+    for (int i = tid; i < pass.chunk; i += kDpThreads) {
         long long base = -1;
         double w = 0.0;
         if (i < rows) {
