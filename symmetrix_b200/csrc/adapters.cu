@@ -221,6 +221,10 @@ void check_plan(const smx_adapter_linear& c) {
     if (!c.tiles) throw ArgError("smx_adapter: null tiles");
     check_aligned(c);
     if (!c.offsets || (c.num_rows > 0 && (!c.order || !c.position))) throw ArgError("smx_adapter: null plan");
+    check_pointers("smx_adapter", sizeof(int), {c.order, c.position, c.offsets});
+    const size_t value = c.precision == SMX_FP32 ? sizeof(float) : sizeof(double);
+    check_pointers("smx_adapter", value, {c.x, c.y, c.grad_y, c.grad_x, c.weights, c.grad_weights});
+    for (int d = 0; d < c.num_degrees; ++d) check_pointers("smx_adapter", value, {c.degrees[d].grad_down, c.degrees[d].grad_up});
 }
 
 void check_rows(const char* what, const void* p, long stride, long width, long rows, bool written) {
@@ -324,8 +328,11 @@ size_t tile_layout(const smx_adapter_linear& c, Matrices (&m)[kMaxDegrees]) {
 void prepare(const smx_adapter_linear& c, int parts) {
     Matrices m[kMaxDegrees];
     const cudaStream_t stream = static_cast<cudaStream_t>(c.stream);
-    for (int d = 0; d < c.num_degrees; ++d)
+    for (int d = 0; d < c.num_degrees; ++d) {
+        check_pointers("smx_adapter_prepare", c.precision == SMX_FP32 ? sizeof(float) : sizeof(double), {(parts & SMX_ADAPTER_SHARED) ? c.degrees[d].shared : nullptr,
+                       (parts & SMX_ADAPTER_MATRICES) ? c.degrees[d].down : nullptr, (parts & SMX_ADAPTER_MATRICES) ? c.degrees[d].up : nullptr});
         if ((parts & SMX_ADAPTER_MATRICES) && (!c.degrees[d].down || !c.degrees[d].up)) throw ArgError("smx_adapter_prepare: null matrix");
+    }
     int n = 0;
     long long most = 0;
     if (c.precision == SMX_FP64) {

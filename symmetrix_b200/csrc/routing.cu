@@ -370,6 +370,13 @@ RowGrid row_grid(long num_rows, long units) {
     return {dim3(static_cast<unsigned>(std::max(1LL, std::min<long long>(blocks, 64LL * sm_count())))), dim3(tx, ty)};
 }
 
+}  // namespace
+void check_pointers(const char* what, size_t bytes, std::initializer_list<const void*> pointers) {
+    for (const void* p : pointers)
+        if (reinterpret_cast<uintptr_t>(p) % bytes) throw ArgError(std::string(what) + ": an array does not start on a multiple of its elements' size");
+}
+namespace {
+
 void launched(const char* what) {
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) throw CudaError(std::string(what) + ": " + cudaGetErrorString(e));
@@ -446,6 +453,7 @@ void counting_sort(const int* ids, long long pairs, int num_groups, int* order, 
 void route_plan(const int* ids, long num_rows, int slots, int num_groups, int* order, int* position, int* offsets, void* workspace,
                 size_t workspace_bytes, cudaStream_t stream) {
     const size_t need = route_plan_bytes(num_rows, slots, num_groups);
+    check_pointers("smx_route_plan", sizeof(int), {ids, order, position, offsets, workspace});
     const long long pairs = static_cast<long long>(num_rows) * slots;
     if (!offsets || (pairs > 0 && (!ids || !order || !position))) throw ArgError("smx_route_plan: null pointer");
     if (workspace_bytes < need || (need && !workspace)) throw ArgError("smx_route_plan: the workspace is smaller than smx_route_plan_bytes says");
@@ -468,6 +476,8 @@ void route_dispatch(const T* x, long x_stride, long num_rows, int slots, long wi
     check_width("smx_route_dispatch", width, x_stride);
     if (num_rows == 0 || width == 0) return;
     if (!x || !position || !offsets || !rows) throw ArgError("smx_route_dispatch: null pointer");
+    check_pointers("smx_route_dispatch", sizeof(int), {position, offsets});
+    check_pointers("smx_route_dispatch", sizeof(T), {x, rows});
     auto go = [&](auto unit) {
         using V = decltype(unit);
         constexpr long per = sizeof(V) / sizeof(T);
@@ -488,6 +498,8 @@ void route_combine(const T* rows, const int* position, long num_rows, int slots,
     check_width("smx_route_combine", width, y_stride);
     if (num_rows == 0 || width == 0) return;
     if (!rows || !position || !y) throw ArgError("smx_route_combine: null pointer");
+    check_pointers("smx_route_combine", sizeof(int), {position});
+    check_pointers("smx_route_combine", sizeof(T), {rows, weights, base, y});
     if (y_stride < width && num_rows > 1) throw ArgError("smx_route_combine: the output's rows overlap");
     if (!base) base_stride = 0;
     auto go = [&](auto unit) {
@@ -511,6 +523,8 @@ void route_combine_backward(const T* grad_y, long grad_y_stride, const T* rows, 
     check_width("smx_route_combine_backward", width, grad_y_stride);
     if (num_rows == 0) return;
     if (!position || !offsets || (width > 0 && (!grad_y || !grad_rows || (grad_weights && !rows)))) throw ArgError("smx_route_combine_backward: null pointer");
+    check_pointers("smx_route_combine_backward", sizeof(int), {position, offsets});
+    check_pointers("smx_route_combine_backward", sizeof(T), {grad_y, rows, weights, grad_rows, grad_weights});
     auto go = [&](auto unit) {
         using V = decltype(unit);
         constexpr long per = sizeof(V) / sizeof(T);

@@ -3,6 +3,7 @@
 // failures throw (common.cuh).
 #pragma once
 
+#include <initializer_list>
 #include <cuda_runtime.h>
 
 #include <atomic>
@@ -22,6 +23,8 @@ void mark_on_device(std::atomic<bool> (&done)[64]);
 size_t route_plan_bytes(long num_rows, int slots, int num_groups);
 void route_plan(const int* ids, long num_rows, int slots, int num_groups, int* order, int* position, int* offsets, void* workspace,
                 size_t workspace_bytes, cudaStream_t stream);
+// Refuses pointers that do not start on a multiple of `bytes` (kernels would fault on them).
+void check_pointers(const char* what, size_t bytes, std::initializer_list<const void*> pointers);
 // The plan slot by slot: places[s * num_rows ..] are the sorted positions of slot s's pairs, ascending, so grouped, empty ones last;
 // slot_offsets[s * (num_groups + 1) + g] is where group g begins among them. A row is in every slot's list once.
 size_t route_slots_bytes(long num_rows, int slots);

@@ -102,6 +102,26 @@ def test_backward_refusals(over, message):
     assert status == _lib.SMX_ERR_INVALID_ARGUMENT and message in text
 
 
+def test_arrays_off_their_elements_boundaries_are_refused():
+    lib, odd = _lib.load(), P + 4
+    row = {"smx_route_plan": (P + 2, 4, 1, 2, P, P, P, None, 0, None),
+           "smx_route_dispatch": (64, odd, 8, 4, 1, 8, P, P, 1, P, 0, None),
+           "smx_route_combine": (64, P, P, 4, 1, 8, odd, None, 0, P, 8, None),
+           "smx_route_combine_backward": (64, P, 8, P, P, P, 1, 4, 1, 8, None, odd, P, 0, None)}
+    for name, args in row.items():
+        status, text = _status(getattr(lib, name), *args)
+        assert status == _lib.SMX_ERR_INVALID_ARGUMENT and "multiple" in text, name
+    for over in ({"x": odd}, {"y": odd}, {"weights": odd}, {"order": P + 2}, {"offsets": P + 1}):
+        status, text = _status(lib.smx_adapter_forward, ctypes.byref(_adapter_call(**over)))
+        assert status == _lib.SMX_ERR_INVALID_ARGUMENT and "multiple" in text, over
+    for over in ({"grad_y": odd}, {"grad_x": odd}, {"grad_weights": odd}, {"degree_grad_down": odd, "degree_grad_up": P}):
+        status, text = _status(lib.smx_adapter_backward, ctypes.byref(_adapter_call(**over)))
+        assert status == _lib.SMX_ERR_INVALID_ARGUMENT and "multiple" in text, over
+    for over in ({"degree_shared": odd}, {"degree_down": odd}, {"degree_up": odd}):
+        status, text = _status(lib.smx_adapter_prepare, ctypes.byref(_adapter_call(**over)), 3)
+        assert status == _lib.SMX_ERR_INVALID_ARGUMENT and "multiple" in text, over
+
+
 def test_prepare_refusals_and_null_calls():
     lib = _lib.load()
     assert _status(lib.smx_adapter_prepare, ctypes.byref(_adapter_call(degree_down=None)), 2)[0] == _lib.SMX_ERR_INVALID_ARGUMENT
