@@ -396,8 +396,10 @@ int smx_adapter_backward(const smx_adapter_linear* call, char* errbuf, int errbu
  * takes a linear's away. smx_assign_adapters names the adapters of nodes 0 .. num_nodes - 1 (host arrays ids[num_nodes * slots], weights of the
  * same size or NULL for ones), as smx_route_plan reads them: an id outside the adapters is an empty slot, a node without any runs the model as it is. The
  * assignment stays until the next one (0 nodes: none, the model for all) or until the number of adapters changes; an evaluation with more nodes
- * than assigned is refused, one with fewer uses the first. smx_adapter_gradients returns, after a whole evaluation, the gradients of the
- * total energy by a linear's adapters (in the layout of smx_set_adapters) and by the weights [active nodes * slots]; any may be NULL. */
+ * than assigned is refused, one with fewer uses the first. smx_set_adapters or smx_assign_adapters that fail on the way (not for their arguments)
+ * leave the linear without adapters, or no assignment. smx_adapter_gradients returns, after a whole evaluation, the gradients of the
+ * total energy by a linear's adapters (in the layout of smx_set_adapters) and by the weights [active nodes * slots]; any may be NULL; a new edge set or
+ * a compute_* stage since then and it is refused until the stages have gone back through the linear. */
 int smx_set_adapters(smx_handle h, const char* linear, int num_adapters, int rank, const double* down, long down_count,
                      const double* up, long up_count);
 int smx_assign_adapters(smx_handle h, int num_nodes, int slots, const int* ids, const double* weights);

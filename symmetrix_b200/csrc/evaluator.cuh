@@ -482,7 +482,10 @@ public:
     void adopt_edges(int n_nodes, long n_edges, bool keep = false, bool rescan = true) {
         N = n_nodes;
         E = n_edges;
-        if (!keep) { h1_rows = N; hm_rows = N; }
+        if (!keep) {
+            h1_rows = N; hm_rows = N;
+            for (auto& a : adapters) a.second.hidden_nodes = -1;
+        }
         sender_rows = -1;
         radial_hidden_valid = false;
         if (rescan) first_host_valid = false;
@@ -804,6 +807,7 @@ public:
 
     void compute_A0() {   // MACE::compute_A0, mace.cpp:150-201
         const int K = model.K;
+        adapters_stale();
         if (!fold_a0) Phi0.resize(static_cast<size_t>(N) * kNumLm * K, stream);
         A0.resize(static_cast<size_t>(N) * kNumLm * K, stream);
         if (N == 0) return;
@@ -978,7 +982,12 @@ public:
         DevBuf<unsigned char> tiles;
         DevBuf<T> hidden;                                         // in . down of the last forward pass, for the gradients
         int hidden_nodes = -1;
+        bool reversed = false;                                    // the adjoints belong to the same evaluation
     };
+    // The arrays of the last whole evaluation are about to change: no gradients until the next one has gone back through the linear.
+    void adapters_stale() {
+        for (auto& a : adapters) a.second.reversed = false;
+    }
     std::map<std::string, AdapterSet> adapters;
     int num_adapters = 0;                                         // of every linear that has some
     DevBuf<int> adapter_ids, adapter_plan;                        // as assigned; order, position and offsets of the first `adapter_planned` nodes
@@ -1078,6 +1087,7 @@ public:
         smx_adapter_linear c = adapter_call(name);
         a.hidden.resize(adapter_hidden_elements(c), stream);
         a.hidden_nodes = N;
+        a.reversed = false;
         c.x = x; c.y = y; c.hidden = a.hidden.p;
         adapter_run(c, false);
     }
@@ -1085,6 +1095,8 @@ public:
         smx_adapter_linear c = adapter_call(name);
         c.grad_y = grad_y; c.grad_x = grad_x;
         adapter_run(c, true);
+        AdapterSet& a = adapters.at(name);
+        a.reversed = a.hidden_nodes == N;
     }
 
     void set_adapters(const std::string& name, int count, int rank, const double* down, long down_count, const double* up, long up_count) override {
@@ -1111,24 +1123,29 @@ public:
         if (down_count != static_cast<long>(want_down) || up_count != static_cast<long>(want_up))
             throw ArgError("smx_set_adapters: " + name + " takes " + std::to_string(want_down) + " and " + std::to_string(want_up) + " values");
         if (count != num_adapters) drop_assignment(count);
-        AdapterSet& a = adapters[name];
-        a.rank = rank;
-        a.hidden_nodes = -1;
-        a.tiles.resize(bytes, stream);
-        c.tiles = a.tiles.p;
-        DevBuf<T> d_down, d_up;
-        d_down.upload(cast_vec<T>(adapter_paths(name, down, count, rank, true)), stream);
-        d_up.upload(cast_vec<T>(std::vector<double>(up, up + want_up)), stream);
-        const T *at_down = d_down.p, *at_up = d_up.p;
-        for (int l = 0; l < c.num_degrees; ++l) {
-            c.degrees[l].down = at_down; c.degrees[l].up = at_up;
-            at_down += static_cast<size_t>(count) * c.degrees[l].in_channels * rank;
-            at_up += static_cast<size_t>(count) * c.degrees[l].out_channels * rank;
+        adapters.erase(name);
+        try {
+            AdapterSet& a = adapters[name];
+            a.rank = rank;
+            a.tiles.resize(bytes, stream);
+            c.tiles = a.tiles.p;
+            DevBuf<T> d_down, d_up;
+            d_down.upload(cast_vec<T>(adapter_paths(name, down, count, rank, true)), stream);
+            d_up.upload(cast_vec<T>(std::vector<double>(up, up + want_up)), stream);
+            const T *at_down = d_down.p, *at_up = d_up.p;
+            for (int l = 0; l < c.num_degrees; ++l) {
+                c.degrees[l].down = at_down; c.degrees[l].up = at_up;
+                at_down += static_cast<size_t>(count) * c.degrees[l].in_channels * rank;
+                at_up += static_cast<size_t>(count) * c.degrees[l].out_channels * rank;
+            }
+            const long before = operator_launches;
+            adapter_prepare(c, SMX_ADAPTER_SHARED | SMX_ADAPTER_MATRICES);
+            launches += operator_launches - before;
+            SMX_CUDA(cudaStreamSynchronize(stream));                  // the uploads are temporary
+        } catch (...) {                                           // matrices that are only half there are not kept
+            adapters.erase(name);
+            throw;
         }
-        const long before = operator_launches;
-        adapter_prepare(c, SMX_ADAPTER_SHARED | SMX_ADAPTER_MATRICES);
-        launches += operator_launches - before;
-        SMX_CUDA(cudaStreamSynchronize(stream));                  // the uploads are temporary
     }
     void drop_assignment(int count) {
         num_adapters = count;
@@ -1142,12 +1159,14 @@ public:
         if (!ids) throw ArgError("smx_assign_adapters: null pointer");
         route_plan_bytes(num_nodes, slots, num_adapters);         // refuses bad sizes
         const size_t pairs = static_cast<size_t>(num_nodes) * slots;
+        adapter_nodes = 0; adapter_planned = -1;                  // a call that fails below leaves no assignment
         adapter_ids.upload(std::vector<int>(ids, ids + pairs), stream);
         if (weights) adapter_weights.upload(cast_vec<T>(std::vector<double>(weights, weights + pairs)), stream);
         SMX_CUDA(cudaStreamSynchronize(stream));
         adapter_weighted = weights != nullptr;
         adapter_nodes = num_nodes; adapter_slots = slots; adapter_planned = -1;
         for (auto& a : adapters) a.second.hidden_nodes = -1;
+        adapters_stale();
     }
     void adapter_gradients(const std::string& name, double* down, double* up, double* weights) override {
         require_edges();
@@ -1157,7 +1176,7 @@ public:
         smx_adapter_linear c = adapter_call(name.c_str());
         const DevBuf<T>& x = name == "H1" ? M0 : name == "Hm" ? Mm : name == "Am" ? Phim : Phi1;
         const DevBuf<T>& gy = name == "H1" ? H1_adj : name == "Hm" ? Hm_adj : name == "Am" ? Am_adj : A1_adj;
-        if (a.hidden_nodes != N || x.n != static_cast<size_t>(N) * c.x_stride || gy.n < static_cast<size_t>(N) * c.grad_y_stride)
+        if (!a.reversed || a.hidden_nodes != N || x.n != static_cast<size_t>(N) * c.x_stride || gy.n < static_cast<size_t>(N) * c.grad_y_stride)
             throw ArgError("smx_adapter_gradients: no evaluation of the current nodes with these adapters has been made");
         c.x = x.p; c.grad_y = gy.p; c.hidden = a.hidden.p;
         size_t downs = 0, ups = 0;
@@ -1746,6 +1765,7 @@ public:
         require_edges();
         SMX_CUDA(cudaSetDevice(device));
         NvtxRange range(s.c_str());
+        if (s.rfind("compute_", 0) == 0) adapters_stale();
         if (s == "compute_Y" || s == "compute_R0" || s == "compute_R1") return;  // fused into the edge kernels
         if (s == "compute_A0") compute_A0();
         else if (s == "compute_ZBL") compute_ZBL();

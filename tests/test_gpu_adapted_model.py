@@ -250,3 +250,30 @@ def test_refusals(model_file):
     ev.set_adapters("H1", down, up)
     with pytest.raises(SymmetrixError):
         ev.adapter_gradients("H1")                            # other adapters than the evaluation's
+
+
+def test_gradients_of_mixed_evaluations_are_refused(model_file):
+    """Gradients need the linear's input and the adjoint of its output from one evaluation: not after new edges, not between stages."""
+    path, model, spec = model_file("fcc128", num_channels=8, num_spline_points=32)
+    ev = MACE(path)
+    down, up = adapters_of(ev, "H1", 2, 3, 1)
+    inp, other = box(spec, model, 2, 1), box(spec, model, 2, 2)
+    n = int(inp["num_nodes"])
+    ev.set_adapters("H1", down, up)
+    ev.assign_adapters(np.arange(n, dtype=np.int32) % 2)
+    run(ev, inp)
+    first = ev.adapter_gradients("H1")
+    args = [other[k] for k in INPUT_KEYS]
+    ev.begin(int(other["num_nodes"]), *args[1:])
+    with pytest.raises(SymmetrixError, match="no evaluation"):
+        ev.adapter_gradients("H1")                            # the old arrays, the new edges
+    for stage in ("compute_A0", "compute_M0", "compute_H1"):
+        ev._stage(stage)
+    with pytest.raises(SymmetrixError, match="no evaluation"):
+        ev.adapter_gradients("H1")                            # the new input, the old adjoint
+    run(ev, other)
+    second = ev.adapter_gradients("H1")
+    assert not np.array_equal(first[0][0], second[0][0])
+    run(ev, inp)
+    for a, b in zip(first[0] + first[1], sum(ev.adapter_gradients("H1")[:2], [])):
+        np.testing.assert_array_equal(a, b)
