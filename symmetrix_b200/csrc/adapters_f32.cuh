@@ -290,9 +290,9 @@ __device__ __forceinline__ void ts_bulk(uint32_t to, const float* from, uint32_t
 //   warp 0      weight images: bulk copies of a chunk's [W | first_g] tiles, or of a round's second_g tiles, into a ring of stages; a stage
 //               is these tiles in shared memory and 32 values of the rows in tensor memory, with one barrier for both
 //   warp 1      the products (one thread)
-//   warp 2      finds the tiles and looks up their atoms and weights (a ring of four, ahead of all others)
-//   warps 4-7   rows: a warp copies 32 values of each of its 32 rows asynchronously, 16 bytes a lane (4 where rows start on no 16-byte boundary), three or four
-//               chunks ahead; a thread splits those of its row and stores them to the tensor memory's row operand. (Loads and stores by
+//   warp 2      finds the tiles and looks up their atoms and weights (a ring, ahead of all others)
+//   warps 4-7   rows: a warp copies 32 values of each of its 32 rows asynchronously, 16 bytes a lane (4 where rows start on no 16-byte boundary),
+//               row_stages - 1 chunks ahead; a thread splits those of its row and stores them to the tensor memory's row operand. (Loads and stores by
 //               the thread that owns a row touch 32 rows an instruction; a bulk copy takes 70 cycles to issue; one warp that copied for all
 //               four took longer than the products: 184 us instead of 160 at 98,304 atoms.)
 //   warps 8-15  a thread adds half of its row's partial sums of every 64 inner values in registers (the tensor core cuts its sums instead of
@@ -302,7 +302,7 @@ __device__ __forceinline__ void ts_bulk(uint32_t to, const float* from, uint32_t
 // stored into the hidden columns of its last two sums (head in the last one's, remainder in the other's); the products with second_g go on
 // top of the last sum, which is read after them.
 // Every wait is bounded; if one runs out, the CTA gives up and fills its remaining tiles with NaN.
-constexpr int kTsPassThreads = 512, kTsWorkRing = 4;
+constexpr int kTsPassThreads = 512;
 constexpr int kTsRowPitch = kTsChunk + 4;                                     // floats: threads that read their rows 16 bytes at a time hit all banks
 constexpr int kTsOutPitch = 17;                                               // floats of a row in the way out of rows that are not aligned
 constexpr int kTsRegsControl = 72, kTsRegsRows = 120, kTsRegsSums = 160, kTsRegsLaunch = 128;
@@ -312,26 +312,32 @@ static_assert(kTsRegsControl + kTsRegsRows + 2 * kTsRegsSums <= 4 * kTsRegsLaunc
 template <int HP, bool kWide>
 struct TsPassLayout {
     static constexpr int row_stages = kWide ? 5 : 4;
+    // Tiles in the ring. Where tiles have one chunk each (up to 32 inner values), the row warps ask for tile i + row_stages - 1 before they are
+    // done with tile i, so the ring holds all of i .. i + row_stages - 1: a shorter one would put the former into the place of the latter, and both
+    // sides would wait for each other.
+    static constexpr int work_ring = row_stages;
+    static_assert(work_ring >= row_stages, "the rows' copies run row_stages - 1 tiles ahead of the tile that is given back last");
     static constexpr int Rp = 16 * HP, sum_cols = 128 + Rp, stages = HP > 2 ? 2 : 3;
     static constexpr int slot0 = 2 * sum_cols;
     static constexpr uint32_t stage_bytes = sum_cols * 256u;
     static constexpr int row_floats = kTsRows * kTsRowPitch;
     static constexpr int smem = stages * static_cast<int>(stage_bytes) + (row_stages * row_floats + (kWide ? 0 : 8 * 32 * kTsOutPitch)) * 4 + 1024;
     static_assert(slot0 + 64 * stages <= 512, "tensor memory has 512 columns");
-    static_assert(smem + 14 * 1024 <= 227 * 1024, "shared memory of one CTA per SM");
+    static constexpr int fixed_smem = work_ring * (kTsRows * 22 + 64) + 256;  // the ring (work_* below) and the barriers
+    static_assert(smem + fixed_smem <= 227 * 1024, "shared memory of one CTA per SM");
 };
 
 template <int HP, bool kWide>
 __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(const __grid_constant__ TsPass pass) {
     using L = TsPassLayout<HP, kWide>;
-    constexpr int NS = L::stages, RS = L::row_stages;
+    constexpr int NS = L::stages, RS = L::row_stages, kRing = L::work_ring;
     extern __shared__ unsigned char ts_smem_raw[];
-    __shared__ __align__(8) unsigned long long work_full[kTsWorkRing], work_free[kTsWorkRing], full[NS], free[NS], d_full[2], d_free[2], t_full, t_done;
-    __shared__ TsWork work[kTsWorkRing];
-    __shared__ long long work_in[kTsWorkRing][kTsRows], work_out[kTsWorkRing][kTsRows];    // where its rows start, in `in`, in `out` without the tile's
-    __shared__ int work_place[kTsWorkRing][kTsRows];                                       // first column; sorted position and component
-    __shared__ short work_comp[kTsWorkRing][kTsRows];
-    __shared__ float work_weight[kTsWorkRing][kTsRows];
+    __shared__ __align__(8) unsigned long long work_full[kRing], work_free[kRing], full[NS], free[NS], d_full[2], d_free[2], t_full, t_done;
+    __shared__ TsWork work[kRing];
+    __shared__ long long work_in[kRing][kTsRows];                                          // where its rows start in `in`;
+    __shared__ int work_atom[kRing][kTsRows], work_place[kRing][kTsRows];                  // their atoms, sorted positions
+    __shared__ short work_comp[kRing][kTsRows];                                            // and components
+    __shared__ float work_weight[kRing][kTsRows];
     __shared__ uint32_t tmem_slot;
     __shared__ int failed;
     const int warp = ts_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -339,7 +345,7 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
     float* row_stages = reinterpret_cast<float*>(stages + NS * L::stage_bytes);
     if (threadIdx.x == 0) {
         failed = 0;
-        for (int q = 0; q < kTsWorkRing; ++q) { mbar_init(&work_full[q], 1); mbar_init(&work_free[q], 14); }
+        for (int q = 0; q < kRing; ++q) { mbar_init(&work_full[q], 1); mbar_init(&work_free[q], 14); }
         for (int q = 0; q < NS; ++q) { mbar_init(&full[q], 5); mbar_init(&free[q], 1); }
         for (int q = 0; q < 2; ++q) { mbar_init(&d_full[q], 1); mbar_init(&d_free[q], 8); }
         mbar_init(&t_full, 8);
@@ -361,8 +367,8 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
             TsCursor cursor;
             int t = blockIdx.x;
             for (int i = 0;; ++i) {
-                const int slot = i % kTsWorkRing;
-                if (i >= kTsWorkRing && !ts_wait_warp(&work_free[slot], (i / kTsWorkRing - 1) & 1, &failed)) break;
+                const int slot = i % kRing;
+                if (i >= kRing && !ts_wait_warp(&work_free[slot], (i / kRing - 1) & 1, &failed)) break;
                 TsWork w{};
                 while (cursor.find(pass, t, w)) {
                     t += gridDim.x;
@@ -380,7 +386,7 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
                         const int ahead = (m0 + at) / comps, comp = live ? m0 + at - ahead * comps : 0, listed = live ? p0 + ahead : p0;
                         const int place = pass.places ? pass.places[listed] : listed, pair = pass.order[place], atom = pass.slots > 1 ? pair / pass.slots : pair;
                         work_in[slot][at] = atom * pass.in_stride + d.in_off + comp * d.Kd;
-                        work_out[slot][at] = atom * pass.out_stride + d.out_off + static_cast<long long>(comp) * d.Nc;
+                        work_atom[slot][at] = atom;
                         work_place[slot][at] = place;
                         work_comp[slot][at] = static_cast<short>(comp);
                         work_weight[slot][at] = weighted ? pass.weights[pair] : 1.f;
@@ -413,8 +419,8 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
                 if (++st == NS) { st = 0; round ^= 1u; }
             };
             for (int i = 0; ok; ++i) {
-                const int slot = i % kTsWorkRing;
-                ok = ts_wait(&work_full[slot], (i / kTsWorkRing) & 1, &failed);
+                const int slot = i % kRing;
+                ok = ts_wait(&work_full[slot], (i / kRing) & 1, &failed);
                 if (!ok) break;
                 const TsWork w = work[slot];
                 mbar_arrive(&work_free[slot]);
@@ -445,8 +451,8 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
             const bool leader = ts_elect();
             const uint32_t base = smem_u32(stages), t0 = ts_uniform(tmem);
             for (int i = 0; ok; ++i) {
-                const int slot = i % kTsWorkRing;
-                ok = ts_wait_warp(&work_full[slot], (i / kTsWorkRing) & 1, &failed);
+                const int slot = i % kRing;
+                ok = ts_wait_warp(&work_full[slot], (i / kRing) & 1, &failed);
                 if (!ok) break;
                 const TsWork w = work[slot];
                 __syncwarp();
@@ -515,8 +521,8 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
         const float* from = nullptr;
         auto copy_next = [&](int stage) {
             if (more && ahead == ahead_nx) {
-                ahead_slot = ahead_tile % kTsWorkRing;
-                if (!ts_wait_warp(&work_full[ahead_slot], (ahead_tile / kTsWorkRing) & 1, &failed)) {
+                ahead_slot = ahead_tile % kRing;
+                if (!ts_wait_warp(&work_full[ahead_slot], (ahead_tile / kRing) & 1, &failed)) {
                     ok = more = false;
                 } else {
                     const TsWork& w = work[ahead_slot];
@@ -552,8 +558,8 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
         };
         for (int q = 0; q < RS - 1; ++q) copy_next(q);
         for (int i = 0; ok; ++i) {
-            const int slot = i % kTsWorkRing;
-            if (!ts_wait_warp(&work_full[slot], (i / kTsWorkRing) & 1, &failed)) break;
+            const int slot = i % kRing;
+            if (!ts_wait_warp(&work_full[slot], (i / kRing) & 1, &failed)) break;
             const TsWork w = work[slot];
             if (!w.found) {
                 __syncwarp();
@@ -624,15 +630,17 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
         int place = 0, comp = 0;
         float weight = 1.f;
         auto next_work = [&]() {
-            const int slot = i % kTsWorkRing;
-            if (!ts_wait_warp(&work_full[slot], (i / kTsWorkRing) & 1, &failed)) { ok = false; return; }
+            const int slot = i % kRing;
+            if (!ts_wait_warp(&work_full[slot], (i / kRing) & 1, &failed)) { ok = false; return; }
             w = work[slot];
-            out_at = work_out[slot][tid];
+            const int atom = work_atom[slot][tid];
             place = work_place[slot][tid];
             comp = work_comp[slot][tid];
             weight = work_weight[slot][tid];
             __syncwarp();
             if (lane == 0) mbar_arrive(&work_free[slot]);
+            const TsDegree& d = pass.degree[w.degree];
+            out_at = atom * pass.out_stride + d.out_off + static_cast<long long>(comp) * d.Nc;
             ++i;
         };
         next_work();
