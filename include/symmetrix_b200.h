@@ -271,8 +271,8 @@ int smx_active_counts(smx_handle h, int* num_nodes, long* num_edges, int* built_
 /* Test switch for the bounded device-side waits (no counterpart in the reference, which has no such waits). With
  * `polls` > 0 the first weight-tile wait of every CTA of the float32 tensor-core GEMM expects 16 bytes more than
  * its copy delivers and gives up after `polls` polls: the kernel records the failure, releases its tensor memory and
- * returns, and the next synchronising call reports SMX_ERR_CUDA. Nothing faults and the handle stays usable; 0 switches
- * it off. */
+ * returns, and the next synchronising call reports SMX_ERR_CUDA. Likewise every CTA of the float32 linears with adapters loses its
+ * weights behind the first 32 inner values. Nothing faults and the handle stays usable; 0 switches it off. */
 int smx_debug_expire_waits(smx_handle h, int polls);
 
 /* Input check. The reference trusts its callers (unchecked spline bin and gather indices, cubic_spline_set.cpp:31-32,
@@ -357,7 +357,8 @@ int smx_route_combine_backward(int precision, const void* grad_y, long grad_y_st
  * length follows from the sizes alone, and added in order: the same call gives the same bits. Outputs must not overlap inputs or one another.
  * The rules of the smx_route_* calls hold: device pointers on the current GPU, `stream`, no allocation, no wait, a workspace of
  * smx_adapter_workspace_bytes bytes for each call that may overlap with another one, errors through `errbuf`. The size functions
- * return -1 for calls that are refused. `tiles`, `hidden` and `workspace` start on 16-byte boundaries. Limits: rank, degrees as below, those of the routing. */
+ * return -1 for calls that are refused. The float32 kernels wait for one another's parts inside a CTA, with a limit: should a wait run out, the rows
+ * and hidden rows that are lost hold NaN, and `status` (a device int, may be NULL) receives a non-zero code, to be read when the stream has come that far. `tiles`, `hidden` and `workspace` start on 16-byte boundaries. Limits: rank, degrees as below, those of the routing. */
 enum { SMX_ADAPTER_MAX_RANK = 64, SMX_ADAPTER_MAX_DEGREES = 8 };
 enum { SMX_ADAPTER_SHARED = 1, SMX_ADAPTER_MATRICES = 2 };
 typedef struct smx_adapter_degree {
@@ -380,6 +381,7 @@ typedef struct smx_adapter_linear {
     void* hidden;
     void* workspace;    long workspace_bytes;
     void* stream;
+    int* status;                             /* NULL, or an int that the caller has zeroed */
 } smx_adapter_linear;
 long smx_adapter_tiles_bytes(const smx_adapter_linear* call);
 int smx_adapter_prepare(const smx_adapter_linear* call, int parts, char* errbuf, int errbuf_len);

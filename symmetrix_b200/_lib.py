@@ -55,7 +55,7 @@ class AdapterCall(ctypes.Structure):
                 ("x", ctypes.c_void_p), ("x_stride", ctypes.c_long), ("y", ctypes.c_void_p), ("y_stride", ctypes.c_long),
                 ("grad_y", ctypes.c_void_p), ("grad_y_stride", ctypes.c_long), ("grad_x", ctypes.c_void_p), ("grad_x_stride", ctypes.c_long),
                 ("grad_weights", ctypes.c_void_p), ("hidden", ctypes.c_void_p), ("workspace", ctypes.c_void_p),
-                ("workspace_bytes", ctypes.c_long), ("stream", ctypes.c_void_p)]
+                ("workspace_bytes", ctypes.c_long), ("stream", ctypes.c_void_p), ("status", ctypes.c_void_p)]
 
 
 _lib = None

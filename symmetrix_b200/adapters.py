@@ -266,8 +266,10 @@ class AdapterLinear:
             raise ValueError("the sizes exceed what smx_adapter_forward supports")
         self._index = self.device.index
         self._home = _stream(self._index)
-        self._tiles = torch.empty(need, dtype=torch.uint8, device=self.device)
-        f.tiles = self._tiles.data_ptr()
+        self._tiles = torch.empty(need + 16, dtype=torch.uint8, device=self.device)
+        self._status = self._tiles[need:need + 4].view(torch.int32)
+        self._status.zero_()
+        f.tiles, f.status = self._tiles.data_ptr(), self._status.data_ptr()
         self.set_adapters(down, up)
         if self._has_shared:
             self.set_shared(shared)
@@ -300,6 +302,14 @@ class AdapterLinear:
         self._prepare(_lib.ADAPTER_SHARED, shared, None, None)
 
     # ------------------------------------------------------------------ calls
+    def check(self) -> None:
+        """Waits for the current stream and raises ``SymmetrixError`` if a bounded wait inside a kernel ran out in a call since the last check:
+        what such a call lost holds NaN. (Calls themselves never wait, so they cannot tell.)"""
+        code = int(self._status.item())
+        if code:
+            self._status.zero_()
+            raise SymmetrixError(_lib.SMX_ERR_CUDA, f"a bounded wait ran out in a device kernel (code {code}); results are invalid")
+
     def _copy(self):
         call = _lib.AdapterCall()
         ctypes.memmove(ctypes.byref(call), ctypes.byref(self._fixed), ctypes.sizeof(call))

@@ -47,6 +47,8 @@ struct Pass {
     T* out; long long out_stride;                    // null: only the hidden rows
     int add;           // to `out`, instead of writing it
     int tail;          // the rows without a group are a last group of their own
+    int* status;       // null, or where a wait that ran out is reported (float32; the float64 kernels have no waits of the kind)
+    int expire_polls;  // test switch of those waits
 };
 
 // Rows of a tile: pairs [pair0, pair0 + ...) of one group, rows counted in components from row0 of the group.
@@ -221,7 +223,7 @@ void check_plan(const smx_adapter_linear& c) {
     if (!c.tiles) throw ArgError("smx_adapter: null tiles");
     check_aligned(c);
     if (!c.offsets || (c.num_rows > 0 && (!c.order || !c.position))) throw ArgError("smx_adapter: null plan");
-    check_pointers("smx_adapter", sizeof(int), {c.order, c.position, c.offsets});
+    check_pointers("smx_adapter", sizeof(int), {c.order, c.position, c.offsets, c.status});
     const size_t value = c.precision == SMX_FP32 ? sizeof(float) : sizeof(double);
     check_pointers("smx_adapter", value, {c.x, c.y, c.grad_y, c.grad_x, c.weights, c.grad_weights});
     for (int d = 0; d < c.num_degrees; ++d) check_pointers("smx_adapter", value, {c.degrees[d].grad_down, c.degrees[d].grad_up});
@@ -455,7 +457,7 @@ void launch_pass(const smx_adapter_linear& c, bool transposed, const Pass<float>
     }
     t.degrees = degrees; t.rank = p.rank; t.groups = p.groups; t.slots = p.slots; t.pairs = p.pairs;
     t.order = p.order; t.offsets = p.offsets; t.places = p.places; t.weights = p.weights; t.in = p.in; t.in_stride = p.in_stride; t.out = p.out; t.out_stride = p.out_stride;
-    t.add = p.add; t.tail = p.tail;
+    t.add = p.add; t.tail = p.tail; t.status = p.status; t.expire_polls = p.expire_polls;
     if (tiles > INT_MAX - 4096) throw ArgError("smx_adapter: too many rows");
     bool bare = false;
     for (int q = 0; q < degrees; ++q) bare = bare || !p.degree[q].W;
@@ -563,11 +565,13 @@ void launch_grads(const GradPass<float>& gp, int problems, cudaStream_t stream) 
 
 // out = in W + adapters, in either direction; `hidden` (may be null) receives in . first of every pair. Without `out` that is all.
 template <typename T>
-void run_pass(const smx_adapter_linear& c, bool transposed, const T* in, long in_stride, T* out, long out_stride, T* hidden, const Buffers<T>& b) {
+void run_pass(const smx_adapter_linear& c, bool transposed, const T* in, long in_stride, T* out, long out_stride, T* hidden, const Buffers<T>& b,
+              int expire_polls) {
     if (c.num_rows == 0) return;
     const cudaStream_t stream = static_cast<cudaStream_t>(c.stream);
     Pass<T> p = make_pass<T>(c, transposed, hidden);
     p.in = in; p.in_stride = in_stride;
+    p.status = c.status; p.expire_polls = expire_polls;
     if (!out) {
         for (int d = 0; d < c.num_degrees; ++d) { p.degree[d].W = nullptr; p.degree[d].Nc = 1; }      // one (unused) block of columns
         launch_pass(c, transposed, p, c.num_degrees, stream);
@@ -588,18 +592,18 @@ void run_pass(const smx_adapter_linear& c, bool transposed, const T* in, long in
 }
 
 template <typename T>
-void forward(const smx_adapter_linear& c) {
+void forward(const smx_adapter_linear& c, int expire_polls) {
     const Buffers<T> b = lay_out<T>(c, false);
     if (c.workspace_bytes < 0 || static_cast<size_t>(c.workspace_bytes) < b.bytes || (b.bytes && !c.workspace))
         throw ArgError("smx_adapter_forward: the workspace is smaller than smx_adapter_workspace_bytes says");
     const Widths w = widths(c);
     check_rows("x", c.x, c.x_stride, w.in, c.num_rows, false);
     check_rows("y", c.y, c.y_stride, w.out, c.num_rows, true);
-    run_pass<T>(c, false, static_cast<const T*>(c.x), c.x_stride, static_cast<T*>(c.y), c.y_stride, static_cast<T*>(c.hidden), b);
+    run_pass<T>(c, false, static_cast<const T*>(c.x), c.x_stride, static_cast<T*>(c.y), c.y_stride, static_cast<T*>(c.hidden), b, expire_polls);
 }
 
 template <typename T>
-void backward(const smx_adapter_linear& c) {
+void backward(const smx_adapter_linear& c, int expire_polls) {
     const Buffers<T> b = lay_out<T>(c, true);
     if (c.workspace_bytes < 0 || static_cast<size_t>(c.workspace_bytes) < b.bytes || (b.bytes && !c.workspace))
         throw ArgError("smx_adapter_backward: the workspace is smaller than smx_adapter_workspace_bytes says");
@@ -620,11 +624,11 @@ void backward(const smx_adapter_linear& c) {
     const size_t pairs = static_cast<size_t>(c.num_rows) * c.slots;
     const T* x = static_cast<const T*>(c.x);
     const T* gy = static_cast<const T*>(c.grad_y);
-    run_pass<T>(c, true, gy, c.grad_y_stride, static_cast<T*>(c.grad_x), c.grad_x_stride, b.back_hidden, b);
+    run_pass<T>(c, true, gy, c.grad_y_stride, static_cast<T*>(c.grad_x), c.grad_x_stride, b.back_hidden, b, expire_polls);
     if (!hidden_needed) return;
     const T* hidden = static_cast<const T*>(c.hidden);
     if (!hidden) {
-        run_pass<T>(c, false, x, c.x_stride, nullptr, 0, b.hidden, b);
+        run_pass<T>(c, false, x, c.x_stride, nullptr, 0, b.hidden, b, expire_polls);
         hidden = b.hidden;
     }
     GradPass<T> gp{};
@@ -690,15 +694,15 @@ void adapter_prepare(const smx_adapter_linear& c, int parts) {
     if (parts & ~(SMX_ADAPTER_SHARED | SMX_ADAPTER_MATRICES)) throw ArgError("smx_adapter_prepare: unknown part");
     prepare(c, parts);
 }
-void adapter_forward(const smx_adapter_linear& c) {
+void adapter_forward(const smx_adapter_linear& c, int expire_polls) {
     check_plan(c);
-    if (c.precision == SMX_FP32) forward<float>(c);
-    else forward<double>(c);
+    if (c.precision == SMX_FP32) forward<float>(c, expire_polls);
+    else forward<double>(c, expire_polls);
 }
-void adapter_backward(const smx_adapter_linear& c) {
+void adapter_backward(const smx_adapter_linear& c, int expire_polls) {
     check_plan(c);
-    if (c.precision == SMX_FP32) backward<float>(c);
-    else backward<double>(c);
+    if (c.precision == SMX_FP32) backward<float>(c, expire_polls);
+    else backward<double>(c, expire_polls);
 }
 
 }  // namespace smx

@@ -12,7 +12,8 @@ size_t adapter_tiles_bytes(const smx_adapter_linear& c);
 void adapter_prepare(const smx_adapter_linear& c, int parts);
 size_t adapter_hidden_elements(const smx_adapter_linear& c);
 size_t adapter_workspace_bytes(const smx_adapter_linear& c, bool backward);
-void adapter_forward(const smx_adapter_linear& c);
-void adapter_backward(const smx_adapter_linear& c);
+// `expire_polls`: test switch, see smx_debug_expire_waits.
+void adapter_forward(const smx_adapter_linear& c, int expire_polls = 0);
+void adapter_backward(const smx_adapter_linear& c, int expire_polls = 0);
 
 }  // namespace smx

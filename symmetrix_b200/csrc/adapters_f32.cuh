@@ -162,7 +162,11 @@ struct TsPass {
     const float* in; long long in_stride;
     float* out; long long out_stride;
     int add, tail;                               // as in Pass
+    int* status;                                 // null, or receives kTsStatusWait if a wait runs out
+    int expire_polls;                            // test switch, zero in normal operation: every CTA loses its weights behind the first chunk and gives up
+                                                 // after this many polls
 };
+constexpr int kTsStatusWait = 7;
 struct TsWork { int index, degree, block, found; TileRows rows; };
 
 // The tiles of a pass one after the other: degrees, then groups, then row tiles, then column blocks (so that a row tile's blocks run side by
@@ -245,7 +249,7 @@ __device__ __forceinline__ void ts_fill(const TsPass& p, const TsWork& w, int th
     }
 }
 
-// Waits of the pass kernel: bounded, and given up at once when another one ran out.
+// Waits of the pass kernel: bounded by guard[1] polls, and given up at once when another one ran out (guard[0]).
 __device__ __forceinline__ bool ts_try(uint32_t addr, unsigned parity) {
     uint32_t done;
     asm volatile(
@@ -255,18 +259,24 @@ __device__ __forceinline__ bool ts_try(uint32_t addr, unsigned parity) {
         : "=r"(done) : "r"(addr), "r"(parity) : "memory");
     return done != 0;
 }
-__device__ __forceinline__ bool ts_wait(unsigned long long* bar, unsigned parity, int* failed) {
+__device__ __forceinline__ bool ts_wait(unsigned long long* bar, unsigned parity, int* guard) {
     const uint32_t addr = smem_u32(bar);
 #pragma unroll 1
     for (unsigned spin = 0; !ts_try(addr, parity); ++spin) {
         if ((spin & 63u) != 63u) continue;
-        if (*reinterpret_cast<volatile int*>(failed)) return false;
-        if (spin >= kMbarSpinLimit) { atomicExch(failed, 1); return false; }
+        if (*reinterpret_cast<volatile int*>(guard)) return false;
+        if (spin >= static_cast<unsigned>(guard[1])) { atomicExch(guard, 1); return false; }
     }
     return true;
 }
-__device__ __forceinline__ bool ts_wait_warp(unsigned long long* bar, unsigned parity, int* failed) {
-    return __all_sync(0xffffffffu, ts_wait(bar, parity, failed));
+__device__ __forceinline__ bool ts_wait_warp(unsigned long long* bar, unsigned parity, int* guard) {
+    return __all_sync(0xffffffffu, ts_wait(bar, parity, guard));
+}
+// All warps of the pass kernel, each from the end of its own part.
+__device__ __forceinline__ void ts_meet() {
+    __syncwarp();
+    ts_fence_before();
+    asm volatile("bar.sync 1, 512;" ::: "memory");
 }
 template <int N> __device__ __forceinline__ void ts_registers_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void ts_registers_less() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -303,8 +313,9 @@ __device__ __forceinline__ void ts_bulk(uint32_t to, const float* from, uint32_t
 // TMEM: two partial sums of 128 + Rp columns, taken in turn, and the stages' row operands of 64. The hidden row of a tile is weighted, split and
 // stored into the hidden columns of its last two sums (head in the last one's, remainder in the other's); the products with second_g go on
 // top of the last sum, which is read after them.
-// Every wait is bounded; if one runs out, the CTA gives up and fills its remaining tiles with NaN.
-constexpr int kTsPassThreads = 512;
+// Every wait is bounded; if one runs out, the CTA gives up, fills its remaining tiles with NaN, reports it to `status` and ends when its copies and
+// products in flight have.
+constexpr int kTsPassThreads = 512;                                          // as in ts_meet
 constexpr int kTsRowPitch = kTsChunk + 4;                                     // floats: threads that read their rows 16 bytes at a time hit all banks
 constexpr int kTsOutPitch = 17;                                               // floats of a row in the way out of rows that are not aligned
 constexpr int kTsRegsControl = 72, kTsRegsRows = 120, kTsRegsSums = 160, kTsRegsLaunch = 128;
@@ -334,24 +345,28 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
     using L = TsPassLayout<HP, kWide>;
     constexpr int NS = L::stages, RS = L::row_stages, kRing = L::work_ring;
     extern __shared__ unsigned char ts_smem_raw[];
-    __shared__ __align__(8) unsigned long long work_full[kRing], work_free[kRing], full[NS], free[NS], d_full[2], d_free[2], t_full, t_done;
+    __shared__ __align__(8) unsigned long long work_full[kRing], work_free[kRing], full[NS], free[NS], d_full[2], d_free[2], t_full, t_done, drained;
     __shared__ TsWork work[kRing];
     __shared__ long long work_in[kRing][kTsRows];                                          // where its rows start in `in`;
     __shared__ int work_atom[kRing][kTsRows], work_place[kRing][kTsRows];                  // their atoms, sorted positions
     __shared__ short work_comp[kRing][kTsRows];                                            // and components
     __shared__ float work_weight[kRing][kTsRows];
     __shared__ uint32_t tmem_slot;
-    __shared__ int failed;
+    __shared__ int guard[2];                                                               // a wait ran out; polls of a wait
+    __shared__ int copies, row_uses[4];                                                    // chunks copied, operands of every row warp
     const int warp = ts_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     unsigned char* stages = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(ts_smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     float* row_stages = reinterpret_cast<float*>(stages + NS * L::stage_bytes);
     if (threadIdx.x == 0) {
-        failed = 0;
+        guard[0] = 0;
+        guard[1] = pass.expire_polls > 0 ? pass.expire_polls : static_cast<int>(kMbarSpinLimit);
+        copies = 0;
         for (int q = 0; q < kRing; ++q) { mbar_init(&work_full[q], 1); mbar_init(&work_free[q], 14); }
         for (int q = 0; q < NS; ++q) { mbar_init(&full[q], 5); mbar_init(&free[q], 1); }
         for (int q = 0; q < 2; ++q) { mbar_init(&d_full[q], 1); mbar_init(&d_free[q], 8); }
         mbar_init(&t_full, 8);
         mbar_init(&t_done, 1);
+        mbar_init(&drained, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) {
@@ -370,7 +385,7 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
             int t = blockIdx.x;
             for (int i = 0;; ++i) {
                 const int slot = i % kRing;
-                if (i >= kRing && !ts_wait_warp(&work_free[slot], (i / kRing - 1) & 1, &failed)) break;
+                if (i >= kRing && !ts_wait_warp(&work_free[slot], (i / kRing - 1) & 1, guard)) break;
                 TsWork w{};
                 while (cursor.find(pass, t, w)) {
                     t += gridDim.x;
@@ -406,7 +421,8 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
             const uint32_t base = smem_u32(stages);
             // one chunk: `rows_a` rows of a 128-column tile and then `rows_b` of a hidden tile, heads and remainders
             auto copy = [&](const float* a, uint32_t rows_a, const float* b, uint32_t rows_b) {
-                if (n >= NS && !ts_wait(&free[st], round, &failed)) { ok = false; return; }
+                if (pass.expire_polls > 0 && n > 0) { ok = false; return; }
+                if (n >= NS && !ts_wait(&free[st], round, guard)) { ok = false; return; }
                 const uint32_t bar = smem_u32(&full[st]), to = base + st * L::stage_bytes, half = (rows_a + rows_b) * 128u;
                 asm volatile("{\n\t.reg .b64 t;\n\tmbarrier.arrive.expect_tx.shared::cta.b64 t, [%0], %1;\n\t}" ::"r"(bar), "r"(2 * half) : "memory");
                 if (rows_a) {
@@ -422,7 +438,7 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
             };
             for (int i = 0; ok; ++i) {
                 const int slot = i % kRing;
-                ok = ts_wait(&work_full[slot], (i / kRing) & 1, &failed);
+                ok = ts_wait(&work_full[slot], (i / kRing) & 1, guard);
                 if (!ok) break;
                 const TsWork w = work[slot];
                 mbar_arrive(&work_free[slot]);
@@ -444,8 +460,7 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
                     }
                 }
             }
-            if (!ok)                                                     // copies in flight write into this CTA's memory: wait for them (bounded)
-                for (int q = max(0, n - NS); q < n; ++q) mbar_wait(&full[q % NS], (q / NS) & 1);
+            copies = n;
         } else if (warp == 1) {
             int st = 0, sum = 0, nd = 0;                                 // stage and partial sum in turn, with the parity of their next and last use
             unsigned st_par = 0, sum_par = 1, hid_par = 0;
@@ -454,7 +469,7 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
             const uint32_t base = smem_u32(stages), t0 = ts_uniform(tmem);
             for (int i = 0; ok; ++i) {
                 const int slot = i % kRing;
-                ok = ts_wait_warp(&work_full[slot], (i / kRing) & 1, &failed);
+                ok = ts_wait_warp(&work_full[slot], (i / kRing) & 1, guard);
                 if (!ok) break;
                 const TsWork w = work[slot];
                 __syncwarp();
@@ -472,14 +487,14 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
                     uint32_t d, hi, lo;
                     bool add;
                     if (inner) {
-                        if ((j & 1) == 0 && nd >= 2) ok = ts_wait_warp(&d_free[sum], sum_par, &failed);
+                        if ((j & 1) == 0 && nd >= 2) ok = ts_wait_warp(&d_free[sum], sum_par, guard);
                         cols = in_cols;
                         d = t0 + sum * L::sum_cols + (main_cols ? 0 : 128);
                         hi = t0 + L::slot0 + 64 * st;
                         lo = hi + 32;
                         add = (j & 1) != 0;
                     } else {
-                        if (e == 0) ok = ts_wait_warp(&t_full, hid_par, &failed);
+                        if (e == 0) ok = ts_wait_warp(&t_full, hid_par, guard);
                         cols = out_cols;
                         steps = min(4, L::Rp / 8 - 4 * e);
                         d = t0 + (sum ^ 1) * L::sum_cols;
@@ -487,7 +502,7 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
                         lo = t0 + sum * L::sum_cols + hid_col + 32 * e;
                         add = main_cols > 0 || e > 0;
                     }
-                    ok = ok && ts_wait_warp(&full[st], st_par, &failed);
+                    ok = ok && ts_wait_warp(&full[st], st_par, guard);
                     if (!ok) break;
                     ts_fence_after();
                     const uint32_t b = base + st * L::stage_bytes;
@@ -509,6 +524,23 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
                 }
             }
         }
+        ts_meet();
+        if (guard[0]) {
+            // what was started ends before the CTA does: products read its shared and tensor memory, copies write into the former
+            if (warp == 1) {
+                if (ts_elect()) ts_commit(&drained);
+                __syncwarp();
+                mbar_wait(&drained, 0);
+            } else if (warp == 0 && lane == 0) {
+                // the last chunks' barriers, with the arrivals that row warps still owed them
+                for (int q = max(0, copies - NS); q < copies; ++q) {
+                    for (int w = 0; w < 4; ++w)
+                        if (row_uses[w] <= q) mbar_arrive(&full[q % NS]);
+                    mbar_wait(&full[q % NS], (q / NS) & 1);
+                }
+                if (pass.status) atomicMax(pass.status, kTsStatusWait);
+            }
+        }
     } else if (warp < 8) {
         ts_registers_less<kTsRegsRows>();
         const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
@@ -524,7 +556,7 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
         auto copy_next = [&](int stage) {
             if (more && ahead == ahead_nx) {
                 ahead_slot = ahead_tile % kRing;
-                if (!ts_wait_warp(&work_full[ahead_slot], (ahead_tile / kRing) & 1, &failed)) {
+                if (!ts_wait_warp(&work_full[ahead_slot], (ahead_tile / kRing) & 1, guard)) {
                     ok = more = false;
                 } else {
                     const TsWork& w = work[ahead_slot];
@@ -561,7 +593,7 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
         for (int q = 0; q < RS - 1; ++q) copy_next(q);
         for (int i = 0; ok; ++i) {
             const int slot = i % kRing;
-            if (!ts_wait_warp(&work_full[slot], (i / kRing) & 1, &failed)) break;
+            if (!ts_wait_warp(&work_full[slot], (i / kRing) & 1, guard)) break;
             const TsWork w = work[slot];
             if (!w.found) {
                 __syncwarp();
@@ -579,7 +611,7 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
                     copy_next(xs == 0 ? RS - 1 : xs - 1);
                     if (!ok) break;
                 }
-                if (na >= NS && !ts_wait_warp(&free[op], op_par, &failed)) { ok = false; break; }
+                if (na >= NS && !ts_wait_warp(&free[op], op_par, guard)) { ok = false; break; }
                 ++na;
                 unsigned long long* const bar = &full[op];
                 const uint32_t to = lanes + L::slot0 + 64 * op;
@@ -617,6 +649,8 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
             if (lane == 0) mbar_arrive(&work_free[slot]);
         }
         asm volatile("cp.async.wait_all;" ::: "memory");                 // none may be in flight when the CTA ends
+        if (lane == 0) row_uses[warp & 3] = na;
+        ts_meet();
     } else {
         ts_registers_more<kTsRegsSums>();
         const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
@@ -633,7 +667,7 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
         float weight = 1.f;
         auto next_work = [&]() {
             const int slot = i % kRing;
-            if (!ts_wait_warp(&work_full[slot], (i / kRing) & 1, &failed)) { ok = false; return; }
+            if (!ts_wait_warp(&work_full[slot], (i / kRing) & 1, guard)) { ok = false; return; }
             w = work[slot];
             const int atom = work_atom[slot][tid];
             place = work_place[slot][tid];
@@ -711,7 +745,7 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
             // with rounds, the last sum's shared columns are read at the end, and the last two are given back there
             const int stay = s.rounds > 0 ? s.sums - 1 : s.sums, kept = s.rounds > 0 ? min(2, s.sums) : 0;
             for (int j = 0; j < s.sums; ++j, ++nd) {
-                if (!ts_wait_warp(&d_full[nd & 1], (nd >> 1) & 1, &failed)) { ok = false; break; }
+                if (!ts_wait_warp(&d_full[nd & 1], (nd >> 1) & 1, guard)) { ok = false; break; }
                 ts_fence_after();
                 const uint32_t from = lanes + (nd & 1) * L::sum_cols;
                 if (s.adapter)
@@ -730,7 +764,7 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
             if (s.rounds > 0) {
                 // the halves read and store hidden blocks of their own; where the tile has one sum, the other partial sum is the previous tile's, which
                 // the other half's warp may still be reading
-                if (s.sums == 1 && nd > 1 && !ts_wait_warp(&d_free[nd & 1], ((nd - 2) >> 1) & 1, &failed)) { ok = false; break; }
+                if (s.sums == 1 && nd > 1 && !ts_wait_warp(&d_free[nd & 1], ((nd - 2) >> 1) & 1, guard)) { ok = false; break; }
                 const uint32_t hi_at = lanes + ((nd - 1) & 1) * L::sum_cols + s.hid_col, lo_at = lanes + (nd & 1) * L::sum_cols + s.hid_col;
 #pragma unroll
                 for (int cc = 0; cc < kLower; ++cc)
@@ -760,7 +794,7 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
                 }
             }
             if (s.rounds > 0) {
-                if (!ts_wait_warp(&t_done, nt & 1, &failed)) { ok = false; break; }
+                if (!ts_wait_warp(&t_done, nt & 1, guard)) { ok = false; break; }
                 ++nt;
                 ts_fence_after();
                 if (kept == 2) release(nd - 2);
@@ -801,9 +835,8 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
             TsWork lost{};
             for (int t = at_hand; cursor.find(pass, t, lost); t += gridDim.x) ts_fill(pass, lost, tid, 128, NAN);
         }
+        ts_meet();
     }
-    __syncwarp();
-    ts_fence_before();
     __syncthreads();
     if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }

@@ -141,7 +141,7 @@ public:
     DevBuf<GemmProblem<T>> dev_ring;
     size_t ring_pos = 0;
     bool own_stream = true;
-    DevBuf<int> kernel_status;    // non-zero if a bounded mbarrier wait ran out (1, 2: tcgen05 GEMM; 3, 4: staged tensor-product reverse)
+    DevBuf<int> kernel_status;    // non-zero if a bounded mbarrier wait ran out (1, 2: tcgen05 GEMM; 3, 4: staged tensor-product reverse; 7: linears with adapters)
     bool staged_reverse = false;  // spline rows of the tensor-product reverse through bulk copies into shared memory
                                   // (SMX_TP_STAGED=1, float64; measured equal on B200)
     // Run-time radial mode (SMX_RADIAL=mlp, float32, two-block models whose file carries the x_radial_* keys): the radial
@@ -1078,8 +1078,12 @@ public:
         c.workspace = adapter_workspace.p;
         c.workspace_bytes = static_cast<long>(adapter_workspace.n);
         const long before = operator_launches;
-        if (back) adapter_backward(c);
-        else adapter_forward(c);
+        if (sizeof(T) == 4) {
+            c.status = kernel_status.p;
+            waits_in_flight = true;
+        }
+        if (back) adapter_backward(c, expire_polls);
+        else adapter_forward(c, expire_polls);
         launches += operator_launches - before;
     }
     void adapter_compute(const char* name, const T* x, T* y) {
@@ -1877,6 +1881,8 @@ public:
         SMX_CUDA(cudaStreamSynchronize(stream));
         waits_in_flight = false;
         if (code != 0) {
+            adapters_stale();                     // no gradients of arrays that are invalid
+            for (auto& a : adapters) a.second.hidden_nodes = -1;
             // re-arm the status word: later evaluations on this handle are judged on their own kernels
             SMX_CUDA(cudaMemsetAsync(kernel_status.p, 0, sizeof(int), stream));
             SMX_CUDA(cudaStreamSynchronize(stream));

@@ -433,7 +433,7 @@ class MACE:
         self._check(self._lib.smx_halo_cache_lists(self._h, 1 if enable else 0))
 
     def debug_expire_waits(self, polls: int) -> None:
-        """Test switch: make the first bounded wait of every float32 tensor-core GEMM CTA run out after `polls` polls."""
+        """Test switch: make a bounded wait of every CTA of the float32 tensor-core GEMM, and of the linears with adapters, run out after `polls` polls."""
         self._check(self._lib.smx_debug_expire_waits(self._h, int(polls)))
 
     # NCCL transport inside the library (smx_comm_init / smx_halo_exchange / smx_allreduce_sum)
