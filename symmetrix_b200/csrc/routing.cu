@@ -427,7 +427,8 @@ void counting_sort(const int* ids, long long pairs, int num_groups, int* order, 
         while (warps > 1 && (warps + 1) * bins > 32768) warps /= 2;
         const int smem = ((warps + 1) * bins + 1) * static_cast<int>(sizeof(int));
         static std::atomic<bool> done[64];
-        if (smem > 48 * 1024 && first_on_device(done)) {
+        // beyond 48 KB a launch has to be allowed, and the kernel's own arrays (the sums of its scan) count too
+        if (smem > 47 * 1024 && first_on_device(done)) {
             SMX_CUDA(cudaFuncSetAttribute(route_plan_small_kernel<kSlots>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
             mark_on_device(done);
         }
