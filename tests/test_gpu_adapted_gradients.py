@@ -7,8 +7,9 @@ import numpy as np
 import pytest
 import torch
 
-from symmetrix_b200 import MACE, structures as st
-from tests.test_gpu_adapted_model import adapters_of
+from symmetrix_b200 import MACE, SymmetrixError, structures as st
+from symmetrix_b200.domain import SlabRank, evaluate_decomposed, make_slab_plan
+from tests.test_gpu_adapted_model import adapters_of, run
 from tests.test_gpu_adapters import EPS
 
 pytestmark = pytest.mark.gpu
@@ -76,3 +77,112 @@ def test_gradients_of_many_atoms(model_file, dtype, channels):
         ev.evaluate(s.positions, types, s.cell, s.pbc)
         for name, (down, up) in sets.items():
             check_gradients(ev, name, down, up, ids, weights, dtype)
+
+
+def molecules(spec, model):
+    s = st.molecular_liquid(3, seed=3)
+    return st.evaluator_inputs(s, st.neighbor_list(s, spec.r_cut), model["atomic_numbers"])
+
+
+def three_blocks(model_file, dtype, channels=16):
+    path, model, spec = model_file("deep256", num_channels=channels, num_spline_points=32)
+    ev = MACE(path, dtype=dtype)
+    inp = molecules(spec, model)
+    sets = {name: adapters_of(ev, name, 2, 3, q) for q, name in enumerate(("H1", "Am", "Hm", "A1"))}
+    n = int(inp["num_nodes"])
+    ids = np.array([[0, 1], [1, -1], [0, 0], [-1, -1]])[np.arange(n) % 4]
+    return ev, inp, sets, ids, np.random.default_rng(3).uniform(0.5, 1.5, size=(n, 2))
+
+
+@pytest.mark.parametrize("dtype", ["float64", "float32"])
+@pytest.mark.parametrize("channels", [16, 33, 64])
+def test_gradients_of_three_blocks(model_file, dtype, channels):
+    ev, inp, sets, ids, weights = three_blocks(model_file, dtype, channels)
+    for name, (down, up) in sets.items():
+        ev.set_adapters(name, down, up)
+    ev.assign_adapters(ids, weights)
+    run(ev, inp)
+    for name, (down, up) in sets.items():
+        check_gradients(ev, name, down, up, ids, weights, dtype)
+
+
+def test_gradients_of_three_blocks_against_differences(model_file):
+    """float64, all four linears; the bound is that of ``tests/test_gpu_adapted_model.py`` for two blocks: with a step h = 1e-4 a central
+    difference is off by about h^2 of the gradient's size and by the energy's rounding over h."""
+    ev, inp, sets, ids, weights = three_blocks(model_file, "float64")
+
+    def energy():
+        for name, (down, up) in sets.items():
+            ev.set_adapters(name, down, up)
+        ev.assign_adapters(ids, weights)
+        return run(ev, inp)[0].sum()
+
+    total = energy()
+    grads = {name: ev.adapter_gradients(name) for name in sets}
+    h, rng = 1e-4, np.random.default_rng(5)
+
+    def check(array, grad):
+        scale = np.abs(grad).max()
+        for _ in range(3):
+            at = tuple(int(rng.integers(0, m)) for m in array.shape)
+            old, d = array[at], []
+            for sign in (1, -1):
+                array[at] = old + sign * h
+                d.append(energy())
+            array[at] = old
+            assert abs((d[0] - d[1]) / (2 * h) - grad[at]) <= 1e-6 * scale + 1e-11 * abs(total)
+
+    for name, (down, up) in sets.items():
+        for q in range(len(down)):
+            check(down[q], grads[name][0][q])
+            check(up[q], grads[name][1][q])
+    check(weights, sum(g[2] for g in grads.values()))
+
+
+@pytest.mark.parametrize("dtype", ["float64", "float32"])
+@pytest.mark.parametrize("mode", ["message_passing", "recompute"])
+def test_decomposed_evaluations(model_file, dtype, mode):
+    """Two ranks (emulated on one GPU), each with the adapters of its own rows, owned atoms and ghosts: energies, forces and the ranks' sum of
+    gradients are those of one domain, to the evaluator's bounds. With recomputed ghosts a linear's gradients are to be had while the
+    receivers that it ran on are the active ones."""
+    path, model, spec = model_file("fcc128", num_channels=32, num_spline_points=32)
+    s = st.fcc_box((8, 3, 3), 3.6, model["atomic_numbers"], seed=17, jitter=0.12)
+    rng = np.random.default_rng(2)
+    ids, weights = rng.integers(-1, 3, size=(s.num_atoms, 2)), rng.uniform(0.5, 1.5, size=(s.num_atoms, 2))
+    one = MACE(path)
+    sets = {name: adapters_of(one, name, 3, 4, q) for q, name in enumerate(("H1", "A1"))}
+
+    def give(ev, rows):
+        for name, (down, up) in sets.items():
+            ev.set_adapters(name, down, up)
+        ev.assign_adapters(ids[rows], weights[rows])
+
+    give(one, np.arange(s.num_atoms))
+    run(one, st.evaluator_inputs(s, st.neighbor_list(s, one.r_cut), one.atomic_numbers))
+    f_ref, _, e_ref = one.reduce_forces()
+    want = {name: one.adapter_gradients(name) for name in sets}
+    ranks = []
+    for r in range(2):
+        ev = MACE(path, dtype=dtype)
+        rk = SlabRank(make_slab_plan(s, spec.r_cut, r, 2, mode=mode), ev, spec.r_cut, ev.atomic_numbers)
+        give(ev, np.concatenate([rk.plan.own_global, rk.plan.ghost_global]))
+        rk.build_edges()
+        ranks.append(rk)
+    rel, fabs = (1e-10, 1e-9) if dtype == "float64" else (1e-4, 1e-3)
+    for _ in range(2):
+        energy, _, owned = evaluate_decomposed(ranks)
+        forces = np.zeros_like(f_ref)
+        for rk, f in zip(ranks, owned):
+            forces[rk.plan.own_global] = f.cpu().numpy()
+        assert abs(energy - e_ref) <= rel * abs(e_ref) and np.abs(forces - f_ref).max() <= fabs
+        for name in ("H1", "A1"):
+            total = [np.zeros(a.shape) for a in (*want[name][0], *want[name][1])]
+            for rk in ranks:
+                if mode == "recompute" and name == "A1":
+                    with pytest.raises(SymmetrixError, match="no evaluation"):
+                        rk.ev.adapter_gradients(name)
+                    rk.ev.set_active_nodes(rk.plan.n_own)
+                down, up, _ = rk.ev.adapter_gradients(name)
+                total = [t + a for t, a in zip(total, (*down, *up))]
+            for t, a in zip(total, (*want[name][0], *want[name][1])):
+                assert np.abs(t - a).max() <= 10 * rel * np.abs(a).max()
