@@ -401,7 +401,8 @@ int smx_adapter_backward(const smx_adapter_linear* call, char* errbuf, int errbu
  * than assigned is refused, one with fewer uses the first. smx_set_adapters or smx_assign_adapters that fail on the way (not for their arguments)
  * leave the linear without adapters, or no assignment. smx_adapter_gradients returns, after a whole evaluation, the gradients of the
  * total energy by a linear's adapters (in the layout of smx_set_adapters) and by the weights [active nodes * slots]; any may be NULL; a new edge set or
- * a compute_* stage since then and it is refused until the stages have gone back through the linear. */
+ * a compute_* stage since then, or other values in the linear's input or in the adjoint of its output (smx_set_array, smx_halo_unpack, a reverse_* stage
+ * that writes there), and it is refused until the stages have gone through the linear again. Values written through smx_device_ptr go unnoticed. */
 int smx_set_adapters(smx_handle h, const char* linear, int num_adapters, int rank, const double* down, long down_count,
                      const double* up, long up_count);
 int smx_assign_adapters(smx_handle h, int num_nodes, int slots, const int* ids, const double* weights);

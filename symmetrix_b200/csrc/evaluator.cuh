@@ -988,6 +988,27 @@ public:
     void adapters_stale() {
         for (auto& a : adapters) a.second.reversed = false;
     }
+    // Other values in an array that a linear's gradients are made of: its input, which `hidden` belongs to, or the adjoint of its output.
+    static const char* adapter_input(const std::string& linear) { return linear == "H1" ? "M0" : linear == "Hm" ? "Mm" : linear == "Am" ? "Phim" : "Phi1"; }
+    void adapter_array_changed(const std::string& array) {
+        for (auto& a : adapters) {
+            const bool input = array == adapter_input(a.first);
+            if (input) a.second.hidden_nodes = -1;
+            if (input || array == a.first + "_adj") a.second.reversed = false;
+        }
+    }
+    // What a stage called by itself writes of those arrays (a whole evaluation goes through all linears both ways).
+    void adapter_stage_writes(const std::string& stage) {
+        const char* feature_adj = deep() ? "Hm_adj" : "H1_adj";
+        if (stage == "compute_M0") adapter_array_changed("M0");
+        else if (stage == "compute_Phi1") adapter_array_changed("Phi1");
+        else if (stage == "compute_Phim") adapter_array_changed("Phim");
+        else if (stage == "compute_Mm") adapter_array_changed("Mm");
+        else if (stage == "reverse_H2" || stage == "reverse_Phi1") adapter_array_changed(feature_adj);
+        else if (stage == "reverse_M1" || stage == "reverse_A1_scaled") adapter_array_changed("A1_adj");
+        else if (stage == "reverse_Hm" || stage == "reverse_Phim") adapter_array_changed("H1_adj");
+        else if (stage == "reverse_Mm") adapter_array_changed("Am_adj");
+    }
     std::map<std::string, AdapterSet> adapters;
     int num_adapters = 0;                                         // of every linear that has some
     DevBuf<int> adapter_ids, adapter_plan;                        // as assigned; order, position and offsets of the first `adapter_planned` nodes
@@ -1178,8 +1199,8 @@ public:
         if (!adapters_on(name.c_str())) throw ArgError("smx_adapter_gradients: " + name + " has no adapters, or no node uses any");
         AdapterSet& a = adapters.at(name);
         smx_adapter_linear c = adapter_call(name.c_str());
-        const DevBuf<T>& x = name == "H1" ? M0 : name == "Hm" ? Mm : name == "Am" ? Phim : Phi1;
-        const DevBuf<T>& gy = name == "H1" ? H1_adj : name == "Hm" ? Hm_adj : name == "Am" ? Am_adj : A1_adj;
+        const DevBuf<T>& x = *field(adapter_input(name)).t;
+        const DevBuf<T>& gy = *field(name + "_adj").t;
         if (!a.reversed || a.hidden_nodes != N || x.n != static_cast<size_t>(N) * c.x_stride || gy.n < static_cast<size_t>(N) * c.grad_y_stride)
             throw ArgError("smx_adapter_gradients: no evaluation of the current nodes with these adapters has been made");
         c.x = x.p; c.grad_y = gy.p; c.hidden = a.hidden.p;
@@ -1770,6 +1791,7 @@ public:
         SMX_CUDA(cudaSetDevice(device));
         NvtxRange range(s.c_str());
         if (s.rfind("compute_", 0) == 0) adapters_stale();
+        adapter_stage_writes(s);
         if (s == "compute_Y" || s == "compute_R0" || s == "compute_R1") return;  // fused into the edge kernels
         if (s == "compute_A0") compute_A0();
         else if (s == "compute_ZBL") compute_ZBL();
@@ -2079,6 +2101,7 @@ public:
         SMX_CUDA(cudaSetDevice(device));
         if (n < 0 || (n > 0 && !src)) throw ArgError("set_array: bad source");
         Field f = field(name);
+        adapter_array_changed(name);
         if (f.d) {
             f.d->resize(n, stream);
             if (n) SMX_CUDA(cudaMemcpyAsync(f.d->p, src, n * sizeof(double),
@@ -2148,6 +2171,7 @@ public:
         SMX_CUDA(cudaSetDevice(device));
         if (n < 0 || (n > 0 && (!rows || !src))) throw ArgError("halo_unpack: bad arguments");
         if (n == 0) return;
+        adapter_array_changed(name);
         const int* grouped_rows = nullptr;
         const int* grouped_pos = nullptr;
         if (add) {

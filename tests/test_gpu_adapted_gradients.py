@@ -9,7 +9,7 @@ import torch
 
 from symmetrix_b200 import MACE, SymmetrixError, structures as st
 from symmetrix_b200.domain import SlabRank, evaluate_decomposed, make_slab_plan
-from tests.test_gpu_adapted_model import adapters_of, run
+from tests.test_gpu_adapted_model import adapters_of, box, run
 from tests.test_gpu_adapters import EPS
 
 pytestmark = pytest.mark.gpu
@@ -186,3 +186,62 @@ def test_decomposed_evaluations(model_file, dtype, mode):
                 total = [t + a for t, a in zip(total, (*down, *up))]
             for t, a in zip(total, (*want[name][0], *want[name][1])):
                 assert np.abs(t - a).max() <= 10 * rel * np.abs(a).max()
+
+
+@pytest.mark.parametrize("dtype", ["float64", "float32"])
+def test_no_gradients_of_arrays_that_were_changed(model_file, dtype):
+    """A linear's gradients are made of its input, the kept products of that input, and the adjoint of its output: other values in one of them
+    (put there, received from another rank, added by a reverse stage) and they are refused until the stages have gone through again."""
+    path, model, spec = model_file("fcc128", num_channels=24, num_spline_points=32)
+    ev = MACE(path, dtype=dtype)
+    inp = box(spec, model, 2, 7)
+    n = int(inp["num_nodes"])
+    ids, weights = np.arange(n)[:, None] % 3 - 1, np.linspace(0.5, 1.5, n)[:, None]
+    sets = {name: adapters_of(ev, name, 2, 3, q) for q, name in enumerate(("H1", "A1"))}
+    for name, (down, up) in sets.items():
+        ev.set_adapters(name, down, up)
+    ev.assign_adapters(ids, weights)
+
+    def refused(*names):
+        for name in sets:
+            if name in names:
+                with pytest.raises(SymmetrixError, match="no evaluation"):
+                    ev.adapter_gradients(name)
+            else:
+                ev.adapter_gradients(name)
+
+    run(ev, inp)
+    refused()
+    ev.set("M0", 2.0 * ev.get("M0"))
+    refused("H1")
+    ev.reverse_H1()
+    refused("H1")                                     # the products kept are those of the old input
+    ev.compute_H1()
+    refused("H1", "A1")
+    run(ev, inp)
+    ev.set("H1_adj", 2.0 * ev.get("H1_adj"))
+    refused("H1")
+    ev.reverse_H1()
+    refused()
+    check_gradients(ev, "H1", *sets["H1"], ids, weights, dtype)
+    ev.set("A1_adj", 2.0 * ev.get("A1_adj"))
+    refused("A1")
+    ev.reverse_A1()
+    refused()
+    check_gradients(ev, "A1", *sets["A1"], ids, weights, dtype)
+    ev.reverse_Phi1(zero_dxyz=False, zero_H1_adj=False)            # adds to the adjoint of H1 once more
+    refused("H1")
+    run(ev, inp)
+    rows = torch.arange(3, dtype=torch.int32, device="cuda")
+    ev.halo_unpack("H1_adj", rows, ev.halo_pack("H1_adj", rows), add=True)
+    refused("H1")
+    run(ev, inp)
+    ev.reverse_M1()
+    refused("A1")
+    run(ev, inp)
+    ev.compute_Phi1()
+    refused("H1", "A1")
+    ev.reverse_A1()
+    refused("H1", "A1")                               # no products of the new input have been kept
+    run(ev, inp)
+    refused()
