@@ -244,6 +244,9 @@ __global__ void __launch_bounds__(kDpThreads) adapter_pass_f64_kernel(const __gr
             if (d.hidden && col_block == 0) d.hidden[hid_row[r] * R + c] = h;
             Hs[r * SF + c] = h * weight[r];
         }
+        // the columns that fill the rank up to four: zeros times the row, so NaN where it holds an infinity, and the rows of second_g they meet are zeros
+        const int pad = -R & 3;
+        for (int i = tid; i < rows * pad; i += kDpThreads) Hs[i / pad * SF + R + i % pad] = 0.0;
         if (!pass.out) return;
         __syncthreads();
     }
@@ -251,7 +254,7 @@ __global__ void __launch_bounds__(kDpThreads) adapter_pass_f64_kernel(const __gr
     for (;;) {
         if (adapter)
 #pragma unroll 2
-        for (int r0 = 0; r0 < R; r0 += 4) {              // hidden columns beyond the rank are sums over zeros
+        for (int r0 = 0; r0 < R; r0 += 4) {
             double a[MB];
 #pragma unroll
             for (int i = 0; i < MB; ++i) a[i] = Hs[(wm * MB * 8 + i * 8 + fr) * SF + r0 + fk];

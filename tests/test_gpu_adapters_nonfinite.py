@@ -65,3 +65,22 @@ def test_nan_made_by_arithmetic(shared):
     got = layer.forward(case.x, routing, case.weights)
     assert torch.isnan(got[5]).all()
     assert torch.equal(got[:5], clean[:5]) and torch.equal(got[6:], clean[6:])
+
+
+@pytest.mark.filterwarnings("ignore:invalid value")
+@pytest.mark.parametrize("shared", [True, False])
+@pytest.mark.parametrize("rank", [1, 2, 3, 5, 6, 7, 9, 61])
+def test_infinities_in_float64(rank, shared):
+    """Positive factors: an infinite value makes positive infinities, and no NaN from the columns that pad the rank. (The reference says where; without
+    shared weights it has zeros in their place, which make NaN there.)"""
+    case = Case(torch.float64, [1, 3], [24, 17], [17, 24], 90, 1, 2, rank, shared=shared)
+    for m in (*case.down, *case.up, *(case.shared or []), case.weights, case.x, case.gy):
+        m.abs_().add_(0.1)
+    case.ids[:] = 1
+    case.x[17, 30], case.gy[40, 3] = float("inf"), float("inf")
+    layer, routing = case.layer(), RowRouting(case.ids, case.groups)
+    y, grads = layer.forward(case.x, routing, case.weights), layer.backward(case.x, case.gy, routing, case.weights)
+    want_y, want_gx, gds, gus, gw = case.reference()
+    for got, want in zip([y, grads.x, *grads.down, *grads.up, grads.weights], [want_y, want_gx, *gds, *gus, gw]):
+        assert (host(got)[~np.isfinite(want)] == np.inf).all()
+        assert np.isfinite(host(got)[np.isfinite(want)]).all()
