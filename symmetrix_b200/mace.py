@@ -26,6 +26,16 @@ class SymmetrixError(RuntimeError):
         self.status = status
 
 
+def _adapter_ids(ids) -> np.ndarray:
+    """`ids` as the library takes them: int32 with everything beyond that range, which is no adapter's number, as -1."""
+    i = np.asarray(ids)
+    if i.ndim not in (1, 2):
+        raise ValueError("ids must have shape [nodes] or [nodes, slots]")
+    if i.dtype.kind not in "iub" and not (i.dtype.kind == "f" and (i == np.trunc(i)).all()):
+        raise ValueError("ids must be whole numbers")
+    return np.ascontiguousarray(np.where((i >= 0) & (i < 2 ** 31), i, -1).astype(np.int32))
+
+
 def _is_device_tensor(x) -> bool:
     return hasattr(x, "data_ptr") and getattr(x, "is_cuda", False)
 
@@ -340,9 +350,7 @@ class MACE:
         if ids is None:
             self._check(self._lib.smx_assign_adapters(self._h, 0, 1, None, None))
             return
-        i = np.ascontiguousarray(ids, dtype=np.int32)
-        if i.ndim not in (1, 2):
-            raise ValueError("ids must have shape [nodes] or [nodes, slots]")
+        i = _adapter_ids(ids)
         w = None if weights is None else np.ascontiguousarray(weights, dtype=np.float64)
         if w is not None and w.shape != i.shape:
             raise ValueError("weights must have the shape of ids")
