@@ -121,7 +121,8 @@ class RowRouting:
         self.num_rows, self.slots = ids.shape[0], ids.shape[1] if ids.dim() == 2 else 1
         self.num_groups, self.device = int(num_groups), ids.device
         self._library = _lib.load()
-        need = self._library.smx_route_plan_bytes(self.num_rows, self.slots, self.num_groups)
+        # (checked here too: a C int would hold what is left of a larger number)
+        need = self._library.smx_route_plan_bytes(self.num_rows, self.slots, self.num_groups) if 1 <= self.num_groups <= _lib.ROUTE_MAX_GROUPS else -1
         if need < 0:
             raise ValueError(f"{self.num_rows} rows with {self.slots} slots and {self.num_groups} groups: the limits are {_lib.ROUTE_MAX_SLOTS} slots, "
                              f"{_lib.ROUTE_MAX_GROUPS} groups and 2^31 - 2^11 pairs, and one slot and group at least")
@@ -248,8 +249,8 @@ class AdapterLinear:
         if len(self.components) != len(down) or any(not 1 <= c <= 1024 for c in self.components):
             raise ValueError("components needs a number in 1 .. 1024 for each degree")
         self.in_channels, self.out_channels = [a.shape[1] for a in down], [b.shape[2] for b in up]
-        if any(n < 1 for n in self.in_channels + self.out_channels):
-            raise ValueError("a degree needs a channel at least")
+        if any(not 1 <= n <= 1 << 20 for n in self.in_channels + self.out_channels):
+            raise ValueError("a degree needs 1 .. 1048576 channels")
         self.in_width = sum(c * i for c, i in zip(self.components, self.in_channels))
         self.out_width = sum(c * o for c, o in zip(self.components, self.out_channels))
         self._library = _lib.load()
