@@ -352,8 +352,8 @@ int smx_route_combine_backward(int precision, const void* grad_y, long grad_y_st
  * smx_adapter_backward reads grad_y, x (and hidden) and writes, each unless NULL, grad_x, the degrees' grad_down / grad_up (both, for all
  * degrees or none; groups without atoms get zeros) and grad_weights [num_rows][slots] (zero in empty slots). The shared weights are
  * frozen: they have no gradient here.
- * float32: products on the tensor cores from operands split in two (3xTF32), sums in float32, for magnitudes up to 2^127 (infinities in x or
- * the matrices give NaN); float64 throughout otherwise. An atom's slots are added in their order. Sums over atoms are split into chunks, whose
+ * float32: products on the tensor cores from operands split in two (3xTF32), sums in float32, for magnitudes up to 2^127 (NaN stays NaN,
+ * infinities in x, the matrices or the weights give NaN); float64 throughout otherwise. An atom's slots are added in their order. Sums over atoms are split into chunks, whose
  * length follows from the sizes alone, and added in order: the same call gives the same bits. Outputs must not overlap inputs or one another.
  * The rules of the smx_route_* calls hold: device pointers on the current GPU, `stream`, no allocation, no wait, a workspace of
  * smx_adapter_workspace_bytes bytes for each call that may overlap with another one, errors through `errbuf`. The size functions

@@ -343,7 +343,7 @@ constexpr int kTsOutPitch = 17;                                               //
 constexpr int kTsRegsControl = 72, kTsRegsRows = 120, kTsRegsSums = 160, kTsRegsLaunch = 128;
 static_assert(kTsRegsControl + kTsRegsRows + 2 * kTsRegsSums <= 4 * kTsRegsLaunch, "the registers of the launch are shared out");
 // HP: hidden columns / 16. kWide: every row's half of a tile starts on 32 bytes and is 64 columns long, so nothing is staged on its way out and the
-// rows have five stages instead of four (160 us instead of 165 at 98,304 atoms, 128 channels, rank 32).
+// rows have five stages instead of four (161 .. 165 us instead of 167 at 98,304 atoms, 128 channels, rank 32).
 template <int HP, bool kWide>
 struct TsPassLayout {
     static constexpr int row_stages = kWide ? 5 : 4;
