@@ -204,12 +204,14 @@ def prepare(case, seed):
         state["flat"] = {t: torch.zeros(n, dtype=t, device="cuda") for t, n in _flat_sizes(case).items()}
         state["out"] = _views(case, state["flat"])
     if own:
-        from symmetrix_b200 import Embedding, GroupedLinear, RowRouting
+        from symmetrix_b200 import Embedding, GradientSet, GroupedLinear, RowRouting
         if kind == "grouped":
             state["routing"] = RowRouting(state["ids"], case["groups"])
             state["layer"] = GroupedLinear(state["matrices"])
         elif kind == "embed":
             state["embedding"] = Embedding(state["table"])
+        else:
+            state["set"] = GradientSet(state["grads"], out=state["out"])
     elif kind == "grouped":
         flat = state["ids"].reshape(-1)
         counts = torch.bincount(flat[flat >= 0], minlength=case["groups"])
@@ -292,7 +294,7 @@ def run(state):
         return {"grouped": _plain_grouped, "embed": _plain_embed, "clip": _plain_clip}[kind](state)
     from symmetrix_b200 import EmbeddingPlan, clip_gradients
     if kind == "clip":
-        return {"norm": clip_gradients(state["grads"], case["max_norm"], out=state["out"]), "grads": list(state["flat"].values())}
+        return {"norm": state["set"].clip(case["max_norm"]), "grads": list(state["flat"].values())}
     if kind == "embed":
         embedding = state["embedding"]
         y = embedding.forward(state["ids"], state["weights"])
