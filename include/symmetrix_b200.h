@@ -390,6 +390,78 @@ long smx_adapter_workspace_bytes(const smx_adapter_linear* call, int backward);
 int smx_adapter_forward(const smx_adapter_linear* call, char* errbuf, int errbuf_len);
 int smx_adapter_backward(const smx_adapter_linear* call, char* errbuf, int errbuf_len);
 
+/* Linears of routed rows, every group (an element, a variant, an expert) with matrices of its own. Rows are in the order of a plan of smx_route_plan, as
+ * smx_route_dispatch leaves them: those of group g are offsets[g] .. offsets[g + 1] - 1 of `num_rows`. A row of `x` holds, degree after degree,
+ * `components` rows of in_channels values, a row of `y` the same with out_channels; with `weight` [num_groups][in][out] of the degree
+ *   y = x weight[g];   grad_x = grad_y weight[g]^T,   grad_weight[g] = sum over the group's rows and components of x^T grad_y.
+ * smx_grouped_backward writes, each unless NULL, grad_x and the degrees' grad_weight (for all degrees or none; groups without rows get
+ * zeros). Rows behind the last group are never read; in `y` they are left as they were, or zeroed with `zero_tail` != 0, in grad_x they are zeroed.
+ * The matrices are read as they are, in every call: changed values count at once. Sums, float32 operands, NaN, infinities, waits inside the float32 kernels,
+ * `status`, streams, workspaces (smx_grouped_workspace_bytes) and limits: as for smx_adapter_*. Outputs must not overlap inputs or one another. */
+enum { SMX_GROUPED_MAX_DEGREES = 8 };
+typedef struct smx_grouped_degree {
+    int components, in_channels, out_channels;
+    const void* weight;
+    void* grad_weight;
+} smx_grouped_degree;
+typedef struct smx_grouped_linear {
+    int precision, num_degrees, num_groups, zero_tail;
+    long num_rows;
+    smx_grouped_degree degrees[8];
+    const int* offsets;                      /* of smx_route_plan */
+    const void* x;      long x_stride;       /* strides: elements from row to row */
+    void* y;            long y_stride;
+    const void* grad_y; long grad_y_stride;
+    void* grad_x;       long grad_x_stride;
+    void* workspace;    long workspace_bytes;
+    void* stream;
+    int* status;                             /* NULL, or an int that the caller has zeroed */
+} smx_grouped_linear;
+long smx_grouped_workspace_bytes(const smx_grouped_linear* call, int backward);
+int smx_grouped_forward(const smx_grouped_linear* call, char* errbuf, int errbuf_len);
+int smx_grouped_backward(const smx_grouped_linear* call, char* errbuf, int errbuf_len);
+
+/* Embeddings: rows of a table named by tokens (elements, or pairs of a variant and an element), `slots` of them for every row n,
+ *   y[n, :] = scale * sum_s weights[n, s] * table[ids[n, s], :]      (`weights` NULL: ones)
+ * An id outside [0, table_rows) is an empty slot: it counts for nothing, and nothing of it is read but the id.
+ * smx_embedding_plan sorts the pairs (n, s) by token, equal ones in the order of the list and empty slots last: order[p] = n * slots + s of the
+ * p-th pair, tokens[p] = its token (table_rows: none). With it smx_embedding_backward writes, each unless NULL,
+ *   grad_table[t, :] = scale * sum over pairs with token t of weights[n, s] * grad_y[n, :]    ([table_rows][width], contiguous; zero without pairs)
+ *   grad_weights[n, s] = scale * <grad_y[n, :], table[ids[n, s], :]>                          (zero in empty slots; alone this one reads `table`)
+ * Sums over pairs are cut into chunks whose length follows from the sizes alone, and added in order: the same call gives the same bits.
+ * The rules of the smx_route_* calls hold, with a workspace of smx_embedding_plan_bytes / smx_embedding_backward_bytes (the latter starts on
+ * a 16-byte boundary) for each call that may overlap with another one. Strides count elements from row to row. */
+enum { SMX_EMBEDDING_MAX_ROWS = (1 << 20) - 1 };
+long smx_embedding_plan_bytes(long num_rows, int slots, int table_rows);
+int smx_embedding_plan(const int* ids, long num_rows, int slots, int table_rows, int* order, int* tokens, void* workspace,
+                       long workspace_bytes, void* stream, char* errbuf, int errbuf_len);
+int smx_embedding_forward(int precision, const void* table, long table_stride, int table_rows, const int* ids, long num_rows, int slots,
+                          long width, const void* weights, double scale, void* y, long y_stride, void* stream, char* errbuf, int errbuf_len);
+long smx_embedding_backward_bytes(int precision, long num_rows, int slots, long width);
+int smx_embedding_backward(int precision, const void* grad_y, long grad_y_stride, const void* table, long table_stride, int table_rows,
+                           const int* order, const int* tokens, long num_rows, int slots, long width, const void* weights, double scale,
+                           void* grad_table, void* grad_weights, void* workspace, long workspace_bytes, void* stream, char* errbuf,
+                           int errbuf_len);
+
+/* The common norm of many tensors, and their scaling to at most a given one, as training does with all gradients before a step:
+ *   norm = sqrt(sum over all values t^2),   out = values * (norm > max_norm ? max_norm / norm : 1)
+ * A tensor is `count` consecutive values of a precision of its own; `out` may be `values`, or memory that overlaps no tensor of the list.
+ * Squares, sums and products are float64; a product is rounded once. A NaN makes the norm and all outputs NaN; an infinity makes the norm
+ * infinite, finite values zero and infinite ones NaN (unless max_norm is infinite too). smx_gradient_norm ignores `out`; `norm` is a device double and may be NULL in
+ * smx_gradient_clip. The list itself is read on the host, during the call. The rules of the smx_route_* calls hold, with a workspace of
+ * smx_gradient_workspace_bytes for each call that may overlap with another one. Limit: 2^40 values a tensor. */
+typedef struct smx_gradient {
+    const void* values;
+    void* out;
+    long count;
+    int precision;
+} smx_gradient;
+long smx_gradient_workspace_bytes(const smx_gradient* list, int count);
+int smx_gradient_norm(const smx_gradient* list, int count, double* norm, void* workspace, long workspace_bytes, void* stream, char* errbuf,
+                      int errbuf_len);
+int smx_gradient_clip(const smx_gradient* list, int count, double max_norm, double* norm, void* workspace, long workspace_bytes, void* stream,
+                      char* errbuf, int errbuf_len);
+
 /* Adapters of an evaluator's own linears: smx_compute, smx_evaluate and the stages then evaluate every node with the variant of the model that
  * it is assigned, in one call for all variants. `linear` is "H1" (compute_H1: M0 to H1), "A1" (compute_A1: Phi1 to A1) or, in three-block
  * models, "Am" or "Hm" (there beside the weights of Mm). smx_set_adapters gives a linear `num_adapters` adapters of rank `rank`, host arrays of

@@ -26,10 +26,14 @@ EXPORTED_SYMBOLS = [
     "smx_comm_unique_id", "smx_comm_init", "smx_comm_destroy", "smx_halo_exchange", "smx_allreduce_sum", "smx_model_digest",
     "smx_set_adapters", "smx_assign_adapters", "smx_adapter_gradients", "smx_route_plan_bytes", "smx_route_plan", "smx_route_dispatch", "smx_route_combine", "smx_route_combine_backward",
     "smx_adapter_tiles_bytes", "smx_adapter_prepare", "smx_adapter_hidden_elements", "smx_adapter_workspace_bytes", "smx_adapter_forward", "smx_adapter_backward",
+    "smx_grouped_workspace_bytes", "smx_grouped_forward", "smx_grouped_backward", "smx_embedding_plan_bytes", "smx_embedding_plan", "smx_embedding_forward",
+    "smx_embedding_backward_bytes", "smx_embedding_backward", "smx_gradient_workspace_bytes", "smx_gradient_norm", "smx_gradient_clip",
 ]
 ROUTE_MAX_GROUPS, ROUTE_MAX_SLOTS = 1024, 64
 ADAPTER_MAX_RANK, ADAPTER_MAX_DEGREES = 64, 8
 ADAPTER_SHARED, ADAPTER_MATRICES = 1, 2
+GROUPED_MAX_DEGREES = 8
+EMBEDDING_MAX_ROWS = (1 << 20) - 1
 
 
 class ModelInfo(ctypes.Structure):
@@ -56,6 +60,23 @@ class AdapterCall(ctypes.Structure):
                 ("grad_y", ctypes.c_void_p), ("grad_y_stride", ctypes.c_long), ("grad_x", ctypes.c_void_p), ("grad_x_stride", ctypes.c_long),
                 ("grad_weights", ctypes.c_void_p), ("hidden", ctypes.c_void_p), ("workspace", ctypes.c_void_p),
                 ("workspace_bytes", ctypes.c_long), ("stream", ctypes.c_void_p), ("status", ctypes.c_void_p)]
+
+
+class GroupedDegree(ctypes.Structure):
+    _fields_ = [("components", ctypes.c_int), ("in_channels", ctypes.c_int), ("out_channels", ctypes.c_int),
+                ("weight", ctypes.c_void_p), ("grad_weight", ctypes.c_void_p)]
+
+
+class GroupedCall(ctypes.Structure):
+    _fields_ = [("precision", ctypes.c_int), ("num_degrees", ctypes.c_int), ("num_groups", ctypes.c_int), ("zero_tail", ctypes.c_int),
+                ("num_rows", ctypes.c_long), ("degrees", GroupedDegree * GROUPED_MAX_DEGREES), ("offsets", ctypes.c_void_p),
+                ("x", ctypes.c_void_p), ("x_stride", ctypes.c_long), ("y", ctypes.c_void_p), ("y_stride", ctypes.c_long),
+                ("grad_y", ctypes.c_void_p), ("grad_y_stride", ctypes.c_long), ("grad_x", ctypes.c_void_p), ("grad_x_stride", ctypes.c_long),
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_long), ("stream", ctypes.c_void_p), ("status", ctypes.c_void_p)]
+
+
+class Gradient(ctypes.Structure):
+    _fields_ = [("values", ctypes.c_void_p), ("out", ctypes.c_void_p), ("count", ctypes.c_long), ("precision", ctypes.c_int)]
 
 
 _lib = None
@@ -140,5 +161,23 @@ def load():
     lib.smx_adapter_workspace_bytes.restype = cl
     lib.smx_adapter_forward.argtypes = [call, *err]
     lib.smx_adapter_backward.argtypes = [call, *err]
+    call = ctypes.POINTER(GroupedCall)
+    lib.smx_grouped_workspace_bytes.argtypes = [call, ci]
+    lib.smx_grouped_workspace_bytes.restype = cl
+    lib.smx_grouped_forward.argtypes = [call, *err]
+    lib.smx_grouped_backward.argtypes = [call, *err]
+    cd = ctypes.c_double
+    lib.smx_embedding_plan_bytes.argtypes = [cl, ci, ci]
+    lib.smx_embedding_plan_bytes.restype = cl
+    lib.smx_embedding_plan.argtypes = [ip, cl, ci, ci, ip, ip, vp, cl, vp, *err]
+    lib.smx_embedding_forward.argtypes = [ci, vp, cl, ci, ip, cl, ci, cl, vp, cd, vp, cl, vp, *err]
+    lib.smx_embedding_backward_bytes.argtypes = [ci, cl, ci, cl]
+    lib.smx_embedding_backward_bytes.restype = cl
+    lib.smx_embedding_backward.argtypes = [ci, vp, cl, vp, cl, ci, ip, ip, cl, ci, cl, vp, cd, vp, vp, vp, cl, vp, *err]
+    gradients = ctypes.POINTER(Gradient)
+    lib.smx_gradient_workspace_bytes.argtypes = [gradients, ci]
+    lib.smx_gradient_workspace_bytes.restype = cl
+    lib.smx_gradient_norm.argtypes = [gradients, ci, vp, vp, cl, vp, *err]
+    lib.smx_gradient_clip.argtypes = [gradients, ci, cd, vp, vp, cl, vp, *err]
     _lib = lib
     return lib

@@ -16,7 +16,8 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libsymmetrix_b200.so"
 BUILD = PKG / "build"
-SOURCES = [CSRC / "evaluator_f64.cu", CSRC / "evaluator_f32.cu", CSRC / "capi.cu", CSRC / "noalloc.cu", CSRC / "routing.cu", CSRC / "adapters.cu"]
+SOURCES = [CSRC / "evaluator_f64.cu", CSRC / "evaluator_f32.cu", CSRC / "capi.cu", CSRC / "noalloc.cu", CSRC / "routing.cu", CSRC / "adapters.cu",
+           CSRC / "grouped.cu", CSRC / "embedding.cu", CSRC / "gradients.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC", "-Xcudafe", "--diag_suppress=177",

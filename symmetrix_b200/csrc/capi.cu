@@ -11,6 +11,9 @@
 
 #include "../../include/symmetrix_b200.h"
 #include "adapters.hpp"
+#include "embedding.hpp"
+#include "gradients.hpp"
+#include "grouped.hpp"
 #include "common.cuh"
 #include "evaluator_base.hpp"
 #include "model_cache.hpp"
@@ -432,6 +435,78 @@ int smx_adapter_backward(const smx_adapter_linear* call, char* errbuf, int errbu
     return guarded_free(errbuf, errbuf_len, [&] {
         if (!call) throw smx::ArgError("smx_adapter_backward: null call");
         smx::adapter_backward(*call);
+    });
+}
+
+long smx_grouped_workspace_bytes(const smx_grouped_linear* call, int backward) {
+    return call ? size_or_refusal([&] { return smx::grouped_workspace_bytes(*call, backward != 0); }) : -1;
+}
+int smx_grouped_forward(const smx_grouped_linear* call, char* errbuf, int errbuf_len) {
+    return guarded_free(errbuf, errbuf_len, [&] {
+        if (!call) throw smx::ArgError("smx_grouped_forward: null call");
+        smx::grouped_forward(*call);
+    });
+}
+int smx_grouped_backward(const smx_grouped_linear* call, char* errbuf, int errbuf_len) {
+    return guarded_free(errbuf, errbuf_len, [&] {
+        if (!call) throw smx::ArgError("smx_grouped_backward: null call");
+        smx::grouped_backward(*call);
+    });
+}
+long smx_embedding_plan_bytes(long num_rows, int slots, int table_rows) {
+    return size_or_refusal([&] { return smx::embedding_plan_bytes(num_rows, slots, table_rows); });
+}
+int smx_embedding_plan(const int* ids, long num_rows, int slots, int table_rows, int* order, int* tokens, void* workspace, long workspace_bytes,
+                       void* stream, char* errbuf, int errbuf_len) {
+    return guarded_free(errbuf, errbuf_len, [&] {
+        if (workspace_bytes < 0) throw smx::ArgError("smx_embedding_plan: negative workspace size");
+        smx::embedding_plan(ids, num_rows, slots, table_rows, order, tokens, workspace, static_cast<size_t>(workspace_bytes), static_cast<cudaStream_t>(stream));
+    });
+}
+int smx_embedding_forward(int precision, const void* table, long table_stride, int table_rows, const int* ids, long num_rows, int slots, long width,
+                          const void* weights, double scale, void* y, long y_stride, void* stream, char* errbuf, int errbuf_len) {
+    return guarded_free(errbuf, errbuf_len, [&] {
+        with_precision(precision, "smx_embedding_forward", [&](auto* t) {
+            using T = std::remove_pointer_t<decltype(t)>;
+            smx::embedding_forward<T>(static_cast<const T*>(table), table_stride, table_rows, ids, num_rows, slots, width, static_cast<const T*>(weights), scale,
+                                      static_cast<T*>(y), y_stride, static_cast<cudaStream_t>(stream));
+        });
+    });
+}
+long smx_embedding_backward_bytes(int precision, long num_rows, int slots, long width) {
+    return size_or_refusal([&] {
+        size_t n = 0;
+        with_precision(precision, "smx_embedding_backward", [&](auto* t) { n = smx::embedding_backward_bytes<std::remove_pointer_t<decltype(t)>>(num_rows, slots, width); });
+        return n;
+    });
+}
+int smx_embedding_backward(int precision, const void* grad_y, long grad_y_stride, const void* table, long table_stride, int table_rows, const int* order,
+                           const int* tokens, long num_rows, int slots, long width, const void* weights, double scale, void* grad_table, void* grad_weights,
+                           void* workspace, long workspace_bytes, void* stream, char* errbuf, int errbuf_len) {
+    return guarded_free(errbuf, errbuf_len, [&] {
+        if (workspace_bytes < 0) throw smx::ArgError("smx_embedding_backward: negative workspace size");
+        with_precision(precision, "smx_embedding_backward", [&](auto* t) {
+            using T = std::remove_pointer_t<decltype(t)>;
+            smx::embedding_backward<T>(static_cast<const T*>(grad_y), grad_y_stride, static_cast<const T*>(table), table_stride, table_rows, order, tokens, num_rows,
+                                       slots, width, static_cast<const T*>(weights), scale, static_cast<T*>(grad_table), static_cast<T*>(grad_weights), workspace,
+                                       static_cast<size_t>(workspace_bytes), static_cast<cudaStream_t>(stream));
+        });
+    });
+}
+long smx_gradient_workspace_bytes(const smx_gradient* list, int count) {
+    return size_or_refusal([&] { return smx::gradient_workspace_bytes(list, count); });
+}
+int smx_gradient_norm(const smx_gradient* list, int count, double* norm, void* workspace, long workspace_bytes, void* stream, char* errbuf, int errbuf_len) {
+    return guarded_free(errbuf, errbuf_len, [&] {
+        if (workspace_bytes < 0) throw smx::ArgError("smx_gradient_norm: negative workspace size");
+        smx::gradient_norm_clip(list, count, false, 0.0, norm, workspace, static_cast<size_t>(workspace_bytes), static_cast<cudaStream_t>(stream));
+    });
+}
+int smx_gradient_clip(const smx_gradient* list, int count, double max_norm, double* norm, void* workspace, long workspace_bytes, void* stream, char* errbuf,
+                      int errbuf_len) {
+    return guarded_free(errbuf, errbuf_len, [&] {
+        if (workspace_bytes < 0) throw smx::ArgError("smx_gradient_clip: negative workspace size");
+        smx::gradient_norm_clip(list, count, true, max_norm, norm, workspace, static_cast<size_t>(workspace_bytes), static_cast<cudaStream_t>(stream));
     });
 }
 

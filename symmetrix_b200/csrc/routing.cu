@@ -26,20 +26,38 @@ constexpr int kMaxGroups = SMX_ROUTE_MAX_GROUPS;
 // Pairs are counted and ranked by warps that own consecutive pairs: 32 at a time, lanes of equal group found with match_any, one counter
 // per (warp, group) in shared memory that only that warp touches. Equal keys therefore keep their order. Latency bounds it: 13.5 us for 7,545
 // pairs in one CTA, 6 + 4 + 10 us for the three kernels at 196,608 pairs (2.4 MB).
-// kSlots: the keys are the slots of pairs, ids[i] = n * groups + slot (see route_slots).
-template <bool kSlots>
-__device__ __forceinline__ int route_key(const int* ids, long long i, int groups) {
-    const int g = ids[i];
-    if (kSlots) return g % groups;
-    return (g < 0 || g >= groups) ? groups : g;
-}
+// What is sorted: key(i) of element i, and what order[] receives for it; kPlan: with positions and offsets.
+struct GroupKeys {                               // pairs by group, empty slots last
+    static constexpr bool kPlan = true;
+    const int* ids; int groups;
+    __device__ __forceinline__ int key(long long i) const {
+        const int g = ids[i];
+        return (g < 0 || g >= groups) ? groups : g;
+    }
+    __device__ __forceinline__ int value(long long i) const { return static_cast<int>(i); }
+};
+struct SlotKeys {                                // places by the slot of their pair, order[i] = n * slots + slot (see route_slots)
+    static constexpr bool kPlan = false;
+    const int* order; int slots;
+    __device__ __forceinline__ int key(long long i) const { return order[i] % slots; }
+    __device__ __forceinline__ int value(long long i) const { return static_cast<int>(i); }
+};
+struct DigitKeys {                               // pairs by a digit of their token, in the order that the lower digits gave (null: as they come)
+    static constexpr bool kPlan = false;
+    const int* ids; int table_rows; const int* before; int shift, mask;
+    __device__ __forceinline__ int key(long long i) const {
+        const int t = ids[value(i)];
+        return ((t < 0 || t >= table_rows ? table_rows : t) >> shift) & mask;
+    }
+    __device__ __forceinline__ int value(long long i) const { return before ? before[i] : static_cast<int>(i); }
+};
 
-template <bool kSlots>
-__device__ __forceinline__ void route_count(const int* __restrict__ ids, long long begin, long long end, int groups, int* __restrict__ hist) {
+template <typename Keys>
+__device__ __forceinline__ void route_count(const Keys& keys, long long begin, long long end, int groups, int* __restrict__ hist) {
     const int lane = threadIdx.x & 31;
     for (long long i0 = begin; i0 < end; i0 += 32) {
         const bool in = i0 + lane < end;
-        const int g = in ? route_key<kSlots>(ids, i0 + lane, groups) : groups + 1;
+        const int g = in ? keys.key(i0 + lane) : groups + 1;
         const unsigned same = __match_any_sync(0xffffffffu, g);
         if (in && lane == __ffs(same) - 1) hist[g] += __popc(same);
         __syncwarp();
@@ -47,21 +65,21 @@ __device__ __forceinline__ void route_count(const int* __restrict__ ids, long lo
 }
 
 // `next[g]`: where this warp's next pair of group g goes.
-template <bool kSlots>
-__device__ __forceinline__ void route_place(const int* __restrict__ ids, long long begin, long long end, int groups, int* __restrict__ next,
+template <typename Keys>
+__device__ __forceinline__ void route_place(const Keys& keys, long long begin, long long end, int groups, int* __restrict__ next,
                                             int* __restrict__ order, int* __restrict__ position) {
     const int lane = threadIdx.x & 31;
     for (long long i0 = begin; i0 < end; i0 += 32) {
         const bool in = i0 + lane < end;
-        const int g = in ? route_key<kSlots>(ids, i0 + lane, groups) : groups + 1;
+        const int g = in ? keys.key(i0 + lane) : groups + 1;
         const unsigned same = __match_any_sync(0xffffffffu, g);
         int first = 0;
         if (in) first = next[g];
         __syncwarp();
         if (in) {
             const int p = first + __popc(same & ((1u << lane) - 1u));
-            order[p] = static_cast<int>(i0 + lane);
-            if (!kSlots) position[i0 + lane] = g < groups ? p : -1;
+            order[p] = keys.value(i0 + lane);
+            if (Keys::kPlan) position[i0 + lane] = g < groups ? p : -1;
             if (lane == __ffs(same) - 1) next[g] = first + __popc(same);
         }
         __syncwarp();
@@ -103,8 +121,8 @@ __device__ __forceinline__ void cta_scan(int* v, int n, int* sums) {
 
 // Few pairs: one CTA does all three steps.
 constexpr int kSmallPlanThreads = 1024, kSmallPlanPairs = 8192;
-template <bool kSlots>
-__global__ void __launch_bounds__(kSmallPlanThreads) route_plan_small_kernel(const int* __restrict__ ids, int pairs, int groups, int warps_used,
+template <typename Keys>
+__global__ void __launch_bounds__(kSmallPlanThreads) route_plan_small_kernel(const Keys keys, int pairs, int groups, int warps_used,
                                                                              int* __restrict__ order, int* __restrict__ position,
                                                                              int* __restrict__ offsets) {
     extern __shared__ int route_smem[];
@@ -116,7 +134,7 @@ __global__ void __launch_bounds__(kSmallPlanThreads) route_plan_small_kernel(con
     __syncthreads();
     const int per = ((pairs + warps_used - 1) / warps_used + 31) & ~31;
     const int begin = min(pairs, warp * per), end = min(pairs, begin + per);
-    if (warp < warps_used) route_count<kSlots>(ids, begin, end, groups, hist + warp * bins);
+    if (warp < warps_used) route_count(keys, begin, end, groups, hist + warp * bins);
     __syncthreads();
     for (int g = threadIdx.x; g < bins; g += blockDim.x) {
         int run = 0;
@@ -126,17 +144,17 @@ __global__ void __launch_bounds__(kSmallPlanThreads) route_plan_small_kernel(con
     __syncthreads();
     cta_scan(total, bins, sums);
     for (int g = threadIdx.x; g < bins; g += blockDim.x) {
-        if (!kSlots) offsets[g] = total[g];     // bins = groups + 1 entries: the start of the empty slots is the end of the groups
+        if (Keys::kPlan) offsets[g] = total[g];     // bins = groups + 1 entries: the start of the empty slots is the end of the groups
         for (int w = 0; w < warps_used; ++w) hist[w * bins + g] += total[g];
     }
     __syncthreads();
-    if (warp < warps_used) route_place<kSlots>(ids, begin, end, groups, hist + warp * bins, order, position);
+    if (warp < warps_used) route_place(keys, begin, end, groups, hist + warp * bins, order, position);
 }
 
 // Many pairs: counts per chunk, a scan over the chunks of every group, then the ranks. chunk_hist is [bins][chunks].
 constexpr int kPlanWarps = 8, kPlanThreads = 32 * kPlanWarps, kPlanChunk = 2048;
-template <bool kSlots>
-__global__ void __launch_bounds__(kPlanThreads) route_count_kernel(const int* __restrict__ ids, long long pairs, int groups, int chunks,
+template <typename Keys>
+__global__ void __launch_bounds__(kPlanThreads) route_count_kernel(const Keys keys, long long pairs, int groups, int chunks,
                                                                    int* __restrict__ chunk_hist) {
     extern __shared__ int route_smem[];
     const int bins = groups + 1, warp = threadIdx.x >> 5;
@@ -144,7 +162,7 @@ __global__ void __launch_bounds__(kPlanThreads) route_count_kernel(const int* __
     __syncthreads();
     constexpr int per = kPlanChunk / kPlanWarps;
     const long long begin = min(pairs, static_cast<long long>(blockIdx.x) * kPlanChunk + warp * per), end = min(pairs, begin + per);
-    route_count<kSlots>(ids, begin, end, groups, route_smem + warp * bins);
+    route_count(keys, begin, end, groups, route_smem + warp * bins);
     __syncthreads();
     for (int g = threadIdx.x; g < bins; g += kPlanThreads) {
         int sum = 0;
@@ -171,8 +189,8 @@ __global__ void __launch_bounds__(256) route_scan_kernel(int bins, int chunks, i
     }
     if (lane == 0) total[g] = run;
 }
-template <bool kSlots>
-__global__ void __launch_bounds__(kPlanThreads) route_place_kernel(const int* __restrict__ ids, long long pairs, int groups, int chunks,
+template <typename Keys>
+__global__ void __launch_bounds__(kPlanThreads) route_place_kernel(const Keys keys, long long pairs, int groups, int chunks,
                                                                    const int* __restrict__ chunk_prefix, const int* __restrict__ total,
                                                                    int* __restrict__ order, int* __restrict__ position, int* __restrict__ offsets) {
     extern __shared__ int route_smem[];
@@ -186,15 +204,15 @@ __global__ void __launch_bounds__(kPlanThreads) route_place_kernel(const int* __
     cta_scan(start, bins, sums);
     constexpr int per = kPlanChunk / kPlanWarps;
     const long long begin = min(pairs, static_cast<long long>(blockIdx.x) * kPlanChunk + warp * per), end = min(pairs, begin + per);
-    route_count<kSlots>(ids, begin, end, groups, hist + warp * bins);
+    route_count(keys, begin, end, groups, hist + warp * bins);
     __syncthreads();
     for (int g = threadIdx.x; g < bins; g += kPlanThreads) {
-        if (!kSlots && blockIdx.x == 0) offsets[g] = start[g];
+        if (Keys::kPlan && blockIdx.x == 0) offsets[g] = start[g];
         int run = start[g] + chunk_prefix[static_cast<long long>(g) * chunks + blockIdx.x];
         for (int w = 0; w < kPlanWarps; ++w) { const int c = hist[w * bins + g]; hist[w * bins + g] = run; run += c; }
     }
     __syncthreads();
-    route_place<kSlots>(ids, begin, end, groups, hist + warp * bins, order, position);
+    route_place(keys, begin, end, groups, hist + warp * bins, order, position);
 }
 
 // Where group g begins among slot s's places (sorted positions, ascending; runs of num_rows): a warp each, cutting the run into 33 pieces per step.
@@ -418,8 +436,8 @@ size_t route_plan_bytes(long num_rows, int slots, int num_groups) {
 }
 
 namespace {
-template <bool kSlots>
-void counting_sort(const int* ids, long long pairs, int num_groups, int* order, int* position, int* offsets, void* workspace, cudaStream_t stream) {
+template <typename Keys>
+void counting_sort(const Keys& keys, long long pairs, int num_groups, int* order, int* position, int* offsets, void* workspace, cudaStream_t stream) {
     const int bins = num_groups + 1;
     if (pairs <= kSmallPlanPairs) {
         // a warp for every 32 pairs, as far as their counters fit into 128 KB
@@ -429,11 +447,11 @@ void counting_sort(const int* ids, long long pairs, int num_groups, int* order, 
         static std::atomic<bool> done[64];
         // beyond 48 KB a launch has to be allowed, and the kernel's own arrays (the sums of its scan) count too
         if (smem > 47 * 1024 && first_on_device(done)) {
-            SMX_CUDA(cudaFuncSetAttribute(route_plan_small_kernel<kSlots>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+            SMX_CUDA(cudaFuncSetAttribute(route_plan_small_kernel<Keys>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
             mark_on_device(done);
         }
         const int threads = std::max(128, 32 * warps);
-        route_plan_small_kernel<kSlots><<<1, threads, smem, stream>>>(ids, static_cast<int>(pairs), num_groups, warps, order, position, offsets);
+        route_plan_small_kernel<Keys><<<1, threads, smem, stream>>>(keys, static_cast<int>(pairs), num_groups, warps, order, position, offsets);
         launched("route_plan_small_kernel");
         return;
     }
@@ -441,11 +459,11 @@ void counting_sort(const int* ids, long long pairs, int num_groups, int* order, 
     int* hist = static_cast<int*>(workspace);
     int* total = hist + static_cast<size_t>(bins) * chunks;
     const int smem = kPlanWarps * bins * static_cast<int>(sizeof(int));
-    route_count_kernel<kSlots><<<chunks, kPlanThreads, smem, stream>>>(ids, pairs, num_groups, chunks, hist);
+    route_count_kernel<Keys><<<chunks, kPlanThreads, smem, stream>>>(keys, pairs, num_groups, chunks, hist);
     launched("route_count_kernel");
     route_scan_kernel<<<(bins * 32 + 255) / 256, 256, 0, stream>>>(bins, chunks, hist, total);
     launched("route_scan_kernel");
-    route_place_kernel<kSlots><<<chunks, kPlanThreads, smem + (bins + 1) * static_cast<int>(sizeof(int)), stream>>>(ids, pairs, num_groups, chunks, hist, total,
+    route_place_kernel<Keys><<<chunks, kPlanThreads, smem + (bins + 1) * static_cast<int>(sizeof(int)), stream>>>(keys, pairs, num_groups, chunks, hist, total,
                                                                                                                    order, position, offsets);
     launched("route_place_kernel");
 }
@@ -458,16 +476,34 @@ void route_plan(const int* ids, long num_rows, int slots, int num_groups, int* o
     const long long pairs = static_cast<long long>(num_rows) * slots;
     if (!offsets || (pairs > 0 && (!ids || !order || !position))) throw ArgError("smx_route_plan: null pointer");
     if (workspace_bytes < need || (need && !workspace)) throw ArgError("smx_route_plan: the workspace is smaller than smx_route_plan_bytes says");
-    counting_sort<false>(ids, pairs, num_groups, order, position, offsets, workspace, stream);
+    counting_sort(GroupKeys{ids, num_groups}, pairs, num_groups, order, position, offsets, workspace, stream);
 }
 
 size_t route_slots_bytes(long num_rows, int slots) { return route_plan_bytes(num_rows * slots, 1, slots); }
 void route_slots(const int* order, long num_rows, int slots, const int* offsets, int num_groups, int* places, int* slot_offsets, void* workspace,
                  cudaStream_t stream) {
-    counting_sort<true>(order, static_cast<long long>(num_rows) * slots, slots, places, nullptr, nullptr, workspace, stream);
+    counting_sort(SlotKeys{order, slots}, static_cast<long long>(num_rows) * slots, slots, places, nullptr, nullptr, workspace, stream);
     const int n = slots * (num_groups + 1);
     route_slot_offsets_kernel<<<(n + 7) / 8, 256, 0, stream>>>(places, static_cast<int>(num_rows), slots, offsets, num_groups, slot_offsets);
     launched("route_slot_offsets_kernel");
+}
+
+// Tokens have up to 21 bits (the number of rows itself stands for pairs without a token): one digit, or two of half of them.
+size_t token_sort_bytes(long pairs, int table_rows) {
+    const size_t sort = route_plan_bytes(pairs, 1, std::min(table_rows + 1, kMaxGroups));
+    return table_rows < kMaxGroups ? sort : (sort + 255) / 256 * 256 + static_cast<size_t>(pairs) * sizeof(int);
+}
+void token_sort(const int* ids, long pairs, int table_rows, int* order, void* workspace, cudaStream_t stream) {
+    if (table_rows < kMaxGroups) {
+        counting_sort(DigitKeys{ids, table_rows, nullptr, 0, 0x7fffffff}, pairs, table_rows + 1, order, nullptr, nullptr, workspace, stream);
+        return;
+    }
+    int bits = 1;
+    while ((table_rows >> bits) >= (1 << bits)) ++bits;
+    const size_t sort = route_plan_bytes(pairs, 1, kMaxGroups);
+    int* half = reinterpret_cast<int*>(static_cast<char*>(workspace) + (sort + 255) / 256 * 256);
+    counting_sort(DigitKeys{ids, table_rows, nullptr, 0, (1 << bits) - 1}, pairs, 1 << bits, half, nullptr, nullptr, workspace, stream);
+    counting_sort(DigitKeys{ids, table_rows, half, bits, 0x7fffffff}, pairs, (table_rows >> bits) + 1, order, nullptr, nullptr, workspace, stream);
 }
 
 template <typename T>
