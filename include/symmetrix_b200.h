@@ -397,7 +397,7 @@ int smx_adapter_backward(const smx_adapter_linear* call, char* errbuf, int errbu
  * smx_grouped_backward writes, each unless NULL, grad_x and the degrees' grad_weight (for all degrees or none; groups without rows get
  * zeros). Rows behind the last group are never read; in `y` they are left as they were, or zeroed with `zero_tail` != 0, in grad_x they are zeroed.
  * The matrices are read as they are, in every call: changed values count at once. Sums, float32 operands, NaN, infinities, waits inside the float32 kernels,
- * `status`, streams, workspaces (smx_grouped_workspace_bytes) and limits: as for smx_adapter_*. Outputs must not overlap inputs or one another. */
+ * `status`, streams, workspaces (smx_grouped_workspace_bytes; it starts on a 32-byte boundary) and limits: as for smx_adapter_*. Outputs must not overlap inputs or one another. */
 enum { SMX_GROUPED_MAX_DEGREES = 8 };
 typedef struct smx_grouped_degree {
     int components, in_channels, out_channels;
@@ -416,6 +416,7 @@ typedef struct smx_grouped_linear {
     void* workspace;    long workspace_bytes;
     void* stream;
     int* status;                             /* NULL, or an int that the caller has zeroed */
+    int expire_polls;                        /* test switch: > 0 makes waits inside the float32 kernels run out after so many polls; leave it 0 */
 } smx_grouped_linear;
 long smx_grouped_workspace_bytes(const smx_grouped_linear* call, int backward);
 int smx_grouped_forward(const smx_grouped_linear* call, char* errbuf, int errbuf_len);

@@ -72,7 +72,8 @@ class GroupedCall(ctypes.Structure):
                 ("num_rows", ctypes.c_long), ("degrees", GroupedDegree * GROUPED_MAX_DEGREES), ("offsets", ctypes.c_void_p),
                 ("x", ctypes.c_void_p), ("x_stride", ctypes.c_long), ("y", ctypes.c_void_p), ("y_stride", ctypes.c_long),
                 ("grad_y", ctypes.c_void_p), ("grad_y_stride", ctypes.c_long), ("grad_x", ctypes.c_void_p), ("grad_x_stride", ctypes.c_long),
-                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_long), ("stream", ctypes.c_void_p), ("status", ctypes.c_void_p)]
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_long), ("stream", ctypes.c_void_p), ("status", ctypes.c_void_p),
+                ("expire_polls", ctypes.c_int)]
 
 
 class Gradient(ctypes.Structure):

@@ -8,6 +8,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <climits>
 #include <cstdint>
 
@@ -132,6 +133,14 @@ __global__ void __launch_bounds__(256) grouped_grad_kernel(const __grid_constant
     }
 }
 
+}  // namespace
+}  // namespace smx
+
+#include "grouped_f32.cuh"
+
+namespace smx {
+namespace {
+
 // ------------------------------------------------------------------------------------------- host side
 void launched(const char* what) {
     const cudaError_t e = cudaGetLastError();
@@ -162,6 +171,7 @@ void check_call(const smx_grouped_linear& c) {
 void check_plan(const smx_grouped_linear& c) {
     check_call(c);
     if (!c.offsets) throw ArgError("smx_grouped: null plan");
+    if (reinterpret_cast<uintptr_t>(c.workspace) & 31) throw ArgError("smx_grouped: the workspace must start on a 32-byte boundary");
     check_pointers("smx_grouped", sizeof(int), {c.offsets, c.status});
     const size_t value = c.precision == SMX_FP32 ? sizeof(float) : sizeof(double);
     check_pointers("smx_grouped", value, {c.x, c.y, c.grad_y, c.grad_x});
@@ -176,9 +186,112 @@ void check_weights(const smx_grouped_linear& c) {
         if (!c.degrees[d].weight) throw ArgError("smx_grouped: null weight");
 }
 
+// What a call allocates nothing for: the partial sums of the matrices' gradients. Their chunks of rows are as long as leaves four tiles for each of 148
+// SMs (a constant, so that sizes and sums do not depend on the device); a group with several chunks has less than twice as many as its rows fill.
+int grad_chunk(const smx_grouped_linear& c) {
+    long long steps = 0;
+    for (int d = 0; d < c.num_degrees; ++d) {
+        const smx_grouped_degree& g = c.degrees[d];
+        steps += (c.num_rows * static_cast<long long>(g.components) + 31) / 32 * ((g.in_channels + 127) / 128) * ((g.out_channels + 127) / 128);
+    }
+    return 32 * static_cast<int>(std::max(4LL, std::min(128LL, (steps + 591) / 592)));
+}
+size_t part_values(const smx_grouped_linear& c, int d) {
+    const smx_grouped_degree& g = c.degrees[d];
+    const long long parts = 2 * (c.num_rows * static_cast<long long>(g.components) / grad_chunk(c));
+    return static_cast<size_t>((parts * g.in_channels * g.out_channels + 63) / 64 * 64);
+}
+
+template <int kMode, bool kWide>
+void launch_gs(const GsPass& p, long long tiles, cudaStream_t stream) {
+    const auto kernel = grouped_f32_kernel<kMode, kWide>;
+    // the warps' shares of registers are drawn from what the launch gives: fewer than planned and they would wait for ever
+    static std::atomic<bool> done[64];
+    if (first_on_device(done)) {
+        cudaFuncAttributes a{};
+        SMX_CUDA(cudaFuncGetAttributes(&a, kernel));
+        if (a.numRegs < kGsRegsLaunch) throw CudaError("grouped_f32_kernel was built with too few registers");
+        SMX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, GsLayout<kMode, kWide>::smem));
+        mark_on_device(done);
+    }
+    kernel<<<static_cast<unsigned>(std::min<long long>(tiles, sm_count())), kGsThreads, GsLayout<kMode, kWide>::smem, stream>>>(p);
+    launched("grouped_f32_kernel");
+}
+
+GsPass gs_pass(const smx_grouped_linear& c, bool transposed) {
+    GsPass p{};
+    long long in_off = 0, out_off = 0;
+    for (int q = 0; q < c.num_degrees; ++q) {
+        const smx_grouped_degree& g = c.degrees[q];
+        GsDegree& d = p.degree[q];
+        d.comps = g.components;
+        d.K = transposed ? g.out_channels : g.in_channels;
+        d.N = transposed ? g.in_channels : g.out_channels;
+        d.a_off = in_off; d.b_off = out_off;
+        d.w = static_cast<const float*>(g.weight);
+        in_off += static_cast<long long>(d.comps) * d.K;
+        out_off += static_cast<long long>(d.comps) * d.N;
+    }
+    p.degrees = c.num_degrees; p.groups = c.num_groups; p.rows = c.num_rows; p.offsets = c.offsets;
+    p.out_width = static_cast<int>(out_off);
+    p.status = c.status; p.expire_polls = c.expire_polls;
+    return p;
+}
+
+void rows_f32(const smx_grouped_linear& c, bool transposed) {
+    GsPass p = gs_pass(c, transposed);
+    p.a = static_cast<const float*>(transposed ? c.grad_y : c.x); p.a_stride = transposed ? c.grad_y_stride : c.x_stride;
+    p.out = static_cast<float*>(transposed ? c.grad_x : c.y); p.out_stride = transposed ? c.grad_x_stride : c.y_stride;
+    p.zero_tail = transposed || c.zero_tail;
+    long long tiles = 0;
+    bool wide = ((static_cast<unsigned long long>(p.out_stride) * 4u | reinterpret_cast<uintptr_t>(p.out)) & 31) == 0;
+    for (int q = 0; q < p.degrees; ++q) {
+        const GsDegree& d = p.degree[q];
+        tiles += (c.num_rows * d.comps / 128 + c.num_groups) * ((d.N + 127) / 128);
+        wide = wide && d.b_off % 8 == 0 && d.N % 64 == 0;
+    }
+    if (tiles > INT_MAX) throw ArgError("smx_grouped: too many rows");
+    const cudaStream_t stream = static_cast<cudaStream_t>(c.stream);
+    if (transposed) {
+        if (wide) launch_gs<kGsBackward, true>(p, tiles, stream);
+        else launch_gs<kGsBackward, false>(p, tiles, stream);
+    } else {
+        if (wide) launch_gs<kGsForward, true>(p, tiles, stream);
+        else launch_gs<kGsForward, false>(p, tiles, stream);
+    }
+}
+
+void gradient_f32(const smx_grouped_linear& c) {
+    GsPass p = gs_pass(c, false);
+    p.a = static_cast<const float*>(c.x); p.a_stride = c.x_stride;
+    p.b = static_cast<const float*>(c.grad_y); p.b_stride = c.grad_y_stride;
+    p.chunk = grad_chunk(c);
+    float* part = static_cast<float*>(c.workspace);
+    long long tiles = 0, most = 0;
+    bool wide = true, split = false;
+    for (int q = 0; q < p.degrees; ++q) {
+        GsDegree& d = p.degree[q];
+        d.grad = static_cast<float*>(c.degrees[q].grad_weight);
+        d.part = part;
+        part += part_values(c, q);
+        split = split || part_values(c, q) > 0;
+        tiles += (c.num_rows * d.comps / p.chunk + c.num_groups) * ((d.N + 127) / 128) * ((d.K + 127) / 128);
+        most = std::max(most, static_cast<long long>(d.K) * d.N);
+        wide = wide && d.N % 64 == 0 && (reinterpret_cast<uintptr_t>(d.grad) & 31) == 0;
+    }
+    if (tiles > INT_MAX) throw ArgError("smx_grouped: too many rows");
+    const cudaStream_t stream = static_cast<cudaStream_t>(c.stream);
+    if (wide) launch_gs<kGsGradient, true>(p, tiles, stream);
+    else launch_gs<kGsGradient, false>(p, tiles, stream);
+    if (!split) return;
+    grouped_join_kernel<<<dim3(c.num_groups, static_cast<unsigned>(std::min(64LL, (most + 255) / 256)), c.num_degrees), 256, 0, stream>>>(p);
+    launched("grouped_join_kernel");
+}
+
 template <typename T>
 void rows_pass(const smx_grouped_linear& c, bool transposed) {
     if (c.num_rows == 0) return;
+    if (sizeof(T) == 4) return rows_f32(c, transposed);
     RowsPass<T> p{};
     long long in_off = 0, out_off = 0, tiles = 0;
     for (int q = 0; q < c.num_degrees; ++q) {
@@ -230,8 +343,14 @@ void backward(const smx_grouped_linear& c) {
         check_weights(c);
     }
     if (matrices) check_rows("x", c.x, c.x_stride, w.in, c.num_rows, false);
+    if (matrices) {
+        const size_t need = grouped_workspace_bytes(c, true);
+        if (c.workspace_bytes < 0 || static_cast<size_t>(c.workspace_bytes) < need || (need && !c.workspace))
+            throw ArgError("smx_grouped_backward: the workspace is smaller than smx_grouped_workspace_bytes says");
+    }
     if (c.grad_x) rows_pass<T>(c, true);
     if (!matrices) return;
+    if (sizeof(T) == 4) return gradient_f32(c);
     GradPass<T> p{};
     long long x_off = 0, y_off = 0;
     for (int q = 0; q < c.num_degrees; ++q) {
@@ -250,9 +369,12 @@ void backward(const smx_grouped_linear& c) {
 
 }  // namespace
 
-size_t grouped_workspace_bytes(const smx_grouped_linear& c, bool) {
+size_t grouped_workspace_bytes(const smx_grouped_linear& c, bool backward) {
     check_call(c);
-    return 0;
+    if (!backward || c.precision == SMX_FP64) return 0;
+    size_t values = 0;
+    for (int d = 0; d < c.num_degrees; ++d) values += part_values(c, d);
+    return values * sizeof(float);
 }
 void grouped_forward(const smx_grouped_linear& c) {
     check_plan(c);

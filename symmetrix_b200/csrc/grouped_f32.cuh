@@ -1,0 +1,745 @@
+// float32 kernel of the linears of routed rows on the 5th-generation tensor cores (tcgen05.mma kind::tf32), included by grouped.cu.
+//
+// One kernel makes all three products, as D [128 rows x 128 columns] += A [128 x inner] B [inner x 128]:
+//   forward    D = rows of y        A = rows of x                 B = W_g
+//   backward   D = rows of grad_x   A = rows of grad_y            B = W_g^T
+//   gradient   D = rows of grad_W   A = x^T (inner: rows)         B = grad_y (inner: rows)
+// float32 accuracy comes from operands v = hi + lo of 11 bits each: lo hi + hi lo + hi hi per product (3xTF32). Both operands are read as they are and
+// split on their way: A, a thread per row, to tensor memory; B, a thread per column, to shared memory in the layout of the instruction. There is
+// no prepared copy of the matrices: training changes them in every step, and few rows per group read them once.
+#pragma once
+
+#include "tcgen05_ops.cuh"
+
+namespace smx {
+namespace {
+
+enum GsMode { kGsForward, kGsBackward, kGsGradient };
+constexpr int kGsThreads = 640, kGsChunk = 32, kGsStages = 4, kGsRing = 6;   // inner values of a step; stages of A and of B; tiles in the ring
+constexpr int kGsTileBytes = 128 * kGsChunk * 4, kGsPitch = kGsChunk + 4, kGsOutPitch = 17;
+constexpr int kGsStatusWait = 8;
+// the warps' shares of the registers, by fours: control, A, sums twice, B
+constexpr int kGsRegsLaunch = 96, kGsRegsControl = 48, kGsRegsOperand = 104, kGsRegsSums = 112;
+static_assert(kGsRegsControl + 2 * kGsRegsOperand + 2 * kGsRegsSums <= 5 * kGsRegsLaunch, "the registers of the launch are shared out");
+
+struct GsDegree {
+    int comps, K, N;                 // rows passes: inner values and columns; gradient: rows and columns of the matrices
+    long long a_off, b_off;          // of `a`; of `out`, or in the gradient of `b`
+    const float* w;                  // the matrices
+    float* grad; float* part;        // gradient: the result, and partial sums of groups with several chunks of rows
+};
+struct GsPass {
+    GsDegree degree[SMX_GROUPED_MAX_DEGREES];
+    int degrees, groups, zero_tail, out_width;
+    int chunk;                       // gradient: rows of a tile's sum, a multiple of 32
+    long long rows;
+    const int* offsets;
+    const float* a; long long a_stride;
+    const float* b; long long b_stride;
+    float* out; long long out_stride;
+    int* status;                     // null, or receives kGsStatusWait if a wait runs out
+    int expire_polls;                // test switch, zero in normal operation: every CTA loses its B behind the first chunk and gives up after this many polls
+};
+// A tile of D. `fresh`: its B is not the one before's; `last`: the next tile's is another one.
+struct GsWork {
+    int found, degree, tile, group, block, mtile, rows, inner, chunks, fresh, last, first_pair;
+    long long row0;
+    float* out;                      // gradient
+};
+
+template <int kMode>
+__device__ __forceinline__ bool gs_resident(const GsDegree& d) { return kMode != kGsGradient && d.K <= kGsChunk * kGsStages; }
+template <int kMode>
+__device__ __forceinline__ int gs_plane(const GsDegree& d) {             // tiles of a group's D that share its rows
+    const int blocks = (d.N + 127) / 128;
+    return kMode == kGsGradient ? blocks * ((d.K + 127) / 128) : blocks;
+}
+template <int kMode>
+__device__ __forceinline__ int gs_runs(const GsPass& p, const GsDegree& d, long long count) {        // row tiles of a group, or chunks of its rows
+    const long long rows = count * d.comps;
+    if (kMode == kGsGradient) return max(1, static_cast<int>((rows + p.chunk - 1) / p.chunk));          // a group without rows gets its zeros
+    return static_cast<int>((rows + 127) / 128);
+}
+
+// The CTA's tiles, the same share of all steps for each: lane q holds begin and end among the tiles of degree q. Called by a warp.
+template <int kMode>
+__device__ __forceinline__ void gs_share(const GsPass& p, int& begin, int& end) {
+    const int lane = threadIdx.x & 31;
+    long long total = 0, before = 0;
+    int mine = 0;
+    auto cost_of = [&](const GsDegree& d) { return (kMode == kGsGradient ? p.chunk / kGsChunk : (d.K + kGsChunk - 1) / kGsChunk) + 2; };
+    for (int q = 0; q < p.degrees; ++q) {
+        const GsDegree& d = p.degree[q];
+        int n = 0;
+        for (int g = lane; g < p.groups; g += 32) n += gs_runs<kMode>(p, d, p.offsets[g + 1] - p.offsets[g]);
+        n = __reduce_add_sync(0xffffffffu, n) * gs_plane<kMode>(d);
+        if (lane == q) { mine = n; before = total; }
+        total += static_cast<long long>(n) * cost_of(d);
+    }
+    begin = end = 0;
+    if (lane < p.degrees) {
+        const long long cost = cost_of(p.degree[lane]);
+        auto cut = [&](long long at) { return static_cast<int>(min(static_cast<long long>(mine), max(0LL, (at - before + cost - 1) / cost))); };
+        begin = cut(total * blockIdx.x / gridDim.x);
+        end = cut(total * (blockIdx.x + 1) / gridDim.x);
+    }
+}
+
+// Finds the tiles of a degree in ascending order: groups, then where a tile's B stays for the next ones column blocks and row tiles, else row tiles and
+// column blocks (neighbours then read the same rows).
+struct GsCursor {
+    int q = -1, g0 = 0, run = 0, parts = 0;          // tiles and partial sums of the groups before g0
+    template <int kMode>
+    __device__ __forceinline__ bool find(const GsPass& p, int degree, int t, GsWork& w) {
+        const int lane = threadIdx.x & 31;
+        if (degree != q) { q = degree; g0 = run = parts = 0; }
+        const GsDegree& d = p.degree[q];
+        const int plane = gs_plane<kMode>(d), blocks = (d.N + 127) / 128;
+        for (; g0 < p.groups; g0 += 32) {
+            const int g = g0 + lane;
+            int first = 0, count = 0, runs = 0;
+            if (g < p.groups) {
+                first = p.offsets[g];
+                count = p.offsets[g + 1] - first;
+                runs = gs_runs<kMode>(p, d, count);
+            }
+            const int split = kMode == kGsGradient && runs > 1 ? runs : 0;
+            int incl = runs * plane, incl_parts = split;
+#pragma unroll
+            for (int s = 1; s < 32; s <<= 1) {
+                const int up = __shfl_up_sync(0xffffffffu, incl, s), up_parts = __shfl_up_sync(0xffffffffu, incl_parts, s);
+                if (lane >= s) { incl += up; incl_parts += up_parts; }
+            }
+            const int begin = run + incl - runs * plane;
+            const unsigned hit = __ballot_sync(0xffffffffu, t >= begin && t < run + incl);
+            if (hit) {
+                const int src = __ffs(hit) - 1;
+                const int local = t - __shfl_sync(0xffffffffu, begin, src);
+                runs = __shfl_sync(0xffffffffu, runs, src);
+                count = __shfl_sync(0xffffffffu, count, src);
+                const long long rows = static_cast<long long>(count) * d.comps;
+                w.found = 1; w.degree = q; w.tile = t; w.group = g0 + src;
+                w.first_pair = __shfl_sync(0xffffffffu, first, src);
+                w.fresh = w.last = 1;
+                if (kMode == kGsGradient) {
+                    const int at = local / plane, in_plane = local - at * plane;
+                    w.mtile = in_plane / blocks;
+                    w.block = in_plane - w.mtile * blocks;
+                    w.row0 = static_cast<long long>(at) * p.chunk;
+                    w.rows = min(128, d.K - 128 * w.mtile);
+                    w.inner = static_cast<int>(min(static_cast<long long>(p.chunk), rows - w.row0));
+                    const long long part = parts + __shfl_sync(0xffffffffu, incl_parts - split, src) + at;
+                    float* to = runs == 1 ? d.grad + static_cast<long long>(w.group) * d.K * d.N : d.part + part * d.K * d.N;
+                    w.out = to + 128LL * w.mtile * d.N + 128 * w.block;
+                } else {
+                    int at;
+                    if (gs_resident<kMode>(d)) {
+                        w.block = local / runs;
+                        at = local - w.block * runs;
+                        w.last = at + 1 == runs;
+                    } else {
+                        at = local / blocks;
+                        w.block = local - at * blocks;
+                    }
+                    w.mtile = 0;
+                    w.row0 = static_cast<long long>(at) * 128;
+                    w.rows = static_cast<int>(min(128LL, rows - w.row0));
+                    w.inner = d.K;
+                }
+                w.chunks = (w.inner + kGsChunk - 1) / kGsChunk;
+                return true;
+            }
+            run += __shfl_sync(0xffffffffu, incl, 31);
+            parts += __shfl_sync(0xffffffffu, incl_parts, 31);
+        }
+        w.found = 0;
+        return false;
+    }
+};
+
+// Where row i of D of a rows pass is: the row of the arrays (a pair of the plan) and its component.
+__device__ __forceinline__ void gs_row(const GsWork& w, int comps, int i, int& pair, int& comp) {
+    const long long r = w.row0 + i;
+    const long long ahead = r < (1LL << 31) ? static_cast<int>(r) / comps : r / comps;
+    pair = w.first_pair + static_cast<int>(ahead);
+    comp = static_cast<int>(r - ahead * comps);
+}
+
+// NaN into a warp's part of a tile, 32 rows of 64 columns.
+template <int kMode>
+__device__ __forceinline__ void gs_lose(const GsPass& p, const GsWork& w, int row0, int col0) {
+    const GsDegree& d = p.degree[w.degree];
+    const int cols = min(col0 + 64, d.N - 128 * w.block);
+    for (int i = row0; i < min(row0 + 32, w.rows); ++i) {
+        float* to = w.out + static_cast<long long>(i) * d.N;
+        if (kMode != kGsGradient) {
+            int pair, comp;
+            gs_row(w, d.comps, i, pair, comp);
+            to = p.out + pair * p.out_stride + d.b_off + static_cast<long long>(comp) * d.N + 128 * w.block;
+        }
+        for (int c = col0 + (threadIdx.x & 31); c < cols; c += 32) to[c] = NAN;
+    }
+}
+
+// hi of 11 bits, rounded; lo cut to 11 bits: the bits of its tail are the only loss, 2^-23 of the value at most. NaN stays NaN in one of the two, an
+// infinity leaves a NaN in lo.
+__device__ __forceinline__ void gs_split(float v, float& hi, float& lo) {
+    hi = ts_round(v);
+    lo = __uint_as_float(__float_as_uint(v - hi) & kTc5HiMask);
+}
+
+__device__ __forceinline__ void gs_meet() {
+    __syncwarp();
+    ts_fence_before();
+    asm volatile("bar.sync 1, 640;" ::: "memory");
+}
+
+// kWide: every row's half of a tile of the output starts on 32 bytes and is 64 columns long.
+template <int kMode, bool kWide>
+struct GsLayout {
+    static constexpr int row_stages = kMode == kGsGradient ? 0 : kWide ? 5 : 4;      // raw rows on their way to tensor memory
+    static_assert(kGsRing > row_stages, "the rows' copies run row_stages - 1 tiles ahead of the tile that is given back last");
+    static constexpr int row_floats = 128 * kGsPitch;
+    static constexpr int smem = kGsStages * 2 * kGsTileBytes + (row_stages * row_floats + (kWide ? 0 : 8 * 32 * kGsOutPitch)) * 4 + 1024;
+    static_assert(smem + 8192 <= 227 * 1024, "shared memory of one CTA per SM");
+};
+
+// One persistent CTA per SM walks its share of the tiles; its warps are specialised, so that the parts of neighbouring tiles overlap:
+//   warp 0       the products (one thread)
+//   warp 1       finds the tiles (a ring, ahead of all others)
+//   warps 2, 3   zeros into the rows behind the last group
+//   warps 4-7    A. Rows passes: a warp copies 32 values of each of its 32 rows asynchronously, row_stages - 1 chunks ahead; a thread splits those of its row
+//                and stores them to tensor memory. Gradient: a thread owns a column of x and reads it row by row, next chunk's values in registers.
+//   warps 8-15   a thread adds half of its row's partial sums of every 64 inner values in registers (the tensor core cuts its sums instead of rounding
+//                them: one sum over 128 inner values is off five times as far as float32) and writes its half of the row
+//   warps 16-19  B, next chunk's values in registers; where a matrix has up to 128 inner values it stays for all row tiles of its group
+// TMEM: two partial sums of 128 columns, taken in turn, and four stages of A of 64 (hi, lo).
+// Every wait is bounded; if one runs out, the CTA gives up, fills its remaining tiles with NaN, reports it to `status` and ends when its products
+// and copies in flight have.
+template <int kMode, bool kWide>
+__global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid_constant__ GsPass pass) {
+    using L = GsLayout<kMode, kWide>;
+    constexpr int RS = L::row_stages;
+    extern __shared__ unsigned char gs_smem_raw[];
+    __shared__ __align__(8) unsigned long long work_full[kGsRing], work_free[kGsRing], a_full[kGsStages], a_free[kGsStages], b_full[kGsStages], b_free[kGsStages],
+        d_full[2], d_free[2], drained;
+    __shared__ GsWork work[kGsRing];
+    __shared__ int work_pair[kMode == kGsGradient ? 1 : kGsRing][128];
+    __shared__ short work_comp[kMode == kGsGradient ? 1 : kGsRing][128];
+    __shared__ __align__(16) long long row_at[kMode == kGsGradient ? 8 : 1][32];         // gradient: where a chunk's rows start, for every operand warp
+    __shared__ uint32_t tmem_slot;
+    __shared__ int guard[2];                                                             // a wait ran out; polls of a wait
+    const int warp = ts_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+    unsigned char* const stages = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(gs_smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    float* const row_stages = reinterpret_cast<float*>(stages + kGsStages * 2 * kGsTileBytes);
+    if (threadIdx.x == 0) {
+        guard[0] = 0;
+        guard[1] = pass.expire_polls > 0 ? pass.expire_polls : static_cast<int>(kMbarSpinLimit);
+        for (int q = 0; q < kGsRing; ++q) { mbar_init(&work_full[q], 1); mbar_init(&work_free[q], 17); }
+        for (int q = 0; q < kGsStages; ++q) { mbar_init(&a_full[q], 4); mbar_init(&a_free[q], 1); mbar_init(&b_full[q], 4); mbar_init(&b_free[q], 1); }
+        for (int q = 0; q < 2; ++q) { mbar_init(&d_full[q], 1); mbar_init(&d_free[q], 8); }
+        mbar_init(&drained, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    ts_fence_before();
+    __syncthreads();
+    ts_fence_after();
+    const uint32_t tmem = tmem_slot, a_at = tmem + 256;
+
+    if (warp < 4) {
+        ts_registers_less<kGsRegsControl>();
+        if (warp == 0) {
+            int na = 0, nb = 0, nd = 0, base_b = 0;                  // stages of A and B used so far, partial sums; B's stages of the tile
+            bool ok = true;
+            const bool leader = ts_elect();
+            const uint32_t b_at = smem_u32(stages);
+            for (int i = 0; ok; ++i) {
+                const int slot = i % kGsRing;
+                ok = ts_wait_warp(&work_full[slot], (i / kGsRing) & 1, guard);
+                if (!ok) break;
+                const GsWork& w = work[slot];
+                const int found = ts_uniform(w.found), chunks = ts_uniform(w.chunks), fresh = ts_uniform(w.fresh), last = ts_uniform(w.last), inner = ts_uniform(w.inner);
+                const int cols = found ? ts_uniform(min(128, (pass.degree[w.degree].N - 128 * w.block + 15) & ~15)) : 0;
+                __syncwarp();
+                if (leader) mbar_arrive(&work_free[slot]);
+                if (!found) break;
+                if (fresh) { base_b = nb; nb += chunks; }
+#pragma unroll 1
+                for (int j = 0; j < chunks; ++j) {
+                    const int st = na % kGsStages, n = base_b + j, bs = n % kGsStages, sum = nd & 1;
+                    if ((j & 1) == 0 && nd >= 2) ok = ts_wait_warp(&d_free[sum], ((nd >> 1) - 1) & 1, guard);
+                    ok = ok && ts_wait_warp(&a_full[st], (na / kGsStages) & 1, guard);
+                    if (fresh) ok = ok && ts_wait_warp(&b_full[bs], (n / kGsStages) & 1, guard);
+                    if (!ok) break;
+                    ts_fence_after();
+                    const uint32_t hi = ts_uniform(a_at + 64 * st), b = ts_uniform(b_at + bs * 2 * kGsTileBytes), d = ts_uniform(tmem + 128 * sum);
+                    const bool ends = (j & 1) != 0 || j + 1 == chunks;
+                    if (leader) {
+                        ts_chunk(d, hi, hi + 32, b, b + kGsTileBytes, ts_idesc(cols), min(4, (inner - kGsChunk * j + 7) / 8), (j & 1) != 0);
+                        ts_commit(&a_free[st]);
+                        if (last) ts_commit(&b_free[bs]);
+                        if (ends) ts_commit(&d_full[sum]);
+                    }
+                    __syncwarp();
+                    ++na;
+                    if (ends) ++nd;
+                }
+            }
+        } else if (warp == 1) {
+            GsCursor cursor;
+            int begin, end, i = 0, last_degree = -1, last_group = 0, last_block = 0;
+            gs_share<kMode>(pass, begin, end);
+            bool ok = true;
+            for (int q = 0; q <= pass.degrees && ok; ++q) {
+                const int t0 = q < pass.degrees ? __shfl_sync(0xffffffffu, begin, q) : 0, t1 = q < pass.degrees ? __shfl_sync(0xffffffffu, end, q) : 1;
+                for (int t = t0; t < t1 && ok; ++t, ++i) {
+                    const int slot = i % kGsRing;
+                    GsWork w{};
+                    if (q < pass.degrees) {
+                        cursor.find<kMode>(pass, q, t, w);
+                        if (gs_resident<kMode>(pass.degree[q])) {
+                            w.fresh = w.degree != last_degree || w.group != last_group || w.block != last_block;
+                            w.last = w.last || t + 1 == t1;
+                        }
+                        last_degree = w.degree; last_group = w.group; last_block = w.block;
+                    }
+                    if (i >= kGsRing && !ts_wait_warp(&work_free[slot], (i / kGsRing - 1) & 1, guard)) { ok = false; break; }
+                    if (kMode != kGsGradient && w.found)
+#pragma unroll 1
+                        for (int at = lane; at < 128; at += 32) {
+                            int pair = w.first_pair, comp = 0;
+                            if (at < w.rows) gs_row(w, pass.degree[q].comps, at, pair, comp);
+                            work_pair[slot][at] = pair;
+                            work_comp[slot][at] = static_cast<short>(comp);
+                        }
+                    if (lane == 0) work[slot] = w;
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&work_full[slot]);
+                }
+            }
+        } else if (kMode != kGsGradient && pass.zero_tail) {
+            for (long long p = pass.offsets[pass.groups] + 2LL * blockIdx.x + (warp - 2); p < pass.rows; p += 2LL * gridDim.x)
+                for (int c = lane; c < pass.out_width; c += 32) pass.out[p * pass.out_stride + c] = 0.f;
+        }
+        gs_meet();
+        if (guard[0] && warp == 0) {
+            // what was started ends before the CTA does: products read its shared and tensor memory
+            if (ts_elect()) ts_commit(&drained);
+            __syncwarp();
+            mbar_wait(&drained, 0);
+            if (lane == 0 && pass.status) atomicMax(pass.status, kGsStatusWait);
+        }
+    } else if (warp < 8) {
+        ts_registers_more<kGsRegsOperand>();
+        const uint32_t lanes = a_at + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+        const int tid = threadIdx.x & 127, first = tid & ~31;            // the warp's rows are its own: no barrier but the work's
+        int na = 0;
+        bool ok = true;
+        auto free_stage = [&]() { return na < kGsStages || ts_wait_warp(&a_free[na % kGsStages], (na / kGsStages - 1) & 1, guard); };
+        auto give = [&]() {
+            ts_wait_store();
+            ts_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&a_full[na % kGsStages]);
+            ++na;
+        };
+        auto put16 = [&](int q, float (&v)[16]) {
+            float hi[16];
+            const uint32_t to = lanes + 64 * (na % kGsStages) + q;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) { float lo; gs_split(v[e], hi[e], lo); v[e] = lo; }
+            ts_store16(to, hi);
+            ts_store16(to + 32, v);
+        };
+        if constexpr (kMode != kGsGradient) {
+            float* const rows_at = row_stages + first * kGsPitch;
+            int xs = 0, ahead_tile = 0, ahead = 0, ahead_chunks = 0, ahead_K = 0, ahead_rows = 0, ahead_slot = 0;
+            long long ahead_off = 0;
+            bool more = true, wide = false;
+            auto copy_next = [&](int stage) {
+                if (more && ahead == ahead_chunks) {
+                    ahead_slot = ahead_tile % kGsRing;
+                    if (!ts_wait_warp(&work_full[ahead_slot], (ahead_tile / kGsRing) & 1, guard)) {
+                        ok = more = false;
+                    } else {
+                        const GsWork& w = work[ahead_slot];
+                        more = w.found != 0;
+                        if (more) {
+                            const GsDegree& d = pass.degree[w.degree];
+                            wide = ((static_cast<unsigned long long>(pass.a_stride | d.a_off | d.K) * 4u | reinterpret_cast<uintptr_t>(pass.a)) & 15) == 0;
+                            ahead = 0; ahead_K = d.K; ahead_chunks = w.chunks; ahead_off = d.a_off;
+                            ahead_rows = min(32, w.rows - first);
+                            ++ahead_tile;
+                        }
+                    }
+                }
+                if (more) {
+                    float* to = rows_at + stage * L::row_floats;
+                    const int left = min(kGsChunk, ahead_K - ahead * kGsChunk);
+                    const float* from = pass.a + ahead_off + ahead * kGsChunk;
+                    const int* pair = work_pair[ahead_slot] + first;
+                    const short* comp = work_comp[ahead_slot] + first;
+                    if (wide) {                          // four rows an instruction, 16 bytes a lane
+                        const int c = (lane & 7) * 4;
+                        if (c < left)
+#pragma unroll 4
+                            for (int r = lane >> 3; r < ahead_rows; r += 4) cp_async16(to + r * kGsPitch + c, from + pair[r] * pass.a_stride + comp[r] * ahead_K + c, 16);
+                    } else if (lane < left) {
+#pragma unroll 4
+                        for (int r = 0; r < ahead_rows; ++r) cp_async4(to + r * kGsPitch + lane, from + pair[r] * pass.a_stride + comp[r] * ahead_K + lane);
+                    }
+                    ++ahead;
+                }
+                cp_async_commit();
+            };
+            for (int q = 0; q < RS - 1; ++q) copy_next(q);
+            for (int i = 0; ok; ++i) {
+                const int slot = i % kGsRing;
+                if (!ts_wait_warp(&work_full[slot], (i / kGsRing) & 1, guard)) break;
+                const int found = work[slot].found, chunks = work[slot].chunks, inner = work[slot].inner;
+                const bool live = tid < work[slot].rows;
+                for (int j = 0; found && j < chunks; ++j) {
+                    cp_async_wait<(RS > 2 ? RS - 2 : 0)>();
+                    __syncwarp();                        // the chunk is there for all lanes, and all have read the one before
+                    copy_next(xs == 0 ? RS - 1 : xs - 1);
+                    if (!ok || !free_stage()) { ok = false; break; }
+                    ts_fence_after();
+                    const float* row = row_stages + xs * L::row_floats + tid * kGsPitch;
+                    if (++xs == RS) xs = 0;
+                    const int good = live ? inner - j * kGsChunk : 0;        // what the stage holds behind the tile's or the row's end is no value
+#pragma unroll 1
+                    for (int q = 0; q < kGsChunk; q += 16) {
+                        float v[16];
+#pragma unroll
+                        for (int e = 0; e < 16; e += 4) {
+                            const float4 f = *reinterpret_cast<const float4*>(row + q + e);
+                            v[e] = f.x; v[e + 1] = f.y; v[e + 2] = f.z; v[e + 3] = f.w;
+                        }
+                        if (good < q + 16)
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) v[e] = q + e < good ? v[e] : 0.f;
+                        put16(q, v);
+                    }
+                    give();
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&work_free[slot]);
+                if (!found) break;
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");             // none may be in flight when the CTA ends
+        }
+        if constexpr (kMode == kGsGradient) {
+            int i = 0, j = 0, chunks = 0, inner = 0, comps = 1, m = 0, width = 0;
+            long long pair = 0;
+            const float* column = nullptr;                               // null: behind the matrix's end
+            auto advance = [&]() {
+                ++j;
+                while (j >= chunks) {
+                    const int slot = i % kGsRing;
+                    if (!ts_wait_warp(&work_full[slot], (i / kGsRing) & 1, guard)) { ok = false; return false; }
+                    const GsWork w = work[slot];
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&work_free[slot]);
+                    if (!w.found) return false;
+                    ++i;
+                    const GsDegree& d = pass.degree[w.degree];
+                    j = 0; chunks = w.chunks; inner = w.inner; comps = d.comps; width = d.K;
+                    const long long r = w.row0 + lane, ahead = r / comps;
+                    pair = w.first_pair + ahead;
+                    m = static_cast<int>(r - ahead * comps);
+                    column = tid < w.rows ? pass.a + d.a_off + 128 * w.mtile + tid : nullptr;
+                }
+                return true;
+            };
+            auto load = [&](float (&v)[32]) {
+                long long* const table = row_at[warp & 3];
+                __syncwarp();
+                table[lane] = pair * pass.a_stride + static_cast<long long>(m) * width;
+                __syncwarp();
+                const int good = column ? inner - j * kGsChunk : 0;
+#pragma unroll
+                for (int r = 0; r < 32; ++r) v[r] = r < good ? __ldg(column + table[r]) : 0.f;
+                m += 32 % comps; pair += 32 / comps;
+                if (m >= comps) { m -= comps; ++pair; }
+            };
+            auto store = [&](float (&v)[32]) {
+                if (!free_stage()) { ok = false; return; }
+                ts_fence_after();
+#pragma unroll
+                for (int q = 0; q < 32; q += 16) {
+                    float part[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) part[e] = v[q + e];
+                    put16(q, part);
+                }
+                give();
+            };
+            float v0[32], v1[32];
+            bool have = advance();
+            if (have) load(v0);
+            while (have && ok) {
+                have = advance();
+                if (have) load(v1);
+                if (ok) store(v0);
+                if (!have || !ok) break;
+                have = advance();
+                if (have) load(v0);
+                if (ok) store(v1);
+            }
+        }
+        gs_meet();
+    } else if (warp >= 16) {
+        ts_registers_more<kGsRegsOperand>();
+        const int tid = threadIdx.x & 127, part = warp & 3;
+        int nb = 0, i = 0, j = 0, chunks = 0, inner = 0, comps = 1, m = 0, width = 0, cols = 0, left = 0;
+        long long pair = 0;
+        const float* from = nullptr;
+        bool ok = true, wide = false, crosses = false;   // crosses: the tile behind this one has a matrix of its own
+        auto advance = [&]() {
+            ++j;
+            while (j >= chunks) {
+                const int slot = i % kGsRing;
+                if (!ts_wait_warp(&work_full[slot], (i / kGsRing) & 1, guard)) { ok = false; return false; }
+                const GsWork w = work[slot];
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&work_free[slot]);
+                if (!w.found) return false;
+                ++i;
+                j = chunks = 0;
+                if (!w.fresh) continue;
+                crosses = w.last != 0;
+                const GsDegree& d = pass.degree[w.degree];
+                chunks = w.chunks; inner = w.inner;
+                left = min(128, d.N - 128 * w.block);
+                cols = (left + 15) & ~15;
+                const float* matrix = d.w + static_cast<long long>(w.group) * d.K * d.N;
+                if (kMode == kGsForward) {
+                    width = d.N;
+                    from = matrix + 128 * w.block + tid;
+                } else if (kMode == kGsBackward) {
+                    width = d.K;
+                    from = matrix + static_cast<long long>(128 * w.block + 32 * part + (lane >> 3)) * d.K + 4 * (lane & 7);
+                    wide = (d.K & 3) == 0 && (reinterpret_cast<uintptr_t>(d.w) & 15) == 0;
+                } else {
+                    comps = d.comps; width = d.N;
+                    const long long r = w.row0 + lane, ahead = r / comps;
+                    pair = w.first_pair + ahead;
+                    m = static_cast<int>(r - ahead * comps);
+                    from = pass.b + d.b_off + 128 * w.block + tid;
+                }
+            }
+            return true;
+        };
+        auto load = [&](float (&v)[32]) {
+            const int good = inner - j * kGsChunk;
+            if constexpr (kMode == kGsForward) {
+                const float* at = from + static_cast<long long>(j) * kGsChunk * width;
+                const int rows = tid < left ? good : 0;
+#pragma unroll
+                for (int r = 0; r < 32; ++r, at += width) v[r] = r < rows ? __ldg(at) : 0.f;
+            } else if constexpr (kMode == kGsBackward) {
+                const float* at = from + j * kGsChunk;
+                const int k = 4 * (lane & 7);
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                    const float* p = at + static_cast<long long>(4 * r) * width;
+                    const bool in = 32 * part + (lane >> 3) + 4 * r < left;
+                    if (wide) {
+                        const float4 f = in && k < good ? __ldg(reinterpret_cast<const float4*>(p)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        v[4 * r] = f.x; v[4 * r + 1] = f.y; v[4 * r + 2] = f.z; v[4 * r + 3] = f.w;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[4 * r + e] = in && k + e < good ? __ldg(p + e) : 0.f;
+                    }
+                }
+            } else {
+                long long* const table = row_at[4 + part];
+                __syncwarp();
+                table[lane] = pair * pass.b_stride + static_cast<long long>(m) * width;
+                __syncwarp();
+                const int rows = tid < left ? good : 0;
+#pragma unroll
+                for (int r = 0; r < 32; ++r) v[r] = r < rows ? __ldg(from + table[r]) : 0.f;
+                m += 32 % comps; pair += 32 / comps;
+                if (m >= comps) { m -= comps; ++pair; }
+            }
+        };
+        int stored_cols = 0;
+        auto store = [&](const float (&v)[32]) {
+            const int bs = nb % kGsStages;
+            if (pass.expire_polls > 0 && nb > 0) { ok = false; return; }
+            if (nb >= kGsStages && !ts_wait_warp(&b_free[bs], (nb / kGsStages - 1) & 1, guard)) { ok = false; return; }
+            unsigned char* const to = stages + bs * 2 * kGsTileBytes;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                // a thread's eight groups of four inner values belong to one column, or to eight
+                const int row = kMode == kGsBackward ? 32 * part + (lane >> 3) + 4 * c : tid, group = kMode == kGsBackward ? lane & 7 : c;
+                if (row >= stored_cols) continue;
+                float4 hi, lo;
+                gs_split(v[4 * c], hi.x, lo.x);
+                gs_split(v[4 * c + 1], hi.y, lo.y);
+                gs_split(v[4 * c + 2], hi.z, lo.z);
+                gs_split(v[4 * c + 3], hi.w, lo.w);
+                const int at = tc5_swizzled_group(row, group);
+                *reinterpret_cast<float4*>(to + at) = hi;
+                *reinterpret_cast<float4*>(to + kGsTileBytes + at) = lo;
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&b_full[bs]);
+            ++nb;
+        };
+        // The next chunk is read before this one is stored, unless it belongs to a tile that other tiles of this matrix come before: the ring may not hold
+        // them all, and they need this chunk.
+        bool have = advance();
+        auto turn = [&](float (&now)[32], float (&next)[32]) {
+            const bool early = j + 1 < chunks || crosses;
+            stored_cols = cols;
+            if (early) {
+                have = advance();
+                if (have) load(next);
+            }
+            if (ok) store(now);
+            if (!early && ok) {
+                have = advance();
+                if (have) load(next);
+            }
+        };
+        float v0[32], v1[32];
+        if (have) load(v0);
+        while (have && ok) {
+            turn(v0, v1);
+            if (!have || !ok) break;
+            turn(v1, v0);
+        }
+        gs_meet();
+    } else {
+        ts_registers_more<kGsRegsSums>();
+        const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+        const int tid = threadIdx.x & 127, half = (warp - 8) >> 2;
+        float* const out_stage = row_stages + RS * L::row_floats + (warp - 8) * 32 * kGsOutPitch;
+        int nd = 0, at_degree = 0, at_tile = 0;      // the tile at hand, for a CTA that gives up (0, 0: none yet)
+        bool ok = true;
+        for (int i = 0;; ++i) {
+            const int slot = i % kGsRing;
+            ok = ts_wait_warp(&work_full[slot], (i / kGsRing) & 1, guard);
+            if (!ok) break;
+            const int found = work[slot].found, chunks = work[slot].chunks, rows = work[slot].rows;
+            float* out_row = nullptr;
+            int left = 0;
+            if (found) {
+                const GsWork& w = work[slot];
+                const GsDegree& d = pass.degree[w.degree];
+                at_degree = w.degree; at_tile = w.tile;
+                left = d.N - 128 * w.block - 64 * half;                  // columns of this half that exist
+                if (tid < rows) {
+                    if (kMode == kGsGradient) out_row = w.out + static_cast<long long>(tid) * d.N + 64 * half;
+                    else out_row = pass.out + work_pair[slot][tid] * pass.out_stride + d.b_off + static_cast<long long>(work_comp[slot][tid]) * d.N + 128 * w.block + 64 * half;
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&work_free[slot]);
+            if (!found) break;
+            float sum[64];
+#pragma unroll
+            for (int q = 0; q < 64; ++q) sum[q] = 0.f;
+            for (int j = 0; j < (chunks + 1) / 2; ++j, ++nd) {
+                if (!ts_wait_warp(&d_full[nd & 1], (nd >> 1) & 1, guard)) { ok = false; break; }
+                ts_fence_after();
+                const uint32_t from = lanes + (nd & 1) * 128 + 64 * half;
+#pragma unroll
+                for (int c = 0; c < 64; c += 16)
+                    if (c < left) {                                      // what a last, odd block holds behind the columns is never written
+                        float v[16];
+                        ts_load16(from + c, v);
+#pragma unroll
+                        for (int q = 0; q < 16; ++q) sum[c + q] += v[q];
+                    }
+                ts_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&d_free[nd & 1]);
+            }
+            if (!ok) break;
+            if (kWide) {
+                if (out_row && left > 0)
+#pragma unroll
+                    for (int q = 0; q < 64; q += 8)
+                        asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out_row + q), "f"(sum[q]), "f"(sum[q + 1]), "f"(sum[q + 2]),
+                                     "f"(sum[q + 3]), "f"(sum[q + 4]), "f"(sum[q + 5]), "f"(sum[q + 6]), "f"(sum[q + 7]) : "memory");
+            } else {
+                // 16 columns of the warp's rows at a time through shared memory, so that a store touches two rows instead of 32
+                const unsigned long long mine = reinterpret_cast<unsigned long long>(out_row);
+#pragma unroll
+                for (int c0 = 0; c0 < 64; c0 += 16) {
+                    if (c0 >= left) continue;
+                    __syncwarp();
+#pragma unroll
+                    for (int q = 0; q < 16; ++q) out_stage[lane * kGsOutPitch + q] = sum[c0 + q];
+                    __syncwarp();
+                    const int c = c0 + (lane & 15);
+#pragma unroll 4
+                    for (int r = lane >> 4; r < 32; r += 2) {
+                        float* to = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, mine, r));
+                        if (to && c < left) to[c] = out_stage[r * kGsOutPitch + (c - c0)];
+                    }
+                }
+                __syncwarp();
+            }
+        }
+        if (!ok) {
+            // NaN into the warp's part of the tile at hand and of all that would have followed
+            GsCursor cursor;
+            GsWork lost{};
+            int begin, end;
+            gs_share<kMode>(pass, begin, end);
+            for (int q = 0; q < pass.degrees; ++q) {
+                const int t0 = __shfl_sync(0xffffffffu, begin, q), t1 = __shfl_sync(0xffffffffu, end, q);
+                for (int t = t0; t < t1; ++t)
+                    if ((q > at_degree || (q == at_degree && t >= at_tile)) && cursor.find<kMode>(pass, q, t, lost))
+                        gs_lose<kMode>(pass, lost, tid & ~31, 64 * half);
+            }
+        }
+        gs_meet();
+    }
+    __syncthreads();
+    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+
+// Gradients of groups with several chunks of rows: their partial sums added in order.
+__global__ void __launch_bounds__(256) grouped_join_kernel(const __grid_constant__ GsPass pass) {
+    const GsDegree& d = pass.degree[blockIdx.z];
+    __shared__ int first, chunks;
+    const int g = blockIdx.x;
+    if (threadIdx.x < 32) {
+        int before = 0;
+        for (int q = threadIdx.x; q < g; q += 32) {
+            const int n = gs_runs<kGsGradient>(pass, d, pass.offsets[q + 1] - pass.offsets[q]);
+            before += n > 1 ? n : 0;
+        }
+        before = __reduce_add_sync(0xffffffffu, before);
+        if (threadIdx.x == 0) { first = before; chunks = gs_runs<kGsGradient>(pass, d, pass.offsets[g + 1] - pass.offsets[g]); }
+    }
+    __syncthreads();
+    const int n = chunks;
+    if (n == 1) return;
+    const long long size = static_cast<long long>(d.K) * d.N;
+    for (long long i = blockIdx.y * 256LL + threadIdx.x; i < size; i += 256LL * gridDim.y) {
+        const float* part = d.part + first * size + i;
+        float s = 0.f;
+        for (int c = 0; c < n; c += 8) {                                 // eight loads in flight, added in order
+            float v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v[u] = c + u < n ? part[(c + u) * size] : 0.f;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) s += v[u];
+        }
+        d.grad[g * size + i] = s;
+    }
+}
+
+}  // namespace
+}  // namespace smx

@@ -12,7 +12,7 @@ import numpy as np
 import pytest
 import torch
 
-from symmetrix_b200 import GroupedLinear, RowRouting, clip_gradients
+from symmetrix_b200 import GroupedLinear, RowRouting, SymmetrixError, clip_gradients
 
 pytestmark = pytest.mark.gpu
 
@@ -366,3 +366,33 @@ def test_refusals():
     shared = torch.zeros(case.n, 30, device="cuda")
     with pytest.raises(ValueError, match="shares memory"):
         GroupedLinear([torch.zeros(2, 4, 4, device="cuda")]).forward(shared[:, :4], routing, out=shared[:, 2:6])
+
+
+def test_waits_that_run_out_are_reported():
+    """The test switch makes every CTA lose the matrices behind the first 32 inner values and give up after a few hundred polls: what is lost holds NaN, the
+    rest is right, and the next calls are."""
+    case = Case(torch.float32, [1500, 0, 2700, 40], [1, 3], [70, 200], [136, 64])
+    y, gx, gw = case.expect()
+    layer = case.layer
+    layer.check()
+    layer._fixed.expire_polls = 300
+    lost_y = layer.forward(case.x, case.routing)
+    with pytest.raises(SymmetrixError, match="ran out"):
+        layer.check()
+    lost = layer.backward(case.x, case.gy, case.routing)
+    with pytest.raises(SymmetrixError, match="ran out"):
+        layer.check()
+    layer._fixed.expire_polls = 0
+    layer.check()
+    for got, expect, widths in [(lost_y, y, case.outs), (lost.x, gx, case.ins)]:
+        got = host(got)
+        gone = 0
+        for a, (want, tol) in zip(case.blocks(got[:case.live], widths), expect):
+            missing = np.isnan(a)
+            gone += missing.sum()
+            assert np.all(missing | (np.abs(a - want) <= tol))
+        assert gone > 0
+        np.testing.assert_array_equal(got[case.live:], 0.0)
+    for a, (want, tol) in zip(lost.weights, gw):
+        assert np.all(np.isnan(host(a)) | (np.abs(host(a) - want) <= tol))
+    case.check()
