@@ -192,9 +192,9 @@ int grad_chunk(const smx_grouped_linear& c) {
     long long steps = 0;
     for (int d = 0; d < c.num_degrees; ++d) {
         const smx_grouped_degree& g = c.degrees[d];
-        steps += (c.num_rows * static_cast<long long>(g.components) + 31) / 32 * ((g.in_channels + 127) / 128) * ((g.out_channels + 127) / 128);
+        steps += (c.num_rows * static_cast<long long>(g.components) + 63) / 64 * ((g.in_channels + 127) / 128) * ((g.out_channels + 127) / 128);
     }
-    return 32 * static_cast<int>(std::max(4LL, std::min(128LL, (steps + 591) / 592)));
+    return 64 * static_cast<int>(std::max(2LL, std::min(64LL, (steps + 591) / 592)));
 }
 size_t part_values(const smx_grouped_linear& c, int d) {
     const smx_grouped_degree& g = c.degrees[d];

@@ -15,12 +15,13 @@ namespace smx {
 namespace {
 
 enum GsMode { kGsForward, kGsBackward, kGsGradient };
-constexpr int kGsThreads = 640, kGsChunk = 32, kGsStages = 4, kGsRing = 6;   // inner values of a step; stages of A and of B; tiles in the ring
-constexpr int kGsTileBytes = 128 * kGsChunk * 4, kGsPitch = kGsChunk + 4, kGsOutPitch = 17;
+constexpr int kGsThreads = 896, kGsChunk = 64, kGsStages = 2, kGsRing = 4;   // inner values of a step; stages of A and of B; tiles in the ring
+constexpr int kGsPartBytes = 128 * 32 * 4, kGsHalfBytes = 2 * kGsPartBytes, kGsStageBytes = 2 * kGsHalfBytes;     // B: 32 inner values; hi or lo; both
+constexpr int kGsRowStages = 2, kGsPitch = 32 + 4, kGsOutPitch = 17;
 constexpr int kGsStatusWait = 8;
-// the warps' shares of the registers, by fours: control, A, sums twice, B
-constexpr int kGsRegsLaunch = 96, kGsRegsControl = 48, kGsRegsOperand = 104, kGsRegsSums = 112;
-static_assert(kGsRegsControl + 2 * kGsRegsOperand + 2 * kGsRegsSums <= 5 * kGsRegsLaunch, "the registers of the launch are shared out");
+// the warps' shares of the registers, by fours: control, A, sums, B
+constexpr int kGsRegsLaunch = 72, kGsRegsControl = 40, kGsRegsA = 64, kGsRegsSums = 104, kGsRegsB = 64;
+static_assert(kGsRegsControl + 2 * (kGsRegsA + kGsRegsSums + kGsRegsB) <= 7 * kGsRegsLaunch, "the registers of the launch are shared out");
 
 struct GsDegree {
     int comps, K, N;                 // rows passes: inner values and columns; gradient: rows and columns of the matrices
@@ -31,7 +32,7 @@ struct GsDegree {
 struct GsPass {
     GsDegree degree[SMX_GROUPED_MAX_DEGREES];
     int degrees, groups, zero_tail, out_width;
-    int chunk;                       // gradient: rows of a tile's sum, a multiple of 32
+    int chunk;                       // gradient: rows of a tile's sum, a multiple of kGsChunk
     long long rows;
     const int* offsets;
     const float* a; long long a_stride;
@@ -165,6 +166,27 @@ __device__ __forceinline__ void gs_row(const GsWork& w, int comps, int i, int& p
     comp = static_cast<int>(r - ahead * comps);
 }
 
+// The gradient's operands: a thread reads one column of 32 consecutive rows, kGsChunk on in every step. Lanes find a row each and share where it starts.
+struct GsRows {
+    long long pair, stride;
+    int comp, comps, width;
+    __device__ __forceinline__ void begin(const GsWork& w, int comps_, int width_, long long stride_, int ahead_of) {
+        comps = comps_; width = width_; stride = stride_;
+        const long long r = w.row0 + ahead_of, ahead = r < (1LL << 31) ? static_cast<int>(r) / comps : r / comps;
+        pair = w.first_pair + ahead;
+        comp = static_cast<int>(r - ahead * comps);
+    }
+    __device__ __forceinline__ void read(long long* table, const float* column, int good, float (&v)[32]) {
+        __syncwarp();
+        table[threadIdx.x & 31] = pair * stride + static_cast<long long>(comp) * width;
+        __syncwarp();
+#pragma unroll
+        for (int r = 0; r < 32; ++r) v[r] = r < good ? __ldg(column + table[r]) : 0.f;
+        comp += kGsChunk % comps; pair += kGsChunk / comps;
+        if (comp >= comps) { comp -= comps; ++pair; }
+    }
+};
+
 // NaN into a warp's part of a tile, 32 rows of 64 columns.
 template <int kMode>
 __device__ __forceinline__ void gs_lose(const GsPass& p, const GsWork& w, int row0, int col0) {
@@ -191,52 +213,67 @@ __device__ __forceinline__ void gs_split(float v, float& hi, float& lo) {
 __device__ __forceinline__ void gs_meet() {
     __syncwarp();
     ts_fence_before();
-    asm volatile("bar.sync 1, 640;" ::: "memory");
+    asm volatile("bar.sync 1, 896;" ::: "memory");
+}
+
+// D of one step, its inner values 8 at a time. The remainders' products come first, while the sum is small: the tensor core cuts its sums, so an addition
+// costs up to 2^-23 of the sum. Descriptors of one step ahead are 32 bytes on, two units of their address field; 32 inner values make a part of B.
+__device__ __forceinline__ void gs_products(uint32_t d, uint32_t a_hi, uint32_t a_lo, uint32_t b, uint32_t idesc, int steps) {
+    const uint64_t hi = tc5_smem_desc(b), lo = tc5_smem_desc(b + kGsHalfBytes);
+#pragma unroll 1
+    for (int k = 0; k < steps; ++k) {
+        const int at = (k >> 2) * (kGsPartBytes >> 4) + (k & 3) * 2;
+        ts_mma(d, a_lo + 8 * k, hi + at, idesc, k > 0);
+        ts_mma(d, a_hi + 8 * k, lo + at, idesc, true);
+    }
+#pragma unroll 1
+    for (int k = 0; k < steps; ++k) ts_mma(d, a_hi + 8 * k, hi + (k >> 2) * (kGsPartBytes >> 4) + (k & 3) * 2, idesc, true);
 }
 
 // kWide: every row's half of a tile of the output starts on 32 bytes and is 64 columns long.
 template <int kMode, bool kWide>
 struct GsLayout {
-    static constexpr int row_stages = kMode == kGsGradient ? 0 : kWide ? 5 : 4;      // raw rows on their way to tensor memory
-    static_assert(kGsRing > row_stages, "the rows' copies run row_stages - 1 tiles ahead of the tile that is given back last");
-    static constexpr int row_floats = 128 * kGsPitch;
-    static constexpr int smem = kGsStages * 2 * kGsTileBytes + (row_stages * row_floats + (kWide ? 0 : 8 * 32 * kGsOutPitch)) * 4 + 1024;
-    static_assert(smem + 8192 <= 227 * 1024, "shared memory of one CTA per SM");
+    static constexpr int row_stages = kMode == kGsGradient ? 0 : kGsRowStages;       // raw rows on their way to tensor memory
+    static_assert(kGsRing > kGsRowStages, "the rows' copies run a step, and so up to a tile, ahead of the tile that is given back last");
+    static constexpr int row_floats = 8 * 32 * kGsPitch;                             // a stage: eight warps' 32 rows of 32 values
+    static constexpr int smem = kGsStages * kGsStageBytes + (row_stages * row_floats + (kWide ? 0 : 8 * 32 * kGsOutPitch)) * 4 + 1024;
+    static_assert(smem + 7168 <= 227 * 1024, "shared memory of one CTA per SM");
 };
 
-// One persistent CTA per SM walks its share of the tiles; its warps are specialised, so that the parts of neighbouring tiles overlap:
-//   warp 0       the products (one thread)
-//   warp 1       finds the tiles (a ring, ahead of all others)
-//   warps 2, 3   zeros into the rows behind the last group
-//   warps 4-7    A. Rows passes: a warp copies 32 values of each of its 32 rows asynchronously, row_stages - 1 chunks ahead; a thread splits those of its row
-//                and stores them to tensor memory. Gradient: a thread owns a column of x and reads it row by row, next chunk's values in registers.
-//   warps 8-15   a thread adds half of its row's partial sums of every 64 inner values in registers (the tensor core cuts its sums instead of rounding
-//                them: one sum over 128 inner values is off five times as far as float32) and writes its half of the row
-//   warps 16-19  B, next chunk's values in registers; where a matrix has up to 128 inner values it stays for all row tiles of its group
-// TMEM: two partial sums of 128 columns, taken in turn, and four stages of A of 64 (hi, lo).
+// One persistent CTA per SM walks its share of the tiles, 64 inner values a step; its warps are specialised, so that the parts of neighbouring tiles overlap:
+//   warp 0        the products (one thread)
+//   warp 1        finds the tiles (a ring, ahead of all others)
+//   warps 2, 3    zeros into the rows behind the last group
+//   warps 4-11    A, 32 rows of 32 inner values a warp. Rows passes: a warp copies its rows asynchronously, a step ahead; a thread splits those of its row and
+//                 stores them to tensor memory. Gradient: a thread owns a column of x and reads it row by row.
+//   warps 12-19   a thread adds half of its row's partial sums of every step in registers (the tensor core cuts its sums instead of rounding them: one
+//                 sum over 128 inner values is off five times as far as float32) and writes its half of the row
+//   warps 20-27   B, 32 inner values of 128 columns for four warps, read when the ones before are stored; where a matrix has up to 128 inner values it
+//                 stays for all row tiles of its group
+// TMEM: two partial sums of 128 columns, taken in turn, and two stages of A of 128 (hi, lo). A hand-over costs its warps some hundred cycles: with steps of
+// 32 inner values and half the warps for A and B the products waited two thirds of the time (98,304 atoms of 89 elements 127 us).
 // Every wait is bounded; if one runs out, the CTA gives up, fills its remaining tiles with NaN, reports it to `status` and ends when its products
 // and copies in flight have.
 template <int kMode, bool kWide>
 __global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid_constant__ GsPass pass) {
     using L = GsLayout<kMode, kWide>;
-    constexpr int RS = L::row_stages;
     extern __shared__ unsigned char gs_smem_raw[];
     __shared__ __align__(8) unsigned long long work_full[kGsRing], work_free[kGsRing], a_full[kGsStages], a_free[kGsStages], b_full[kGsStages], b_free[kGsStages],
         d_full[2], d_free[2], drained;
     __shared__ GsWork work[kGsRing];
     __shared__ int work_pair[kMode == kGsGradient ? 1 : kGsRing][128];
     __shared__ short work_comp[kMode == kGsGradient ? 1 : kGsRing][128];
-    __shared__ __align__(16) long long row_at[kMode == kGsGradient ? 8 : 1][32];         // gradient: where a chunk's rows start, for every operand warp
+    __shared__ __align__(16) long long row_at[kMode == kGsGradient ? 16 : 1][32];        // gradient: where a chunk's rows start, for every operand warp
     __shared__ uint32_t tmem_slot;
     __shared__ int guard[2];                                                             // a wait ran out; polls of a wait
     const int warp = ts_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     unsigned char* const stages = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(gs_smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    float* const row_stages = reinterpret_cast<float*>(stages + kGsStages * 2 * kGsTileBytes);
+    float* const row_stages = reinterpret_cast<float*>(stages + kGsStages * kGsStageBytes);
     if (threadIdx.x == 0) {
         guard[0] = 0;
         guard[1] = pass.expire_polls > 0 ? pass.expire_polls : static_cast<int>(kMbarSpinLimit);
-        for (int q = 0; q < kGsRing; ++q) { mbar_init(&work_full[q], 1); mbar_init(&work_free[q], 17); }
-        for (int q = 0; q < kGsStages; ++q) { mbar_init(&a_full[q], 4); mbar_init(&a_free[q], 1); mbar_init(&b_full[q], 4); mbar_init(&b_free[q], 1); }
+        for (int q = 0; q < kGsRing; ++q) { mbar_init(&work_full[q], 1); mbar_init(&work_free[q], 25); }
+        for (int q = 0; q < kGsStages; ++q) { mbar_init(&a_full[q], 8); mbar_init(&a_free[q], 1); mbar_init(&b_full[q], 8); mbar_init(&b_free[q], 1); }
         for (int q = 0; q < 2; ++q) { mbar_init(&d_full[q], 1); mbar_init(&d_free[q], 8); }
         mbar_init(&drained, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -253,7 +290,7 @@ __global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid
     if (warp < 4) {
         ts_registers_less<kGsRegsControl>();
         if (warp == 0) {
-            int na = 0, nb = 0, nd = 0, base_b = 0;                  // stages of A and B used so far, partial sums; B's stages of the tile
+            int na = 0, nb = 0, base_b = 0;                          // stages of A (and partial sums) and of B used so far; B's first one of the tile
             bool ok = true;
             const bool leader = ts_elect();
             const uint32_t b_at = smem_u32(stages);
@@ -269,24 +306,21 @@ __global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid
                 if (!found) break;
                 if (fresh) { base_b = nb; nb += chunks; }
 #pragma unroll 1
-                for (int j = 0; j < chunks; ++j) {
-                    const int st = na % kGsStages, n = base_b + j, bs = n % kGsStages, sum = nd & 1;
-                    if ((j & 1) == 0 && nd >= 2) ok = ts_wait_warp(&d_free[sum], ((nd >> 1) - 1) & 1, guard);
+                for (int j = 0; j < chunks; ++j, ++na) {
+                    const int st = na % kGsStages, n = base_b + j, bs = n % kGsStages;           // the partial sums have two stages too
+                    if (na >= 2) ok = ts_wait_warp(&d_free[st], ((na >> 1) - 1) & 1, guard);
                     ok = ok && ts_wait_warp(&a_full[st], (na / kGsStages) & 1, guard);
                     if (fresh) ok = ok && ts_wait_warp(&b_full[bs], (n / kGsStages) & 1, guard);
                     if (!ok) break;
                     ts_fence_after();
-                    const uint32_t hi = ts_uniform(a_at + 64 * st), b = ts_uniform(b_at + bs * 2 * kGsTileBytes), d = ts_uniform(tmem + 128 * sum);
-                    const bool ends = (j & 1) != 0 || j + 1 == chunks;
+                    const uint32_t hi = ts_uniform(a_at + 128 * st), b = ts_uniform(b_at + bs * kGsStageBytes), d = ts_uniform(tmem + 128 * st);
                     if (leader) {
-                        ts_chunk(d, hi, hi + 32, b, b + kGsTileBytes, ts_idesc(cols), min(4, (inner - kGsChunk * j + 7) / 8), (j & 1) != 0);
+                        gs_products(d, hi, hi + 64, b, ts_idesc(cols), min(8, (inner - kGsChunk * j + 7) / 8));
                         ts_commit(&a_free[st]);
                         if (last) ts_commit(&b_free[bs]);
-                        if (ends) ts_commit(&d_full[sum]);
+                        ts_commit(&d_full[st]);
                     }
                     __syncwarp();
-                    ++na;
-                    if (ends) ++nd;
                 }
             }
         } else if (warp == 1) {
@@ -333,10 +367,10 @@ __global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid
             mbar_wait(&drained, 0);
             if (lane == 0 && pass.status) atomicMax(pass.status, kGsStatusWait);
         }
-    } else if (warp < 8) {
-        ts_registers_more<kGsRegsOperand>();
+    } else if (warp < 12) {
+        ts_registers_less<kGsRegsA>();
         const uint32_t lanes = a_at + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-        const int tid = threadIdx.x & 127, first = tid & ~31;            // the warp's rows are its own: no barrier but the work's
+        const int tid = threadIdx.x & 127, first = tid & ~31, k_part = 32 * ((warp - 4) >> 2);   // the warp's rows and inner values are its own
         int na = 0;
         bool ok = true;
         auto free_stage = [&]() { return na < kGsStages || ts_wait_warp(&a_free[na % kGsStages], (na / kGsStages - 1) & 1, guard); };
@@ -349,14 +383,14 @@ __global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid
         };
         auto put16 = [&](int q, float (&v)[16]) {
             float hi[16];
-            const uint32_t to = lanes + 64 * (na % kGsStages) + q;
+            const uint32_t to = lanes + 128 * (na % kGsStages) + k_part + q;
 #pragma unroll
             for (int e = 0; e < 16; ++e) { float lo; gs_split(v[e], hi[e], lo); v[e] = lo; }
             ts_store16(to, hi);
-            ts_store16(to + 32, v);
+            ts_store16(to + 64, v);
         };
         if constexpr (kMode != kGsGradient) {
-            float* const rows_at = row_stages + first * kGsPitch;
+            float* const rows_at = row_stages + (warp - 4) * 32 * kGsPitch;
             int xs = 0, ahead_tile = 0, ahead = 0, ahead_chunks = 0, ahead_K = 0, ahead_rows = 0, ahead_slot = 0;
             long long ahead_off = 0;
             bool more = true, wide = false;
@@ -379,8 +413,8 @@ __global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid
                 }
                 if (more) {
                     float* to = rows_at + stage * L::row_floats;
-                    const int left = min(kGsChunk, ahead_K - ahead * kGsChunk);
-                    const float* from = pass.a + ahead_off + ahead * kGsChunk;
+                    const int k = ahead * kGsChunk + k_part, left = min(32, ahead_K - k);
+                    const float* from = pass.a + ahead_off + k;
                     const int* pair = work_pair[ahead_slot] + first;
                     const short* comp = work_comp[ahead_slot] + first;
                     if (wide) {                          // four rows an instruction, 16 bytes a lane
@@ -396,23 +430,24 @@ __global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid
                 }
                 cp_async_commit();
             };
-            for (int q = 0; q < RS - 1; ++q) copy_next(q);
+            copy_next(0);
             for (int i = 0; ok; ++i) {
                 const int slot = i % kGsRing;
                 if (!ts_wait_warp(&work_full[slot], (i / kGsRing) & 1, guard)) break;
                 const int found = work[slot].found, chunks = work[slot].chunks, inner = work[slot].inner;
                 const bool live = tid < work[slot].rows;
                 for (int j = 0; found && j < chunks; ++j) {
-                    cp_async_wait<(RS > 2 ? RS - 2 : 0)>();
-                    __syncwarp();                        // the chunk is there for all lanes, and all have read the one before
-                    copy_next(xs == 0 ? RS - 1 : xs - 1);
+                    __syncwarp();                        // all lanes have read what the next copy overwrites
+                    copy_next(xs ^ 1);
+                    cp_async_wait<1>();
+                    __syncwarp();
                     if (!ok || !free_stage()) { ok = false; break; }
                     ts_fence_after();
-                    const float* row = row_stages + xs * L::row_floats + tid * kGsPitch;
-                    if (++xs == RS) xs = 0;
-                    const int good = live ? inner - j * kGsChunk : 0;        // what the stage holds behind the tile's or the row's end is no value
+                    const float* row = rows_at + xs * L::row_floats + lane * kGsPitch;
+                    xs ^= 1;
+                    const int good = live ? inner - j * kGsChunk - k_part : 0;       // what the stage holds behind the tile's or the row's end is no value
 #pragma unroll 1
-                    for (int q = 0; q < kGsChunk; q += 16) {
+                    for (int q = 0; q < 32; q += 16) {
                         float v[16];
 #pragma unroll
                         for (int e = 0; e < 16; e += 4) {
@@ -433,195 +468,131 @@ __global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid
             asm volatile("cp.async.wait_all;" ::: "memory");             // none may be in flight when the CTA ends
         }
         if constexpr (kMode == kGsGradient) {
-            int i = 0, j = 0, chunks = 0, inner = 0, comps = 1, m = 0, width = 0;
-            long long pair = 0;
-            const float* column = nullptr;                               // null: behind the matrix's end
-            auto advance = [&]() {
-                ++j;
-                while (j >= chunks) {
-                    const int slot = i % kGsRing;
-                    if (!ts_wait_warp(&work_full[slot], (i / kGsRing) & 1, guard)) { ok = false; return false; }
-                    const GsWork w = work[slot];
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&work_free[slot]);
-                    if (!w.found) return false;
-                    ++i;
+            int i = 0;
+            for (;;) {
+                const int slot = i % kGsRing;
+                if (!ts_wait_warp(&work_full[slot], (i / kGsRing) & 1, guard)) break;
+                const int found = work[slot].found, chunks = work[slot].chunks, inner = work[slot].inner;
+                GsRows at;
+                const float* column = nullptr;                           // null: behind the matrix's end
+                if (found) {
+                    const GsWork& w = work[slot];
                     const GsDegree& d = pass.degree[w.degree];
-                    j = 0; chunks = w.chunks; inner = w.inner; comps = d.comps; width = d.K;
-                    const long long r = w.row0 + lane, ahead = r / comps;
-                    pair = w.first_pair + ahead;
-                    m = static_cast<int>(r - ahead * comps);
-                    column = tid < w.rows ? pass.a + d.a_off + 128 * w.mtile + tid : nullptr;
+                    at.begin(w, d.comps, d.K, pass.a_stride, k_part + lane);
+                    if (tid < w.rows) column = pass.a + d.a_off + 128 * w.mtile + tid;
                 }
-                return true;
-            };
-            auto load = [&](float (&v)[32]) {
-                long long* const table = row_at[warp & 3];
                 __syncwarp();
-                table[lane] = pair * pass.a_stride + static_cast<long long>(m) * width;
-                __syncwarp();
-                const int good = column ? inner - j * kGsChunk : 0;
+                if (lane == 0) mbar_arrive(&work_free[slot]);
+                if (!found) break;
+                ++i;
+                for (int j = 0; j < chunks; ++j) {
+                    float v[32];
+                    at.read(row_at[warp - 4], column, column ? inner - j * kGsChunk - k_part : 0, v);
+                    if (!free_stage()) { ok = false; break; }
+                    ts_fence_after();
 #pragma unroll
-                for (int r = 0; r < 32; ++r) v[r] = r < good ? __ldg(column + table[r]) : 0.f;
-                m += 32 % comps; pair += 32 / comps;
-                if (m >= comps) { m -= comps; ++pair; }
-            };
-            auto store = [&](float (&v)[32]) {
-                if (!free_stage()) { ok = false; return; }
-                ts_fence_after();
+                    for (int q = 0; q < 32; q += 16) {
+                        float part[16];
 #pragma unroll
-                for (int q = 0; q < 32; q += 16) {
-                    float part[16];
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) part[e] = v[q + e];
-                    put16(q, part);
+                        for (int e = 0; e < 16; ++e) part[e] = v[q + e];
+                        put16(q, part);
+                    }
+                    give();
                 }
-                give();
-            };
-            float v0[32], v1[32];
-            bool have = advance();
-            if (have) load(v0);
-            while (have && ok) {
-                have = advance();
-                if (have) load(v1);
-                if (ok) store(v0);
-                if (!have || !ok) break;
-                have = advance();
-                if (have) load(v0);
-                if (ok) store(v1);
+                if (!ok) break;
             }
         }
         gs_meet();
-    } else if (warp >= 16) {
-        ts_registers_more<kGsRegsOperand>();
-        const int tid = threadIdx.x & 127, part = warp & 3;
-        int nb = 0, i = 0, j = 0, chunks = 0, inner = 0, comps = 1, m = 0, width = 0, cols = 0, left = 0;
-        long long pair = 0;
-        const float* from = nullptr;
-        bool ok = true, wide = false, crosses = false;   // crosses: the tile behind this one has a matrix of its own
-        auto advance = [&]() {
-            ++j;
-            while (j >= chunks) {
-                const int slot = i % kGsRing;
-                if (!ts_wait_warp(&work_full[slot], (i / kGsRing) & 1, guard)) { ok = false; return false; }
-                const GsWork w = work[slot];
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&work_free[slot]);
-                if (!w.found) return false;
-                ++i;
-                j = chunks = 0;
-                if (!w.fresh) continue;
-                crosses = w.last != 0;
+    } else if (warp >= 20) {
+        ts_registers_less<kGsRegsB>();
+        const int tid = threadIdx.x & 127, part = warp & 3, k_part = 32 * ((warp - 20) >> 2);
+        int nb = 0;
+        bool ok = true;
+        for (int i = 0; ok; ++i) {
+            const int slot = i % kGsRing;
+            if (!ts_wait_warp(&work_full[slot], (i / kGsRing) & 1, guard)) break;
+            const GsWork& w = work[slot];
+            const int found = w.found, chunks = w.fresh ? w.chunks : 0, inner = w.inner;
+            int width = 0, left = 0;
+            const float* from = nullptr;
+            bool wide = false;
+            GsRows at;
+            if (found) {
                 const GsDegree& d = pass.degree[w.degree];
-                chunks = w.chunks; inner = w.inner;
                 left = min(128, d.N - 128 * w.block);
-                cols = (left + 15) & ~15;
                 const float* matrix = d.w + static_cast<long long>(w.group) * d.K * d.N;
                 if (kMode == kGsForward) {
                     width = d.N;
-                    from = matrix + 128 * w.block + tid;
+                    from = matrix + static_cast<long long>(k_part) * width + 128 * w.block + tid;
                 } else if (kMode == kGsBackward) {
                     width = d.K;
-                    from = matrix + static_cast<long long>(128 * w.block + 32 * part + (lane >> 3)) * d.K + 4 * (lane & 7);
-                    wide = (d.K & 3) == 0 && (reinterpret_cast<uintptr_t>(d.w) & 15) == 0;
+                    from = matrix + static_cast<long long>(128 * w.block + 32 * part + (lane >> 3)) * width + k_part + 4 * (lane & 7);
+                    wide = (width & 3) == 0 && (reinterpret_cast<uintptr_t>(d.w) & 15) == 0;
                 } else {
-                    comps = d.comps; width = d.N;
-                    const long long r = w.row0 + lane, ahead = r / comps;
-                    pair = w.first_pair + ahead;
-                    m = static_cast<int>(r - ahead * comps);
+                    at.begin(w, d.comps, d.N, pass.b_stride, k_part + lane);
                     from = pass.b + d.b_off + 128 * w.block + tid;
                 }
             }
-            return true;
-        };
-        auto load = [&](float (&v)[32]) {
-            const int good = inner - j * kGsChunk;
-            if constexpr (kMode == kGsForward) {
-                const float* at = from + static_cast<long long>(j) * kGsChunk * width;
-                const int rows = tid < left ? good : 0;
-#pragma unroll
-                for (int r = 0; r < 32; ++r, at += width) v[r] = r < rows ? __ldg(at) : 0.f;
-            } else if constexpr (kMode == kGsBackward) {
-                const float* at = from + j * kGsChunk;
-                const int k = 4 * (lane & 7);
-#pragma unroll
-                for (int r = 0; r < 8; ++r) {
-                    const float* p = at + static_cast<long long>(4 * r) * width;
-                    const bool in = 32 * part + (lane >> 3) + 4 * r < left;
-                    if (wide) {
-                        const float4 f = in && k < good ? __ldg(reinterpret_cast<const float4*>(p)) : make_float4(0.f, 0.f, 0.f, 0.f);
-                        v[4 * r] = f.x; v[4 * r + 1] = f.y; v[4 * r + 2] = f.z; v[4 * r + 3] = f.w;
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) v[4 * r + e] = in && k + e < good ? __ldg(p + e) : 0.f;
-                    }
-                }
-            } else {
-                long long* const table = row_at[4 + part];
-                __syncwarp();
-                table[lane] = pair * pass.b_stride + static_cast<long long>(m) * width;
-                __syncwarp();
-                const int rows = tid < left ? good : 0;
-#pragma unroll
-                for (int r = 0; r < 32; ++r) v[r] = r < rows ? __ldg(from + table[r]) : 0.f;
-                m += 32 % comps; pair += 32 / comps;
-                if (m >= comps) { m -= comps; ++pair; }
-            }
-        };
-        int stored_cols = 0;
-        auto store = [&](const float (&v)[32]) {
-            const int bs = nb % kGsStages;
-            if (pass.expire_polls > 0 && nb > 0) { ok = false; return; }
-            if (nb >= kGsStages && !ts_wait_warp(&b_free[bs], (nb / kGsStages - 1) & 1, guard)) { ok = false; return; }
-            unsigned char* const to = stages + bs * 2 * kGsTileBytes;
-#pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                // a thread's eight groups of four inner values belong to one column, or to eight
-                const int row = kMode == kGsBackward ? 32 * part + (lane >> 3) + 4 * c : tid, group = kMode == kGsBackward ? lane & 7 : c;
-                if (row >= stored_cols) continue;
-                float4 hi, lo;
-                gs_split(v[4 * c], hi.x, lo.x);
-                gs_split(v[4 * c + 1], hi.y, lo.y);
-                gs_split(v[4 * c + 2], hi.z, lo.z);
-                gs_split(v[4 * c + 3], hi.w, lo.w);
-                const int at = tc5_swizzled_group(row, group);
-                *reinterpret_cast<float4*>(to + at) = hi;
-                *reinterpret_cast<float4*>(to + kGsTileBytes + at) = lo;
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
-            if (lane == 0) mbar_arrive(&b_full[bs]);
-            ++nb;
-        };
-        // The next chunk is read before this one is stored, unless it belongs to a tile that other tiles of this matrix come before: the ring may not hold
-        // them all, and they need this chunk.
-        bool have = advance();
-        auto turn = [&](float (&now)[32], float (&next)[32]) {
-            const bool early = j + 1 < chunks || crosses;
-            stored_cols = cols;
-            if (early) {
-                have = advance();
-                if (have) load(next);
+            if (lane == 0) mbar_arrive(&work_free[slot]);
+            if (!found) break;
+            const int cols = (left + 15) & ~15;
+#pragma unroll 1
+            for (int j = 0; j < chunks; ++j) {
+                const int good = inner - j * kGsChunk - k_part;
+                float v[32];
+                if constexpr (kMode == kGsForward) {
+                    const float* p = from + static_cast<long long>(j) * kGsChunk * width;
+                    const int rows = tid < left ? good : 0;
+#pragma unroll
+                    for (int r = 0; r < 32; ++r, p += width) v[r] = r < rows ? __ldg(p) : 0.f;
+                } else if constexpr (kMode == kGsBackward) {
+                    const int k = 4 * (lane & 7);
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) {
+                        const float* p = from + j * kGsChunk + static_cast<long long>(4 * r) * width;
+                        const bool in = 32 * part + (lane >> 3) + 4 * r < left;
+                        if (wide) {
+                            const float4 f = in && k < good ? __ldg(reinterpret_cast<const float4*>(p)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                            v[4 * r] = f.x; v[4 * r + 1] = f.y; v[4 * r + 2] = f.z; v[4 * r + 3] = f.w;
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) v[4 * r + e] = in && k + e < good ? __ldg(p + e) : 0.f;
+                        }
+                    }
+                } else {
+                    at.read(row_at[warp - 12], from, tid < left ? good : 0, v);
+                }
+                const int bs = nb % kGsStages;
+                if (pass.expire_polls > 0 && nb > 0) { ok = false; break; }
+                if (nb >= kGsStages && !ts_wait_warp(&b_free[bs], (nb / kGsStages - 1) & 1, guard)) { ok = false; break; }
+                unsigned char* const to = stages + bs * kGsStageBytes + (k_part >> 5) * kGsPartBytes;
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    // a thread's eight groups of four inner values belong to one column, or to eight
+                    const int row = kMode == kGsBackward ? 32 * part + (lane >> 3) + 4 * c : tid, group = kMode == kGsBackward ? lane & 7 : c;
+                    if (row >= cols) continue;
+                    float4 hi, lo;
+                    gs_split(v[4 * c], hi.x, lo.x);
+                    gs_split(v[4 * c + 1], hi.y, lo.y);
+                    gs_split(v[4 * c + 2], hi.z, lo.z);
+                    gs_split(v[4 * c + 3], hi.w, lo.w);
+                    const int off = tc5_swizzled_group(row, group);
+                    *reinterpret_cast<float4*>(to + off) = hi;
+                    *reinterpret_cast<float4*>(to + kGsHalfBytes + off) = lo;
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&b_full[bs]);
+                ++nb;
             }
-            if (ok) store(now);
-            if (!early && ok) {
-                have = advance();
-                if (have) load(next);
-            }
-        };
-        float v0[32], v1[32];
-        if (have) load(v0);
-        while (have && ok) {
-            turn(v0, v1);
-            if (!have || !ok) break;
-            turn(v1, v0);
         }
         gs_meet();
     } else {
         ts_registers_more<kGsRegsSums>();
         const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-        const int tid = threadIdx.x & 127, half = (warp - 8) >> 2;
-        float* const out_stage = row_stages + RS * L::row_floats + (warp - 8) * 32 * kGsOutPitch;
+        const int tid = threadIdx.x & 127, half = (warp - 12) >> 2;
+        float* const out_stage = row_stages + L::row_stages * L::row_floats + (warp - 12) * 32 * kGsOutPitch;
         int nd = 0, at_degree = 0, at_tile = 0;      // the tile at hand, for a CTA that gives up (0, 0: none yet)
         bool ok = true;
         for (int i = 0;; ++i) {
@@ -647,7 +618,7 @@ __global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid
             float sum[64];
 #pragma unroll
             for (int q = 0; q < 64; ++q) sum[q] = 0.f;
-            for (int j = 0; j < (chunks + 1) / 2; ++j, ++nd) {
+            for (int j = 0; j < chunks; ++j, ++nd) {
                 if (!ts_wait_warp(&d_full[nd & 1], (nd >> 1) & 1, guard)) { ok = false; break; }
                 ts_fence_after();
                 const uint32_t from = lanes + (nd & 1) * 128 + 64 * half;
