@@ -21,122 +21,11 @@ namespace {
 
 constexpr int kMaxDegrees = SMX_GROUPED_MAX_DEGREES;
 
-// out[row][n] = sum_k in[row][k] W_g[k * w_k + n * w_n]
-template <typename T>
-struct RowsDegree { int comps, K, N; long long in_off, out_off; const T* w; long long w_group, w_k, w_n; };
-template <typename T>
-struct RowsPass {
-    RowsDegree<T> degree[kMaxDegrees];
-    int degrees, groups; long long rows; const int* offsets;
-    const T* in; long long in_stride; T* out; long long out_stride;
-    int zero_tail, out_width;
-};
-
-constexpr int kTile = 64, kStep = 16;
-template <typename T>
-__global__ void __launch_bounds__(256) grouped_rows_kernel(const __grid_constant__ RowsPass<T> pass) {
-    __shared__ T as[kStep][kTile + 1], bs[kStep][kTile + 1];
-    __shared__ TileRows tile;
-    __shared__ int which, block;
-    const int tid = threadIdx.x;
-    if (tid < 32) {
-        long long at = blockIdx.x, tiles = 0;
-        TileRows t{};
-        int hit = -1, b = 0;
-        for (int q = 0; q < pass.degrees && hit < 0; ++q) {
-            const int blocks = (pass.degree[q].N + kTile - 1) / kTile;
-            if (find_tile(pass.offsets, pass.groups, false, pass.rows, pass.degree[q].comps, kTile, at / blocks, t, tiles)) { hit = q; b = static_cast<int>(at % blocks); }
-            else at -= tiles * blocks;
-        }
-        if (tid == 0) { which = hit; block = b; tile = t; }
-    }
-    if (pass.zero_tail)
-        for (long long p = pass.offsets[pass.groups] + blockIdx.x; p < pass.rows; p += gridDim.x)
-            for (int c = tid; c < pass.out_width; c += 256) pass.out[p * pass.out_stride + c] = T(0);
-    __syncthreads();
-    if (which < 0) return;
-    const RowsDegree<T>& d = pass.degree[which];
-    const T* w = d.w + tile.group * d.w_group;
-    const int col0 = block * kTile, ty = tid / 16, tx = tid % 16;
-    auto row_at = [&](long long r, long long stride, long long off, int width) {
-        const long long q = tile.row0 + r;
-        return (tile.first_pair + q / d.comps) * stride + off + q % d.comps * width;
-    };
-    T acc[4][4] = {};
-    for (int k0 = 0; k0 < d.K; k0 += kStep) {
-        for (int i = tid; i < kTile * kStep; i += 256) {
-            const int r = i / kStep, k = i % kStep;
-            as[k][r] = r < tile.rows && k0 + k < d.K ? pass.in[row_at(r, pass.in_stride, d.in_off, d.K) + k0 + k] : T(0);
-            const int n = i % kTile, kb = i / kTile;
-            bs[kb][n] = col0 + n < d.N && k0 + kb < d.K ? w[(k0 + kb) * d.w_k + (col0 + n) * d.w_n] : T(0);
-        }
-        __syncthreads();
-        for (int k = 0; k < kStep; ++k)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] += as[k][ty + 16 * i] * bs[k][tx + 16 * j];
-        __syncthreads();
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int r = ty + 16 * i;
-        if (r >= tile.rows) continue;
-        const long long to = row_at(r, pass.out_stride, d.out_off, d.N) + col0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (col0 + tx + 16 * j < d.N) pass.out[to + tx + 16 * j] = acc[i][j];
-    }
-}
-
-// grad_w[g][k][n] = sum over the group's rows of x[row][k] gy[row][n]
-template <typename T>
-struct GradDegree { int comps, K, N; long long x_off, y_off; T* grad; };
-template <typename T>
-struct GradPass {
-    GradDegree<T> degree[kMaxDegrees];
-    int groups; const int* offsets;
-    const T* x; long long x_stride; const T* gy; long long gy_stride;
-};
-template <typename T>
-__global__ void __launch_bounds__(256) grouped_grad_kernel(const __grid_constant__ GradPass<T> pass) {
-    __shared__ T as[kStep][kTile + 1], bs[kStep][kTile + 1];
-    const GradDegree<T>& d = pass.degree[blockIdx.z];
-    const int blocks = (d.N + kTile - 1) / kTile, tiles = blocks * ((d.K + kTile - 1) / kTile);
-    const int tid = threadIdx.x, ty = tid / 16, tx = tid % 16, g = blockIdx.x;
-    const long long first = pass.offsets[g], rows = (pass.offsets[g + 1] - first) * d.comps;
-    for (int t = blockIdx.y; t < tiles; t += gridDim.y) {
-        const int k0 = t / blocks * kTile, n0 = t % blocks * kTile;
-        T acc[4][4] = {};
-        for (long long r0 = 0; r0 < rows; r0 += kStep) {
-            for (int i = tid; i < kTile * kStep; i += 256) {
-                const int c = i % kTile, r = i / kTile;
-                const long long q = r0 + r, p = first + q / d.comps, m = q % d.comps;
-                as[r][c] = q < rows && k0 + c < d.K ? pass.x[p * pass.x_stride + d.x_off + m * d.K + k0 + c] : T(0);
-                bs[r][c] = q < rows && n0 + c < d.N ? pass.gy[p * pass.gy_stride + d.y_off + m * d.N + n0 + c] : T(0);
-            }
-            __syncthreads();
-            for (int r = 0; r < kStep; ++r)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[i][j] += as[r][ty + 16 * i] * bs[r][tx + 16 * j];
-            __syncthreads();
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int k = k0 + ty + 16 * i, n = n0 + tx + 16 * j;
-                if (k < d.K && n < d.N) d.grad[(static_cast<long long>(g) * d.K + k) * d.N + n] = acc[i][j];
-            }
-    }
-}
-
 }  // namespace
 }  // namespace smx
 
 #include "grouped_f32.cuh"
+#include "grouped_f64.cuh"
 
 namespace smx {
 namespace {
@@ -189,10 +78,11 @@ void check_weights(const smx_grouped_linear& c) {
 // What a call allocates nothing for: the partial sums of the matrices' gradients. Their chunks of rows are as long as leaves four tiles for each of 148
 // SMs (a constant, so that sizes and sums do not depend on the device); a group with several chunks has less than twice as many as its rows fill.
 int grad_chunk(const smx_grouped_linear& c) {
+    const int tile = c.precision == SMX_FP32 ? 128 : 64;
     long long steps = 0;
     for (int d = 0; d < c.num_degrees; ++d) {
         const smx_grouped_degree& g = c.degrees[d];
-        steps += (c.num_rows * static_cast<long long>(g.components) + 63) / 64 * ((g.in_channels + 127) / 128) * ((g.out_channels + 127) / 128);
+        steps += (c.num_rows * static_cast<long long>(g.components) + 63) / 64 * ((g.in_channels + tile - 1) / tile) * ((g.out_channels + tile - 1) / tile);
     }
     return 64 * static_cast<int>(std::max(2LL, std::min(64LL, (steps + 591) / 592)));
 }
@@ -200,6 +90,67 @@ size_t part_values(const smx_grouped_linear& c, int d) {
     const smx_grouped_degree& g = c.degrees[d];
     const long long parts = 2 * (c.num_rows * static_cast<long long>(g.components) / grad_chunk(c));
     return static_cast<size_t>((parts * g.in_channels * g.out_channels + 63) / 64 * 64);
+}
+
+// Gradients of groups with several sums: added in order.
+template <typename T>
+struct JoinPass {
+    struct { int comps; long long size; const T* part; T* grad; } degree[kMaxDegrees];
+    int chunk; const int* offsets;
+};
+template <typename T>
+__global__ void __launch_bounds__(256) grouped_join_kernel(const __grid_constant__ JoinPass<T> pass) {
+    const auto& d = pass.degree[blockIdx.z];
+    __shared__ int first, sums;
+    const int g = blockIdx.x;
+    auto sums_of = [&](int q) { return static_cast<int>((static_cast<long long>(pass.offsets[q + 1] - pass.offsets[q]) * d.comps + pass.chunk - 1) / pass.chunk); };
+    if (threadIdx.x < 32) {
+        int before = 0;
+        for (int q = threadIdx.x; q < g; q += 32) {
+            const int n = sums_of(q);
+            before += n > 1 ? n : 0;
+        }
+        before = __reduce_add_sync(0xffffffffu, before);
+        if (threadIdx.x == 0) { first = before; sums = sums_of(g); }
+    }
+    __syncthreads();
+    const int n = sums;
+    if (n <= 1) return;
+    for (long long i = blockIdx.y * 256LL + threadIdx.x; i < d.size; i += 256LL * gridDim.y) {
+        const T* part = d.part + first * d.size + i;
+        T s = T(0);
+        for (int c = 0; c < n; c += 8) {                                 // eight loads in flight, added in order
+            T v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v[u] = c + u < n ? part[(c + u) * d.size] : T(0);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) s += v[u];
+        }
+        d.grad[g * d.size + i] = s;
+    }
+}
+template <typename T>
+void join(const smx_grouped_linear& c) {
+    JoinPass<T> p{};
+    const T* part = static_cast<const T*>(c.workspace);
+    long long most = 0;
+    bool split = false;
+    for (int q = 0; q < c.num_degrees; ++q) {
+        const smx_grouped_degree& g = c.degrees[q];
+        auto& d = p.degree[q];
+        d.comps = g.components;
+        d.size = static_cast<long long>(g.in_channels) * g.out_channels;
+        d.part = part;
+        d.grad = static_cast<T*>(g.grad_weight);
+        part += part_values(c, q);
+        split = split || part_values(c, q) > 0;
+        most = std::max(most, d.size);
+    }
+    if (!split) return;
+    p.chunk = grad_chunk(c); p.offsets = c.offsets;
+    grouped_join_kernel<T><<<dim3(c.num_groups, static_cast<unsigned>(std::min(64LL, (most + 255) / 256)), c.num_degrees), 256, 0,
+                             static_cast<cudaStream_t>(c.stream)>>>(p);
+    launched("grouped_join_kernel");
 }
 
 template <int kMode, bool kWide>
@@ -267,56 +218,101 @@ void gradient_f32(const smx_grouped_linear& c) {
     p.b = static_cast<const float*>(c.grad_y); p.b_stride = c.grad_y_stride;
     p.chunk = grad_chunk(c);
     float* part = static_cast<float*>(c.workspace);
-    long long tiles = 0, most = 0;
-    bool wide = true, split = false;
+    long long tiles = 0;
+    bool wide = true;
     for (int q = 0; q < p.degrees; ++q) {
         GsDegree& d = p.degree[q];
         d.grad = static_cast<float*>(c.degrees[q].grad_weight);
         d.part = part;
         part += part_values(c, q);
-        split = split || part_values(c, q) > 0;
         tiles += (c.num_rows * d.comps / p.chunk + c.num_groups) * ((d.N + 127) / 128) * ((d.K + 127) / 128);
-        most = std::max(most, static_cast<long long>(d.K) * d.N);
         wide = wide && d.N % 64 == 0 && (reinterpret_cast<uintptr_t>(d.grad) & 31) == 0;
     }
     if (tiles > INT_MAX) throw ArgError("smx_grouped: too many rows");
     const cudaStream_t stream = static_cast<cudaStream_t>(c.stream);
     if (wide) launch_gs<kGsGradient, true>(p, tiles, stream);
     else launch_gs<kGsGradient, false>(p, tiles, stream);
-    if (!split) return;
-    grouped_join_kernel<<<dim3(c.num_groups, static_cast<unsigned>(std::min(64LL, (most + 255) / 256)), c.num_degrees), 256, 0, stream>>>(p);
-    launched("grouped_join_kernel");
+    join<float>(c);
+}
+
+// float64: tiles of 64 x 64, or of 16 x 32 while those leave SMs idle.
+template <int kMode, int BM, int BN, int WM, int WN, int ST>
+void launch_gd(const GdPass& p, long long tiles, cudaStream_t stream) {
+    using L = GdLayout<kMode, BM, BN, ST>;
+    if (tiles > INT_MAX) throw ArgError("smx_grouped: too many rows");
+    const auto kernel = grouped_f64_kernel<kMode, BM, BN, WM, WN, ST>;
+    static std::atomic<bool> done[64];
+    if (first_on_device(done)) {
+        SMX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::smem));
+        mark_on_device(done);
+    }
+    kernel<<<static_cast<unsigned>(tiles), kGdThreads, L::smem, stream>>>(p);
+    launched("grouped_f64_kernel");
+}
+template <int kMode>
+void launch_gd(const GdPass& p, cudaStream_t stream) {
+    auto tiles = [&](int BM, int BN) {
+        long long n = 0;
+        for (int q = 0; q < p.degrees; ++q) {
+            const GdDegree& d = p.degree[q];
+            if (kMode == kGsGradient) n += (p.rows * d.comps / p.chunk + p.groups) * ((d.K + BM - 1) / BM) * ((d.N + BN - 1) / BN);
+            else n += (p.rows * d.comps / BM + p.groups) * ((d.N + BN - 1) / BN);
+        }
+        return n;
+    };
+    if (tiles(64, 64) > 2LL * sm_count()) launch_gd<kMode, 64, 64, 2, 2, 3>(p, tiles(64, 64), stream);
+    else launch_gd<kMode, 16, 32, 1, 4, 4>(p, tiles(16, 32), stream);
+}
+
+GdPass gd_pass(const smx_grouped_linear& c, bool transposed) {
+    GdPass p{};
+    long long in_off = 0, out_off = 0;
+    for (int q = 0; q < c.num_degrees; ++q) {
+        const smx_grouped_degree& g = c.degrees[q];
+        GdDegree& d = p.degree[q];
+        d.comps = g.components;
+        d.K = transposed ? g.out_channels : g.in_channels;
+        d.N = transposed ? g.in_channels : g.out_channels;
+        d.a_off = in_off; d.b_off = out_off;
+        d.w = static_cast<const double*>(g.weight);
+        in_off += static_cast<long long>(d.comps) * d.K;
+        out_off += static_cast<long long>(d.comps) * d.N;
+    }
+    p.degrees = c.num_degrees; p.groups = c.num_groups; p.rows = c.num_rows; p.offsets = c.offsets;
+    p.out_width = static_cast<int>(out_off);
+    return p;
+}
+
+void rows_f64(const smx_grouped_linear& c, bool transposed) {
+    GdPass p = gd_pass(c, transposed);
+    p.a = static_cast<const double*>(transposed ? c.grad_y : c.x); p.a_stride = transposed ? c.grad_y_stride : c.x_stride;
+    p.out = static_cast<double*>(transposed ? c.grad_x : c.y); p.out_stride = transposed ? c.grad_x_stride : c.y_stride;
+    p.zero_tail = transposed || c.zero_tail;
+    if (transposed) launch_gd<kGsBackward>(p, static_cast<cudaStream_t>(c.stream));
+    else launch_gd<kGsForward>(p, static_cast<cudaStream_t>(c.stream));
+}
+
+void gradient_f64(const smx_grouped_linear& c) {
+    GdPass p = gd_pass(c, false);
+    p.a = static_cast<const double*>(c.x); p.a_stride = c.x_stride;
+    p.b = static_cast<const double*>(c.grad_y); p.b_stride = c.grad_y_stride;
+    p.chunk = grad_chunk(c);
+    double* part = static_cast<double*>(c.workspace);
+    for (int q = 0; q < p.degrees; ++q) {
+        GdDegree& d = p.degree[q];
+        d.grad = static_cast<double*>(c.degrees[q].grad_weight);
+        d.part = part;
+        part += part_values(c, q);
+    }
+    launch_gd<kGsGradient>(p, static_cast<cudaStream_t>(c.stream));
+    join<double>(c);
 }
 
 template <typename T>
 void rows_pass(const smx_grouped_linear& c, bool transposed) {
     if (c.num_rows == 0) return;
-    if (sizeof(T) == 4) return rows_f32(c, transposed);
-    RowsPass<T> p{};
-    long long in_off = 0, out_off = 0, tiles = 0;
-    for (int q = 0; q < c.num_degrees; ++q) {
-        const smx_grouped_degree& g = c.degrees[q];
-        RowsDegree<T>& d = p.degree[q];
-        d.comps = g.components;
-        d.K = transposed ? g.out_channels : g.in_channels;
-        d.N = transposed ? g.in_channels : g.out_channels;
-        d.in_off = in_off; d.out_off = out_off;
-        d.w = static_cast<const T*>(g.weight);
-        d.w_group = static_cast<long long>(g.in_channels) * g.out_channels;
-        d.w_k = transposed ? 1 : g.out_channels;
-        d.w_n = transposed ? g.out_channels : 1;
-        in_off += static_cast<long long>(d.comps) * d.K;
-        out_off += static_cast<long long>(d.comps) * d.N;
-        tiles += (c.num_rows * d.comps / kTile + c.num_groups) * ((d.N + kTile - 1) / kTile);
-    }
-    p.degrees = c.num_degrees; p.groups = c.num_groups; p.rows = c.num_rows; p.offsets = c.offsets;
-    p.in = static_cast<const T*>(transposed ? c.grad_y : c.x); p.in_stride = transposed ? c.grad_y_stride : c.x_stride;
-    p.out = static_cast<T*>(transposed ? c.grad_x : c.y); p.out_stride = transposed ? c.grad_x_stride : c.y_stride;
-    p.zero_tail = transposed || c.zero_tail;
-    p.out_width = static_cast<int>(out_off);
-    if (tiles > INT_MAX) throw ArgError("smx_grouped: too many rows");
-    grouped_rows_kernel<T><<<static_cast<unsigned>(tiles), 256, 0, static_cast<cudaStream_t>(c.stream)>>>(p);
-    launched("grouped_rows_kernel");
+    if (sizeof(T) == 4) rows_f32(c, transposed);
+    else rows_f64(c, transposed);
 }
 
 template <typename T>
@@ -350,31 +346,18 @@ void backward(const smx_grouped_linear& c) {
     }
     if (c.grad_x) rows_pass<T>(c, true);
     if (!matrices) return;
-    if (sizeof(T) == 4) return gradient_f32(c);
-    GradPass<T> p{};
-    long long x_off = 0, y_off = 0;
-    for (int q = 0; q < c.num_degrees; ++q) {
-        const smx_grouped_degree& g = c.degrees[q];
-        GradDegree<T>& d = p.degree[q];
-        d.comps = g.components; d.K = g.in_channels; d.N = g.out_channels; d.x_off = x_off; d.y_off = y_off;
-        d.grad = static_cast<T*>(g.grad_weight);
-        x_off += static_cast<long long>(d.comps) * d.K;
-        y_off += static_cast<long long>(d.comps) * d.N;
-    }
-    p.groups = c.num_groups; p.offsets = c.offsets;
-    p.x = static_cast<const T*>(c.x); p.x_stride = c.x_stride; p.gy = static_cast<const T*>(c.grad_y); p.gy_stride = c.grad_y_stride;
-    grouped_grad_kernel<T><<<dim3(c.num_groups, 64, c.num_degrees), 256, 0, static_cast<cudaStream_t>(c.stream)>>>(p);
-    launched("grouped_grad_kernel");
+    if (sizeof(T) == 4) gradient_f32(c);
+    else gradient_f64(c);
 }
 
 }  // namespace
 
 size_t grouped_workspace_bytes(const smx_grouped_linear& c, bool backward) {
     check_call(c);
-    if (!backward || c.precision == SMX_FP64) return 0;
+    if (!backward) return 0;
     size_t values = 0;
     for (int d = 0; d < c.num_degrees; ++d) values += part_values(c, d);
-    return values * sizeof(float);
+    return values * (c.precision == SMX_FP32 ? sizeof(float) : sizeof(double));
 }
 void grouped_forward(const smx_grouped_linear& c) {
     check_plan(c);

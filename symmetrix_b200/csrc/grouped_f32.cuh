@@ -680,37 +680,5 @@ __global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid
     if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
-// Gradients of groups with several chunks of rows: their partial sums added in order.
-__global__ void __launch_bounds__(256) grouped_join_kernel(const __grid_constant__ GsPass pass) {
-    const GsDegree& d = pass.degree[blockIdx.z];
-    __shared__ int first, chunks;
-    const int g = blockIdx.x;
-    if (threadIdx.x < 32) {
-        int before = 0;
-        for (int q = threadIdx.x; q < g; q += 32) {
-            const int n = gs_runs<kGsGradient>(pass, d, pass.offsets[q + 1] - pass.offsets[q]);
-            before += n > 1 ? n : 0;
-        }
-        before = __reduce_add_sync(0xffffffffu, before);
-        if (threadIdx.x == 0) { first = before; chunks = gs_runs<kGsGradient>(pass, d, pass.offsets[g + 1] - pass.offsets[g]); }
-    }
-    __syncthreads();
-    const int n = chunks;
-    if (n == 1) return;
-    const long long size = static_cast<long long>(d.K) * d.N;
-    for (long long i = blockIdx.y * 256LL + threadIdx.x; i < size; i += 256LL * gridDim.y) {
-        const float* part = d.part + first * size + i;
-        float s = 0.f;
-        for (int c = 0; c < n; c += 8) {                                 // eight loads in flight, added in order
-            float v[8];
-#pragma unroll
-            for (int u = 0; u < 8; ++u) v[u] = c + u < n ? part[(c + u) * size] : 0.f;
-#pragma unroll
-            for (int u = 0; u < 8; ++u) s += v[u];
-        }
-        d.grad[g * size + i] = s;
-    }
-}
-
 }  // namespace
 }  // namespace smx
