@@ -5,6 +5,8 @@
 //   gradient   D = rows of grad_W   A = x^T (inner: rows)         B = grad_y (inner: rows)
 #pragma once
 
+#include <type_traits>
+
 #include "gemm_tcgen05.cuh"
 
 namespace smx {
@@ -47,7 +49,7 @@ struct GdLayout {
 };
 
 // The tile-th tile of a pass: degrees, groups, row tiles or sums, then blocks of D. Called by a warp.
-struct GdWork { int degree, group, block, mtile, rows, inner, runs, part; long long first_pair, row0; };
+struct GdWork { int degree, group, block, mtile, rows, inner, runs, part, comp0; long long first_pair, row0; };   // gradient: from first_pair, comp0 on
 template <int kMode>
 __device__ __forceinline__ bool gd_find(const GdPass& p, int BM, int BN, long long tile, GdWork& w) {
     const int lane = threadIdx.x & 31;
@@ -87,6 +89,8 @@ __device__ __forceinline__ bool gd_find(const GdPass& p, int BM, int BN, long lo
                 const long long left = rows - w.row0;
                 if (kMode == kGsGradient) {
                     w.inner = static_cast<int>(min(static_cast<long long>(p.chunk), left));
+                    w.first_pair += w.row0 / d.comps;
+                    w.comp0 = static_cast<int>(w.row0 % d.comps);
                     w.rows = min(BM, d.K - BM * w.mtile);
                 } else {
                     w.inner = d.K;
@@ -141,48 +145,50 @@ __global__ void __launch_bounds__(kGdThreads) grouped_f64_kernel(const __grid_co
     const bool wide_a = ((pass.a_stride | d.a_off | d.K) & 1) == 0 && (reinterpret_cast<uintptr_t>(pass.a) & 15) == 0;
     const bool wide_b = kMode == kGsGradient ? ((pass.b_stride | d.b_off | d.N) & 1) == 0 && (reinterpret_cast<uintptr_t>(pass.b) & 15) == 0
                                              : ((kMode == kGsForward ? d.N : d.K) & 1) == 0 && (reinterpret_cast<uintptr_t>(d.w) & 15) == 0;
-    // where inner value k of the gradient's operands begins
+    // Where inner value k of the gradient's operands begins. (comp0 + k lies below 2^13, where the quotient by a reciprocal is exact.)
+    const float reciprocal = 1.f / d.comps;
     auto inner_row = [&](int k, long long stride, int width) {
-        const long long r = work.row0 + k, ahead = r / d.comps;
-        return (work.first_pair + ahead) * stride + (r - ahead * d.comps) * width;
+        const int r = work.comp0 + k, ahead = __float2int_rd((r + 0.5f) * reciprocal);
+        return (work.first_pair + ahead) * stride + static_cast<long long>(r - ahead * d.comps) * width;
     };
     auto issue = [&](int chunk) {
         double* const As = gd_smem + (chunk % ST) * L::stage;
         double* const Bs = As + TA::doubles;
         const int k0 = chunk * kGdStep;
-        auto copy = [&](double* to, const double* base, long long from, bool in, bool wide) {
-            if (wide) cp_async16(to, base + (in ? from : 0), in ? 16 : 0);
-            else gd_copy8(to, base + (in ? from : 0), in ? 8 : 0);
+        auto copies = [&](bool wide, auto&& fn) {        // fn(values of a copy, copy to, from, offset, whether there is anything)
+            if (wide) fn(std::integral_constant<int, 2>{}, [](double* to, const double* base, long long from, bool in) { cp_async16(to, base + (in ? from : 0), in ? 16 : 0); });
+            else fn(std::integral_constant<int, 1>{}, [](double* to, const double* base, long long from, bool in) { gd_copy8(to, base + (in ? from : 0), in ? 8 : 0); });
         };
-        if constexpr (kRows) {
-            const int per = wide_a ? 2 : 1, n = kGdStep / per;
-            for (int i = tid; i < BM * n; i += kGdThreads) {
-                const int r = i / n, k = (i % n) * per;
-                copy(As + TA::at(r, k), pass.a, a_base[r] + k0 + k, a_base[r] >= 0 && k0 + k < inner, wide_a);
+        copies(wide_a, [&](auto values, auto copy) {
+            constexpr int per = decltype(values)::value, n = (kRows ? kGdStep : BM) / per;
+            const int m0 = BM * work.mtile;
+#pragma unroll 4
+            for (int i = tid; i < BM * kGdStep / per; i += kGdThreads) {
+                if constexpr (kRows) {
+                    const int r = i / n, k = (i % n) * per;
+                    copy(As + TA::at(r, k), pass.a, a_base[r] + k0 + k, a_base[r] >= 0 && k0 + k < inner);
+                } else {
+                    const int k = i / n, c = (i % n) * per;
+                    const bool in = k0 + k < inner && m0 + c < d.K;
+                    copy(As + TA::at(c, k), pass.a, inner_row(k0 + k, pass.a_stride, d.K) + d.a_off + m0 + c, in);
+                }
             }
-        } else {
-            const int per = wide_a ? 2 : 1, n = BM / per, m0 = BM * work.mtile;
-            for (int i = tid; i < kGdStep * n; i += kGdThreads) {
-                const int k = i / n, c = (i % n) * per;
-                const bool in = k0 + k < inner && m0 + c < d.K;
-                copy(As + TA::at(c, k), pass.a, in ? inner_row(k0 + k, pass.a_stride, d.K) + d.a_off + m0 + c : 0, in, wide_a);
+        });
+        copies(wide_b, [&](auto values, auto copy) {
+            constexpr int per = decltype(values)::value, n = (kMode == kGsBackward ? kGdStep : BN) / per;
+#pragma unroll 4
+            for (int i = tid; i < BN * kGdStep / per; i += kGdThreads) {
+                if constexpr (kMode == kGsBackward) {
+                    const int c = i / n, k = (i % n) * per;
+                    copy(Bs + TB::at(c, k), matrix, static_cast<long long>(col0 + c) * d.K + k0 + k, c < cols && k0 + k < inner);
+                } else {
+                    const int k = i / n, c = (i % n) * per;
+                    const bool in = k0 + k < inner && c < cols;
+                    if constexpr (kMode == kGsForward) copy(Bs + TB::at(c, k), matrix, static_cast<long long>(k0 + k) * d.N + col0 + c, in);
+                    else copy(Bs + TB::at(c, k), pass.b, inner_row(k0 + k, pass.b_stride, d.N) + d.b_off + col0 + c, in);
+                }
             }
-        }
-        if constexpr (kMode == kGsBackward) {
-            const int per = wide_b ? 2 : 1, n = kGdStep / per;
-            for (int i = tid; i < BN * n; i += kGdThreads) {
-                const int c = i / n, k = (i % n) * per;
-                copy(Bs + TB::at(c, k), matrix, static_cast<long long>(col0 + c) * d.K + k0 + k, c < cols && k0 + k < inner, wide_b);
-            }
-        } else {
-            const int per = wide_b ? 2 : 1, n = BN / per;
-            for (int i = tid; i < kGdStep * n; i += kGdThreads) {
-                const int k = i / n, c = (i % n) * per;
-                const bool in = k0 + k < inner && c < cols;
-                if (kMode == kGsForward) copy(Bs + TB::at(c, k), matrix, static_cast<long long>(k0 + k) * d.N + col0 + c, in, wide_b);
-                else copy(Bs + TB::at(c, k), pass.b, in ? inner_row(k0 + k, pass.b_stride, d.N) + d.b_off + col0 + c : 0, in, wide_b);
-            }
-        }
+        });
     };
     const int chunks = (inner + kGdStep - 1) / kGdStep;
 #pragma unroll
