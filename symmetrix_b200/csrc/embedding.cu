@@ -29,92 +29,168 @@ union Lanes {
     T t[n];
 };
 
-__global__ void __launch_bounds__(256) embedding_tokens_kernel(const int* __restrict__ ids, const int* __restrict__ order, long long pairs, int table_rows,
-                                                               int* __restrict__ tokens) {
-    for (long long p = blockIdx.x * 256LL + threadIdx.x; p < pairs; p += 256LL * gridDim.x) {
-        const int t = ids[order[p]];
-        tokens[p] = t < 0 || t >= table_rows ? table_rows : t;
-    }
-}
-
+// blockDim.x threads (up to a warp) along a row, blockDim.y rows at a time; a thread has kAhead units of its row in flight, so that the wait for the id is
+// shared among them, and the next row's id is read ahead. 98,304 rows of 512 floats: 39 us for 201 MB, 5.2 TB/s; 57 with a thread for every unit of 16 bytes, since
+// an id and a weight then are read with each. The reads of the table come from L2 and are as many as the writes.
+constexpr int kAhead = 4;
 template <typename T, typename V>
 __global__ void __launch_bounds__(256) embedding_forward_kernel(const V* __restrict__ table, long long table_stride, int table_rows, const int* __restrict__ ids,
                                                                 long long num_rows, int slots, int units, const T* __restrict__ weights, T scale,
                                                                 V* __restrict__ y, long long y_stride) {
     using L = Lanes<T, V>;
-    for (long long n = static_cast<long long>(blockIdx.x) * blockDim.y + threadIdx.y; n < num_rows; n += static_cast<long long>(gridDim.x) * blockDim.y) {
-        for (int u = threadIdx.x; u < units; u += blockDim.x) {
-            L sum{};
+    const int tx = blockDim.x;
+    const long long step = static_cast<long long>(gridDim.x) * blockDim.y;
+    long long n = static_cast<long long>(blockIdx.x) * blockDim.y + threadIdx.y;
+    int next = n < num_rows ? ids[n * slots] : -1;                       // the first slot's id, read a row ahead
+    for (; n < num_rows; n += step) {
+        const int first = next;
+        if (n + step < num_rows) next = ids[(n + step) * slots];
+        for (int u = threadIdx.x; u < units; u += kAhead * tx) {
+            L sum[kAhead] = {};
             for (int s = 0; s < slots; ++s) {
-                const int t = ids[n * slots + s];
+                const int t = s == 0 ? first : ids[n * slots + s];
                 if (t < 0 || t >= table_rows) continue;
                 const T w = weights ? scale * weights[n * slots + s] : scale;
-                L r;
-                r.v = table[t * table_stride + u];
+                const V* row = table + t * table_stride + u;
+                L r[kAhead];
 #pragma unroll
-                for (int q = 0; q < L::n; ++q) sum.t[q] += w * r.t[q];
+                for (int a = 0; a < kAhead; ++a) {
+                    r[a].v = V{};
+                    if (u + a * tx < units) r[a].v = row[a * tx];
+                }
+#pragma unroll
+                for (int a = 0; a < kAhead; ++a)
+#pragma unroll
+                    for (int q = 0; q < L::n; ++q) sum[a].t[q] += w * r[a].t[q];
             }
-            y[n * y_stride + u] = sum.v;
+#pragma unroll
+            for (int a = 0; a < kAhead; ++a)
+                if (u + a * tx < units) y[n * y_stride + u + a * tx] = sum[a].v;
         }
     }
 }
 
 // Sums of the runs of a chunk of sorted pairs, kGradThreads units of a row a CTA. parts: [chunk][2][units]: the run that an earlier chunk began, and the
-// run that goes on in the next one.
-constexpr int kGradThreads = 128, kMaxChunk = 512;
-template <typename T, typename V>
-__global__ void __launch_bounds__(kGradThreads) embedding_grad_kernel(const V* __restrict__ grad_y, long long grad_y_stride, const int* __restrict__ order,
-                                                                      const int* __restrict__ tokens, long long pairs, int slots, int table_rows, int units,
-                                                                      const T* __restrict__ weights, T scale, int chunk, V* __restrict__ grad_table,
-                                                                      V* __restrict__ parts) {
+// run that goes on in the next one. kWeights: the weights' gradients too, since a run's row of the table then is read once (49,152 rows of 512 floats, two
+// slots, 1,424 tokens, all of the backward pass: 64 us; 79 with the weights row by row in a kernel of their own). Their sums over the units of a CTA go to `dots` [slab][pairs], or straight
+// to the gradient where one CTA has the whole row.
+constexpr int kGradThreads = 128, kMaxChunk = 512, kLoads = 8, kRows = 4;
+template <typename T, typename V, bool kWeights>
+__global__ void __launch_bounds__(kGradThreads, sizeof(T) == 4 ? 8 : 5) embedding_grad_kernel(const V* __restrict__ grad_y, long long grad_y_stride, const V* __restrict__ table,
+                                                                      long long table_stride, const int* __restrict__ order, const int* __restrict__ tokens,
+                                                                      long long pairs, int slots, int table_rows, int units, const T* __restrict__ weights, T scale,
+                                                                      int chunk, V* __restrict__ grad_table, V* __restrict__ parts, T* __restrict__ dots,
+                                                                      T* __restrict__ grad_weights) {
     using L = Lanes<T, V>;
-    constexpr int kAhead = 8;
+    constexpr int kWarps = kGradThreads / 32;
     __shared__ long long row[kMaxChunk];
     __shared__ T weight[kMaxChunk];
     __shared__ int token[kMaxChunk + 2];                                 // with the neighbours
+    __shared__ T warp_dot[kWeights ? kWarps : 1][kWeights ? kMaxChunk : 1];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // the joining kernel comes in as CTAs of this one end
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const long long begin = static_cast<long long>(blockIdx.x) * chunk;
     const int count = static_cast<int>(min(static_cast<long long>(chunk), pairs - begin));
-    for (int i = threadIdx.x; i < count + 2; i += kGradThreads) {
+    int live = 0;                                                        // pairs without a token come last
+    for (int i0 = 0; i0 < count + 2; i0 += kGradThreads) {
+        const int i = i0 + threadIdx.x;
         const long long p = begin + i - 1;
-        token[i] = p >= 0 && p < pairs ? tokens[p] : -1;
-        if (i >= 1 && i <= count) {
+        const int t = i < count + 2 && p >= 0 && p < pairs ? tokens[p] : -1;
+        if (i < count + 2) token[i] = t;
+        const bool in = i >= 1 && i <= count && t < table_rows;
+        if (in) {
             const int pair = order[p];
             row[i - 1] = pair / slots * grad_y_stride;
             weight[i - 1] = weights ? scale * weights[pair] : scale;
         }
+        live += __syncthreads_count(in);
     }
-    __syncthreads();
     const int u = blockIdx.y * kGradThreads + threadIdx.x;
-    if (u >= units) return;
-    L sum{};
-    int from = 0;                                                        // where the run at hand began
-    for (int i0 = 0; i0 < count; i0 += kAhead) {
-        L g[kAhead];
+    const bool mine = u < units;
+    L sum{}, last{};                                                     // the run at hand; the row of the table of the pair before
+    int from = 0, last_token = -1;                                       // where the run began
+    for (int i0 = 0; i0 < live; i0 += kLoads) {
+        L g[kLoads];
 #pragma unroll
-        for (int q = 0; q < kAhead; ++q) {
+        for (int q = 0; q < kLoads; ++q) {
             g[q].v = V{};
-            if (i0 + q < count && token[i0 + q + 1] < table_rows) g[q].v = grad_y[row[i0 + q] + u];
+            if (mine && i0 + q < live) g[q].v = grad_y[row[i0 + q] + u];
         }
+        if constexpr (kWeights) {
+            T d[kLoads];
 #pragma unroll
-        for (int q = 0; q < kAhead; ++q) {
+            for (int q0 = 0; q0 < kLoads; q0 += kRows) {
+                L r[kRows];                                              // read where the token changes
+#pragma unroll
+                for (int q = 0; q < kRows; ++q) {
+                    const int i = i0 + q0 + q, t = i < live ? token[i + 1] : last_token;
+                    if (t != last_token && mine) last.v = table[t * table_stride + u];
+                    last_token = t;
+                    r[q] = last;
+                }
+#pragma unroll
+                for (int q = 0; q < kRows; ++q) {
+                    d[q0 + q] = T(0);
+#pragma unroll
+                    for (int e = 0; e < L::n; ++e) d[q0 + q] += g[q0 + q].t[e] * r[q].t[e];
+                }
+            }
+            // eight sums over the warp at once: every step halves the values that a lane carries on
+#pragma unroll
+            for (int h = kLoads / 2, m = 16; h >= 1; h /= 2, m /= 2)
+#pragma unroll
+                for (int q = 0; q < h; ++q) {
+                    const bool upper = lane & m;
+                    const T keep = upper ? d[q + h] : d[q], send = upper ? d[q] : d[q + h];
+                    d[q] = keep + __shfl_xor_sync(0xffffffffu, send, m);
+                }
+            d[0] += __shfl_xor_sync(0xffffffffu, d[0], 2);
+            d[0] += __shfl_xor_sync(0xffffffffu, d[0], 1);
+            const int i = i0 + (lane >> 2);                              // of the three uppermost bits of the lane's number
+            if ((lane & 3) == 0 && i < live) warp_dot[warp][i] = d[0];
+        }
+        if (!grad_table) continue;
+#pragma unroll
+        for (int q = 0; q < kLoads; ++q) {
             const int i = i0 + q;
-            if (i >= count) break;
+            if (i >= live) break;
             const int t = token[i + 1];
-            if (t >= table_rows) return;                                 // pairs without a token come last
             const T w = weight[i];
 #pragma unroll
             for (int e = 0; e < L::n; ++e) sum.t[e] += w * g[q].t[e];
             if (token[i + 2] == t && i + 1 < count) continue;
             const bool began = from > 0 || token[0] != t, ends = token[i + 2] != t;
-            if (began && ends) grad_table[static_cast<long long>(t) * units + u] = sum.v;
-            else parts[(2LL * blockIdx.x + (began ? 1 : 0)) * units + u] = sum.v;
+            if (mine) {
+                if (began && ends) grad_table[static_cast<long long>(t) * units + u] = sum.v;
+                else parts[(2LL * blockIdx.x + (began ? 1 : 0)) * units + u] = sum.v;
+            }
             sum = L{};
             from = i + 1;
         }
     }
+    if constexpr (kWeights) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < count; i += kGradThreads) {
+            T s = T(0);
+            if (i < live)
+                for (int w = 0; w < kWarps; ++w) s += warp_dot[w][i];
+            const int pair = order[begin + i];
+            if (gridDim.y == 1) grad_weights[pair] = scale * s;
+            else dots[blockIdx.y * pairs + pair] = s;
+        }
+    }
+}
+template <typename T>
+__global__ void __launch_bounds__(256) embedding_dots_kernel(const T* __restrict__ dots, long long pairs, int slabs, T scale, T* __restrict__ grad_weights) {
+    for (long long i = blockIdx.x * 256LL + threadIdx.x; i < pairs; i += 256LL * gridDim.x) {
+        T s = T(0);
+        for (int q = 0; q < slabs; ++q) s += dots[q * pairs + i];
+        grad_weights[i] = scale * s;
+    }
 }
 
-// The runs that cross chunks: the CTAs of the chunk where one begins add its parts in order, four of them side by side.
+// The runs that cross chunks: the CTAs of the chunk where one begins add its parts in order, kJoinWays of them side by side. Most CTAs have none; they
+// see that from the tokens, before the sums are there.
 constexpr int kJoinUnits = 32, kJoinWays = 8;
 template <typename T, typename V>
 __global__ void __launch_bounds__(kJoinUnits * kJoinWays) embedding_join_kernel(const int* __restrict__ tokens, long long pairs, int table_rows, int units, int chunk,
@@ -122,9 +198,16 @@ __global__ void __launch_bounds__(kJoinUnits * kJoinWays) embedding_join_kernel(
     using L = Lanes<T, V>;
     __shared__ V joined[kJoinWays][kJoinUnits];
     const long long begin = static_cast<long long>(blockIdx.x) * chunk, end = begin + chunk;
-    if (end >= pairs) return;
-    const int t = tokens[end - 1];
-    if (t >= table_rows || tokens[end] != t || (begin > 0 && tokens[begin - 1] == t)) return;      // no run, or not its beginning
+    int t = table_rows, after = -1, before = -1;
+    if (end < pairs) {
+        t = tokens[end - 1];
+        after = tokens[end];
+        if (begin > 0) before = tokens[begin - 1];
+    }
+    const bool mine = t < table_rows && after == t && before != t;       // a run, and its beginning
+    // (one CTA waits in any case, so that this kernel does not end before the one whose sums it reads)
+    if (mine || (blockIdx.x == 0 && blockIdx.y == 0)) asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (!mine) return;
     int more = 0;                                                        // chunks that go on with it
     for (int c0 = blockIdx.x + 1;; c0 += kJoinUnits * kJoinWays) {
         const int c = c0 + threadIdx.x;
@@ -159,31 +242,6 @@ __global__ void __launch_bounds__(kJoinUnits * kJoinWays) embedding_join_kernel(
         for (int e = 0; e < L::n; ++e) sum.t[e] += v.t[e];
     }
     grad_table[static_cast<long long>(t) * units + u] = sum.v;
-}
-
-// grad_w: a warp per pair, in sorted order (the table's rows then come from the cache).
-template <typename T, typename V>
-__global__ void __launch_bounds__(256) embedding_weight_grad_kernel(const V* __restrict__ grad_y, long long grad_y_stride, const V* __restrict__ table,
-                                                                    long long table_stride, int table_rows, const int* __restrict__ order,
-                                                                    const int* __restrict__ tokens, long long pairs, int slots, int units, T scale,
-                                                                    T* __restrict__ grad_weights) {
-    using L = Lanes<T, V>;
-    const int lane = threadIdx.x & 31;
-    for (long long p = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) >> 5; p < pairs; p += static_cast<long long>(gridDim.x) * 8) {
-        const int pair = order[p], t = tokens[p];
-        T dot = T(0);
-        if (t < table_rows)
-            for (int u = lane; u < units; u += 32) {
-                L g, r;
-                g.v = grad_y[pair / slots * grad_y_stride + u];
-                r.v = table[t * table_stride + u];
-#pragma unroll
-                for (int e = 0; e < L::n; ++e) dot += g.t[e] * r.t[e];
-            }
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
-        if (lane == 0) grad_weights[pair] = scale * dot;
-    }
 }
 
 // ------------------------------------------------------------------------------------------- host side
@@ -231,9 +289,7 @@ void embedding_plan(const int* ids, long num_rows, int slots, int table_rows, in
     if (!ids || !order || !tokens) throw ArgError("smx_embedding_plan: null pointer");
     check_pointers("smx_embedding_plan", sizeof(int), {ids, order, tokens, workspace});
     if (workspace_bytes < need || (need && !workspace)) throw ArgError("smx_embedding_plan: the workspace is smaller than smx_embedding_plan_bytes says");
-    token_sort(ids, pairs, table_rows, order, workspace, stream);
-    embedding_tokens_kernel<<<static_cast<unsigned>(std::min<long>((pairs + 255) / 256, 8L * sm_count())), 256, 0, stream>>>(ids, order, pairs, table_rows, tokens);
-    launched("embedding_tokens_kernel");
+    token_sort(ids, pairs, table_rows, order, tokens, workspace, stream);
 }
 
 template <typename T>
@@ -250,10 +306,10 @@ void embedding_forward(const T* table, long table_stride, int table_rows, const 
     by_unit<T>(wide_rows<T>({table, y}, {table_stride, y_stride, width}), [&](auto unit) {
         using V = decltype(unit);
         constexpr long per = sizeof(V) / sizeof(T);
-        unsigned tx = 32;
-        while (tx < 256 && tx < width / per) tx *= 2;
+        unsigned tx = 1;
+        while (tx < 32 && kAhead * tx < width / per) tx *= 2;
         const unsigned ty = 256 / tx;
-        const unsigned blocks = static_cast<unsigned>(std::min<long long>((num_rows + ty - 1) / ty, 64LL * sm_count()));
+        const unsigned blocks = static_cast<unsigned>(std::min<long long>((num_rows + ty - 1) / ty, 8LL * sm_count()));
         embedding_forward_kernel<T, V><<<blocks, dim3(tx, ty), 0, stream>>>(reinterpret_cast<const V*>(table), table_stride / per, table_rows, ids, num_rows, slots,
                                                                             static_cast<int>(width / per), weights, static_cast<T>(scale), reinterpret_cast<V*>(y),
                                                                             y_stride / per);
@@ -261,12 +317,20 @@ void embedding_forward(const T* table, long table_stride, int table_rows, const 
     launched("embedding_forward_kernel");
 }
 
+namespace {
+// Workspace: the parts of runs that cross chunks, and the dots of rows that several CTAs share (single values, if rows start anywhere).
+struct Room { size_t parts, dots; };
+template <typename T>
+Room room(long pairs, long width) {
+    const long chunks = pairs > 0 ? (pairs + grad_chunk(pairs) - 1) / grad_chunk(pairs) : 0, slabs = (width + kGradThreads - 1) / kGradThreads;
+    return {(static_cast<size_t>(chunks) * 2 * width * sizeof(T) + 255) / 256 * 256, slabs > 1 ? static_cast<size_t>(slabs) * pairs * sizeof(T) : 0};
+}
+}  // namespace
 template <typename T>
 size_t embedding_backward_bytes(long num_rows, int slots, long width) {
     check_sizes("smx_embedding_backward", num_rows, slots, 1, width);
-    const long pairs = num_rows * slots;
-    const long chunks = pairs > 0 ? (pairs + grad_chunk(pairs) - 1) / grad_chunk(pairs) : 0;
-    return static_cast<size_t>(chunks) * 2 * width * sizeof(T);
+    const Room r = room<T>(num_rows * slots, width);
+    return r.parts + r.dots;
 }
 template <typename T>
 void embedding_backward(const T* grad_y, long grad_y_stride, const T* table, long table_stride, int table_rows, const int* order, const int* tokens,
@@ -283,39 +347,39 @@ void embedding_backward(const T* grad_y, long grad_y_stride, const T* table, lon
         check_stride(what, table_stride, width, table_rows, false);
         if (pairs > 0 && width > 0 && !table) throw ArgError("smx_embedding_backward: the weights' gradient needs the table");
     }
-    if (grad_table) {
-        const size_t need = embedding_backward_bytes<T>(num_rows, slots, width);
-        if (workspace_bytes < need || (need && !workspace)) throw ArgError("smx_embedding_backward: the workspace is smaller than smx_embedding_backward_bytes says");
-        if (reinterpret_cast<uintptr_t>(workspace) & 15) throw ArgError("smx_embedding_backward: the workspace must start on a 16-byte boundary");
-        if (width > 65535L * kJoinUnits) throw ArgError("smx_embedding_backward: rows are too wide");
-    }
-    if (grad_weights && pairs > 0) {
-        by_unit<T>(wide_rows<T>({grad_y, table}, {grad_y_stride, table_stride, width}), [&](auto unit) {
-            using V = decltype(unit);
-            constexpr long per = sizeof(V) / sizeof(T);
-            embedding_weight_grad_kernel<T, V><<<static_cast<unsigned>(std::min<long long>((pairs + 7) / 8, 64LL * sm_count())), 256, 0, stream>>>(
-                reinterpret_cast<const V*>(grad_y), grad_y_stride / per, reinterpret_cast<const V*>(table), table_stride / per, table_rows, order, tokens, pairs, slots,
-                static_cast<int>(width / per), static_cast<T>(scale), grad_weights);
-        });
-        launched("embedding_weight_grad_kernel");
-    }
-    if (!grad_table || width == 0) return;
-    SMX_CUDA(cudaMemsetAsync(grad_table, 0, static_cast<size_t>(table_rows) * width * sizeof(T), stream));
+    if (!grad_table && !grad_weights) return;
+    const size_t need = embedding_backward_bytes<T>(num_rows, slots, width);
+    if (workspace_bytes < need || (need && !workspace)) throw ArgError("smx_embedding_backward: the workspace is smaller than smx_embedding_backward_bytes says");
+    if (reinterpret_cast<uintptr_t>(workspace) & 15) throw ArgError("smx_embedding_backward: the workspace must start on a 16-byte boundary");
+    if (width > 65535L * kJoinUnits) throw ArgError("smx_embedding_backward: rows are too wide");
+    if (grad_table && width > 0) SMX_CUDA(cudaMemsetAsync(grad_table, 0, static_cast<size_t>(table_rows) * width * sizeof(T), stream));
     if (pairs == 0) return;
+    if (width == 0) {
+        if (grad_weights) SMX_CUDA(cudaMemsetAsync(grad_weights, 0, static_cast<size_t>(pairs) * sizeof(T), stream));
+        return;
+    }
+    T* const dots = reinterpret_cast<T*>(static_cast<char*>(workspace) + room<T>(pairs, width).parts);
     const int chunk = grad_chunk(pairs), chunks = static_cast<int>((pairs + chunk - 1) / chunk);
-    by_unit<T>(wide_rows<T>({grad_y, grad_table}, {grad_y_stride, width}), [&](auto unit) {
+    by_unit<T>(wide_rows<T>({grad_y, grad_table, grad_weights ? table : nullptr}, {grad_y_stride, width, grad_weights ? table_stride : 0}), [&](auto unit) {
         using V = decltype(unit);
         constexpr long per = sizeof(V) / sizeof(T);
         const int units = static_cast<int>(width / per);
         const int slabs = (units + kGradThreads - 1) / kGradThreads, joins = (units + kJoinUnits - 1) / kJoinUnits;
-        embedding_grad_kernel<T, V><<<dim3(chunks, slabs), kGradThreads, 0, stream>>>(reinterpret_cast<const V*>(grad_y), grad_y_stride / per, order, tokens, pairs,
-                                                                                      slots, table_rows, units, weights, static_cast<T>(scale), chunk,
-                                                                                      reinterpret_cast<V*>(grad_table), static_cast<V*>(workspace));
+        const auto kernel = grad_weights ? embedding_grad_kernel<T, V, true> : embedding_grad_kernel<T, V, false>;
+        kernel<<<dim3(chunks, slabs), kGradThreads, 0, stream>>>(reinterpret_cast<const V*>(grad_y), grad_y_stride / per, reinterpret_cast<const V*>(table),
+                                                                 table_stride / per, order, tokens, pairs, slots, table_rows, units, weights, static_cast<T>(scale),
+                                                                 chunk, reinterpret_cast<V*>(grad_table), static_cast<V*>(workspace), dots, grad_weights);
         launched("embedding_grad_kernel");
-        if (chunks == 1) return;
-        embedding_join_kernel<T, V><<<dim3(chunks, joins), kJoinUnits * kJoinWays, 0, stream>>>(tokens, pairs, table_rows, units, chunk, chunks,
-                                                                                                static_cast<const V*>(workspace), reinterpret_cast<V*>(grad_table));
-        launched("embedding_join_kernel");
+        if (grad_table && chunks > 1) {
+            chain_launch(Launcher{stream, true}, embedding_join_kernel<T, V>, dim3(chunks, joins), kJoinUnits * kJoinWays, 0, 1, tokens,
+                         static_cast<long long>(pairs), table_rows, units, chunk, chunks, static_cast<const V*>(workspace), reinterpret_cast<V*>(grad_table));
+            ++operator_launches;
+        }
+        if (grad_weights && slabs > 1) {
+            embedding_dots_kernel<T><<<static_cast<unsigned>(std::min(8LL * sm_count(), (pairs + 255LL) / 256)), 256, 0, stream>>>(dots, pairs, slabs, static_cast<T>(scale),
+                                                                                                                                  grad_weights);
+            launched("embedding_dots_kernel");
+        }
     });
 }
 

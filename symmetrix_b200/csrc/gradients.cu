@@ -105,6 +105,7 @@ __device__ __forceinline__ double tile_squares(const T* from, int n, bool wide) 
 template <int N>
 __global__ void __launch_bounds__(kThreads) gradient_norm_kernel(const __grid_constant__ TensorList<N> list, double* __restrict__ partial) {
     __shared__ double shared[kThreads / 32];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // the scaling kernel comes in as CTAs of this one end
     double s = 0.0;
     for_tiles(list, false, [&](const Tensor& x, long long from, int n) {
         if (x.wide & 1) s += tile_squares(static_cast<const double*>(x.from) + from, n, (x.wide & 2) != 0);
@@ -124,7 +125,7 @@ __device__ __forceinline__ void tile_scale(const T* from, T* to, int n, bool wid
 #pragma unroll
         for (int q = 0; q < kUnits; ++q) {
             const int i = (q * kThreads + threadIdx.x) * per;
-            if (i + per <= n) u[q].v = *reinterpret_cast<const V*>(from + i);
+            if (i + per <= n) u[q].v = __ldcs(reinterpret_cast<const V*>(from + i));
         }
 #pragma unroll
         for (int q = 0; q < kUnits; ++q) {
@@ -132,7 +133,7 @@ __device__ __forceinline__ void tile_scale(const T* from, T* to, int n, bool wid
             if (i + per <= n) {
 #pragma unroll
                 for (int e = 0; e < per; ++e) u[q].t[e] = static_cast<T>(static_cast<double>(u[q].t[e]) * factor);
-                *reinterpret_cast<V*>(to + i) = u[q].v;
+                __stcs(reinterpret_cast<V*>(to + i), u[q].v);
             } else {
                 for (int e = 0; e < per; ++e)
                     if (i + e < n) to[i + e] = static_cast<T>(static_cast<double>(from[i + e]) * factor);
@@ -153,6 +154,7 @@ template <int N>
 __global__ void __launch_bounds__(kThreads) gradient_scale_kernel(const __grid_constant__ TensorList<N> list, const double* __restrict__ partial, int partials,
                                                                   double max_norm, double* __restrict__ norm) {
     __shared__ double shared[kThreads / 32];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const double n = norm_of(partial, partials, shared);
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = n;
     // a NaN makes the norm NaN, and that the factor and all values
@@ -223,7 +225,8 @@ void with_list(const smx_gradient* list, int a, int b, int tiles, Fn&& fn) {
         fn(l);
     };
     if (b - a <= 32) fill(ListSize<32>{});
-    else if (b - a <= 256) fill(ListSize<256>{});
+    else if (b - a <= 128) fill(ListSize<128>{});
+    else if (b - a <= 512) fill(ListSize<512>{});
     else fill(ListSize<kLargestList>{});
 }
 
@@ -271,8 +274,9 @@ void gradient_norm_clip(const smx_gradient* list, int count, bool clip, double m
     for_launches(list, count, [&](int a, int b, int tiles) {
         if (tiles == 0) return;
         with_list(list, a, b, tiles, [&](const auto& l) {
-            gradient_scale_kernel<<<grid_of(tiles), kThreads, 0, stream>>>(l, partial, partials, max_norm, first ? norm : nullptr);
-            launched("gradient_scale_kernel");
+            constexpr int N = sizeof(l.tensor) / sizeof(Tensor);
+            chain_launch(Launcher{stream, first}, gradient_scale_kernel<N>, dim3(grid_of(tiles)), kThreads, 0, 1, l, partial, partials, max_norm, first ? norm : nullptr);
+            ++operator_launches;
             first = false;
         });
     });

@@ -260,7 +260,7 @@ void launch_gd(const GdPass& p, cudaStream_t stream) {
         }
         return n;
     };
-    if (tiles(64, 64) > 2LL * sm_count()) launch_gd<kMode, 64, 64, 2, 2, 3>(p, tiles(64, 64), stream);
+    if (tiles(64, 64) > 2LL * sm_count()) launch_gd<kMode, 64, 64, 2, 2, 2>(p, tiles(64, 64), stream);
     else launch_gd<kMode, 16, 32, 1, 4, 4>(p, tiles(16, 32), stream);
 }
 

@@ -26,9 +26,10 @@ constexpr int kMaxGroups = SMX_ROUTE_MAX_GROUPS;
 // Pairs are counted and ranked by warps that own consecutive pairs: 32 at a time, lanes of equal group found with match_any, one counter
 // per (warp, group) in shared memory that only that warp touches. Equal keys therefore keep their order. Latency bounds it: 13.5 us for 7,545
 // pairs in one CTA, 6 + 4 + 10 us for the three kernels at 196,608 pairs (2.4 MB).
-// What is sorted: key(i) of element i, and what order[] receives for it; kPlan: with positions and offsets.
+// What is sorted: key(i) of element i, and what order[] receives for it; kPlan: with positions and offsets. kNames: `position` receives the name
+// of every place.
 struct GroupKeys {                               // pairs by group, empty slots last
-    static constexpr bool kPlan = true;
+    static constexpr bool kPlan = true, kNames = false;
     const int* ids; int groups;
     __device__ __forceinline__ int key(long long i) const {
         const int g = ids[i];
@@ -37,30 +38,42 @@ struct GroupKeys {                               // pairs by group, empty slots 
     __device__ __forceinline__ int value(long long i) const { return static_cast<int>(i); }
 };
 struct SlotKeys {                                // places by the slot of their pair, order[i] = n * slots + slot (see route_slots)
-    static constexpr bool kPlan = false;
+    static constexpr bool kPlan = false, kNames = false;
     const int* order; int slots;
     __device__ __forceinline__ int key(long long i) const { return order[i] % slots; }
     __device__ __forceinline__ int value(long long i) const { return static_cast<int>(i); }
 };
 struct DigitKeys {                               // pairs by a digit of their token, in the order that the lower digits gave (null: as they come)
-    static constexpr bool kPlan = false;
+    static constexpr bool kPlan = false, kNames = true;
     const int* ids; int table_rows; const int* before; int shift, mask;
-    __device__ __forceinline__ int key(long long i) const {
-        const int t = ids[value(i)];
-        return ((t < 0 || t >= table_rows ? table_rows : t) >> shift) & mask;
-    }
     __device__ __forceinline__ int value(long long i) const { return before ? before[i] : static_cast<int>(i); }
+    __device__ __forceinline__ int name(int pair) const {
+        const int t = ids[pair];
+        return t < 0 || t >= table_rows ? table_rows : t;
+    }
+    __device__ __forceinline__ int key(long long i) const { return (name(value(i)) >> shift) & mask; }
 };
 
+// The keys are read ahead: one after the other, each would wait for memory (one CTA, 4,001 tokens: 15.4 us a plan, 12.3 with eight ahead and the
+// warps' counters added up by lanes).
+constexpr int kKeysAhead = 8;
 template <typename Keys>
 __device__ __forceinline__ void route_count(const Keys& keys, long long begin, long long end, int groups, int* __restrict__ hist) {
     const int lane = threadIdx.x & 31;
-    for (long long i0 = begin; i0 < end; i0 += 32) {
-        const bool in = i0 + lane < end;
-        const int g = in ? keys.key(i0 + lane) : groups + 1;
-        const unsigned same = __match_any_sync(0xffffffffu, g);
-        if (in && lane == __ffs(same) - 1) hist[g] += __popc(same);
-        __syncwarp();
+    for (long long i1 = begin; i1 < end; i1 += 32 * kKeysAhead) {
+        int key[kKeysAhead];
+#pragma unroll
+        for (int q = 0; q < kKeysAhead; ++q) key[q] = i1 + 32 * q + lane < end ? keys.key(i1 + 32 * q + lane) : groups + 1;
+#pragma unroll
+        for (int q = 0; q < kKeysAhead; ++q) {
+            const long long i0 = i1 + 32 * q;
+            if (i0 >= end) break;
+            const bool in = i0 + lane < end;
+            const int g = key[q];
+            const unsigned same = __match_any_sync(0xffffffffu, g);
+            if (in && lane == __ffs(same) - 1) hist[g] += __popc(same);
+            __syncwarp();
+        }
     }
 }
 
@@ -69,20 +82,30 @@ template <typename Keys>
 __device__ __forceinline__ void route_place(const Keys& keys, long long begin, long long end, int groups, int* __restrict__ next,
                                             int* __restrict__ order, int* __restrict__ position) {
     const int lane = threadIdx.x & 31;
-    for (long long i0 = begin; i0 < end; i0 += 32) {
-        const bool in = i0 + lane < end;
-        const int g = in ? keys.key(i0 + lane) : groups + 1;
-        const unsigned same = __match_any_sync(0xffffffffu, g);
-        int first = 0;
-        if (in) first = next[g];
-        __syncwarp();
-        if (in) {
-            const int p = first + __popc(same & ((1u << lane) - 1u));
-            order[p] = keys.value(i0 + lane);
-            if (Keys::kPlan) position[i0 + lane] = g < groups ? p : -1;
-            if (lane == __ffs(same) - 1) next[g] = first + __popc(same);
+    for (long long i1 = begin; i1 < end; i1 += 32 * kKeysAhead) {
+        int key[kKeysAhead];
+#pragma unroll
+        for (int q = 0; q < kKeysAhead; ++q) key[q] = i1 + 32 * q + lane < end ? keys.key(i1 + 32 * q + lane) : groups + 1;
+#pragma unroll
+        for (int q = 0; q < kKeysAhead; ++q) {
+            const long long i0 = i1 + 32 * q;
+            if (i0 >= end) break;
+            const bool in = i0 + lane < end;
+            const int g = key[q];
+            const unsigned same = __match_any_sync(0xffffffffu, g);
+            int first = 0;
+            if (in) first = next[g];
+            __syncwarp();
+            if (in) {
+                const int p = first + __popc(same & ((1u << lane) - 1u)), value = keys.value(i0 + lane);
+                order[p] = value;
+                if constexpr (Keys::kPlan) position[i0 + lane] = g < groups ? p : -1;
+                if constexpr (Keys::kNames)
+                    if (position) position[p] = keys.name(value);
+                if (lane == __ffs(same) - 1) next[g] = first + __popc(same);
+            }
+            __syncwarp();
         }
-        __syncwarp();
     }
 }
 
@@ -136,16 +159,23 @@ __global__ void __launch_bounds__(kSmallPlanThreads) route_plan_small_kernel(con
     const int begin = min(pairs, warp * per), end = min(pairs, begin + per);
     if (warp < warps_used) route_count(keys, begin, end, groups, hist + warp * bins);
     __syncthreads();
-    for (int g = threadIdx.x; g < bins; g += blockDim.x) {
-        int run = 0;
-        for (int w = 0; w < warps_used; ++w) { const int c = hist[w * bins + g]; hist[w * bins + g] = run; run += c; }
-        total[g] = run;
+    const int lane = threadIdx.x & 31;               // a warp takes a group, a lane the counter of one warp
+    for (int g = warp; g < bins; g += blockDim.x >> 5) {
+        const int c = lane < warps_used ? hist[lane * bins + g] : 0;
+        int incl = c;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, incl, d);
+            if (lane >= d) incl += up;
+        }
+        if (lane < warps_used) hist[lane * bins + g] = incl - c;
+        if (lane == 31) total[g] = incl;
     }
     __syncthreads();
     cta_scan(total, bins, sums);
-    for (int g = threadIdx.x; g < bins; g += blockDim.x) {
-        if (Keys::kPlan) offsets[g] = total[g];     // bins = groups + 1 entries: the start of the empty slots is the end of the groups
-        for (int w = 0; w < warps_used; ++w) hist[w * bins + g] += total[g];
+    for (int g = warp; g < bins; g += blockDim.x >> 5) {
+        if (Keys::kPlan && lane == 0) offsets[g] = total[g];     // bins = groups + 1 entries: the start of the empty slots is the end of the groups
+        if (lane < warps_used) hist[lane * bins + g] += total[g];
     }
     __syncthreads();
     if (warp < warps_used) route_place(keys, begin, end, groups, hist + warp * bins, order, position);
@@ -199,6 +229,7 @@ __global__ void __launch_bounds__(kPlanThreads) route_place_kernel(const Keys ke
     int* start = route_smem;                    // bins + 1
     int* hist = route_smem + bins + 1;
     for (int i = threadIdx.x; i < kPlanWarps * bins; i += kPlanThreads) hist[i] = 0;
+#pragma unroll 4
     for (int g = threadIdx.x; g < bins; g += kPlanThreads) start[g] = total[g];
     __syncthreads();
     cta_scan(start, bins, sums);
@@ -206,9 +237,11 @@ __global__ void __launch_bounds__(kPlanThreads) route_place_kernel(const Keys ke
     const long long begin = min(pairs, static_cast<long long>(blockIdx.x) * kPlanChunk + warp * per), end = min(pairs, begin + per);
     route_count(keys, begin, end, groups, hist + warp * bins);
     __syncthreads();
+#pragma unroll 4
     for (int g = threadIdx.x; g < bins; g += kPlanThreads) {
         if (Keys::kPlan && blockIdx.x == 0) offsets[g] = start[g];
         int run = start[g] + chunk_prefix[static_cast<long long>(g) * chunks + blockIdx.x];
+#pragma unroll
         for (int w = 0; w < kPlanWarps; ++w) { const int c = hist[w * bins + g]; hist[w * bins + g] = run; run += c; }
     }
     __syncthreads();
@@ -459,6 +492,12 @@ void counting_sort(const Keys& keys, long long pairs, int num_groups, int* order
     int* hist = static_cast<int*>(workspace);
     int* total = hist + static_cast<size_t>(bins) * chunks;
     const int smem = kPlanWarps * bins * static_cast<int>(sizeof(int));
+    static std::atomic<bool> done[64];
+    if (smem + (bins + 1) * static_cast<int>(sizeof(int)) > 47 * 1024 && first_on_device(done)) {
+        SMX_CUDA(cudaFuncSetAttribute(route_count_kernel<Keys>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+        SMX_CUDA(cudaFuncSetAttribute(route_place_kernel<Keys>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
+        mark_on_device(done);
+    }
     route_count_kernel<Keys><<<chunks, kPlanThreads, smem, stream>>>(keys, pairs, num_groups, chunks, hist);
     launched("route_count_kernel");
     route_scan_kernel<<<(bins * 32 + 255) / 256, 256, 0, stream>>>(bins, chunks, hist, total);
@@ -488,22 +527,33 @@ void route_slots(const int* order, long num_rows, int slots, const int* offsets,
     launched("route_slot_offsets_kernel");
 }
 
-// Tokens have up to 21 bits (the number of rows itself stands for pairs without a token): one digit, or two of half of them.
-size_t token_sort_bytes(long pairs, int table_rows) {
-    const size_t sort = route_plan_bytes(pairs, 1, std::min(table_rows + 1, kMaxGroups));
-    return table_rows < kMaxGroups ? sort : (sort + 255) / 256 * 256 + static_cast<size_t>(pairs) * sizeof(int);
-}
-void token_sort(const int* ids, long pairs, int table_rows, int* order, void* workspace, cudaStream_t stream) {
-    if (table_rows < kMaxGroups) {
-        counting_sort(DigitKeys{ids, table_rows, nullptr, 0, 0x7fffffff}, pairs, table_rows + 1, order, nullptr, nullptr, workspace, stream);
-        return;
-    }
+// Tokens have up to 20 bits (the number of rows itself stands for pairs without a token): one digit as far as the counters of its values fit into shared
+// memory, or two of half of the bits. (98,304 pairs, 1,424 rows: 34 us by one digit; 60 by two, with keys that were not read ahead.)
+namespace {
+constexpr int kDigitValues = 4096;
+int digit_bits(int table_rows) {
     int bits = 1;
     while ((table_rows >> bits) >= (1 << bits)) ++bits;
-    const size_t sort = route_plan_bytes(pairs, 1, kMaxGroups);
-    int* half = reinterpret_cast<int*>(static_cast<char*>(workspace) + (sort + 255) / 256 * 256);
+    return bits;
+}
+size_t sort_bytes(long pairs, int values) {
+    if (pairs <= kSmallPlanPairs) return 0;
+    return static_cast<size_t>(values + 1) * ((pairs + kPlanChunk - 1) / kPlanChunk + 1) * sizeof(int);
+}
+}  // namespace
+size_t token_sort_bytes(long pairs, int table_rows) {
+    if (table_rows < kDigitValues) return sort_bytes(pairs, table_rows + 1);
+    return (sort_bytes(pairs, 1 << digit_bits(table_rows)) + 255) / 256 * 256 + static_cast<size_t>(pairs) * sizeof(int);
+}
+void token_sort(const int* ids, long pairs, int table_rows, int* order, int* names, void* workspace, cudaStream_t stream) {
+    if (table_rows < kDigitValues) {
+        counting_sort(DigitKeys{ids, table_rows, nullptr, 0, 0x7fffffff}, pairs, table_rows + 1, order, names, nullptr, workspace, stream);
+        return;
+    }
+    const int bits = digit_bits(table_rows);
+    int* half = reinterpret_cast<int*>(static_cast<char*>(workspace) + (sort_bytes(pairs, 1 << bits) + 255) / 256 * 256);
     counting_sort(DigitKeys{ids, table_rows, nullptr, 0, (1 << bits) - 1}, pairs, 1 << bits, half, nullptr, nullptr, workspace, stream);
-    counting_sort(DigitKeys{ids, table_rows, half, bits, 0x7fffffff}, pairs, (table_rows >> bits) + 1, order, nullptr, nullptr, workspace, stream);
+    counting_sort(DigitKeys{ids, table_rows, half, bits, 0x7fffffff}, pairs, (table_rows >> bits) + 1, order, names, nullptr, workspace, stream);
 }
 
 template <typename T>

@@ -30,10 +30,10 @@ void check_pointers(const char* what, size_t bytes, std::initializer_list<const 
 size_t route_slots_bytes(long num_rows, int slots);
 void route_slots(const int* order, long num_rows, int slots, const int* offsets, int num_groups, int* places, int* slot_offsets, void* workspace,
                  cudaStream_t stream);
-// Pairs by token, equal ones in the order of the list, those without one (outside 0 .. table_rows - 1) last: order[p] is the p-th. At most
-// 2^20 table rows; the caller has checked the sizes.
+// Pairs by token, equal ones in the order of the list, those without one (outside 0 .. table_rows - 1) last: order[p] is the p-th, names[p] its token
+// (table_rows: none). Fewer than 2^20 table rows; the caller has checked the sizes.
 size_t token_sort_bytes(long pairs, int table_rows);
-void token_sort(const int* ids, long pairs, int table_rows, int* order, void* workspace, cudaStream_t stream);
+void token_sort(const int* ids, long pairs, int table_rows, int* order, int* names, void* workspace, cudaStream_t stream);
 template <typename T>
 void route_dispatch(const T* x, long x_stride, long num_rows, int slots, long width, const int* position, const int* offsets, int num_groups,
                     T* rows, bool zero_tail, cudaStream_t stream);

@@ -134,7 +134,7 @@ class Embedding:
         weights = _weights(weights, rows, slots, self.dtype, self.device)
         grad_table = self.table.new_empty((self.table_rows, self.width)) if want_table else None
         grad_weights = self.table.new_empty((rows, slots)) if want_weights else None
-        need = self._library.smx_embedding_backward_bytes(self._precision, rows, slots, self.width) if want_table else 0
+        need = self._library.smx_embedding_backward_bytes(self._precision, rows, slots, self.width)
         if need < 0:
             raise ValueError("the sizes exceed what smx_embedding_backward supports")
         ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
