@@ -162,10 +162,10 @@ void launch_gs(const GsPass& p, long long tiles, cudaStream_t stream) {
         cudaFuncAttributes a{};
         SMX_CUDA(cudaFuncGetAttributes(&a, kernel));
         if (a.numRegs < kGsRegsLaunch) throw CudaError("grouped_f32_kernel was built with too few registers");
-        SMX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, GsLayout<kMode, kWide>::smem));
+        SMX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, GsLayout<kWide>::smem));
         mark_on_device(done);
     }
-    kernel<<<static_cast<unsigned>(std::min<long long>(tiles, sm_count())), kGsThreads, GsLayout<kMode, kWide>::smem, stream>>>(p);
+    kernel<<<static_cast<unsigned>(std::min<long long>(tiles, sm_count())), kGsThreads, GsLayout<kWide>::smem, stream>>>(p);
     launched("grouped_f32_kernel");
 }
 

@@ -17,7 +17,7 @@ namespace {
 enum GsMode { kGsForward, kGsBackward, kGsGradient };
 constexpr int kGsThreads = 896, kGsChunk = 64, kGsStages = 2, kGsRing = 4;   // inner values of a step; stages of A and of B; tiles in the ring
 constexpr int kGsPartBytes = 128 * 32 * 4, kGsHalfBytes = 2 * kGsPartBytes, kGsStageBytes = 2 * kGsHalfBytes;     // B: 32 inner values; hi or lo; both
-constexpr int kGsRowStages = 2, kGsPitch = 32 + 4, kGsOutPitch = 17;
+constexpr int kGsPitch = 32 + 4, kGsOutPitch = 17;                           // floats of a row in a warp's tile, and on the way out of rows that are not aligned
 constexpr int kGsStatusWait = 8;
 // the warps' shares of the registers, by fours: control, A, sums, B
 constexpr int kGsRegsLaunch = 72, kGsRegsControl = 40, kGsRegsA = 64, kGsRegsSums = 104, kGsRegsB = 64;
@@ -166,24 +166,49 @@ __device__ __forceinline__ void gs_row(const GsWork& w, int comps, int i, int& p
     comp = static_cast<int>(r - ahead * comps);
 }
 
-// The gradient's operands: a thread reads one column of 32 consecutive rows, kGsChunk on in every step. Lanes find a row each and share where it starts.
-struct GsRows {
-    long long pair, stride;
-    int comp, comps, width;
-    __device__ __forceinline__ void begin(const GsWork& w, int comps_, int width_, long long stride_, int ahead_of) {
-        comps = comps_; width = width_; stride = stride_;
-        const long long r = w.row0 + ahead_of, ahead = r < (1LL << 31) ? static_cast<int>(r) / comps : r / comps;
-        pair = w.first_pair + ahead;
-        comp = static_cast<int>(r - ahead * comps);
-    }
-    __device__ __forceinline__ void read(long long* table, const float* column, int good, float (&v)[32]) {
-        __syncwarp();
-        table[threadIdx.x & 31] = pair * stride + static_cast<long long>(comp) * width;
-        __syncwarp();
+// Tiles of 32 x 32 values on their way from global memory to the registers of a warp, through 4,608 bytes of shared memory of the warp's own: copied
+// asynchronously, the next one as soon as the registers hold this one. A lane owns a row of A or a column of B and gets its 32 inner values. kInner: rows
+// of the array are inner values (their owners follow one another); else rows are owners (their inner values follow one another).
+template <bool kInner>
+struct GsTile {
+    float* buffer;
+    // at(r): where row r of the array begins, from `base` on; `rows` x `cols` of the tile exist
+    template <typename At>
+    __device__ __forceinline__ void copy(const float* base, At&& at, int rows, int cols, bool wide) const {
+        constexpr int pitch = kInner ? 32 : kGsPitch;
+        const int lane = threadIdx.x & 31;
+        if (wide) {                                  // four rows an instruction, 16 bytes a lane
+            const int c = (lane & 7) * 4;
 #pragma unroll
-        for (int r = 0; r < 32; ++r) v[r] = r < good ? __ldg(column + table[r]) : 0.f;
-        comp += kGsChunk % comps; pair += kGsChunk / comps;
-        if (comp >= comps) { comp -= comps; ++pair; }
+            for (int r = lane >> 3; r < 32; r += 4)
+                if (r < rows && c < cols) cp_async16(buffer + r * pitch + c, base + at(r) + c, 16);
+        } else {
+#pragma unroll 4
+            for (int r = 0; r < 32; ++r)
+                if (r < rows && lane < cols) cp_async4(buffer + r * pitch + lane, base + at(r) + lane);
+        }
+        cp_async_commit();
+    }
+    // the lane's values, zero where the tile has none
+    __device__ __forceinline__ void read(int rows, int cols, float (&v)[32]) const {
+        const int lane = threadIdx.x & 31;
+        cp_async_wait<0>();
+        __syncwarp();
+        if (kInner) {
+#pragma unroll
+            for (int r = 0; r < 32; ++r) v[r] = buffer[32 * r + lane];
+        } else {
+#pragma unroll
+            for (int c = 0; c < 32; c += 4) {
+                const float4 f = *reinterpret_cast<const float4*>(buffer + lane * kGsPitch + c);
+                v[c] = f.x; v[c + 1] = f.y; v[c + 2] = f.z; v[c + 3] = f.w;
+            }
+        }
+        __syncwarp();                                // the next copies may come in
+        const int good = kInner ? (lane < cols ? rows : 0) : (lane < rows ? cols : 0);
+        if (good < 32)
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = e < good ? v[e] : 0.f;
     }
 };
 
@@ -231,44 +256,41 @@ __device__ __forceinline__ void gs_products(uint32_t d, uint32_t a_hi, uint32_t 
 }
 
 // kWide: every row's half of a tile of the output starts on 32 bytes and is 64 columns long.
-template <int kMode, bool kWide>
+template <bool kWide>
 struct GsLayout {
-    static constexpr int row_stages = kMode == kGsGradient ? 0 : kGsRowStages;       // raw rows on their way to tensor memory
-    static_assert(kGsRing > kGsRowStages, "the rows' copies run a step, and so up to a tile, ahead of the tile that is given back last");
-    static constexpr int row_floats = 8 * 32 * kGsPitch;                             // a stage: eight warps' 32 rows of 32 values
-    static constexpr int smem = kGsStages * kGsStageBytes + (row_stages * row_floats + (kWide ? 0 : 8 * 32 * kGsOutPitch)) * 4 + 1024;
-    static_assert(smem + 7168 <= 227 * 1024, "shared memory of one CTA per SM");
+    static constexpr int raw_at = kGsStages * kGsStageBytes, raw_floats = 32 * kGsPitch;                   // a tile for each of sixteen operand warps
+    static constexpr int out_at = raw_at + 16 * raw_floats * 4;
+    static constexpr int smem = out_at + (kWide ? 0 : 8 * 32 * kGsOutPitch * 4) + 1024;
+    static_assert(smem + 6144 <= 227 * 1024, "shared memory of one CTA per SM");
 };
 
 // One persistent CTA per SM walks its share of the tiles, 64 inner values a step; its warps are specialised, so that the parts of neighbouring tiles overlap:
 //   warp 0        the products (one thread)
 //   warp 1        finds the tiles (a ring, ahead of all others)
 //   warps 2, 3    zeros into the rows behind the last group
-//   warps 4-11    A, 32 rows of 32 inner values a warp. Rows passes: a warp copies its rows asynchronously, a step ahead; a thread splits those of its row and
-//                 stores them to tensor memory. Gradient: a thread owns a column of x and reads it row by row.
+//   warps 4-11    A, 32 rows of 32 inner values a warp: copied while the ones before are split and stored to tensor memory
 //   warps 12-19   a thread adds half of its row's partial sums of every step in registers (the tensor core cuts its sums instead of rounding them: one
 //                 sum over 128 inner values is off five times as far as float32) and writes its half of the row
-//   warps 20-27   B, 32 inner values of 128 columns for four warps, read when the ones before are stored; where a matrix has up to 128 inner values it
-//                 stays for all row tiles of its group
+//   warps 20-27   B, 32 columns of 32 inner values a warp, in the same way, stored to shared memory; where a matrix has up to 128 inner values it stays for
+//                 all row tiles of its group
 // TMEM: two partial sums of 128 columns, taken in turn, and two stages of A of 128 (hi, lo). A hand-over costs its warps some hundred cycles: with steps of
 // 32 inner values and half the warps for A and B the products waited two thirds of the time (98,304 atoms of 89 elements 127 us).
 // Every wait is bounded; if one runs out, the CTA gives up, fills its remaining tiles with NaN, reports it to `status` and ends when its products
 // and copies in flight have.
 template <int kMode, bool kWide>
 __global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid_constant__ GsPass pass) {
-    using L = GsLayout<kMode, kWide>;
+    using L = GsLayout<kWide>;
+    constexpr bool kRows = kMode != kGsGradient;
     extern __shared__ unsigned char gs_smem_raw[];
     __shared__ __align__(8) unsigned long long work_full[kGsRing], work_free[kGsRing], a_full[kGsStages], a_free[kGsStages], b_full[kGsStages], b_free[kGsStages],
         d_full[2], d_free[2], drained;
     __shared__ GsWork work[kGsRing];
-    __shared__ int work_pair[kMode == kGsGradient ? 1 : kGsRing][128];
-    __shared__ short work_comp[kMode == kGsGradient ? 1 : kGsRing][128];
-    __shared__ __align__(16) long long row_at[kMode == kGsGradient ? 16 : 1][32];        // gradient: where a chunk's rows start, for every operand warp
+    __shared__ __align__(16) long long row_at[16][32];                                   // where the rows of an operand warp's tile start
     __shared__ uint32_t tmem_slot;
     __shared__ int guard[2];                                                             // a wait ran out; polls of a wait
     const int warp = ts_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     unsigned char* const stages = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(gs_smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    float* const row_stages = reinterpret_cast<float*>(stages + kGsStages * kGsStageBytes);
+    float* const raw = reinterpret_cast<float*>(stages + L::raw_at);
     if (threadIdx.x == 0) {
         guard[0] = 0;
         guard[1] = pass.expire_polls > 0 ? pass.expire_polls : static_cast<int>(kMbarSpinLimit);
@@ -342,14 +364,6 @@ __global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid
                         last_degree = w.degree; last_group = w.group; last_block = w.block;
                     }
                     if (i >= kGsRing && !ts_wait_warp(&work_free[slot], (i / kGsRing - 1) & 1, guard)) { ok = false; break; }
-                    if (kMode != kGsGradient && w.found)
-#pragma unroll 1
-                        for (int at = lane; at < 128; at += 32) {
-                            int pair = w.first_pair, comp = 0;
-                            if (at < w.rows) gs_row(w, pass.degree[q].comps, at, pair, comp);
-                            work_pair[slot][at] = pair;
-                            work_comp[slot][at] = static_cast<short>(comp);
-                        }
                     if (lane == 0) work[slot] = w;
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&work_full[slot]);
@@ -389,210 +403,186 @@ __global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid
             ts_store16(to, hi);
             ts_store16(to + 64, v);
         };
-        if constexpr (kMode != kGsGradient) {
-            float* const rows_at = row_stages + (warp - 4) * 32 * kGsPitch;
-            int xs = 0, ahead_tile = 0, ahead = 0, ahead_chunks = 0, ahead_K = 0, ahead_rows = 0, ahead_slot = 0;
-            long long ahead_off = 0;
-            bool more = true, wide = false;
-            auto copy_next = [&](int stage) {
-                if (more && ahead == ahead_chunks) {
-                    ahead_slot = ahead_tile % kGsRing;
-                    if (!ts_wait_warp(&work_full[ahead_slot], (ahead_tile / kGsRing) & 1, guard)) {
-                        ok = more = false;
-                    } else {
-                        const GsWork& w = work[ahead_slot];
-                        more = w.found != 0;
-                        if (more) {
-                            const GsDegree& d = pass.degree[w.degree];
-                            wide = ((static_cast<unsigned long long>(pass.a_stride | d.a_off | d.K) * 4u | reinterpret_cast<uintptr_t>(pass.a)) & 15) == 0;
-                            ahead = 0; ahead_K = d.K; ahead_chunks = w.chunks; ahead_off = d.a_off;
-                            ahead_rows = min(32, w.rows - first);
-                            ++ahead_tile;
-                        }
-                    }
-                }
-                if (more) {
-                    float* to = rows_at + stage * L::row_floats;
-                    const int k = ahead * kGsChunk + k_part, left = min(32, ahead_K - k);
-                    const float* from = pass.a + ahead_off + k;
-                    const int* pair = work_pair[ahead_slot] + first;
-                    const short* comp = work_comp[ahead_slot] + first;
-                    if (wide) {                          // four rows an instruction, 16 bytes a lane
-                        const int c = (lane & 7) * 4;
-                        if (c < left)
-#pragma unroll 4
-                            for (int r = lane >> 3; r < ahead_rows; r += 4) cp_async16(to + r * kGsPitch + c, from + pair[r] * pass.a_stride + comp[r] * ahead_K + c, 16);
-                    } else if (lane < left) {
-#pragma unroll 4
-                        for (int r = 0; r < ahead_rows; ++r) cp_async4(to + r * kGsPitch + lane, from + pair[r] * pass.a_stride + comp[r] * ahead_K + lane);
-                    }
-                    ++ahead;
-                }
-                cp_async_commit();
-            };
-            copy_next(0);
-            for (int i = 0; ok; ++i) {
+        const GsTile<!kRows> tile{raw + (warp - 4) * L::raw_floats};
+        long long* const table = row_at[warp - 4];
+        // the chunk that is copied: tile i - 1, chunk j
+        int i = 0, j = 0, chunks = 0, inner = 0, owned = 0, comps = 1, comp = 0, width = 0;
+        long long pair = 0;
+        const float* base = nullptr;
+        bool wide = false;
+        auto advance = [&]() {
+            ++j;
+            while (j >= chunks) {
                 const int slot = i % kGsRing;
-                if (!ts_wait_warp(&work_full[slot], (i / kGsRing) & 1, guard)) break;
-                const int found = work[slot].found, chunks = work[slot].chunks, inner = work[slot].inner;
-                const bool live = tid < work[slot].rows;
-                for (int j = 0; found && j < chunks; ++j) {
-                    __syncwarp();                        // all lanes have read what the next copy overwrites
-                    copy_next(xs ^ 1);
-                    cp_async_wait<1>();
-                    __syncwarp();
-                    if (!ok || !free_stage()) { ok = false; break; }
-                    ts_fence_after();
-                    const float* row = rows_at + xs * L::row_floats + lane * kGsPitch;
-                    xs ^= 1;
-                    const int good = live ? inner - j * kGsChunk - k_part : 0;       // what the stage holds behind the tile's or the row's end is no value
-#pragma unroll 1
-                    for (int q = 0; q < 32; q += 16) {
-                        float v[16];
-#pragma unroll
-                        for (int e = 0; e < 16; e += 4) {
-                            const float4 f = *reinterpret_cast<const float4*>(row + q + e);
-                            v[e] = f.x; v[e + 1] = f.y; v[e + 2] = f.z; v[e + 3] = f.w;
-                        }
-                        if (good < q + 16)
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) v[e] = q + e < good ? v[e] : 0.f;
-                        put16(q, v);
-                    }
-                    give();
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&work_free[slot]);
-                if (!found) break;
-            }
-            asm volatile("cp.async.wait_all;" ::: "memory");             // none may be in flight when the CTA ends
-        }
-        if constexpr (kMode == kGsGradient) {
-            int i = 0;
-            for (;;) {
-                const int slot = i % kGsRing;
-                if (!ts_wait_warp(&work_full[slot], (i / kGsRing) & 1, guard)) break;
-                const int found = work[slot].found, chunks = work[slot].chunks, inner = work[slot].inner;
-                GsRows at;
-                const float* column = nullptr;                           // null: behind the matrix's end
+                if (!ts_wait_warp(&work_full[slot], (i / kGsRing) & 1, guard)) { ok = false; return false; }
+                const GsWork& w = work[slot];
+                const int found = w.found;
                 if (found) {
-                    const GsWork& w = work[slot];
                     const GsDegree& d = pass.degree[w.degree];
-                    at.begin(w, d.comps, d.K, pass.a_stride, k_part + lane);
-                    if (tid < w.rows) column = pass.a + d.a_off + 128 * w.mtile + tid;
+                    chunks = w.chunks; inner = w.inner;
+                    owned = min(32, w.rows - first);
+                    comps = d.comps; width = d.K;
+                    wide = ((static_cast<unsigned long long>(pass.a_stride | d.a_off | d.K) * 4u | reinterpret_cast<uintptr_t>(pass.a)) & 15) == 0;
+                    int at;
+                    gs_row(w, comps, kRows ? first + lane : k_part + lane, at, comp);
+                    pair = at;
+                    base = pass.a + d.a_off + (kRows ? k_part : 128 * w.mtile + first);
+                    if (kRows) table[lane] = pair * pass.a_stride + static_cast<long long>(comp) * width;
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&work_free[slot]);
-                if (!found) break;
+                if (!found) return false;
                 ++i;
-                for (int j = 0; j < chunks; ++j) {
-                    float v[32];
-                    at.read(row_at[warp - 4], column, column ? inner - j * kGsChunk - k_part : 0, v);
-                    if (!free_stage()) { ok = false; break; }
-                    ts_fence_after();
-#pragma unroll
-                    for (int q = 0; q < 32; q += 16) {
-                        float part[16];
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) part[e] = v[q + e];
-                        put16(q, part);
-                    }
-                    give();
-                }
-                if (!ok) break;
+                j = 0;
             }
+            return true;
+        };
+        auto copy = [&]() {
+            const int left = inner - j * kGsChunk - k_part;
+            if constexpr (kRows) {
+                const float* from = base + j * kGsChunk;
+                tile.copy(from, [&](int r) { return table[r]; }, owned, left, wide);
+            } else {
+                __syncwarp();
+                table[lane] = pair * pass.a_stride + static_cast<long long>(comp) * width;
+                comp += kGsChunk % comps; pair += kGsChunk / comps;
+                if (comp >= comps) { comp -= comps; ++pair; }
+                __syncwarp();
+                tile.copy(base, [&](int r) { return table[r]; }, left, owned, wide);
+            }
+        };
+        bool have = advance();
+        if (have) copy();
+        while (have && ok) {
+            const int left = inner - j * kGsChunk - k_part;
+            float v[32];
+            if (kRows) tile.read(owned, left, v);
+            else tile.read(left, owned, v);
+            have = advance();
+            if (have) copy();
+            if (!ok || !free_stage()) { ok = false; break; }
+            ts_fence_after();
+#pragma unroll
+            for (int q = 0; q < 32; q += 16) {
+                float part[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) part[e] = v[q + e];
+                put16(q, part);
+            }
+            give();
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");                 // none may be in flight when the CTA ends
         gs_meet();
     } else if (warp >= 20) {
         ts_registers_less<kGsRegsB>();
-        const int tid = threadIdx.x & 127, part = warp & 3, k_part = 32 * ((warp - 20) >> 2);
-        int nb = 0;
-        bool ok = true;
-        for (int i = 0; ok; ++i) {
-            const int slot = i % kGsRing;
-            if (!ts_wait_warp(&work_full[slot], (i / kGsRing) & 1, guard)) break;
-            const GsWork& w = work[slot];
-            const int found = w.found, chunks = w.fresh ? w.chunks : 0, inner = w.inner;
-            int width = 0, left = 0;
-            const float* from = nullptr;
-            bool wide = false;
-            GsRows at;
-            if (found) {
-                const GsDegree& d = pass.degree[w.degree];
-                left = min(128, d.N - 128 * w.block);
-                const float* matrix = d.w + static_cast<long long>(w.group) * d.K * d.N;
-                if (kMode == kGsForward) {
-                    width = d.N;
-                    from = matrix + static_cast<long long>(k_part) * width + 128 * w.block + tid;
-                } else if (kMode == kGsBackward) {
-                    width = d.K;
-                    from = matrix + static_cast<long long>(128 * w.block + 32 * part + (lane >> 3)) * width + k_part + 4 * (lane & 7);
-                    wide = (width & 3) == 0 && (reinterpret_cast<uintptr_t>(d.w) & 15) == 0;
-                } else {
-                    at.begin(w, d.comps, d.N, pass.b_stride, k_part + lane);
-                    from = pass.b + d.b_off + 128 * w.block + tid;
-                }
-            }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&work_free[slot]);
-            if (!found) break;
-            const int cols = (left + 15) & ~15;
-#pragma unroll 1
-            for (int j = 0; j < chunks; ++j) {
-                const int good = inner - j * kGsChunk - k_part;
-                float v[32];
-                if constexpr (kMode == kGsForward) {
-                    const float* p = from + static_cast<long long>(j) * kGsChunk * width;
-                    const int rows = tid < left ? good : 0;
-#pragma unroll
-                    for (int r = 0; r < 32; ++r, p += width) v[r] = r < rows ? __ldg(p) : 0.f;
-                } else if constexpr (kMode == kGsBackward) {
-                    const int k = 4 * (lane & 7);
-#pragma unroll
-                    for (int r = 0; r < 8; ++r) {
-                        const float* p = from + j * kGsChunk + static_cast<long long>(4 * r) * width;
-                        const bool in = 32 * part + (lane >> 3) + 4 * r < left;
-                        if (wide) {
-                            const float4 f = in && k < good ? __ldg(reinterpret_cast<const float4*>(p)) : make_float4(0.f, 0.f, 0.f, 0.f);
-                            v[4 * r] = f.x; v[4 * r + 1] = f.y; v[4 * r + 2] = f.z; v[4 * r + 3] = f.w;
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) v[4 * r + e] = in && k + e < good ? __ldg(p + e) : 0.f;
-                        }
+        const int first = 32 * (warp & 3), part = (warp - 20) >> 2, k_part = 32 * part;          // the warp's columns and inner values are its own
+        const GsTile<kMode != kGsBackward> tile{raw + (warp - 12) * L::raw_floats};
+        long long* const table = row_at[warp - 12];
+        // the chunk that is copied: tile i - 1, chunk j. `crosses`: the tile behind this one has a matrix of its own
+        int i = 0, j = 0, chunks = 0, inner = 0, owned = 0, cols = 0, comps = 1, comp = 0, width = 0, nb = 0;
+        long long pair = 0;
+        const float* base = nullptr;
+        bool ok = true, wide = false, crosses = false;
+        auto advance = [&]() {
+            ++j;
+            while (j >= chunks) {
+                const int slot = i % kGsRing;
+                if (!ts_wait_warp(&work_full[slot], (i / kGsRing) & 1, guard)) { ok = false; return false; }
+                const GsWork& w = work[slot];
+                const int found = w.found;
+                j = chunks = 0;
+                if (found && w.fresh) {
+                    const GsDegree& d = pass.degree[w.degree];
+                    const int left = min(128, d.N - 128 * w.block);
+                    chunks = w.chunks; inner = w.inner; crosses = w.last != 0;
+                    cols = ((left + 15) & ~15) - first;
+                    owned = min(32, left - first);
+                    const float* matrix = d.w + static_cast<long long>(w.group) * d.K * d.N;
+                    if (kMode == kGsForward) {
+                        width = d.N;
+                        base = matrix + static_cast<long long>(k_part) * width + 128 * w.block + first;
+                    } else if (kMode == kGsBackward) {
+                        width = d.K;
+                        base = matrix + static_cast<long long>(128 * w.block + first) * width + k_part;
+                    } else {
+                        width = d.N; comps = d.comps;
+                        int at;
+                        gs_row(w, comps, k_part + lane, at, comp);
+                        pair = at;
+                        base = pass.b + d.b_off + 128 * w.block + first;
                     }
-                } else {
-                    at.read(row_at[warp - 12], from, tid < left ? good : 0, v);
+                    wide = kMode == kGsGradient ? ((static_cast<unsigned long long>(pass.b_stride | d.b_off | width) * 4u | reinterpret_cast<uintptr_t>(pass.b)) & 15) == 0
+                                                : ((static_cast<unsigned long long>(width) * 4u | reinterpret_cast<uintptr_t>(d.w)) & 15) == 0;
                 }
-                const int bs = nb % kGsStages;
-                if (pass.expire_polls > 0 && nb > 0) { ok = false; break; }
-                if (nb >= kGsStages && !ts_wait_warp(&b_free[bs], (nb / kGsStages - 1) & 1, guard)) { ok = false; break; }
-                unsigned char* const to = stages + bs * kGsStageBytes + (k_part >> 5) * kGsPartBytes;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&work_free[slot]);
+                if (!found) return false;
+                ++i;
+            }
+            return true;
+        };
+        auto copy = [&]() {
+            const int left = inner - j * kGsChunk - k_part;
+            if constexpr (kMode == kGsForward) {
+                tile.copy(base + static_cast<long long>(j) * kGsChunk * width, [&](int r) { return static_cast<long long>(r) * width; }, left, owned, wide);
+            } else if constexpr (kMode == kGsBackward) {
+                tile.copy(base + j * kGsChunk, [&](int r) { return static_cast<long long>(r) * width; }, owned, left, wide);
+            } else {
+                __syncwarp();
+                table[lane] = pair * pass.b_stride + static_cast<long long>(comp) * width;
+                comp += kGsChunk % comps; pair += kGsChunk / comps;
+                if (comp >= comps) { comp -= comps; ++pair; }
+                __syncwarp();
+                tile.copy(base, [&](int r) { return table[r]; }, left, owned, wide);
+            }
+        };
+        bool have = advance();
+        if (have) copy();
+        while (have && ok) {
+            const int left = inner - j * kGsChunk - k_part, stored = cols;
+            float v[32];
+            if (kMode == kGsBackward) tile.read(owned, left, v);
+            else tile.read(left, owned, v);
+            // The next chunk is on its way while this one is stored, unless it belongs to a tile that other tiles of this matrix come before: the ring may not
+            // hold them all, and they need this chunk.
+            const bool early = j + 1 < chunks || crosses;
+            if (early) {
+                have = advance();
+                if (have) copy();
+            }
+            const int bs = nb % kGsStages;
+            if (!ok || (pass.expire_polls > 0 && nb > 0)) { ok = false; break; }
+            if (nb >= kGsStages && !ts_wait_warp(&b_free[bs], (nb / kGsStages - 1) & 1, guard)) { ok = false; break; }
+            unsigned char* const to = stages + bs * kGsStageBytes + part * kGsPartBytes;
+            if (lane < stored) {
 #pragma unroll
                 for (int c = 0; c < 8; ++c) {
-                    // a thread's eight groups of four inner values belong to one column, or to eight
-                    const int row = kMode == kGsBackward ? 32 * part + (lane >> 3) + 4 * c : tid, group = kMode == kGsBackward ? lane & 7 : c;
-                    if (row >= cols) continue;
                     float4 hi, lo;
                     gs_split(v[4 * c], hi.x, lo.x);
                     gs_split(v[4 * c + 1], hi.y, lo.y);
                     gs_split(v[4 * c + 2], hi.z, lo.z);
                     gs_split(v[4 * c + 3], hi.w, lo.w);
-                    const int off = tc5_swizzled_group(row, group);
+                    const int off = tc5_swizzled_group(first + lane, c);
                     *reinterpret_cast<float4*>(to + off) = hi;
                     *reinterpret_cast<float4*>(to + kGsHalfBytes + off) = lo;
                 }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&b_full[bs]);
-                ++nb;
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&b_full[bs]);
+            ++nb;
+            if (!early) {
+                have = advance();
+                if (have) copy();
             }
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");
         gs_meet();
     } else {
         ts_registers_more<kGsRegsSums>();
         const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
         const int tid = threadIdx.x & 127, half = (warp - 12) >> 2;
-        float* const out_stage = row_stages + L::row_stages * L::row_floats + (warp - 12) * 32 * kGsOutPitch;
+        float* const out_stage = reinterpret_cast<float*>(stages + L::out_at) + (warp - 12) * 32 * kGsOutPitch;
         int nd = 0, at_degree = 0, at_tile = 0;      // the tile at hand, for a CTA that gives up (0, 0: none yet)
         bool ok = true;
         for (int i = 0;; ++i) {
@@ -608,8 +598,13 @@ __global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid
                 at_degree = w.degree; at_tile = w.tile;
                 left = d.N - 128 * w.block - 64 * half;                  // columns of this half that exist
                 if (tid < rows) {
-                    if (kMode == kGsGradient) out_row = w.out + static_cast<long long>(tid) * d.N + 64 * half;
-                    else out_row = pass.out + work_pair[slot][tid] * pass.out_stride + d.b_off + static_cast<long long>(work_comp[slot][tid]) * d.N + 128 * w.block + 64 * half;
+                    if (kRows) {
+                        int pair, comp;
+                        gs_row(w, d.comps, tid, pair, comp);
+                        out_row = pass.out + pair * pass.out_stride + d.b_off + static_cast<long long>(comp) * d.N + 128 * w.block + 64 * half;
+                    } else {
+                        out_row = w.out + static_cast<long long>(tid) * d.N + 64 * half;
+                    }
                 }
             }
             __syncwarp();
