@@ -17,7 +17,7 @@ namespace {
 enum GsMode { kGsForward, kGsBackward, kGsGradient };
 constexpr int kGsThreads = 896, kGsChunk = 64, kGsStages = 2, kGsRing = 4;   // inner values of a step; stages of A and of B; tiles in the ring
 constexpr int kGsPartBytes = 128 * 32 * 4, kGsHalfBytes = 2 * kGsPartBytes, kGsStageBytes = 2 * kGsHalfBytes;     // B: 32 inner values; hi or lo; both
-constexpr int kGsPitch = 32 + 4, kGsOutPitch = 17;                           // floats of a row in a warp's tile, and on the way out of rows that are not aligned
+constexpr int kGsOutPitch = 17;                                              // floats of a row on its way out of rows that are not aligned
 constexpr int kGsStatusWait = 8;
 // the warps' shares of the registers, by fours: control, A, sums, B
 constexpr int kGsRegsLaunch = 72, kGsRegsControl = 40, kGsRegsA = 64, kGsRegsSums = 104, kGsRegsB = 64;
@@ -166,26 +166,27 @@ __device__ __forceinline__ void gs_row(const GsWork& w, int comps, int i, int& p
     comp = static_cast<int>(r - ahead * comps);
 }
 
-// Tiles of 32 x 32 values on their way from global memory to the registers of a warp, through 4,608 bytes of shared memory of the warp's own: copied
-// asynchronously, the next one as soon as the registers hold this one. A lane owns a row of A or a column of B and gets its 32 inner values. kInner: rows
+// Tiles of 32 x 32 values on their way from global memory to the registers of a warp, through 4 KB of shared memory of the warp's own: copied
+// asynchronously, the next one as soon as the registers hold this one. A row of the array is a line of 128 bytes there (rows that straddle lines cost
+// the copies twice the time in the data pipe, which is what bounds this kernel); where lanes read rows, their 16-byte pieces are permuted by the row. A lane owns a row of A or a column of B and gets its 32 inner values. kInner: rows
 // of the array are inner values (their owners follow one another); else rows are owners (their inner values follow one another).
 template <bool kInner>
 struct GsTile {
     float* buffer;
+    static __device__ __forceinline__ int place(int r, int c) { return 32 * r + (kInner ? c : ((((c >> 2) ^ r) & 7) << 2) + (c & 3)); }
     // at(r): where row r of the array begins, from `base` on; `rows` x `cols` of the tile exist
     template <typename At>
     __device__ __forceinline__ void copy(const float* base, At&& at, int rows, int cols, bool wide) const {
-        constexpr int pitch = kInner ? 32 : kGsPitch;
         const int lane = threadIdx.x & 31;
         if (wide) {                                  // four rows an instruction, 16 bytes a lane
             const int c = (lane & 7) * 4;
 #pragma unroll
             for (int r = lane >> 3; r < 32; r += 4)
-                if (r < rows && c < cols) cp_async16(buffer + r * pitch + c, base + at(r) + c, 16);
+                if (r < rows && c < cols) cp_async16(buffer + place(r, c), base + at(r) + c, 16);
         } else {
 #pragma unroll 4
             for (int r = 0; r < 32; ++r)
-                if (r < rows && lane < cols) cp_async4(buffer + r * pitch + lane, base + at(r) + lane);
+                if (r < rows && lane < cols) cp_async4(buffer + place(r, lane), base + at(r) + lane);
         }
         cp_async_commit();
     }
@@ -200,7 +201,7 @@ struct GsTile {
         } else {
 #pragma unroll
             for (int c = 0; c < 32; c += 4) {
-                const float4 f = *reinterpret_cast<const float4*>(buffer + lane * kGsPitch + c);
+                const float4 f = *reinterpret_cast<const float4*>(buffer + place(lane, c));
                 v[c] = f.x; v[c + 1] = f.y; v[c + 2] = f.z; v[c + 3] = f.w;
             }
         }
@@ -245,20 +246,24 @@ __device__ __forceinline__ void gs_meet() {
 // costs up to 2^-23 of the sum. Descriptors of one step ahead are 32 bytes on, two units of their address field; 32 inner values make a part of B.
 __device__ __forceinline__ void gs_products(uint32_t d, uint32_t a_hi, uint32_t a_lo, uint32_t b, uint32_t idesc, int steps) {
     const uint64_t hi = tc5_smem_desc(b), lo = tc5_smem_desc(b + kGsHalfBytes);
-#pragma unroll 1
-    for (int k = 0; k < steps; ++k) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        if (k >= steps) break;
         const int at = (k >> 2) * (kGsPartBytes >> 4) + (k & 3) * 2;
         ts_mma(d, a_lo + 8 * k, hi + at, idesc, k > 0);
         ts_mma(d, a_hi + 8 * k, lo + at, idesc, true);
     }
-#pragma unroll 1
-    for (int k = 0; k < steps; ++k) ts_mma(d, a_hi + 8 * k, hi + (k >> 2) * (kGsPartBytes >> 4) + (k & 3) * 2, idesc, true);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        if (k >= steps) break;
+        ts_mma(d, a_hi + 8 * k, hi + (k >> 2) * (kGsPartBytes >> 4) + (k & 3) * 2, idesc, true);
+    }
 }
 
 // kWide: every row's half of a tile of the output starts on 32 bytes and is 64 columns long.
 template <bool kWide>
 struct GsLayout {
-    static constexpr int raw_at = kGsStages * kGsStageBytes, raw_floats = 32 * kGsPitch;                   // a tile for each of sixteen operand warps
+    static constexpr int raw_at = kGsStages * kGsStageBytes, raw_floats = 32 * 32;                   // a tile for each of sixteen operand warps
     static constexpr int out_at = raw_at + 16 * raw_floats * 4;
     static constexpr int smem = out_at + (kWide ? 0 : 8 * 32 * kGsOutPitch * 4) + 1024;
     static_assert(smem + 6144 <= 227 * 1024, "shared memory of one CTA per SM");
@@ -273,7 +278,7 @@ struct GsLayout {
 //                 sum over 128 inner values is off five times as far as float32) and writes its half of the row
 //   warps 20-27   B, 32 columns of 32 inner values a warp, in the same way, stored to shared memory; where a matrix has up to 128 inner values it stays for
 //                 all row tiles of its group
-// TMEM: two partial sums of 128 columns, taken in turn, and two stages of A of 128 (hi, lo). A hand-over costs its warps some hundred cycles: with steps of
+// TMEM: two stages of a partial sum of 128 columns and 128 of A (hi, lo), taken in turn. A hand-over costs its warps some hundred cycles: with steps of
 // 32 inner values and half the warps for A and B the products waited two thirds of the time (98,304 atoms of 89 elements 127 us).
 // Every wait is bounded; if one runs out, the CTA gives up, fills its remaining tiles with NaN, reports it to `status` and ends when its products
 // and copies in flight have.
@@ -282,8 +287,8 @@ __global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid
     using L = GsLayout<kWide>;
     constexpr bool kRows = kMode != kGsGradient;
     extern __shared__ unsigned char gs_smem_raw[];
-    __shared__ __align__(8) unsigned long long work_full[kGsRing], work_free[kGsRing], a_full[kGsStages], a_free[kGsStages], b_full[kGsStages], b_free[kGsStages],
-        d_full[2], d_free[2], drained;
+    // ready: a stage of A is there and its partial sum has been read; done: its products are
+    __shared__ __align__(8) unsigned long long work_full[kGsRing], work_free[kGsRing], ready[kGsStages], done[kGsStages], b_full[kGsStages], b_free[kGsStages], drained;
     __shared__ GsWork work[kGsRing];
     __shared__ __align__(16) long long row_at[16][32];                                   // where the rows of an operand warp's tile start
     __shared__ uint32_t tmem_slot;
@@ -295,8 +300,7 @@ __global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid
         guard[0] = 0;
         guard[1] = pass.expire_polls > 0 ? pass.expire_polls : static_cast<int>(kMbarSpinLimit);
         for (int q = 0; q < kGsRing; ++q) { mbar_init(&work_full[q], 1); mbar_init(&work_free[q], 25); }
-        for (int q = 0; q < kGsStages; ++q) { mbar_init(&a_full[q], 8); mbar_init(&a_free[q], 1); mbar_init(&b_full[q], 8); mbar_init(&b_free[q], 1); }
-        for (int q = 0; q < 2; ++q) { mbar_init(&d_full[q], 1); mbar_init(&d_free[q], 8); }
+        for (int q = 0; q < kGsStages; ++q) { mbar_init(&ready[q], 16); mbar_init(&done[q], 1); mbar_init(&b_full[q], 8); mbar_init(&b_free[q], 1); }
         mbar_init(&drained, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -329,18 +333,16 @@ __global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid
                 if (fresh) { base_b = nb; nb += chunks; }
 #pragma unroll 1
                 for (int j = 0; j < chunks; ++j, ++na) {
-                    const int st = na % kGsStages, n = base_b + j, bs = n % kGsStages;           // the partial sums have two stages too
-                    if (na >= 2) ok = ts_wait_warp(&d_free[st], ((na >> 1) - 1) & 1, guard);
-                    ok = ok && ts_wait_warp(&a_full[st], (na / kGsStages) & 1, guard);
+                    const int st = na % kGsStages, n = base_b + j, bs = n % kGsStages;
+                    ok = ts_wait_warp(&ready[st], (na / kGsStages) & 1, guard);
                     if (fresh) ok = ok && ts_wait_warp(&b_full[bs], (n / kGsStages) & 1, guard);
                     if (!ok) break;
                     ts_fence_after();
                     const uint32_t hi = ts_uniform(a_at + 128 * st), b = ts_uniform(b_at + bs * kGsStageBytes), d = ts_uniform(tmem + 128 * st);
                     if (leader) {
                         gs_products(d, hi, hi + 64, b, ts_idesc(cols), min(8, (inner - kGsChunk * j + 7) / 8));
-                        ts_commit(&a_free[st]);
                         if (last) ts_commit(&b_free[bs]);
-                        ts_commit(&d_full[st]);
+                        ts_commit(&done[st]);
                     }
                     __syncwarp();
                 }
@@ -369,7 +371,7 @@ __global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid
                     if (lane == 0) mbar_arrive(&work_full[slot]);
                 }
             }
-        } else if (kMode != kGsGradient && pass.zero_tail) {
+        } else if (kRows && pass.zero_tail) {
             for (long long p = pass.offsets[pass.groups] + 2LL * blockIdx.x + (warp - 2); p < pass.rows; p += 2LL * gridDim.x)
                 for (int c = lane; c < pass.out_width; c += 32) pass.out[p * pass.out_stride + c] = 0.f;
         }
@@ -387,12 +389,12 @@ __global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid
         const int tid = threadIdx.x & 127, first = tid & ~31, k_part = 32 * ((warp - 4) >> 2);   // the warp's rows and inner values are its own
         int na = 0;
         bool ok = true;
-        auto free_stage = [&]() { return na < kGsStages || ts_wait_warp(&a_free[na % kGsStages], (na / kGsStages - 1) & 1, guard); };
+        auto free_stage = [&]() { return na < kGsStages || ts_wait_warp(&done[na % kGsStages], (na / kGsStages - 1) & 1, guard); };
         auto give = [&]() {
             ts_wait_store();
             ts_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&a_full[na % kGsStages]);
+            if (lane == 0) mbar_arrive(&ready[na % kGsStages]);
             ++na;
         };
         auto put16 = [&](int q, float (&v)[16]) {
@@ -584,6 +586,7 @@ __global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid
         const int tid = threadIdx.x & 127, half = (warp - 12) >> 2;
         float* const out_stage = reinterpret_cast<float*>(stages + L::out_at) + (warp - 12) * 32 * kGsOutPitch;
         int nd = 0, at_degree = 0, at_tile = 0;      // the tile at hand, for a CTA that gives up (0, 0: none yet)
+        if (lane < kGsStages) mbar_arrive(&ready[lane]);                 // the first two sums have nothing to wait for
         bool ok = true;
         for (int i = 0;; ++i) {
             const int slot = i % kGsRing;
@@ -614,7 +617,7 @@ __global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid
 #pragma unroll
             for (int q = 0; q < 64; ++q) sum[q] = 0.f;
             for (int j = 0; j < chunks; ++j, ++nd) {
-                if (!ts_wait_warp(&d_full[nd & 1], (nd >> 1) & 1, guard)) { ok = false; break; }
+                if (!ts_wait_warp(&done[nd & 1], (nd >> 1) & 1, guard)) { ok = false; break; }
                 ts_fence_after();
                 const uint32_t from = lanes + (nd & 1) * 128 + 64 * half;
 #pragma unroll
@@ -627,7 +630,7 @@ __global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid
                     }
                 ts_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&d_free[nd & 1]);
+                if (lane == 0) mbar_arrive(&ready[nd & 1]);                  // for the step after the next one
             }
             if (!ok) break;
             if (kWide) {
