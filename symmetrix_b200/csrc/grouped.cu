@@ -156,16 +156,22 @@ void join(const smx_grouped_linear& c) {
 template <int kMode, bool kWide>
 void launch_gs(const GsPass& p, long long tiles, cudaStream_t stream) {
     const auto kernel = grouped_f32_kernel<kMode, kWide>;
-    // the warps' shares of registers are drawn from what the launch gives: fewer than planned and they would wait for ever
+    // The warps' shares of registers are drawn from what the launch gives: fewer than planned and they would wait for ever. What the kernel's own arrays
+    // leave of the shared memory starts on a multiple of 1,024 bytes.
     static std::atomic<bool> done[64];
+    static std::atomic<int> smem{0};
     if (first_on_device(done)) {
         cudaFuncAttributes a{};
         SMX_CUDA(cudaFuncGetAttributes(&a, kernel));
         if (a.numRegs < kGsRegsLaunch) throw CudaError("grouped_f32_kernel was built with too few registers");
-        SMX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, GsLayout<kWide>::smem));
+        const int own = static_cast<int>(a.sharedSizeBytes), bytes = GsLayout<kWide>::bytes + std::min(1024, GsLayout<kWide>::largest);
+        if (own > 2048) throw CudaError("grouped_f32_kernel was built with too much shared memory");
+        SMX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        smem.store(bytes, std::memory_order_relaxed);
         mark_on_device(done);
     }
-    kernel<<<static_cast<unsigned>(std::min<long long>(tiles, sm_count())), kGsThreads, GsLayout<kWide>::smem, stream>>>(p);
+    if (tiles > INT_MAX) throw ArgError("smx_grouped: too many rows");
+    kernel<<<static_cast<unsigned>(std::min<long long>(tiles, sm_count())), kGsThreads, smem.load(std::memory_order_relaxed), stream>>>(p);
     launched("grouped_f32_kernel");
 }
 
@@ -201,7 +207,6 @@ void rows_f32(const smx_grouped_linear& c, bool transposed) {
         tiles += (c.num_rows * d.comps / 128 + c.num_groups) * ((d.N + 127) / 128);
         wide = wide && d.b_off % 8 == 0 && d.N % 64 == 0;
     }
-    if (tiles > INT_MAX) throw ArgError("smx_grouped: too many rows");
     const cudaStream_t stream = static_cast<cudaStream_t>(c.stream);
     if (transposed) {
         if (wide) launch_gs<kGsBackward, true>(p, tiles, stream);
@@ -228,7 +233,6 @@ void gradient_f32(const smx_grouped_linear& c) {
         tiles += (c.num_rows * d.comps / p.chunk + c.num_groups) * ((d.N + 127) / 128) * ((d.K + 127) / 128);
         wide = wide && d.N % 64 == 0 && (reinterpret_cast<uintptr_t>(d.grad) & 31) == 0;
     }
-    if (tiles > INT_MAX) throw ArgError("smx_grouped: too many rows");
     const cudaStream_t stream = static_cast<cudaStream_t>(c.stream);
     if (wide) launch_gs<kGsGradient, true>(p, tiles, stream);
     else launch_gs<kGsGradient, false>(p, tiles, stream);

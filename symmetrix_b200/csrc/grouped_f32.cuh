@@ -15,13 +15,13 @@ namespace smx {
 namespace {
 
 enum GsMode { kGsForward, kGsBackward, kGsGradient };
-constexpr int kGsThreads = 896, kGsChunk = 64, kGsStages = 2, kGsRing = 4;   // inner values of a step; stages of A and of B; tiles in the ring
+constexpr int kGsThreads = 1024, kGsChunk = 64, kGsStages = 2, kGsRing = 4;   // inner values of a step; stages of A and of B; tiles in the ring
 constexpr int kGsPartBytes = 128 * 32 * 4, kGsHalfBytes = 2 * kGsPartBytes, kGsStageBytes = 2 * kGsHalfBytes;     // B: 32 inner values; hi or lo; both
 constexpr int kGsOutPitch = 17;                                              // floats of a row on its way out of rows that are not aligned
 constexpr int kGsStatusWait = 8;
-// the warps' shares of the registers, by fours: control, A, sums, B
-constexpr int kGsRegsLaunch = 72, kGsRegsControl = 40, kGsRegsA = 64, kGsRegsSums = 104, kGsRegsB = 64;
-static_assert(kGsRegsControl + 2 * (kGsRegsA + kGsRegsSums + kGsRegsB) <= 7 * kGsRegsLaunch, "the registers of the launch are shared out");
+// the warps' shares of the registers, by fours: control, A, sums, B, copies
+constexpr int kGsRegsLaunch = 64, kGsRegsControl = 40, kGsRegsOperand = 56, kGsRegsSums = 104, kGsRegsCopies = 40;
+static_assert(kGsRegsControl + 4 * kGsRegsOperand + 2 * kGsRegsSums + kGsRegsCopies <= 8 * kGsRegsLaunch, "the registers of the launch are shared out");
 
 struct GsDegree {
     int comps, K, N;                 // rows passes: inner values and columns; gradient: rows and columns of the matrices
@@ -166,35 +166,34 @@ __device__ __forceinline__ void gs_row(const GsWork& w, int comps, int i, int& p
     comp = static_cast<int>(r - ahead * comps);
 }
 
-// Tiles of 32 x 32 values on their way from global memory to the registers of a warp, through 4 KB of shared memory of the warp's own: copied
-// asynchronously, the next one as soon as the registers hold this one. A row of the array is a line of 128 bytes there (rows that straddle lines cost
-// the copies twice the time in the data pipe, which is what bounds this kernel); where lanes read rows, their 16-byte pieces are permuted by the row. A lane owns a row of A or a column of B and gets its 32 inner values. kInner: rows
-// of the array are inner values (their owners follow one another); else rows are owners (their inner values follow one another).
+// Tiles of 32 x 32 values on their way from global memory to the registers of an operand warp, through 4 KB of shared memory each. A row of the array is a
+// line of 128 bytes there. kInner: rows are inner values, and a lane owns a column; else a lane owns a row, and its 16-byte pieces are permuted by the row.
 template <bool kInner>
 struct GsTile {
-    float* buffer;
     static __device__ __forceinline__ int place(int r, int c) { return 32 * r + (kInner ? c : ((((c >> 2) ^ r) & 7) << 2) + (c & 3)); }
-    // at(r): where row r of the array begins, from `base` on; `rows` x `cols` of the tile exist
-    template <typename At>
-    __device__ __forceinline__ void copy(const float* base, At&& at, int rows, int cols, bool wide) const {
+    // `rows` x `cols` of the tile exist. at(u): where row lane / 8 + 4 u begins, if `wide` (four rows an instruction, 16 bytes a lane); row_at(r): row r
+    template <typename At, typename RowAt>
+    static __device__ __forceinline__ void copy(float* buffer, const float* base, int rows, int cols, bool wide, At&& at, RowAt&& row_at) {
         const int lane = threadIdx.x & 31;
-        if (wide) {                                  // four rows an instruction, 16 bytes a lane
+        if (wide) {
             const int c = (lane & 7) * 4;
 #pragma unroll
-            for (int r = lane >> 3; r < 32; r += 4)
-                if (r < rows && c < cols) cp_async16(buffer + place(r, c), base + at(r) + c, 16);
+            for (int u = 0; u < 8; ++u) {
+                const int r = (lane >> 3) + 4 * u;
+                const long long from = at(u);
+                if (r < rows && c < cols) cp_async16(buffer + place(r, c), base + from + c, 16);
+            }
         } else {
-#pragma unroll 4
-            for (int r = 0; r < 32; ++r)
-                if (r < rows && lane < cols) cp_async4(buffer + place(r, lane), base + at(r) + lane);
+#pragma unroll 2
+            for (int r = 0; r < 32; ++r) {
+                const long long from = row_at(r);
+                if (r < rows && lane < cols) cp_async4(buffer + place(r, lane), base + from + lane);
+            }
         }
-        cp_async_commit();
     }
     // the lane's values, zero where the tile has none
-    __device__ __forceinline__ void read(int rows, int cols, float (&v)[32]) const {
+    static __device__ __forceinline__ void read(const float* buffer, int rows, int cols, float (&v)[32]) {
         const int lane = threadIdx.x & 31;
-        cp_async_wait<0>();
-        __syncwarp();
         if (kInner) {
 #pragma unroll
             for (int r = 0; r < 32; ++r) v[r] = buffer[32 * r + lane];
@@ -205,13 +204,16 @@ struct GsTile {
                 v[c] = f.x; v[c + 1] = f.y; v[c + 2] = f.z; v[c + 3] = f.w;
             }
         }
-        __syncwarp();                                // the next copies may come in
         const int good = kInner ? (lane < cols ? rows : 0) : (lane < rows ? cols : 0);
         if (good < 32)
 #pragma unroll
             for (int e = 0; e < 32; ++e) v[e] = e < good ? v[e] : 0.f;
     }
 };
+// Arrives when the thread's copies so far have.
+__device__ __forceinline__ void gs_arrive_behind_copies(unsigned long long* bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
 
 // NaN into a warp's part of a tile, 32 rows of 64 columns.
 template <int kMode>
@@ -239,7 +241,7 @@ __device__ __forceinline__ void gs_split(float v, float& hi, float& lo) {
 __device__ __forceinline__ void gs_meet() {
     __syncwarp();
     ts_fence_before();
-    asm volatile("bar.sync 1, 896;" ::: "memory");
+    asm volatile("bar.sync 1, 1024;" ::: "memory");
 }
 
 // D of one step, its inner values 8 at a time. The remainders' products come first, while the sum is small: the tensor core cuts its sums, so an addition
@@ -263,21 +265,25 @@ __device__ __forceinline__ void gs_products(uint32_t d, uint32_t a_hi, uint32_t 
 // kWide: every row's half of a tile of the output starts on 32 bytes and is 64 columns long.
 template <bool kWide>
 struct GsLayout {
-    static constexpr int raw_at = kGsStages * kGsStageBytes, raw_floats = 32 * 32;                   // a tile for each of sixteen operand warps
-    static constexpr int out_at = raw_at + 16 * raw_floats * 4;
-    static constexpr int smem = out_at + (kWide ? 0 : 8 * 32 * kGsOutPitch * 4) + 1024;
-    static_assert(smem + 6144 <= 227 * 1024, "shared memory of one CTA per SM");
+    static constexpr int raw_a = kWide ? 2 : 1;                                                            // tiles that an A warp's rows have room for
+    static constexpr int raw_at = kGsStages * kGsStageBytes, tile_floats = 32 * 32;
+    static constexpr int out_at = raw_at + 8 * (raw_a + 1) * tile_floats * 4;
+    static constexpr int bytes = out_at + (kWide ? 0 : 8 * 32 * kGsOutPitch * 4);
+    static constexpr int largest = 227 * 1024 - 2048 - bytes;                                              // what the kernel's own arrays may take, with the alignment
+    static_assert(largest >= 1024, "shared memory of one CTA per SM");
 };
 
 // One persistent CTA per SM walks its share of the tiles, 64 inner values a step; its warps are specialised, so that the parts of neighbouring tiles overlap:
 //   warp 0        the products (one thread)
 //   warp 1        finds the tiles (a ring, ahead of all others)
 //   warps 2, 3    zeros into the rows behind the last group
-//   warps 4-11    A, 32 rows of 32 inner values a warp: copied while the ones before are split and stored to tensor memory
+//   warps 4-11    A, 32 rows of 32 inner values a warp, split and stored to tensor memory
 //   warps 12-19   a thread adds half of its row's partial sums of every step in registers (the tensor core cuts its sums instead of rounding them: one
 //                 sum over 128 inner values is off five times as far as float32) and writes its half of the row
-//   warps 20-27   B, 32 columns of 32 inner values a warp, in the same way, stored to shared memory; where a matrix has up to 128 inner values it stays for
-//                 all row tiles of its group
+//   warps 20-27   B, 32 columns of 32 inner values a warp, split and stored to shared memory; where a matrix has up to 128 inner values it stays for all
+//                 row tiles of its group
+//   warps 28-31   copies for both: a copy takes the time that memory needs for it to be issued (200 to 300 cycles for 512 bytes), and operand warps
+//                 that issued their own waited for that 2,000 to 2,900 of 4,300 cycles a step
 // TMEM: two stages of a partial sum of 128 columns and 128 of A (hi, lo), taken in turn. A hand-over costs its warps some hundred cycles: with steps of
 // 32 inner values and half the warps for A and B the products waited two thirds of the time (98,304 atoms of 89 elements 127 us).
 // Every wait is bounded; if one runs out, the CTA gives up, fills its remaining tiles with NaN, reports it to `status` and ends when its products
@@ -286,11 +292,12 @@ template <int kMode, bool kWide>
 __global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid_constant__ GsPass pass) {
     using L = GsLayout<kWide>;
     constexpr bool kRows = kMode != kGsGradient;
+    constexpr int kRawA = L::raw_a;
     extern __shared__ unsigned char gs_smem_raw[];
-    // ready: a stage of A is there and its partial sum has been read; done: its products are
-    __shared__ __align__(8) unsigned long long work_full[kGsRing], work_free[kGsRing], ready[kGsStages], done[kGsStages], b_full[kGsStages], b_free[kGsStages], drained;
+    // ready: a stage of A is there and its partial sum has been read; done: its products are; raw_*: tiles of the operand warps, A's first
+    __shared__ __align__(8) unsigned long long work_full[kGsRing], work_free[kGsRing], ready[kGsStages], done[kGsStages], b_full[kGsStages], b_free[kGsStages],
+        raw_full[8 * (kRawA + 1)], raw_free[8 * (kRawA + 1)], drained;
     __shared__ GsWork work[kGsRing];
-    __shared__ __align__(16) long long row_at[16][32];                                   // where the rows of an operand warp's tile start
     __shared__ uint32_t tmem_slot;
     __shared__ int guard[2];                                                             // a wait ran out; polls of a wait
     const int warp = ts_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -299,8 +306,9 @@ __global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid
     if (threadIdx.x == 0) {
         guard[0] = 0;
         guard[1] = pass.expire_polls > 0 ? pass.expire_polls : static_cast<int>(kMbarSpinLimit);
-        for (int q = 0; q < kGsRing; ++q) { mbar_init(&work_full[q], 1); mbar_init(&work_free[q], 25); }
+        for (int q = 0; q < kGsRing; ++q) { mbar_init(&work_full[q], 1); mbar_init(&work_free[q], 29); }
         for (int q = 0; q < kGsStages; ++q) { mbar_init(&ready[q], 16); mbar_init(&done[q], 1); mbar_init(&b_full[q], 8); mbar_init(&b_free[q], 1); }
+        for (int q = 0; q < 8 * (kRawA + 1); ++q) { mbar_init(&raw_full[q], 32); mbar_init(&raw_free[q], 1); }
         mbar_init(&drained, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -384,7 +392,7 @@ __global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid
             if (lane == 0 && pass.status) atomicMax(pass.status, kGsStatusWait);
         }
     } else if (warp < 12) {
-        ts_registers_less<kGsRegsA>();
+        ts_registers_less<kGsRegsOperand>();
         const uint32_t lanes = a_at + (static_cast<uint32_t>((warp & 3) * 32) << 16);
         const int tid = threadIdx.x & 127, first = tid & ~31, k_part = 32 * ((warp - 4) >> 2);   // the warp's rows and inner values are its own
         int na = 0;
@@ -405,180 +413,165 @@ __global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid
             ts_store16(to, hi);
             ts_store16(to + 64, v);
         };
-        const GsTile<!kRows> tile{raw + (warp - 4) * L::raw_floats};
-        long long* const table = row_at[warp - 4];
-        // the chunk that is copied: tile i - 1, chunk j
-        int i = 0, j = 0, chunks = 0, inner = 0, owned = 0, comps = 1, comp = 0, width = 0;
-        long long pair = 0;
-        const float* base = nullptr;
-        bool wide = false;
-        auto advance = [&]() {
-            ++j;
-            while (j >= chunks) {
-                const int slot = i % kGsRing;
-                if (!ts_wait_warp(&work_full[slot], (i / kGsRing) & 1, guard)) { ok = false; return false; }
-                const GsWork& w = work[slot];
-                const int found = w.found;
-                if (found) {
-                    const GsDegree& d = pass.degree[w.degree];
-                    chunks = w.chunks; inner = w.inner;
-                    owned = min(32, w.rows - first);
-                    comps = d.comps; width = d.K;
-                    wide = ((static_cast<unsigned long long>(pass.a_stride | d.a_off | d.K) * 4u | reinterpret_cast<uintptr_t>(pass.a)) & 15) == 0;
-                    int at;
-                    gs_row(w, comps, kRows ? first + lane : k_part + lane, at, comp);
-                    pair = at;
-                    base = pass.a + d.a_off + (kRows ? k_part : 128 * w.mtile + first);
-                    if (kRows) table[lane] = pair * pass.a_stride + static_cast<long long>(comp) * width;
+        const int mine = warp - 4;                                       // tiles mine, mine + 8
+        for (int i = 0; ok; ++i) {
+            const int slot = i % kGsRing;
+            if (!ts_wait_warp(&work_full[slot], (i / kGsRing) & 1, guard)) break;
+            const int found = work[slot].found, chunks = work[slot].chunks, inner = work[slot].inner, owned = min(32, work[slot].rows - first);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&work_free[slot]);
+            if (!found) break;
+#pragma unroll 1
+            for (int j = 0; j < chunks; ++j) {
+                const int left = inner - j * kGsChunk - k_part, place = mine + 8 * (na % kRawA);
+                if (!ts_wait_warp(&raw_full[place], (na / kRawA) & 1, guard)) { ok = false; break; }
+                float v[32];
+                if (kRows) GsTile<false>::read(raw + place * L::tile_floats, owned, left, v);
+                else GsTile<true>::read(raw + place * L::tile_floats, left, owned, v);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&raw_free[place]);
+                if (!free_stage()) { ok = false; break; }
+                ts_fence_after();
+#pragma unroll
+                for (int q = 0; q < 32; q += 16) {
+                    float part[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) part[e] = v[q + e];
+                    put16(q, part);
                 }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&work_free[slot]);
-                if (!found) return false;
-                ++i;
-                j = 0;
+                give();
             }
-            return true;
-        };
-        auto copy = [&]() {
-            const int left = inner - j * kGsChunk - k_part;
-            if constexpr (kRows) {
-                const float* from = base + j * kGsChunk;
-                tile.copy(from, [&](int r) { return table[r]; }, owned, left, wide);
-            } else {
-                __syncwarp();
-                table[lane] = pair * pass.a_stride + static_cast<long long>(comp) * width;
-                comp += kGsChunk % comps; pair += kGsChunk / comps;
-                if (comp >= comps) { comp -= comps; ++pair; }
-                __syncwarp();
-                tile.copy(base, [&](int r) { return table[r]; }, left, owned, wide);
+        }
+        gs_meet();
+    } else if (warp >= 28) {
+        ts_registers_less<kGsRegsCopies>();
+        // Rows 32 q .. of A and columns 32 q .. of B, for the operand warps q and q + 4 of each.
+        const int q = warp - 28, first = 32 * q;
+        int na = 0, nb = 0;                                              // steps so far, and those with a B of their own
+        bool ok = true;
+        for (int i = 0; ok; ++i) {
+            const int slot = i % kGsRing;
+            if (!ts_wait_warp(&work_full[slot], (i / kGsRing) & 1, guard)) break;
+            const GsWork& w = work[slot];
+            const int found = w.found, chunks = w.chunks, inner = w.inner, degree = w.degree, fresh = w.fresh;
+            const int owned_a = min(32, w.rows - first);
+            int comp = 0, pair = 0, owned_b = 0;
+            const float *a_base = nullptr, *b_base = nullptr;
+            long long mine = 0;                                          // rows passes: where the lane's row of A begins
+            if (found) {
+                const GsDegree& d = pass.degree[degree];
+                owned_b = min(32, d.N - 128 * w.block - first);
+                gs_row(w, d.comps, kRows ? first + lane : lane, pair, comp);
+                const float* matrix = d.w + static_cast<long long>(w.group) * d.K * d.N;
+                if (kRows) {
+                    mine = pair * pass.a_stride + static_cast<long long>(comp) * d.K;
+                    a_base = pass.a + d.a_off;
+                    b_base = kMode == kGsForward ? matrix + 128 * w.block + first : matrix + static_cast<long long>(128 * w.block + first) * d.K;
+                } else {
+                    a_base = pass.a + d.a_off + 128 * w.mtile + first;
+                    b_base = pass.b + d.b_off + 128 * w.block + first;
+                }
             }
-        };
-        bool have = advance();
-        if (have) copy();
-        while (have && ok) {
-            const int left = inner - j * kGsChunk - k_part;
-            float v[32];
-            if (kRows) tile.read(owned, left, v);
-            else tile.read(left, owned, v);
-            have = advance();
-            if (have) copy();
-            if (!ok || !free_stage()) { ok = false; break; }
-            ts_fence_after();
-#pragma unroll
-            for (int q = 0; q < 32; q += 16) {
-                float part[16];
-#pragma unroll
-                for (int e = 0; e < 16; ++e) part[e] = v[q + e];
-                put16(q, part);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&work_free[slot]);
+            if (!found) break;
+            const GsDegree& d = pass.degree[degree];
+            const bool wide_a = ((static_cast<unsigned long long>(pass.a_stride | d.a_off | d.K) * 4u | reinterpret_cast<uintptr_t>(pass.a)) & 15) == 0;
+            const bool wide_b = kMode == kGsGradient ? ((static_cast<unsigned long long>(pass.b_stride | d.b_off | d.N) * 4u | reinterpret_cast<uintptr_t>(pass.b)) & 15) == 0
+                                                     : ((static_cast<unsigned long long>(kMode == kGsForward ? d.N : d.K) * 4u | reinterpret_cast<uintptr_t>(d.w)) & 15) == 0;
+            auto shared_row = [&](long long v) { return [v](int r) { return __shfl_sync(0xffffffffu, v, r); }; };
+            auto place_of = [&](int part, int n, int room) { return q + 4 * part + 8 * (n % room); };
+#pragma unroll 1
+            for (int j = 0; j < chunks && ok; ++j, ++na) {
+#pragma unroll 1
+                for (int part = 0; part < 2; ++part) {
+                    const int k = j * kGsChunk + 32 * part, left = inner - k;
+                    {
+                        const int place = place_of(part, na, kRawA);
+                        if (na >= kRawA && !ts_wait_warp(&raw_free[place], (na / kRawA - 1) & 1, guard)) { ok = false; break; }
+                        float* const to = raw + place * L::tile_floats;
+                        if constexpr (kRows) {
+                            const auto row = shared_row(mine);
+                            GsTile<false>::copy(to, a_base + k, owned_a, left, wide_a, [&](int u) { return row((lane >> 3) + 4 * u); }, row);
+                        } else {
+                            const auto row = shared_row(pair * pass.a_stride + static_cast<long long>(comp) * d.K);
+                            GsTile<true>::copy(to, a_base, left, owned_a, wide_a, [&](int u) { return row((lane >> 3) + 4 * u); }, row);
+                        }
+                        gs_arrive_behind_copies(&raw_full[place]);
+                    }
+                    if (fresh) {
+                        const int place = 8 * kRawA + q + 4 * part;
+                        if (nb > 0 && !ts_wait_warp(&raw_free[place], (nb - 1) & 1, guard)) { ok = false; break; }
+                        float* const to = raw + place * L::tile_floats;
+                        if constexpr (kMode == kGsForward) {
+                            const long long step = d.N;
+                            GsTile<true>::copy(to, b_base + k * step, left, owned_b, wide_b, [&](int u) { return ((lane >> 3) + 4 * u) * step; }, [&](int r) { return r * step; });
+                        } else if constexpr (kMode == kGsBackward) {
+                            const long long step = d.K;
+                            GsTile<false>::copy(to, b_base + k, owned_b, left, wide_b, [&](int u) { return ((lane >> 3) + 4 * u) * step; }, [&](int r) { return r * step; });
+                        } else {
+                            const auto row = shared_row(pair * pass.b_stride + static_cast<long long>(comp) * d.N);
+                            GsTile<true>::copy(to, b_base, left, owned_b, wide_b, [&](int u) { return row((lane >> 3) + 4 * u); }, row);
+                        }
+                        gs_arrive_behind_copies(&raw_full[place]);
+                    }
+                    if (!kRows) {
+                        comp += 32 % d.comps; pair += 32 / d.comps;
+                        if (comp >= d.comps) { comp -= d.comps; ++pair; }
+                    }
+                }
+                if (fresh) ++nb;
             }
-            give();
         }
         asm volatile("cp.async.wait_all;" ::: "memory");                 // none may be in flight when the CTA ends
         gs_meet();
     } else if (warp >= 20) {
-        ts_registers_less<kGsRegsB>();
+        ts_registers_less<kGsRegsOperand>();
         const int first = 32 * (warp & 3), part = (warp - 20) >> 2, k_part = 32 * part;          // the warp's columns and inner values are its own
-        const GsTile<kMode != kGsBackward> tile{raw + (warp - 12) * L::raw_floats};
-        long long* const table = row_at[warp - 12];
-        // the chunk that is copied: tile i - 1, chunk j. `crosses`: the tile behind this one has a matrix of its own
-        int i = 0, j = 0, chunks = 0, inner = 0, owned = 0, cols = 0, comps = 1, comp = 0, width = 0, nb = 0;
-        long long pair = 0;
-        const float* base = nullptr;
-        bool ok = true, wide = false, crosses = false;
-        auto advance = [&]() {
-            ++j;
-            while (j >= chunks) {
-                const int slot = i % kGsRing;
-                if (!ts_wait_warp(&work_full[slot], (i / kGsRing) & 1, guard)) { ok = false; return false; }
-                const GsWork& w = work[slot];
-                const int found = w.found;
-                j = chunks = 0;
-                if (found && w.fresh) {
-                    const GsDegree& d = pass.degree[w.degree];
-                    const int left = min(128, d.N - 128 * w.block);
-                    chunks = w.chunks; inner = w.inner; crosses = w.last != 0;
-                    cols = ((left + 15) & ~15) - first;
-                    owned = min(32, left - first);
-                    const float* matrix = d.w + static_cast<long long>(w.group) * d.K * d.N;
-                    if (kMode == kGsForward) {
-                        width = d.N;
-                        base = matrix + static_cast<long long>(k_part) * width + 128 * w.block + first;
-                    } else if (kMode == kGsBackward) {
-                        width = d.K;
-                        base = matrix + static_cast<long long>(128 * w.block + first) * width + k_part;
-                    } else {
-                        width = d.N; comps = d.comps;
-                        int at;
-                        gs_row(w, comps, k_part + lane, at, comp);
-                        pair = at;
-                        base = pass.b + d.b_off + 128 * w.block + first;
-                    }
-                    wide = kMode == kGsGradient ? ((static_cast<unsigned long long>(pass.b_stride | d.b_off | width) * 4u | reinterpret_cast<uintptr_t>(pass.b)) & 15) == 0
-                                                : ((static_cast<unsigned long long>(width) * 4u | reinterpret_cast<uintptr_t>(d.w)) & 15) == 0;
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&work_free[slot]);
-                if (!found) return false;
-                ++i;
-            }
-            return true;
-        };
-        auto copy = [&]() {
-            const int left = inner - j * kGsChunk - k_part;
-            if constexpr (kMode == kGsForward) {
-                tile.copy(base + static_cast<long long>(j) * kGsChunk * width, [&](int r) { return static_cast<long long>(r) * width; }, left, owned, wide);
-            } else if constexpr (kMode == kGsBackward) {
-                tile.copy(base + j * kGsChunk, [&](int r) { return static_cast<long long>(r) * width; }, owned, left, wide);
-            } else {
-                __syncwarp();
-                table[lane] = pair * pass.b_stride + static_cast<long long>(comp) * width;
-                comp += kGsChunk % comps; pair += kGsChunk / comps;
-                if (comp >= comps) { comp -= comps; ++pair; }
-                __syncwarp();
-                tile.copy(base, [&](int r) { return table[r]; }, left, owned, wide);
-            }
-        };
-        bool have = advance();
-        if (have) copy();
-        while (have && ok) {
-            const int left = inner - j * kGsChunk - k_part, stored = cols;
-            float v[32];
-            if (kMode == kGsBackward) tile.read(owned, left, v);
-            else tile.read(left, owned, v);
-            // The next chunk is on its way while this one is stored, unless it belongs to a tile that other tiles of this matrix come before: the ring may not
-            // hold them all, and they need this chunk.
-            const bool early = j + 1 < chunks || crosses;
-            if (early) {
-                have = advance();
-                if (have) copy();
-            }
-            const int bs = nb % kGsStages;
-            if (!ok || (pass.expire_polls > 0 && nb > 0)) { ok = false; break; }
-            if (nb >= kGsStages && !ts_wait_warp(&b_free[bs], (nb / kGsStages - 1) & 1, guard)) { ok = false; break; }
-            unsigned char* const to = stages + bs * kGsStageBytes + part * kGsPartBytes;
-            if (lane < stored) {
-#pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    float4 hi, lo;
-                    gs_split(v[4 * c], hi.x, lo.x);
-                    gs_split(v[4 * c + 1], hi.y, lo.y);
-                    gs_split(v[4 * c + 2], hi.z, lo.z);
-                    gs_split(v[4 * c + 3], hi.w, lo.w);
-                    const int off = tc5_swizzled_group(first + lane, c);
-                    *reinterpret_cast<float4*>(to + off) = hi;
-                    *reinterpret_cast<float4*>(to + kGsHalfBytes + off) = lo;
-                }
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        const int place = 8 * kRawA + warp - 20;
+        int nb = 0;
+        bool ok = true;
+        for (int i = 0; ok; ++i) {
+            const int slot = i % kGsRing;
+            if (!ts_wait_warp(&work_full[slot], (i / kGsRing) & 1, guard)) break;
+            const GsWork& w = work[slot];
+            const int found = w.found, chunks = w.fresh ? w.chunks : 0, inner = w.inner;
+            const int left = found ? min(128, pass.degree[w.degree].N - 128 * w.block) : 0, cols = ((left + 15) & ~15) - first, owned = min(32, left - first);
             __syncwarp();
-            if (lane == 0) mbar_arrive(&b_full[bs]);
-            ++nb;
-            if (!early) {
-                have = advance();
-                if (have) copy();
+            if (lane == 0) mbar_arrive(&work_free[slot]);
+            if (!found) break;
+#pragma unroll 1
+            for (int j = 0; j < chunks; ++j) {
+                const int good = inner - j * kGsChunk - k_part;
+                if (!ts_wait_warp(&raw_full[place], nb & 1, guard)) { ok = false; break; }
+                float v[32];
+                if (kMode == kGsBackward) GsTile<false>::read(raw + place * L::tile_floats, owned, good, v);
+                else GsTile<true>::read(raw + place * L::tile_floats, good, owned, v);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&raw_free[place]);
+                const int bs = nb % kGsStages;
+                if (pass.expire_polls > 0 && nb > 0) { ok = false; break; }
+                if (nb >= kGsStages && !ts_wait_warp(&b_free[bs], (nb / kGsStages - 1) & 1, guard)) { ok = false; break; }
+                unsigned char* const to = stages + bs * kGsStageBytes + part * kGsPartBytes;
+                if (lane < cols) {
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        float4 hi, lo;
+                        gs_split(v[4 * c], hi.x, lo.x);
+                        gs_split(v[4 * c + 1], hi.y, lo.y);
+                        gs_split(v[4 * c + 2], hi.z, lo.z);
+                        gs_split(v[4 * c + 3], hi.w, lo.w);
+                        const int off = tc5_swizzled_group(first + lane, c);
+                        *reinterpret_cast<float4*>(to + off) = hi;
+                        *reinterpret_cast<float4*>(to + kGsHalfBytes + off) = lo;
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&b_full[bs]);
+                ++nb;
             }
         }
-        asm volatile("cp.async.wait_all;" ::: "memory");
         gs_meet();
     } else {
         ts_registers_more<kGsRegsSums>();
