@@ -15,12 +15,12 @@ namespace smx {
 namespace {
 
 enum GsMode { kGsForward, kGsBackward, kGsGradient };
-constexpr int kGsThreads = 1024, kGsChunk = 64, kGsStages = 2, kGsRing = 4;   // inner values of a step; stages of A and of B; tiles in the ring
+constexpr int kGsThreads = 1024, kGsChunk = 64, kGsStages = 2, kGsRing = 8;   // inner values of a step; stages of A and of B; tiles in the ring
 constexpr int kGsPartBytes = 128 * 32 * 4, kGsHalfBytes = 2 * kGsPartBytes, kGsStageBytes = 2 * kGsHalfBytes;     // B: 32 inner values; hi or lo; both
 constexpr int kGsOutPitch = 17;                                              // floats of a row on its way out of rows that are not aligned
 constexpr int kGsStatusWait = 8;
 // the warps' shares of the registers, by fours: control, A, sums, B, copies
-constexpr int kGsRegsLaunch = 64, kGsRegsControl = 40, kGsRegsOperand = 56, kGsRegsSums = 104, kGsRegsCopies = 40;
+constexpr int kGsRegsLaunch = 64, kGsRegsControl = 40, kGsRegsOperand = 56, kGsRegsSums = 96, kGsRegsCopies = 56;
 static_assert(kGsRegsControl + 4 * kGsRegsOperand + 2 * kGsRegsSums + kGsRegsCopies <= 8 * kGsRegsLaunch, "the registers of the launch are shared out");
 
 struct GsDegree {
@@ -88,73 +88,86 @@ __device__ __forceinline__ void gs_share(const GsPass& p, int& begin, int& end) 
 
 // Finds the tiles of a degree in ascending order: groups, then where a tile's B stays for the next ones column blocks and row tiles, else row tiles and
 // column blocks (neighbours then read the same rows).
+// The bounds of 32 groups stay in a warp's registers: read and added up for every tile, they would take as long as the products of a short one.
 struct GsCursor {
     int q = -1, g0 = 0, run = 0, parts = 0;          // tiles and partial sums of the groups before g0
+    int end = 0, first, count, runs, begin, part;    // tiles up to the last of the 32 groups; the lane's group
+    template <int kMode>
+    __device__ __forceinline__ void look(const GsPass& p, const GsDegree& d) {
+        const int lane = threadIdx.x & 31, g = g0 + lane;
+        first = count = runs = 0;
+        if (g < p.groups) {
+            first = p.offsets[g];
+            count = p.offsets[g + 1] - first;
+            runs = gs_runs<kMode>(p, d, count);
+        }
+        const int mine = runs * gs_plane<kMode>(d), split = kMode == kGsGradient && runs > 1 ? runs : 0;
+        int incl = mine, incl_parts = split;
+#pragma unroll
+        for (int s = 1; s < 32; s <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, incl, s);
+            if (lane >= s) incl += up;
+            if (kMode == kGsGradient) {
+                const int up_parts = __shfl_up_sync(0xffffffffu, incl_parts, s);
+                if (lane >= s) incl_parts += up_parts;
+            }
+        }
+        begin = run + incl - mine;
+        part = parts + incl_parts - split;
+        end = run + __shfl_sync(0xffffffffu, incl, 31);
+        parts += __shfl_sync(0xffffffffu, incl_parts, 31);
+    }
     template <int kMode>
     __device__ __forceinline__ bool find(const GsPass& p, int degree, int t, GsWork& w) {
-        const int lane = threadIdx.x & 31;
-        if (degree != q) { q = degree; g0 = run = parts = 0; }
-        const GsDegree& d = p.degree[q];
-        const int plane = gs_plane<kMode>(d), blocks = (d.N + 127) / 128;
-        for (; g0 < p.groups; g0 += 32) {
-            const int g = g0 + lane;
-            int first = 0, count = 0, runs = 0;
-            if (g < p.groups) {
-                first = p.offsets[g];
-                count = p.offsets[g + 1] - first;
-                runs = gs_runs<kMode>(p, d, count);
-            }
-            const int split = kMode == kGsGradient && runs > 1 ? runs : 0;
-            int incl = runs * plane, incl_parts = split;
-#pragma unroll
-            for (int s = 1; s < 32; s <<= 1) {
-                const int up = __shfl_up_sync(0xffffffffu, incl, s), up_parts = __shfl_up_sync(0xffffffffu, incl_parts, s);
-                if (lane >= s) { incl += up; incl_parts += up_parts; }
-            }
-            const int begin = run + incl - runs * plane;
-            const unsigned hit = __ballot_sync(0xffffffffu, t >= begin && t < run + incl);
-            if (hit) {
-                const int src = __ffs(hit) - 1;
-                const int local = t - __shfl_sync(0xffffffffu, begin, src);
-                runs = __shfl_sync(0xffffffffu, runs, src);
-                count = __shfl_sync(0xffffffffu, count, src);
-                const long long rows = static_cast<long long>(count) * d.comps;
-                w.found = 1; w.degree = q; w.tile = t; w.group = g0 + src;
-                w.first_pair = __shfl_sync(0xffffffffu, first, src);
-                w.fresh = w.last = 1;
-                if (kMode == kGsGradient) {
-                    const int at = local / plane, in_plane = local - at * plane;
-                    w.mtile = in_plane / blocks;
-                    w.block = in_plane - w.mtile * blocks;
-                    w.row0 = static_cast<long long>(at) * p.chunk;
-                    w.rows = min(128, d.K - 128 * w.mtile);
-                    w.inner = static_cast<int>(min(static_cast<long long>(p.chunk), rows - w.row0));
-                    const long long part = parts + __shfl_sync(0xffffffffu, incl_parts - split, src) + at;
-                    float* to = runs == 1 ? d.grad + static_cast<long long>(w.group) * d.K * d.N : d.part + part * d.K * d.N;
-                    w.out = to + 128LL * w.mtile * d.N + 128 * w.block;
-                } else {
-                    int at;
-                    if (gs_resident<kMode>(d)) {
-                        w.block = local / runs;
-                        at = local - w.block * runs;
-                        w.last = at + 1 == runs;
-                    } else {
-                        at = local / blocks;
-                        w.block = local - at * blocks;
-                    }
-                    w.mtile = 0;
-                    w.row0 = static_cast<long long>(at) * 128;
-                    w.rows = static_cast<int>(min(128LL, rows - w.row0));
-                    w.inner = d.K;
-                }
-                w.chunks = (w.inner + kGsChunk - 1) / kGsChunk;
-                return true;
-            }
-            run += __shfl_sync(0xffffffffu, incl, 31);
-            parts += __shfl_sync(0xffffffffu, incl_parts, 31);
+        const GsDegree& d = p.degree[degree];
+        if (degree != q) {
+            q = degree;
+            g0 = run = parts = 0;
+            look<kMode>(p, d);
         }
-        w.found = 0;
-        return false;
+        while (t >= end) {
+            g0 += 32;
+            run = end;
+            if (g0 >= p.groups) { w.found = 0; return false; }
+            look<kMode>(p, d);
+        }
+        const int src = __ffs(__ballot_sync(0xffffffffu, t >= begin && t < begin + runs * gs_plane<kMode>(d))) - 1;
+        const int local = t - __shfl_sync(0xffffffffu, begin, src), group_runs = __shfl_sync(0xffffffffu, runs, src);
+        const long long rows = static_cast<long long>(__shfl_sync(0xffffffffu, count, src)) * d.comps;
+        const int blocks = (d.N + 127) / 128;
+        w.found = 1; w.degree = q; w.tile = t; w.group = g0 + src;
+        w.first_pair = __shfl_sync(0xffffffffu, first, src);
+        w.fresh = w.last = 1;
+        if (kMode == kGsGradient) {
+            const int plane = gs_plane<kMode>(d), at = local / plane, in_plane = local - at * plane;
+            w.mtile = in_plane / blocks;
+            w.block = in_plane - w.mtile * blocks;
+            w.row0 = static_cast<long long>(at) * p.chunk;
+            w.rows = min(128, d.K - 128 * w.mtile);
+            w.inner = static_cast<int>(min(static_cast<long long>(p.chunk), rows - w.row0));
+            const long long place = __shfl_sync(0xffffffffu, part, src) + at;
+            float* to = group_runs == 1 ? d.grad + static_cast<long long>(w.group) * d.K * d.N : d.part + place * d.K * d.N;
+            w.out = to + 128LL * w.mtile * d.N + 128 * w.block;
+        } else {
+            int at = local;
+            w.block = 0;
+            if (gs_resident<kMode>(d)) {
+                if (blocks > 1) {
+                    w.block = local / group_runs;
+                    at = local - w.block * group_runs;
+                }
+                w.last = at + 1 == group_runs;
+            } else if (blocks > 1) {
+                at = local / blocks;
+                w.block = local - at * blocks;
+            }
+            w.mtile = 0;
+            w.row0 = static_cast<long long>(at) * 128;
+            w.rows = static_cast<int>(min(128LL, rows - w.row0));
+            w.inner = d.K;
+        }
+        w.chunks = (w.inner + kGsChunk - 1) / kGsChunk;
+        return true;
     }
 };
 
@@ -479,6 +492,11 @@ __global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid
             const bool wide_a = ((static_cast<unsigned long long>(pass.a_stride | d.a_off | d.K) * 4u | reinterpret_cast<uintptr_t>(pass.a)) & 15) == 0;
             const bool wide_b = kMode == kGsGradient ? ((static_cast<unsigned long long>(pass.b_stride | d.b_off | d.N) * 4u | reinterpret_cast<uintptr_t>(pass.b)) & 15) == 0
                                                      : ((static_cast<unsigned long long>(kMode == kGsForward ? d.N : d.K) * 4u | reinterpret_cast<uintptr_t>(d.w)) & 15) == 0;
+            long long ahead[8];                                          // rows passes: where the rows that the lane copies begin
+            if (kRows)
+#pragma unroll
+                for (int u = 0; u < 8; ++u) ahead[u] = __shfl_sync(0xffffffffu, mine, (lane >> 3) + 4 * u);
+            const int comps_more = 32 % d.comps, pairs_more = 32 / d.comps;
             auto shared_row = [&](long long v) { return [v](int r) { return __shfl_sync(0xffffffffu, v, r); }; };
             auto place_of = [&](int part, int n, int room) { return q + 4 * part + 8 * (n % room); };
 #pragma unroll 1
@@ -492,7 +510,7 @@ __global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid
                         float* const to = raw + place * L::tile_floats;
                         if constexpr (kRows) {
                             const auto row = shared_row(mine);
-                            GsTile<false>::copy(to, a_base + k, owned_a, left, wide_a, [&](int u) { return row((lane >> 3) + 4 * u); }, row);
+                            GsTile<false>::copy(to, a_base + k, owned_a, left, wide_a, [&](int u) { return ahead[u]; }, row);
                         } else {
                             const auto row = shared_row(pair * pass.a_stride + static_cast<long long>(comp) * d.K);
                             GsTile<true>::copy(to, a_base, left, owned_a, wide_a, [&](int u) { return row((lane >> 3) + 4 * u); }, row);
@@ -516,7 +534,7 @@ __global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid
                         gs_arrive_behind_copies(&raw_full[place]);
                     }
                     if (!kRows) {
-                        comp += 32 % d.comps; pair += 32 / d.comps;
+                        comp += comps_more; pair += pairs_more;
                         if (comp >= d.comps) { comp -= d.comps; ++pair; }
                     }
                 }
