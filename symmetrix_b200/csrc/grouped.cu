@@ -154,7 +154,7 @@ void join(const smx_grouped_linear& c) {
 }
 
 template <int kMode, bool kWide>
-void launch_gs(const GsPass& p, long long tiles, cudaStream_t stream) {
+void launch_gs(const GsPass& p, long long tiles, const Launcher& on) {
     const auto kernel = grouped_f32_kernel<kMode, kWide>;
     // The warps' shares of registers are drawn from what the launch gives: fewer than planned and they would wait for ever. What the kernel's own arrays
     // leave of the shared memory starts on a multiple of 1,024 bytes.
@@ -171,8 +171,8 @@ void launch_gs(const GsPass& p, long long tiles, cudaStream_t stream) {
         mark_on_device(done);
     }
     if (tiles > INT_MAX) throw ArgError("smx_grouped: too many rows");
-    kernel<<<static_cast<unsigned>(std::min<long long>(tiles, sm_count())), kGsThreads, smem.load(std::memory_order_relaxed), stream>>>(p);
-    launched("grouped_f32_kernel");
+    chain_launch(on, kernel, dim3(static_cast<unsigned>(std::min<long long>(tiles, sm_count()))), kGsThreads, smem.load(std::memory_order_relaxed), 1, p);
+    ++operator_launches;
 }
 
 GsPass gs_pass(const smx_grouped_linear& c, bool transposed) {
@@ -190,7 +190,7 @@ GsPass gs_pass(const smx_grouped_linear& c, bool transposed) {
         out_off += static_cast<long long>(d.comps) * d.N;
     }
     p.degrees = c.num_degrees; p.groups = c.num_groups; p.rows = c.num_rows; p.offsets = c.offsets;
-    p.out_width = static_cast<int>(out_off);
+    p.out_width = out_off;
     p.status = c.status; p.expire_polls = c.expire_polls;
     return p;
 }
@@ -207,17 +207,18 @@ void rows_f32(const smx_grouped_linear& c, bool transposed) {
         tiles += (c.num_rows * d.comps / 128 + c.num_groups) * ((d.N + 127) / 128);
         wide = wide && d.b_off % 8 == 0 && d.N % 64 == 0;
     }
-    const cudaStream_t stream = static_cast<cudaStream_t>(c.stream);
+    const Launcher on{static_cast<cudaStream_t>(c.stream), false};
     if (transposed) {
-        if (wide) launch_gs<kGsBackward, true>(p, tiles, stream);
-        else launch_gs<kGsBackward, false>(p, tiles, stream);
+        if (wide) launch_gs<kGsBackward, true>(p, tiles, on);
+        else launch_gs<kGsBackward, false>(p, tiles, on);
     } else {
-        if (wide) launch_gs<kGsForward, true>(p, tiles, stream);
-        else launch_gs<kGsForward, false>(p, tiles, stream);
+        if (wide) launch_gs<kGsForward, true>(p, tiles, on);
+        else launch_gs<kGsForward, false>(p, tiles, on);
     }
 }
 
-void gradient_f32(const smx_grouped_linear& c) {
+// `behind_rows`: right behind the rows' pass of the same call
+void gradient_f32(const smx_grouped_linear& c, bool behind_rows) {
     GsPass p = gs_pass(c, false);
     p.a = static_cast<const float*>(c.x); p.a_stride = c.x_stride;
     p.b = static_cast<const float*>(c.grad_y); p.b_stride = c.grad_y_stride;
@@ -233,15 +234,15 @@ void gradient_f32(const smx_grouped_linear& c) {
         tiles += (c.num_rows * d.comps / p.chunk + c.num_groups) * ((d.N + 127) / 128) * ((d.K + 127) / 128);
         wide = wide && d.N % 64 == 0 && (reinterpret_cast<uintptr_t>(d.grad) & 31) == 0;
     }
-    const cudaStream_t stream = static_cast<cudaStream_t>(c.stream);
-    if (wide) launch_gs<kGsGradient, true>(p, tiles, stream);
-    else launch_gs<kGsGradient, false>(p, tiles, stream);
+    const Launcher on{static_cast<cudaStream_t>(c.stream), behind_rows};
+    if (wide) launch_gs<kGsGradient, true>(p, tiles, on);
+    else launch_gs<kGsGradient, false>(p, tiles, on);
     join<float>(c);
 }
 
 // float64: tiles of 64 x 64, or of 16 x 32 while those leave SMs idle.
 template <int kMode, int BM, int BN, int WM, int WN, int ST>
-void launch_gd(const GdPass& p, long long tiles, cudaStream_t stream) {
+void launch_gd(const GdPass& p, long long tiles, const Launcher& on) {
     using L = GdLayout<kMode, BM, BN, ST>;
     if (tiles > INT_MAX) throw ArgError("smx_grouped: too many rows");
     const auto kernel = grouped_f64_kernel<kMode, BM, BN, WM, WN, ST>;
@@ -250,11 +251,11 @@ void launch_gd(const GdPass& p, long long tiles, cudaStream_t stream) {
         SMX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::smem));
         mark_on_device(done);
     }
-    kernel<<<static_cast<unsigned>(tiles), kGdThreads, L::smem, stream>>>(p);
-    launched("grouped_f64_kernel");
+    chain_launch(on, kernel, dim3(static_cast<unsigned>(tiles)), kGdThreads, L::smem, 1, p);
+    ++operator_launches;
 }
 template <int kMode>
-void launch_gd(const GdPass& p, cudaStream_t stream) {
+void launch_gd(const GdPass& p, const Launcher& on) {
     auto tiles = [&](int BM, int BN) {
         long long n = 0;
         for (int q = 0; q < p.degrees; ++q) {
@@ -264,8 +265,8 @@ void launch_gd(const GdPass& p, cudaStream_t stream) {
         }
         return n;
     };
-    if (tiles(64, 64) > 2LL * sm_count()) launch_gd<kMode, 64, 64, 2, 2, 2>(p, tiles(64, 64), stream);
-    else launch_gd<kMode, 16, 32, 1, 4, 4>(p, tiles(16, 32), stream);
+    if (tiles(64, 64) > 2LL * sm_count()) launch_gd<kMode, 64, 64, 2, 2, 2>(p, tiles(64, 64), on);
+    else launch_gd<kMode, 16, 32, 1, 4, 4>(p, tiles(16, 32), on);
 }
 
 GdPass gd_pass(const smx_grouped_linear& c, bool transposed) {
@@ -283,7 +284,7 @@ GdPass gd_pass(const smx_grouped_linear& c, bool transposed) {
         out_off += static_cast<long long>(d.comps) * d.N;
     }
     p.degrees = c.num_degrees; p.groups = c.num_groups; p.rows = c.num_rows; p.offsets = c.offsets;
-    p.out_width = static_cast<int>(out_off);
+    p.out_width = out_off;
     return p;
 }
 
@@ -292,11 +293,12 @@ void rows_f64(const smx_grouped_linear& c, bool transposed) {
     p.a = static_cast<const double*>(transposed ? c.grad_y : c.x); p.a_stride = transposed ? c.grad_y_stride : c.x_stride;
     p.out = static_cast<double*>(transposed ? c.grad_x : c.y); p.out_stride = transposed ? c.grad_x_stride : c.y_stride;
     p.zero_tail = transposed || c.zero_tail;
-    if (transposed) launch_gd<kGsBackward>(p, static_cast<cudaStream_t>(c.stream));
-    else launch_gd<kGsForward>(p, static_cast<cudaStream_t>(c.stream));
+    const Launcher on{static_cast<cudaStream_t>(c.stream), false};
+    if (transposed) launch_gd<kGsBackward>(p, on);
+    else launch_gd<kGsForward>(p, on);
 }
 
-void gradient_f64(const smx_grouped_linear& c) {
+void gradient_f64(const smx_grouped_linear& c, bool behind_rows) {
     GdPass p = gd_pass(c, false);
     p.a = static_cast<const double*>(c.x); p.a_stride = c.x_stride;
     p.b = static_cast<const double*>(c.grad_y); p.b_stride = c.grad_y_stride;
@@ -308,7 +310,7 @@ void gradient_f64(const smx_grouped_linear& c) {
         d.part = part;
         part += part_values(c, q);
     }
-    launch_gd<kGsGradient>(p, static_cast<cudaStream_t>(c.stream));
+    launch_gd<kGsGradient>(p, Launcher{static_cast<cudaStream_t>(c.stream), behind_rows});
     join<double>(c);
 }
 
@@ -350,8 +352,9 @@ void backward(const smx_grouped_linear& c) {
     }
     if (c.grad_x) rows_pass<T>(c, true);
     if (!matrices) return;
-    if (sizeof(T) == 4) gradient_f32(c);
-    else gradient_f64(c);
+    const bool behind_rows = c.grad_x && c.num_rows > 0;
+    if (sizeof(T) == 4) gradient_f32(c, behind_rows);
+    else gradient_f64(c, behind_rows);
 }
 
 }  // namespace

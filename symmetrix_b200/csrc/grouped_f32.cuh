@@ -31,7 +31,8 @@ struct GsDegree {
 };
 struct GsPass {
     GsDegree degree[SMX_GROUPED_MAX_DEGREES];
-    int degrees, groups, zero_tail, out_width;
+    int degrees, groups, zero_tail;
+    long long out_width;
     int chunk;                       // gradient: rows of a tile's sum, a multiple of kGsChunk
     long long rows;
     const int* offsets;
@@ -325,6 +326,8 @@ __global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid
         mbar_init(&drained, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    // The gradient reads nothing that the rows' pass before it writes: its CTAs come in as that one's end.
+    if (kMode == kGsBackward) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -394,7 +397,7 @@ __global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid
             }
         } else if (kRows && pass.zero_tail) {
             for (long long p = pass.offsets[pass.groups] + 2LL * blockIdx.x + (warp - 2); p < pass.rows; p += 2LL * gridDim.x)
-                for (int c = lane; c < pass.out_width; c += 32) pass.out[p * pass.out_stride + c] = 0.f;
+                for (long long c = lane; c < pass.out_width; c += 32) pass.out[p * pass.out_stride + c] = 0.f;
         }
         gs_meet();
         if (guard[0] && warp == 0) {
@@ -686,6 +689,8 @@ __global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid
         gs_meet();
     }
     __syncthreads();
+    // (one CTA waits for that pass, so that this kernel does not end before it)
+    if (kMode == kGsGradient && blockIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
     if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 

@@ -20,7 +20,8 @@ struct GdDegree {
 };
 struct GdPass {
     GdDegree degree[SMX_GROUPED_MAX_DEGREES];
-    int degrees, groups, zero_tail, out_width;
+    int degrees, groups, zero_tail;
+    long long out_width;
     int chunk;                       // gradient: rows of a sum
     long long rows;
     const int* offsets;
@@ -120,6 +121,9 @@ __global__ void __launch_bounds__(kGdThreads) grouped_f64_kernel(const __grid_co
     __shared__ GdWork work;
     __shared__ int found;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, wm = warp / WN, wn = warp % WN;
+    // The gradient reads nothing that the rows' pass before it writes: its CTAs come in as that one's end (one of them waits, so that it does not end first).
+    if (kMode == kGsBackward) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (kMode == kGsGradient && blockIdx.x == gridDim.x - 1) asm volatile("griddepcontrol.wait;" ::: "memory");
     if (warp == 0) {
         GdWork w{};
         const bool hit = gd_find<kMode>(pass, BM, BN, blockIdx.x, w);
@@ -127,7 +131,7 @@ __global__ void __launch_bounds__(kGdThreads) grouped_f64_kernel(const __grid_co
     }
     if (kRows && pass.zero_tail)
         for (long long p = pass.offsets[pass.groups] + blockIdx.x; p < pass.rows; p += gridDim.x)
-            for (int c = tid; c < pass.out_width; c += kGdThreads) pass.out[p * pass.out_stride + c] = 0.0;
+            for (long long c = tid; c < pass.out_width; c += kGdThreads) pass.out[p * pass.out_stride + c] = 0.0;
     __syncthreads();
     if (!found) return;
     const GdDegree& d = pass.degree[work.degree];

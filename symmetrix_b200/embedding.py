@@ -101,11 +101,20 @@ class Embedding:
         self.table, self.scale = table, float(scale)
         self.table_rows, self.width = table.shape
         self.dtype, self.device = table.dtype, table.device
-        self._stride = table.stride(0) if self.table_rows > 1 else self.width
+        self._shape, self._row = tuple(table.shape), table.stride(0)
+        self._stride = self._row if self.table_rows > 1 else self.width
         self._library, self._index, self._precision = _lib.load(), self.device.index, _precision(table.dtype)
+
+    def _check(self):
+        t = self.table
+        if t.requires_grad or t.shape != self._shape:
+            _values(t, "table", self._shape, self.dtype, self.device)
+        if t.stride(0) != self._row:
+            raise ValueError("table has other strides than when the embedding was made")
 
     def forward(self, ids, weights=None, out=None):
         """``y`` ``[rows, width]``; ``ids`` as for ``EmbeddingPlan``, ``weights`` ``[rows, slots]`` (None: ones)."""
+        self._check()
         ids, rows, slots = _tokens(ids, self.device)
         if not 1 <= slots <= _lib.ROUTE_MAX_SLOTS:
             raise ValueError(f"ids has {slots} slots: 1 .. {_lib.ROUTE_MAX_SLOTS} are supported")
@@ -123,6 +132,7 @@ class Embedding:
         """Gradients ``(table, weights)`` of a forward pass with the plan's ids and the same weights, None where not wanted: ``[table_rows, width]``,
         zero for rows without a token, and ``[rows, slots]``, zero in empty slots."""
         import torch
+        self._check()
         if not isinstance(plan, EmbeddingPlan):
             raise ValueError("plan must be an EmbeddingPlan")
         if plan.device != self.device:

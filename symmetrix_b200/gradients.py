@@ -30,7 +30,7 @@ class GradientSet:
     receives the scaled values, the tensors themselves without it. Nothing in the lists may overlap, except an output with its own tensor
     where both are the same memory.
 
-    The tensors are kept: a program whose gradients have buffers of their own makes the set once."""
+    The set holds on to the tensors' memory as it is when the set is made: a program whose gradients have buffers of their own makes it once."""
 
     def __init__(self, tensors, out=None):
         tensors = list(tensors)
@@ -42,14 +42,15 @@ class GradientSet:
         self.device = None
         spans, entries = [], (_lib.Gradient * len(tensors))()
         for q, t in enumerate(tensors):
-            _dense(t, f"tensors[{q}]", self.device)
+            # (another tensor of the same memory, which stays even if the program gives this one other memory)
+            tensors[q] = t = _dense(t, f"tensors[{q}]", self.device).detach()
             self.device = t.device
             e, at, size = entries[q], t.data_ptr(), t.element_size() * t.numel()
             e.values, e.out, e.count, e.precision = at, at, t.numel(), _precision(t.dtype)
             spans.append((at, at + size))
             if outs is None:
                 continue
-            o = _dense(outs[q], f"out[{q}]", self.device)
+            outs[q] = o = _dense(outs[q], f"out[{q}]", self.device).detach()
             if o.shape != t.shape or o.dtype is not t.dtype:
                 raise ValueError(f"out[{q}] has shape {tuple(o.shape)} and dtype {o.dtype}, expected {tuple(t.shape)} and {t.dtype}")
             e.out = o.data_ptr()

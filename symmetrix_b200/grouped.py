@@ -52,7 +52,8 @@ class GroupedLinear:
         f = self._fixed = _lib.GroupedCall()
         f.precision, f.num_degrees, f.num_groups, f.status = _precision(self.dtype), len(weights), self.num_groups, self._status.data_ptr()
         for d, w, c in zip(f.degrees, weights, self.components):
-            d.components, d.in_channels, d.out_channels, d.weight = c, w.shape[1], w.shape[2], w.data_ptr()
+            d.components, d.in_channels, d.out_channels = c, w.shape[1], w.shape[2]
+        self._shapes = tuple(tuple(w.shape) for w in weights)
 
     def check(self) -> None:
         """Waits for the current stream and raises ``SymmetrixError`` if a bounded wait inside a kernel ran out in a call since the last check:
@@ -71,6 +72,10 @@ class GroupedLinear:
             raise ValueError(f"routing has {routing.num_groups} groups, the linear {self.num_groups}")
         call = _lib.GroupedCall()
         ctypes.memmove(ctypes.byref(call), ctypes.byref(self._fixed), ctypes.sizeof(call))
+        for d, w, shape in zip(call.degrees, self.weights, self._shapes):
+            if w.requires_grad or w.shape != shape:
+                _values(w, "weights", shape, self.dtype, self.device)
+            d.weight = w.data_ptr()                  # (as it is now: a program may have given the tensor other memory)
         call.num_rows, call.offsets = routing._pairs, routing._offsets
         call.stream = _stream(self._index)
         if call.stream != self._home:

@@ -65,6 +65,7 @@ def check(got, want):
 @pytest.mark.parametrize("n,slots,rows", [
     (0, 1, 1), (1, 1, 1), (1, 64, 5), (33, 1, 3), (100, 3, 1022), (100, 3, 1023), (100, 3, 1024), (500, 2, 1025), (1000, 1, 5000), (8192, 1, 1023), (8193, 1, 1023),
     (8193, 1, 1024), (4097, 2, 20000), (30000, 3, 1424), (70001, 1, 1048575), (200000, 2, 89), (300, 1, 1048575),
+    (5000, 1, 4095), (9000, 1, 4094), (9000, 1, 4095), (9000, 1, 4096), (30000, 2, 4097),
 ])
 @pytest.mark.parametrize("kind", ["random", "skewed", "one", "outside", "empty"])
 def test_plan(n, slots, rows, kind):
@@ -276,6 +277,22 @@ def test_a_step_of_training():
         table -= buffer
         moved = embedding.forward(ids) - before[ids[:, 0].long()]
         assert torch.allclose(moved, -buffer[ids[:, 0].long()], rtol=0.0, atol=2.0 ** -22 * float(before.abs().max()))
+
+
+def test_a_table_that_changes():
+    table = torch.randn(5, 8, device="cuda")
+    ids = torch.tensor([4, 0], dtype=torch.int32, device="cuda")
+    embedding = Embedding(table)
+    table.data = torch.randn(5, 8, device="cuda")            # other memory
+    assert torch.equal(embedding.forward(ids), table[[4, 0]])
+    table.requires_grad_()
+    with pytest.raises(ValueError, match="autograd"):
+        embedding.forward(ids)
+    with torch.no_grad():
+        assert torch.equal(embedding.forward(ids), table[[4, 0]])
+        table.data = torch.randn(6, 8, device="cuda")
+        with pytest.raises(ValueError, match="shape"):
+            embedding.forward(ids)
 
 
 def test_refusals():

@@ -171,6 +171,14 @@ def test_sets_streams_and_graphs():
     check(outs, want, 105003)
 
 
+def test_a_set_keeps_its_memory():
+    t = torch.full((1000,), 3.0, device="cuda")
+    kept, old = GradientSet([t]), t.detach()
+    t.data = torch.zeros(1000, device="cuda")
+    torch.empty(1000, device="cuda").fill_(7.0)      # would take the old memory, were it free
+    assert abs(float(kept.clip(1.0)) - 3.0 * np.sqrt(1000.0)) < 1e-10 and abs(float(old.norm()) - 1.0) < 1e-6 and not t.any()
+
+
 def test_a_long_tensor():
     n = 2 ** 31 + 4099
     if torch.cuda.mem_get_info()[0] < 1.2 * 4 * n:

@@ -348,6 +348,21 @@ def test_experts_of_an_atom(dtype):
     assert abs(float(norm) - float(want_norm)) <= rel * float(want_norm)
 
 
+def test_matrices_that_change():
+    case = Case(torch.float32, [30, 40], [1], [36], [64])
+    w = case.weights[0]
+    w.data = torch.randn_like(w)                     # other memory
+    case.check_rows(case.layer.forward(case.x, case.routing), case.expect([w])[0], case.outs)
+    w.requires_grad_()
+    with pytest.raises(ValueError, match="autograd"):
+        case.layer.forward(case.x, case.routing)
+    with torch.no_grad():
+        case.layer.forward(case.x, case.routing)
+        w.data = torch.randn(2, 36, 65, device="cuda")
+        with pytest.raises(ValueError, match="shape"):
+            case.layer.forward(case.x, case.routing)
+
+
 def test_refusals():
     case = Case(torch.float32, [3, 4], [1, 3], [4, 5], [6, 7])
     layer, routing, x, gy = case.layer, case.routing, case.x, case.gy
