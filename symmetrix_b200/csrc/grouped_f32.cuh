@@ -252,6 +252,18 @@ __device__ __forceinline__ void gs_split(float v, float& hi, float& lo) {
     lo = __uint_as_float(__float_as_uint(v - hi) & kTc5HiMask);
 }
 
+// Two by two blocks of eight values are turned between a lane and the one kLane on: the lower one gets both first blocks, the upper one both second ones.
+template <int kLane>
+__device__ __forceinline__ void gs_turn(float* first, float* second) {
+    const bool upper = threadIdx.x & kLane;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float got = __shfl_xor_sync(0xffffffffu, upper ? first[e] : second[e], kLane);
+        if (upper) first[e] = got;
+        else second[e] = got;
+    }
+}
+
 __device__ __forceinline__ void gs_meet() {
     __syncwarp();
     ts_fence_before();
@@ -648,11 +660,27 @@ __global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid
             }
             if (!ok) break;
             if (kWide) {
-                if (out_row && left > 0)
+                // Four lanes share out their rows' lines, so that a store touches eight lines instead of 32.
+                const unsigned long long mine = reinterpret_cast<unsigned long long>(out_row);
+                float* rows_of[4];
 #pragma unroll
-                    for (int q = 0; q < 64; q += 8)
-                        asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out_row + q), "f"(sum[q]), "f"(sum[q + 1]), "f"(sum[q + 2]),
-                                     "f"(sum[q + 3]), "f"(sum[q + 4]), "f"(sum[q + 5]), "f"(sum[q + 6]), "f"(sum[q + 7]) : "memory");
+                for (int i = 0; i < 4; ++i) rows_of[i] = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, mine, (lane & ~3) + i)) + 8 * (lane & 3);
+                const unsigned there = __ballot_sync(0xffffffffu, mine != 0) >> (lane & ~3);
+                if (left > 0)
+#pragma unroll
+                    for (int c = 0; c < 64; c += 32) {
+                        gs_turn<1>(sum + c, sum + c + 8);
+                        gs_turn<1>(sum + c + 16, sum + c + 24);
+                        gs_turn<2>(sum + c, sum + c + 16);
+                        gs_turn<2>(sum + c + 8, sum + c + 24);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float* v = sum + c + 8 * i;
+                            if ((there >> i) & 1u)
+                                asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(rows_of[i] + c), "f"(v[0]), "f"(v[1]), "f"(v[2]),
+                                             "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]) : "memory");
+                        }
+                    }
             } else {
                 // 16 columns of the warp's rows at a time through shared memory, so that a store touches two rows instead of 32
                 const unsigned long long mine = reinterpret_cast<unsigned long long>(out_row);

@@ -101,15 +101,15 @@ class Embedding:
         self.table, self.scale = table, float(scale)
         self.table_rows, self.width = table.shape
         self.dtype, self.device = table.dtype, table.device
-        self._shape, self._row = tuple(table.shape), table.stride(0)
-        self._stride = self._row if self.table_rows > 1 else self.width
+        self._shape, self._strides = tuple(table.shape), table.stride()
+        self._stride = self._strides[0] if self.table_rows > 1 else self.width
         self._library, self._index, self._precision = _lib.load(), self.device.index, _precision(table.dtype)
 
     def _check(self):
         t = self.table
-        if t.requires_grad or t.shape != self._shape:
+        if t.requires_grad or t.shape != self._shape or t.dtype is not self.dtype:
             _values(t, "table", self._shape, self.dtype, self.device)
-        if t.stride(0) != self._row:
+        if t.stride() != self._strides:
             raise ValueError("table has other strides than when the embedding was made")
 
     def forward(self, ids, weights=None, out=None):

@@ -70,35 +70,26 @@ class GroupedLinear:
             raise ValueError(f"routing is on {routing.device}, expected {self.device}")
         if routing.num_groups != self.num_groups:
             raise ValueError(f"routing has {routing.num_groups} groups, the linear {self.num_groups}")
-        call = _lib.GroupedCall()
-        ctypes.memmove(ctypes.byref(call), ctypes.byref(self._fixed), ctypes.sizeof(call))
+        call = _lib.GroupedCall.from_buffer_copy(self._fixed)
         for d, w, shape in zip(call.degrees, self.weights, self._shapes):
-            if w.requires_grad or w.shape != shape:
-                _values(w, "weights", shape, self.dtype, self.device)
+            if w.requires_grad or w.shape != shape or w.dtype is not self.dtype or not w.is_contiguous():
+                if not _values(w, "weights", shape, self.dtype, self.device).is_contiguous():
+                    raise ValueError("weights must be contiguous")
             d.weight = w.data_ptr()                  # (as it is now: a program may have given the tensor other memory)
         call.num_rows, call.offsets = routing._pairs, routing._offsets
-        call.stream = _stream(self._index)
-        if call.stream != self._home:
+        stream = _stream(self._index)
+        call.stream = stream
+        if stream != self._home:
             import torch
             self._status.record_stream(torch.cuda.current_stream(self._index))
-        if call.stream != routing._home:
+        if stream != routing._home:
             routing._use()
         return call
-
-    def _run(self, fn, call, backward):
-        need = self._library.smx_grouped_workspace_bytes(ctypes.byref(call), backward)
-        if need < 0:
-            raise ValueError("the sizes exceed what smx_grouped_forward supports")
-        if need:
-            import torch
-            ws = torch.empty(need, dtype=torch.uint8, device=self.device)
-            call.workspace, call.workspace_bytes = ws.data_ptr(), need
-        _call(fn, self._index, ctypes.byref(call))
 
     def forward(self, x, routing: RowRouting, out=None):
         """``y`` of ``x`` ``[rows * slots, in_width]`` in the order of ``routing``. Rows behind the last group are zero, or left as they were in ``out``."""
         call = self._begin(routing)
-        n = call.num_rows
+        n = routing._pairs
         x, call.x_stride = _rows(x, "x", (n, self.in_width), self.dtype, self.device)
         if out is None:
             y, call.y_stride, call.zero_tail = x.new_empty((n, self.out_width)), self.out_width, 1
@@ -106,14 +97,14 @@ class GroupedLinear:
             y, call.y_stride = _out(out, "out", (n, self.out_width), self.dtype, self.device)
             _apart(y, x, *self.weights)
         call.x, call.y = _ptr(x), _ptr(y)
-        self._run(self._library.smx_grouped_forward, call, 0)
+        _call(self._library.smx_grouped_forward, self._index, ctypes.byref(call))
         return y
 
     def backward(self, x, grad_y, routing: RowRouting, want_x: bool = True, want_weights: bool = True):
         """Gradients ``(x, weights)`` of a forward pass with the same ``x``, routing and matrices, None where not wanted; rows behind the last group and
         matrices of groups without rows get zeros. ``x`` is not read (and may be None) without ``want_weights``."""
         call = self._begin(routing)
-        n = call.num_rows
+        n = routing._pairs
         grad_y, call.grad_y_stride = _rows(grad_y, "grad_y", (n, self.out_width), self.dtype, self.device)
         call.grad_y = _ptr(grad_y)
         grad_x = grad_weights = None
@@ -132,5 +123,11 @@ class GroupedLinear:
                 d.grad_weight = base + size * at
                 grad_weights.append(flat.as_strided((g, i, o), (i * o, o, 1), at))
                 at += -(-s // 4) * 4
-        self._run(self._library.smx_grouped_backward, call, 1)
+            need = self._library.smx_grouped_workspace_bytes(ctypes.byref(call), 1)
+            if need < 0:
+                raise ValueError("the sizes exceed what smx_grouped_backward supports")
+            if need:
+                ws = grad_y.new_empty(-(-need // size))
+                call.workspace, call.workspace_bytes = ws.data_ptr(), need
+        _call(self._library.smx_grouped_backward, self._index, ctypes.byref(call))
         return GroupedGradients(grad_x, grad_weights)

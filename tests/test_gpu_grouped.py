@@ -358,9 +358,10 @@ def test_matrices_that_change():
         case.layer.forward(case.x, case.routing)
     with torch.no_grad():
         case.layer.forward(case.x, case.routing)
-        w.data = torch.randn(2, 36, 65, device="cuda")
-        with pytest.raises(ValueError, match="shape"):
-            case.layer.forward(case.x, case.routing)
+        for other, text in [(torch.randn(2, 36, 65, device="cuda"), "shape"), (torch.randn(2, 64, 36, device="cuda").transpose(1, 2), "contiguous")]:
+            w.data = other
+            with pytest.raises(ValueError, match=text):
+                case.layer.forward(case.x, case.routing)
 
 
 def test_refusals():
