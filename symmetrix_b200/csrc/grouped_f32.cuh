@@ -507,10 +507,6 @@ __global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid
             const bool wide_a = ((static_cast<unsigned long long>(pass.a_stride | d.a_off | d.K) * 4u | reinterpret_cast<uintptr_t>(pass.a)) & 15) == 0;
             const bool wide_b = kMode == kGsGradient ? ((static_cast<unsigned long long>(pass.b_stride | d.b_off | d.N) * 4u | reinterpret_cast<uintptr_t>(pass.b)) & 15) == 0
                                                      : ((static_cast<unsigned long long>(kMode == kGsForward ? d.N : d.K) * 4u | reinterpret_cast<uintptr_t>(d.w)) & 15) == 0;
-            long long ahead[8];                                          // rows passes: where the rows that the lane copies begin
-            if (kRows)
-#pragma unroll
-                for (int u = 0; u < 8; ++u) ahead[u] = __shfl_sync(0xffffffffu, mine, (lane >> 3) + 4 * u);
             const int comps_more = 32 % d.comps, pairs_more = 32 / d.comps;
             auto shared_row = [&](long long v) { return [v](int r) { return __shfl_sync(0xffffffffu, v, r); }; };
             auto place_of = [&](int part, int n, int room) { return q + 4 * part + 8 * (n % room); };
@@ -525,7 +521,7 @@ __global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid
                         float* const to = raw + place * L::tile_floats;
                         if constexpr (kRows) {
                             const auto row = shared_row(mine);
-                            GsTile<false>::copy(to, a_base + k, owned_a, left, wide_a, [&](int u) { return ahead[u]; }, row);
+                            GsTile<false>::copy(to, a_base + k, owned_a, left, wide_a, [&](int u) { return row((lane >> 3) + 4 * u); }, row);
                         } else {
                             const auto row = shared_row(pair * pass.a_stride + static_cast<long long>(comp) * d.K);
                             GsTile<true>::copy(to, a_base, left, owned_a, wide_a, [&](int u) { return row((lane >> 3) + 4 * u); }, row);
