@@ -431,7 +431,8 @@ int smx_grouped_backward(const smx_grouped_linear* call, char* errbuf, int errbu
  *   grad_weights[n, s] = scale * <grad_y[n, :], table[ids[n, s], :]>                          (zero in empty slots; alone this one reads `table`)
  * Sums over pairs are cut into chunks whose length follows from the sizes alone, and added in order: the same call gives the same bits.
  * The rules of the smx_route_* calls hold, with a workspace of smx_embedding_plan_bytes / smx_embedding_backward_bytes (the latter starts on
- * a 16-byte boundary) for each call that may overlap with another one. Strides count elements from row to row. */
+ * a 16-byte boundary) for each call that may overlap with another one. Strides count elements from row to row. Limits: `width` 2^30, in the backward
+ * pass 65,535 * 32; otherwise those of the routing. */
 enum { SMX_EMBEDDING_MAX_ROWS = (1 << 20) - 1 };
 long smx_embedding_plan_bytes(long num_rows, int slots, int table_rows);
 int smx_embedding_plan(const int* ids, long num_rows, int slots, int table_rows, int* order, int* tokens, void* workspace,

@@ -253,7 +253,7 @@ void launched(const char* what) {
 void check_sizes(const char* what, long num_rows, int slots, int table_rows, long width) {
     if (table_rows < 1 || table_rows > SMX_EMBEDDING_MAX_ROWS)
         throw ArgError(std::string(what) + ": the number of table rows must lie in 1 .. " + std::to_string(SMX_EMBEDDING_MAX_ROWS));
-    if (width < 0 || width > INT_MAX) throw ArgError(std::string(what) + ": bad row width");
+    if (width < 0 || width > (1L << 30)) throw ArgError(std::string(what) + ": the row width must lie in 0 .. 2^30");         // (so that steps along a row stay ints)
     route_plan_bytes(num_rows, slots, 1);                                // rows and slots as there
 }
 void check_stride(const char* what, long stride, long width, long rows, bool written) {
@@ -329,6 +329,7 @@ Room room(long pairs, long width) {
 template <typename T>
 size_t embedding_backward_bytes(long num_rows, int slots, long width) {
     check_sizes("smx_embedding_backward", num_rows, slots, 1, width);
+    if (width > 65535L * kJoinUnits) throw ArgError("smx_embedding_backward: the row width must lie in 0 .. 2097120");
     const Room r = room<T>(num_rows * slots, width);
     return r.parts + r.dots;
 }
@@ -348,10 +349,9 @@ void embedding_backward(const T* grad_y, long grad_y_stride, const T* table, lon
         if (pairs > 0 && width > 0 && !table) throw ArgError("smx_embedding_backward: the weights' gradient needs the table");
     }
     if (!grad_table && !grad_weights) return;
-    const size_t need = embedding_backward_bytes<T>(num_rows, slots, width);
+    const size_t need = embedding_backward_bytes<T>(num_rows, slots, width);                                                  // (which checks the width too)
     if (workspace_bytes < need || (need && !workspace)) throw ArgError("smx_embedding_backward: the workspace is smaller than smx_embedding_backward_bytes says");
     if (reinterpret_cast<uintptr_t>(workspace) & 15) throw ArgError("smx_embedding_backward: the workspace must start on a 16-byte boundary");
-    if (width > 65535L * kJoinUnits) throw ArgError("smx_embedding_backward: rows are too wide");
     if (grad_table && width > 0) SMX_CUDA(cudaMemsetAsync(grad_table, 0, static_cast<size_t>(table_rows) * width * sizeof(T), stream));
     if (pairs == 0) return;
     if (width == 0) {

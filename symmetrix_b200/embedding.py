@@ -107,7 +107,7 @@ class Embedding:
 
     def _check(self):
         t = self.table
-        if t.requires_grad or t.shape != self._shape or t.dtype is not self.dtype:
+        if t.requires_grad or t.shape != self._shape or t.dtype is not self.dtype or t.get_device() != self._index:
             _values(t, "table", self._shape, self.dtype, self.device)
         if t.stride() != self._strides:
             raise ValueError("table has other strides than when the embedding was made")

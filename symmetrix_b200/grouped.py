@@ -72,7 +72,7 @@ class GroupedLinear:
             raise ValueError(f"routing has {routing.num_groups} groups, the linear {self.num_groups}")
         call = _lib.GroupedCall.from_buffer_copy(self._fixed)
         for d, w, shape in zip(call.degrees, self.weights, self._shapes):
-            if w.requires_grad or w.shape != shape or w.dtype is not self.dtype or not w.is_contiguous():
+            if w.requires_grad or w.shape != shape or w.dtype is not self.dtype or w.get_device() != self._index or not w.is_contiguous():
                 if not _values(w, "weights", shape, self.dtype, self.device).is_contiguous():
                     raise ValueError("weights must be contiguous")
             d.weight = w.data_ptr()                  # (as it is now: a program may have given the tensor other memory)

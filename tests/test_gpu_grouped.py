@@ -106,6 +106,7 @@ SHAPES = [
     ([127, 128, 129], [1], [32], [128]), ([64, 0, 65, 63], [3], [64], [64]), ([5, 300, 1, 44], [1, 3], [128, 128], [128, 128]),
     ([40, 41], [2, 1, 4], [31, 1, 130], [7, 129, 1]), ([1000], [1], [768], [96]), ([17, 90], [1, 3, 5, 7], [48, 72, 72, 48], [24, 24, 24, 24]),
     ([3] * 70, [1], [20], [36]), ([700, 2, 700], [5], [36], [132]), ([9, 0, 2500], [1, 3], [66, 258], [130, 62]), ([6] * 1024, [1], [4], [4]),
+    ([3, 0, 9], [40, 1], [36, 64], [64, 33]), ([2, 5], [1000], [7], [64]), ([1, 3], [1024, 33], [8, 64], [64, 8]), ([130], [31, 32], [64, 1], [1, 64]),
 ]
 
 
@@ -385,7 +386,7 @@ def test_refusals():
 
 
 def test_waits_that_run_out_are_reported():
-    """The test switch makes every CTA lose the matrices behind the first 32 inner values and give up after a few hundred polls: what is lost holds NaN, the
+    """The test switch makes every CTA lose the matrices behind its first step of inner values and give up after a few hundred polls: what is lost holds NaN, the
     rest is right, and the next calls are."""
     case = Case(torch.float32, [1500, 0, 2700, 40], [1, 3], [70, 200], [136, 64])
     y, gx, gw = case.expect()

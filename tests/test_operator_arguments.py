@@ -85,7 +85,7 @@ def test_embedding_sizes():
     for bad in [(-1, 1, 1), (1, 0, 1), (1, 65, 1), (1, 1, 0), (1, 1, 1 << 20), (1 << 31, 1, 1)]:
         assert lib.smx_embedding_plan_bytes(*bad) == -1
     assert lib.smx_embedding_backward_bytes(32, 0, 1, 8) == 0
-    for bad in [(16, 1, 1, 8), (32, -1, 1, 8), (32, 1, 0, 8), (32, 1, 1, -1)]:
+    for bad in [(16, 1, 1, 8), (32, -1, 1, 8), (32, 1, 0, 8), (32, 1, 1, -1), (32, 1, 1, 65535 * 32 + 1)]:
         assert lib.smx_embedding_backward_bytes(*bad) == -1
 
 
@@ -95,6 +95,7 @@ def test_embedding_sizes():
     ("smx_embedding_forward", (32, P, -1, 4, P, 4, 1, 8, None, 1.0, P, 8, None), "stride"),
     ("smx_embedding_forward", (32, P, 8, 4, P, 4, 1, 8, None, 1.0, P, 7, None), "stride"),
     ("smx_embedding_forward", (32, P, 8, 4, P, 4, 1, -8, None, 1.0, P, 8, None), "width"),
+    ("smx_embedding_forward", (32, P, 1 << 31, 4, P, 4, 1, (1 << 30) + 1, None, 1.0, P, 1 << 31, None), "width"),
     ("smx_embedding_forward", (32, P, 8, 4, P, 4, 99, 8, None, 1.0, P, 8, None), "slots"),
     ("smx_embedding_forward", (32, None, 8, 4, P, 4, 1, 8, None, 1.0, P, 8, None), "null"),
     ("smx_embedding_forward", (64, P + 4, 8, 4, P, 4, 1, 8, None, 1.0, P, 8, None), "multiple"),
