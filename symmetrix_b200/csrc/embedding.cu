@@ -71,12 +71,14 @@ __global__ void __launch_bounds__(256) embedding_forward_kernel(const V* __restr
 }
 
 // Sums of the runs of a chunk of sorted pairs, kGradThreads units of a row a CTA. parts: [chunk][2][units]: the run that an earlier chunk began, and the
-// run that goes on in the next one. kWeights: the weights' gradients too, since a run's row of the table then is read once (49,152 rows of 512 floats, two
-// slots, 1,424 tokens, all of the backward pass: 64 us; 79 with the weights row by row in a kernel of their own). Their sums over the units of a CTA go to `dots` [slab][pairs], or straight
-// to the gradient where one CTA has the whole row.
+// run that goes on in the next one. kWeights: the weights' gradients too, since a run's row of the table then is read once. Their sums over the units of a
+// CTA go to `dots` [slab][pairs], or straight to the gradient where one CTA has the whole row.
+// 49,152 rows of 512 floats, two slots, 1,424 tokens, all of the backward pass: 47 us, of which this kernel 33 for 201 MB of rows, 6.1 TB/s; 64 with a look
+// at every pair's token (its instructions bounded it), 56 with the rows copied ahead through shared memory, 50 with eight CTAs of 64 registers an SM.
 constexpr int kGradThreads = 128, kMaxChunk = 512, kLoads = 8, kRows = 4;
+template <typename T> constexpr int grad_ctas = sizeof(T) == 4 ? 6 : 5;  // of an SM
 template <typename T, typename V, bool kWeights>
-__global__ void __launch_bounds__(kGradThreads, sizeof(T) == 4 ? 8 : 5) embedding_grad_kernel(const V* __restrict__ grad_y, long long grad_y_stride, const V* __restrict__ table,
+__global__ void __launch_bounds__(kGradThreads, grad_ctas<T>) embedding_grad_kernel(const V* __restrict__ grad_y, long long grad_y_stride, const V* __restrict__ table,
                                                                       long long table_stride, const int* __restrict__ order, const int* __restrict__ tokens,
                                                                       long long pairs, int slots, int table_rows, int units, const T* __restrict__ weights, T scale,
                                                                       int chunk, V* __restrict__ grad_table, V* __restrict__ parts, T* __restrict__ dots,
@@ -109,7 +111,19 @@ __global__ void __launch_bounds__(kGradThreads, sizeof(T) == 4 ? 8 : 5) embeddin
     const bool mine = u < units;
     L sum{}, last{};                                                     // the run at hand; the row of the table of the pair before
     int from = 0, last_token = -1;                                       // where the run began
+    auto give = [&](int i, int t) {                                      // the run of token t ends with pair i, or is cut behind it
+        const bool began = from > 0 || token[0] != t, ends = token[i + 2] != t;
+        if (mine) {
+            if (began && ends) grad_table[static_cast<long long>(t) * units + u] = sum.v;
+            else parts[(2LL * blockIdx.x + (began ? 1 : 0)) * units + u] = sum.v;
+        }
+        sum = L{};
+        from = i + 1;
+    };
     for (int i0 = 0; i0 < live; i0 += kLoads) {
+        // One token for all (the pairs are sorted) is what long runs mostly meet: without a look at every pair a batch takes a third of the instructions.
+        const int t0 = token[i0 + 1];
+        const bool one = i0 + kLoads <= live && token[i0 + kLoads] == t0;
         L g[kLoads];
 #pragma unroll
         for (int q = 0; q < kLoads; ++q) {
@@ -118,6 +132,16 @@ __global__ void __launch_bounds__(kGradThreads, sizeof(T) == 4 ? 8 : 5) embeddin
         }
         if constexpr (kWeights) {
             T d[kLoads];
+            if (one) {
+                if (t0 != last_token && mine) last.v = table[t0 * table_stride + u];
+                last_token = t0;
+#pragma unroll
+                for (int q = 0; q < kLoads; ++q) {
+                    d[q] = T(0);
+#pragma unroll
+                    for (int e = 0; e < L::n; ++e) d[q] += g[q].t[e] * last.t[e];
+                }
+            } else
 #pragma unroll
             for (int q0 = 0; q0 < kLoads; q0 += kRows) {
                 L r[kRows];                                              // read where the token changes
@@ -150,6 +174,17 @@ __global__ void __launch_bounds__(kGradThreads, sizeof(T) == 4 ? 8 : 5) embeddin
             if ((lane & 3) == 0 && i < live) warp_dot[warp][i] = d[0];
         }
         if (!grad_table) continue;
+        if (one) {
+#pragma unroll
+            for (int q = 0; q < kLoads; ++q) {
+                const T w = weight[i0 + q];
+#pragma unroll
+                for (int e = 0; e < L::n; ++e) sum.t[e] += w * g[q].t[e];
+            }
+            const int i = i0 + kLoads - 1;
+            if (token[i + 2] != t0 || i + 1 == count) give(i, t0);
+            continue;
+        }
 #pragma unroll
         for (int q = 0; q < kLoads; ++q) {
             const int i = i0 + q;
@@ -159,13 +194,7 @@ __global__ void __launch_bounds__(kGradThreads, sizeof(T) == 4 ? 8 : 5) embeddin
 #pragma unroll
             for (int e = 0; e < L::n; ++e) sum.t[e] += w * g[q].t[e];
             if (token[i + 2] == t && i + 1 < count) continue;
-            const bool began = from > 0 || token[0] != t, ends = token[i + 2] != t;
-            if (mine) {
-                if (began && ends) grad_table[static_cast<long long>(t) * units + u] = sum.v;
-                else parts[(2LL * blockIdx.x + (began ? 1 : 0)) * units + u] = sum.v;
-            }
-            sum = L{};
-            from = i + 1;
+            give(i, t);
         }
     }
     if constexpr (kWeights) {
@@ -272,8 +301,13 @@ void by_unit(bool wide, Fn&& fn) {
     else fn(T{});
 }
 
-// Chunks of the sorted pairs: eight CTAs for each of 148 SMs where there are enough pairs (a constant, so that sizes do not depend on the device).
-int grad_chunk(long pairs) { return static_cast<int>(std::max(16L, std::min<long>(kMaxChunk, (pairs + 1183) / 1184))); }
+// Chunks of the sorted pairs: as many CTAs as 148 SMs hold where there are enough pairs (a constant, so that sizes do not depend on the device).
+template <typename T>
+int grad_chunk(long pairs, long width) {
+    constexpr long ctas = 148 * grad_ctas<T>, per = 16 / sizeof(T) * kGradThreads;
+    const long slabs = std::max(1L, (width + per - 1) / per);
+    return static_cast<int>(std::max(16L, std::min<long>(kMaxChunk, (pairs * slabs + ctas - 1) / ctas)));
+}
 
 }  // namespace
 
@@ -322,7 +356,7 @@ namespace {
 struct Room { size_t parts, dots; };
 template <typename T>
 Room room(long pairs, long width) {
-    const long chunks = pairs > 0 ? (pairs + grad_chunk(pairs) - 1) / grad_chunk(pairs) : 0, slabs = (width + kGradThreads - 1) / kGradThreads;
+    const long chunk = grad_chunk<T>(pairs, width), chunks = (pairs + chunk - 1) / chunk, slabs = (width + kGradThreads - 1) / kGradThreads;
     return {(static_cast<size_t>(chunks) * 2 * width * sizeof(T) + 255) / 256 * 256, slabs > 1 ? static_cast<size_t>(slabs) * pairs * sizeof(T) : 0};
 }
 }  // namespace
@@ -359,7 +393,7 @@ void embedding_backward(const T* grad_y, long grad_y_stride, const T* table, lon
         return;
     }
     T* const dots = reinterpret_cast<T*>(static_cast<char*>(workspace) + room<T>(pairs, width).parts);
-    const int chunk = grad_chunk(pairs), chunks = static_cast<int>((pairs + chunk - 1) / chunk);
+    const int chunk = grad_chunk<T>(pairs, width), chunks = static_cast<int>((pairs + chunk - 1) / chunk);
     by_unit<T>(wide_rows<T>({grad_y, grad_table, grad_weights ? table : nullptr}, {grad_y_stride, width, grad_weights ? table_stride : 0}), [&](auto unit) {
         using V = decltype(unit);
         constexpr long per = sizeof(V) / sizeof(T);

@@ -25,7 +25,7 @@ constexpr int kMaxGroups = SMX_ROUTE_MAX_GROUPS;
 // ------------------------------------------------------------------------------------------- plan
 // Pairs are counted and ranked by warps that own consecutive pairs: 32 at a time, lanes of equal group found with match_any, one counter
 // per (warp, group) in shared memory that only that warp touches. Equal keys therefore keep their order. Latency bounds it: 13.5 us for 7,545
-// pairs in one CTA, 6 + 4 + 10 us for the three kernels at 196,608 pairs (2.4 MB).
+// pairs in one CTA, 25 us for the three kernels at 196,608 pairs of 64 groups (2.4 MB).
 // What is sorted: key(i) of element i, and what order[] receives for it; kPlan: with positions and offsets. kNames: `position` receives the name
 // of every place.
 struct GroupKeys {                               // pairs by group, empty slots last
@@ -183,15 +183,22 @@ __global__ void __launch_bounds__(kSmallPlanThreads) route_plan_small_kernel(con
 
 // Many pairs: counts per chunk, a scan over the chunks of every group, then the ranks. chunk_hist is [bins][chunks].
 constexpr int kPlanWarps = 8, kPlanThreads = 32 * kPlanWarps, kPlanChunk = 2048;
+// Plans of tokens have shorter chunks while longer ones leave SMs idle, down to 512 pairs (148 SMs: a constant, so that sizes do not depend on the device). 1,424 rows
+// of a table, 98,304 pairs: 27 us in 96 chunks of 1,024, 34 in 48 of 2,048. 4,000 rows, 196,608 pairs: 64 us in 192 chunks, 46 in 96.
+inline int token_chunk(long long pairs) {
+    int chunk = 512;
+    while (chunk < kPlanChunk && pairs > 148LL * chunk) chunk *= 2;
+    return chunk;
+}
 template <typename Keys>
-__global__ void __launch_bounds__(kPlanThreads) route_count_kernel(const Keys keys, long long pairs, int groups, int chunks,
+__global__ void __launch_bounds__(kPlanThreads) route_count_kernel(const Keys keys, long long pairs, int groups, int chunk, int chunks,
                                                                    int* __restrict__ chunk_hist) {
     extern __shared__ int route_smem[];
     const int bins = groups + 1, warp = threadIdx.x >> 5;
     for (int i = threadIdx.x; i < kPlanWarps * bins; i += kPlanThreads) route_smem[i] = 0;
     __syncthreads();
-    constexpr int per = kPlanChunk / kPlanWarps;
-    const long long begin = min(pairs, static_cast<long long>(blockIdx.x) * kPlanChunk + warp * per), end = min(pairs, begin + per);
+    const int per = chunk / kPlanWarps;
+    const long long begin = min(pairs, static_cast<long long>(blockIdx.x) * chunk + warp * per), end = min(pairs, begin + per);
     route_count(keys, begin, end, groups, route_smem + warp * bins);
     __syncthreads();
     for (int g = threadIdx.x; g < bins; g += kPlanThreads) {
@@ -220,7 +227,7 @@ __global__ void __launch_bounds__(256) route_scan_kernel(int bins, int chunks, i
     if (lane == 0) total[g] = run;
 }
 template <typename Keys>
-__global__ void __launch_bounds__(kPlanThreads) route_place_kernel(const Keys keys, long long pairs, int groups, int chunks,
+__global__ void __launch_bounds__(kPlanThreads) route_place_kernel(const Keys keys, long long pairs, int groups, int chunk, int chunks,
                                                                    const int* __restrict__ chunk_prefix, const int* __restrict__ total,
                                                                    int* __restrict__ order, int* __restrict__ position, int* __restrict__ offsets) {
     extern __shared__ int route_smem[];
@@ -233,8 +240,8 @@ __global__ void __launch_bounds__(kPlanThreads) route_place_kernel(const Keys ke
     for (int g = threadIdx.x; g < bins; g += kPlanThreads) start[g] = total[g];
     __syncthreads();
     cta_scan(start, bins, sums);
-    constexpr int per = kPlanChunk / kPlanWarps;
-    const long long begin = min(pairs, static_cast<long long>(blockIdx.x) * kPlanChunk + warp * per), end = min(pairs, begin + per);
+    const int per = chunk / kPlanWarps;
+    const long long begin = min(pairs, static_cast<long long>(blockIdx.x) * chunk + warp * per), end = min(pairs, begin + per);
     route_count(keys, begin, end, groups, hist + warp * bins);
     __syncthreads();
 #pragma unroll 4
@@ -488,7 +495,7 @@ void counting_sort(const Keys& keys, long long pairs, int num_groups, int* order
         launched("route_plan_small_kernel");
         return;
     }
-    const int chunks = static_cast<int>((pairs + kPlanChunk - 1) / kPlanChunk);
+    const int chunk = Keys::kNames ? token_chunk(pairs) : kPlanChunk, chunks = static_cast<int>((pairs + chunk - 1) / chunk);
     int* hist = static_cast<int*>(workspace);
     int* total = hist + static_cast<size_t>(bins) * chunks;
     const int smem = kPlanWarps * bins * static_cast<int>(sizeof(int));
@@ -498,11 +505,11 @@ void counting_sort(const Keys& keys, long long pairs, int num_groups, int* order
         SMX_CUDA(cudaFuncSetAttribute(route_place_kernel<Keys>, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024));
         mark_on_device(done);
     }
-    route_count_kernel<Keys><<<chunks, kPlanThreads, smem, stream>>>(keys, pairs, num_groups, chunks, hist);
+    route_count_kernel<Keys><<<chunks, kPlanThreads, smem, stream>>>(keys, pairs, num_groups, chunk, chunks, hist);
     launched("route_count_kernel");
     route_scan_kernel<<<(bins * 32 + 255) / 256, 256, 0, stream>>>(bins, chunks, hist, total);
     launched("route_scan_kernel");
-    route_place_kernel<Keys><<<chunks, kPlanThreads, smem + (bins + 1) * static_cast<int>(sizeof(int)), stream>>>(keys, pairs, num_groups, chunks, hist, total,
+    route_place_kernel<Keys><<<chunks, kPlanThreads, smem + (bins + 1) * static_cast<int>(sizeof(int)), stream>>>(keys, pairs, num_groups, chunk, chunks, hist, total,
                                                                                                                    order, position, offsets);
     launched("route_place_kernel");
 }
@@ -527,10 +534,11 @@ void route_slots(const int* order, long num_rows, int slots, const int* offsets,
     launched("route_slot_offsets_kernel");
 }
 
-// Tokens have up to 20 bits (the number of rows itself stands for pairs without a token): one digit as far as the counters of its values fit into shared
-// memory, or two of half of the bits. (98,304 pairs, 1,424 rows: 34 us by one digit; 60 by two, with keys that were not read ahead.)
+// Tokens have up to 20 bits (the number of rows itself stands for pairs without a token): one digit while its counters, one a warp and value, take less
+// than a second pass (and fit into shared memory), or two of half of the bits. 4,000 rows: 40 us by one digit, 42 by two at 98,304 pairs, 46 and 54 at 196,608, 233
+// and 155 at 2,000,000, where 2,000 rows take 141 by one and 2,900 rows 165.
 namespace {
-constexpr int kDigitValues = 4096;
+bool one_digit(long long pairs, int table_rows) { return table_rows < (pairs <= 148LL * kPlanChunk ? 4096 : 2500); }
 int digit_bits(int table_rows) {
     int bits = 1;
     while ((table_rows >> bits) >= (1 << bits)) ++bits;
@@ -538,15 +546,16 @@ int digit_bits(int table_rows) {
 }
 size_t sort_bytes(long pairs, int values) {
     if (pairs <= kSmallPlanPairs) return 0;
-    return static_cast<size_t>(values + 1) * ((pairs + kPlanChunk - 1) / kPlanChunk + 1) * sizeof(int);
+    const int chunk = token_chunk(pairs);
+    return static_cast<size_t>(values + 1) * ((pairs + chunk - 1) / chunk + 1) * sizeof(int);
 }
 }  // namespace
 size_t token_sort_bytes(long pairs, int table_rows) {
-    if (table_rows < kDigitValues) return sort_bytes(pairs, table_rows + 1);
+    if (one_digit(pairs, table_rows)) return sort_bytes(pairs, table_rows + 1);
     return (sort_bytes(pairs, 1 << digit_bits(table_rows)) + 255) / 256 * 256 + static_cast<size_t>(pairs) * sizeof(int);
 }
 void token_sort(const int* ids, long pairs, int table_rows, int* order, int* names, void* workspace, cudaStream_t stream) {
-    if (table_rows < kDigitValues) {
+    if (one_digit(pairs, table_rows)) {
         counting_sort(DigitKeys{ids, table_rows, nullptr, 0, 0x7fffffff}, pairs, table_rows + 1, order, names, nullptr, workspace, stream);
         return;
     }

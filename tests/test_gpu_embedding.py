@@ -65,7 +65,7 @@ def check(got, want):
 @pytest.mark.parametrize("n,slots,rows", [
     (0, 1, 1), (1, 1, 1), (1, 64, 5), (33, 1, 3), (100, 3, 1022), (100, 3, 1023), (100, 3, 1024), (500, 2, 1025), (1000, 1, 5000), (8192, 1, 1023), (8193, 1, 1023),
     (8193, 1, 1024), (4097, 2, 20000), (30000, 3, 1424), (70001, 1, 1048575), (200000, 2, 89), (300, 1, 1048575),
-    (5000, 1, 4095), (9000, 1, 4094), (9000, 1, 4095), (9000, 1, 4096), (30000, 2, 4097),
+    (5000, 1, 4095), (9000, 1, 4094), (9000, 1, 4095), (9000, 1, 4096), (30000, 2, 4097), (303105, 1, 2499), (303105, 1, 2500), (303104, 1, 4095), (75776, 1, 7), (75777, 1, 7), (151552, 1, 40), (50519, 3, 40),
 ])
 @pytest.mark.parametrize("kind", ["random", "skewed", "one", "outside", "empty"])
 def test_plan(n, slots, rows, kind):
