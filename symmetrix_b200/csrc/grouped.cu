@@ -201,6 +201,7 @@ void rows_f32(const smx_grouped_linear& c, bool transposed) {
     p.out = static_cast<float*>(transposed ? c.grad_x : c.y); p.out_stride = transposed ? c.grad_x_stride : c.y_stride;
     p.zero_tail = transposed || c.zero_tail;
     long long tiles = 0;
+    // whole lines are written straight from registers (98,304 atoms of 89 elements 92 us, 156 through shared memory, as other widths and starts have to go)
     bool wide = ((static_cast<unsigned long long>(p.out_stride) * 4u | reinterpret_cast<uintptr_t>(p.out)) & 31) == 0;
     for (int q = 0; q < p.degrees; ++q) {
         const GsDegree& d = p.degree[q];
@@ -240,7 +241,8 @@ void gradient_f32(const smx_grouped_linear& c, bool behind_rows) {
     join<float>(c);
 }
 
-// float64: tiles of 64 x 64, or of 16 x 32 while those leave SMs idle.
+// float64: tiles of 64 x 64, or of 16 x 32 while those leave SMs idle. 300 atoms of three groups (scalars and vectors, 128 x 128) 16.4 us with tiles of 64 x 64,
+// 10.2 with 16 x 32; 4,001 atoms of eight 30.7 and 34.8; 20,000 atoms of 16 groups behind two and three paths 223 and 297.
 template <int kMode, int BM, int BN, int WM, int WN, int ST>
 void launch_gd(const GdPass& p, long long tiles, const Launcher& on) {
     using L = GdLayout<kMode, BM, BN, ST>;
