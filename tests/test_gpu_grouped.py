@@ -7,12 +7,13 @@ unit roundoff, also in float64, where it covers the reference's own roundings. T
 further additions of small numbers: 24 steps cover them all.
 """
 import itertools
+import threading
 
 import numpy as np
 import pytest
 import torch
 
-from symmetrix_b200 import GroupedLinear, RowRouting, SymmetrixError, clip_gradients
+from symmetrix_b200 import Embedding, EmbeddingPlan, GroupedLinear, RowRouting, SymmetrixError, clip_gradients
 
 pytestmark = pytest.mark.gpu
 
@@ -285,6 +286,41 @@ def test_other_streams_and_graphs(dtype):
     graphs[0].replay()
     torch.cuda.synchronize()
     assert torch.equal(results[0][0], y2) and not torch.equal(y2, y)
+
+
+@BOTH
+def test_threads_share_the_operators(dtype):
+    """Four threads, each on a stream of its own, with the same linear, embedding, plan and inputs; the sets of gradients are each thread's own."""
+    case = Case(dtype, [300, 0, 170, 5], [1, 3], [64, 40], [48, 56])
+    ids = torch.as_tensor(np.random.default_rng(3).integers(-1, 40, (9000, 2)).astype(np.int32)).cuda()
+    table, gy = case.rand(40, 64), case.rand(9000, 64)
+    embedding, plan = Embedding(table), EmbeddingPlan(ids, 40)
+
+    def step():
+        y, grads = case.layer.forward(case.x, case.routing), case.layer.backward(case.x, case.gy, case.routing)
+        back = embedding.backward(gy, plan)
+        mine = [g.clone() for g in grads.weights] + [back.table.clone()]
+        norm = clip_gradients(mine, 0.5)
+        return [y, grads.x, *grads.weights, embedding.forward(ids), EmbeddingPlan(ids, 40).order, back.table, back.weights, norm, *mine]
+
+    want = step()
+    torch.cuda.synchronize()
+    results = [[] for _ in range(4)]
+
+    def work(q):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(5):
+                results[q].append(step())
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(q,)) for q in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    case.layer.check()
+    for runs in results:
+        assert len(runs) == 5 and all(torch.equal(a, b) for got in runs for a, b in zip(got, want))
 
 
 @BOTH
