@@ -218,12 +218,12 @@ void rows_f32(const smx_grouped_linear& c, bool transposed) {
     p.out = static_cast<float*>(transposed ? c.grad_x : c.y); p.out_stride = transposed ? c.grad_x_stride : c.y_stride;
     p.zero_tail = transposed || c.zero_tail;
     long long tiles = 0;
-    // whole lines are written straight from registers (98,304 atoms of 89 elements 92 us, 156 through shared memory, as other widths and starts have to go)
+    // whole sectors are written straight from registers (98,304 atoms of 89 elements 92 us, 156 through shared memory, as other widths and starts have to go)
     bool wide = ((static_cast<unsigned long long>(p.out_stride) * 4u | reinterpret_cast<uintptr_t>(p.out)) & 31) == 0;
     for (int q = 0; q < p.degrees; ++q) {
         const GsDegree& d = p.degree[q];
         tiles += (c.num_rows * d.comps / 128 + c.num_groups) * ((d.N + 127) / 128);
-        wide = wide && d.b_off % 8 == 0 && d.N % 64 == 0;
+        wide = wide && d.b_off % 8 == 0 && d.N % 8 == 0;
     }
     const Launcher on{static_cast<cudaStream_t>(c.stream), false};
     if (transposed) {
@@ -250,7 +250,7 @@ void gradient_f32(const smx_grouped_linear& c, bool behind_rows) {
         d.part = part;
         part += part_values(c, q);
         tiles += (c.num_rows * d.comps / p.chunk + c.num_groups) * ((d.N + 127) / 128) * ((d.K + 127) / 128);
-        wide = wide && d.N % 64 == 0 && (reinterpret_cast<uintptr_t>(d.grad) & 31) == 0;
+        wide = wide && d.N % 8 == 0 && (reinterpret_cast<uintptr_t>(d.grad) & 31) == 0;
     }
     const Launcher on{static_cast<cudaStream_t>(c.stream), behind_rows};
     if (wide) launch_gs<kGsGradient, true>(p, tiles, on);

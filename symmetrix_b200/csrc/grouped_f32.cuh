@@ -288,7 +288,7 @@ __device__ __forceinline__ void gs_products(uint32_t d, uint32_t a_hi, uint32_t 
     }
 }
 
-// kWide: every row's half of a tile of the output starts on 32 bytes and is 64 columns long.
+// kWide: every row of a tile of the output starts on 32 bytes, and its columns are a multiple of eight.
 template <bool kWide>
 struct GsLayout {
     static constexpr int raw_a = kWide ? 2 : 1;                                                            // tiles that an A warp's rows have room for
@@ -666,9 +666,9 @@ __global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid
 #pragma unroll
                 for (int i = 0; i < 4; ++i) rows_of[i] = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, mine, (lane & ~3) + i)) + 8 * (lane & 3);
                 const unsigned there = __ballot_sync(0xffffffffu, mine != 0) >> (lane & ~3);
-                if (left > 0)
 #pragma unroll
-                    for (int c = 0; c < 64; c += 32) {
+                for (int c = 0; c < 64; c += 32)
+                    if (c < left) {
                         gs_turn<1>(sum + c, sum + c + 8);
                         gs_turn<1>(sum + c + 16, sum + c + 24);
                         gs_turn<2>(sum + c, sum + c + 16);
@@ -676,7 +676,7 @@ __global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const float* v = sum + c + 8 * i;
-                            if ((there >> i) & 1u)
+                            if (((there >> i) & 1u) && c + 8 * (lane & 3) < left)
                                 asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(rows_of[i] + c), "f"(v[0]), "f"(v[1]), "f"(v[2]),
                                              "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]) : "memory");
                         }

@@ -107,6 +107,7 @@ SHAPES = [
     ([127, 128, 129], [1], [32], [128]), ([64, 0, 65, 63], [3], [64], [64]), ([5, 300, 1, 44], [1, 3], [128, 128], [128, 128]),
     ([40, 41], [2, 1, 4], [31, 1, 130], [7, 129, 1]), ([1000], [1], [768], [96]), ([17, 90], [1, 3, 5, 7], [48, 72, 72, 48], [24, 24, 24, 24]),
     ([3] * 70, [1], [20], [36]), ([700, 2, 700], [5], [36], [132]), ([9, 0, 2500], [1, 3], [66, 258], [130, 62]), ([6] * 1024, [1], [4], [4]),
+    ([140, 1, 77], [1, 3], [96, 40], [40, 96]), ([300, 20], [1], [72], [136]), ([200], [3, 1], [8, 24], [24, 200]),
     ([3, 0, 9], [40, 1], [36, 64], [64, 33]), ([2, 5], [1000], [7], [64]), ([1, 3], [1024, 33], [8, 64], [64, 8]), ([130], [31, 32], [64, 1], [1, 64]),
 ]
 
