@@ -29,7 +29,8 @@ struct ArgError : std::runtime_error {
 // between them matters. There they are launched with programmatic stream serialization (Launcher::overlap): a kernel may become
 // resident while its predecessor runs, and chain_begin(), the first statement of every kernel launched this way, waits until
 // the predecessor has finished and its writes are visible, then lets the successor come in (without the attribute both
-// instructions do nothing).
+// instructions do nothing). A kernel that waits later than that takes what its predecessor writes through plain pointers: `const __restrict__` would promise
+// that it does not change while the kernel runs, and allow its loads to come before the wait.
 __device__ __forceinline__ void chain_begin() {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");

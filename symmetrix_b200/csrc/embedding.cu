@@ -219,11 +219,11 @@ __global__ void __launch_bounds__(256) embedding_dots_kernel(const T* __restrict
 }
 
 // The runs that cross chunks: the CTAs of the chunk where one begins add its parts in order, kJoinWays of them side by side. Most CTAs have none; they
-// see that from the tokens, before the sums are there.
+// see that from the tokens, before the sums are there. (`parts` is written while CTAs of this kernel start: no promise that it is constant.)
 constexpr int kJoinUnits = 32, kJoinWays = 8;
 template <typename T, typename V>
 __global__ void __launch_bounds__(kJoinUnits * kJoinWays) embedding_join_kernel(const int* __restrict__ tokens, long long pairs, int table_rows, int units, int chunk,
-                                                                                int chunks, const V* __restrict__ parts, V* __restrict__ grad_table) {
+                                                                                int chunks, const V* parts, V* grad_table) {
     using L = Lanes<T, V>;
     __shared__ V joined[kJoinWays][kJoinUnits];
     const long long begin = static_cast<long long>(blockIdx.x) * chunk, end = begin + chunk;

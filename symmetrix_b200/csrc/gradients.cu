@@ -162,9 +162,10 @@ __device__ __forceinline__ double norm_of(const double* partial, int partials, d
     return sqrt(cta_sum(s, shared));
 }
 
+// `partial` is written while CTAs of this kernel start: no promise that it is constant.
 template <int N>
-__global__ void __launch_bounds__(kThreads) gradient_scale_kernel(const __grid_constant__ TensorList<N> list, const double* __restrict__ partial, int partials,
-                                                                  double max_norm, double* __restrict__ norm) {
+__global__ void __launch_bounds__(kThreads) gradient_scale_kernel(const __grid_constant__ TensorList<N> list, const double* partial, int partials,
+                                                                  double max_norm, double* norm) {
     __shared__ double shared[kThreads / 32];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const double n = norm_of(partial, partials, shared);
