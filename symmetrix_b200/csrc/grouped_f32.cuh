@@ -326,7 +326,7 @@ __global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid
     extern __shared__ unsigned char gs_smem_raw[];
     // ready: a stage of A is there and its partial sum has been read; done: its products are; raw_*: tiles of the operand warps, A's first
     __shared__ __align__(8) unsigned long long work_full[kGsRing], work_free[kGsRing], ready[kGsStages], done[kGsStages], b_full[kGsStages], b_free[kGsStages],
-        raw_full[8 * (kRawA + 1)], raw_free[8 * (kRawA + 1)], drained;
+        raw_full[8 * (kRawA + 1)], raw_free[8 * (kRawA + 1)];
     __shared__ GsWork work[kGsRing];
     __shared__ uint32_t tmem_slot;
     __shared__ int guard[2];                                                             // a wait ran out; polls of a wait
@@ -339,7 +339,6 @@ __global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid
         for (int q = 0; q < kGsRing; ++q) { mbar_init(&work_full[q], 1); mbar_init(&work_free[q], 29); }
         for (int q = 0; q < kGsStages; ++q) { mbar_init(&ready[q], 16); mbar_init(&done[q], 1); mbar_init(&b_full[q], 8); mbar_init(&b_free[q], 1); }
         for (int q = 0; q < 8 * (kRawA + 1); ++q) { mbar_init(&raw_full[q], 32); mbar_init(&raw_free[q], 1); }
-        mbar_init(&drained, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     // The gradient reads nothing that the rows' pass before it writes: its CTAs come in as that one's end.
@@ -356,7 +355,7 @@ __global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid
     if (warp < 4) {
         ts_registers_less<kGsRegsControl>();
         if (warp == 0) {
-            int na = 0, nb = 0, base_b = 0;                          // stages of A (and partial sums) and of B used so far; B's first one of the tile
+            int na = 0, nb = 0, base_b = 0, freed = 0;               // stages of A (and partial sums) and of B used so far; B's first one of the tile; those given back
             bool ok = true;
             const bool leader = ts_elect();
             const uint32_t b_at = smem_u32(stages);
@@ -385,8 +384,13 @@ __global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid
                         ts_commit(&done[st]);
                     }
                     __syncwarp();
+                    if (last) freed = n + 1;
                 }
             }
+            // What was started ends, and what it arrives at is told, before the CTA ends: products read its shared and tensor memory, and nobody else waits for the last
+            // stages of B.
+            for (int q = max(0, na - kGsStages); q < na; ++q) mbar_wait(&done[q % kGsStages], (q / kGsStages) & 1);
+            for (int q = max(0, freed - kGsStages); q < freed; ++q) mbar_wait(&b_free[q % kGsStages], (q / kGsStages) & 1);
         } else if (warp == 1) {
             GsCursor cursor;
             int begin, end, i = 0, last_degree = -1, last_group = 0, last_block = 0;
@@ -416,13 +420,7 @@ __global__ void __launch_bounds__(kGsThreads, 1) grouped_f32_kernel(const __grid
                 for (long long c = lane; c < pass.out_width; c += 32) pass.out[p * pass.out_stride + c] = 0.f;
         }
         gs_meet();
-        if (guard[0] && warp == 0) {
-            // what was started ends before the CTA does: products read its shared and tensor memory
-            if (ts_elect()) ts_commit(&drained);
-            __syncwarp();
-            mbar_wait(&drained, 0);
-            if (lane == 0 && pass.status) atomicMax(pass.status, kGsStatusWait);
-        }
+        if (guard[0] && threadIdx.x == 0 && pass.status) atomicMax(pass.status, kGsStatusWait);
     } else if (warp < 12) {
         ts_registers_less<kGsRegsOperand>();
         const uint32_t lanes = a_at + (static_cast<uint32_t>((warp & 3) * 32) << 16);
