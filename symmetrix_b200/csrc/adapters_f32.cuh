@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
     using L = TsPassLayout<HP, kWide>;
     constexpr int NS = L::stages, RS = L::row_stages, kRing = L::work_ring;
     extern __shared__ unsigned char ts_smem_raw[];
-    __shared__ __align__(8) unsigned long long work_full[kRing], work_free[kRing], full[NS], free[NS], d_full[2], d_free[2], t_full, t_done, drained;
+    __shared__ __align__(8) unsigned long long work_full[kRing], work_free[kRing], full[NS], free[NS], d_full[2], d_free[2], t_full, t_done;
     __shared__ TsWork work[kRing];
     __shared__ long long work_in[kRing][kTsRows];                                          // where its rows start in `in`;
     __shared__ int work_atom[kRing][kTsRows], work_place[kRing][kTsRows];                  // their atoms, sorted positions
@@ -278,7 +278,6 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
         for (int q = 0; q < 2; ++q) { mbar_init(&d_full[q], 1); mbar_init(&d_free[q], 8); }
         mbar_init(&t_full, 8);
         mbar_init(&t_done, 1);
-        mbar_init(&drained, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) {
@@ -374,7 +373,7 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
             }
             copies = n;
         } else if (warp == 1) {
-            int st = 0, sum = 0, nd = 0;                                 // stage and partial sum in turn, with the parity of their next and last use
+            int st = 0, sum = 0, nd = 0, used = 0, added = 0;            // stage and partial sum in turn, with the parity of their next and last use; stages, tiles with rounds so far
             unsigned st_par = 0, sum_par = 1, hid_par = 0;
             bool ok = true;
             const bool leader = ts_elect();
@@ -426,25 +425,26 @@ __global__ void __launch_bounds__(kTsPassThreads, 1) adapter_pass_f32_kernel(con
                         if (last_round) ts_commit(&t_done);
                     }
                     __syncwarp();
+                    ++used;
                     if (++st == NS) { st = 0; st_par ^= 1u; }
                     if (last_sum) {
                         ++nd;
                         sum ^= 1;
                         if (sum == 0) sum_par ^= 1u;
                     }
-                    if (last_round) hid_par ^= 1u;
+                    if (last_round) { hid_par ^= 1u; ++added; }
                 }
             }
+            // What was started ends, and what it arrives at is told, before the CTA ends: products read its shared and tensor memory, and nobody else waits for
+            // the last stages.
+            for (int q = max(0, used - NS); q < used; ++q) mbar_wait(&free[q % NS], (q / NS) & 1);
+            for (int q = max(0, nd - 2); q < nd; ++q) mbar_wait(&d_full[q & 1], (q >> 1) & 1);
+            if (added > 0) mbar_wait(&t_done, (added - 1) & 1);
         }
         ts_meet();
         if (guard[0]) {
-            // what was started ends before the CTA does: products read its shared and tensor memory, copies write into the former
-            if (warp == 1) {
-                if (ts_elect()) ts_commit(&drained);
-                __syncwarp();
-                mbar_wait(&drained, 0);
-            } else if (warp == 0 && lane == 0) {
-                // the last chunks' barriers, with the arrivals that row warps still owed them
+            if (warp == 0 && lane == 0) {
+                // copies write into the CTA's shared memory: the last chunks' barriers, with the arrivals that row warps still owed them
                 for (int q = max(0, copies - NS); q < copies; ++q) {
                     for (int w = 0; w < 4; ++w)
                         if (row_uses[w] <= q) mbar_arrive(&full[q % NS]);

@@ -29,7 +29,7 @@ def test_waits_for_the_last_uses_of_all_stages(stages, count):
         assert all(bars[q % stages].wait((q // stages) & 1) for q in last) == (missing is None)
 
 
-@pytest.mark.parametrize("file,kernel", [("grouped_f32.cuh", "grouped_f32_kernel")])
+@pytest.mark.parametrize("file,kernel", [("grouped_f32.cuh", "grouped_f32_kernel"), ("adapters_f32.cuh", "adapter_pass_f32_kernel")])
 def test_whoever_commits_products_waits_for_every_barrier_they_arrive_at(file, kernel):
     text = (CSRC / file).read_text()
     body = text[text.index(f" {kernel}("):]
