@@ -25,26 +25,31 @@ constexpr int kMaxGroups = SMX_ROUTE_MAX_GROUPS;
 // ------------------------------------------------------------------------------------------- plan
 // Pairs are counted and ranked by warps that own consecutive pairs: 32 at a time, lanes of equal group found with match_any, one counter
 // per (warp, group) in shared memory that only that warp touches. Equal keys therefore keep their order. Latency bounds it: 13.5 us for 7,545
-// pairs in one CTA, 25 us for the three kernels at 196,608 pairs of 64 groups (2.4 MB).
+// pairs in one CTA, 14.4 us for the three kernels at 196,608 pairs of 64 groups (2.4 MB).
 // What is sorted: key(i) of element i, and what order[] receives for it; kPlan: with positions and offsets. kNames: `position` receives the name
-// of every place.
+// of every place. kAheadSmall, kAhead: keys read ahead in one CTA, and in the three kernels. Where keys come from an array that is known to be constant the compiler
+// reads ahead by itself in those (98,304 pairs of one group 9.0 us; 9.3 with four ahead by hand, 9.6 with eight), and four are as good as eight in one CTA. Digits
+// of tokens are looked up behind one another: eight.
 struct GroupKeys {                               // pairs by group, empty slots last
     static constexpr bool kPlan = true, kNames = false;
+    static constexpr int kAheadSmall = 4, kAhead = 1;
     const int* ids; int groups;
     __device__ __forceinline__ int key(long long i) const {
-        const int g = ids[i];
+        const int g = __ldg(ids + i);
         return (g < 0 || g >= groups) ? groups : g;
     }
     __device__ __forceinline__ int value(long long i) const { return static_cast<int>(i); }
 };
 struct SlotKeys {                                // places by the slot of their pair, order[i] = n * slots + slot (see route_slots)
     static constexpr bool kPlan = false, kNames = false;
+    static constexpr int kAheadSmall = 4, kAhead = 1;
     const int* order; int slots;
-    __device__ __forceinline__ int key(long long i) const { return order[i] % slots; }
+    __device__ __forceinline__ int key(long long i) const { return __ldg(order + i) % slots; }
     __device__ __forceinline__ int value(long long i) const { return static_cast<int>(i); }
 };
 struct DigitKeys {                               // pairs by a digit of their token, in the order that the lower digits gave (null: as they come)
     static constexpr bool kPlan = false, kNames = true;
+    static constexpr int kAheadSmall = 8, kAhead = 8;
     const int* ids; int table_rows; const int* before; int shift, mask;
     __device__ __forceinline__ int value(long long i) const { return before ? before[i] : static_cast<int>(i); }
     __device__ __forceinline__ int name(int pair) const {
@@ -54,10 +59,8 @@ struct DigitKeys {                               // pairs by a digit of their to
     __device__ __forceinline__ int key(long long i) const { return (name(value(i)) >> shift) & mask; }
 };
 
-// The keys are read ahead: one after the other, each would wait for memory (one CTA, 4,001 tokens: 15.4 us a plan, 12.3 with eight ahead and the
-// warps' counters added up by lanes).
-constexpr int kKeysAhead = 8;
-template <typename Keys>
+// kKeysAhead keys at a time: one after the other, each would wait for memory.
+template <int kKeysAhead, typename Keys>
 __device__ __forceinline__ void route_count(const Keys& keys, long long begin, long long end, int groups, int* __restrict__ hist) {
     const int lane = threadIdx.x & 31;
     for (long long i1 = begin; i1 < end; i1 += 32 * kKeysAhead) {
@@ -78,7 +81,7 @@ __device__ __forceinline__ void route_count(const Keys& keys, long long begin, l
 }
 
 // `next[g]`: where this warp's next pair of group g goes.
-template <typename Keys>
+template <int kKeysAhead, typename Keys>
 __device__ __forceinline__ void route_place(const Keys& keys, long long begin, long long end, int groups, int* __restrict__ next,
                                             int* __restrict__ order, int* __restrict__ position) {
     const int lane = threadIdx.x & 31;
@@ -142,7 +145,9 @@ __device__ __forceinline__ void cta_scan(int* v, int n, int* sums) {
     __syncthreads();
 }
 
-// Few pairs: one CTA does all three steps.
+// Few pairs: one CTA does all three steps. The warps' counters of a group are added up by the lanes of a warp where every group can have one, by a thread otherwise (4,001
+// pairs, in us by lanes and by a thread: 3 groups 5.1 and 5.6; 63 groups 14.9 and 11.1, 511 groups 48 and 13.4). With 32 counters in a row, those of a group lie in one bank: a thread
+// then, too.
 constexpr int kSmallPlanThreads = 1024, kSmallPlanPairs = 8192;
 template <typename Keys>
 __global__ void __launch_bounds__(kSmallPlanThreads) route_plan_small_kernel(const Keys keys, int pairs, int groups, int warps_used,
@@ -157,28 +162,45 @@ __global__ void __launch_bounds__(kSmallPlanThreads) route_plan_small_kernel(con
     __syncthreads();
     const int per = ((pairs + warps_used - 1) / warps_used + 31) & ~31;
     const int begin = min(pairs, warp * per), end = min(pairs, begin + per);
-    if (warp < warps_used) route_count(keys, begin, end, groups, hist + warp * bins);
+    if (warp < warps_used) route_count<Keys::kAheadSmall>(keys, begin, end, groups, hist + warp * bins);
     __syncthreads();
-    const int lane = threadIdx.x & 31;               // a warp takes a group, a lane the counter of one warp
-    for (int g = warp; g < bins; g += blockDim.x >> 5) {
-        const int c = lane < warps_used ? hist[lane * bins + g] : 0;
-        int incl = c;
+    const int lane = threadIdx.x & 31;
+    const bool by_lanes = bins < 32 && bins <= static_cast<int>(blockDim.x >> 5);
+    if (by_lanes) {
+        if (warp < bins) {
+            const int c = lane < warps_used ? hist[lane * bins + warp] : 0;
+            int incl = c;
 #pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const int up = __shfl_up_sync(0xffffffffu, incl, d);
-            if (lane >= d) incl += up;
+            for (int d = 1; d < 32; d <<= 1) {
+                const int up = __shfl_up_sync(0xffffffffu, incl, d);
+                if (lane >= d) incl += up;
+            }
+            if (lane < warps_used) hist[lane * bins + warp] = incl - c;
+            if (lane == 31) total[warp] = incl;
         }
-        if (lane < warps_used) hist[lane * bins + g] = incl - c;
-        if (lane == 31) total[g] = incl;
+    } else {
+        for (int g = threadIdx.x; g < bins; g += blockDim.x) {
+            int run = 0;
+            for (int w = 0; w < warps_used; ++w) { const int c = hist[w * bins + g]; hist[w * bins + g] = run; run += c; }
+            total[g] = run;
+        }
     }
     __syncthreads();
     cta_scan(total, bins, sums);
-    for (int g = warp; g < bins; g += blockDim.x >> 5) {
-        if (Keys::kPlan && lane == 0) offsets[g] = total[g];     // bins = groups + 1 entries: the start of the empty slots is the end of the groups
-        if (lane < warps_used) hist[lane * bins + g] += total[g];
+    // bins = groups + 1 entries: the start of the empty slots is the end of the groups
+    if (by_lanes) {
+        if (warp < bins) {
+            if (Keys::kPlan && lane == 0) offsets[warp] = total[warp];
+            if (lane < warps_used) hist[lane * bins + warp] += total[warp];
+        }
+    } else {
+        for (int g = threadIdx.x; g < bins; g += blockDim.x) {
+            if (Keys::kPlan) offsets[g] = total[g];
+            for (int w = 0; w < warps_used; ++w) hist[w * bins + g] += total[g];
+        }
     }
     __syncthreads();
-    if (warp < warps_used) route_place(keys, begin, end, groups, hist + warp * bins, order, position);
+    if (warp < warps_used) route_place<Keys::kAheadSmall>(keys, begin, end, groups, hist + warp * bins, order, position);
 }
 
 // Many pairs: counts per chunk, a scan over the chunks of every group, then the ranks. chunk_hist is [bins][chunks].
@@ -191,15 +213,15 @@ inline int token_chunk(long long pairs) {
     return chunk;
 }
 template <typename Keys>
-__global__ void __launch_bounds__(kPlanThreads) route_count_kernel(const Keys keys, long long pairs, int groups, int chunk, int chunks,
+__global__ void __launch_bounds__(kPlanThreads) route_count_kernel(const Keys keys, long long pairs, int groups, int chunk_of_tokens, int chunks,
                                                                    int* __restrict__ chunk_hist) {
     extern __shared__ int route_smem[];
     const int bins = groups + 1, warp = threadIdx.x >> 5;
     for (int i = threadIdx.x; i < kPlanWarps * bins; i += kPlanThreads) route_smem[i] = 0;
     __syncthreads();
-    const int per = chunk / kPlanWarps;
+    const int chunk = Keys::kNames ? chunk_of_tokens : kPlanChunk, per = chunk / kPlanWarps;
     const long long begin = min(pairs, static_cast<long long>(blockIdx.x) * chunk + warp * per), end = min(pairs, begin + per);
-    route_count(keys, begin, end, groups, route_smem + warp * bins);
+    route_count<Keys::kAhead>(keys, begin, end, groups, route_smem + warp * bins);
     __syncthreads();
     for (int g = threadIdx.x; g < bins; g += kPlanThreads) {
         int sum = 0;
@@ -227,7 +249,7 @@ __global__ void __launch_bounds__(256) route_scan_kernel(int bins, int chunks, i
     if (lane == 0) total[g] = run;
 }
 template <typename Keys>
-__global__ void __launch_bounds__(kPlanThreads) route_place_kernel(const Keys keys, long long pairs, int groups, int chunk, int chunks,
+__global__ void __launch_bounds__(kPlanThreads) route_place_kernel(const Keys keys, long long pairs, int groups, int chunk_of_tokens, int chunks,
                                                                    const int* __restrict__ chunk_prefix, const int* __restrict__ total,
                                                                    int* __restrict__ order, int* __restrict__ position, int* __restrict__ offsets) {
     extern __shared__ int route_smem[];
@@ -240,9 +262,9 @@ __global__ void __launch_bounds__(kPlanThreads) route_place_kernel(const Keys ke
     for (int g = threadIdx.x; g < bins; g += kPlanThreads) start[g] = total[g];
     __syncthreads();
     cta_scan(start, bins, sums);
-    const int per = chunk / kPlanWarps;
+    const int chunk = Keys::kNames ? chunk_of_tokens : kPlanChunk, per = chunk / kPlanWarps;
     const long long begin = min(pairs, static_cast<long long>(blockIdx.x) * chunk + warp * per), end = min(pairs, begin + per);
-    route_count(keys, begin, end, groups, hist + warp * bins);
+    route_count<Keys::kAhead>(keys, begin, end, groups, hist + warp * bins);
     __syncthreads();
 #pragma unroll 4
     for (int g = threadIdx.x; g < bins; g += kPlanThreads) {
@@ -252,7 +274,7 @@ __global__ void __launch_bounds__(kPlanThreads) route_place_kernel(const Keys ke
         for (int w = 0; w < kPlanWarps; ++w) { const int c = hist[w * bins + g]; hist[w * bins + g] = run; run += c; }
     }
     __syncthreads();
-    route_place(keys, begin, end, groups, hist + warp * bins, order, position);
+    route_place<Keys::kAhead>(keys, begin, end, groups, hist + warp * bins, order, position);
 }
 
 // Where group g begins among slot s's places (sorted positions, ascending; runs of num_rows): a warp each, cutting the run into 33 pieces per step.

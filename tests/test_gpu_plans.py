@@ -1,0 +1,72 @@
+"""Plans of few pairs, around the sizes where one CTA adds its warps' counters up in another way: against a stable sort on the host, and their time with many groups."""
+import numpy as np
+import pytest
+import torch
+
+from symmetrix_b200 import EmbeddingPlan, RowRouting
+
+pytestmark = pytest.mark.gpu
+
+COUNTS = [1, 2, 5, 14, 15, 16, 28, 29, 30, 31, 32, 33, 63]
+PAIRS = [1, 31, 33, 97, 128, 129, 500, 961, 993, 1025, 8192]
+
+
+def ids_of(pairs, count, seed):
+    ids = np.random.default_rng(seed).integers(-1, count + 1, size=pairs).astype(np.int32)
+    key = np.where((ids < 0) | (ids >= count), count, ids)
+    return torch.as_tensor(ids).cuda(), key, np.argsort(key, kind="stable")
+
+
+@pytest.mark.parametrize("pairs", PAIRS)
+@pytest.mark.parametrize("groups", COUNTS)
+def test_plan_of_rows(pairs, groups):
+    ids, key, order = ids_of(pairs, groups, pairs + groups)
+    plan = RowRouting(ids, groups)
+    np.testing.assert_array_equal(plan.order.cpu().numpy(), order)
+    np.testing.assert_array_equal(plan.offsets.cpu().numpy(), np.searchsorted(key[order], np.arange(groups + 1)))
+    position = np.empty(pairs, np.int64)
+    position[order] = np.arange(pairs)
+    np.testing.assert_array_equal(plan.position.cpu().numpy().reshape(-1), np.where(key < groups, position, -1))
+
+
+@pytest.mark.parametrize("pairs", PAIRS)
+@pytest.mark.parametrize("rows", COUNTS)
+def test_plan_of_tokens(pairs, rows):
+    ids, key, order = ids_of(pairs, rows, pairs + rows)
+    plan = EmbeddingPlan(ids, rows)
+    np.testing.assert_array_equal(plan.order.cpu().numpy(), order)
+    np.testing.assert_array_equal(plan.tokens.cpu().numpy(), key[order])
+
+
+def _graph_us(fn, calls=20):
+    """Least time of a call inside a replayed graph."""
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        fn()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        for _ in range(calls):
+            fn()
+    times = []
+    for _ in range(20):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        graph.replay()
+        b.record()
+        torch.cuda.synchronize()
+        times.append(a.elapsed_time(b) * 1e3 / calls)
+    return min(times)
+
+
+# measured ratios: 1.8, 1.8, 1.9 and 4.8; 13, 12, 6.9 and 36 where a warp adds up each group's counters, one after the other
+@pytest.mark.parametrize("make,pairs,few,many,most", [(RowRouting, 18, 16, 1023, 4.0), (RowRouting, 300, 16, 1023, 4.0), (RowRouting, 4001, 16, 1023, 4.0), (EmbeddingPlan, 300, 2, 4000, 12.0)])
+def test_many_groups_do_not_slow_a_small_plan_down(make, pairs, few, many, most):
+    """Ratios of times on the same GPU: the sort of a few pairs costs what its pairs cost, not a chain of steps for each group."""
+    torch.manual_seed(3)
+    us = []
+    for count in (few, many):
+        ids = torch.randint(0, count, (pairs,), device="cuda", dtype=torch.int32)
+        plan = make(ids, count)
+        us.append(_graph_us(lambda: plan.update(ids)))
+    assert us[1] <= most * us[0], us
