@@ -4,8 +4,9 @@
 //   grad_table[t] = scale sum over pairs (n, s) with ids[n, s] = t of w[n, s] grad_y[n],   grad_w[n, s] = scale <grad_y[n], table[ids[n, s]]>
 //
 // A pair whose id is no row of the table (negative or too large) counts for nothing. The sums of the table's gradient go over the pairs sorted by
-// token (csrc/routing.cu), cut into chunks of equal length: a token's run inside a chunk is one sum; runs that cross chunks leave partial sums,
-// which are added in order. No atomics: the same call gives the same bits.
+// token (csrc/routing.cu), cut into chunks of equal length: a token's run inside a chunk is one sum, of sums of eight where it is long; runs that cross chunks leave
+// partial sums, which are added in order and in 64 bits. So a sum's error does not grow with its length: at most some 90 roundings whatever the number of pairs. No
+// atomics: the same call gives the same bits.
 #include "embedding.hpp"
 
 #include <algorithm>
@@ -175,12 +176,15 @@ __global__ void __launch_bounds__(kGradThreads, grad_ctas<T>) embedding_grad_ker
         }
         if (!grad_table) continue;
         if (one) {
+            L eight{};
 #pragma unroll
             for (int q = 0; q < kLoads; ++q) {
                 const T w = weight[i0 + q];
 #pragma unroll
-                for (int e = 0; e < L::n; ++e) sum.t[e] += w * g[q].t[e];
+                for (int e = 0; e < L::n; ++e) eight.t[e] += w * g[q].t[e];
             }
+#pragma unroll
+            for (int e = 0; e < L::n; ++e) sum.t[e] += eight.t[e];
             const int i = i0 + kLoads - 1;
             if (token[i + 2] != t0 || i + 1 == count) give(i, t0);
             continue;
@@ -212,9 +216,9 @@ __global__ void __launch_bounds__(kGradThreads, grad_ctas<T>) embedding_grad_ker
 template <typename T>
 __global__ void __launch_bounds__(256) embedding_dots_kernel(const T* __restrict__ dots, long long pairs, int slabs, T scale, T* __restrict__ grad_weights) {
     for (long long i = blockIdx.x * 256LL + threadIdx.x; i < pairs; i += 256LL * gridDim.x) {
-        T s = T(0);
+        double s = 0.0;
         for (int q = 0; q < slabs; ++q) s += dots[q * pairs + i];
-        grad_weights[i] = scale * s;
+        grad_weights[i] = static_cast<T>(scale * s);
     }
 }
 
@@ -225,7 +229,7 @@ template <typename T, typename V>
 __global__ void __launch_bounds__(kJoinUnits * kJoinWays) embedding_join_kernel(const int* __restrict__ tokens, long long pairs, int table_rows, int units, int chunk,
                                                                                 int chunks, const V* parts, V* grad_table) {
     using L = Lanes<T, V>;
-    __shared__ V joined[kJoinWays][kJoinUnits];
+    __shared__ double joined[kJoinWays][L::n][kJoinUnits];
     const long long begin = static_cast<long long>(blockIdx.x) * chunk, end = begin + chunk;
     int t = table_rows, after = -1, before = -1;
     if (end < pairs) {
@@ -246,7 +250,7 @@ __global__ void __launch_bounds__(kJoinUnits * kJoinWays) embedding_join_kernel(
     }
     const int lane = threadIdx.x % kJoinUnits, way = threadIdx.x / kJoinUnits, u = blockIdx.y * kJoinUnits + lane;
     const int per = (more + 1 + kJoinWays - 1) / kJoinWays, first = way * per, last = min(more + 1, first + per);
-    L sum{};
+    double sum[L::n] = {};
     if (u < units) {
         for (int i0 = first; i0 < last; i0 += 8) {
             L v[8];
@@ -258,19 +262,20 @@ __global__ void __launch_bounds__(kJoinUnits * kJoinWays) embedding_join_kernel(
 #pragma unroll
             for (int q = 0; q < 8; ++q)
 #pragma unroll
-                for (int e = 0; e < L::n; ++e) sum.t[e] += v[q].t[e];
+                for (int e = 0; e < L::n; ++e) sum[e] += v[q].t[e];
         }
     }
-    joined[way][lane] = sum.v;
+#pragma unroll
+    for (int e = 0; e < L::n; ++e) joined[way][e][lane] = sum[e];
     __syncthreads();
     if (way > 0 || u >= units) return;
-    for (int w = 1; w < kJoinWays; ++w) {
-        L v;
-        v.v = joined[w][lane];
+    L out;
 #pragma unroll
-        for (int e = 0; e < L::n; ++e) sum.t[e] += v.t[e];
+    for (int e = 0; e < L::n; ++e) {
+        for (int w = 1; w < kJoinWays; ++w) sum[e] += joined[w][e][lane];
+        out.t[e] = static_cast<T>(sum[e]);
     }
-    grad_table[static_cast<long long>(t) * units + u] = sum.v;
+    grad_table[static_cast<long long>(t) * units + u] = out.v;
 }
 
 // ------------------------------------------------------------------------------------------- host side
