@@ -397,7 +397,9 @@ int smx_adapter_backward(const smx_adapter_linear* call, char* errbuf, int errbu
  * smx_grouped_backward writes, each unless NULL, grad_x and the degrees' grad_weight (for all degrees or none; groups without rows get
  * zeros). Rows behind the last group are never read; in `y` they are left as they were, or zeroed with `zero_tail` != 0, in grad_x they are zeroed.
  * The matrices are read as they are, in every call: changed values count at once. Sums, float32 operands, NaN, infinities, waits inside the float32 kernels,
- * `status`, streams, workspaces (smx_grouped_workspace_bytes; it starts on a 32-byte boundary) and limits: as for smx_adapter_*. Outputs must not overlap inputs or one another. */
+ * `status`, streams, workspaces (smx_grouped_workspace_bytes; it starts on a 32-byte boundary) and limits: as for smx_adapter_*. Outputs must not overlap inputs or one another.
+ * The workspace of the matrices' gradients grows with the rows and the matrices' size: a matrix for every 4,096 component rows, more of them where there are few tiles, and up to one more
+ * for each group (98,304 rows of seven components, 2,048 x 2,048 in float32, one group: 2.8 GB). */
 enum { SMX_GROUPED_MAX_DEGREES = 8 };
 typedef struct smx_grouped_degree {
     int components, in_channels, out_channels;

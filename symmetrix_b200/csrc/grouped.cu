@@ -77,7 +77,8 @@ void check_weights(const smx_grouped_linear& c) {
 }
 
 // What a call allocates nothing for: the partial sums of the matrices' gradients. Their chunks of rows are as long as leaves four tiles for each of 148
-// SMs (a constant, so that sizes and sums do not depend on the device); a group with several chunks has less than twice as many as its rows fill.
+// SMs (a constant, so that sizes and sums do not depend on the device), and 4,096 rows at most: longer float32 sums lose more, and joining them costs little beside the
+// products (98,304 atoms, seven components, 2,048 x 2,048: 2.8 GB of sums, joined in 1.7 of 41 ms).
 int grad_chunk(const smx_grouped_linear& c) {
     const int tile = c.precision == SMX_FP32 ? 128 : 64;
     long long steps = 0;
@@ -89,7 +90,8 @@ int grad_chunk(const smx_grouped_linear& c) {
 }
 size_t part_values(const smx_grouped_linear& c, int d) {
     const smx_grouped_degree& g = c.degrees[d];
-    const long long parts = 2 * (c.num_rows * static_cast<long long>(g.components) / grad_chunk(c));
+    // a group with several chunks has one more at most than its rows fill
+    const long long whole = c.num_rows * static_cast<long long>(g.components) / grad_chunk(c), parts = whole + std::min<long long>(c.num_groups, whole);
     return static_cast<size_t>((parts * g.in_channels * g.out_channels + 63) / 64 * 64);
 }
 
