@@ -448,10 +448,11 @@ int smx_embedding_backward(int precision, const void* grad_y, long grad_y_stride
                            int errbuf_len);
 
 /* The common norm of many tensors, and their scaling to at most a given one, as training does with all gradients before a step:
- *   norm = sqrt(sum over all values t^2),   out = values * (norm > max_norm ? max_norm / norm : 1)
+ *   norm = sqrt(sum over all values t^2),   out = values * (norm <= max_norm ? 1 : max_norm / norm)
  * A tensor is `count` consecutive values of a precision of its own; `out` may be `values`, or memory that overlaps no tensor of the list.
  * Squares, sums and products are float64; a product is rounded once. A NaN makes the norm and all outputs NaN; an infinity makes the norm
- * infinite, finite values zero and infinite ones NaN (unless max_norm is infinite too). smx_gradient_norm ignores `out`; `norm` is a device double and may be NULL in
+ * infinite, finite values zero and infinite ones NaN (unless max_norm is infinite too). Squares beyond float64's range, of float64 values from 1e154 on, make the norm infinite too, and
+ * those of values below 1e-162 are zero. smx_gradient_norm ignores `out`; `norm` is a device double and may be NULL in
  * smx_gradient_clip. The list itself is read on the host, during the call. The rules of the smx_route_* calls hold, with a workspace of
  * smx_gradient_workspace_bytes for each call that may overlap with another one. Limit: 2^40 values a tensor. */
 typedef struct smx_gradient {

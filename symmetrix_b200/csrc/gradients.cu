@@ -1,6 +1,6 @@
 // The common norm of many tensors, and their scaling to at most a given norm (smx_gradient_*).
 //
-//   norm = sqrt(sum over tensors and values of t^2),   out = t * (norm > max_norm ? max_norm / norm : 1)
+//   norm = sqrt(sum over tensors and values of t^2),   out = t * (norm <= max_norm ? 1 : max_norm / norm)
 //
 // Squares and sums are float64 whatever the tensors' type: a float32 square leaves the type's range from 1e19 on upwards and below 1e-23. Tensors are cut into
 // tiles; the CTAs of the first kernel own consecutive tiles and write one partial sum each, the CTAs of the second one add all of them in the same

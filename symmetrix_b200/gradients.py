@@ -30,7 +30,8 @@ class GradientSet:
     receives the scaled values, the tensors themselves without it. Nothing in the lists may overlap, except an output with its own tensor
     where both are the same memory.
 
-    The set holds on to the tensors' memory as it is when the set is made: a program whose gradients have buffers of their own makes it once."""
+    The set holds on to the tensors' memory as it is when the set is made: a program whose gradients have buffers of their own makes it once. That memory must stay theirs: a
+    tensor whose storage is resized afterwards needs another set."""
 
     def __init__(self, tensors, out=None):
         tensors = list(tensors)
@@ -75,8 +76,8 @@ class GradientSet:
         return buffer[0]
 
     def clip(self, max_norm: float):
-        """Multiplies the tensors by ``max_norm / norm`` where the norm exceeds ``max_norm`` (into ``out``, which otherwise receives copies) and returns the
-        norm before that."""
+        """Multiplies the tensors by ``max_norm / norm`` unless the norm is ``max_norm`` or less (into ``out``, which then receives copies) and returns the
+        norm before that. A NaN among the values makes the norm and all results NaN; an infinite norm (infinities, float64 values from 1e154 on) makes finite values zero."""
         import torch
         max_norm = float(max_norm)
         if not max_norm >= 0.0:
