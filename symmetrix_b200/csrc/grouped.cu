@@ -15,7 +15,6 @@
 
 #include "common.cuh"
 #include "routing.hpp"
-#include "row_tiles.cuh"
 
 namespace smx {
 namespace {

@@ -63,7 +63,8 @@ __device__ __forceinline__ int gs_runs(const GsPass& p, const GsDegree& d, long 
     return static_cast<int>((rows + 127) / 128);
 }
 
-// The CTA's tiles, the same share of all steps for each: lane q holds begin and end among the tiles of degree q. Called by a warp.
+// The CTA's tiles, the same share of all steps for each (a sum of the gradient counts as a whole chunk, whatever the group's rows): lane q holds begin and end among the tiles of
+// degree q. Called by a warp.
 template <int kMode>
 __device__ __forceinline__ void gs_share(const GsPass& p, int& begin, int& end) {
     const int lane = threadIdx.x & 31;
@@ -313,9 +314,11 @@ struct GsLayout {
 // TMEM: two stages of a partial sum of 128 columns and 128 of A (hi, lo), taken in turn. A hand-over costs its warps some hundred cycles: with steps of
 // 32 inner values and half the warps for A and B the products waited two thirds of the time (98,304 atoms of 89 elements 127 us).
 // 98,304 atoms of 89 elements, scalars and vectors, 128 x 128 (414 MB): 92 us, 4.5 TB/s, 140 TFLOP/s. 8,001 atoms in two slots behind the tensor product, 21 GFLOP each:
-// forward 154 us, the rows' gradient 123, the matrices' 155 with their joins (171 to 136 TFLOP/s; three tf32 products of them could reach 272). A step takes some 4,000 cycles, 1,536
+// forward 154 us, the rows' gradient 127, the matrices' 155 with their joins (166 to 136 TFLOP/s; three tf32 products of them could reach 272). A step takes some 4,000 cycles, 1,536
 // of them the products': its warps issue in 53 to 57 % of the cycles (splitting, copies and sums, some 300 instructions a warp and step), the data pipe of shared memory
-// is 41 % busy beside the reads of the products, and each of the five hand-overs between warps costs some hundred cycles.
+// is 41 % busy beside the reads of the products, and each of the five hand-overs between warps costs some hundred cycles. A step takes as long where B stays (44 an SM in the 92 us)
+// as where it is copied and split every time (68 in the 154), so what bounds it is the loop over a stage of tensor memory: A is stored behind its last products, and the products wait for
+// all sixteen warps of A and of the sums.
 // Every wait is bounded; if one runs out, the CTA gives up, fills its remaining tiles with NaN, reports it to `status` and ends when its products
 // and copies in flight have.
 template <int kMode, bool kWide>

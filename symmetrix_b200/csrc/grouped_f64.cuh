@@ -109,7 +109,7 @@ __device__ __forceinline__ bool gd_find(const GdPass& p, int BM, int BN, long lo
 
 // A CTA of four warps (WM x WN) makes a tile from ST stages of 16 inner values in flight. The double-precision tensor pipe bounds large calls: 20,000 atoms of 16
 // groups, 7.2 GFLOP, 223 us, 32 TFLOP/s of 36. Calls of a few hundred tiles are a chain of copies and products a tile: 1,029 atoms, 131 x 97 (0.24 GFLOP, rows of
-// odd length in copies of 8 bytes), 27 us forward; neither tiles of 32 x 64, eight warps a tile, a third stage nor leaving out the blocks behind a tile's end shorten
+// odd length in copies of 8 bytes), 25 us forward; neither tiles of 32 x 64, eight warps a tile, a third stage nor leaving out the blocks behind a tile's end shorten
 // that by more than a tenth, and all of them cost large calls 3 to 15 %.
 template <int kMode, int BM, int BN, int WM, int WN, int ST>
 __global__ void __launch_bounds__(kGdThreads) grouped_f64_kernel(const __grid_constant__ GdPass pass) {

@@ -1,4 +1,5 @@
-// Tiles of rows that never mix groups: what a CTA of the operators on routed rows finds its work with.
+// Tiles of rows that never mix groups: what a CTA of the linears with adapters finds its work with. (Linears of routed rows walk degrees and blocks of
+// columns as well, in an order of their own: csrc/grouped_f32.cuh, csrc/grouped_f64.cuh.)
 #pragma once
 
 namespace smx {
