@@ -96,7 +96,7 @@ size_t part_values(const smx_grouped_linear& c, int d) {
 
 // Gradients of groups with several sums: added in order, by eights and those in 64 bits (a long list loses no more than eight roundings; conversions of every sum would
 // take another 7 us of the case below), in units V of 16 bytes where all matrices allow it (sums of 8,001 atoms in two slots behind the tensor
-// product, 41 MB: 11 us; 17 value by value).
+// product, 41 MB: 12.5 us; value by value half as long again).
 template <typename V>
 struct JoinPass {
     struct { int comps; long long size; const V* part; V* grad; } degree[kMaxDegrees];     // size: units of a matrix
