@@ -103,6 +103,15 @@ def _apart(out, *inputs) -> None:
                 raise ValueError("out shares memory with an input")
 
 
+def _not_of_plan(ids, plan):
+    """`ids` in one piece; refused where they lie in the plan that they would be sorted into."""
+    ids = ids.contiguous()
+    at, to = ids.data_ptr(), plan.data_ptr()
+    if at < to + 4 * plan.numel() and to < at + 4 * ids.numel():
+        raise ValueError("ids share memory with the plan")
+    return ids
+
+
 class RowRouting:
     """Rows sorted by group, and back. ``ids`` is an int32 CUDA tensor ``[rows]`` or ``[rows, slots]`` of groups in ``0 .. num_groups - 1``;
     any other value is an empty slot.
@@ -152,7 +161,7 @@ class RowRouting:
         if not isinstance(ids, torch.Tensor) or ids.dtype != torch.int32 or ids.device != self.device or ids.numel() != self._pairs \
                 or ids.dim() not in (1, 2) or ids.shape[0] != self.num_rows:
             raise ValueError(f"ids must be an int32 tensor of {self.num_rows} rows with {self.slots} slots on {self.device}")
-        self._make(ids)
+        self._make(_not_of_plan(ids, self._plan))
 
     def _make(self, ids):
         import torch

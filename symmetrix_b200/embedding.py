@@ -9,7 +9,7 @@ from __future__ import annotations
 from collections import namedtuple
 
 from . import _lib
-from .adapters import _apart, _call, _out, _precision, _ptr, _rows, _stream, _values
+from .adapters import _apart, _call, _not_of_plan, _out, _precision, _ptr, _rows, _stream, _values
 
 EmbeddingGradients = namedtuple("EmbeddingGradients", ["table", "weights"])
 
@@ -69,7 +69,7 @@ class EmbeddingPlan:
         ids, rows, slots = _tokens(ids, self.device)
         if (rows, slots) != (self.num_rows, self.slots):
             raise ValueError(f"ids must have {self.num_rows} rows with {self.slots} slots")
-        self._make(ids)
+        self._make(_not_of_plan(ids, self._plan))
 
     def _make(self, ids):
         import torch

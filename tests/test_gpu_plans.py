@@ -70,3 +70,20 @@ def test_many_groups_do_not_slow_a_small_plan_down(make, pairs, few, many, most)
         plan = make(ids, count)
         us.append(_graph_us(lambda: plan.update(ids)))
     assert us[1] <= most * us[0], us
+
+
+@pytest.mark.parametrize("make", [RowRouting, EmbeddingPlan])
+@pytest.mark.parametrize("pairs", [300, 9000])
+def test_ids_that_lie_in_the_plan_are_refused(make, pairs):
+    """The sort reads its ids while it writes the plan: a plan of its own arrays needs a copy of them."""
+    ids, _, order = ids_of(pairs, 7, 1)
+    plan = make(ids, 7)
+    parts = [plan.order, plan.tokens] if make is EmbeddingPlan else [plan.order, plan.position, plan.position.reshape(-1)]
+    for own in parts:
+        with pytest.raises(ValueError, match="share memory"):
+            plan.update(own)
+    np.testing.assert_array_equal(plan.order.cpu().numpy(), order)
+    again = plan.order.clone()
+    plan.update(again)
+    key = np.where(again.cpu().numpy() < 7, again.cpu().numpy(), 7)
+    np.testing.assert_array_equal(plan.order.cpu().numpy(), np.argsort(key, kind="stable"))
