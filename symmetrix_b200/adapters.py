@@ -156,7 +156,7 @@ class RowRouting:
         return self._plan[2 * self._pairs:]
 
     def update(self, ids) -> None:
-        """The plan of other ids of the same shape, in the same tensors."""
+        """The plan of other ids of the same shape, in the same tensors (of which `ids` must not be a part)."""
         import torch
         if not isinstance(ids, torch.Tensor) or ids.dtype != torch.int32 or ids.device != self.device or ids.numel() != self._pairs \
                 or ids.dim() not in (1, 2) or ids.shape[0] != self.num_rows:

@@ -65,7 +65,7 @@ class EmbeddingPlan:
         return self._plan[self._pairs:]
 
     def update(self, ids) -> None:
-        """The plan of other ids of the same shape, in the same tensors."""
+        """The plan of other ids of the same shape, in the same tensors (of which `ids` must not be a part)."""
         ids, rows, slots = _tokens(ids, self.device)
         if (rows, slots) != (self.num_rows, self.slots):
             raise ValueError(f"ids must have {self.num_rows} rows with {self.slots} slots")
